@@ -416,6 +416,102 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
                      int64_t ignore_index, void* stream);
 
 /*
+ * Losses of the model's head from its hidden states, the logits z = hidden
+ * weight^T never in memory. Beside mhs_xent_*, which read given logits; the
+ * reference forms them (mamba_metal/model.py:294-297).
+ *
+ *   hidden (rows, dim) rows ldh elements apart, weight (vocab, dim) rows ldw
+ *   apart, both of `dtype`, 16-byte aligned; dim and the row strides multiples of
+ *   8 (of 4 for MHS_F32), row strides below 2^21. fp32 products are those of
+ *   mhs_gemm_f32; 16-bit ones multiply exactly and add in fp32.
+ *
+ * Cross entropy against targets (rows) int64:
+ *   loss_rows[r] = ln(2) lse2[r] - picked[r], lse2[r] = log2 sum_v exp(z[r, v]),
+ *   picked[r] = z[r, targets[r]]; 0 with keep[r] = 0 where targets[r] ==
+ *   ignore_index, else keep[r] = 1; NaN for any other target outside [0, vocab).
+ * reduction MHS_REDUCE_MEAN: loss[0] = the sum over rows of loss_rows / keep
+ *   (NaN if no row is kept), MHS_REDUCE_SUM: the sum; count[0] = the rows kept
+ *   (both untouched, and may be NULL, for MHS_REDUCE_NONE).
+ * Backward: with upstream[0] (per row, upstream[r], for MHS_REDUCE_NONE) the
+ *   gradient that reaches the loss, dhidden (rows, dim) and dweight (vocab, dim),
+ *   contiguous, of `dtype`; either may be NULL. A piece of the vocabulary at a
+ *   time: the gradient of its logits is in the workspace, at most 256 MB or 256
+ *   words of it. Of 16-bit operands it is rounded to 16 bits there (fp16 scaled
+ *   by a power of two), as the products' operands are; the sums are fp32. Rows
+ *   that are not kept add nothing, whatever they hold, and get zeros.
+ * Every sum runs in a fixed order (bit-for-bit reproducible). The workspace is
+ * 256-byte aligned; its size is 0 for arguments that the calls reject.
+ */
+#define MHS_F32 0
+#define MHS_BF16 1
+#define MHS_F16 2
+#define MHS_REDUCE_NONE 0
+#define MHS_REDUCE_MEAN 1
+#define MHS_REDUCE_SUM 2
+
+size_t mhs_linear_xent_fwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim);
+int mhs_linear_xent_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
+                        int64_t ldw, const int64_t* targets, float* lse2, float* picked,
+                        float* keep, float* loss_rows, float* loss, float* count, int64_t rows,
+                        int64_t vocab, int64_t dim, int64_t ignore_index, int reduction,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim);
+int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
+                        int64_t ldw, const int64_t* targets, const float* lse2,
+                        const float* picked, const float* keep, const float* upstream,
+                        const float* count, void* dhidden, void* dweight, int64_t rows,
+                        int64_t vocab, int64_t dim, int reduction, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * Distillation from a teacher's top words: per row `top` (1..MHS_MAX_TOP) words
+ * ids (rows, top) int64 with the teacher's logits teacher (rows, top) fp32, an id
+ * below 0 being padding. With t the temperature, q = softmax(teacher / t) over
+ * the row's kept ids and p = softmax(z / t) over the whole vocabulary,
+ *   loss_rows[r] = t^2 sum_k q_k (ln q_k - ln p[ids_k])
+ * (terms with q_k = 0 are 0). A row that keeps no id, or whose kept logits are all
+ * -inf, is empty: loss 0, keep 0; an id at or past vocab makes the row's loss NaN.
+ * Outputs as above, and q, picked (rows, top) and lse2 = log2 sum_v exp(z / t) for
+ * the backward; dz[r, v] = t (p[v] - sum_{ids_k = v} q_k) times the gradient that
+ * reaches the row's loss. The teacher gets no gradient. The workspaces are the
+ * cross entropy's. No counterpart in the reference.
+ */
+#define MHS_MAX_TOP 1024
+
+int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
+                           int64_t ldw, const float* teacher, const int64_t* ids, float* lse2,
+                           float* picked, float* q, float* keep, float* loss_rows, float* loss,
+                           float* count, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
+                           float temperature, int reduction, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
+                           int64_t ldw, const int64_t* ids, const float* lse2,
+                           const float* picked, const float* q, const float* keep,
+                           const float* upstream, const float* count, void* dhidden,
+                           void* dweight, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
+                           float temperature, int reduction, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
+ * The same distillation of given logits (rows, vocab) of `dtype`, rows ld
+ * elements apart, at any alignment of whole elements; dlogits (rows, vocab) is
+ * contiguous, 16-byte aligned, fully written, and may not alias logits. The
+ * workspace (the forward's) is mhs_distill_workspace_bytes(rows).
+ */
+size_t mhs_distill_workspace_bytes(int64_t rows);
+int mhs_distill_fwd(int dtype, const void* logits, int64_t ld, const float* teacher,
+                    const int64_t* ids, float* lse2, float* q, float* keep, float* loss_rows,
+                    float* loss, float* count, int64_t rows, int64_t vocab, int64_t top,
+                    float temperature, int reduction, void* workspace, size_t workspace_bytes,
+                    void* stream);
+int mhs_distill_bwd(int dtype, const void* logits, int64_t ld, const int64_t* ids,
+                    const float* lse2, const float* q, const float* keep, const float* upstream,
+                    const float* count, void* dlogits, int64_t rows, int64_t vocab, int64_t top,
+                    float temperature, int reduction, void* stream);
+
+
+/*
  * RMSNorm of the residual stream, fp32: for each of `rows` rows of `cols`
  * features, y = x * r * weight with r = 1 / sqrt(mean(x^2) + eps); rstd[row]
  * receives r. Replaces the reference's RMSNorm.forward

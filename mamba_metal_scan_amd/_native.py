@@ -41,6 +41,10 @@ EXPORTED_SYMBOLS = (
     "mhs_gemm_workspace_bytes", "mhs_gemm_f32", "mhs_decode_workspace_bytes",
     "mhs_decode_f32", "mhs_block_saved_bytes", "mhs_block_fwd_workspace_bytes",
     "mhs_block_fwd_f32", "mhs_block_bwd_workspace_bytes", "mhs_block_bwd_f32",
+    "mhs_linear_xent_fwd_workspace_bytes", "mhs_linear_xent_fwd",
+    "mhs_linear_xent_bwd_workspace_bytes", "mhs_linear_xent_bwd", "mhs_linear_distill_fwd",
+    "mhs_linear_distill_bwd", "mhs_distill_workspace_bytes", "mhs_distill_fwd",
+    "mhs_distill_bwd",
 )
 
 # Size of the static device scratch of mhs_scan_fwd_noalloc_f32 (the header's
@@ -173,6 +177,27 @@ def library() -> ctypes.CDLL:
             lib.mhs_block_bwd_f32.restype = ctypes.c_int
             lib.mhs_block_bwd_f32.argtypes = ([ctypes.c_char_p] + [_P] * 5 + [ctypes.c_char_p]
                                               + [_I64] * 7 + [_P, ctypes.c_size_t, _P])
+            _int, _size = ctypes.c_int, ctypes.c_size_t
+            head = [_int, _P, _I64, _P, _I64]       # dtype, hidden and weight with row strides
+            for name in ("mhs_linear_xent_fwd_workspace_bytes",
+                         "mhs_linear_xent_bwd_workspace_bytes"):
+                getattr(lib, name).restype = _size
+                getattr(lib, name).argtypes = [_int] + [_I64] * 3
+            lib.mhs_distill_workspace_bytes.restype = _size
+            lib.mhs_distill_workspace_bytes.argtypes = [_I64]
+            for name, args in (
+                    ("mhs_linear_xent_fwd", head + [_P] * 7 + [_I64] * 4 + [_int, _P, _size, _P]),
+                    ("mhs_linear_xent_bwd", head + [_P] * 8 + [_I64] * 3 + [_int, _P, _size, _P]),
+                    ("mhs_linear_distill_fwd",
+                     head + [_P] * 9 + [_I64] * 4 + [_F32, _int, _P, _size, _P]),
+                    ("mhs_linear_distill_bwd",
+                     head + [_P] * 9 + [_I64] * 4 + [_F32, _int, _P, _size, _P]),
+                    ("mhs_distill_fwd",
+                     [_int, _P, _I64] + [_P] * 8 + [_I64] * 3 + [_F32, _int, _P, _size, _P]),
+                    ("mhs_distill_bwd",
+                     [_int, _P, _I64] + [_P] * 7 + [_I64] * 3 + [_F32, _int, _P])):
+                getattr(lib, name).restype = _int
+                getattr(lib, name).argtypes = args
             _lib = lib
     return _lib
 
@@ -1229,3 +1254,349 @@ gemm_add = _register("gemm_add", _gemm_add_impl, ("out",),
 @gemm_add.register_fake
 def _gemm_add_fake(out, a, b, form):
     return None
+
+
+# --------------------------------------------------------- the head's losses
+#
+# Cross entropy and distillation from hidden states and the head's weight, and
+# distillation of given logits. What a forward keeps for its backward is one
+# fp32 tensor, `saved`: the count of rows kept (in the first of 4 elements),
+# then per row lse2, keep, the losses, and picked and q of its `top` words (q
+# not for the cross entropy, picked not for given logits).
+
+REDUCE = {"none": 0, "mean": 1, "sum": 2}
+HEAD_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_TOP = 1024   # the header's MHS_MAX_TOP
+
+
+def head_rows(t: torch.Tensor) -> bool:
+    """Whether the head's kernels read the 2-D t in place: rows of whole 16-byte
+    accesses, 16-byte aligned, less than 2^21 elements apart."""
+    v = 16 // t.element_size()
+    ld = t.stride(0)
+    return (t.shape[1] % v == 0 and t.stride(1) == 1 and ld % v == 0
+            and t.shape[1] <= ld < 1 << 21 and t.data_ptr() % 16 == 0)
+
+
+def _saved_parts(saved: torch.Tensor, rows: int, *tops: int) -> list[int]:
+    """Addresses of count, lse2, keep and the losses in saved, then of (rows,
+    top) arrays for each of tops."""
+    sizes = [4, rows, rows, rows, *(rows * t for t in tops)]
+    at, out = saved.data_ptr(), []
+    for n in sizes:
+        out.append(at)
+        at += 4 * n
+    return out
+
+
+def _saved_size(rows: int, *tops: int) -> int:
+    return 4 + rows * (3 + sum(tops))
+
+
+def _check_head(what: str, hidden, weight, reduction) -> None:
+    _on_one_device(what, hidden, weight)
+    _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1], what,
+          f"hidden must be (rows, dim) and weight (vocab, dim); got {tuple(hidden.shape)}, "
+          f"{tuple(weight.shape)}")
+    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, what,
+          f"weight must not be empty; got {tuple(weight.shape)}")
+    _need(hidden.dtype in HEAD_DTYPES and weight.dtype == hidden.dtype, what,
+          "hidden and weight must both be float32, bfloat16 or float16; got "
+          f"{hidden.dtype}, {weight.dtype}")
+    for name, t in (("hidden", hidden), ("weight", weight)):
+        _need(t.numel() == 0 or head_rows(t), what,
+              f"{name} needs rows of whole 16-byte accesses, 16-byte aligned and less than "
+              f"2^21 elements apart; got shape {tuple(t.shape)}, strides {t.stride()}")
+    _need(reduction in REDUCE.values(), what, f"reduction must be 0, 1 or 2; got {reduction!r}")
+
+
+def _check_top(what: str, rows: int, teacher_logits, ids, temperature) -> None:
+    _need(ids.dim() == 2 and ids.shape[0] == rows and 1 <= ids.shape[1] <= MAX_TOP, what,
+          f"the teacher's words must be ({rows}, k) with k in [1, {MAX_TOP}]; got "
+          f"{tuple(ids.shape)}")
+    _need(ids.dtype == torch.int64, what, f"the teacher's words must be int64; got {ids.dtype}")
+    _dense(what, teacher_ids=ids, teacher_logits=teacher_logits)
+    if teacher_logits is not None:
+        _fp32(what, teacher_logits=teacher_logits)
+        _shaped(what, "teacher_logits", teacher_logits, ids.shape)
+    _need(temperature > 0 and temperature < float("inf"), what,
+          f"temperature must be positive and finite; got {temperature}")
+
+
+def _check_bwd_head(what: str, grad, saved, rows: int, reduction: int, *tops: int) -> None:
+    _fp32(what, grad=grad, saved=saved)
+    _dense(what, grad=grad, saved=saved)
+    _shaped(what, "grad", grad, (rows,) if reduction == 0 else ())
+    _shaped(what, "saved", saved, (_saved_size(rows, *tops),))
+
+
+def _workspace(nbytes: int, what: str, dev: torch.device) -> torch.Tensor:
+    if nbytes == 0:
+        raise HipScanError(f"{what}: {library().mhs_last_error().decode()}")
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def _new_loss(t: torch.Tensor, rows: int, reduction: int) -> torch.Tensor:
+    return torch.empty((rows,) if reduction == 0 else (), dtype=torch.float32, device=t.device)
+
+
+def _linear_xent_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                          ignore_index: int, reduction: int
+                          ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss () or (rows,), saved) of hidden (rows, dim) against targets (rows)."""
+    rows, dim = hidden.shape
+    vocab = weight.shape[0]
+    dev = hidden.device
+    lib = library()
+    dt = HEAD_DTYPES[hidden.dtype]
+    loss = _new_loss(hidden, rows, reduction)
+    saved = torch.empty(_saved_size(rows, 1), dtype=torch.float32, device=dev)
+    count, lse2, keep, losses, picked = _saved_parts(saved, rows, 1)
+    with _on(dev):
+        nbytes = lib.mhs_linear_xent_fwd_workspace_bytes(dt, rows, vocab, dim)
+        ws = _workspace(nbytes, "linear_xent_fwd", dev)
+        rc = lib.mhs_linear_xent_fwd(
+            dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
+            weight.stride(0), targets.data_ptr(), lse2, picked, keep,
+            losses if reduction else loss.data_ptr(), loss.data_ptr(), count, rows, vocab, dim,
+            ignore_index, reduction, ws.data_ptr(), nbytes, _stream(dev))
+    _check(rc, "mhs_linear_xent_fwd")
+    return loss, saved
+
+
+def _check_linear_xent(what: str, hidden, weight, targets, reduction) -> None:
+    _check_head(what, hidden, weight, reduction)
+    _on_one_device(what, hidden, targets)
+    _shaped(what, "targets", targets, (hidden.shape[0],))
+    _need(targets.dtype == torch.int64, what, f"targets must be int64; got {targets.dtype}")
+    _dense(what, targets=targets)
+
+
+linear_xent_fwd = _register(
+    "linear_xent_fwd", _linear_xent_fwd_impl, (),
+    lambda hidden, weight, targets, ignore_index, reduction:
+    _check_linear_xent("linear_xent_fwd", hidden, weight, targets, reduction))
+
+
+@linear_xent_fwd.register_fake
+def _linear_xent_fwd_fake(hidden, weight, targets, ignore_index, reduction):
+    rows = hidden.shape[0]
+    return (_new_loss(hidden, rows, reduction),
+            hidden.new_empty((_saved_size(rows, 1),), dtype=torch.float32))
+
+
+def _head_grads(hidden, weight, need_hidden: bool, need_weight: bool):
+    """Contiguous gradients of the shapes of hidden and weight, or empty ones."""
+    return (hidden.new_empty(hidden.shape if need_hidden else (0,)),
+            weight.new_empty(weight.shape if need_weight else (0,)))
+
+
+def _linear_xent_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
+                          targets: torch.Tensor, saved: torch.Tensor, reduction: int,
+                          need_hidden: bool, need_weight: bool
+                          ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(dhidden, dweight) for the forward that gave saved; empty where not needed."""
+    rows, dim = hidden.shape
+    vocab = weight.shape[0]
+    dev = hidden.device
+    lib = library()
+    dt = HEAD_DTYPES[hidden.dtype]
+    dhidden, dweight = _head_grads(hidden, weight, need_hidden, need_weight)
+    count, lse2, keep, _, picked = _saved_parts(saved, rows, 1)
+    with _on(dev):
+        nbytes = lib.mhs_linear_xent_bwd_workspace_bytes(dt, rows, vocab, dim)
+        ws = _workspace(nbytes, "linear_xent_bwd", dev)
+        rc = lib.mhs_linear_xent_bwd(
+            dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
+            weight.stride(0), targets.data_ptr(), lse2, picked, keep, grad.data_ptr(), count,
+            dhidden.data_ptr() if need_hidden else None,
+            dweight.data_ptr() if need_weight else None, rows, vocab, dim, reduction,
+            ws.data_ptr(), nbytes, _stream(dev))
+    _check(rc, "mhs_linear_xent_bwd")
+    return dhidden, dweight
+
+
+def _check_linear_xent_bwd(grad, hidden, weight, targets, saved, reduction, need_hidden,
+                           need_weight):
+    what = "linear_xent_bwd"
+    _check_linear_xent(what, hidden, weight, targets, reduction)
+    _on_one_device(what, hidden, grad, saved)
+    _check_bwd_head(what, grad, saved, hidden.shape[0], reduction, 1)
+
+
+linear_xent_bwd = _register("linear_xent_bwd", _linear_xent_bwd_impl, (), _check_linear_xent_bwd)
+
+
+@linear_xent_bwd.register_fake
+def _linear_xent_bwd_fake(grad, hidden, weight, targets, saved, reduction, need_hidden,
+                          need_weight):
+    return _head_grads(hidden, weight, need_hidden, need_weight)
+
+
+def _linear_distill_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor,
+                             teacher_logits: torch.Tensor, ids: torch.Tensor,
+                             temperature: float, reduction: int
+                             ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss () or (rows,), saved) against the teacher's words ids (rows, top) and
+    their logits."""
+    rows, dim = hidden.shape
+    vocab, top = weight.shape[0], ids.shape[1]
+    dev = hidden.device
+    lib = library()
+    dt = HEAD_DTYPES[hidden.dtype]
+    loss = _new_loss(hidden, rows, reduction)
+    saved = torch.empty(_saved_size(rows, top, top), dtype=torch.float32, device=dev)
+    count, lse2, keep, losses, picked, q = _saved_parts(saved, rows, top, top)
+    with _on(dev):
+        nbytes = lib.mhs_linear_xent_fwd_workspace_bytes(dt, rows, vocab, dim)
+        ws = _workspace(nbytes, "linear_distill_fwd", dev)
+        rc = lib.mhs_linear_distill_fwd(
+            dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
+            weight.stride(0), teacher_logits.data_ptr(), ids.data_ptr(), lse2, picked, q, keep,
+            losses if reduction else loss.data_ptr(), loss.data_ptr(), count, rows, vocab, dim,
+            top, temperature, reduction, ws.data_ptr(), nbytes, _stream(dev))
+    _check(rc, "mhs_linear_distill_fwd")
+    return loss, saved
+
+
+def _check_linear_distill(what: str, hidden, weight, teacher_logits, ids, temperature,
+                          reduction) -> None:
+    _check_head(what, hidden, weight, reduction)
+    _on_one_device(what, hidden, teacher_logits, ids)
+    _check_top(what, hidden.shape[0], teacher_logits, ids, temperature)
+
+
+linear_distill_fwd = _register(
+    "linear_distill_fwd", _linear_distill_fwd_impl, (),
+    lambda hidden, weight, teacher_logits, ids, temperature, reduction:
+    _check_linear_distill("linear_distill_fwd", hidden, weight, teacher_logits, ids, temperature,
+                          reduction))
+
+
+@linear_distill_fwd.register_fake
+def _linear_distill_fwd_fake(hidden, weight, teacher_logits, ids, temperature, reduction):
+    rows, top = ids.shape
+    return (_new_loss(hidden, rows, reduction),
+            hidden.new_empty((_saved_size(rows, top, top),), dtype=torch.float32))
+
+
+def _linear_distill_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
+                             ids: torch.Tensor, saved: torch.Tensor, temperature: float,
+                             reduction: int, need_hidden: bool, need_weight: bool
+                             ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(dhidden, dweight) for the forward that gave saved; empty where not needed."""
+    rows, dim = hidden.shape
+    vocab, top = weight.shape[0], ids.shape[1]
+    dev = hidden.device
+    lib = library()
+    dt = HEAD_DTYPES[hidden.dtype]
+    dhidden, dweight = _head_grads(hidden, weight, need_hidden, need_weight)
+    count, lse2, keep, _, picked, q = _saved_parts(saved, rows, top, top)
+    with _on(dev):
+        nbytes = lib.mhs_linear_xent_bwd_workspace_bytes(dt, rows, vocab, dim)
+        ws = _workspace(nbytes, "linear_distill_bwd", dev)
+        rc = lib.mhs_linear_distill_bwd(
+            dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
+            weight.stride(0), ids.data_ptr(), lse2, picked, q, keep, grad.data_ptr(), count,
+            dhidden.data_ptr() if need_hidden else None,
+            dweight.data_ptr() if need_weight else None, rows, vocab, dim, top, temperature,
+            reduction, ws.data_ptr(), nbytes, _stream(dev))
+    _check(rc, "mhs_linear_distill_bwd")
+    return dhidden, dweight
+
+
+def _check_linear_distill_bwd(grad, hidden, weight, ids, saved, temperature, reduction,
+                              need_hidden, need_weight):
+    what = "linear_distill_bwd"
+    _check_linear_distill(what, hidden, weight, None, ids, temperature, reduction)
+    _on_one_device(what, hidden, grad, saved)
+    _check_bwd_head(what, grad, saved, hidden.shape[0], reduction, ids.shape[1], ids.shape[1])
+
+
+linear_distill_bwd = _register("linear_distill_bwd", _linear_distill_bwd_impl, (),
+                               _check_linear_distill_bwd)
+
+
+@linear_distill_bwd.register_fake
+def _linear_distill_bwd_fake(grad, hidden, weight, ids, saved, temperature, reduction,
+                             need_hidden, need_weight):
+    return _head_grads(hidden, weight, need_hidden, need_weight)
+
+
+def _distill_fwd_impl(logits: torch.Tensor, teacher_logits: torch.Tensor, ids: torch.Tensor,
+                      temperature: float, reduction: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss () or (rows,), saved) of logits (rows, vocab), rows of any stride."""
+    rows, vocab = logits.shape
+    top = ids.shape[1]
+    dev = logits.device
+    lib = library()
+    loss = _new_loss(logits, rows, reduction)
+    saved = torch.empty(_saved_size(rows, top), dtype=torch.float32, device=dev)
+    count, lse2, keep, losses, q = _saved_parts(saved, rows, top)
+    with _on(dev):
+        nbytes = lib.mhs_distill_workspace_bytes(rows)
+        ws = _workspace(nbytes, "distill_fwd", dev)
+        rc = lib.mhs_distill_fwd(
+            HEAD_DTYPES[logits.dtype], logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+            teacher_logits.data_ptr(), ids.data_ptr(), lse2, q, keep,
+            losses if reduction else loss.data_ptr(), loss.data_ptr(), count, rows, vocab, top,
+            temperature, reduction, ws.data_ptr(), nbytes, _stream(dev))
+    _check(rc, "mhs_distill_fwd")
+    return loss, saved
+
+
+def _check_distill(what: str, logits, teacher_logits, ids, temperature, reduction) -> None:
+    _on_one_device(what, logits, teacher_logits, ids)
+    _need(logits.dim() == 2 and logits.shape[1] >= 1, what,
+          f"logits must be (rows, vocab); got {tuple(logits.shape)}")
+    _need(logits.dtype in HEAD_DTYPES, what,
+          f"logits must be float32, bfloat16 or float16; got {logits.dtype}")
+    _need(logits.stride(1) == 1 and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1]),
+          what, f"logits need contiguous rows; got strides {logits.stride()}")
+    _check_top(what, logits.shape[0], teacher_logits, ids, temperature)
+    _need(reduction in REDUCE.values(), what, f"reduction must be 0, 1 or 2; got {reduction!r}")
+
+
+distill_fwd = _register(
+    "distill_fwd", _distill_fwd_impl, (),
+    lambda logits, teacher_logits, ids, temperature, reduction:
+    _check_distill("distill_fwd", logits, teacher_logits, ids, temperature, reduction))
+
+
+@distill_fwd.register_fake
+def _distill_fwd_fake(logits, teacher_logits, ids, temperature, reduction):
+    rows, top = ids.shape
+    return (_new_loss(logits, rows, reduction),
+            logits.new_empty((_saved_size(rows, top),), dtype=torch.float32))
+
+
+def _distill_bwd_impl(grad: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor,
+                      saved: torch.Tensor, temperature: float, reduction: int) -> torch.Tensor:
+    """dlogits (rows, vocab), contiguous, for the forward that gave saved."""
+    rows, vocab = logits.shape
+    top = ids.shape[1]
+    dev = logits.device
+    dlogits = logits.new_empty((rows, vocab))
+    count, lse2, keep, _, q = _saved_parts(saved, rows, top)
+    with _on(dev):
+        rc = library().mhs_distill_bwd(
+            HEAD_DTYPES[logits.dtype], logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+            ids.data_ptr(), lse2, q, keep, grad.data_ptr(), count, dlogits.data_ptr(), rows, vocab,
+            top, temperature, reduction, _stream(dev))
+    _check(rc, "mhs_distill_bwd")
+    return dlogits
+
+
+def _check_distill_bwd(grad, logits, ids, saved, temperature, reduction):
+    what = "distill_bwd"
+    _check_distill(what, logits, None, ids, temperature, reduction)
+    _on_one_device(what, logits, grad, saved)
+    _check_bwd_head(what, grad, saved, logits.shape[0], reduction, ids.shape[1])
+
+
+distill_bwd = _register("distill_bwd", _distill_bwd_impl, (), _check_distill_bwd)
+
+
+@distill_bwd.register_fake
+def _distill_bwd_fake(grad, logits, ids, saved, temperature, reduction):
+    return logits.new_empty(logits.shape)

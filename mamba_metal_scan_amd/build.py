@@ -21,15 +21,15 @@ LIB_NAME = "libmamba_hip_scan.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 ARCH = "gfx950"
 
-# The host code and small kernels, and the scan kernels' instantiations in
-# five units (forward / backward x fp32 / bf16, and the fp32 backward with
-# atomics) compiled in parallel.
+# The host code and small kernels, the scan kernels' instantiations in six units
+# (forward / backward x fp32 / bf16, and the backwards with atomics) and the
+# head's losses, compiled in parallel.
 SOURCES = ["mhs_capi.hip", "mhs_kern_fwd_f32.hip", "mhs_kern_fwd_bf16.hip",
            "mhs_kern_bwd_f32.hip", "mhs_kern_bwd_bf16.hip", "mhs_kern_bwd_atom.hip",
-           "mhs_kern_bwd_atom_bf16.hip"]
+           "mhs_kern_bwd_atom_bf16.hip", "mhs_head_capi.hip"]
 HEADERS = ["mhs_common.hpp", "mhs_fwd.hpp", "mhs_bwd.hpp", "mhs_step.hpp", "mhs_conv.hpp",
            "mhs_gate.hpp", "mhs_instances.hpp", "mhs_xent.hpp", "mhs_norm.hpp", "mhs_gemm.hpp",
-           "mhs_decode.hpp"]
+           "mhs_decode.hpp", "mhs_host.hpp", "mhs_mm16.hpp", "mhs_head.hpp", "mhs_distill.hpp"]
 
 
 def hipcc() -> str:
@@ -46,6 +46,8 @@ def compile_flags() -> list[str]:
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-I", str(REPO_DIR / "include"), "-I", str(CSRC),
         "-Wall", "-Wno-unused-result",
+        # the direct loads to LDS set m0, which the compiler keeps nothing in
+        "-Wno-inline-asm",
     ]
 
 

@@ -23,6 +23,7 @@
 #include "mhs_fwd.hpp"
 #include "mhs_gate.hpp"
 #include "mhs_gemm.hpp"
+#include "mhs_host.hpp"
 #include "mhs_instances.hpp"
 #include "mhs_step.hpp"
 #include "mhs_xent.hpp"
@@ -44,6 +45,10 @@ constexpr int kVersion = (0 << 16) | (7 << 8) | 0;   // 0.7: quad-broadcast B/C 
 
 thread_local char g_err[512] = "";
 
+}  // namespace
+
+namespace mhs {
+
 int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -52,13 +57,23 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+void clear_error() { g_err[0] = '\0'; }
+
 int check_launch(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(MHS_EHIP, "%s: %s", what, hipGetErrorString(e));
   return MHS_OK;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+}  // namespace mhs
+
+namespace {
+
+using mhs::aligned16;
+using mhs::check_launch;
+using mhs::device_cus;
+using mhs::fail;
+using mhs::round_up;
 
 // Forced states per lane (0 = automatic); see mhs_set_variant.
 std::atomic<int> g_npl_override{0};
@@ -92,10 +107,12 @@ constexpr int kMinSegChunks = 8; // automatic split: at least 8 chunks per segme
 std::atomic<int> g_cu_override{0};
 std::atomic<int> g_cu_cache[kMaxDevices];   // per device, 0 until queried
 
+}  // namespace
+
 // Compute units of the current device, queried once per device and cached
 // (a partitioned MI355X exposes fewer than 256). Without a usable device the
 // MI355X count, so that the host-side size queries still answer.
-int device_cus() {
+int mhs::device_cus() {
   const int forced = g_cu_override.load(std::memory_order_relaxed);
   if (forced > 0) return forced;
   int dev = 0;
@@ -116,6 +133,8 @@ int device_cus() {
   if (dev >= 0 && dev < kMaxDevices) g_cu_cache[dev].store(n, std::memory_order_relaxed);
   return n;
 }
+
+namespace {
 
 // Time segments for this shape (see FwdArgs in mhs_fwd.hpp and BwdArgs in
 // mhs_bwd.hpp), in units of nch chunks (16-step sub-chunks in the forward,
@@ -544,7 +563,6 @@ int check_shape(int64_t batch, int64_t seqlen, int64_t d_inner, int64_t d_state,
   return MHS_OK;
 }
 
-size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
 
 // Backward workspace. Fixed-order reduction: per-block dB / dC partials
 // (nblk, batch, T, N), per (segment, batch row) dAneg and dt-bias partials.

@@ -235,25 +235,23 @@ __device__ __forceinline__ void plain_products(f32x16 (&acc)[FM][FN], const Gemm
   }
 }
 
-// One 128 x 128 tile per block, 2 x 2 waves of 64 x 64 (or 64 x 64 of 32 x 32,
-// for products of few tiles), k 16 deep and double
-// buffered: while a wave multiplies a tile it splits the next one into the
-// other buffer and loads the one after it into registers.
-// Bound by the matrix cores at the power limit: per k tile a wave issues 24
-// MFMAs (768 cycles of its SIMD's matrix core) beside 96 VALU (the split) and
-// 12 + 6 LDS accesses of 1 KB; SQ_VALU_MFMA_BUSY_CYCLES 66% of the CU cycles
-// at 1.6-1.8 GHz (2.4 nominal), three blocks per CU. Measured, against the
-// fp32 library product, us (TFLOP/s of fp32 work):
-//   NT 8192 x 1464 x 1432   195 (176) / 310       NN 8192 x 1432 x 1464  191 / 307
-//   NT 8192 x 2864 x 640    171 (176) / 255       TN 1464 x 1432 x 8192  215 / 349
-//   NT 8192 x 32768 x 640  1850 (186) / 2490      TN 32768 x 640 x 8192 1640 / 2260
-// i.e. 1.05-1.2 PFLOP/s of bf16, what an 8192^3 bf16 library product reaches
-// here (1.25). 256 x 128 tiles (two blocks per CU, a quarter fewer LDS reads)
-// were within 4% either way; each k tile's products summed from zero and then
-// added (a third of the error) took 8% longer.
+// The block's tile. Blocks go round the 8 XCDs: each XCD takes a contiguous run
+// of tiles, so that the rows of A and B it shares stay in its own L2.
+template <int TILE>
+__device__ __forceinline__ void gemm3_place(const GemmArgs& g, int& m0, int& n0) {
+  const int tiles = g.grid_m * g.grid_n;
+  const int xcd = blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
+  const int tile = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+  m0 = tile / g.grid_n * TILE;
+  n0 = tile % g.grid_n * TILE;
+}
+
+// acc = the tile's sums over k's k_first .. k_first + k_len - 1 (2 x 2 waves). A
+// fragment's element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32.
 template <bool AK, bool BK, int TILE>
-__global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
-gemm3_kernel(GemmArgs g) {
+__device__ __forceinline__ void gemm3_products(f32x16 (&acc)[TILE / 64][TILE / 64],
+                                               const GemmArgs& g, int m0, int n0, int k_first,
+                                               int k_len) {
   constexpr int BM = TILE, BN = TILE;
   constexpr int FM = BM / 64, FN = BN / 64;   // 32 x 32 fragments per wave
   extern __shared__ float lds_f[];
@@ -262,20 +260,11 @@ gemm3_kernel(GemmArgs g) {
   constexpr int BUF = 3 * (PA + PB);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Blocks go round the 8 XCDs: each XCD takes a contiguous run of tiles,
-  // so that the rows of A and B it shares stay in its own L2.
-  const int tiles = g.grid_m * g.grid_n;
-  const int xcd = blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
-  const int tile = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
-  const int m0 = tile / g.grid_n * BM, n0 = tile % g.grid_n * BN;
-  const int k_first = blockIdx.y * g.kt_per_split * kGemmBK;
-  const int k_len = min(g.K - k_first, g.kt_per_split * kGemmBK);
   const int nk = (k_len + kGemmBK - 1) / kGemmBK;
 
   GemmLoader<BM, AK, false> la(g.A, g.lda, m0, g.M, k_first);
   GemmLoader<BN, BK, true> lb(g.B, g.ldb, n0, g.N, k_first);
   float va[la.T][8], vb[lb.T][8];
-  f32x16 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -363,9 +352,38 @@ gemm3_kernel(GemmArgs g) {
   if (__builtin_amdgcn_ballot_w64(odd != odd || tiny.x + tiny.y + tiny.z + tiny.w != 0.f) != 0)
     plain_products<AK, BK>(acc, g, m0 + wm * (BM / 2), n0 + wn * (BN / 2), k_first,
                            k_first + k_len);
+}
 
-  // A fragment's element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4,
-  // column l % 32.
+// One 128 x 128 tile per block, 2 x 2 waves of 64 x 64 (or 64 x 64 of 32 x 32,
+// for products of few tiles), k 16 deep and double
+// buffered: while a wave multiplies a tile it splits the next one into the
+// other buffer and loads the one after it into registers.
+// Bound by the matrix cores at the power limit: per k tile a wave issues 24
+// MFMAs (768 cycles of its SIMD's matrix core) beside 96 VALU (the split) and
+// 12 + 6 LDS accesses of 1 KB; SQ_VALU_MFMA_BUSY_CYCLES 66% of the CU cycles
+// at 1.6-1.8 GHz (2.4 nominal), three blocks per CU. Measured, against the
+// fp32 library product, us (TFLOP/s of fp32 work):
+//   NT 8192 x 1464 x 1432   195 (176) / 310       NN 8192 x 1432 x 1464  191 / 307
+//   NT 8192 x 2864 x 640    171 (176) / 255       TN 1464 x 1432 x 8192  215 / 349
+//   NT 8192 x 32768 x 640  1850 (186) / 2490      TN 32768 x 640 x 8192 1640 / 2260
+// i.e. 1.05-1.2 PFLOP/s of bf16, what an 8192^3 bf16 library product reaches
+// here (1.25). 256 x 128 tiles (two blocks per CU, a quarter fewer LDS reads)
+// were within 4% either way; each k tile's products summed from zero and then
+// added (a third of the error) took 8% longer.
+template <bool AK, bool BK, int TILE>
+__global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
+gemm3_kernel(GemmArgs g) {
+  constexpr int BM = TILE, BN = TILE;
+  constexpr int FM = BM / 64, FN = BN / 64;   // 32 x 32 fragments per wave
+  int m0, n0;
+  gemm3_place<TILE>(g, m0, n0);
+  const int k_first = blockIdx.y * g.kt_per_split * kGemmBK;
+  f32x16 acc[FM][FN];
+  gemm3_products<AK, BK, TILE>(acc, g, m0, n0, k_first,
+                               min(g.K - k_first, g.kt_per_split * kGemmBK));
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
   float* const cb = g.C + (long long)blockIdx.y * g.M * g.ldc;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {

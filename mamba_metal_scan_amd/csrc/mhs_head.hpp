@@ -1,0 +1,727 @@
+// Losses of a language model's head from its hidden states, for gfx950: the
+// logits z = h W^T (h (rows, dim), W (vocab, dim)) are formed tile by tile and
+// never kept. With c = log2(e) / temperature and everything in base 2,
+//   lse2_r = log2 sum_v 2^(c z_rv),       p_rv = 2^(c z_rv - lse2_r)
+// and a row's targets (ids id_k with weights q_k; one of weight 1 for the
+// cross entropy, the teacher's words for distillation) give
+//   cross entropy   loss_r = ln(2) lse2_r - z_r,id             (temperature 1)
+//   distillation    loss_r = t^2 sum_k q_k (ln q_k - z_r,k / t + ln(2) lse2_r)
+//   dz_rv = coef_r (p_rv - sum_{k: id_k = v} q_k)
+//   dh = dz W,  dW = dz^T h
+// with coef_r the gradient that reaches the row's loss, times t for
+// distillation.
+//
+// Forward: the product W h^T, whose epilogue reduces each tile to a maximum and
+// a sum per row (head_lse); a pass over the rows joins the tiles, forms the
+// logits of the row's ids again as dot products, and the loss.
+// Backward, a piece of the vocabulary at a time: the product again, whose
+// epilogue writes dz (16 bits, or fp32 for fp32 operands) to the workspace,
+// then the products with W and h. dW's rows are complete with their piece, dh
+// sums over the pieces in fp32.
+#pragma once
+
+#include "mhs_common.hpp"
+#include "mhs_gemm.hpp"
+#include "mhs_mm16.hpp"
+#include "mhs_xent.hpp"
+
+namespace mhs {
+
+// ---------------------------------------------------------------- elements
+
+// fp32 beside Bf16 and Fp16: an element's storage and conversions.
+struct Fp32 {
+  typedef float type;
+  static __device__ __forceinline__ float from(float v) { return v; }
+  static __device__ __forceinline__ float to(float v) { return v; }
+};
+template <class T>
+struct ElemOf {
+  typedef unsigned short type;
+};
+template <>
+struct ElemOf<Fp32> {
+  typedef float type;
+};
+template <class T>
+using elem_t = typename ElemOf<T>::type;
+template <class T>
+constexpr int kVec = 16 / sizeof(elem_t<T>);   // elements of a 16-byte access
+
+template <class T>
+struct alignas(16) Vec {
+  elem_t<T> v[kVec<T>];
+};
+
+// ------------------------------------------------------- sums of exponentials
+
+// The log-sum-exp of a column of an accumulated tile (rows of the vocabulary in
+// the lane's registers): maximum and sum in base 2 of y = c z over rows below
+// `left`, NaN in the sum wherever a logit is NaN.
+template <int FM>
+__device__ __forceinline__ void column_lse2(const f32x16 (&z)[FM], float c, int row0, int left,
+                                            float& m, float& s) {
+  m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      m = fmaxf(m, row0 + i * 32 + 8 * (e / 4) + e % 4 < left ? z[i][e] * c : -INFINITY);
+  const float sh = lse2_shift(m);
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float y = __builtin_fmaf(z[i][e], c, -sh);
+      s += row0 + i * 32 + 8 * (e / 4) + e % 4 < left ? exp2_hw(y) : 0.f;
+    }
+}
+
+// Joins the (m, s) of a tile's WM waves per column (cols columns, red: 2 WM cols
+// floats of LDS) and writes the tile's row of the partials.
+template <int WM>
+__device__ __forceinline__ void store_partials(float* red, float2* part, int n0, int rows,
+                                               int cols, long long at) {
+  __syncthreads();
+  for (int n = threadIdx.x; n < cols; n += blockDim.x) {
+    float m = red[n], s = red[cols + n];
+#pragma unroll
+    for (int w = 1; w < WM; ++w) lse2_combine(m, s, red[2 * w * cols + n], red[(2 * w + 1) * cols + n]);
+    if (n0 + n < rows) part[at * rows + n0 + n] = make_float2(m, s);
+  }
+}
+
+// part[tile of the vocabulary][row] = (m, s) of the tile's logits. A = W (M =
+// vocab), B = h (N = rows).
+template <class T, class S>
+__global__ void __launch_bounds__(S::kThreads, 2)
+head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
+  extern __shared__ float lds_f[];
+  int tm, tn;
+  mm_tile(g, tm, tn);
+  const int m0 = tm * S::BM, n0 = tn * S::BN;
+  f32x16 acc[S::FM][S::FN];
+  mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+#pragma unroll
+  for (int j = 0; j < S::FN; ++j) {
+    f32x16 col[S::FM];
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) col[i] = acc[i][j];
+    float m, s;
+    column_lse2<S::FM>(col, c, m0 + wm * (S::FM * 32) + 4 * (lane >> 5), g.M, m, s);
+    lse2_combine(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
+    const int n = wn * (S::FN * 32) + j * 32 + (lane & 31);
+    if (lane < 32) {
+      lds_f[2 * wm * S::BN + n] = m;
+      lds_f[(2 * wm + 1) * S::BN + n] = s;
+    }
+  }
+  store_partials<S::WM>(lds_f, part, n0, g.N, S::BN, tm);
+}
+
+// The same for fp32 operands, on the products of three bf16 parts.
+template <int TILE>
+__global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
+head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part) {
+  extern __shared__ float lds_f[];
+  constexpr int F = TILE / 64;
+  int m0, n0;
+  gemm3_place<TILE>(g, m0, n0);
+  f32x16 acc[F][F];
+  gemm3_products<true, true, TILE>(acc, g, m0, n0, 0, g.K);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave >> 1, wn = wave & 1;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < F; ++j) {
+    f32x16 col[F];
+#pragma unroll
+    for (int i = 0; i < F; ++i) col[i] = acc[i][j];
+    float m, s;
+    column_lse2<F>(col, c, m0 + wm * (TILE / 2) + 4 * (lane >> 5), g.M, m, s);
+    lse2_combine(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
+    const int n = wn * (TILE / 2) + j * 32 + (lane & 31);
+    if (lane < 32) {
+      lds_f[2 * wm * TILE + n] = m;
+      lds_f[(2 * wm + 1) * TILE + n] = s;
+    }
+  }
+  store_partials<2>(lds_f, part, n0, g.N, TILE, m0 / TILE);
+}
+
+// --------------------------------------------------------------- few rows
+//
+// Up to 16 NF rows: bound by reading W once. A wave takes 16 words at a time
+// straight from memory as operands of 16 x 16 MFMAs (lane: word lane % 16, 16
+// bytes at lane / 16 of each 64), the rows' operands beside them (in L1 and L2),
+// so nothing is staged.
+
+constexpr int kSmallWords = 64;   // per block of 4 waves
+
+template <class T>
+struct SmallMma {   // 64 bytes of k per step
+  static constexpr int kDepth = 32;
+  typedef s16x8 frag;
+  static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 acc) {
+    if constexpr (__is_same(T, Bf16))
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                     __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                    __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  }
+};
+template <>
+struct SmallMma<Fp32> {   // element e of every lane: one MFMA, its k's 4 (lane / 16) + e
+  static constexpr int kDepth = 16;
+  typedef f32x4 frag;
+  static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 acc) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], acc, 0, 0, 0);
+    return acc;
+  }
+};
+
+struct SmallArgs {
+  const void* h;
+  const void* w;
+  long long ldh, ldw;   // rows 16-byte aligned
+  int rows, vocab, dim; // dim a multiple of a 16-byte access
+};
+
+// One operand's 16 bytes for k step `k` of a row (zeros past the row's end).
+template <class T>
+__device__ __forceinline__ typename SmallMma<T>::frag small_load(const elem_t<T>* p, int k,
+                                                                 int dim, bool ok) {
+  typedef typename SmallMma<T>::frag frag;
+  frag f = {};
+  if (ok && k < dim) f = *reinterpret_cast<const frag*>(p + k);
+  return f;
+}
+
+template <class T, int NF>
+__global__ void __launch_bounds__(256)
+head_small_kernel(SmallArgs g, float c, float2* __restrict__ part) {
+  typedef SmallMma<T> M;
+  __shared__ float red[2][4][16 * NF];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int word = blockIdx.x * kSmallWords + wave * 16 + (lane & 15);
+  const int k0 = kVec<T> * (lane >> 4);
+  const elem_t<T>* w = static_cast<const elem_t<T>*>(g.w) + (long long)word * g.ldw;
+  const elem_t<T>* h[NF];
+  bool ok[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const int r = 16 * j + (lane & 15);
+    ok[j] = r < g.rows;
+    h[j] = static_cast<const elem_t<T>*>(g.h) + (long long)(ok[j] ? r : 0) * g.ldh;
+  }
+  f32x4 acc[NF] = {};
+  constexpr int U = 8;   // k steps whose loads are in flight together
+  for (int k = 0; k < g.dim; k += U * M::kDepth) {
+    typename M::frag a[U], b[U][NF];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = k + u * M::kDepth + k0;
+      a[u] = small_load<T>(w, at, g.dim, word < g.vocab);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) b[u][j] = small_load<T>(h[j], at, g.dim, ok[j]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) acc[j] = M::mma(a[u], b[u][j], acc[j]);
+  }
+  // Element e of a lane: word 4 (lane / 16) + e, row lane % 16.
+  const int left = g.vocab - (blockIdx.x * kSmallWords + wave * 16 + 4 * (lane >> 4));
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = fmaxf(m, e < left ? acc[j][e] * c : -INFINITY);
+    const float sh = lse2_shift(m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      s += e < left ? exp2_hw(__builtin_fmaf(acc[j][e], c, -sh)) : 0.f;
+#pragma unroll
+    for (int o = 16; o <= 32; o *= 2)
+      lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    if (lane < 16) {
+      red[0][wave][16 * j + lane] = m;
+      red[1][wave][16 * j + lane] = s;
+    }
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < min(g.rows, 16 * NF)) {
+    const int r = threadIdx.x;
+    float m = red[0][0][r], s = red[1][0][r];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) lse2_combine(m, s, red[0][v][r], red[1][v][r]);
+    part[(long long)blockIdx.x * g.rows + r] = make_float2(m, s);
+  }
+}
+
+// ---------------------------------------------------------------- the rows
+
+// The dot product of two rows of dim elements, over the wave's lanes; every lane
+// returns it. 16-byte accesses where both rows are aligned (dim a multiple).
+template <class T>
+__device__ __forceinline__ float wave_dot(const elem_t<T>* a, const elem_t<T>* b, int dim) {
+  float s = 0.f;
+  for (int i = (threadIdx.x & 63) * kVec<T>; i < dim; i += 64 * kVec<T>) {
+    const Vec<T> x = *reinterpret_cast<const Vec<T>*>(a + i);
+    const Vec<T> y = *reinterpret_cast<const Vec<T>*>(b + i);
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) s = __builtin_fmaf(T::to(x.v[e]), T::to(y.v[e]), s);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  return s;
+}
+
+struct HeadRows {
+  const void* h;          // (rows, dim)
+  const void* w;          // (vocab, dim)
+  long long ldh, ldw;
+  const float2* part;     // (tiles, rows)
+  const long long* ids;   // (rows) targets, or (rows, k) the teacher's words
+  const float* teacher;   // (rows, k) the teacher's logits
+  float* lse2;            // (rows)
+  float* picked;          // (rows, k) logits of the ids
+  float* q;               // (rows, k) the teacher's probabilities
+  float* loss;            // (rows)
+  float* keep;            // (rows) 1: the row counts, 0: ignored or empty
+  int rows, vocab, dim, k, tiles;
+  long long ignore;
+  float temperature;
+};
+
+// Cross entropy: a wave per row.
+template <class T>
+__global__ void __launch_bounds__(256)
+head_xent_rows_kernel(HeadRows g) {
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= g.rows) return;   // (whole waves; no barrier below)
+  float m = -INFINITY, s = 0.f;
+  for (int t = lane; t < g.tiles; t += 64) {
+    const float2 p = g.part[(long long)t * g.rows + r];
+    lse2_combine(m, s, p.x, p.y);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1)
+    lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+  const float lse2 = m + log2f(s);
+  const long long t = g.ids[r];
+  const bool in = t >= 0 && t < g.vocab;
+  float z = 0.f;
+  if (in)
+    z = wave_dot<T>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh,
+                    static_cast<const elem_t<T>*>(g.w) + t * g.ldw, g.dim);
+  if (lane == 0) {
+    const bool keep = t != g.ignore;
+    g.lse2[r] = lse2;
+    g.picked[r] = z;
+    g.loss[r] = !keep ? 0.f : in ? lse2 * kLn2 - z : __builtin_nanf("");
+    g.keep[r] = keep ? 1.f : 0.f;
+  }
+}
+
+// The block's sum of v, the same in every thread (256 threads, fixed order).
+__device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// The teacher's probabilities of row r over its kept words (id >= 0), to q, and
+// the row's loss from the student's logits zk at the ids (LDS) and lse2. A row
+// that keeps no word, or whose kept logits are all -inf, is empty: loss 0,
+// probabilities 0. An id at or past the vocabulary: NaN.
+__device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2, const float* zk,
+                                            float* red) {
+  const long long at = (long long)r * g.k;
+  const float c = kLog2e / g.temperature;
+  float m = -INFINITY, bad = 0.f;
+  for (int k = threadIdx.x; k < g.k; k += 256) {
+    const long long id = g.ids[at + k];
+    if (id >= 0) m = fmaxf(m, g.teacher[at + k]);
+    if (id >= g.vocab) bad = 1.f;
+  }
+  m = block_max(m, red);
+  bad = block_max(bad, red);
+  float any = 0.f, s = 0.f;
+  const float sh = lse2_shift(m);   // (the difference first: no loss to a common offset)
+  for (int k = threadIdx.x; k < g.k; k += 256)
+    if (g.ids[at + k] >= 0) {
+      const float e = exp2_hw((g.teacher[at + k] - sh) * c);
+      s += e;
+      if (e != 0.f) any = 1.f;   // (NaN counts: the row's loss is NaN)
+    }
+  s = block_sum(s, red);
+  any = block_max(any, red);
+  const float log2s = log2f(s), inv = any != 0.f ? 1.f / s : 0.f;
+  float loss = 0.f;
+  for (int k = threadIdx.x; k < g.k; k += 256) {
+    float q = 0.f;
+    if (any != 0.f && g.ids[at + k] >= 0) {
+      const float y = (g.teacher[at + k] - sh) * c;
+      q = exp2_hw(y) * inv;
+      if (q != 0.f)
+        loss += q * ((y - log2s + lse2) * kLn2 - zk[k] / g.temperature);
+    }
+    g.q[at + k] = q;
+  }
+  loss = block_sum(loss, red);
+  if (threadIdx.x == 0) {
+    g.lse2[r] = lse2;
+    g.keep[r] = any;
+    g.loss[r] = any == 0.f ? 0.f
+                : bad != 0.f ? __builtin_nanf("") : g.temperature * g.temperature * loss;
+  }
+}
+
+// Distillation: a block per row.
+template <class T>
+__global__ void __launch_bounds__(256)
+head_distill_rows_kernel(HeadRows g) {
+  extern __shared__ float zk[];   // k floats
+  __shared__ float red[4];
+  const int r = blockIdx.x, wave = threadIdx.x >> 6;
+  const elem_t<T>* h = static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh;
+  for (int k = wave; k < g.k; k += 4) {
+    const long long id = g.ids[(long long)r * g.k + k];
+    float z = 0.f;
+    if (id >= 0 && id < g.vocab)
+      z = wave_dot<T>(h, static_cast<const elem_t<T>*>(g.w) + id * g.ldw, g.dim);
+    if ((threadIdx.x & 63) == 0) {
+      zk[k] = z;
+      g.picked[(long long)r * g.k + k] = z;
+    }
+  }
+  float m = -INFINITY, s = 0.f;
+  for (int t = threadIdx.x; t < g.tiles; t += 256) {
+    const float2 p = g.part[(long long)t * g.rows + r];
+    lse2_combine(m, s, p.x, p.y);
+  }
+  block_lse2(m, s);   // (its barrier publishes zk)
+  teacher_row(g, r, m + log2f(s), zk, red);
+}
+
+// loss[0] = the sum of the rows' losses, over the count of rows kept for the
+// mean (0 / 0 = NaN where none is); count[0] = that count. Blocks of 4096 rows
+// leave their sums in `sums` (2 doubles each) for a last block of the same
+// kernel; one block's rows need none. Sums in 64 bits, in a fixed order.
+constexpr int kLossThreads = 1024, kLossRows = 4096;
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(kLossThreads)
+head_loss_kernel(const float* __restrict__ rows_loss, const float* __restrict__ keep,
+                 const double2* __restrict__ in, double2* __restrict__ out,
+                 float* __restrict__ loss, float* __restrict__ count, long long n, int mean) {
+  __shared__ double sums[2][kLossThreads];
+  double s = 0.0, k = 0.0;
+  const long long first = (long long)blockIdx.x * kLossRows;
+  const long long end = out ? min(n, first + kLossRows) : n;
+  for (long long i = first + threadIdx.x; i < end; i += kLossThreads) {
+    const double2 v = in ? in[i] : make_double2((double)rows_loss[i], (double)keep[i]);
+    s += v.x;
+    k += v.y;
+  }
+  sums[0][threadIdx.x] = s;
+  sums[1][threadIdx.x] = k;
+  for (int h = kLossThreads / 2; h >= 1; h >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < h) {
+      sums[0][threadIdx.x] += sums[0][threadIdx.x + h];
+      sums[1][threadIdx.x] += sums[1][threadIdx.x + h];
+    }
+  }
+  if (threadIdx.x != 0) return;
+  if (out) {
+    out[blockIdx.x] = make_double2(sums[0][0], sums[1][0]);
+  } else {
+    loss[0] = (float)(mean ? sums[0][0] / sums[1][0] : sums[0][0]);
+    count[0] = (float)sums[1][0];
+  }
+}
+
+// ---------------------------------------------------------------- backward
+
+// The gradient that reaches each row's loss: upstream[0] (over count[0] for the
+// mean), or upstream[r] where the rows' losses are the output; 0 for rows that
+// do not count.
+struct RowScale {
+  const float* upstream;
+  const float* count;   // null: no mean
+  const float* keep;
+  int per_row;
+  float factor;         // distillation: the temperature
+  __device__ __forceinline__ float at(long long r) const {
+    if (keep[r] == 0.f) return 0.f;
+    const float u = upstream[per_row ? r : 0] * factor;
+    return count ? u / count[0] : u;
+  }
+};
+
+// coef[r], and scale[0..1] = (s, 1 / s), the power of two by which dz is stored
+// larger: for fp16 (`lift`) such that the largest |coef| lies in [2^14, 2^15)
+// (|dz| stays below 2^16, and probabilities below 2^-24 of it keep their bits),
+// else 1. One block.
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(1024)
+head_coef_kernel(RowScale rs, float* __restrict__ coef, float* __restrict__ scale, long long rows,
+                 int lift) {
+  __shared__ float red[1024];
+  float m = 0.f;
+  for (long long r = threadIdx.x; r < rows; r += 1024) {
+    const float v = rs.at(r);
+    coef[r] = v;
+    m = fmaxf(m, fabsf(v));
+  }
+  red[threadIdx.x] = m;
+  for (int h = 512; h >= 1; h >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < h) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + h]);
+  }
+  if (threadIdx.x == 0) {
+    m = red[0];
+    float s = 1.f;
+    if (lift && m > 0.f && m < INFINITY) {
+      int e = 0;
+      (void)frexpf(m, &e);              // m in [2^(e-1), 2^e)
+      s = ldexpf(1.f, min(max(15 - e, -126), 126));
+    }
+    scale[0] = s;
+    scale[1] = 1.f / s;
+  }
+}
+
+// out (out_rows, dim) = in (rows, dim), rows ldi apart (16-byte aligned rows of
+// whole vectors); zeros in the rows past `rows` and those whose coef is 0: what a
+// padded row holds, NaN too, does not reach dW.
+template <class T>
+__global__ void __launch_bounds__(256)
+head_copy_kernel(const elem_t<T>* __restrict__ in, long long ldi, const float* __restrict__ coef,
+                 elem_t<T>* __restrict__ out, long long rows, long long out_rows, int dim) {
+  const int per = dim / kVec<T>;
+  const long long n = out_rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
+       i += (long long)gridDim.x * 256) {
+    const long long r = i / per;
+    Vec<T> v = {};
+    if (r < rows && coef[r] != 0.f)
+      v = *reinterpret_cast<const Vec<T>*>(in + r * ldi + (i % per) * kVec<T>);
+    *reinterpret_cast<Vec<T>*>(out + i * kVec<T>) = v;
+  }
+}
+
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(256)
+head_zero_kernel(unsigned* __restrict__ out, long long n) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
+       i += (long long)gridDim.x * 256)
+    out[i] = 0u;
+}
+
+struct HeadGrad {
+  const float* lse2;       // (rows)
+  const float* coef;       // (rows)
+  const float* scale;      // [s, 1 / s]
+  const long long* ids;    // (rows, k)
+  const float* q;          // (rows, k), or null: 1
+  const float* picked;     // (rows, k)
+  int k;
+  int v0;                  // the piece's first word; M words in it
+  float c;
+  void* dz;                // (rows, ldz), or for fp32 (words, ldz)
+  long long ldz;
+};
+
+// dz at id k of row r (the piece's word v0 + word): from the logit kept in fp32,
+// so that p - q is rounded once.
+__device__ __forceinline__ float dz_at(const HeadGrad& a, long long r, int k, float coef) {
+  const long long at = r * a.k;
+  float q = 1.f;
+  if (a.q) {
+    const long long id = a.ids[at + k];
+    q = 0.f;
+    for (int j = 0; j < a.k; ++j)   // (the same word twice: both weights)
+      if (a.ids[at + j] == id) q += a.q[at + j];
+  }
+  return coef * (exp2_hw(__builtin_fmaf(a.picked[at + k], a.c, -a.lse2[r])) - q);
+}
+
+// dz of a piece, 16 bits, (rows, ldz): the tile goes through LDS, transposed
+// into rows of BM words, where the rows' ids are put right before it is stored.
+template <class T, class S>
+__global__ void __launch_bounds__(S::kThreads, 2)
+head_dz_kernel(MmArgs g, HeadGrad a) {
+  extern __shared__ float lds_f[];
+  unsigned short* const tile = reinterpret_cast<unsigned short*>(lds_f);
+  constexpr int LD = S::BM + 8;   // (16-byte rows; 4 banks on per row)
+  static_assert(S::BN * LD * 2 <= S::kLds, "the tile fits");
+  int tm, tn;
+  mm_tile(g, tm, tn);
+  const int m0 = tm * S::BM, n0 = tn * S::BN;
+  f32x16 acc[S::FM][S::FN];
+  mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  const float scale = a.scale[0];
+#pragma unroll
+  for (int j = 0; j < S::FN; ++j) {
+    const int n = wn * (S::FN * 32) + j * 32 + (lane & 31);
+    const int r = min(n0 + n, g.N - 1);
+    const float cf = a.coef[r], l2 = a.lse2[r];
+    // coef 2^(cz - lse2); an ignored row's zeros whatever its logits are
+    const float f = cf * scale;
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int m = wm * (S::FM * 32) + i * 32 + 8 * (e / 4) + 4 * (lane >> 5);
+        s16x4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float p = exp2_hw(__builtin_fmaf(acc[i][j][e + x], a.c, -l2)) * f;
+          v[x] = (short)T::from(cf == 0.f || m0 + m + x >= g.M ? 0.f : p);
+        }
+        *reinterpret_cast<s16x4*>(tile + n * LD + m) = v;
+      }
+  }
+  __syncthreads();
+  const int rows = min(S::BN, g.N - n0);
+  for (int i = threadIdx.x; i < rows * a.k; i += S::kThreads) {
+    const int n = i / a.k, k = i % a.k;
+    const long long r = n0 + n;
+    const long long word = a.ids[r * a.k + k] - a.v0 - m0;
+    if (word < 0 || word >= S::BM || m0 + word >= g.M) continue;
+    const float cf = a.coef[r];
+    if (cf != 0.f) tile[n * LD + word] = T::from(dz_at(a, r, k, cf * scale));
+  }
+  __syncthreads();
+  constexpr int CH = S::BM / 8;   // 16-byte chunks per row
+  for (int i = threadIdx.x; i < rows * CH; i += S::kThreads) {
+    const int n = i / CH, ch = i % CH;
+    *reinterpret_cast<s16x8*>(static_cast<unsigned short*>(a.dz) + (n0 + n) * a.ldz + m0 +
+                              8 * ch) = *reinterpret_cast<const s16x8*>(tile + n * LD + 8 * ch);
+  }
+}
+
+// dz of a piece in fp32, transposed: (words, ldz), rows of it contiguous.
+template <int TILE>
+__global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
+head_dz3_kernel(GemmArgs g, HeadGrad a) {
+  constexpr int F = TILE / 64;
+  int m0, n0;
+  gemm3_place<TILE>(g, m0, n0);
+  f32x16 acc[F][F];
+  gemm3_products<true, true, TILE>(acc, g, m0, n0, 0, g.K);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave >> 1, wn = wave & 1;
+  float* const dz = static_cast<float*>(a.dz);
+#pragma unroll
+  for (int j = 0; j < F; ++j) {
+    const int r = n0 + wn * (TILE / 2) + j * 32 + (lane & 31);
+    const int rc = min(r, g.N - 1);
+    const float cf = a.coef[rc], l2 = a.lse2[rc];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int m = m0 + wm * (TILE / 2) + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        const float p = exp2_hw(__builtin_fmaf(acc[i][j][e], a.c, -l2)) * cf;
+        // (columns past the rows, up to ldz: zeros for the next product)
+        if (m < g.M && r < a.ldz) dz[m * a.ldz + r] = cf == 0.f || r >= g.N ? 0.f : p;
+      }
+  }
+  __syncthreads();   // the block's stores before the ids'
+  const int rows = min(TILE, g.N - n0);
+  for (int i = threadIdx.x; i < rows * a.k; i += kGemmThreads) {
+    const int n = i / a.k, k = i % a.k;
+    const long long r = n0 + n;
+    const long long word = a.ids[r * a.k + k] - a.v0 - m0;
+    if (word < 0 || word >= TILE || m0 + word >= g.M) continue;
+    const float cf = a.coef[r];
+    if (cf != 0.f) dz[(m0 + word) * a.ldz + r] = dz_at(a, r, k, cf);
+  }
+}
+
+// What becomes of a 16-bit product: fp32 sums of split blockIdx.y (overwritten,
+// or added to for later pieces), or the rounded result times scale[1].
+struct MmOut {
+  float* part;          // (splits, M, N), or null
+  int accumulate;
+  unsigned short* out;  // (M, N) rows ldo apart
+  long long ldo;
+  const float* scale;
+};
+
+template <class T, class S, bool AK, bool BK>
+__global__ void __launch_bounds__(S::kThreads, 2)
+head_mm_kernel(MmArgs g, MmOut o) {
+  extern __shared__ float lds_f[];
+  int tm, tn;
+  mm_tile(g, tm, tn);
+  const int k_first = blockIdx.y * g.kt_per_split * kMmBK;
+  f32x16 acc[S::FM][S::FN];
+  mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
+                            min(g.K - k_first, g.kt_per_split * kMmBK),
+                            reinterpret_cast<char*>(lds_f));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int mb = tm * S::BM + wave / S::WN * (S::FM * 32) + 4 * (lane >> 5);
+  const int nb = tn * S::BN + wave % S::WN * (S::FN * 32) + (lane & 31);
+  const float scale = o.part ? 1.f : o.scale[1];
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int m = mb + i * 32 + 8 * (e / 4) + e % 4;
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) {
+        const int n = nb + j * 32;
+        if (m >= g.M || n >= g.N) continue;
+        if (o.part) {
+          float* p = o.part + ((long long)blockIdx.y * g.M + m) * g.N + n;
+          *p = o.accumulate ? *p + acc[i][j][e] : acc[i][j][e];
+        } else {
+          o.out[(long long)m * o.ldo + n] = T::from(acc[i][j][e] * scale);
+        }
+      }
+    }
+}
+
+// out (M, N; rows ldo apart) = scale[1] times the sum of the splits' sums, in
+// order, rounded; rows whose coef is 0 (coef given) are zeros.
+template <class T>
+__global__ void __launch_bounds__(256)
+head_mm_reduce_kernel(const float* __restrict__ part, unsigned short* __restrict__ out,
+                      const float* __restrict__ scale, const float* __restrict__ coef, int splits,
+                      long long M, int N, long long ldo) {
+  const long long n = M * N;
+  const float f = scale[1];
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
+       i += (long long)gridDim.x * 256) {
+    float s = part[i];
+    for (int k = 1; k < splits; ++k) s += part[k * n + i];
+    const long long m = i / N;
+    out[m * ldo + i % N] = T::from(coef && coef[m] == 0.f ? 0.f : s * f);
+  }
+}
+
+}  // namespace mhs

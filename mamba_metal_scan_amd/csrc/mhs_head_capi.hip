@@ -1,0 +1,694 @@
+// C ABI of the head's losses (declared in include/mamba_hip_scan.h): cross
+// entropy and distillation from hidden states, distillation of given logits.
+//
+// Host-side responsibilities as in mhs_capi.hip: argument checks, grids, the
+// workspace's layout, the pieces of the vocabulary. No allocation.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "mamba_hip_scan.h"
+#include "mhs_distill.hpp"
+#include "mhs_head.hpp"
+#include "mhs_host.hpp"
+
+namespace {
+
+using mhs::aligned16;
+using mhs::Bf16;
+using mhs::check_launch;
+using mhs::device_cus;
+using mhs::fail;
+using mhs::Fp16;
+using mhs::Fp32;
+using mhs::round_up;
+
+typedef mhs::MmShape<256, 128, 4, 2, 3> Shape;
+
+// Rows that the kernel for few rows takes.
+constexpr int64_t kSmallRows = 32;
+// Bytes of dz that the backward holds at a time (at least 256 words' worth).
+constexpr int64_t kPieceBytes = 256LL << 20;
+constexpr int64_t kLossOneBlock = 16384;   // rows that one block sums
+
+int elem_bytes(int dtype) { return dtype == MHS_F32 ? 4 : 2; }
+
+int check_dtype(int dtype) {
+  if (dtype != MHS_F32 && dtype != MHS_BF16 && dtype != MHS_F16)
+    return fail(MHS_EINVAL, "dtype must be MHS_F32, MHS_BF16 or MHS_F16; got %d", dtype);
+  return MHS_OK;
+}
+
+int check_reduction(int reduction) {
+  if (reduction != MHS_REDUCE_NONE && reduction != MHS_REDUCE_MEAN && reduction != MHS_REDUCE_SUM)
+    return fail(MHS_EINVAL, "reduction must be MHS_REDUCE_NONE, _MEAN or _SUM; got %d", reduction);
+  return MHS_OK;
+}
+
+// The head's sizes. Rows of hidden and weight are read 16 bytes at a time.
+struct Head {
+  int dtype;
+  int64_t rows, vocab, dim;
+  const void* hidden = nullptr;
+  const void* weight = nullptr;
+  int64_t ldh = 0, ldw = 0;
+};
+
+int check_sizes(const Head& p) {
+  int rc = check_dtype(p.dtype);
+  if (rc) return rc;
+  if (p.rows < 0 || p.vocab < 1 || p.dim < 1 || p.rows > (1LL << 30) || p.vocab > (1LL << 30))
+    return fail(MHS_EINVAL, "rows must be in [0, 2^30], vocab in [1, 2^30], dim >= 1; got %lld, "
+                "%lld, %lld", (long long)p.rows, (long long)p.vocab, (long long)p.dim);
+  const int v = 16 / elem_bytes(p.dtype);
+  if (p.dim % v || p.dim > (1LL << 20))
+    return fail(MHS_EINVAL, "dim must be a multiple of %d up to 2^20; got %lld", v,
+                (long long)p.dim);
+  // One block per tile: the grid of the products and of the rows.
+  if (((p.vocab + 63) / 64) * ((p.rows + 63) / 64) > 0x7FFFFFFF)
+    return fail(MHS_EINVAL, "%lld rows x %lld words is too large", (long long)p.rows,
+                (long long)p.vocab);
+  return MHS_OK;
+}
+
+int check_head(const Head& p) {
+  int rc = check_sizes(p);
+  if (rc) return rc;
+  if (!p.weight || (p.rows > 0 && !p.hidden)) return fail(MHS_EINVAL, "null pointer argument");
+  const int v = 16 / elem_bytes(p.dtype);
+  for (const int64_t ld : {p.ldh, p.ldw})
+    if (ld < p.dim || ld % v || ld >= (1LL << 21))
+      return fail(MHS_EINVAL, "row strides must be multiples of %d, at least dim and below 2^21; "
+                  "got %lld", v, (long long)ld);
+  if (!aligned16(p.hidden) || !aligned16(p.weight))
+    return fail(MHS_EINVAL, "hidden and weight must be 16-byte aligned");
+  return MHS_OK;
+}
+
+int check_top(int64_t top, float temperature) {
+  if (top < 1 || top > mhs::kMaxTop)
+    return fail(MHS_EINVAL, "the teacher's words per row must be in [1, %d]; got %lld",
+                mhs::kMaxTop, (long long)top);
+  if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(1.f / temperature))
+    return fail(MHS_EINVAL, "temperature must be positive and finite; got %g", temperature);
+  return MHS_OK;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (need && (!ws || have < need))
+    return fail(MHS_EINVAL, "workspace too small: %zu < %zu bytes", have, need);
+  if (need && (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(MHS_EINVAL, "workspace must be 256-byte aligned");
+  return MHS_OK;
+}
+
+// ----------------------------------------------------------------- forward
+
+// Tiles of the vocabulary in the forward's partials.
+int64_t lse_tiles(const Head& p) {
+  if (p.rows <= kSmallRows) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
+  const int bm = p.dtype == MHS_F32 ? mhs::kGemmTile : Shape::BM;
+  return (p.vocab + bm - 1) / bm;
+}
+
+size_t loss_ws(int64_t rows) {
+  return rows <= kLossOneBlock
+             ? 0
+             : round_up((size_t)((rows + mhs::kLossRows - 1) / mhs::kLossRows) * 16, 256);
+}
+
+size_t fwd_ws(const Head& p) {
+  return round_up((size_t)lse_tiles(p) * p.rows * 8, 256) + loss_ws(p.rows);
+}
+
+template <class F>
+void allow_lds(F* fn, int bytes) {
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+// Tiles in m per group of the block order (mm_tile).
+constexpr int kGroupM = 4;
+
+template <class S>
+mhs::MmArgs mm_args(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N,
+                    int64_t K) {
+  mhs::MmArgs g;
+  g.A = a;
+  g.B = b;
+  g.lda = lda;
+  g.ldb = ldb;
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.kt_per_split = (int)((K + mhs::kMmBK - 1) / mhs::kMmBK);
+  g.grid_m = (int)((M + S::BM - 1) / S::BM);
+  g.grid_n = (int)((N + S::BN - 1) / S::BN);
+  g.group_m = kGroupM;
+  return g;
+}
+
+// The logits' product for fp32: W (v0 .. v0 + words) h^T.
+mhs::GemmArgs gemm3_args(const Head& p, int64_t v0, int64_t words) {
+  mhs::GemmArgs g{};
+  g.A = static_cast<const float*>(p.weight) + v0 * p.ldw;
+  g.B = static_cast<const float*>(p.hidden);
+  g.lda = p.ldw;
+  g.ldb = p.ldh;
+  g.M = (int)words;
+  g.N = (int)p.rows;
+  g.K = (int)p.dim;
+  g.grid_m = (int)((words + mhs::kGemmTile - 1) / mhs::kGemmTile);
+  g.grid_n = (int)((p.rows + mhs::kGemmTile - 1) / mhs::kGemmTile);
+  return g;
+}
+
+template <class T>
+int launch_lse16(const Head& p, float c, float2* part, hipStream_t s) {
+  const mhs::MmArgs g = mm_args<Shape>(p.weight, p.ldw, p.hidden, p.ldh, p.vocab, p.rows, p.dim);
+  const auto fn = &mhs::head_lse_kernel<T, Shape>;
+  allow_lds(fn, Shape::kLds);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads), Shape::kLds,
+                     s, g, c, part);
+  return check_launch("head log-sum-exp kernel");
+}
+
+template <class T>
+int launch_small(const Head& p, float c, float2* part, hipStream_t s) {
+  const mhs::SmallArgs g{p.hidden, p.weight, p.ldh, p.ldw, (int)p.rows, (int)p.vocab, (int)p.dim};
+  hipLaunchKernelGGL((p.rows <= 16 ? &mhs::head_small_kernel<T, 1> : &mhs::head_small_kernel<T, 2>),
+                     dim3((unsigned)lse_tiles(p)), dim3(256), 0, s, g, c, part);
+  return check_launch("head log-sum-exp kernel of few rows");
+}
+
+int launch_lse(const Head& p, float c, float2* part, hipStream_t s) {
+  if (p.rows <= kSmallRows)
+    return p.dtype == MHS_F32    ? launch_small<Fp32>(p, c, part, s)
+           : p.dtype == MHS_BF16 ? launch_small<Bf16>(p, c, part, s)
+                                 : launch_small<Fp16>(p, c, part, s);
+  if (p.dtype == MHS_BF16) return launch_lse16<Bf16>(p, c, part, s);
+  if (p.dtype == MHS_F16) return launch_lse16<Fp16>(p, c, part, s);
+  const mhs::GemmArgs g = gemm3_args(p, 0, p.vocab);
+  hipLaunchKernelGGL(mhs::head_lse3_kernel<mhs::kGemmTile>,
+                     dim3((unsigned)g.grid_m * (unsigned)g.grid_n), dim3(mhs::kGemmThreads),
+                     mhs::gemm_lds_bytes(mhs::kGemmTile, mhs::kGemmTile), s, g, c, part);
+  return check_launch("head log-sum-exp kernel");
+}
+
+// loss[0] and count[0] from the rows' losses.
+int launch_loss(const float* rows_loss, const float* keep, float* loss, float* count, int64_t rows,
+                int reduction, void* ws, hipStream_t s) {
+  const int mean = reduction == MHS_REDUCE_MEAN;
+  if (rows <= kLossOneBlock) {
+    hipLaunchKernelGGL(mhs::head_loss_kernel<>, dim3(1), dim3(mhs::kLossThreads), 0, s, rows_loss,
+                       keep, static_cast<const double2*>(nullptr), static_cast<double2*>(nullptr),
+                       loss, count, (long long)rows, mean);
+    return check_launch("loss kernel");
+  }
+  const int64_t blocks = (rows + mhs::kLossRows - 1) / mhs::kLossRows;
+  double2* sums = static_cast<double2*>(ws);
+  hipLaunchKernelGGL(mhs::head_loss_kernel<>, dim3((unsigned)blocks), dim3(mhs::kLossThreads), 0, s,
+                     rows_loss, keep, static_cast<const double2*>(nullptr), sums, loss, count,
+                     (long long)rows, mean);
+  int rc = check_launch("loss kernel");
+  if (rc) return rc;
+  hipLaunchKernelGGL(mhs::head_loss_kernel<>, dim3(1), dim3(mhs::kLossThreads), 0, s, rows_loss,
+                     keep, static_cast<const double2*>(sums), static_cast<double2*>(nullptr), loss,
+                     count, (long long)blocks, mean);
+  return check_launch("loss kernel");
+}
+
+template <class T>
+int launch_rows(const mhs::HeadRows& g, hipStream_t s) {
+  if (g.teacher)
+    hipLaunchKernelGGL(mhs::head_distill_rows_kernel<T>, dim3((unsigned)g.rows), dim3(256),
+                       g.k * sizeof(float), s, g);
+  else
+    hipLaunchKernelGGL(mhs::head_xent_rows_kernel<T>, dim3((unsigned)((g.rows + 3) / 4)), dim3(256),
+                       0, s, g);
+  return check_launch("head rows kernel");
+}
+
+// The forward from the hidden states: g's ids, teacher and outputs are set.
+int head_fwd(const Head& p, mhs::HeadRows g, float* loss, float* count, int reduction,
+             void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_workspace(workspace, workspace_bytes, fwd_ws(p));
+  if (rc) return rc;
+  if (reduction != MHS_REDUCE_NONE && (!loss || !count))
+    return fail(MHS_EINVAL, "null pointer argument");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  float2* part = static_cast<float2*>(workspace);
+  if (p.rows > 0) {
+    if (!g.ids || !g.lse2 || !g.picked || !g.loss || !g.keep)
+      return fail(MHS_EINVAL, "null pointer argument");
+    rc = launch_lse(p, mhs::kLog2e / g.temperature, part, s);
+    if (rc) return rc;
+    g.h = p.hidden;
+    g.w = p.weight;
+    g.ldh = p.ldh;
+    g.ldw = p.ldw;
+    g.part = part;
+    g.rows = (int)p.rows;
+    g.vocab = (int)p.vocab;
+    g.dim = (int)p.dim;
+    g.tiles = (int)lse_tiles(p);
+    rc = p.dtype == MHS_F32    ? launch_rows<Fp32>(g, s)
+         : p.dtype == MHS_BF16 ? launch_rows<Bf16>(g, s)
+                               : launch_rows<Fp16>(g, s);
+    if (rc) return rc;
+  }
+  if (reduction == MHS_REDUCE_NONE) return MHS_OK;
+  return launch_loss(g.loss, g.keep, loss, count, p.rows, reduction,
+                     static_cast<char*>(workspace) + round_up((size_t)lse_tiles(p) * p.rows * 8, 256),
+                     s);
+}
+
+// ---------------------------------------------------------------- backward
+
+// Where things lie in the backward's workspace, and how it is cut up.
+struct BwdPlan {
+  int64_t piece, ldz;      // words per piece; dz's row stride
+  int64_t rows4;           // fp32: the rows, to a multiple of 4
+  int splits = 1;          // of dh's sums over a piece's words
+  int kt_per_split = 0;
+  size_t coef, hidden, dz, part, bytes;
+};
+
+int64_t piece_words(int64_t rows, int64_t vocab, int es) {
+  const int64_t fit = kPieceBytes / (std::max<int64_t>(rows, 1) * es) / 256 * 256;
+  return std::min(round_up(vocab, 256), (size_t)std::max<int64_t>(fit, 256));
+}
+
+BwdPlan bwd_plan(const Head& p) {
+  BwdPlan b;
+  const int es = elem_bytes(p.dtype);
+  b.piece = std::min<int64_t>(piece_words(p.rows, p.vocab, es), 1 << 20);
+  b.rows4 = p.dtype == MHS_F32 ? (int64_t)round_up(p.rows, 4) : p.rows;
+  b.ldz = p.dtype == MHS_F32 ? b.rows4 : b.piece;
+  b.coef = 256;
+  b.hidden = b.coef + round_up((size_t)p.rows * 4, 256);
+  b.dz = b.hidden + round_up((size_t)b.rows4 * p.dim * es, 256);
+  b.part = b.dz + round_up((size_t)(p.dtype == MHS_F32 ? b.piece * b.rows4 : p.rows * b.piece) * es,
+                           256);
+  size_t part;
+  if (p.dtype == MHS_F32) {
+    const int64_t words = std::min(b.piece, p.vocab);
+    // (the last piece may be shorter, and its products' splits other ones)
+    const int64_t last = p.vocab % b.piece ? p.vocab % b.piece : words;
+    part = 0;
+    for (const int64_t w : {words, last})
+      part = std::max({part, (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(p.rows, p.dim, w), 0),
+                       (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(w, p.dim, b.rows4), 0)});
+  } else {
+    // Splits of dh's sums such that the tiles fill the CUs: rounds of one tile
+    // per CU, each its k tiles and about 6 more for its start and end, and the
+    // partials written and read.
+    const int64_t tiles = (p.rows + Shape::BM - 1) / Shape::BM *
+                          ((p.dim + Shape::BN - 1) / Shape::BN);
+    const int64_t kt = (std::min(b.piece, p.vocab) + mhs::kMmBK - 1) / mhs::kMmBK;
+    const int cus = device_cus();
+    double best = 0;
+    for (int64_t n = 1; n <= std::min<int64_t>(16, kt); ++n) {
+      const double t = std::ceil((double)tiles * n / cus) * ((kt + n - 1) / n + 6) +
+                       n * (double)p.rows * p.dim * 8 / 4e6;   // (a k tile takes about 1 us)
+      if (n > 1 && t >= best) continue;
+      best = t;
+      b.splits = (int)n;
+      b.kt_per_split = (int)((kt + n - 1) / n);
+    }
+    b.splits = (int)((kt + b.kt_per_split - 1) / b.kt_per_split);
+    part = (size_t)b.splits * p.rows * p.dim * 4;
+  }
+  b.bytes = b.part + round_up(part, 256);
+  return b;
+}
+
+size_t bwd_ws(const Head& p) { return p.rows == 0 ? 0 : bwd_plan(p).bytes; }
+
+struct BwdOut {
+  void* dhidden;   // (rows, dim), or null
+  void* dweight;   // (vocab, dim), or null
+};
+
+template <class T>
+int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, char* ws,
+          hipStream_t s) {
+  const auto fz = &mhs::head_dz_kernel<T, Shape>;
+  const auto fh = &mhs::head_mm_kernel<T, Shape, true, false>;
+  const auto fw = &mhs::head_mm_kernel<T, Shape, false, false>;
+  allow_lds(fz, Shape::kLds);
+  allow_lds(fh, Shape::kLds);
+  allow_lds(fw, Shape::kLds);
+  typedef unsigned short u16;
+  const u16* w = static_cast<const u16*>(p.weight);
+  u16* hz = reinterpret_cast<u16*>(ws + b.hidden);
+  float* part = reinterpret_cast<float*>(ws + b.part);
+  int rc;
+  for (int64_t v0 = 0; v0 < p.vocab; v0 += b.piece) {
+    const int64_t words = std::min(b.piece, p.vocab - v0);
+    mhs::MmArgs g = mm_args<Shape>(w + v0 * p.ldw, p.ldw, p.hidden, p.ldh, words, p.rows, p.dim);
+    a.v0 = (int)v0;
+    hipLaunchKernelGGL(fz, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads),
+                       Shape::kLds, s, g, a);
+    if ((rc = check_launch("head gradient kernel")) != 0) return rc;
+    mhs::MmOut o{};
+    o.scale = a.scale;
+    if (out.dhidden) {
+      g = mm_args<Shape>(a.dz, b.ldz, w + v0 * p.ldw, p.ldw, p.rows, p.dim, words);
+      g.kt_per_split = b.kt_per_split;
+      o.part = part;
+      o.accumulate = v0 > 0;
+      hipLaunchKernelGGL(fh, dim3((unsigned)(g.grid_m * g.grid_n), (unsigned)b.splits),
+                         dim3(Shape::kThreads), Shape::kLds, s, g, o);
+      if ((rc = check_launch("hidden gradient kernel")) != 0) return rc;
+    }
+    if (out.dweight) {
+      g = mm_args<Shape>(a.dz, b.ldz, hz, p.dim, words, p.dim, p.rows);
+      o.part = nullptr;
+      o.accumulate = 0;
+      o.out = static_cast<u16*>(out.dweight) + v0 * p.dim;
+      o.ldo = p.dim;
+      hipLaunchKernelGGL(fw, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads),
+                         Shape::kLds, s, g, o);
+      if ((rc = check_launch("weight gradient kernel")) != 0) return rc;
+    }
+  }
+  if (out.dhidden) {
+    const int64_t n = p.rows * p.dim;
+    hipLaunchKernelGGL(mhs::head_mm_reduce_kernel<T>,
+                       dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, s,
+                       part, static_cast<u16*>(out.dhidden), a.scale, a.coef, b.splits,
+                       (long long)p.rows, (int)p.dim, (long long)p.dim);
+    if ((rc = check_launch("hidden gradient reduction kernel")) != 0) return rc;
+  }
+  return MHS_OK;
+}
+
+int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, char* ws,
+          hipStream_t s) {
+  const float* w = static_cast<const float*>(p.weight);
+  const float* hz = reinterpret_cast<const float*>(ws + b.hidden);
+  float* dz = static_cast<float*>(a.dz);
+  void* part = ws + b.part;
+  const size_t part_bytes = b.bytes - b.part;
+  int rc;
+  for (int64_t v0 = 0; v0 < p.vocab; v0 += b.piece) {
+    const int64_t words = std::min(b.piece, p.vocab - v0);
+    const mhs::GemmArgs g = gemm3_args(p, v0, words);
+    a.v0 = (int)v0;
+    hipLaunchKernelGGL(mhs::head_dz3_kernel<mhs::kGemmTile>,
+                       dim3((unsigned)g.grid_m * (unsigned)g.grid_n), dim3(mhs::kGemmThreads),
+                       mhs::gemm_lds_bytes(mhs::kGemmTile, mhs::kGemmTile), s, g, a);
+    if ((rc = check_launch("head gradient kernel")) != 0) return rc;
+    if (out.dhidden &&
+        (rc = mhs_gemm_f32(MHS_GEMM_TN, dz, b.ldz, w + v0 * p.ldw, p.ldw,
+                           static_cast<float*>(out.dhidden), p.dim, p.rows, p.dim, words, v0 > 0,
+                           part, part_bytes, s)) != 0)
+      return rc;
+    if (out.dweight &&
+        (rc = mhs_gemm_f32(MHS_GEMM_NN, dz, b.ldz, hz, p.dim,
+                           static_cast<float*>(out.dweight) + v0 * p.dim, p.dim, words, p.dim,
+                           b.rows4, 0, part, part_bytes, s)) != 0)
+      return rc;
+  }
+  return MHS_OK;
+}
+
+template <class T>
+int launch_hidden(const Head& p, const BwdPlan& b, const float* coef, char* ws, hipStream_t s) {
+  const int64_t n = b.rows4 * p.dim / mhs::kVec<T>;
+  hipLaunchKernelGGL(mhs::head_copy_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8192)),
+                     dim3(256), 0, s, static_cast<const mhs::elem_t<T>*>(p.hidden),
+                     (long long)p.ldh, coef, reinterpret_cast<mhs::elem_t<T>*>(ws + b.hidden),
+                     (long long)p.rows, (long long)b.rows4, (int)p.dim);
+  return check_launch("hidden copy kernel");
+}
+
+// zeros: a gradient that no row reaches.
+int launch_zero(void* p, int64_t n, int es, hipStream_t s) {
+  const int64_t words = n * es / 4;   // (dim is a multiple of 16 bytes)
+  hipLaunchKernelGGL(mhs::head_zero_kernel<>, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 4096)),
+                     dim3(256), 0, s, static_cast<unsigned*>(p), (long long)words);
+  return check_launch("zero fill kernel");
+}
+
+int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const BwdOut& out, void* workspace,
+             size_t workspace_bytes, void* stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int es = elem_bytes(p.dtype);
+  if (out.dhidden == nullptr && out.dweight == nullptr) return MHS_OK;
+  if (p.rows == 0) return out.dweight ? launch_zero(out.dweight, p.vocab * p.dim, es, s) : MHS_OK;
+  if (!a.ids || !a.lse2 || !a.picked || !rs.keep || !rs.upstream)
+    return fail(MHS_EINVAL, "null pointer argument");
+  if (!aligned16(out.dhidden) || !aligned16(out.dweight))
+    return fail(MHS_EINVAL, "dhidden and dweight must be 16-byte aligned");
+  int rc = check_workspace(workspace, workspace_bytes, bwd_ws(p));
+  if (rc) return rc;
+  const BwdPlan b = bwd_plan(p);
+  char* ws = static_cast<char*>(workspace);
+  float* scale = reinterpret_cast<float*>(ws);
+  float* coef = reinterpret_cast<float*>(ws + b.coef);
+  hipLaunchKernelGGL(mhs::head_coef_kernel<>, dim3(1), dim3(1024), 0, s, rs, coef, scale,
+                     (long long)p.rows, p.dtype == MHS_F16 ? 1 : 0);
+  if ((rc = check_launch("row coefficient kernel")) != 0) return rc;
+  if (out.dweight) {
+    rc = p.dtype == MHS_F32 ? launch_hidden<Fp32>(p, b, coef, ws, s)
+                            : launch_hidden<Bf16>(p, b, coef, ws, s);   // (a copy of 16 bits)
+    if (rc) return rc;
+  }
+  a.coef = coef;
+  a.scale = scale;
+  a.dz = ws + b.dz;
+  a.ldz = b.ldz;
+  return p.dtype == MHS_F32    ? bwd32(p, b, a, out, ws, s)
+         : p.dtype == MHS_BF16 ? bwd16<Bf16>(p, b, a, out, ws, s)
+                               : bwd16<Fp16>(p, b, a, out, ws, s);
+}
+
+mhs::RowScale row_scale(const float* upstream, const float* count, const float* keep, int reduction,
+                        float factor) {
+  mhs::RowScale rs;
+  rs.upstream = upstream;
+  rs.count = reduction == MHS_REDUCE_MEAN ? count : nullptr;
+  rs.keep = keep;
+  rs.per_row = reduction == MHS_REDUCE_NONE;
+  rs.factor = factor;
+  return rs;
+}
+
+Head head_of(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+             int64_t rows, int64_t vocab, int64_t dim) {
+  Head p;
+  p.dtype = dtype;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.dim = dim;
+  p.hidden = hidden;
+  p.weight = weight;
+  p.ldh = ldh;
+  p.ldw = ldw;
+  return p;
+}
+
+const long long* ll(const int64_t* p) { return reinterpret_cast<const long long*>(p); }
+
+template <class T>
+int launch_distill_bwd(const void* logits, int64_t ld, const int64_t* ids, const float* q,
+                       const float* lse2, const mhs::RowScale& rs, void* dlogits, int64_t rows,
+                       int64_t vocab, int64_t top, float c, hipStream_t s) {
+  hipLaunchKernelGGL(mhs::distill_bwd_kernel<T>, dim3((unsigned)rows), dim3(mhs::kXentThreads), 0, s,
+                     static_cast<const mhs::elem_t<T>*>(logits), (long long)ld, ll(ids), q, lse2, rs,
+                     static_cast<mhs::elem_t<T>*>(dlogits), (long long)vocab, (int)top, c);
+  return check_launch("distillation backward kernel");
+}
+
+int check_logits(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
+                 int64_t top, float temperature, int reduction) {
+  int rc = check_dtype(dtype);
+  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature))) return rc;
+  if (rows < 0 || rows > 0x7FFFFFFF || vocab < 1 || vocab > 0x7FFFFFFF || ld < vocab)
+    return fail(MHS_EINVAL, "rows must be in [0, 2^31), vocab in [1, 2^31) and the row stride at "
+                "least vocab; got %lld, %lld, %lld", (long long)rows, (long long)vocab,
+                (long long)ld);
+  if (rows > 0 && !logits) return fail(MHS_EINVAL, "null pointer argument");
+  if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype))
+    return fail(MHS_EINVAL, "logits must be aligned to their elements");
+  return MHS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mhs_linear_xent_fwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim) {
+  mhs::clear_error();
+  const Head p = head_of(dtype, nullptr, dim, nullptr, dim, rows, vocab, dim);
+  return check_sizes(p) ? 0 : std::max(fwd_ws(p), (size_t)256);
+}
+
+int mhs_linear_xent_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                        const int64_t* targets, float* lse2, float* picked, float* keep,
+                        float* loss_rows, float* loss, float* count, int64_t rows, int64_t vocab,
+                        int64_t dim, int64_t ignore_index, int reduction, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  mhs::clear_error();
+  const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
+  int rc = check_head(p);
+  if (rc || (rc = check_reduction(reduction))) return rc;
+  mhs::HeadRows g{};
+  g.ids = ll(targets);
+  g.lse2 = lse2;
+  g.picked = picked;
+  g.loss = loss_rows;
+  g.keep = keep;
+  g.k = 1;
+  g.ignore = ignore_index;
+  g.temperature = 1.f;
+  return head_fwd(p, g, loss, count, reduction, workspace, workspace_bytes, stream);
+}
+
+size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim) {
+  mhs::clear_error();
+  const Head p = head_of(dtype, nullptr, dim, nullptr, dim, rows, vocab, dim);
+  return check_sizes(p) ? 0 : std::max(bwd_ws(p), (size_t)256);
+}
+
+int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                        const int64_t* targets, const float* lse2, const float* picked,
+                        const float* keep, const float* upstream, const float* count,
+                        void* dhidden, void* dweight, int64_t rows, int64_t vocab, int64_t dim,
+                        int reduction, void* workspace, size_t workspace_bytes, void* stream) {
+  mhs::clear_error();
+  const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
+  int rc = check_head(p);
+  if (rc || (rc = check_reduction(reduction))) return rc;
+  if (reduction == MHS_REDUCE_MEAN && rows > 0 && !count)
+    return fail(MHS_EINVAL, "null pointer argument");
+  mhs::HeadGrad a{};
+  a.lse2 = lse2;
+  a.ids = ll(targets);
+  a.picked = picked;
+  a.k = 1;
+  a.c = mhs::kLog2e;
+  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, 1.f), BwdOut{dhidden, dweight},
+                  workspace, workspace_bytes, stream);
+}
+
+int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
+                           int64_t ldw, const float* teacher, const int64_t* ids, float* lse2,
+                           float* picked, float* q, float* keep, float* loss_rows, float* loss,
+                           float* count, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
+                           float temperature, int reduction, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  mhs::clear_error();
+  const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
+  int rc = check_head(p);
+  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature))) return rc;
+  if (rows > 0 && (!teacher || !q)) return fail(MHS_EINVAL, "null pointer argument");
+  mhs::HeadRows g{};
+  g.ids = ll(ids);
+  g.teacher = teacher;
+  g.lse2 = lse2;
+  g.picked = picked;
+  g.q = q;
+  g.loss = loss_rows;
+  g.keep = keep;
+  g.k = (int)top;
+  g.temperature = temperature;
+  return head_fwd(p, g, loss, count, reduction, workspace, workspace_bytes, stream);
+}
+
+int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
+                           int64_t ldw, const int64_t* ids, const float* lse2, const float* picked,
+                           const float* q, const float* keep, const float* upstream,
+                           const float* count, void* dhidden, void* dweight, int64_t rows,
+                           int64_t vocab, int64_t dim, int64_t top, float temperature,
+                           int reduction, void* workspace, size_t workspace_bytes, void* stream) {
+  mhs::clear_error();
+  const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
+  int rc = check_head(p);
+  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature))) return rc;
+  if (rows > 0 && (!q || (reduction == MHS_REDUCE_MEAN && !count)))
+    return fail(MHS_EINVAL, "null pointer argument");
+  mhs::HeadGrad a{};
+  a.lse2 = lse2;
+  a.ids = ll(ids);
+  a.q = q;
+  a.picked = picked;
+  a.k = (int)top;
+  a.c = mhs::kLog2e / temperature;
+  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, temperature),
+                  BwdOut{dhidden, dweight}, workspace, workspace_bytes, stream);
+}
+
+size_t mhs_distill_workspace_bytes(int64_t rows) {
+  mhs::clear_error();
+  return rows < 0 ? 0 : std::max(loss_ws(rows), (size_t)256);
+}
+
+int mhs_distill_fwd(int dtype, const void* logits, int64_t ld, const float* teacher,
+                    const int64_t* ids, float* lse2, float* q, float* keep, float* loss_rows,
+                    float* loss, float* count, int64_t rows, int64_t vocab, int64_t top,
+                    float temperature, int reduction, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  mhs::clear_error();
+  int rc = check_logits(dtype, logits, ld, rows, vocab, top, temperature, reduction);
+  if (rc) return rc;
+  if ((rows > 0 && (!teacher || !ids || !lse2 || !q || !keep || !loss_rows)) ||
+      (reduction != MHS_REDUCE_NONE && (!loss || !count)))
+    return fail(MHS_EINVAL, "null pointer argument");
+  rc = check_workspace(workspace, workspace_bytes,
+                       reduction == MHS_REDUCE_NONE ? 0 : loss_ws(rows));
+  if (rc) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows > 0) {
+    mhs::HeadRows g{};
+    g.h = logits;
+    g.ldh = ld;
+    g.ids = ll(ids);
+    g.teacher = teacher;
+    g.lse2 = lse2;
+    g.q = q;
+    g.loss = loss_rows;
+    g.keep = keep;
+    g.rows = (int)rows;
+    g.vocab = (int)vocab;
+    g.k = (int)top;
+    g.temperature = temperature;
+    const auto fn = dtype == MHS_F32    ? &mhs::distill_fwd_kernel<Fp32>
+                    : dtype == MHS_BF16 ? &mhs::distill_fwd_kernel<Bf16>
+                                        : &mhs::distill_fwd_kernel<Fp16>;
+    hipLaunchKernelGGL(fn, dim3((unsigned)rows), dim3(mhs::kXentThreads),
+                       (size_t)top * sizeof(float), s, g);
+    if ((rc = check_launch("distillation forward kernel")) != 0) return rc;
+  }
+  if (reduction == MHS_REDUCE_NONE) return MHS_OK;
+  return launch_loss(loss_rows, keep, loss, count, rows, reduction, workspace, s);
+}
+
+int mhs_distill_bwd(int dtype, const void* logits, int64_t ld, const int64_t* ids,
+                    const float* lse2, const float* q, const float* keep, const float* upstream,
+                    const float* count, void* dlogits, int64_t rows, int64_t vocab, int64_t top,
+                    float temperature, int reduction, void* stream) {
+  mhs::clear_error();
+  int rc = check_logits(dtype, logits, ld, rows, vocab, top, temperature, reduction);
+  if (rc) return rc;
+  if (rows == 0) return MHS_OK;
+  if (!ids || !lse2 || !q || !keep || !upstream || !dlogits ||
+      (reduction == MHS_REDUCE_MEAN && !count))
+    return fail(MHS_EINVAL, "null pointer argument");
+  if (dlogits == logits) return fail(MHS_EINVAL, "dlogits may not alias logits");
+  if (!aligned16(dlogits)) return fail(MHS_EINVAL, "dlogits must be 16-byte aligned");
+  const mhs::RowScale rs = row_scale(upstream, count, keep, reduction, temperature);
+  const float c = mhs::kLog2e / temperature;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == MHS_F32
+             ? launch_distill_bwd<Fp32>(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c, s)
+         : dtype == MHS_BF16
+             ? launch_distill_bwd<Bf16>(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c, s)
+             : launch_distill_bwd<Fp16>(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c,
+                                        s);
+}
+
+}  // extern "C"

@@ -1,0 +1,276 @@
+// Matrix products of 16-bit operands (bf16, fp16) on gfx950's matrix cores:
+//   acc(m, n) = sum_k A(m, k) B(n, k),  fp32 sums,
+// one BM x BN tile per block, fragments of 32 x 32 per wave; what becomes of a tile is up to the kernel's epilogue
+// (mhs_head.hpp).
+//
+// An operand is K-major ((rows, K), k contiguous) or row-major ((K, rows)); both
+// stage a k tile (32 deep) by 16-byte global loads that write LDS directly, and
+// differ in how a wave then reads its fragments: K-major with 16-byte LDS
+// reads, row-major with the transposing 8-byte reads (within 16 lanes, lane i
+// gives the address of row i / 4, columns 4 (i % 4) .. + 3 and receives column
+// i of those four rows).
+//
+// The loads go kMmStages - 1 k tiles ahead of the products: a k tile's LDS
+// buffer is refilled as soon as every wave holds its fragments in registers,
+// and one barrier per k tile both publishes the next tile and frees this one.
+#pragma once
+
+#include "mhs_common.hpp"
+#include "mhs_gemm.hpp"
+
+namespace mhs {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMmBK = 64;        // k depth of a tile: four 32x32x16 MFMAs
+
+// Element types: tags with the MFMA and the conversions.
+struct Bf16 {
+  static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned short from(float v) {
+    return __builtin_bit_cast(unsigned short, (__bf16)v);
+  }
+  static __device__ __forceinline__ float to(unsigned short u) {
+    return __uint_as_float((unsigned)u << 16);
+  }
+};
+struct Fp16 {
+  static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned short from(float v) {
+    return __builtin_bit_cast(unsigned short, (_Float16)v);
+  }
+  static __device__ __forceinline__ float to(unsigned short u) {
+    return (float)__builtin_bit_cast(_Float16, u);
+  }
+};
+
+struct MmArgs {
+  const void* A;        // K-major: (M, K) rows lda apart; else (K, M) rows lda apart
+  const void* B;        // K-major: (N, K) rows ldb apart; else (K, N) rows ldb apart
+  long long lda, ldb;   // multiples of 8; both operands 16-byte aligned
+  int M, N, K;          // a K-major operand's K, a row-major one's rows: multiples of 8
+  int kt_per_split;     // k tiles per split (blockIdx.y)
+  int grid_m, grid_n;
+  int group_m;          // tiles of a group share the operands' tiles in L2 (see mm_tile)
+};
+
+// Bytes of one operand's k tile of R rows.
+__host__ __device__ constexpr int mm_tile_bytes(int R) { return R * kMmBK * 2; }
+__host__ __device__ constexpr int mm_lds_bytes(int BM, int BN, int stages) {
+  return stages * (mm_tile_bytes(BM) + mm_tile_bytes(BN));
+}
+
+// 64 lanes x 16 bytes from memory straight into LDS at `lds` + 16 lane; lanes at
+// or past the resource's end write zeros. Not tracked by the compiler: the
+// kernel waits for it with mm_wait, and no register is written.
+__device__ __forceinline__ void mm_load_lds(i32x4 rsrc, unsigned voff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(rsrc)
+               : "m0");
+}
+
+// The wave's LDS reads done, all but its last N direct loads done, then the
+// block's barrier.
+template <int N>
+__device__ __forceinline__ void mm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// The swizzle of a K-major tile: 128-byte rows of eight 16-byte chunks, chunk c
+// of row r at place c ^ mm_swz(r), so that the 8 (and 16) lanes of one pass of a
+// 16-byte read, on consecutive rows, hit different banks.
+__device__ __forceinline__ constexpr int mm_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+// One operand of a block of WAVES waves: R rows from r0 of `rows`.
+template <int R, bool KMAJOR, int WAVES>
+struct MmOperand {
+  static constexpr int kLoads = R / 8 / WAVES; // direct loads (1 KB) per wave and k tile
+  static constexpr int kLanes = R / 8;         // row-major: lanes per k row
+  static_assert(kLoads * 8 * WAVES == R, "whole loads");
+  unsigned voff[kLoads];                       // byte offset of load j at a k tile, or kOOB
+  int kpos[kLoads];                            // the k it starts at within the tile
+  const char* base;                            // the block's rows at the next k tile to load
+  long long step;                              // bytes per k tile
+  unsigned frag;                               // byte offset of the lane's first fragment
+
+  // wrow: the wave's first row within the tile.
+  __device__ __forceinline__ MmOperand(const void* p, long long ld, int r0, int rows, int k_first,
+                                       int wave, int lane, int wrow) {
+    if constexpr (KMAJOR) {
+      base = static_cast<const char*>(p) + ((long long)r0 * ld + k_first) * 2;
+      step = kMmBK * 2;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int row = (wave * kLoads + j) * 8 + (lane >> 3);
+        const int c = (lane & 7) ^ mm_swz(row);
+        voff[j] = r0 + row < rows ? 2u * ((unsigned)row * (unsigned)ld + 8u * c) : kOOB;
+        kpos[j] = 8 * c;
+      }
+      frag = (wrow + (lane & 31)) * 128 + (((lane >> 5) ^ mm_swz(lane & 15)) << 4);
+    } else {
+      base = static_cast<const char*>(p) + ((long long)k_first * ld + r0) * 2;
+      step = ld * (2 * kMmBK);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int k = (wave * kLoads + j) * (64 / kLanes) + lane / kLanes;
+        const int c = (lane % kLanes) ^ ((k & 3) << 2);
+        voff[j] = r0 + 8 * c < rows ? 2u * ((unsigned)k * (unsigned)ld + 8u * c) : kOOB;
+        kpos[j] = k;
+      }
+      // Fragment element (row, k) of a lane: row lane % 32, k 8 (lane / 32) + 0..7;
+      // the transposing read's own address: k row 8 (lane / 32) + (lane % 16) / 4
+      // (+ 4 for its second half), 4 rows from 16 (lane / 16 % 2) + 4 (lane % 4).
+      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
+      const int row = wrow + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      frag = k * (2 * R) + ((2 * row) ^ ((k & 3) << 6));
+    }
+  }
+  // The resource over the next k tile to load, and on to the one after it.
+  __device__ __forceinline__ i32x4 next() {
+    i32x4 r;
+    const unsigned long long a = reinterpret_cast<unsigned long long>(base);
+    r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32));
+    r[2] = (int)(kOOB - 1u);
+    r[3] = 0x00020000;
+    base += step;
+    return r;
+  }
+  // Load j of that tile (`left` k's remain from its start) into LDS at byte
+  // address `lds`, the operand's buffer.
+  __device__ __forceinline__ void load(i32x4 r, int j, unsigned lds, int left, int wave) const {
+    mm_load_lds(r, kpos[j] < left ? voff[j] : kOOB, lds + (wave * kLoads + j) * 1024);
+  }
+  // Fragment f (32 rows) of the 16-deep step kk, from the operand's buffer.
+  __device__ __forceinline__ s16x8 read(const char* buf, int f, int kk) const {
+    if constexpr (KMAJOR) {
+      return *reinterpret_cast<const s16x8*>(buf + f * 4096 + (frag ^ (kk << 5)));
+    } else {
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      // (32 rows are 64 bytes, bits that the swizzle flips and wrow leaves 0
+      // where there is more than one fragment)
+      const char* p = buf + kk * (16 * 2 * R) + (frag ^ (f << 6));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 2 * R));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// The block's tile (m0, n0) of grid_m x grid_n. Blocks go round the 8 XCDs: each
+// takes a contiguous run of tiles, so that the rows of A and B it shares stay in
+// its own L2; a run goes through groups of group_m tiles in m, n after n.
+__device__ __forceinline__ void mm_tile(const MmArgs& g, int& tm, int& tn) {
+  const int tiles = g.grid_m * g.grid_n;
+  const int xcd = blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
+  const int t = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+  const int in_group = g.group_m * g.grid_n;
+  const int first = t / in_group * g.group_m;
+  const int size = min(g.group_m, g.grid_m - first);
+  const int i = t % in_group;
+  tm = first + i % size;
+  tn = i / size;
+}
+
+// A block's shape: BM x BN tile, WM x WN waves of FM x FN fragments (32 x 32),
+// ST k tiles in LDS.
+template <int BM_, int BN_, int WM_, int WN_, int ST_>
+struct MmShape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_;
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
+  static constexpr int kLds = mm_lds_bytes(BM, BN, ST);
+};
+
+// acc = the tile's sums over k's k_first .. k_first + k_len - 1. A fragment's
+// element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32. Ends on
+// a barrier, the LDS free.
+template <class T, class S, bool AK, bool BK>
+__device__ __forceinline__ void mm_products(f32x16 (&acc)[S::FM][S::FN], const MmArgs& g, int m0,
+                                            int n0, int k_first, int k_len, char* lds) {
+  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, KS = kMmBK / 16;
+  constexpr int TA = mm_tile_bytes(S::BM), BUF = TA + mm_tile_bytes(S::BN);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typedef MmOperand<S::BM, AK, S::kWaves> OA;
+  typedef MmOperand<S::BN, BK, S::kWaves> OB;
+  constexpr int LA = OA::kLoads, LB = OB::kLoads, L = LA + LB;
+  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, (wave / S::WN) * (FM * 32));
+  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, (wave % S::WN) * (FN * 32));
+  const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  const int nk = (k_len + kMmBK - 1) / kMmBK;
+#pragma unroll
+  for (int s = 0; s < ST; ++s) {
+    const i32x4 ra = a.next(), rb = b.next();
+#pragma unroll
+    for (int j = 0; j < LA; ++j) a.load(ra, j, at + s * BUF, k_len - s * kMmBK, wave);
+#pragma unroll
+    for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, k_len - s * kMmBK, wave);
+  }
+  mm_wait<(ST - 1) * L>();
+  s16x8 fa[2][FM], fb[2][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) fa[0][i] = a.read(lds, i, 0);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) fb[0][j] = b.read(lds + TA, j, 0);
+  int cur = 0;   // the buffer of tile kt
+  for (int kt = 0; kt < nk; ++kt) {
+    const int next = cur + 1 == ST ? 0 : cur + 1;
+    const int left = k_len - (kt + ST) * kMmBK;
+    i32x4 ra, rb;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if (s == KS - 1) {
+        // Tile kt + 1 has landed, and every wave holds its last fragments of
+        // tile kt: its buffer takes tile kt + ST.
+        mm_wait<(ST - 2) * L>();
+        ra = a.next();
+        rb = b.next();
+      }
+      const char* nb = lds + (s == KS - 1 ? next : cur) * BUF;
+      // A row of fragments' products at a time, with each its share of the
+      // next step's fragments and of the direct loads: the wave issues them
+      // while the matrix core works.
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        constexpr int R = FM + FN;
+#pragma unroll
+        for (int f = i * R / FM; f < (i + 1) * R / FM; ++f) {
+          if (f < FM) fa[1 - s % 2][f] = a.read(nb, f, (s + 1) % KS);
+          else fb[1 - s % 2][f - FM] = b.read(nb + TA, f - FM, (s + 1) % KS);
+        }
+        if (s == KS - 1) {
+#pragma unroll
+          for (int l = i * L / FM; l < (i + 1) * L / FM; ++l) {
+            if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
+            else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fa[s % 2][i], fb[s % 2][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    cur = next;
+  }
+  mm_wait<0>();
+}
+
+}  // namespace mhs

@@ -1,0 +1,245 @@
+"""Losses of TinyMamba's head from its hidden states, on the HIP kernels.
+
+The reference forms the head's logits and takes their cross entropy
+(mamba_metal/model.py:294-297): at the 80M model's batch (8192 rows x 32768
+words) 1.07 GB of fp32 logits and as much again for their gradient.
+``linear_cross_entropy`` computes the same loss and both gradients from the
+hidden states and the head's weight, the logits formed tile by tile on the
+matrix cores and never kept: the forward reduces each tile to its rows' maxima
+and sums of exponentials, the backward forms the tiles again, a piece of the
+vocabulary at a time, and multiplies their gradient with the weight and the
+hidden states.
+
+``distill_loss`` is the distillation of given logits from a teacher's top words,
+``linear_distill_loss`` the same from the hidden states.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from . import _native
+from ._native import REDUCE, HipScanError, dispatch
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """The 2-D t, or a copy of it whose rows the kernels read in place (zeros
+    in the columns that fill up its rows)."""
+    if _native.head_rows(t):
+        return t
+    pad = -t.shape[1] % (16 // t.element_size())
+    return F.pad(t, (0, pad)) if pad else t.clone(memory_format=torch.contiguous_format)
+
+
+def _cut(g: torch.Tensor, dim: int) -> torch.Tensor:
+    """A gradient without the columns that _rows16 added."""
+    return g if g.shape[1] == dim else g[:, :dim].contiguous()
+
+
+def _once() -> None:
+    """The gradients have none of their own: refuses a backward that is to be
+    differentiated (create_graph) rather than leave their part out."""
+    if torch.is_grad_enabled() and not torch.compiler.is_compiling():
+        raise HipScanError("the head's losses are once differentiable (create_graph is not "
+                           "supported); take the loss of the logits instead")
+
+
+def _grads(ctx, dhidden: torch.Tensor, dweight: torch.Tensor):
+    return (_cut(dhidden, ctx.dim) if ctx.needs_input_grad[0] else None,
+            _cut(dweight, ctx.dim) if ctx.needs_input_grad[1] else None)
+
+
+class LinearCrossEntropyHIP(torch.autograd.Function):
+    """Cross entropy of hidden (R, D) weight (V, D)^T against targets (R)
+    int64; rows with target == ignore_index excluded."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+        ctx.dim = hidden.shape[1]
+        ctx.reduction = reduction
+        hidden, weight = _rows16(hidden), _rows16(weight)
+        targets = targets.contiguous()
+        if not torch.compiler.is_compiling():   # (the registered op checks itself)
+            _native._check_linear_xent("linear_cross_entropy", hidden, weight, targets, reduction)
+        loss, saved = dispatch("linear_xent_fwd")(hidden, weight, targets, ignore_index,
+                                                  reduction)
+        ctx.save_for_backward(hidden, weight, targets, saved)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        _once()
+        hidden, weight, targets, saved = ctx.saved_tensors
+        return (*_grads(ctx, *dispatch("linear_xent_bwd")(
+            g.contiguous(), hidden, weight, targets, saved, ctx.reduction,
+            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None)
+
+
+class LinearDistillHIP(torch.autograd.Function):
+    """Distillation of hidden (R, D) weight (V, D)^T from the teacher's words
+    ids (R, K) and their logits."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, teacher_logits, ids, temperature, reduction):
+        ctx.dim = hidden.shape[1]
+        ctx.temperature, ctx.reduction = temperature, reduction
+        hidden, weight = _rows16(hidden), _rows16(weight)
+        if not torch.compiler.is_compiling():
+            _native._check_linear_distill("linear_distill_loss", hidden, weight, teacher_logits,
+                                          ids, temperature, reduction)
+        loss, saved = dispatch("linear_distill_fwd")(hidden, weight, teacher_logits, ids,
+                                                     temperature, reduction)
+        ctx.save_for_backward(hidden, weight, ids, saved)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        _once()
+        hidden, weight, ids, saved = ctx.saved_tensors
+        return (*_grads(ctx, *dispatch("linear_distill_bwd")(
+            g.contiguous(), hidden, weight, ids, saved, ctx.temperature, ctx.reduction,
+            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None, None)
+
+
+class DistillHIP(torch.autograd.Function):
+    """Distillation of logits (R, V) from the teacher's words ids (R, K) and
+    their logits."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, ids, temperature, reduction):
+        ctx.temperature, ctx.reduction = temperature, reduction
+        if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+            logits = logits.contiguous()
+        if not torch.compiler.is_compiling():
+            _native._check_distill("distill_loss", logits, teacher_logits, ids, temperature,
+                                   reduction)
+        loss, saved = dispatch("distill_fwd")(logits, teacher_logits, ids, temperature, reduction)
+        ctx.save_for_backward(logits, ids, saved)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        _once()
+        logits, ids, saved = ctx.saved_tensors
+        return (dispatch("distill_bwd")(g.contiguous(), logits, ids, saved, ctx.temperature,
+                                        ctx.reduction), None, None, None, None)
+
+
+def _reduction(what: str, reduction: str) -> int:
+    if reduction not in REDUCE:
+        raise ValueError(f"{what}: reduction must be 'mean', 'sum' or 'none'; got {reduction!r}")
+    return REDUCE[reduction]
+
+
+def _hip(what: str, *ts: torch.Tensor) -> None:
+    if torch.version.hip is None or not all(t.is_cuda for t in ts):
+        raise RuntimeError(f"{what} needs its tensors on the ROCm device; got "
+                           + ", ".join(str(t.device) for t in ts))
+
+
+def _head(what: str, hidden: torch.Tensor, weight: torch.Tensor):
+    """hidden as (rows, dim), and weight; both in autocast's type where that is
+    enabled, as the head's linear layer takes them."""
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: hidden must be (..., dim) and weight (vocab, dim); got "
+                         f"{tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if 0 in weight.shape:
+        raise ValueError(f"{what}: weight must not be empty; got {tuple(weight.shape)}")
+    if torch.is_autocast_enabled():
+        t = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(t), weight.to(t)
+    if hidden.dtype != weight.dtype or hidden.dtype not in _native.HEAD_DTYPES:
+        raise RuntimeError(f"{what}: hidden and weight must both be float32, bfloat16 or "
+                           f"float16; got {hidden.dtype}, {weight.dtype}")
+    return hidden.reshape(-1, hidden.shape[-1]), weight
+
+
+def _teacher(what: str, lead: torch.Size, teacher_logits: torch.Tensor,
+             teacher_ids: torch.Tensor, temperature: float):
+    """The teacher's logits (rows, k) fp32 and words (rows, k) int64, contiguous."""
+    if (teacher_ids.dim() < 1 or teacher_ids.shape != teacher_logits.shape
+            or teacher_ids.shape[:-1] != lead):
+        raise ValueError(f"{what}: teacher_logits and teacher_ids must be {tuple(lead)} + (k,); "
+                         f"got {tuple(teacher_logits.shape)}, {tuple(teacher_ids.shape)}")
+    k = teacher_ids.shape[-1]
+    if not 1 <= k <= _native.MAX_TOP:
+        raise ValueError(f"{what}: the teacher's words per row must be in "
+                         f"[1, {_native.MAX_TOP}]; got {k}")
+    if teacher_ids.is_floating_point() or teacher_ids.is_complex() \
+            or teacher_ids.dtype == torch.bool or not teacher_logits.is_floating_point():
+        raise RuntimeError(f"{what}: teacher_ids must be integers and teacher_logits floating "
+                           f"point; got {teacher_ids.dtype}, {teacher_logits.dtype}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"{what}: temperature must be positive and finite; got {temperature}")
+    return (teacher_logits.detach().to(torch.float32).reshape(-1, k).contiguous(),
+            teacher_ids.to(torch.int64).reshape(-1, k).contiguous())
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(hidden @ weight.T, targets, ignore_index=ignore_index,
+    reduction=reduction)`` without the logits: hidden (..., D) and weight (V, D)
+    in float32, bfloat16 or float16 on one ROCm device, targets (...) integers.
+
+    The loss is float32: a scalar, or with reduction "none" one per row, of
+    targets' shape (0 where ignored). Rows that are ignored add nothing to the
+    gradients, whatever they hold. A target outside [0, V) that is not
+    ignore_index makes its row's loss NaN. Under autocast hidden and weight are
+    taken in its type. The gradients are once differentiable."""
+    what = "linear_cross_entropy"
+    _hip(what, hidden, weight, targets)
+    red = _reduction(what, reduction)
+    if targets.shape != hidden.shape[:-1] or targets.is_floating_point() \
+            or targets.is_complex() or targets.dtype == torch.bool:
+        raise ValueError(f"{what}: targets must be integers of shape {tuple(hidden.shape[:-1])}; "
+                         f"got {targets.dtype} {tuple(targets.shape)}")
+    h, w = _head(what, hidden, weight)
+    loss = LinearCrossEntropyHIP.apply(h, w, targets.to(torch.int64).reshape(-1),
+                                       int(ignore_index), red)
+    return loss if red else loss.view(targets.shape)
+
+
+def linear_distill_loss(hidden: torch.Tensor, weight: torch.Tensor,
+                        teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                        temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """``distill_loss(hidden @ weight.T, ...)`` without the logits: hidden (..., D)
+    and weight (V, D) as linear_cross_entropy takes them, teacher_logits and
+    teacher_ids (..., K)."""
+    what = "linear_distill_loss"
+    _hip(what, hidden, weight, teacher_logits, teacher_ids)
+    red = _reduction(what, reduction)
+    temperature = float(temperature)
+    lead = hidden.shape[:-1]
+    t, ids = _teacher(what, lead, teacher_logits, teacher_ids, temperature)
+    h, w = _head(what, hidden, weight)
+    loss = LinearDistillHIP.apply(h, w, t, ids, temperature, red)
+    return loss if red else loss.view(lead)
+
+
+def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                 temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """Distillation of the student's logits (..., V) (float32, bfloat16 or
+    float16) from a teacher's top words: teacher_ids (..., K) and their
+    teacher_logits, K up to 1024, an id below 0 being padding.
+
+    With q = softmax(teacher_logits / temperature) over a row's kept words and
+    p = softmax(logits / temperature) over the vocabulary, a row's loss is
+    temperature^2 sum_k q_k (log q_k - log p_k), terms with q_k = 0 being 0. A
+    row that keeps no word, or whose kept logits are all -inf, has loss 0 and no
+    gradient, and the mean leaves it out (NaN where it leaves out all); an id at
+    or past V makes its row's loss NaN; a word named twice has both weights. The
+    teacher gets no gradient; the student's is once differentiable. The loss is
+    float32: a scalar, or with reduction "none" of the rows' shape."""
+    what = "distill_loss"
+    _hip(what, logits, teacher_logits, teacher_ids)
+    red = _reduction(what, reduction)
+    temperature = float(temperature)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits must be (..., vocab); got {tuple(logits.shape)}")
+    if logits.dtype not in _native.HEAD_DTYPES:
+        raise RuntimeError(f"{what}: logits must be float32, bfloat16 or float16; got "
+                           f"{logits.dtype}")
+    lead = logits.shape[:-1]
+    t, ids = _teacher(what, lead, teacher_logits, teacher_ids, temperature)
+    loss = DistillHIP.apply(logits.reshape(-1, logits.shape[-1]), t, ids, temperature, red)
+    return loss if red else loss.view(lead)
