@@ -55,27 +55,32 @@ struct alignas(16) Vec {
 
 // ------------------------------------------------------- sums of exponentials
 
-// The log-sum-exp of a column of an accumulated tile (rows of the vocabulary in
-// the lane's registers): maximum and sum in base 2 of y = c z over rows below
-// `left`, NaN in the sum wherever a logit is NaN.
-template <int FM>
-__device__ __forceinline__ void column_lse2(const f32x16 (&z)[FM], float c, int row0, int left,
-                                            float& m, float& s) {
+// The log-sum-exp of a lane's part of a column of an accumulated tile (N values,
+// value i at row row(i) of the vocabulary), in base 2 of y = c z over rows below
+// `left`. A NaN logit makes the sum NaN.
+template <int N, class Z, class R>
+__device__ __forceinline__ void column_lse2(const Z& z, const R& row, float c, int left, float& m,
+                                            float& s) {
   m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      m = fmaxf(m, row0 + i * 32 + 8 * (e / 4) + e % 4 < left ? z[i][e] * c : -INFINITY);
-  const float sh = lse2_shift(m);
   s = 0.f;
+  if (row(N - 1) < left) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < N; ++i) m = fmaxf(m, z(i));
+    m *= c;
+    const float sh = lse2_shift(m);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float y = __builtin_fmaf(z[i][e], c, -sh);
-      s += row0 + i * 32 + 8 * (e / 4) + e % 4 < left ? exp2_hw(y) : 0.f;
+    for (int i = 0; i < N; ++i) s += exp2_hw(__builtin_fmaf(z(i), c, -sh));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, row(i) < left ? z(i) : -INFINITY);
+    m *= c;
+    const float sh = lse2_shift(m);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = exp2_hw(__builtin_fmaf(z(i), c, -sh));
+      s += row(i) < left ? e : 0.f;
     }
+  }
 }
 
 // Joins the (m, s) of a tile's WM waves per column (cols columns, red: 2 WM cols
@@ -101,20 +106,22 @@ head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
   int tm, tn;
   mm_tile(g, tm, tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
-  f32x16 acc[S::FM][S::FN];
+  typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / S::WN, wn = wave % S::WN;
+  const int left = g.M - m0 - wm * (S::FM * S::MI) - 4 * (lane / S::MI);
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
-    f32x16 col[S::FM];
-#pragma unroll
-    for (int i = 0; i < S::FM; ++i) col[i] = acc[i][j];
     float m, s;
-    column_lse2<S::FM>(col, c, m0 + wm * (S::FM * 32) + 4 * (lane >> 5), g.M, m, s);
-    lse2_combine(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
-    const int n = wn * (S::FN * 32) + j * 32 + (lane & 31);
-    if (lane < 32) {
+    column_lse2<S::FM * S::E>(
+        [&](int i) { return acc[i / S::E][j][i % S::E]; },
+        [](int i) { return i / S::E * S::MI + 8 * (i % S::E / 4) + i % 4; }, c, left, m, s);
+#pragma unroll
+    for (int o = S::MI; o < 64; o *= 2)
+      lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    const int n = (wn * S::FN + j) * S::MI + lane;
+    if (lane < S::MI) {
       lds_f[2 * wm * S::BN + n] = m;
       lds_f[(2 * wm + 1) * S::BN + n] = s;
     }
@@ -137,13 +144,12 @@ head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part) {
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < F; ++j) {
-    f32x16 col[F];
-#pragma unroll
-    for (int i = 0; i < F; ++i) col[i] = acc[i][j];
     float m, s;
-    column_lse2<F>(col, c, m0 + wm * (TILE / 2) + 4 * (lane >> 5), g.M, m, s);
+    column_lse2<F * 16>([&](int i) { return acc[i / 16][j][i % 16]; },
+                        [](int i) { return i / 16 * 32 + 8 * (i % 16 / 4) + i % 4; }, c,
+                        g.M - m0 - wm * (TILE / 2) - 4 * (lane >> 5), m, s);
     lse2_combine(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
-    const int n = wn * (TILE / 2) + j * 32 + (lane & 31);
+    const int n = wn * (TILE / 2) + j * 32 + lane;
     if (lane < 32) {
       lds_f[2 * wm * TILE + n] = m;
       lds_f[(2 * wm + 1) * TILE + n] = s;
@@ -267,20 +273,29 @@ head_small_kernel(SmallArgs g, float c, float2* __restrict__ part) {
 
 // ---------------------------------------------------------------- the rows
 
-// The dot product of two rows of dim elements, over the wave's lanes; every lane
-// returns it. 16-byte accesses where both rows are aligned (dim a multiple).
-template <class T>
-__device__ __forceinline__ float wave_dot(const elem_t<T>* a, const elem_t<T>* b, int dim) {
-  float s = 0.f;
+// The dot products of row a with U rows b[u] of dim elements (16-byte aligned,
+// whole accesses) over the wave's lanes, their loads in flight together; every
+// lane returns them.
+template <class T, int U>
+__device__ __forceinline__ void wave_dots(const elem_t<T>* a, const elem_t<T>* const (&b)[U],
+                                          int dim, float (&s)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) s[u] = 0.f;
   for (int i = (threadIdx.x & 63) * kVec<T>; i < dim; i += 64 * kVec<T>) {
     const Vec<T> x = *reinterpret_cast<const Vec<T>*>(a + i);
-    const Vec<T> y = *reinterpret_cast<const Vec<T>*>(b + i);
+    Vec<T> y[U];
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) s = __builtin_fmaf(T::to(x.v[e]), T::to(y.v[e]), s);
+    for (int u = 0; u < U; ++u) y[u] = *reinterpret_cast<const Vec<T>*>(b[u] + i);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e)
+        s[u] = __builtin_fmaf(T::to(x.v[e]), T::to(y[u].v[e]), s[u]);
   }
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-  return s;
+  for (int o = 32; o >= 1; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] += __shfl_xor(s[u], o, 64);
 }
 
 struct HeadRows {
@@ -318,10 +333,10 @@ head_xent_rows_kernel(HeadRows g) {
   const float lse2 = m + log2f(s);
   const long long t = g.ids[r];
   const bool in = t >= 0 && t < g.vocab;
-  float z = 0.f;
-  if (in)
-    z = wave_dot<T>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh,
-                    static_cast<const elem_t<T>*>(g.w) + t * g.ldw, g.dim);
+  const elem_t<T>* const word[1] = {static_cast<const elem_t<T>*>(g.w) + (in ? t : 0) * g.ldw};
+  float dot[1];
+  wave_dots<T, 1>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh, word, g.dim, dot);
+  const float z = in ? dot[0] : 0.f;
   if (lane == 0) {
     const bool keep = t != g.ignore;
     g.lse2[r] = lse2;
@@ -404,15 +419,24 @@ head_distill_rows_kernel(HeadRows g) {
   __shared__ float red[4];
   const int r = blockIdx.x, wave = threadIdx.x >> 6;
   const elem_t<T>* h = static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh;
-  for (int k = wave; k < g.k; k += 4) {
-    const long long id = g.ids[(long long)r * g.k + k];
-    float z = 0.f;
-    if (id >= 0 && id < g.vocab)
-      z = wave_dot<T>(h, static_cast<const elem_t<T>*>(g.w) + id * g.ldw, g.dim);
-    if ((threadIdx.x & 63) == 0) {
-      zk[k] = z;
-      g.picked[(long long)r * g.k + k] = z;
+  constexpr int U = 4;   // words at a time (one: 138 us at 8192 x 640, 64 words; four: see below)
+  for (int k = U * wave; k < g.k; k += 4 * U) {
+    const elem_t<T>* word[U];
+    bool in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long id = k + u < g.k ? g.ids[(long long)r * g.k + k + u] : -1;
+      in[u] = id >= 0 && id < g.vocab;
+      word[u] = static_cast<const elem_t<T>*>(g.w) + (in[u] ? id : 0) * g.ldw;
     }
+    float z[U];
+    wave_dots<T, U>(h, word, g.dim, z);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((int)(threadIdx.x & 63) == u && k + u < g.k) {
+        zk[k + u] = in[u] ? z[u] : 0.f;
+        g.picked[(long long)r * g.k + k + u] = in[u] ? z[u] : 0.f;
+      }
   }
   float m = -INFINITY, s = 0.f;
   for (int t = threadIdx.x; t < g.tiles; t += 256) {
@@ -518,15 +542,15 @@ template <class T>
 __global__ void __launch_bounds__(256)
 head_copy_kernel(const elem_t<T>* __restrict__ in, long long ldi, const float* __restrict__ coef,
                  elem_t<T>* __restrict__ out, long long rows, long long out_rows, int dim) {
-  const int per = dim / kVec<T>;
-  const long long n = out_rows * per;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
-       i += (long long)gridDim.x * 256) {
-    const long long r = i / per;
-    Vec<T> v = {};
-    if (r < rows && coef[r] != 0.f)
-      v = *reinterpret_cast<const Vec<T>*>(in + r * ldi + (i % per) * kVec<T>);
-    *reinterpret_cast<Vec<T>*>(out + i * kVec<T>) = v;
+  const int per = dim / kVec<T>;   // a wave per row
+  for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < out_rows;
+       r += (long long)gridDim.x * 4) {
+    const bool keep = r < rows && coef[r] != 0.f;
+    for (int i = threadIdx.x & 63; i < per; i += 64) {
+      Vec<T> v = {};
+      if (keep) v = *reinterpret_cast<const Vec<T>*>(in + r * ldi + i * kVec<T>);
+      *reinterpret_cast<Vec<T>*>(out + r * dim + i * kVec<T>) = v;
+    }
   }
 }
 
@@ -552,69 +576,44 @@ struct HeadGrad {
   long long ldz;
 };
 
-// dz at id k of row r (the piece's word v0 + word): from the logit kept in fp32,
-// so that p - q is rounded once.
-__device__ __forceinline__ float dz_at(const HeadGrad& a, long long r, int k, float coef) {
-  const long long at = r * a.k;
-  float q = 1.f;
-  if (a.q) {
-    const long long id = a.ids[at + k];
-    q = 0.f;
-    for (int j = 0; j < a.k; ++j)   // (the same word twice: both weights)
-      if (a.ids[at + j] == id) q += a.q[at + j];
-  }
-  return coef * (exp2_hw(__builtin_fmaf(a.picked[at + k], a.c, -a.lse2[r])) - q);
-}
-
-// dz of a piece, 16 bits, (rows, ldz): the tile goes through LDS, transposed
-// into rows of BM words, where the rows' ids are put right before it is stored.
+// p's part of dz of a piece, 16 bits, (rows, ldz): the tile goes through LDS,
+// transposed into rows of BM words.
 template <class T, class S>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_dz_kernel(MmArgs g, HeadGrad a) {
   extern __shared__ float lds_f[];
   unsigned short* const tile = reinterpret_cast<unsigned short*>(lds_f);
-  constexpr int LD = S::BM + 8;   // (16-byte rows; 4 banks on per row)
-  static_assert(S::BN * LD * 2 <= S::kLds, "the tile fits");
+  constexpr int LD = S::kRow;
   int tm, tn;
   mm_tile(g, tm, tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
-  f32x16 acc[S::FM][S::FN];
+  typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / S::WN, wn = wave % S::WN;
   const float scale = a.scale[0];
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
-    const int n = wn * (S::FN * 32) + j * 32 + (lane & 31);
+    const int n = (wn * S::FN + j) * S::MI + lane % S::MI;
     const int r = min(n0 + n, g.N - 1);
-    const float cf = a.coef[r], l2 = a.lse2[r];
-    // coef 2^(cz - lse2); an ignored row's zeros whatever its logits are
-    const float f = cf * scale;
+    const float f = a.coef[r] * scale, l2 = a.lse2[r];
 #pragma unroll
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int m = wm * (S::FM * 32) + i * 32 + 8 * (e / 4) + 4 * (lane >> 5);
+      for (int e = 0; e < S::E; e += 4) {
+        const int m = (wm * S::FM + i) * S::MI + 8 * (e / 4) + 4 * (lane / S::MI);
         s16x4 v;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float p = exp2_hw(__builtin_fmaf(acc[i][j][e + x], a.c, -l2)) * f;
-          v[x] = (short)T::from(cf == 0.f || m0 + m + x >= g.M ? 0.f : p);
+          // (an ignored row's zeros whatever its logits are)
+          v[x] = (short)T::from(f == 0.f || m0 + m + x >= g.M ? 0.f : p);
         }
         *reinterpret_cast<s16x4*>(tile + n * LD + m) = v;
       }
   }
   __syncthreads();
   const int rows = min(S::BN, g.N - n0);
-  for (int i = threadIdx.x; i < rows * a.k; i += S::kThreads) {
-    const int n = i / a.k, k = i % a.k;
-    const long long r = n0 + n;
-    const long long word = a.ids[r * a.k + k] - a.v0 - m0;
-    if (word < 0 || word >= S::BM || m0 + word >= g.M) continue;
-    const float cf = a.coef[r];
-    if (cf != 0.f) tile[n * LD + word] = T::from(dz_at(a, r, k, cf * scale));
-  }
-  __syncthreads();
   constexpr int CH = S::BM / 8;   // 16-byte chunks per row
   for (int i = threadIdx.x; i < rows * CH; i += S::kThreads) {
     const int n = i / CH, ch = i % CH;
@@ -623,7 +622,7 @@ head_dz_kernel(MmArgs g, HeadGrad a) {
   }
 }
 
-// dz of a piece in fp32, transposed: (words, ldz), rows of it contiguous.
+// The same in fp32, transposed: (words, ldz), its rows contiguous.
 template <int TILE>
 __global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
 head_dz3_kernel(GemmArgs g, HeadGrad a) {
@@ -650,15 +649,33 @@ head_dz3_kernel(GemmArgs g, HeadGrad a) {
         if (m < g.M && r < a.ldz) dz[m * a.ldz + r] = cf == 0.f || r >= g.N ? 0.f : p;
       }
   }
-  __syncthreads();   // the block's stores before the ids'
-  const int rows = min(TILE, g.N - n0);
-  for (int i = threadIdx.x; i < rows * a.k; i += kGemmThreads) {
-    const int n = i / a.k, k = i % a.k;
-    const long long r = n0 + n;
-    const long long word = a.ids[r * a.k + k] - a.v0 - m0;
-    if (word < 0 || word >= TILE || m0 + word >= g.M) continue;
-    const float cf = a.coef[r];
-    if (cf != 0.f) dz[(m0 + word) * a.ldz + r] = dz_at(a, r, k, cf);
+}
+
+// dz at the rows' ids within a piece of `words` words, over what head_dz wrote:
+// coef (p - q) from the logit kept in fp32, rounded once; a word that a row names
+// twice gets both weights. A wave per row. (Within head_dz, where every tile
+// looks through its rows' ids, 64 ids a row cost 2400 us more at 8192 x 640 x
+// 32768; this takes 20.)
+template <class T>
+__global__ void __launch_bounds__(256)
+head_ids_kernel(HeadGrad a, long long rows, int words) {
+  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const float f = a.coef[r] * a.scale[0], l2 = a.lse2[r];
+  if (f == 0.f) return;
+  const long long at = r * a.k;
+  for (int k = threadIdx.x & 63; k < a.k; k += 64) {
+    const long long id = a.ids[at + k], word = id - a.v0;
+    if (word < 0 || word >= words) continue;
+    float q = 1.f;
+    if (a.q) {
+      q = 0.f;
+      for (int j = 0; j < a.k; ++j)
+        if (a.ids[at + j] == id) q += a.q[at + j];
+    }
+    const float v = f * (exp2_hw(__builtin_fmaf(a.picked[at + k], a.c, -l2)) - q);
+    elem_t<T>* const dz = static_cast<elem_t<T>*>(a.dz);
+    dz[__is_same(T, Fp32) ? word * a.ldz + r : r * a.ldz + word] = T::from(v);
   }
 }
 
@@ -679,22 +696,22 @@ head_mm_kernel(MmArgs g, MmOut o) {
   int tm, tn;
   mm_tile(g, tm, tn);
   const int k_first = blockIdx.y * g.kt_per_split * kMmBK;
-  f32x16 acc[S::FM][S::FN];
+  typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
                             min(g.K - k_first, g.kt_per_split * kMmBK),
                             reinterpret_cast<char*>(lds_f));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int mb = tm * S::BM + wave / S::WN * (S::FM * 32) + 4 * (lane >> 5);
-  const int nb = tn * S::BN + wave % S::WN * (S::FN * 32) + (lane & 31);
+  const int mb = tm * S::BM + wave / S::WN * (S::FM * S::MI) + 4 * (lane / S::MI);
+  const int nb = tn * S::BN + wave % S::WN * (S::FN * S::MI) + lane % S::MI;
   const float scale = o.part ? 1.f : o.scale[1];
 #pragma unroll
   for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int m = mb + i * 32 + 8 * (e / 4) + e % 4;
+    for (int e = 0; e < S::E; ++e) {
+      const int m = mb + i * S::MI + 8 * (e / 4) + e % 4;
 #pragma unroll
       for (int j = 0; j < S::FN; ++j) {
-        const int n = nb + j * 32;
+        const int n = nb + j * S::MI;
         if (m >= g.M || n >= g.N) continue;
         if (o.part) {
           float* p = o.part + ((long long)blockIdx.y * g.M + m) * g.N + n;

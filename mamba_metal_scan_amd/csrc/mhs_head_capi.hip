@@ -24,7 +24,7 @@ using mhs::Fp16;
 using mhs::Fp32;
 using mhs::round_up;
 
-typedef mhs::MmShape<256, 128, 4, 2, 3> Shape;
+typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1> Shape;
 
 // Rows that the kernel for few rows takes.
 constexpr int64_t kSmallRows = 32;
@@ -332,12 +332,19 @@ struct BwdOut {
 };
 
 template <class T>
+int launch_ids(const Head& p, const mhs::HeadGrad& a, int64_t words, hipStream_t s) {
+  hipLaunchKernelGGL(mhs::head_ids_kernel<T>, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s, a,
+                     (long long)p.rows, (int)words);
+  return check_launch("gradient of the ids kernel");
+}
+
+template <class T>
 int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, char* ws,
           hipStream_t s) {
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
   const auto fh = &mhs::head_mm_kernel<T, Shape, true, false>;
   const auto fw = &mhs::head_mm_kernel<T, Shape, false, false>;
-  allow_lds(fz, Shape::kLds);
+  allow_lds(fz, Shape::kTileLds);
   allow_lds(fh, Shape::kLds);
   allow_lds(fw, Shape::kLds);
   typedef unsigned short u16;
@@ -350,8 +357,9 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
     mhs::MmArgs g = mm_args<Shape>(w + v0 * p.ldw, p.ldw, p.hidden, p.ldh, words, p.rows, p.dim);
     a.v0 = (int)v0;
     hipLaunchKernelGGL(fz, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads),
-                       Shape::kLds, s, g, a);
+                       Shape::kTileLds, s, g, a);
     if ((rc = check_launch("head gradient kernel")) != 0) return rc;
+    if ((rc = launch_ids<T>(p, a, words, s)) != 0) return rc;
     mhs::MmOut o{};
     o.scale = a.scale;
     if (out.dhidden) {
@@ -401,6 +409,7 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
                        dim3((unsigned)g.grid_m * (unsigned)g.grid_n), dim3(mhs::kGemmThreads),
                        mhs::gemm_lds_bytes(mhs::kGemmTile, mhs::kGemmTile), s, g, a);
     if ((rc = check_launch("head gradient kernel")) != 0) return rc;
+    if ((rc = launch_ids<Fp32>(p, a, words, s)) != 0) return rc;
     if (out.dhidden &&
         (rc = mhs_gemm_f32(MHS_GEMM_TN, dz, b.ldz, w + v0 * p.ldw, p.ldw,
                            static_cast<float*>(out.dhidden), p.dim, p.rows, p.dim, words, v0 > 0,
@@ -417,8 +426,7 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
 
 template <class T>
 int launch_hidden(const Head& p, const BwdPlan& b, const float* coef, char* ws, hipStream_t s) {
-  const int64_t n = b.rows4 * p.dim / mhs::kVec<T>;
-  hipLaunchKernelGGL(mhs::head_copy_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8192)),
+  hipLaunchKernelGGL(mhs::head_copy_kernel<T>, dim3((unsigned)std::min<int64_t>((b.rows4 + 3) / 4, 8192)),
                      dim3(256), 0, s, static_cast<const mhs::elem_t<T>*>(p.hidden),
                      (long long)p.ldh, coef, reinterpret_cast<mhs::elem_t<T>*>(ws + b.hidden),
                      (long long)p.rows, (long long)b.rows4, (int)p.dim);

@@ -28,10 +28,15 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMmBK = 64;        // k depth of a tile: four 32x32x16 MFMAs
 
-// Element types: tags with the MFMA and the conversions.
+// Element types: tags with the MFMAs (32 x 32 x 16 and 16 x 16 x 32) and the
+// conversions.
 struct Bf16 {
   static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ unsigned short from(float v) {
@@ -44,6 +49,10 @@ struct Bf16 {
 struct Fp16 {
   static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ unsigned short from(float v) {
@@ -93,7 +102,7 @@ __device__ __forceinline__ void mm_wait() {
 __device__ __forceinline__ constexpr int mm_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
 
 // One operand of a block of WAVES waves: R rows from r0 of `rows`.
-template <int R, bool KMAJOR, int WAVES>
+template <int R, bool KMAJOR, int WAVES, int MI>
 struct MmOperand {
   static constexpr int kLoads = R / 8 / WAVES; // direct loads (1 KB) per wave and k tile
   static constexpr int kLanes = R / 8;         // row-major: lanes per k row
@@ -117,24 +126,30 @@ struct MmOperand {
         voff[j] = r0 + row < rows ? 2u * ((unsigned)row * (unsigned)ld + 8u * c) : kOOB;
         kpos[j] = 8 * c;
       }
-      frag = (wrow + (lane & 31)) * 128 + (((lane >> 5) ^ mm_swz(lane & 15)) << 4);
+      frag = (wrow + lane % MI) * 128 + ((lane / MI ^ mm_swz(lane & 15)) << 4);
     } else {
       base = static_cast<const char*>(p) + ((long long)k_first * ld + r0) * 2;
       step = ld * (2 * kMmBK);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int k = (wave * kLoads + j) * (64 / kLanes) + lane / kLanes;
-        const int c = (lane % kLanes) ^ ((k & 3) << 2);
+        const int c = (lane % kLanes) ^ swz(k);
         voff[j] = r0 + 8 * c < rows ? 2u * ((unsigned)k * (unsigned)ld + 8u * c) : kOOB;
         kpos[j] = k;
       }
-      // Fragment element (row, k) of a lane: row lane % 32, k 8 (lane / 32) + 0..7;
-      // the transposing read's own address: k row 8 (lane / 32) + (lane % 16) / 4
-      // (+ 4 for its second half), 4 rows from 16 (lane / 16 % 2) + 4 (lane % 4).
-      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
-      const int row = wrow + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      frag = k * (2 * R) + ((2 * row) ^ ((k & 3) << 6));
+      // Fragment element (row, k) of a lane: row lane % MI, k 8 (lane / MI) + 0..7;
+      // the transposing read's own address: k row 8 (lane / MI) + (lane % 16) / 4
+      // (+ 4 for its second half), 4 rows from 16 (lane % MI / 16) + 4 (lane % 4).
+      const int k = 8 * (lane / MI) + ((lane & 15) >> 2);
+      const int row = wrow + 16 * (lane % MI / 16) + 4 * (lane & 3);
+      frag = k * (2 * R) + ((2 * row) ^ (swz(k) << 4));
     }
+  }
+  // The swizzle of a row-major tile: 16-byte chunk c of k row k at place c ^
+  // swz(k), so that the k rows that one pass of the transposing reads meets
+  // (4 in a row, and with 16 x 16 fragments those 8 further) hit different banks.
+  static __device__ __forceinline__ constexpr int swz(int k) {
+    return ((k & 3) << 2) ^ (MI == 16 ? ((k >> 3) & 1) << 1 : 0);
   }
   // The resource over the next k tile to load, and on to the one after it.
   __device__ __forceinline__ i32x4 next() {
@@ -152,15 +167,15 @@ struct MmOperand {
   __device__ __forceinline__ void load(i32x4 r, int j, unsigned lds, int left, int wave) const {
     mm_load_lds(r, kpos[j] < left ? voff[j] : kOOB, lds + (wave * kLoads + j) * 1024);
   }
-  // Fragment f (32 rows) of the 16-deep step kk, from the operand's buffer.
+  // Fragment f (MI rows, 512 / MI deep) of step kk, from the operand's buffer.
   __device__ __forceinline__ s16x8 read(const char* buf, int f, int kk) const {
     if constexpr (KMAJOR) {
-      return *reinterpret_cast<const s16x8*>(buf + f * 4096 + (frag ^ (kk << 5)));
+      return *reinterpret_cast<const s16x8*>(buf + f * (MI * 128) + (frag ^ (kk * (1024 / MI))));
     } else {
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      // (32 rows are 64 bytes, bits that the swizzle flips and wrow leaves 0
-      // where there is more than one fragment)
-      const char* p = buf + kk * (16 * 2 * R) + (frag ^ (f << 6));
+      // (MI rows are 2 MI bytes, bits that the swizzle flips and wrow leaves 0
+      // where there is more than one fragment; a step's k rows are 0 mod 16)
+      const char* p = buf + kk * (512 / MI * 2 * R) + (frag ^ (f * (2 * MI)));
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 2 * R));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -183,38 +198,45 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g, int& tm, int& tn) {
   tn = i / size;
 }
 
-// A block's shape: BM x BN tile, WM x WN waves of FM x FN fragments (32 x 32),
-// ST k tiles in LDS.
-template <int BM_, int BN_, int WM_, int WN_, int ST_>
+// A block's shape: BM x BN tile, WM x WN waves of FM x FN fragments (MI x MI),
+// ST k tiles in LDS; a wave's registers hold the fragments of SUB steps (512 / MI
+// deep) while it multiplies those of the SUB steps before.
+template <int BM_, int BN_, int WM_, int WN_, int ST_, int MI_, int SUB_>
 struct MmShape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_, MI = MI_, SUB = SUB_;
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
+  static constexpr int FM = BM / WM / MI, FN = BN / WN / MI;
+  static constexpr int E = MI * MI / 64;   // a lane's elements of a fragment
+  typedef float acc __attribute__((ext_vector_type(E)));
   static constexpr int kLds = mm_lds_bytes(BM, BN, ST);
+  // The tile in 16 bits, transposed: rows of BM elements, 16 bytes (4 banks) on
+  // per row.
+  static constexpr int kRow = BM + 8;
+  static constexpr int kTileLds = kLds > BN * kRow * 2 ? kLds : BN * kRow * 2;
 };
 
 // acc = the tile's sums over k's k_first .. k_first + k_len - 1. A fragment's
-// element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32. Ends on
+// element e of lane l: row 8 (e / 4) + 4 (l / MI) + e % 4, column l % MI. Ends on
 // a barrier, the LDS free.
 template <class T, class S, bool AK, bool BK>
-__device__ __forceinline__ void mm_products(f32x16 (&acc)[S::FM][S::FN], const MmArgs& g, int m0,
-                                            int n0, int k_first, int k_len, char* lds) {
-  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, KS = kMmBK / 16;
+__device__ __forceinline__ void mm_products(typename S::acc (&acc)[S::FM][S::FN], const MmArgs& g,
+                                            int m0, int n0, int k_first, int k_len, char* lds) {
+  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, MI = S::MI, KS = kMmBK * MI / 512;
   constexpr int TA = mm_tile_bytes(S::BM), BUF = TA + mm_tile_bytes(S::BN);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  typedef MmOperand<S::BM, AK, S::kWaves> OA;
-  typedef MmOperand<S::BN, BK, S::kWaves> OB;
+  typedef MmOperand<S::BM, AK, S::kWaves, MI> OA;
+  typedef MmOperand<S::BN, BK, S::kWaves, MI> OB;
   constexpr int LA = OA::kLoads, LB = OB::kLoads, L = LA + LB;
-  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, (wave / S::WN) * (FM * 32));
-  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, (wave % S::WN) * (FN * 32));
+  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, (wave / S::WN) * (FM * MI));
+  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, (wave % S::WN) * (FN * MI));
   const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      for (int e = 0; e < S::E; ++e) acc[i][j][e] = 0.f;
   const int nk = (k_len + kMmBK - 1) / kMmBK;
 #pragma unroll
   for (int s = 0; s < ST; ++s) {
@@ -225,46 +247,54 @@ __device__ __forceinline__ void mm_products(f32x16 (&acc)[S::FM][S::FN], const M
     for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, k_len - s * kMmBK, wave);
   }
   mm_wait<(ST - 1) * L>();
-  s16x8 fa[2][FM], fb[2][FN];
+  constexpr int SUB = S::SUB, PH = KS / SUB;   // phases of SUB steps per k tile
+  static_assert(PH * SUB == KS && PH % 2 == 0, "the register sets alternate within a k tile");
+  s16x8 fa[2][SUB][FM], fb[2][SUB][FN];
 #pragma unroll
-  for (int i = 0; i < FM; ++i) fa[0][i] = a.read(lds, i, 0);
+  for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-  for (int j = 0; j < FN; ++j) fb[0][j] = b.read(lds + TA, j, 0);
+    for (int i = 0; i < FM; ++i) fa[0][u][i] = a.read(lds, i, u);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[0][u][j] = b.read(lds + TA, j, u);
+  }
   int cur = 0;   // the buffer of tile kt
   for (int kt = 0; kt < nk; ++kt) {
     const int next = cur + 1 == ST ? 0 : cur + 1;
     const int left = k_len - (kt + ST) * kMmBK;
     i32x4 ra, rb;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if (s == KS - 1) {
+    for (int p = 0; p < PH; ++p) {
+      if (p == PH - 1) {
         // Tile kt + 1 has landed, and every wave holds its last fragments of
         // tile kt: its buffer takes tile kt + ST.
         mm_wait<(ST - 2) * L>();
         ra = a.next();
         rb = b.next();
       }
-      const char* nb = lds + (s == KS - 1 ? next : cur) * BUF;
+      const char* nb = lds + (p == PH - 1 ? next : cur) * BUF;
       // A row of fragments' products at a time, with each its share of the
-      // next step's fragments and of the direct loads: the wave issues them
+      // next phase's fragments and of the direct loads: the wave issues them
       // while the matrix core works.
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        constexpr int R = FM + FN;
+      for (int q = 0; q < SUB * FM; ++q) {
+        constexpr int F = FM + FN, R = SUB * F;
+        const int u = q / FM, i = q % FM;
 #pragma unroll
-        for (int f = i * R / FM; f < (i + 1) * R / FM; ++f) {
-          if (f < FM) fa[1 - s % 2][f] = a.read(nb, f, (s + 1) % KS);
-          else fb[1 - s % 2][f - FM] = b.read(nb + TA, f - FM, (s + 1) % KS);
+        for (int x = q * R / (SUB * FM); x < (q + 1) * R / (SUB * FM); ++x) {
+          const int step = (p + 1) % PH * SUB + x / F, f = x % F;
+          if (f < FM) fa[1 - p % 2][x / F][f] = a.read(nb, f, step);
+          else fb[1 - p % 2][x / F][f - FM] = b.read(nb + TA, f - FM, step);
         }
-        if (s == KS - 1) {
+        if (p == PH - 1) {
 #pragma unroll
-          for (int l = i * L / FM; l < (i + 1) * L / FM; ++l) {
+          for (int l = q * L / (SUB * FM); l < (q + 1) * L / (SUB * FM); ++l) {
             if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
             else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
           }
         }
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fa[s % 2][i], fb[s % 2][j], acc[i][j]);
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = T::mfma(fa[p % 2][u][i], fb[p % 2][u][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
