@@ -472,8 +472,9 @@ int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* 
  *   loss_rows[r] = t^2 sum_k q_k (ln q_k - ln p[ids_k])
  * (terms with q_k = 0 are 0). A row that keeps no id, or whose kept logits are all
  * -inf, is empty: loss 0, keep 0; an id at or past vocab makes the row's loss NaN.
- * Outputs as above, and q, picked (rows, top) and lse2 = log2 sum_v exp(z / t) for
- * the backward; dz[r, v] = t (p[v] - sum_{ids_k = v} q_k) times the gradient that
+ * Outputs as above, and for the backward picked (rows, top), lse2 = log2 sum_v
+ * exp(z / t) and q (rows, top), each word's whole weight in its row (a word that a
+ * row names twice has the sum at both); dz[r, v] = t (p[v] - sum_{ids_k = v} q_k) times the gradient that
  * reaches the row's loss. The teacher gets no gradient. The workspaces are the
  * cross entropy's. No counterpart in the reference.
  */

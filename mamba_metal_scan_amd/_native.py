@@ -332,10 +332,11 @@ def _need(ok: bool, what: str, msg: str) -> None:
 
 
 def _on_one_device(what: str, *ts: Optional[torch.Tensor]) -> None:
-    ts = [t for t in ts if t is not None]
-    dev = ts[0].device
-    _need(dev.type == "cuda" and all(t.device == dev for t in ts), what,
-          "every tensor must be on one ROCm device; got " + ", ".join(str(t.device) for t in ts))
+    devs = [t.device for t in ts if t is not None]
+    dev = devs[0]
+    if dev.type != "cuda" or devs.count(dev) != len(devs):
+        raise HipScanError(f"{what}: every tensor must be on one ROCm device; got "
+                           + ", ".join(map(str, devs)))
 
 
 def _dense(what: str, **ts: Optional[torch.Tensor]) -> None:
@@ -1295,32 +1296,35 @@ def _saved_size(rows: int, *tops: int) -> int:
 
 def _check_head(what: str, hidden, weight, reduction) -> None:
     _on_one_device(what, hidden, weight)
-    _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1], what,
-          f"hidden must be (rows, dim) and weight (vocab, dim); got {tuple(hidden.shape)}, "
-          f"{tuple(weight.shape)}")
-    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, what,
-          f"weight must not be empty; got {tuple(weight.shape)}")
-    _need(hidden.dtype in HEAD_DTYPES and weight.dtype == hidden.dtype, what,
-          "hidden and weight must both be float32, bfloat16 or float16; got "
-          f"{hidden.dtype}, {weight.dtype}")
+    if not (hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1]):
+        raise HipScanError(f"{what}: hidden must be (rows, dim) and weight (vocab, dim); got "
+                           f"{tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if weight.numel() == 0:
+        raise HipScanError(f"{what}: weight must not be empty; got {tuple(weight.shape)}")
+    if not (hidden.dtype in HEAD_DTYPES and weight.dtype == hidden.dtype):
+        raise HipScanError(f"{what}: hidden and weight must both be float32, bfloat16 or "
+                           f"float16; got {hidden.dtype}, {weight.dtype}")
     for name, t in (("hidden", hidden), ("weight", weight)):
-        _need(t.numel() == 0 or head_rows(t), what,
-              f"{name} needs rows of whole 16-byte accesses, 16-byte aligned and less than "
-              f"2^21 elements apart; got shape {tuple(t.shape)}, strides {t.stride()}")
-    _need(reduction in REDUCE.values(), what, f"reduction must be 0, 1 or 2; got {reduction!r}")
+        if t.numel() != 0 and not head_rows(t):
+            raise HipScanError(f"{what}: {name} needs rows of whole 16-byte accesses, 16-byte "
+                               f"aligned and less than 2^21 elements apart; got shape "
+                               f"{tuple(t.shape)}, strides {t.stride()}")
+    if reduction not in (0, 1, 2):
+        raise HipScanError(f"{what}: reduction must be 0, 1 or 2; got {reduction!r}")
 
 
 def _check_top(what: str, rows: int, teacher_logits, ids, temperature) -> None:
-    _need(ids.dim() == 2 and ids.shape[0] == rows and 1 <= ids.shape[1] <= MAX_TOP, what,
-          f"the teacher's words must be ({rows}, k) with k in [1, {MAX_TOP}]; got "
-          f"{tuple(ids.shape)}")
-    _need(ids.dtype == torch.int64, what, f"the teacher's words must be int64; got {ids.dtype}")
+    if not (ids.dim() == 2 and ids.shape[0] == rows and 1 <= ids.shape[1] <= MAX_TOP):
+        raise HipScanError(f"{what}: the teacher's words must be ({rows}, k) with k in "
+                           f"[1, {MAX_TOP}]; got {tuple(ids.shape)}")
+    if ids.dtype != torch.int64:
+        raise HipScanError(f"{what}: the teacher's words must be int64; got {ids.dtype}")
     _dense(what, teacher_ids=ids, teacher_logits=teacher_logits)
     if teacher_logits is not None:
         _fp32(what, teacher_logits=teacher_logits)
         _shaped(what, "teacher_logits", teacher_logits, ids.shape)
-    _need(temperature > 0 and temperature < float("inf"), what,
-          f"temperature must be positive and finite; got {temperature}")
+    if not 0 < temperature < float("inf"):
+        raise HipScanError(f"{what}: temperature must be positive and finite; got {temperature}")
 
 
 def _check_bwd_head(what: str, grad, saved, rows: int, reduction: int, *tops: int) -> None:
@@ -1368,7 +1372,8 @@ def _check_linear_xent(what: str, hidden, weight, targets, reduction) -> None:
     _check_head(what, hidden, weight, reduction)
     _on_one_device(what, hidden, targets)
     _shaped(what, "targets", targets, (hidden.shape[0],))
-    _need(targets.dtype == torch.int64, what, f"targets must be int64; got {targets.dtype}")
+    if targets.dtype != torch.int64:
+        raise HipScanError(f"{what}: targets must be int64; got {targets.dtype}")
     _dense(what, targets=targets)
 
 
@@ -1547,14 +1552,17 @@ def _distill_fwd_impl(logits: torch.Tensor, teacher_logits: torch.Tensor, ids: t
 
 def _check_distill(what: str, logits, teacher_logits, ids, temperature, reduction) -> None:
     _on_one_device(what, logits, teacher_logits, ids)
-    _need(logits.dim() == 2 and logits.shape[1] >= 1, what,
-          f"logits must be (rows, vocab); got {tuple(logits.shape)}")
-    _need(logits.dtype in HEAD_DTYPES, what,
-          f"logits must be float32, bfloat16 or float16; got {logits.dtype}")
-    _need(logits.stride(1) == 1 and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1]),
-          what, f"logits need contiguous rows; got strides {logits.stride()}")
+    if not (logits.dim() == 2 and logits.shape[1] >= 1):
+        raise HipScanError(f"{what}: logits must be (rows, vocab); got {tuple(logits.shape)}")
+    if logits.dtype not in HEAD_DTYPES:
+        raise HipScanError(f"{what}: logits must be float32, bfloat16 or float16; got "
+                           f"{logits.dtype}")
+    if not (logits.stride(1) == 1
+            and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1])):
+        raise HipScanError(f"{what}: logits need contiguous rows; got strides {logits.stride()}")
     _check_top(what, logits.shape[0], teacher_logits, ids, temperature)
-    _need(reduction in REDUCE.values(), what, f"reduction must be 0, 1 or 2; got {reduction!r}")
+    if reduction not in (0, 1, 2):
+        raise HipScanError(f"{what}: reduction must be 0, 1 or 2; got {reduction!r}")
 
 
 distill_fwd = _register(

@@ -109,7 +109,7 @@ head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
   typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave / S::WN, wn = wave % S::WN;
+  const int wm = S::wave_m(wave), wn = S::wave_n(wave);
   const int left = g.M - m0 - wm * (S::FM * S::MI) - 4 * (lane / S::MI);
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
@@ -307,7 +307,7 @@ struct HeadRows {
   const float* teacher;   // (rows, k) the teacher's logits
   float* lse2;            // (rows)
   float* picked;          // (rows, k) logits of the ids
-  float* q;               // (rows, k) the teacher's probabilities
+  float* q;               // (rows, k) the words' weights, see teacher_row
   float* loss;            // (rows)
   float* keep;            // (rows) 1: the row counts, 0: ignored or empty
   int rows, vocab, dim, k, tiles;
@@ -364,11 +364,13 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// The teacher's probabilities of row r over its kept words (id >= 0), to q, and
-// the row's loss from the student's logits zk at the ids (LDS) and lse2. A row
-// that keeps no word, or whose kept logits are all -inf, is empty: loss 0,
-// probabilities 0. An id at or past the vocabulary: NaN.
-__device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2, const float* zk,
+// The teacher's probabilities of row r over its kept words (id >= 0), and the
+// row's loss from the student's logits zk at the ids (LDS, k floats, then room
+// for k more) and lse2. To q goes each word's whole weight in the row: a word
+// that the row names twice has both entries' sum at each. A row that keeps no
+// word, or whose kept logits are all -inf, is empty: loss 0, probabilities 0. An
+// id at or past the vocabulary: NaN.
+__device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2, float* zk,
                                             float* red) {
   const long long at = (long long)r * g.k;
   const float c = kLog2e / g.temperature;
@@ -400,9 +402,15 @@ __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2
       if (q != 0.f)
         loss += q * ((y - log2s + lse2) * kLn2 - zk[k] / g.temperature);
     }
+    zk[g.k + k] = q;
+  }
+  loss = block_sum(loss, red);   // (its barriers publish the q's)
+  for (int k = threadIdx.x; k < g.k; k += 256) {
+    const long long id = g.ids[at + k];
+    float q = 0.f;
+    for (int j = 0; j < g.k; ++j) q += g.ids[at + j] == id ? zk[g.k + j] : 0.f;
     g.q[at + k] = q;
   }
-  loss = block_sum(loss, red);
   if (threadIdx.x == 0) {
     g.lse2[r] = lse2;
     g.keep[r] = any;
@@ -415,7 +423,7 @@ __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2
 template <class T>
 __global__ void __launch_bounds__(256)
 head_distill_rows_kernel(HeadRows g) {
-  extern __shared__ float zk[];   // k floats
+  extern __shared__ float zk[];   // 2 k floats
   __shared__ float red[4];
   const int r = blockIdx.x, wave = threadIdx.x >> 6;
   const elem_t<T>* h = static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh;
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(kLossThreads)
 head_loss_kernel(const float* __restrict__ rows_loss, const float* __restrict__ keep,
                  const double2* __restrict__ in, double2* __restrict__ out,
                  float* __restrict__ loss, float* __restrict__ count, long long n, int mean) {
-  __shared__ double sums[2][kLossThreads];
+  __shared__ double sums[2][kLossThreads / 64];
   double s = 0.0, k = 0.0;
   const long long first = (long long)blockIdx.x * kLossRows;
   const long long end = out ? min(n, first + kLossRows) : n;
@@ -466,21 +474,26 @@ head_loss_kernel(const float* __restrict__ rows_loss, const float* __restrict__ 
     s += v.x;
     k += v.y;
   }
-  sums[0][threadIdx.x] = s;
-  sums[1][threadIdx.x] = k;
-  for (int h = kLossThreads / 2; h >= 1; h >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < h) {
-      sums[0][threadIdx.x] += sums[0][threadIdx.x + h];
-      sums[1][threadIdx.x] += sums[1][threadIdx.x + h];
-    }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    k += __shfl_xor(k, o, 64);
   }
+  if ((threadIdx.x & 63) == 0) {
+    sums[0][threadIdx.x >> 6] = s;
+    sums[1][threadIdx.x >> 6] = k;
+  }
+  __syncthreads();
   if (threadIdx.x != 0) return;
+  for (int w = 1; w < kLossThreads / 64; ++w) {
+    s += sums[0][w];
+    k += sums[1][w];
+  }
   if (out) {
-    out[blockIdx.x] = make_double2(sums[0][0], sums[1][0]);
+    out[blockIdx.x] = make_double2(s, k);
   } else {
-    loss[0] = (float)(mean ? sums[0][0] / sums[1][0] : sums[0][0]);
-    count[0] = (float)sums[1][0];
+    loss[0] = (float)(mean ? s / k : s);
+    count[0] = (float)k;
   }
 }
 
@@ -495,62 +508,76 @@ struct RowScale {
   const float* keep;
   int per_row;
   float factor;         // distillation: the temperature
-  __device__ __forceinline__ float at(long long r) const {
-    if (keep[r] == 0.f) return 0.f;
+  __device__ __forceinline__ float reaching(long long r) const {
     const float u = upstream[per_row ? r : 0] * factor;
     return count ? u / count[0] : u;
   }
+  __device__ __forceinline__ float at(long long r) const {
+    return keep[r] == 0.f ? 0.f : reaching(r);
+  }
 };
 
-// coef[r], and scale[0..1] = (s, 1 / s), the power of two by which dz is stored
-// larger: for fp16 (`lift`) such that the largest |coef| lies in [2^14, 2^15)
-// (|dz| stays below 2^16, and probabilities below 2^-24 of it keep their bits),
-// else 1. One block.
+// largest[0] = the largest |gradient| that reaches a row (per-row upstreams of
+// fp16 products). One block.
 template <int UNUSED = 0>
 __global__ void __launch_bounds__(1024)
-head_coef_kernel(RowScale rs, float* __restrict__ coef, float* __restrict__ scale, long long rows,
-                 int lift) {
-  __shared__ float red[1024];
+head_largest_kernel(RowScale rs, float* __restrict__ largest, long long rows) {
+  __shared__ float red[16];
   float m = 0.f;
-  for (long long r = threadIdx.x; r < rows; r += 1024) {
-    const float v = rs.at(r);
-    coef[r] = v;
-    m = fmaxf(m, fabsf(v));
+  for (long long r = threadIdx.x; r < rows; r += 1024) m = fmaxf(m, fabsf(rs.at(r)));
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
+  largest[0] = m;
+}
+
+// The power of two by which dz is stored larger, for fp16: such that the largest
+// |coef| lies in [2^14, 2^15) (|dz| stays below 2^16, and probabilities below
+// 2^-24 of it keep their bits); 1 where that is 0 or not finite.
+__device__ __forceinline__ float lift_of(float largest) {
+  if (!(largest > 0.f && largest < INFINITY)) return 1.f;
+  int e = 0;
+  (void)frexpf(largest, &e);   // largest in [2^(e-1), 2^e)
+  return ldexpf(1.f, min(max(15 - e, -126), 126));
+}
+
+constexpr int kCopyRows = 8;   // rows per block
+
+// coef[r]; scale[0..1] = (s, 1 / s), dz's power of two (lift: fp16; scale[2] the
+// largest per-row gradient), else 1; and, `out` given, out (out_rows, per) = in
+// (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
+// `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
+// reach dW.
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(256)
+head_rows_in_kernel(const uint4* __restrict__ in, long long ldi, RowScale rs,
+                    float* __restrict__ coef, float* __restrict__ scale, uint4* __restrict__ out,
+                    long long rows, long long out_rows, int per, int lift) {
+  __shared__ float cf[kCopyRows];
+  const long long r0 = (long long)blockIdx.x * kCopyRows;
+  if (threadIdx.x < kCopyRows) {
+    const long long r = r0 + threadIdx.x;
+    const float c = r < rows ? rs.at(r) : 0.f;
+    cf[threadIdx.x] = c;
+    if (r < rows) coef[r] = c;
   }
-  red[threadIdx.x] = m;
-  for (int h = 512; h >= 1; h >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < h) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + h]);
-  }
-  if (threadIdx.x == 0) {
-    m = red[0];
-    float s = 1.f;
-    if (lift && m > 0.f && m < INFINITY) {
-      int e = 0;
-      (void)frexpf(m, &e);              // m in [2^(e-1), 2^e)
-      s = ldexpf(1.f, min(max(15 - e, -126), 126));
-    }
+  if (blockIdx.x == 0 && threadIdx.x == 64) {
+    // (without per-row gradients the largest is the one that every kept row has)
+    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : fabsf(rs.reaching(0)));
     scale[0] = s;
     scale[1] = 1.f / s;
   }
-}
-
-// out (out_rows, dim) = in (rows, dim), rows ldi apart (16-byte aligned rows of
-// whole vectors); zeros in the rows past `rows` and those whose coef is 0: what a
-// padded row holds, NaN too, does not reach dW.
-template <class T>
-__global__ void __launch_bounds__(256)
-head_copy_kernel(const elem_t<T>* __restrict__ in, long long ldi, const float* __restrict__ coef,
-                 elem_t<T>* __restrict__ out, long long rows, long long out_rows, int dim) {
-  const int per = dim / kVec<T>;   // a wave per row
-  for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < out_rows;
-       r += (long long)gridDim.x * 4) {
-    const bool keep = r < rows && coef[r] != 0.f;
-    for (int i = threadIdx.x & 63; i < per; i += 64) {
-      Vec<T> v = {};
-      if (keep) v = *reinterpret_cast<const Vec<T>*>(in + r * ldi + i * kVec<T>);
-      *reinterpret_cast<Vec<T>*>(out + r * dim + i * kVec<T>) = v;
-    }
+  if (!out) return;
+  __syncthreads();
+  const int n = (int)min((long long)kCopyRows, out_rows - r0) * per;   // (dim <= 2^20)
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int row = i / per;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (cf[row] != 0.f) v = in[(r0 + row) * ldi + i - row * per];
+    out[r0 * per + i] = v;
   }
 }
 
@@ -567,7 +594,7 @@ struct HeadGrad {
   const float* coef;       // (rows)
   const float* scale;      // [s, 1 / s]
   const long long* ids;    // (rows, k)
-  const float* q;          // (rows, k), or null: 1
+  const float* q;          // (rows, k) the words' whole weights, or null: 1
   const float* picked;     // (rows, k)
   int k;
   int v0;                  // the piece's first word; M words in it
@@ -590,7 +617,7 @@ head_dz_kernel(MmArgs g, HeadGrad a) {
   typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave / S::WN, wn = wave % S::WN;
+  const int wm = S::wave_m(wave), wn = S::wave_n(wave);
   const float scale = a.scale[0];
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
@@ -652,8 +679,8 @@ head_dz3_kernel(GemmArgs g, HeadGrad a) {
 }
 
 // dz at the rows' ids within a piece of `words` words, over what head_dz wrote:
-// coef (p - q) from the logit kept in fp32, rounded once; a word that a row names
-// twice gets both weights. A wave per row. (Within head_dz, where every tile
+// coef (p - q) from the logit kept in fp32, rounded once (a word that a row names
+// twice: the same value twice). A wave per row. (Within head_dz, where every tile
 // looks through its rows' ids, 64 ids a row cost 2400 us more at 8192 x 640 x
 // 32768; this takes 20.)
 template <class T>
@@ -665,14 +692,9 @@ head_ids_kernel(HeadGrad a, long long rows, int words) {
   if (f == 0.f) return;
   const long long at = r * a.k;
   for (int k = threadIdx.x & 63; k < a.k; k += 64) {
-    const long long id = a.ids[at + k], word = id - a.v0;
+    const long long word = a.ids[at + k] - a.v0;
     if (word < 0 || word >= words) continue;
-    float q = 1.f;
-    if (a.q) {
-      q = 0.f;
-      for (int j = 0; j < a.k; ++j)
-        if (a.ids[at + j] == id) q += a.q[at + j];
-    }
+    const float q = a.q ? a.q[at + k] : 1.f;
     const float v = f * (exp2_hw(__builtin_fmaf(a.picked[at + k], a.c, -l2)) - q);
     elem_t<T>* const dz = static_cast<elem_t<T>*>(a.dz);
     dz[__is_same(T, Fp32) ? word * a.ldz + r : r * a.ldz + word] = T::from(v);
@@ -695,14 +717,14 @@ head_mm_kernel(MmArgs g, MmOut o) {
   extern __shared__ float lds_f[];
   int tm, tn;
   mm_tile(g, tm, tn);
-  const int k_first = blockIdx.y * g.kt_per_split * kMmBK;
+  const int k_first = blockIdx.y * g.kt_per_split * S::BK;
   typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
-                            min(g.K - k_first, g.kt_per_split * kMmBK),
+                            min(g.K - k_first, g.kt_per_split * S::BK),
                             reinterpret_cast<char*>(lds_f));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int mb = tm * S::BM + wave / S::WN * (S::FM * S::MI) + 4 * (lane / S::MI);
-  const int nb = tn * S::BN + wave % S::WN * (S::FN * S::MI) + lane % S::MI;
+  const int mb = tm * S::BM + S::wave_m(wave) * (S::FM * S::MI) + 4 * (lane / S::MI);
+  const int nb = tn * S::BN + S::wave_n(wave) * (S::FN * S::MI) + lane % S::MI;
   const float scale = o.part ? 1.f : o.scale[1];
 #pragma unroll
   for (int i = 0; i < S::FM; ++i)
@@ -723,21 +745,23 @@ head_mm_kernel(MmArgs g, MmOut o) {
     }
 }
 
-// out (M, N; rows ldo apart) = scale[1] times the sum of the splits' sums, in
-// order, rounded; rows whose coef is 0 (coef given) are zeros.
+// out (M, 4 N4) = scale[1] times the sum of the splits' sums, in order, rounded;
+// rows whose coef is 0 are zeros.
 template <class T>
 __global__ void __launch_bounds__(256)
-head_mm_reduce_kernel(const float* __restrict__ part, unsigned short* __restrict__ out,
+head_mm_reduce_kernel(const float4* __restrict__ part, ushort4* __restrict__ out,
                       const float* __restrict__ scale, const float* __restrict__ coef, int splits,
-                      long long M, int N, long long ldo) {
-  const long long n = M * N;
+                      long long M, int N4) {
+  const long long n = M * N4;
   const float f = scale[1];
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
        i += (long long)gridDim.x * 256) {
-    float s = part[i];
-    for (int k = 1; k < splits; ++k) s += part[k * n + i];
-    const long long m = i / N;
-    out[m * ldo + i % N] = T::from(coef && coef[m] == 0.f ? 0.f : s * f);
+    float4 s = part[i];
+    for (int k = 1; k < splits; ++k) s = add(s, part[k * n + i]);
+    const bool zero = coef[i / N4] == 0.f;
+    out[i] = zero ? make_ushort4(0, 0, 0, 0)
+                  : make_ushort4(T::from(s.x * f), T::from(s.y * f), T::from(s.z * f),
+                                 T::from(s.w * f));
   }
 }
 

@@ -24,11 +24,15 @@ using mhs::Fp16;
 using mhs::Fp32;
 using mhs::round_up;
 
-typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1> Shape;
+typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64, false> Shape;
+typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64, true> HalfShape;   // (the gradients')
 
 // Rows that the kernel for few rows takes.
 constexpr int64_t kSmallRows = 32;
-// Bytes of dz that the backward holds at a time (at least 256 words' worth).
+// Bytes of dz that the backward holds at a time (at least 256 words' worth). us
+// with 64, 128, 256 and 512 MB: 8192 x 640 x 32768 bf16 2550, 1780, 1559, 1589;
+// 8192 x 4096 x 131072 29520, 27080, 26130, 25700; fp32 (the first) 8640, 7755,
+// 7407, 7257.
 constexpr int64_t kPieceBytes = 256LL << 20;
 constexpr int64_t kLossOneBlock = 16384;   // rows that one block sums
 
@@ -142,7 +146,7 @@ mhs::MmArgs mm_args(const void* a, int64_t lda, const void* b, int64_t ldb, int6
   g.M = (int)M;
   g.N = (int)N;
   g.K = (int)K;
-  g.kt_per_split = (int)((K + mhs::kMmBK - 1) / mhs::kMmBK);
+  g.kt_per_split = (int)((K + S::BK - 1) / S::BK);
   g.grid_m = (int)((M + S::BM - 1) / S::BM);
   g.grid_n = (int)((N + S::BN - 1) / S::BN);
   g.group_m = kGroupM;
@@ -223,7 +227,7 @@ template <class T>
 int launch_rows(const mhs::HeadRows& g, hipStream_t s) {
   if (g.teacher)
     hipLaunchKernelGGL(mhs::head_distill_rows_kernel<T>, dim3((unsigned)g.rows), dim3(256),
-                       g.k * sizeof(float), s, g);
+                       2 * g.k * sizeof(float), s, g);
   else
     hipLaunchKernelGGL(mhs::head_xent_rows_kernel<T>, dim3((unsigned)((g.rows + 3) / 4)), dim3(256),
                        0, s, g);
@@ -301,17 +305,19 @@ BwdPlan bwd_plan(const Head& p) {
       part = std::max({part, (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(p.rows, p.dim, w), 0),
                        (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(w, p.dim, b.rows4), 0)});
   } else {
-    // Splits of dh's sums such that the tiles fill the CUs: rounds of one tile
-    // per CU, each its k tiles and about 6 more for its start and end, and the
-    // partials written and read.
+    // Splits of dh's sums such that the tiles fill the CUs. A k tile takes 1.5 us
+    // of a CU, a block's start and end about 4 more, and the sums of a split are
+    // written and read at about 4 TB/s.
+    // (1001 x 384 x 16384, us: 4 splits 80, 16 35, 32 32; 8192 x 640 x 16384: 2
+    // splits 182, 5 206.)
     const int64_t tiles = (p.rows + Shape::BM - 1) / Shape::BM *
                           ((p.dim + Shape::BN - 1) / Shape::BN);
-    const int64_t kt = (std::min(b.piece, p.vocab) + mhs::kMmBK - 1) / mhs::kMmBK;
+    const int64_t kt = (std::min(b.piece, p.vocab) + Shape::BK - 1) / Shape::BK;
     const int cus = device_cus();
     double best = 0;
-    for (int64_t n = 1; n <= std::min<int64_t>(16, kt); ++n) {
-      const double t = std::ceil((double)tiles * n / cus) * ((kt + n - 1) / n + 6) +
-                       n * (double)p.rows * p.dim * 8 / 4e6;   // (a k tile takes about 1 us)
+    for (int64_t n = 1; n <= std::min<int64_t>(64, kt); ++n) {
+      const double t = std::ceil((double)tiles * n / cus) * 1.5 * ((double)((kt + n - 1) / n) + 4) +
+                       n * (double)p.rows * p.dim * 8 / 4e6;
       if (n > 1 && t >= best) continue;
       best = t;
       b.splits = (int)n;
@@ -342,8 +348,8 @@ template <class T>
 int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, char* ws,
           hipStream_t s) {
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
-  const auto fh = &mhs::head_mm_kernel<T, Shape, true, false>;
-  const auto fw = &mhs::head_mm_kernel<T, Shape, false, false>;
+  const auto fh = &mhs::head_mm_kernel<T, HalfShape, true, false>;
+  const auto fw = &mhs::head_mm_kernel<T, HalfShape, false, false>;
   allow_lds(fz, Shape::kTileLds);
   allow_lds(fh, Shape::kLds);
   allow_lds(fw, Shape::kLds);
@@ -383,11 +389,11 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
     }
   }
   if (out.dhidden) {
-    const int64_t n = p.rows * p.dim;
+    const int64_t n = p.rows * p.dim / 4;
     hipLaunchKernelGGL(mhs::head_mm_reduce_kernel<T>,
                        dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, s,
-                       part, static_cast<u16*>(out.dhidden), a.scale, a.coef, b.splits,
-                       (long long)p.rows, (int)p.dim, (long long)p.dim);
+                       reinterpret_cast<const float4*>(part), static_cast<ushort4*>(out.dhidden),
+                       a.scale, a.coef, b.splits, (long long)p.rows, (int)(p.dim / 4));
     if ((rc = check_launch("hidden gradient reduction kernel")) != 0) return rc;
   }
   return MHS_OK;
@@ -424,13 +430,16 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
   return MHS_OK;
 }
 
-template <class T>
-int launch_hidden(const Head& p, const BwdPlan& b, const float* coef, char* ws, hipStream_t s) {
-  hipLaunchKernelGGL(mhs::head_copy_kernel<T>, dim3((unsigned)std::min<int64_t>((b.rows4 + 3) / 4, 8192)),
-                     dim3(256), 0, s, static_cast<const mhs::elem_t<T>*>(p.hidden),
-                     (long long)p.ldh, coef, reinterpret_cast<mhs::elem_t<T>*>(ws + b.hidden),
-                     (long long)p.rows, (long long)b.rows4, (int)p.dim);
-  return check_launch("hidden copy kernel");
+// coef, scale and (hidden given) the copy of the rows.
+int launch_rows_in(const Head& p, const BwdPlan& b, const mhs::RowScale& rs, float* coef,
+                   float* scale, void* hidden, hipStream_t s) {
+  const int64_t es = elem_bytes(p.dtype);
+  const int64_t blocks = (b.rows4 + mhs::kCopyRows - 1) / mhs::kCopyRows;
+  hipLaunchKernelGGL(mhs::head_rows_in_kernel<>, dim3((unsigned)blocks), dim3(256), 0, s,
+                     static_cast<const uint4*>(p.hidden), (long long)(p.ldh * es / 16), rs, coef,
+                     scale, static_cast<uint4*>(hidden), (long long)p.rows, (long long)b.rows4,
+                     (int)(p.dim * es / 16), p.dtype == MHS_F16 ? 1 : 0);
+  return check_launch("rows kernel");
 }
 
 // zeros: a gradient that no row reaches.
@@ -457,14 +466,13 @@ int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const BwdOut& out
   char* ws = static_cast<char*>(workspace);
   float* scale = reinterpret_cast<float*>(ws);
   float* coef = reinterpret_cast<float*>(ws + b.coef);
-  hipLaunchKernelGGL(mhs::head_coef_kernel<>, dim3(1), dim3(1024), 0, s, rs, coef, scale,
-                     (long long)p.rows, p.dtype == MHS_F16 ? 1 : 0);
-  if ((rc = check_launch("row coefficient kernel")) != 0) return rc;
-  if (out.dweight) {
-    rc = p.dtype == MHS_F32 ? launch_hidden<Fp32>(p, b, coef, ws, s)
-                            : launch_hidden<Bf16>(p, b, coef, ws, s);   // (a copy of 16 bits)
-    if (rc) return rc;
+  if (p.dtype == MHS_F16 && rs.per_row) {
+    hipLaunchKernelGGL(mhs::head_largest_kernel<>, dim3(1), dim3(1024), 0, s, rs, scale + 2,
+                       (long long)p.rows);
+    if ((rc = check_launch("largest gradient kernel")) != 0) return rc;
   }
+  rc = launch_rows_in(p, b, rs, coef, scale, out.dweight ? ws + b.hidden : nullptr, s);
+  if (rc) return rc;
   a.coef = coef;
   a.scale = scale;
   a.dz = ws + b.dz;
@@ -668,7 +676,7 @@ int mhs_distill_fwd(int dtype, const void* logits, int64_t ld, const float* teac
                     : dtype == MHS_BF16 ? &mhs::distill_fwd_kernel<Bf16>
                                         : &mhs::distill_fwd_kernel<Fp16>;
     hipLaunchKernelGGL(fn, dim3((unsigned)rows), dim3(mhs::kXentThreads),
-                       (size_t)top * sizeof(float), s, g);
+                       2 * (size_t)top * sizeof(float), s, g);
     if ((rc = check_launch("distillation forward kernel")) != 0) return rc;
   }
   if (reduction == MHS_REDUCE_NONE) return MHS_OK;

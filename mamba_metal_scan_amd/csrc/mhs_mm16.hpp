@@ -26,7 +26,6 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kMmBK = 64;        // k depth of a tile: four 32x32x16 MFMAs
 
 // Element types: tags with the MFMAs (32 x 32 x 16 and 16 x 16 x 32) and the
 // conversions.
@@ -73,12 +72,6 @@ struct MmArgs {
   int group_m;          // tiles of a group share the operands' tiles in L2 (see mm_tile)
 };
 
-// Bytes of one operand's k tile of R rows.
-__host__ __device__ constexpr int mm_tile_bytes(int R) { return R * kMmBK * 2; }
-__host__ __device__ constexpr int mm_lds_bytes(int BM, int BN, int stages) {
-  return stages * (mm_tile_bytes(BM) + mm_tile_bytes(BN));
-}
-
 // 64 lanes x 16 bytes from memory straight into LDS at `lds` + 16 lane; lanes at
 // or past the resource's end write zeros. Not tracked by the compiler: the
 // kernel waits for it with mm_wait, and no register is written.
@@ -96,43 +89,50 @@ __device__ __forceinline__ void mm_wait() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 
-// The swizzle of a K-major tile: 128-byte rows of eight 16-byte chunks, chunk c
-// of row r at place c ^ mm_swz(r), so that the 8 (and 16) lanes of one pass of a
-// 16-byte read, on consecutive rows, hit different banks.
-__device__ __forceinline__ constexpr int mm_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
-
-// One operand of a block of WAVES waves: R rows from r0 of `rows`.
-template <int R, bool KMAJOR, int WAVES, int MI>
+// One operand of a block of WAVES waves: R rows from r0 of `rows`, k tiles BK deep.
+template <int R, bool KMAJOR, int WAVES, int MI, int BK>
 struct MmOperand {
-  static constexpr int kLoads = R / 8 / WAVES; // direct loads (1 KB) per wave and k tile
-  static constexpr int kLanes = R / 8;         // row-major: lanes per k row
-  static_assert(kLoads * 8 * WAVES == R, "whole loads");
+  static constexpr int kBytes = R * BK * 2;                // of a k tile
+  static constexpr int kLoads = kBytes / 1024 / WAVES;     // direct loads per wave and k tile
+  static constexpr int kLanes = (KMAJOR ? BK : R) / 8;     // lanes per row (K-major) or k row
+  static_assert(kLoads * 1024 * WAVES == kBytes, "whole loads");
   unsigned voff[kLoads];                       // byte offset of load j at a k tile, or kOOB
   int kpos[kLoads];                            // the k it starts at within the tile
   const char* base;                            // the block's rows at the next k tile to load
   long long step;                              // bytes per k tile
   unsigned frag;                               // byte offset of the lane's first fragment
 
+  // Chunk c (16 bytes) of row r (K-major) or k row r lies at place c ^ swz(r).
+  // K-major: the 8 (and 16) lanes of one pass of a 16-byte read, on consecutive
+  // rows of 128 or 64 bytes, then hit different banks; row-major: the k rows that
+  // one pass of the transposing reads meets (4 in a row, and with 16 x 16
+  // fragments those 8 further) do. SQ_LDS_BANK_CONFLICT is 0.
+  static __device__ __forceinline__ constexpr int swz(int r) {
+    if (!KMAJOR) return ((r & 3) << 2) ^ (MI == 16 ? ((r >> 3) & 1) << 1 : 0);
+    return BK == 64 ? (r & 7) ^ ((r >> 3) & 1) : ((r >> 1) & 3) ^ ((r >> 3) & 1);
+  }
+
   // wrow: the wave's first row within the tile.
   __device__ __forceinline__ MmOperand(const void* p, long long ld, int r0, int rows, int k_first,
                                        int wave, int lane, int wrow) {
+    const int first = wave * kLoads * (64 / kLanes) + lane / kLanes;   // (k) row of load 0
     if constexpr (KMAJOR) {
       base = static_cast<const char*>(p) + ((long long)r0 * ld + k_first) * 2;
-      step = kMmBK * 2;
+      step = BK * 2;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int row = (wave * kLoads + j) * 8 + (lane >> 3);
-        const int c = (lane & 7) ^ mm_swz(row);
+        const int row = first + j * (64 / kLanes);
+        const int c = (lane % kLanes) ^ swz(row);
         voff[j] = r0 + row < rows ? 2u * ((unsigned)row * (unsigned)ld + 8u * c) : kOOB;
         kpos[j] = 8 * c;
       }
-      frag = (wrow + lane % MI) * 128 + ((lane / MI ^ mm_swz(lane & 15)) << 4);
+      frag = (wrow + lane % MI) * (2 * BK) + ((lane / MI ^ swz(lane & 15)) << 4);
     } else {
       base = static_cast<const char*>(p) + ((long long)k_first * ld + r0) * 2;
-      step = ld * (2 * kMmBK);
+      step = ld * (2 * BK);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int k = (wave * kLoads + j) * (64 / kLanes) + lane / kLanes;
+        const int k = first + j * (64 / kLanes);
         const int c = (lane % kLanes) ^ swz(k);
         voff[j] = r0 + 8 * c < rows ? 2u * ((unsigned)k * (unsigned)ld + 8u * c) : kOOB;
         kpos[j] = k;
@@ -144,12 +144,6 @@ struct MmOperand {
       const int row = wrow + 16 * (lane % MI / 16) + 4 * (lane & 3);
       frag = k * (2 * R) + ((2 * row) ^ (swz(k) << 4));
     }
-  }
-  // The swizzle of a row-major tile: 16-byte chunk c of k row k at place c ^
-  // swz(k), so that the k rows that one pass of the transposing reads meets
-  // (4 in a row, and with 16 x 16 fragments those 8 further) hit different banks.
-  static __device__ __forceinline__ constexpr int swz(int k) {
-    return ((k & 3) << 2) ^ (MI == 16 ? ((k >> 3) & 1) << 1 : 0);
   }
   // The resource over the next k tile to load, and on to the one after it.
   __device__ __forceinline__ i32x4 next() {
@@ -170,7 +164,7 @@ struct MmOperand {
   // Fragment f (MI rows, 512 / MI deep) of step kk, from the operand's buffer.
   __device__ __forceinline__ s16x8 read(const char* buf, int f, int kk) const {
     if constexpr (KMAJOR) {
-      return *reinterpret_cast<const s16x8*>(buf + f * (MI * 128) + (frag ^ (kk * (1024 / MI))));
+      return *reinterpret_cast<const s16x8*>(buf + f * (MI * 2 * BK) + (frag ^ (kk * (1024 / MI))));
     } else {
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
       // (MI rows are 2 MI bytes, bits that the swizzle flips and wrow leaves 0
@@ -199,16 +193,24 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g, int& tm, int& tn) {
 }
 
 // A block's shape: BM x BN tile, WM x WN waves of FM x FN fragments (MI x MI),
-// ST k tiles in LDS; a wave's registers hold the fragments of SUB steps (512 / MI
-// deep) while it multiplies those of the SUB steps before.
-template <int BM_, int BN_, int WM_, int WN_, int ST_, int MI_, int SUB_>
+// ST k tiles BK deep in LDS; a wave's registers hold the fragments of SUB steps
+// (512 / MI deep) while it multiplies those of the SUB steps before.
+template <int BM_, int BN_, int WM_, int WN_, int ST_, int MI_, int SUB_, int BK_, bool HALF_>
 struct MmShape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_, MI = MI_, SUB = SUB_;
+  static constexpr int BK = BK_;
+  static constexpr bool HALF = HALF_;
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int FM = BM / WM / MI, FN = BN / WN / MI;
   static constexpr int E = MI * MI / 64;   // a lane's elements of a fragment
+  // A wave's place in the tile. HALF: waves w and w + 4, which share a SIMD, lie
+  // half a tile apart in n, so that in a tile half past the end each SIMD has one
+  // wave at work (8192 x 640 x 16384, two of its five half tiles: 196 / 184 us;
+  // without such tiles the loss is 2-4%, so only products of few columns take it).
+  static __device__ __forceinline__ int wave_m(int wave) { return HALF ? wave % WM : wave / WN; }
+  static __device__ __forceinline__ int wave_n(int wave) { return HALF ? wave / WM : wave % WN; }
   typedef float acc __attribute__((ext_vector_type(E)));
-  static constexpr int kLds = mm_lds_bytes(BM, BN, ST);
+  static constexpr int kLds = ST * (BM + BN) * BK * 2;
   // The tile in 16 bits, transposed: rows of BM elements, 16 bytes (4 banks) on
   // per row.
   static constexpr int kRow = BM + 8;
@@ -218,18 +220,18 @@ struct MmShape {
 // acc = the tile's sums over k's k_first .. k_first + k_len - 1. A fragment's
 // element e of lane l: row 8 (e / 4) + 4 (l / MI) + e % 4, column l % MI. Ends on
 // a barrier, the LDS free.
-template <class T, class S, bool AK, bool BK>
+template <class T, class S, bool AK, bool BKM>
 __device__ __forceinline__ void mm_products(typename S::acc (&acc)[S::FM][S::FN], const MmArgs& g,
                                             int m0, int n0, int k_first, int k_len, char* lds) {
-  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, MI = S::MI, KS = kMmBK * MI / 512;
-  constexpr int TA = mm_tile_bytes(S::BM), BUF = TA + mm_tile_bytes(S::BN);
+  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, MI = S::MI, BK = S::BK, KS = BK * MI / 512;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  typedef MmOperand<S::BM, AK, S::kWaves, MI> OA;
-  typedef MmOperand<S::BN, BK, S::kWaves, MI> OB;
+  typedef MmOperand<S::BM, AK, S::kWaves, MI, BK> OA;
+  typedef MmOperand<S::BN, BKM, S::kWaves, MI, BK> OB;
   constexpr int LA = OA::kLoads, LB = OB::kLoads, L = LA + LB;
-  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, (wave / S::WN) * (FM * MI));
-  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, (wave % S::WN) * (FN * MI));
+  constexpr int TA = OA::kBytes, BUF = TA + OB::kBytes;
+  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, S::wave_m(wave) * (FM * MI));
+  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, S::wave_n(wave) * (FN * MI));
   const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -237,18 +239,35 @@ __device__ __forceinline__ void mm_products(typename S::acc (&acc)[S::FM][S::FN]
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int e = 0; e < S::E; ++e) acc[i][j][e] = 0.f;
-  const int nk = (k_len + kMmBK - 1) / kMmBK;
+  // Phases of SUB steps per k tile; the register sets alternate, so the loop goes
+  // over an even number of them (a k tile past the end is zeros).
+  constexpr int SUB = S::SUB, PH = KS / SUB, KT = PH % 2 ? 2 : 1;
+  static_assert(PH * SUB == KS, "whole phases");
+  const int nk = (k_len + BK - 1) / BK, round_nk = (nk + KT - 1) / KT * KT;
 #pragma unroll
   for (int s = 0; s < ST; ++s) {
     const i32x4 ra = a.next(), rb = b.next();
 #pragma unroll
-    for (int j = 0; j < LA; ++j) a.load(ra, j, at + s * BUF, k_len - s * kMmBK, wave);
+    for (int j = 0; j < LA; ++j) a.load(ra, j, at + s * BUF, k_len - s * BK, wave);
 #pragma unroll
-    for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, k_len - s * kMmBK, wave);
+    for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, k_len - s * BK, wave);
   }
   mm_wait<(ST - 1) * L>();
-  constexpr int SUB = S::SUB, PH = KS / SUB;   // phases of SUB steps per k tile
-  static_assert(PH * SUB == KS && PH % 2 == 0, "the register sets alternate within a k tile");
+  if (m0 + S::wave_m(wave) * (FM * MI) >= g.M || n0 + S::wave_n(wave) * (FN * MI) >= g.N) {
+    // Nothing of this wave's is within the product: its share of the loads alone.
+    for (int kt = 0, cur = 0; kt < round_nk; ++kt) {
+      mm_wait<(ST - 2) * L>();
+      const i32x4 ra = a.next(), rb = b.next();
+      const int left = k_len - (kt + ST) * BK;
+#pragma unroll
+      for (int j = 0; j < LA; ++j) a.load(ra, j, at + cur * BUF, left, wave);
+#pragma unroll
+      for (int j = 0; j < LB; ++j) b.load(rb, j, at + cur * BUF + TA, left, wave);
+      cur = cur + 1 == ST ? 0 : cur + 1;
+    }
+    mm_wait<0>();
+    return;
+  }
   s16x8 fa[2][SUB][FM], fb[2][SUB][FN];
 #pragma unroll
   for (int u = 0; u < SUB; ++u) {
@@ -257,48 +276,52 @@ __device__ __forceinline__ void mm_products(typename S::acc (&acc)[S::FM][S::FN]
 #pragma unroll
     for (int j = 0; j < FN; ++j) fb[0][u][j] = b.read(lds + TA, j, u);
   }
-  int cur = 0;   // the buffer of tile kt
-  for (int kt = 0; kt < nk; ++kt) {
-    const int next = cur + 1 == ST ? 0 : cur + 1;
-    const int left = k_len - (kt + ST) * kMmBK;
-    i32x4 ra, rb;
+  int cur = 0;   // the buffer of the k tile
+  for (int kt = 0; kt < round_nk; kt += KT) {
 #pragma unroll
-    for (int p = 0; p < PH; ++p) {
-      if (p == PH - 1) {
-        // Tile kt + 1 has landed, and every wave holds its last fragments of
-        // tile kt: its buffer takes tile kt + ST.
-        mm_wait<(ST - 2) * L>();
-        ra = a.next();
-        rb = b.next();
-      }
-      const char* nb = lds + (p == PH - 1 ? next : cur) * BUF;
-      // A row of fragments' products at a time, with each its share of the
-      // next phase's fragments and of the direct loads: the wave issues them
-      // while the matrix core works.
+    for (int t = 0; t < KT; ++t) {
+      const int next = cur + 1 == ST ? 0 : cur + 1;
+      const int left = k_len - (kt + t + ST) * BK;
+      i32x4 ra, rb;
 #pragma unroll
-      for (int q = 0; q < SUB * FM; ++q) {
-        constexpr int F = FM + FN, R = SUB * F;
-        const int u = q / FM, i = q % FM;
-#pragma unroll
-        for (int x = q * R / (SUB * FM); x < (q + 1) * R / (SUB * FM); ++x) {
-          const int step = (p + 1) % PH * SUB + x / F, f = x % F;
-          if (f < FM) fa[1 - p % 2][x / F][f] = a.read(nb, f, step);
-          else fb[1 - p % 2][x / F][f - FM] = b.read(nb + TA, f - FM, step);
-        }
+      for (int p = 0; p < PH; ++p) {
+        const int set = (t * PH + p) % 2;
         if (p == PH - 1) {
-#pragma unroll
-          for (int l = q * L / (SUB * FM); l < (q + 1) * L / (SUB * FM); ++l) {
-            if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
-            else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
-          }
+          // The next tile has landed, and every wave holds its last fragments of
+          // this one: its buffer takes the tile ST further.
+          mm_wait<(ST - 2) * L>();
+          ra = a.next();
+          rb = b.next();
         }
+        const char* nb = lds + (p == PH - 1 ? next : cur) * BUF;
+        // A row of fragments' products at a time, with each its share of the
+        // next phase's fragments and of the direct loads: the wave issues them
+        // while the matrix core works.
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = T::mfma(fa[p % 2][u][i], fb[p % 2][u][j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int q = 0; q < SUB * FM; ++q) {
+          constexpr int F = FM + FN, R = SUB * F;
+          const int u = q / FM, i = q % FM;
+#pragma unroll
+          for (int x = q * R / (SUB * FM); x < (q + 1) * R / (SUB * FM); ++x) {
+            const int step = (p + 1) % PH * SUB + x / F, f = x % F;
+            if (f < FM) fa[1 - set][x / F][f] = a.read(nb, f, step);
+            else fb[1 - set][x / F][f - FM] = b.read(nb + TA, f - FM, step);
+          }
+          if (p == PH - 1) {
+#pragma unroll
+            for (int l = q * L / (SUB * FM); l < (q + 1) * L / (SUB * FM); ++l) {
+              if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
+              else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = T::mfma(fa[set][u][i], fb[set][u][j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
+      cur = next;
     }
-    cur = next;
   }
   mm_wait<0>();
 }

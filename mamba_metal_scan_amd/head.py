@@ -54,16 +54,22 @@ class LinearCrossEntropyHIP(torch.autograd.Function):
     int64; rows with target == ignore_index excluded."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        ctx.dim = hidden.shape[1]
-        ctx.reduction = reduction
+    def loss(hidden, weight, targets, ignore_index, reduction):
+        """(loss, what the backward needs)."""
         hidden, weight = _rows16(hidden), _rows16(weight)
         targets = targets.contiguous()
         if not torch.compiler.is_compiling():   # (the registered op checks itself)
             _native._check_linear_xent("linear_cross_entropy", hidden, weight, targets, reduction)
         loss, saved = dispatch("linear_xent_fwd")(hidden, weight, targets, ignore_index,
                                                   reduction)
-        ctx.save_for_backward(hidden, weight, targets, saved)
+        return loss, (hidden, weight, targets, saved)
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+        ctx.dim = hidden.shape[1]
+        ctx.reduction = reduction
+        loss, saved = LinearCrossEntropyHIP.loss(hidden, weight, targets, ignore_index, reduction)
+        ctx.save_for_backward(*saved)
         return loss
 
     @staticmethod
@@ -80,16 +86,23 @@ class LinearDistillHIP(torch.autograd.Function):
     ids (R, K) and their logits."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, teacher_logits, ids, temperature, reduction):
-        ctx.dim = hidden.shape[1]
-        ctx.temperature, ctx.reduction = temperature, reduction
+    def loss(hidden, weight, teacher_logits, ids, temperature, reduction):
+        """(loss, what the backward needs)."""
         hidden, weight = _rows16(hidden), _rows16(weight)
         if not torch.compiler.is_compiling():
             _native._check_linear_distill("linear_distill_loss", hidden, weight, teacher_logits,
                                           ids, temperature, reduction)
         loss, saved = dispatch("linear_distill_fwd")(hidden, weight, teacher_logits, ids,
                                                      temperature, reduction)
-        ctx.save_for_backward(hidden, weight, ids, saved)
+        return loss, (hidden, weight, ids, saved)
+
+    @staticmethod
+    def forward(ctx, hidden, weight, teacher_logits, ids, temperature, reduction):
+        ctx.dim = hidden.shape[1]
+        ctx.temperature, ctx.reduction = temperature, reduction
+        loss, saved = LinearDistillHIP.loss(hidden, weight, teacher_logits, ids, temperature,
+                                            reduction)
+        ctx.save_for_backward(*saved)
         return loss
 
     @staticmethod
@@ -106,15 +119,21 @@ class DistillHIP(torch.autograd.Function):
     their logits."""
 
     @staticmethod
-    def forward(ctx, logits, teacher_logits, ids, temperature, reduction):
-        ctx.temperature, ctx.reduction = temperature, reduction
+    def loss(logits, teacher_logits, ids, temperature, reduction):
+        """(loss, what the backward needs)."""
         if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
             logits = logits.contiguous()
         if not torch.compiler.is_compiling():
             _native._check_distill("distill_loss", logits, teacher_logits, ids, temperature,
                                    reduction)
         loss, saved = dispatch("distill_fwd")(logits, teacher_logits, ids, temperature, reduction)
-        ctx.save_for_backward(logits, ids, saved)
+        return loss, (logits, ids, saved)
+
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, ids, temperature, reduction):
+        ctx.temperature, ctx.reduction = temperature, reduction
+        loss, saved = DistillHIP.loss(logits, teacher_logits, ids, temperature, reduction)
+        ctx.save_for_backward(*saved)
         return loss
 
     @staticmethod
@@ -123,6 +142,15 @@ class DistillHIP(torch.autograd.Function):
         logits, ids, saved = ctx.saved_tensors
         return (dispatch("distill_bwd")(g.contiguous(), logits, ids, saved, ctx.temperature,
                                         ctx.reduction), None, None, None, None)
+
+
+def _apply(cls, leaves: int, *args):
+    """cls.apply, or without autograd to record (scoring, serving) its forward
+    alone."""
+    if torch.compiler.is_compiling() or (torch.is_grad_enabled()
+                                         and any(t.requires_grad for t in args[:leaves])):
+        return cls.apply(*args)
+    return cls.loss(*args)[0]
 
 
 def _reduction(what: str, reduction: str) -> int:
@@ -194,8 +222,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"{what}: targets must be integers of shape {tuple(hidden.shape[:-1])}; "
                          f"got {targets.dtype} {tuple(targets.shape)}")
     h, w = _head(what, hidden, weight)
-    loss = LinearCrossEntropyHIP.apply(h, w, targets.to(torch.int64).reshape(-1),
-                                       int(ignore_index), red)
+    loss = _apply(LinearCrossEntropyHIP, 2, h, w, targets.to(torch.int64).reshape(-1),
+                  int(ignore_index), red)
     return loss if red else loss.view(targets.shape)
 
 
@@ -212,7 +240,7 @@ def linear_distill_loss(hidden: torch.Tensor, weight: torch.Tensor,
     lead = hidden.shape[:-1]
     t, ids = _teacher(what, lead, teacher_logits, teacher_ids, temperature)
     h, w = _head(what, hidden, weight)
-    loss = LinearDistillHIP.apply(h, w, t, ids, temperature, red)
+    loss = _apply(LinearDistillHIP, 2, h, w, t, ids, temperature, red)
     return loss if red else loss.view(lead)
 
 
@@ -241,5 +269,5 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
                            f"{logits.dtype}")
     lead = logits.shape[:-1]
     t, ids = _teacher(what, lead, teacher_logits, teacher_ids, temperature)
-    loss = DistillHIP.apply(logits.reshape(-1, logits.shape[-1]), t, ids, temperature, red)
+    loss = _apply(DistillHIP, 1, logits.reshape(-1, logits.shape[-1]), t, ids, temperature, red)
     return loss if red else loss.view(lead)
