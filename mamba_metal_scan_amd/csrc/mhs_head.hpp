@@ -88,7 +88,6 @@ __device__ __forceinline__ void column_lse2(const Z& z, const R& row, float c, i
 template <int WM>
 __device__ __forceinline__ void store_partials(float* red, float2* part, int n0, int rows,
                                                int cols, long long at) {
-  __syncthreads();
   for (int n = threadIdx.x; n < cols; n += blockDim.x) {
     float m = red[n], s = red[cols + n];
 #pragma unroll
@@ -103,30 +102,31 @@ template <class T, class S>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
   extern __shared__ float lds_f[];
-  int tm, tn;
-  mm_tile(g, tm, tn);
-  const int m0 = tm * S::BM, n0 = tn * S::BN;
-  typename S::acc acc[S::FM][S::FN];
-  mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float* const red = lds_f + S::kLds / 4;   // [WM][max, sum][BN]
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = S::wave_m(wave), wn = S::wave_n(wave);
-  const int left = g.M - m0 - wm * (S::FM * S::MI) - 4 * (lane / S::MI);
+  const auto none = [](int, int) {};
+  mm_stream<T, S>(g, reinterpret_cast<char*>(lds_f), none, [&](auto& acc, int m0, int n0, int) {
+    const int lane = mm_opaque(threadIdx.x & 63);
+    const int left = g.M - m0 - wm * (S::FM * 16) - 32 * (lane >> 5) - 4 * ((lane >> 4) & 1);
 #pragma unroll
-  for (int j = 0; j < S::FN; ++j) {
-    float m, s;
-    column_lse2<S::FM * S::E>(
-        [&](int i) { return acc[i / S::E][j][i % S::E]; },
-        [](int i) { return i / S::E * S::MI + 8 * (i % S::E / 4) + i % 4; }, c, left, m, s);
+    for (int j = 0; j < S::FN; ++j) {
+      float m, s;
+      column_lse2<S::FM * 4>([&](int i) { return acc[i / 4][j][i % 4]; },
+                             [](int i) { return 64 * (i / 16) + 8 * (i / 4 % 4) + i % 4; }, c,
+                             left, m, s);
 #pragma unroll
-    for (int o = S::MI; o < 64; o *= 2)
-      lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
-    const int n = (wn * S::FN + j) * S::MI + lane;
-    if (lane < S::MI) {
-      lds_f[2 * wm * S::BN + n] = m;
-      lds_f[(2 * wm + 1) * S::BN + n] = s;
+      for (int o = 16; o < 64; o *= 2)
+        lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+      const int n = (wn * S::FN + j) * 16 + lane;
+      if (lane < 16) {
+        red[2 * wm * S::BN + n] = m;
+        red[(2 * wm + 1) * S::BN + n] = s;
+      }
     }
-  }
-  store_partials<S::WM>(lds_f, part, n0, g.N, S::BN, tm);
+    mm_lds_barrier();
+    store_partials<S::WM>(red, part, n0, g.N, S::BN, m0 / S::BM);
+  });
 }
 
 // The same for fp32 operands, on the products of three bf16 parts.
@@ -155,6 +155,7 @@ head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part) {
       lds_f[(2 * wm + 1) * TILE + n] = s;
     }
   }
+  __syncthreads();
   store_partials<2>(lds_f, part, n0, g.N, TILE, m0 / TILE);
 }
 
@@ -546,29 +547,30 @@ __device__ __forceinline__ float lift_of(float largest) {
 
 constexpr int kCopyRows = 8;   // rows per block
 
-// coef[r]; scale[0..1] = (s, 1 / s), dz's power of two (lift: fp16; scale[2] the
-// largest per-row gradient), else 1; and, `out` given, out (out_rows, per) = in
+// scale[0..1] = (s, 1 / s), dz's power of two (lift: fp16; scale[2] the largest
+// per-row gradient), else 1; rows2[r] = (coef s, lse2); and, `out` given, out (out_rows, per) = in
 // (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
 // `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
 // reach dW.
 template <int UNUSED = 0>
 __global__ void __launch_bounds__(256)
 head_rows_in_kernel(const uint4* __restrict__ in, long long ldi, RowScale rs,
-                    float* __restrict__ coef, float* __restrict__ scale, uint4* __restrict__ out,
-                    long long rows, long long out_rows, int per, int lift) {
+                    const float* __restrict__ lse2, float2* __restrict__ rows2,
+                    float* __restrict__ scale, uint4* __restrict__ out, long long rows,
+                    long long out_rows, int per, int lift) {
   __shared__ float cf[kCopyRows];
   const long long r0 = (long long)blockIdx.x * kCopyRows;
   if (threadIdx.x < kCopyRows) {
+    // (without per-row gradients the largest is the one that every kept row has)
+    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : fabsf(rs.reaching(0)));
     const long long r = r0 + threadIdx.x;
     const float c = r < rows ? rs.at(r) : 0.f;
     cf[threadIdx.x] = c;
-    if (r < rows) coef[r] = c;
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 64) {
-    // (without per-row gradients the largest is the one that every kept row has)
-    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : fabsf(rs.reaching(0)));
-    scale[0] = s;
-    scale[1] = 1.f / s;
+    if (r < ((rows + 1) & ~1LL)) rows2[r] = make_float2(c * s, r < rows ? lse2[r] : 0.f);
+    if (r == 0) {
+      scale[0] = s;
+      scale[1] = 1.f / s;
+    }
   }
   if (!out) return;
   __syncthreads();
@@ -590,8 +592,7 @@ head_zero_kernel(unsigned* __restrict__ out, long long n) {
 }
 
 struct HeadGrad {
-  const float* lse2;       // (rows)
-  const float* coef;       // (rows)
+  const float2* rows2;     // (rows, to an even number) (coef s, lse2)
   const float* scale;      // [s, 1 / s]
   const long long* ids;    // (rows, k)
   const float* q;          // (rows, k) the words' whole weights, or null: 1
@@ -603,50 +604,78 @@ struct HeadGrad {
   long long ldz;
 };
 
-// p's part of dz of a piece, 16 bits, (rows, ldz): the tile goes through LDS,
-// transposed into rows of BM words.
+// Exchanges 4 registers' groups of 16 lanes: v[q] then holds in group g what
+// v[g] held in group q.
+__device__ __forceinline__ void exchange4(unsigned (&v)[4]) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v[q], v[q + 2], false, false);
+    v[q] = r[0];
+    v[q + 2] = r[1];
+  }
+#pragma unroll
+  for (int q = 0; q < 4; q += 2) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v[q], v[q + 1], false, false);
+    v[q] = r[0];
+    v[q + 1] = r[1];
+  }
+}
+
+// p's part of dz of a piece, 16 bits, (rows, ldz). The tile has the words in m, dz
+// the rows: a lane's 4 words of 4 fragments become 16 of one row (exchange4), in
+// two stores of 16 bytes, each 64 bytes of 16 rows at a time; no LDS.
 template <class T, class S>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_dz_kernel(MmArgs g, HeadGrad a) {
   extern __shared__ float lds_f[];
-  unsigned short* const tile = reinterpret_cast<unsigned short*>(lds_f);
-  constexpr int LD = S::kRow;
-  int tm, tn;
-  mm_tile(g, tm, tn);
-  const int m0 = tm * S::BM, n0 = tn * S::BN;
-  typename S::acc acc[S::FM][S::FN];
-  mm_products<T, S, true, true>(acc, g, m0, n0, 0, g.K, reinterpret_cast<char*>(lds_f));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // Two tiles' rows' (coef, lse2).
+  static_assert(S::BN == 256, "two direct loads hold a tile's rows");
+  char* const pairs = reinterpret_cast<char*>(lds_f) + S::kLds;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = S::wave_m(wave), wn = S::wave_n(wave);
-  const float scale = a.scale[0];
+  const auto load_pairs = [&](int n0, int odd) {
+    if (wave >= 2) return;
+    const int at = 128 * wave + 2 * (int)(threadIdx.x & 63);   // 2 rows a lane
+    mm_load_lds(mm_resource(a.rows2 + n0), at < g.N - n0 ? 8u * (unsigned)at : kOOB,
+                (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)pairs +
+                    2048 * odd + 1024 * wave);
+  };
+  mm_stream<T, S>(g, reinterpret_cast<char*>(lds_f), load_pairs, [&](auto& acc, int m0, int n0,
+                                                                    int odd) {
+    const int lane = mm_opaque(threadIdx.x & 63);
+    m0 += wm * (S::FM * 16);
+    const int left = g.M - m0 - 32 * (lane >> 5) - 4 * ((lane >> 4) & 1);
 #pragma unroll
-  for (int j = 0; j < S::FN; ++j) {
-    const int n = (wn * S::FN + j) * S::MI + lane % S::MI;
-    const int r = min(n0 + n, g.N - 1);
-    const float f = a.coef[r] * scale, l2 = a.lse2[r];
+    for (int j = 0; j < S::FN; ++j) {
+      const int in = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + in;
+      const float2 row2 = *reinterpret_cast<const float2*>(pairs + 2048 * odd + 8 * in);
+      const float f = row2.x, l2 = row2.y;
+      unsigned short* const row = static_cast<unsigned short*>(a.dz) + (long long)n * a.ldz + m0 +
+                                  8 * (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < S::FM; ++i)
+      for (int h = 0; h < S::FM / 4; ++h) {
+        unsigned lo[4], hi[4];
 #pragma unroll
-      for (int e = 0; e < S::E; e += 4) {
-        const int m = (wm * S::FM + i) * S::MI + 8 * (e / 4) + 4 * (lane / S::MI);
-        s16x4 v;
+        for (int i = 0; i < 4; ++i) {
+          unsigned short v[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p = exp2_hw(__builtin_fmaf(acc[i][j][e + x], a.c, -l2)) * f;
-          // (an ignored row's zeros whatever its logits are)
-          v[x] = (short)T::from(f == 0.f || m0 + m + x >= g.M ? 0.f : p);
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp2_hw(__builtin_fmaf(acc[4 * h + i][j][e], a.c, -l2)) * f;
+            // (an ignored row's zeros whatever its logits are)
+            v[e] = T::from(f == 0.f || 64 * h + 8 * i + e >= left ? 0.f : p);
+          }
+          lo[i] = v[0] | (unsigned)v[1] << 16;
+          hi[i] = v[2] | (unsigned)v[3] << 16;
         }
-        *reinterpret_cast<s16x4*>(tile + n * LD + m) = v;
+        exchange4(lo);
+        exchange4(hi);
+        if (n < g.N) {
+          *reinterpret_cast<uint4*>(row + 64 * h) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+          *reinterpret_cast<uint4*>(row + 64 * h + 32) = make_uint4(lo[2], hi[2], lo[3], hi[3]);
+        }
       }
-  }
-  __syncthreads();
-  const int rows = min(S::BN, g.N - n0);
-  constexpr int CH = S::BM / 8;   // 16-byte chunks per row
-  for (int i = threadIdx.x; i < rows * CH; i += S::kThreads) {
-    const int n = i / CH, ch = i % CH;
-    *reinterpret_cast<s16x8*>(static_cast<unsigned short*>(a.dz) + (n0 + n) * a.ldz + m0 +
-                              8 * ch) = *reinterpret_cast<const s16x8*>(tile + n * LD + 8 * ch);
-  }
+    }
+  });
 }
 
 // The same in fp32, transposed: (words, ldz), its rows contiguous.
@@ -665,7 +694,7 @@ head_dz3_kernel(GemmArgs g, HeadGrad a) {
   for (int j = 0; j < F; ++j) {
     const int r = n0 + wn * (TILE / 2) + j * 32 + (lane & 31);
     const int rc = min(r, g.N - 1);
-    const float cf = a.coef[rc], l2 = a.lse2[rc];
+    const float cf = a.rows2[rc].x, l2 = a.rows2[rc].y;
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
@@ -688,7 +717,7 @@ __global__ void __launch_bounds__(256)
 head_ids_kernel(HeadGrad a, long long rows, int words) {
   const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
-  const float f = a.coef[r] * a.scale[0], l2 = a.lse2[r];
+  const float f = a.rows2[r].x, l2 = a.rows2[r].y;
   if (f == 0.f) return;
   const long long at = r * a.k;
   for (int k = threadIdx.x & 63; k < a.k; k += 64) {
@@ -716,7 +745,7 @@ __global__ void __launch_bounds__(S::kThreads, 2)
 head_mm_kernel(MmArgs g, MmOut o) {
   extern __shared__ float lds_f[];
   int tm, tn;
-  mm_tile(g, tm, tn);
+  mm_tile(g, blockIdx.x, tm, tn);
   const int k_first = blockIdx.y * g.kt_per_split * S::BK;
   typename S::acc acc[S::FM][S::FN];
   mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
@@ -750,15 +779,15 @@ head_mm_kernel(MmArgs g, MmOut o) {
 template <class T>
 __global__ void __launch_bounds__(256)
 head_mm_reduce_kernel(const float4* __restrict__ part, ushort4* __restrict__ out,
-                      const float* __restrict__ scale, const float* __restrict__ coef, int splits,
-                      long long M, int N4) {
+                      const float* __restrict__ scale, const float2* __restrict__ rows2,
+                      int splits, long long M, int N4) {
   const long long n = M * N4;
   const float f = scale[1];
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
        i += (long long)gridDim.x * 256) {
     float4 s = part[i];
     for (int k = 1; k < splits; ++k) s = add(s, part[k * n + i]);
-    const bool zero = coef[i / N4] == 0.f;
+    const bool zero = rows2[i / N4].x == 0.f;
     out[i] = zero ? make_ushort4(0, 0, 0, 0)
                   : make_ushort4(T::from(s.x * f), T::from(s.y * f), T::from(s.z * f),
                                  T::from(s.w * f));

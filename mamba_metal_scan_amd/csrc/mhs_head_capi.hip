@@ -153,6 +153,11 @@ mhs::MmArgs mm_args(const void* a, int64_t lda, const void* b, int64_t ldb, int6
   return g;
 }
 
+// Blocks of a streamed product: as many as run at once (one per CU).
+unsigned stream_blocks(const mhs::MmArgs& g) {
+  return (unsigned)std::min<int64_t>((int64_t)g.grid_m * g.grid_n, device_cus());
+}
+
 // The logits' product for fp32: W (v0 .. v0 + words) h^T.
 mhs::GemmArgs gemm3_args(const Head& p, int64_t v0, int64_t words) {
   mhs::GemmArgs g{};
@@ -172,9 +177,9 @@ template <class T>
 int launch_lse16(const Head& p, float c, float2* part, hipStream_t s) {
   const mhs::MmArgs g = mm_args<Shape>(p.weight, p.ldw, p.hidden, p.ldh, p.vocab, p.rows, p.dim);
   const auto fn = &mhs::head_lse_kernel<T, Shape>;
-  allow_lds(fn, Shape::kLds);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads), Shape::kLds,
-                     s, g, c, part);
+  constexpr int lds = Shape::kLds + 2 * Shape::WM * Shape::BN * 4;
+  allow_lds(fn, lds);
+  hipLaunchKernelGGL(fn, dim3(stream_blocks(g)), dim3(Shape::kThreads), lds, s, g, c, part);
   return check_launch("head log-sum-exp kernel");
 }
 
@@ -276,7 +281,7 @@ struct BwdPlan {
   int64_t rows4;           // fp32: the rows, to a multiple of 4
   int splits = 1;          // of dh's sums over a piece's words
   int kt_per_split = 0;
-  size_t coef, hidden, dz, part, bytes;
+  size_t rows2, hidden, dz, part, bytes;
 };
 
 int64_t piece_words(int64_t rows, int64_t vocab, int es) {
@@ -290,8 +295,8 @@ BwdPlan bwd_plan(const Head& p) {
   b.piece = std::min<int64_t>(piece_words(p.rows, p.vocab, es), 1 << 20);
   b.rows4 = p.dtype == MHS_F32 ? (int64_t)round_up(p.rows, 4) : p.rows;
   b.ldz = p.dtype == MHS_F32 ? b.rows4 : b.piece;
-  b.coef = 256;
-  b.hidden = b.coef + round_up((size_t)p.rows * 4, 256);
+  b.rows2 = 256;
+  b.hidden = b.rows2 + round_up((size_t)(p.rows + 1) * 8, 256);
   b.dz = b.hidden + round_up((size_t)b.rows4 * p.dim * es, 256);
   b.part = b.dz + round_up((size_t)(p.dtype == MHS_F32 ? b.piece * b.rows4 : p.rows * b.piece) * es,
                            256);
@@ -350,7 +355,8 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
   const auto fh = &mhs::head_mm_kernel<T, HalfShape, true, false>;
   const auto fw = &mhs::head_mm_kernel<T, HalfShape, false, false>;
-  allow_lds(fz, Shape::kTileLds);
+  constexpr int lds_z = Shape::kLds + 2 * 2048;
+  allow_lds(fz, lds_z);
   allow_lds(fh, Shape::kLds);
   allow_lds(fw, Shape::kLds);
   typedef unsigned short u16;
@@ -362,8 +368,8 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
     const int64_t words = std::min(b.piece, p.vocab - v0);
     mhs::MmArgs g = mm_args<Shape>(w + v0 * p.ldw, p.ldw, p.hidden, p.ldh, words, p.rows, p.dim);
     a.v0 = (int)v0;
-    hipLaunchKernelGGL(fz, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads),
-                       Shape::kTileLds, s, g, a);
+    hipLaunchKernelGGL(fz, dim3(stream_blocks(g)), dim3(Shape::kThreads),
+                       lds_z, s, g, a);
     if ((rc = check_launch("head gradient kernel")) != 0) return rc;
     if ((rc = launch_ids<T>(p, a, words, s)) != 0) return rc;
     mhs::MmOut o{};
@@ -393,7 +399,7 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
     hipLaunchKernelGGL(mhs::head_mm_reduce_kernel<T>,
                        dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, s,
                        reinterpret_cast<const float4*>(part), static_cast<ushort4*>(out.dhidden),
-                       a.scale, a.coef, b.splits, (long long)p.rows, (int)(p.dim / 4));
+                       a.scale, a.rows2, b.splits, (long long)p.rows, (int)(p.dim / 4));
     if ((rc = check_launch("hidden gradient reduction kernel")) != 0) return rc;
   }
   return MHS_OK;
@@ -430,15 +436,17 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
   return MHS_OK;
 }
 
-// coef, scale and (hidden given) the copy of the rows.
-int launch_rows_in(const Head& p, const BwdPlan& b, const mhs::RowScale& rs, float* coef,
-                   float* scale, void* hidden, hipStream_t s) {
+// The rows' coefficients, the scale and (hidden given) the copy of the rows.
+int launch_rows_in(const Head& p, const BwdPlan& b, const mhs::RowScale& rs, const float* lse2,
+                   float2* rows2, float* scale, void* hidden, hipStream_t s) {
   const int64_t es = elem_bytes(p.dtype);
-  const int64_t blocks = (b.rows4 + mhs::kCopyRows - 1) / mhs::kCopyRows;
+  // (rows2 has an even number of rows, hidden rows4)
+  const int64_t out_rows = std::max<int64_t>(b.rows4, (int64_t)round_up(p.rows, 2));
+  const int64_t blocks = (out_rows + mhs::kCopyRows - 1) / mhs::kCopyRows;
   hipLaunchKernelGGL(mhs::head_rows_in_kernel<>, dim3((unsigned)blocks), dim3(256), 0, s,
-                     static_cast<const uint4*>(p.hidden), (long long)(p.ldh * es / 16), rs, coef,
-                     scale, static_cast<uint4*>(hidden), (long long)p.rows, (long long)b.rows4,
-                     (int)(p.dim * es / 16), p.dtype == MHS_F16 ? 1 : 0);
+                     static_cast<const uint4*>(p.hidden), (long long)(p.ldh * es / 16), rs, lse2,
+                     rows2, scale, static_cast<uint4*>(hidden), (long long)p.rows,
+                     (long long)b.rows4, (int)(p.dim * es / 16), p.dtype == MHS_F16 ? 1 : 0);
   return check_launch("rows kernel");
 }
 
@@ -450,13 +458,13 @@ int launch_zero(void* p, int64_t n, int es, hipStream_t s) {
   return check_launch("zero fill kernel");
 }
 
-int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const BwdOut& out, void* workspace,
-             size_t workspace_bytes, void* stream) {
+int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const float* lse2,
+             const BwdOut& out, void* workspace, size_t workspace_bytes, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int es = elem_bytes(p.dtype);
   if (out.dhidden == nullptr && out.dweight == nullptr) return MHS_OK;
   if (p.rows == 0) return out.dweight ? launch_zero(out.dweight, p.vocab * p.dim, es, s) : MHS_OK;
-  if (!a.ids || !a.lse2 || !a.picked || !rs.keep || !rs.upstream)
+  if (!a.ids || !lse2 || !a.picked || !rs.keep || !rs.upstream)
     return fail(MHS_EINVAL, "null pointer argument");
   if (!aligned16(out.dhidden) || !aligned16(out.dweight))
     return fail(MHS_EINVAL, "dhidden and dweight must be 16-byte aligned");
@@ -465,15 +473,15 @@ int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const BwdOut& out
   const BwdPlan b = bwd_plan(p);
   char* ws = static_cast<char*>(workspace);
   float* scale = reinterpret_cast<float*>(ws);
-  float* coef = reinterpret_cast<float*>(ws + b.coef);
+  float2* rows2 = reinterpret_cast<float2*>(ws + b.rows2);
   if (p.dtype == MHS_F16 && rs.per_row) {
     hipLaunchKernelGGL(mhs::head_largest_kernel<>, dim3(1), dim3(1024), 0, s, rs, scale + 2,
                        (long long)p.rows);
     if ((rc = check_launch("largest gradient kernel")) != 0) return rc;
   }
-  rc = launch_rows_in(p, b, rs, coef, scale, out.dweight ? ws + b.hidden : nullptr, s);
+  rc = launch_rows_in(p, b, rs, lse2, rows2, scale, out.dweight ? ws + b.hidden : nullptr, s);
   if (rc) return rc;
-  a.coef = coef;
+  a.rows2 = rows2;
   a.scale = scale;
   a.dz = ws + b.dz;
   a.ldz = b.ldz;
@@ -582,13 +590,12 @@ int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* 
   if (reduction == MHS_REDUCE_MEAN && rows > 0 && !count)
     return fail(MHS_EINVAL, "null pointer argument");
   mhs::HeadGrad a{};
-  a.lse2 = lse2;
   a.ids = ll(targets);
   a.picked = picked;
   a.k = 1;
   a.c = mhs::kLog2e;
-  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, 1.f), BwdOut{dhidden, dweight},
-                  workspace, workspace_bytes, stream);
+  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, 1.f), lse2,
+                  BwdOut{dhidden, dweight}, workspace, workspace_bytes, stream);
 }
 
 int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
@@ -628,13 +635,12 @@ int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const voi
   if (rows > 0 && (!q || (reduction == MHS_REDUCE_MEAN && !count)))
     return fail(MHS_EINVAL, "null pointer argument");
   mhs::HeadGrad a{};
-  a.lse2 = lse2;
   a.ids = ll(ids);
   a.q = q;
   a.picked = picked;
   a.k = (int)top;
   a.c = mhs::kLog2e / temperature;
-  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, temperature),
+  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, temperature), lse2,
                   BwdOut{dhidden, dweight}, workspace, workspace_bytes, stream);
 }
 

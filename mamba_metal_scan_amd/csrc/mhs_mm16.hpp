@@ -72,6 +72,14 @@ struct MmArgs {
   int group_m;          // tiles of a group share the operands' tiles in L2 (see mm_tile)
 };
 
+// The resource of a direct load from p on (offsets below kOOB).
+__device__ __forceinline__ i32x4 mm_resource(const void* p) {
+  const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a),
+               __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)), (int)(kOOB - 1u),
+               0x00020000};
+}
+
 // 64 lanes x 16 bytes from memory straight into LDS at `lds` + 16 lane; lanes at
 // or past the resource's end write zeros. Not tracked by the compiler: the
 // kernel waits for it with mm_wait, and no register is written.
@@ -89,8 +97,17 @@ __device__ __forceinline__ void mm_wait() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 
-// One operand of a block of WAVES waves: R rows from r0 of `rows`, k tiles BK deep.
-template <int R, bool KMAJOR, int WAVES, int MI, int BK>
+// The row of the tile that a transposing epilogue's LDS row x holds: within 64
+// rows (4 fragments i of 16 rows x % 16) the first halves of the fragments follow
+// each other, then the second halves. After the epilogue has exchanged fragments
+// and groups of 16 lanes, a lane then holds 8 neighbours, and the 4 groups 32.
+__device__ __forceinline__ constexpr int mm_perm(int x) {
+  return (x & ~63) + (x & 8) * 4 + ((x >> 4) & 3) * 8 + (x & 7);
+}
+
+// One operand of a block of WAVES waves: R rows from r0 of `rows`, k tiles BK
+// deep. PERM: its rows lie in LDS in mm_perm's order (K-major).
+template <int R, bool KMAJOR, int WAVES, int MI, int BK, bool PERM = false>
 struct MmOperand {
   static constexpr int kBytes = R * BK * 2;                // of a k tile
   static constexpr int kLoads = kBytes / 1024 / WAVES;     // direct loads per wave and k tile
@@ -115,28 +132,12 @@ struct MmOperand {
   // wrow: the wave's first row within the tile.
   __device__ __forceinline__ MmOperand(const void* p, long long ld, int r0, int rows, int k_first,
                                        int wave, int lane, int wrow) {
-    const int first = wave * kLoads * (64 / kLanes) + lane / kLanes;   // (k) row of load 0
+    place(p, ld, r0, rows, k_first, wave, lane);
     if constexpr (KMAJOR) {
-      base = static_cast<const char*>(p) + ((long long)r0 * ld + k_first) * 2;
       step = BK * 2;
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int row = first + j * (64 / kLanes);
-        const int c = (lane % kLanes) ^ swz(row);
-        voff[j] = r0 + row < rows ? 2u * ((unsigned)row * (unsigned)ld + 8u * c) : kOOB;
-        kpos[j] = 8 * c;
-      }
       frag = (wrow + lane % MI) * (2 * BK) + ((lane / MI ^ swz(lane & 15)) << 4);
     } else {
-      base = static_cast<const char*>(p) + ((long long)k_first * ld + r0) * 2;
       step = ld * (2 * BK);
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int k = first + j * (64 / kLanes);
-        const int c = (lane % kLanes) ^ swz(k);
-        voff[j] = r0 + 8 * c < rows ? 2u * ((unsigned)k * (unsigned)ld + 8u * c) : kOOB;
-        kpos[j] = k;
-      }
       // Fragment element (row, k) of a lane: row lane % MI, k 8 (lane / MI) + 0..7;
       // the transposing read's own address: k row 8 (lane / MI) + (lane % 16) / 4
       // (+ 4 for its second half), 4 rows from 16 (lane % MI / 16) + 4 (lane % 4).
@@ -145,14 +146,25 @@ struct MmOperand {
       frag = k * (2 * R) + ((2 * row) ^ (swz(k) << 4));
     }
   }
+  // The loads at rows r0 .., k's k_first ...
+  __device__ __forceinline__ void place(const void* p, long long ld, int r0, int rows, int k_first,
+                                        int wave, int lane) {
+    const int first = wave * kLoads * (64 / kLanes) + lane / kLanes;   // (k) row of load 0
+    base = static_cast<const char*>(p) +
+           (KMAJOR ? (long long)r0 * ld + k_first : (long long)k_first * ld + r0) * 2;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int row = first + j * (64 / kLanes);   // (row-major: k)
+      const int c = (lane % kLanes) ^ swz(row);
+      const int at = PERM ? mm_perm(row) : row;
+      voff[j] = (KMAJOR ? r0 + at : r0 + 8 * c) < rows
+                    ? 2u * ((unsigned)at * (unsigned)ld + 8u * c) : kOOB;
+      kpos[j] = KMAJOR ? 8 * c : row;
+    }
+  }
   // The resource over the next k tile to load, and on to the one after it.
   __device__ __forceinline__ i32x4 next() {
-    i32x4 r;
-    const unsigned long long a = reinterpret_cast<unsigned long long>(base);
-    r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
-    r[1] = __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32));
-    r[2] = (int)(kOOB - 1u);
-    r[3] = 0x00020000;
+    const i32x4 r = mm_resource(base);
     base += step;
     return r;
   }
@@ -177,13 +189,13 @@ struct MmOperand {
   }
 };
 
-// The block's tile (m0, n0) of grid_m x grid_n. Blocks go round the 8 XCDs: each
-// takes a contiguous run of tiles, so that the rows of A and B it shares stay in
-// its own L2; a run goes through groups of group_m tiles in m, n after n.
-__device__ __forceinline__ void mm_tile(const MmArgs& g, int& tm, int& tn) {
+// Tile `index` of grid_m x grid_n. Blocks go round the 8 XCDs: each takes a
+// contiguous run of tiles, so that the rows of A and B it shares stay in its own
+// L2; a run goes through groups of group_m tiles in m, n after n.
+__device__ __forceinline__ void mm_tile(const MmArgs& g, int index, int& tm, int& tn) {
   const int tiles = g.grid_m * g.grid_n;
-  const int xcd = blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
-  const int t = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+  const int xcd = index & 7, per = tiles >> 3, rem = tiles & 7;
+  const int t = xcd * per + min(xcd, rem) + (index >> 3);
   const int in_group = g.group_m * g.grid_n;
   const int first = t / in_group * g.group_m;
   const int size = min(g.group_m, g.grid_m - first);
@@ -211,10 +223,6 @@ struct MmShape {
   static __device__ __forceinline__ int wave_n(int wave) { return HALF ? wave / WM : wave % WN; }
   typedef float acc __attribute__((ext_vector_type(E)));
   static constexpr int kLds = ST * (BM + BN) * BK * 2;
-  // The tile in 16 bits, transposed: rows of BM elements, 16 bytes (4 banks) on
-  // per row.
-  static constexpr int kRow = BM + 8;
-  static constexpr int kTileLds = kLds > BN * kRow * 2 ? kLds : BN * kRow * 2;
 };
 
 // acc = the tile's sums over k's k_first .. k_first + k_len - 1. A fragment's
@@ -324,6 +332,126 @@ __device__ __forceinline__ void mm_products(typename S::acc (&acc)[S::FM][S::FN]
     }
   }
   mm_wait<0>();
+}
+
+// v, without the compiler's knowledge of it: what is computed from it within a
+// loop is computed there, not kept in registers across the loop.
+__device__ __forceinline__ int mm_opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// The tiles blockIdx.x, + gridDim.x, ... of a product of two K-major operands as
+// one stream of k tiles: the direct loads run on into the next tile while this
+// one's last k tiles are multiplied and while epi(acc, m0, n0) works on its sums
+// (without the stages' LDS), so that only the first tile waits for memory. A's rows
+// lie in mm_perm's order: a fragment's element e of lane l in fragment i is row
+// 64 (i / 4) + 32 (l / 32) + 8 (i % 4) + 4 (l / 16 % 2) + e of the wave's.
+template <class T, class S, class Side, class Epi>
+__device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side& side,
+                                          const Epi& epi) {
+  static_assert(S::ST == 2, "every k tile waits for all loads before it: side's too");
+  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, BK = S::BK, PH = BK * S::MI / 512;
+  static_assert(S::MI == 16 && S::SUB == 1 && PH % 2 == 0 && FM % 4 == 0, "the shape streams");
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typedef MmOperand<S::BM, true, S::kWaves, 16, BK, true> OA;
+  typedef MmOperand<S::BN, true, S::kWaves, 16, BK> OB;
+  constexpr int LA = OA::kLoads, LB = OB::kLoads, L = LA + LB;
+  constexpr int TA = OA::kBytes, BUF = TA + OB::kBytes;
+  const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
+  const int tiles = g.grid_m * g.grid_n, nk = (g.K + BK - 1) / BK;
+  // Where the loads are: k tile load_kt of tile load_tile.
+  int load_tile = blockIdx.x, load_kt = 0, load_odd = 0, tm, tn;
+  mm_tile(g, load_tile, tm, tn);
+  OA a(g.A, g.lda, tm * S::BM, g.M, 0, wave, lane, S::wave_m(wave) * (FM * 16));
+  OB b(g.B, g.ldb, tn * S::BN, g.N, 0, wave, lane, S::wave_n(wave) * (FN * 16));
+  side(tn * S::BN, 0);
+  // The resources of the next k tile to load, and the k's from its start.
+  auto next = [&](i32x4& ra, i32x4& rb) {
+    if (load_kt == nk) {
+      load_kt = 0;
+      load_tile += gridDim.x;
+      load_odd ^= 1;
+      if (load_tile < tiles) {
+        mm_tile(g, load_tile, tm, tn);
+        const int l = mm_opaque(lane);
+        a.place(g.A, g.lda, tm * S::BM, g.M, 0, wave, l);
+        b.place(g.B, g.ldb, tn * S::BN, g.N, 0, wave, l);
+        side(tn * S::BN, load_odd);
+      }
+    }
+    ra = a.next();
+    rb = b.next();
+    return load_tile < tiles ? g.K - load_kt++ * BK : 0;
+  };
+#pragma unroll
+  for (int s = 0; s < ST; ++s) {
+    i32x4 ra, rb;
+    const int left = next(ra, rb);
+#pragma unroll
+    for (int j = 0; j < LA; ++j) a.load(ra, j, at + s * BUF, left, wave);
+#pragma unroll
+    for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, left, wave);
+  }
+  mm_wait<(ST - 1) * L>();
+  s16x8 fa[2][FM], fb[2][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) fa[0][i] = a.read(lds, i, 0);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) fb[0][j] = b.read(lds + TA, j, 0);
+  int cur = 0, odd = 0;   // the buffer of the k tile; the tile's side
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, odd ^= 1) {
+    typename S::acc acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = typename S::acc{0.f, 0.f, 0.f, 0.f};
+    for (int kt = 0; kt < nk; ++kt) {
+      const int next_buf = cur + 1 == ST ? 0 : cur + 1;
+      i32x4 ra, rb;
+      int left = 0;
+#pragma unroll
+      for (int p = 0; p < PH; ++p) {
+        if (p == PH - 1) {   // (as in mm_products)
+          mm_wait<(ST - 2) * L>();
+          left = next(ra, rb);
+        }
+        const char* nb = lds + (p == PH - 1 ? next_buf : cur) * BUF;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          constexpr int F = FM + FN;
+#pragma unroll
+          for (int f = i * F / FM; f < (i + 1) * F / FM; ++f) {
+            if (f < FM) fa[1 - p % 2][f] = a.read(nb, f, (p + 1) % PH);
+            else fb[1 - p % 2][f - FM] = b.read(nb + TA, f - FM, (p + 1) % PH);
+          }
+          if (p == PH - 1) {
+#pragma unroll
+            for (int l = i * L / FM; l < (i + 1) * L / FM; ++l) {
+              if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
+              else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = T::mfma(fa[p % 2][i], fb[p % 2][j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      cur = next_buf;
+    }
+    int em, en;
+    mm_tile(g, tile, em, en);
+    epi(acc, em * S::BM, en * S::BN, odd);
+  }
+  mm_wait<0>();   // (no load may outlive the block)
+}
+
+// LDS written before by any wave of the block is visible after (without a wait
+// for the direct loads, as __syncthreads would have).
+__device__ __forceinline__ void mm_lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
 }  // namespace mhs
