@@ -161,10 +161,15 @@ head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part) {
 
 // --------------------------------------------------------------- few rows
 //
-// Up to 16 NF rows: bound by reading W once. A wave takes 16 words at a time
-// straight from memory as operands of 16 x 16 MFMAs (lane: word lane % 16, 16
-// bytes at lane / 16 of each 64), the rows' operands beside them (in L1 and L2),
-// so nothing is staged.
+// Up to 16 NF rows: bound by reading W once. A block takes 64 words straight from
+// memory as operands of 16 x 16 MFMAs (lane: word lane % 16, 16 bytes at lane / 16
+// of each 64), the rows' operands beside them (in L1 and L2), so nothing is
+// staged. The waves share the block's words and cut up k, 128 bytes of each row in
+// turn, so that a row's operand serves four of the words'; their sums meet in LDS.
+// (With 16 words and all of k to a wave the rows' operands are read as often as
+// the words': 16 rows of 4096 x 131072 words took 584 us in fp32 and 294 in bf16,
+// against 476 and 254, which is 4.5 TB/s and 4.2; one row 447 and 222 against 436
+// and 218. 640 x 32768, 16 rows, with the loss: 29 us and 19.)
 
 constexpr int kSmallWords = 64;   // per block of 4 waves
 
@@ -214,46 +219,65 @@ template <class T, int NF>
 __global__ void __launch_bounds__(256)
 head_small_kernel(SmallArgs g, float c, float2* __restrict__ part) {
   typedef SmallMma<T> M;
+  constexpr int FW = kSmallWords / 16;   // fragments of words; one for each wave at the end
+  __shared__ f32x4 sums[FW][4][NF][64];
   __shared__ float red[2][4][16 * NF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int word = blockIdx.x * kSmallWords + wave * 16 + (lane & 15);
+  const int word = blockIdx.x * kSmallWords + (lane & 15);
   const int k0 = kVec<T> * (lane >> 4);
-  const elem_t<T>* w = static_cast<const elem_t<T>*>(g.w) + (long long)word * g.ldw;
+  const elem_t<T>* w[FW];
   const elem_t<T>* h[NF];
-  bool ok[NF];
+  bool okw[FW], ok[NF];
+#pragma unroll
+  for (int i = 0; i < FW; ++i) {
+    okw[i] = word + 16 * i < g.vocab;
+    w[i] = static_cast<const elem_t<T>*>(g.w) + (long long)(okw[i] ? word + 16 * i : 0) * g.ldw;
+  }
 #pragma unroll
   for (int j = 0; j < NF; ++j) {
     const int r = 16 * j + (lane & 15);
     ok[j] = r < g.rows;
     h[j] = static_cast<const elem_t<T>*>(g.h) + (long long)(ok[j] ? r : 0) * g.ldh;
   }
-  f32x4 acc[NF] = {};
-  constexpr int U = 8;   // k steps whose loads are in flight together
-  for (int k = 0; k < g.dim; k += U * M::kDepth) {
-    typename M::frag a[U], b[U][NF];
+  f32x4 acc[FW][NF] = {};
+  constexpr int U = 2;   // k steps whose loads are in flight together, 128 bytes of each row
+                         // (503 us with 4, 520 with 8 where 2 take 476: 16 x 4096 x 131072, fp32)
+  for (int k = 2 * wave * M::kDepth; k < g.dim; k += 4 * U * M::kDepth) {
+    typename M::frag a[U][FW], b[U][NF];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = k + u * M::kDepth + k0;
-      a[u] = small_load<T>(w, at, g.dim, word < g.vocab);
+#pragma unroll
+      for (int i = 0; i < FW; ++i) a[u][i] = small_load<T>(w[i], at, g.dim, okw[i]);
 #pragma unroll
       for (int j = 0; j < NF; ++j) b[u][j] = small_load<T>(h[j], at, g.dim, ok[j]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < NF; ++j) acc[j] = M::mma(a[u], b[u][j], acc[j]);
+      for (int i = 0; i < FW; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = M::mma(a[u][i], b[u][j], acc[i][j]);
   }
-  // Element e of a lane: word 4 (lane / 16) + e, row lane % 16.
+#pragma unroll
+  for (int i = 0; i < FW; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) sums[i][wave][j][lane] = acc[i][j];
+  __syncthreads();
+  // The wave joins fragment `wave`. Element e of a lane: word 4 (lane / 16) + e,
+  // row lane % 16.
   const int left = g.vocab - (blockIdx.x * kSmallWords + wave * 16 + 4 * (lane >> 4));
 #pragma unroll
   for (int j = 0; j < NF; ++j) {
+    f32x4 z = sums[wave][0][j][lane];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) z += sums[wave][v][j][lane];
     float m = -INFINITY, s = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) m = fmaxf(m, e < left ? acc[j][e] * c : -INFINITY);
+    for (int e = 0; e < 4; ++e) m = fmaxf(m, e < left ? z[e] * c : -INFINITY);
     const float sh = lse2_shift(m);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      s += e < left ? exp2_hw(__builtin_fmaf(acc[j][e], c, -sh)) : 0.f;
+    for (int e = 0; e < 4; ++e) s += e < left ? exp2_hw(__builtin_fmaf(z[e], c, -sh)) : 0.f;
 #pragma unroll
     for (int o = 16; o <= 32; o *= 2)
       lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
@@ -428,7 +452,7 @@ head_distill_rows_kernel(HeadRows g) {
   __shared__ float red[4];
   const int r = blockIdx.x, wave = threadIdx.x >> 6;
   const elem_t<T>* h = static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh;
-  constexpr int U = 4;   // words at a time (one: 138 us at 8192 x 640, 64 words; four: see below)
+  constexpr int U = 4;   // words at a time (8192 x 640, 64 words: one 138 us, four 105)
   for (int k = U * wave; k < g.k; k += 4 * U) {
     const elem_t<T>* word[U];
     bool in[U];

@@ -27,14 +27,21 @@ using mhs::round_up;
 typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64, false> Shape;
 typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64, true> HalfShape;   // (the gradients')
 
-// Rows that the kernel for few rows takes.
-constexpr int64_t kSmallRows = 32;
+// Rows that the kernel for few rows takes, by bytes of an element. us of it and of
+// the tiles, with the loss's kernel: fp32, 32 rows, 640 x 32768 36 and 46, 4096 x
+// 131072 654 and 702 (its registers hold no more rows); 16 bits, 16 rows, 19 and 25,
+// 254 and 236, and one row 17 and 24, 218 and 239; at 32 rows it took 20 and 25, but
+// 62 and 54 with 2048 x 50257 and 282 and 239 with 4096 x 131072.
+constexpr int64_t small_rows(int elem) { return elem == 4 ? 32 : 16; }
 // Bytes of dz that the backward holds at a time (at least 256 words' worth). us
 // with 64, 128, 256 and 512 MB: 8192 x 640 x 32768 bf16 2550, 1780, 1559, 1589;
 // 8192 x 4096 x 131072 29520, 27080, 26130, 25700; fp32 (the first) 8640, 7755,
 // 7407, 7257.
 constexpr int64_t kPieceBytes = 256LL << 20;
-constexpr int64_t kLossOneBlock = 16384;   // rows that one block sums
+// Rows that one block sums. (us with one block and with blocks of 4096 rows and a
+// last one, behind a kernel of one block per row: 4096 rows 32.7 and 34.9, 8192 56.6
+// and 57.8, 16384 101.9 and 100.5, 65536 384 and 367.)
+constexpr int64_t kLossOneBlock = 8192;
 
 int elem_bytes(int dtype) { return dtype == MHS_F32 ? 4 : 2; }
 
@@ -109,9 +116,11 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 
 // ----------------------------------------------------------------- forward
 
+bool few_rows(const Head& p) { return p.rows <= small_rows(elem_bytes(p.dtype)); }
+
 // Tiles of the vocabulary in the forward's partials.
 int64_t lse_tiles(const Head& p) {
-  if (p.rows <= kSmallRows) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
+  if (few_rows(p)) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
   const int bm = p.dtype == MHS_F32 ? mhs::kGemmTile : Shape::BM;
   return (p.vocab + bm - 1) / bm;
 }
@@ -132,7 +141,9 @@ void allow_lds(F* fn, int bytes) {
                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-// Tiles in m per group of the block order (mm_tile).
+// Tiles in m per group of the block order (mm_tile). (us of the loss and its
+// gradients with 1, 2, 4, 8 and 16, bf16: 8192 x 640 x 32768 1633, 1485, 1473, 1506,
+// 1539; 8192 x 4096 x 131072 28090, 26580, 26120, 26520, 27210.)
 constexpr int kGroupM = 4;
 
 template <class S>
@@ -186,13 +197,15 @@ int launch_lse16(const Head& p, float c, float2* part, hipStream_t s) {
 template <class T>
 int launch_small(const Head& p, float c, float2* part, hipStream_t s) {
   const mhs::SmallArgs g{p.hidden, p.weight, p.ldh, p.ldw, (int)p.rows, (int)p.vocab, (int)p.dim};
-  hipLaunchKernelGGL((p.rows <= 16 ? &mhs::head_small_kernel<T, 1> : &mhs::head_small_kernel<T, 2>),
-                     dim3((unsigned)lse_tiles(p)), dim3(256), 0, s, g, c, part);
+  auto fn = &mhs::head_small_kernel<T, 1>;
+  if constexpr (small_rows(sizeof(mhs::elem_t<T>)) > 16)
+    if (p.rows > 16) fn = &mhs::head_small_kernel<T, 2>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)lse_tiles(p)), dim3(256), 0, s, g, c, part);
   return check_launch("head log-sum-exp kernel of few rows");
 }
 
 int launch_lse(const Head& p, float c, float2* part, hipStream_t s) {
-  if (p.rows <= kSmallRows)
+  if (few_rows(p))
     return p.dtype == MHS_F32    ? launch_small<Fp32>(p, c, part, s)
            : p.dtype == MHS_BF16 ? launch_small<Bf16>(p, c, part, s)
                                  : launch_small<Fp16>(p, c, part, s);

@@ -67,7 +67,8 @@ def _run(f, h, w, up, *args, **kw):
 
 
 SIZES = [(1, 8, 1), (1, 64, 7), (3, 64, 257), (16, 640, 1000), (17, 128, 65), (32, 72, 256),
-         (33, 64, 255), (127, 192, 300), (129, 64, 513), (300, 1024, 1001), (515, 56, 5003)]
+         (33, 64, 255), (127, 192, 300), (129, 64, 513), (300, 1024, 1001), (515, 56, 5003),
+         (13, 1160, 1030), (24, 2056, 131)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -291,7 +292,7 @@ def test_no_rows():
     assert torch.isnan(got[0]) and (got[2] == 0).all()
 
 
-@pytest.mark.parametrize("rows", [16384, 16385, 20000])
+@pytest.mark.parametrize("rows", [8192, 8193, 16384, 16385, 20000])
 def test_many_rows_of_losses(rows):
     """On both sides of the loss's one block."""
     h, w, t = _operands(rows, 8, 5, F32)

@@ -142,14 +142,16 @@ def test_logits_entries_refuse():
 
 
 def test_workspace_sizes():
-    """Forward: 8 bytes per row and tile of the vocabulary (64 words for up to 32
-    rows, 256, or 128 in fp32). Backward: the logits' gradient is bounded, a
+    """Forward: 8 bytes per row and tile of the vocabulary (64 words for up to 16
+    rows, 32 in fp32; above, 256, or 128 in fp32). Backward: the logits' gradient is bounded, a
     piece of the vocabulary; none for sizes that the calls reject."""
     lib = _native.library()
     fwd, bwd = lib.mhs_linear_xent_fwd_workspace_bytes, lib.mhs_linear_xent_bwd_workspace_bytes
     assert fwd(1, 8192, 32768, 640) == 8192 * 128 * 8
     assert fwd(0, 8192, 32768, 640) == 8192 * 256 * 8
     assert fwd(1, 4, 32768, 640) == 4 * 512 * 8
+    assert fwd(1, 17, 32768, 640) == 17 * 128 * 8
+    assert fwd(0, 32, 32768, 640) == 32 * 512 * 8
     whole = 8192 * 131072 * 2
     assert bwd(1, 8192, 131072, 64) < whole / 4
     assert bwd(1, 1, 131072, 640) < 2 << 20
