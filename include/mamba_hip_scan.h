@@ -417,7 +417,7 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
 
 /*
  * Losses of the model's head from its hidden states, the logits z = hidden
- * weight^T never in memory. Beside mhs_xent_*, which read given logits; the
+ * weight^T not in memory (but where a caller keeps them, below). Beside mhs_xent_*, which read given logits; the
  * reference forms them (mamba_metal/model.py:294-297).
  *
  *   hidden (rows, dim) rows ldh elements apart, weight (vocab, dim) rows ldw
@@ -439,6 +439,10 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
  *   words of it. Of 16-bit operands it is rounded to 16 bits there (fp16 scaled
  *   by a power of two), as the products' operands are; the sums are fp32. Rows
  *   that are not kept add nothing, whatever they hold, and get zeros.
+ * logits, if given (16-byte aligned, else NULL): the forward keeps the fp32 logits
+ *   there, (rows, vocab to a multiple of 4), for MHS_F32 (vocab, rows to a multiple
+ *   of 4), and the backward reads them instead of forming them a second time. The
+ *   other calls hold no more of them than a tile.
  * Every sum runs in a fixed order (bit-for-bit reproducible). The workspace is
  * 256-byte aligned; its size is 0 for arguments that the calls reject.
  */
@@ -452,15 +456,15 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
 size_t mhs_linear_xent_fwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim);
 int mhs_linear_xent_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                         int64_t ldw, const int64_t* targets, float* lse2, float* picked,
-                        float* keep, float* loss_rows, float* loss, float* count, int64_t rows,
-                        int64_t vocab, int64_t dim, int64_t ignore_index, int reduction,
-                        void* workspace, size_t workspace_bytes, void* stream);
+                        float* keep, float* logits, float* loss_rows, float* loss, float* count,
+                        int64_t rows, int64_t vocab, int64_t dim, int64_t ignore_index,
+                        int reduction, void* workspace, size_t workspace_bytes, void* stream);
 
 size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim);
 int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                         int64_t ldw, const int64_t* targets, const float* lse2,
-                        const float* picked, const float* keep, const float* upstream,
-                        const float* count, void* dhidden, void* dweight, int64_t rows,
+                        const float* picked, const float* keep, const float* logits,
+                        const float* upstream, const float* count, void* dhidden, void* dweight, int64_t rows,
                         int64_t vocab, int64_t dim, int reduction, void* workspace,
                         size_t workspace_bytes, void* stream);
 
@@ -474,25 +478,25 @@ int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* 
  * -inf, is empty: loss 0, keep 0; an id at or past vocab makes the row's loss NaN.
  * Outputs as above, and for the backward picked (rows, top), lse2 = log2 sum_v
  * exp(z / t) and q (rows, top), each word's whole weight in its row (a word that a
- * row names twice has the sum at both); dz[r, v] = t (p[v] - sum_{ids_k = v} q_k) times the gradient that
- * reaches the row's loss. The teacher gets no gradient. The workspaces are the
- * cross entropy's. No counterpart in the reference.
+ * row names twice has the sum at both); dz[r, v] = t (p[v] - sum_{ids_k = v} q_k)
+ * times the gradient that reaches the row's loss. The teacher gets no gradient. The
+ * workspaces are the cross entropy's. No counterpart in the reference.
  */
 #define MHS_MAX_TOP 1024
 
 int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                            int64_t ldw, const float* teacher, const int64_t* ids, float* lse2,
-                           float* picked, float* q, float* keep, float* loss_rows, float* loss,
-                           float* count, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
-                           float temperature, int reduction, void* workspace,
-                           size_t workspace_bytes, void* stream);
+                           float* picked, float* q, float* keep, float* logits,
+                           float* loss_rows, float* loss, float* count, int64_t rows,
+                           int64_t vocab, int64_t dim, int64_t top, float temperature,
+                           int reduction, void* workspace, size_t workspace_bytes, void* stream);
 int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                            int64_t ldw, const int64_t* ids, const float* lse2,
                            const float* picked, const float* q, const float* keep,
-                           const float* upstream, const float* count, void* dhidden,
-                           void* dweight, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
-                           float temperature, int reduction, void* workspace,
-                           size_t workspace_bytes, void* stream);
+                           const float* logits, const float* upstream, const float* count,
+                           void* dhidden, void* dweight, int64_t rows, int64_t vocab,
+                           int64_t dim, int64_t top, float temperature, int reduction,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The same distillation of given logits (rows, vocab) of `dtype`, rows ld

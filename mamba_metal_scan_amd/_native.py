@@ -186,12 +186,12 @@ def library() -> ctypes.CDLL:
             lib.mhs_distill_workspace_bytes.restype = _size
             lib.mhs_distill_workspace_bytes.argtypes = [_I64]
             for name, args in (
-                    ("mhs_linear_xent_fwd", head + [_P] * 7 + [_I64] * 4 + [_int, _P, _size, _P]),
-                    ("mhs_linear_xent_bwd", head + [_P] * 8 + [_I64] * 3 + [_int, _P, _size, _P]),
+                    ("mhs_linear_xent_fwd", head + [_P] * 8 + [_I64] * 4 + [_int, _P, _size, _P]),
+                    ("mhs_linear_xent_bwd", head + [_P] * 9 + [_I64] * 3 + [_int, _P, _size, _P]),
                     ("mhs_linear_distill_fwd",
-                     head + [_P] * 9 + [_I64] * 4 + [_F32, _int, _P, _size, _P]),
+                     head + [_P] * 10 + [_I64] * 4 + [_F32, _int, _P, _size, _P]),
                     ("mhs_linear_distill_bwd",
-                     head + [_P] * 9 + [_I64] * 4 + [_F32, _int, _P, _size, _P]),
+                     head + [_P] * 10 + [_I64] * 4 + [_F32, _int, _P, _size, _P]),
                     ("mhs_distill_fwd",
                      [_int, _P, _I64] + [_P] * 8 + [_I64] * 3 + [_F32, _int, _P, _size, _P]),
                     ("mhs_distill_bwd",
@@ -1263,7 +1263,8 @@ def _gemm_add_fake(out, a, b, form):
 # distillation of given logits. What a forward keeps for its backward is one
 # fp32 tensor, `saved`: the count of rows kept (in the first of 4 elements),
 # then per row lse2, keep, the losses, and picked and q of its `top` words (q
-# not for the cross entropy, picked not for given logits).
+# not for the cross entropy, picked not for given logits); and at a multiple of 4
+# elements, if the forward was to keep them, the logits.
 
 REDUCE = {"none": 0, "mean": 1, "sum": 2}
 HEAD_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -1292,6 +1293,42 @@ def _saved_parts(saved: torch.Tensor, rows: int, *tops: int) -> list[int]:
 
 def _saved_size(rows: int, *tops: int) -> int:
     return 4 + rows * (3 + sum(tops))
+
+
+KEPT_BYTES = 1 << 30
+
+
+def keeps_logits(rows: int, vocab: int, dim: int, dtype: torch.dtype) -> bool:
+    """Whether a forward that has a backward keeps its fp32 logits for it, up to
+    1 GB of them: three products instead of four, against writing and reading
+    them. us of the loss and its gradients, formed twice and kept: fp32 512 x 256
+    x 32768 266 and 243, 512 x 4096 x 131072 11420 and 8770; bf16 by the rows, 128
+    x 640 x 32768 149 and 138, 256 152 and 150, 512 174 and 181, 2048 409 and 575,
+    but with 1024 columns 512 x 50257 335 either way, with 2048 563 and 510, with
+    4096 512 x 131072 2370 and 2040."""
+    return rows * vocab * 4 <= KEPT_BYTES and (dtype == torch.float32 or rows <= 256
+                                               or dim >= 2048)
+
+
+def _kept_size(hidden: torch.Tensor, weight: torch.Tensor) -> int:
+    """Elements of the kept logits: (rows, vocab to a multiple of 4), or (vocab,
+    rows to a multiple of 4) in fp32."""
+    rows, vocab = hidden.shape[0], weight.shape[0]
+    if hidden.dtype == torch.float32:
+        rows, vocab = vocab, rows
+    return rows * ((vocab + 3) // 4 * 4)
+
+
+def _saved_sizes(hidden, weight, *tops: int) -> tuple[int, int]:
+    """saved's elements without and with the logits."""
+    n = _saved_size(hidden.shape[0], *tops)
+    return n, (n + 3) // 4 * 4 + _kept_size(hidden, weight)
+
+
+def _kept_logits(saved: torch.Tensor, hidden: torch.Tensor, *tops: int) -> int | None:
+    """The address of the logits in saved, or None."""
+    n = _saved_size(hidden.shape[0], *tops)
+    return None if saved.shape[0] == n else saved.data_ptr() + (n + 3) // 4 * 16
 
 
 def _check_head(what: str, hidden, weight, reduction) -> None:
@@ -1327,11 +1364,16 @@ def _check_top(what: str, rows: int, teacher_logits, ids, temperature) -> None:
         raise HipScanError(f"{what}: temperature must be positive and finite; got {temperature}")
 
 
-def _check_bwd_head(what: str, grad, saved, rows: int, reduction: int, *tops: int) -> None:
+def _check_bwd_head(what: str, grad, saved, rows: int, reduction: int, size: int,
+                    kept: int = -1) -> None:
+    """saved of `size` elements or, with the logits, `kept`."""
     _fp32(what, grad=grad, saved=saved)
     _dense(what, grad=grad, saved=saved)
     _shaped(what, "grad", grad, (rows,) if reduction == 0 else ())
-    _shaped(what, "saved", saved, (_saved_size(rows, *tops),))
+    if tuple(saved.shape) != (kept,):
+        _shaped(what, "saved", saved, (size,))
+    elif saved.data_ptr() % 16:
+        raise HipScanError(f"{what}: saved must be 16-byte aligned")
 
 
 def _workspace(nbytes: int, what: str, dev: torch.device) -> torch.Tensor:
@@ -1345,7 +1387,7 @@ def _new_loss(t: torch.Tensor, rows: int, reduction: int) -> torch.Tensor:
 
 
 def _linear_xent_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
-                          ignore_index: int, reduction: int
+                          ignore_index: int, reduction: int, keep_logits: bool = False
                           ) -> tuple[torch.Tensor, torch.Tensor]:
     """(loss () or (rows,), saved) of hidden (rows, dim) against targets (rows)."""
     rows, dim = hidden.shape
@@ -1354,14 +1396,15 @@ def _linear_xent_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor, targets: t
     lib = library()
     dt = HEAD_DTYPES[hidden.dtype]
     loss = _new_loss(hidden, rows, reduction)
-    saved = torch.empty(_saved_size(rows, 1), dtype=torch.float32, device=dev)
+    saved = torch.empty(_saved_sizes(hidden, weight, 1)[keep_logits], dtype=torch.float32,
+                        device=dev)
     count, lse2, keep, losses, picked = _saved_parts(saved, rows, 1)
     with _on(dev):
         nbytes = lib.mhs_linear_xent_fwd_workspace_bytes(dt, rows, vocab, dim)
         ws = _workspace(nbytes, "linear_xent_fwd", dev)
         rc = lib.mhs_linear_xent_fwd(
             dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
-            weight.stride(0), targets.data_ptr(), lse2, picked, keep,
+            weight.stride(0), targets.data_ptr(), lse2, picked, keep, _kept_logits(saved, hidden, 1),
             losses if reduction else loss.data_ptr(), loss.data_ptr(), count, rows, vocab, dim,
             ignore_index, reduction, ws.data_ptr(), nbytes, _stream(dev))
     _check(rc, "mhs_linear_xent_fwd")
@@ -1379,15 +1422,15 @@ def _check_linear_xent(what: str, hidden, weight, targets, reduction) -> None:
 
 linear_xent_fwd = _register(
     "linear_xent_fwd", _linear_xent_fwd_impl, (),
-    lambda hidden, weight, targets, ignore_index, reduction:
+    lambda hidden, weight, targets, ignore_index, reduction, keep_logits=False:
     _check_linear_xent("linear_xent_fwd", hidden, weight, targets, reduction))
 
 
 @linear_xent_fwd.register_fake
-def _linear_xent_fwd_fake(hidden, weight, targets, ignore_index, reduction):
-    rows = hidden.shape[0]
-    return (_new_loss(hidden, rows, reduction),
-            hidden.new_empty((_saved_size(rows, 1),), dtype=torch.float32))
+def _linear_xent_fwd_fake(hidden, weight, targets, ignore_index, reduction, keep_logits=False):
+    return (_new_loss(hidden, hidden.shape[0], reduction),
+            hidden.new_empty((_saved_sizes(hidden, weight, 1)[keep_logits],),
+                             dtype=torch.float32))
 
 
 def _head_grads(hidden, weight, need_hidden: bool, need_weight: bool):
@@ -1413,7 +1456,8 @@ def _linear_xent_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: torc
         ws = _workspace(nbytes, "linear_xent_bwd", dev)
         rc = lib.mhs_linear_xent_bwd(
             dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
-            weight.stride(0), targets.data_ptr(), lse2, picked, keep, grad.data_ptr(), count,
+            weight.stride(0), targets.data_ptr(), lse2, picked, keep,
+            _kept_logits(saved, hidden, 1), grad.data_ptr(), count,
             dhidden.data_ptr() if need_hidden else None,
             dweight.data_ptr() if need_weight else None, rows, vocab, dim, reduction,
             ws.data_ptr(), nbytes, _stream(dev))
@@ -1426,7 +1470,7 @@ def _check_linear_xent_bwd(grad, hidden, weight, targets, saved, reduction, need
     what = "linear_xent_bwd"
     _check_linear_xent(what, hidden, weight, targets, reduction)
     _on_one_device(what, hidden, grad, saved)
-    _check_bwd_head(what, grad, saved, hidden.shape[0], reduction, 1)
+    _check_bwd_head(what, grad, saved, hidden.shape[0], reduction, *_saved_sizes(hidden, weight, 1))
 
 
 linear_xent_bwd = _register("linear_xent_bwd", _linear_xent_bwd_impl, (), _check_linear_xent_bwd)
@@ -1440,7 +1484,7 @@ def _linear_xent_bwd_fake(grad, hidden, weight, targets, saved, reduction, need_
 
 def _linear_distill_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor,
                              teacher_logits: torch.Tensor, ids: torch.Tensor,
-                             temperature: float, reduction: int
+                             temperature: float, reduction: int, keep_logits: bool = False
                              ) -> tuple[torch.Tensor, torch.Tensor]:
     """(loss () or (rows,), saved) against the teacher's words ids (rows, top) and
     their logits."""
@@ -1450,7 +1494,8 @@ def _linear_distill_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor,
     lib = library()
     dt = HEAD_DTYPES[hidden.dtype]
     loss = _new_loss(hidden, rows, reduction)
-    saved = torch.empty(_saved_size(rows, top, top), dtype=torch.float32, device=dev)
+    saved = torch.empty(_saved_sizes(hidden, weight, top, top)[keep_logits],
+                        dtype=torch.float32, device=dev)
     count, lse2, keep, losses, picked, q = _saved_parts(saved, rows, top, top)
     with _on(dev):
         nbytes = lib.mhs_linear_xent_fwd_workspace_bytes(dt, rows, vocab, dim)
@@ -1458,6 +1503,7 @@ def _linear_distill_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor,
         rc = lib.mhs_linear_distill_fwd(
             dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
             weight.stride(0), teacher_logits.data_ptr(), ids.data_ptr(), lse2, picked, q, keep,
+            _kept_logits(saved, hidden, top, top),
             losses if reduction else loss.data_ptr(), loss.data_ptr(), count, rows, vocab, dim,
             top, temperature, reduction, ws.data_ptr(), nbytes, _stream(dev))
     _check(rc, "mhs_linear_distill_fwd")
@@ -1473,16 +1519,18 @@ def _check_linear_distill(what: str, hidden, weight, teacher_logits, ids, temper
 
 linear_distill_fwd = _register(
     "linear_distill_fwd", _linear_distill_fwd_impl, (),
-    lambda hidden, weight, teacher_logits, ids, temperature, reduction:
+    lambda hidden, weight, teacher_logits, ids, temperature, reduction, keep_logits=False:
     _check_linear_distill("linear_distill_fwd", hidden, weight, teacher_logits, ids, temperature,
                           reduction))
 
 
 @linear_distill_fwd.register_fake
-def _linear_distill_fwd_fake(hidden, weight, teacher_logits, ids, temperature, reduction):
+def _linear_distill_fwd_fake(hidden, weight, teacher_logits, ids, temperature, reduction,
+                             keep_logits=False):
     rows, top = ids.shape
     return (_new_loss(hidden, rows, reduction),
-            hidden.new_empty((_saved_size(rows, top, top),), dtype=torch.float32))
+            hidden.new_empty((_saved_sizes(hidden, weight, top, top)[keep_logits],),
+                             dtype=torch.float32))
 
 
 def _linear_distill_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
@@ -1502,7 +1550,8 @@ def _linear_distill_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: t
         ws = _workspace(nbytes, "linear_distill_bwd", dev)
         rc = lib.mhs_linear_distill_bwd(
             dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
-            weight.stride(0), ids.data_ptr(), lse2, picked, q, keep, grad.data_ptr(), count,
+            weight.stride(0), ids.data_ptr(), lse2, picked, q, keep,
+            _kept_logits(saved, hidden, top, top), grad.data_ptr(), count,
             dhidden.data_ptr() if need_hidden else None,
             dweight.data_ptr() if need_weight else None, rows, vocab, dim, top, temperature,
             reduction, ws.data_ptr(), nbytes, _stream(dev))
@@ -1515,7 +1564,8 @@ def _check_linear_distill_bwd(grad, hidden, weight, ids, saved, temperature, red
     what = "linear_distill_bwd"
     _check_linear_distill(what, hidden, weight, None, ids, temperature, reduction)
     _on_one_device(what, hidden, grad, saved)
-    _check_bwd_head(what, grad, saved, hidden.shape[0], reduction, ids.shape[1], ids.shape[1])
+    _check_bwd_head(what, grad, saved, hidden.shape[0], reduction,
+                    *_saved_sizes(hidden, weight, ids.shape[1], ids.shape[1]))
 
 
 linear_distill_bwd = _register("linear_distill_bwd", _linear_distill_bwd_impl, (),
@@ -1599,7 +1649,8 @@ def _check_distill_bwd(grad, logits, ids, saved, temperature, reduction):
     what = "distill_bwd"
     _check_distill(what, logits, None, ids, temperature, reduction)
     _on_one_device(what, logits, grad, saved)
-    _check_bwd_head(what, grad, saved, logits.shape[0], reduction, ids.shape[1])
+    _check_bwd_head(what, grad, saved, logits.shape[0], reduction,
+                    _saved_size(logits.shape[0], ids.shape[1]))
 
 
 distill_bwd = _register("distill_bwd", _distill_bwd_impl, (), _check_distill_bwd)

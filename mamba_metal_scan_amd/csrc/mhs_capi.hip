@@ -1716,6 +1716,15 @@ int mhs_gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t 
                  int64_t ldc, int64_t m, int64_t n, int64_t k, int accumulate, void* workspace,
                  size_t workspace_bytes, void* stream) {
   g_err[0] = '\0';
+  return mhs::gemm_f32(form, a, lda, b, ldb, c, ldc, m, n, k, accumulate, nullptr, workspace,
+                       workspace_bytes, stream);
+}
+
+}  // extern "C"
+
+int mhs::gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t ldb, float* c,
+                  int64_t ldc, int64_t m, int64_t n, int64_t k, int accumulate,
+                  const float* alpha, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_gemm(m, n, k);
   if (rc) return rc;
   if (form < MHS_GEMM_NT || form > MHS_GEMM_TN)
@@ -1741,6 +1750,7 @@ int mhs_gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t 
   g.lda = lda; g.ldb = ldb; g.ldc = ldc;
   g.kt_per_split = p.kt_per_split;
   g.accumulate = accumulate;
+  g.alpha = alpha;
   g.grid_m = p.grid_m;
   g.grid_n = p.grid_n;
   if (p.splits > 1) {
@@ -1778,8 +1788,6 @@ int mhs_gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t 
                        (long long)ldc, accumulate);
   return check_launch("matrix product reduction kernel");
 }
-
-}  // extern "C"
 
 // ------------------------------------------------------- one token, whole model
 

@@ -47,6 +47,7 @@ struct GemmArgs {
   long long lda, ldb, ldc;
   int kt_per_split;   // 16-deep k tiles per split
   int accumulate;     // C += (one split only)
+  const float* alpha; // device scalar that the product is multiplied by, or null: 1
   int grid_m, grid_n;
 };
 
@@ -385,6 +386,7 @@ gemm3_kernel(GemmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   float* const cb = g.C + (long long)blockIdx.y * g.M * g.ldc;
+  const float f = g.alpha ? *g.alpha : 1.f;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -396,7 +398,7 @@ gemm3_kernel(GemmArgs g) {
         const int m = mb + 8 * (e / 4) + e % 4;
         if (m < g.M && n < g.N) {
           float* p = cb + (long long)m * g.ldc + n;
-          *p = g.accumulate ? *p + acc[i][j][e] : acc[i][j][e];
+          *p = g.accumulate ? *p + acc[i][j][e] * f : acc[i][j][e] * f;
         }
       }
     }

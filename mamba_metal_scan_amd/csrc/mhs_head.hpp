@@ -96,11 +96,18 @@ __device__ __forceinline__ void store_partials(float* red, float2* part, int n0,
   }
 }
 
-// part[tile of the vocabulary][row] = (m, s) of the tile's logits. A = W (M =
-// vocab), B = h (N = rows).
-template <class T, class S>
+// Logits that a forward keeps for its backward, fp32: (rows, ld) of 16-bit
+// operands, (words, ld) of fp32 ones, as dz; ld a multiple of 4. Null: none.
+struct KeptLogits {
+  float* z;
+  long long ld;
+};
+
+// part[tile of the vocabulary][row] = (m, s) of the tile's logits, and, KEEP, the
+// logits. A = W (M = vocab), B = h (N = rows).
+template <class T, class S, bool KEEP>
 __global__ void __launch_bounds__(S::kThreads, 2)
-head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
+head_lse_kernel(MmArgs g, float c, float2* __restrict__ part, KeptLogits kept) {
   extern __shared__ float lds_f[];
   float* const red = lds_f + S::kLds / 4;   // [WM][max, sum][BN]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -123,6 +130,16 @@ head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
         red[2 * wm * S::BN + n] = m;
         red[(2 * wm + 1) * S::BN + n] = s;
       }
+      if (!KEEP) continue;
+      // 16 bytes a lane, 32 of 16 rows at a time; four stores fill a row's 128.
+      const int r = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+      float* const row = kept.z + (long long)r * kept.ld + g.M - left;
+      if (r < g.N)
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+          if (64 * (i / 4) + 8 * (i % 4) < left)
+            *reinterpret_cast<f32x4*>(row + 64 * (i / 4) + 8 * (i % 4)) =
+                f32x4{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
     }
     mm_lds_barrier();
     store_partials<S::WM>(red, part, n0, g.N, S::BN, m0 / S::BM);
@@ -132,7 +149,7 @@ head_lse_kernel(MmArgs g, float c, float2* __restrict__ part) {
 // The same for fp32 operands, on the products of three bf16 parts.
 template <int TILE>
 __global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
-head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part) {
+head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part, KeptLogits kept) {
   extern __shared__ float lds_f[];
   constexpr int F = TILE / 64;
   int m0, n0;
@@ -154,6 +171,13 @@ head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part) {
       lds_f[2 * wm * TILE + n] = m;
       lds_f[(2 * wm + 1) * TILE + n] = s;
     }
+    const int r = n0 + wn * (TILE / 2) + j * 32 + (lane & 31);
+    if (kept.z && r < g.N)
+#pragma unroll
+      for (int i = 0; i < F * 16; ++i) {
+        const int v = m0 + wm * (TILE / 2) + i / 16 * 32 + 8 * (i % 16 / 4) + 4 * (lane >> 5) + i % 4;
+        if (v < g.M) kept.z[v * kept.ld + r] = acc[i / 16][j][i % 16];
+      }
   }
   __syncthreads();
   store_partials<2>(lds_f, part, n0, g.N, TILE, m0 / TILE);
@@ -217,7 +241,7 @@ __device__ __forceinline__ typename SmallMma<T>::frag small_load(const elem_t<T>
 
 template <class T, int NF>
 __global__ void __launch_bounds__(256)
-head_small_kernel(SmallArgs g, float c, float2* __restrict__ part) {
+head_small_kernel(SmallArgs g, float c, float2* __restrict__ part, KeptLogits kept) {
   typedef SmallMma<T> M;
   constexpr int FW = kSmallWords / 16;   // fragments of words; one for each wave at the end
   __shared__ f32x4 sums[FW][4][NF][64];
@@ -272,6 +296,16 @@ head_small_kernel(SmallArgs g, float c, float2* __restrict__ part) {
     f32x4 z = sums[wave][0][j][lane];
 #pragma unroll
     for (int v = 1; v < 4; ++v) z += sums[wave][v][j][lane];
+    if (kept.z && ok[j] && left > 0) {
+      const long long v = g.vocab - left, r = 16 * j + (lane & 15);
+      if constexpr (__is_same(T, Fp32)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) kept.z[(v + e) * kept.ld + r] = z[e];
+      } else {
+        *reinterpret_cast<f32x4*>(kept.z + r * kept.ld + v) = z;
+      }
+    }
     float m = -INFINITY, s = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = fmaxf(m, e < left ? z[e] * c : -INFINITY);
@@ -542,8 +576,8 @@ struct RowScale {
   }
 };
 
-// largest[0] = the largest |gradient| that reaches a row (per-row upstreams of
-// fp16 products). One block.
+// largest[0] = the largest |gradient| that reaches a row (per-row upstreams). One
+// block.
 template <int UNUSED = 0>
 __global__ void __launch_bounds__(1024)
 head_largest_kernel(RowScale rs, float* __restrict__ largest, long long rows) {
@@ -559,20 +593,24 @@ head_largest_kernel(RowScale rs, float* __restrict__ largest, long long rows) {
   largest[0] = m;
 }
 
-// The power of two by which dz is stored larger, for fp16: such that the largest
-// |coef| lies in [2^14, 2^15) (|dz| stays below 2^16, and probabilities below
-// 2^-24 of it keep their bits); 1 where that is 0 or not finite.
-__device__ __forceinline__ float lift_of(float largest) {
+// The power of two by which dz is stored larger, such that the largest |coef| lies
+// in [2^(to-1), 2^to); 1 where that is 0 or not finite. fp16: to 2^15, |dz| stays
+// below 2^16, and probabilities below 2^-24 of it keep their bits. fp32: to 2^32,
+// which takes the smallest probabilities (2^-126) to 2^-95, below which the fp32
+// product goes by fp32 MFMAs at half its rate (gemm3; 1024 x 4096 x 131072 of
+// logits of std 64 without it: 41.2 ms for loss and gradients, 22.5 with std 1).
+// bf16 products have no such bounds.
+__device__ __forceinline__ float lift_of(float largest, int to) {
   if (!(largest > 0.f && largest < INFINITY)) return 1.f;
   int e = 0;
   (void)frexpf(largest, &e);   // largest in [2^(e-1), 2^e)
-  return ldexpf(1.f, min(max(15 - e, -126), 126));
+  return ldexpf(1.f, min(max(to - e, -126), 126));
 }
 
 constexpr int kCopyRows = 8;   // rows per block
 
-// scale[0..1] = (s, 1 / s), dz's power of two (lift: fp16; scale[2] the largest
-// per-row gradient), else 1; rows2[r] = (coef s, lse2); and, `out` given, out (out_rows, per) = in
+// scale[0..1] = (s, 1 / s), dz's power of two (lift_of to `lift`, scale[2] the largest
+// per-row gradient; lift 0: 1); rows2[r] = (coef s, lse2); and, `out` given, out (out_rows, per) = in
 // (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
 // `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
 // reach dW.
@@ -586,7 +624,7 @@ head_rows_in_kernel(const uint4* __restrict__ in, long long ldi, RowScale rs,
   const long long r0 = (long long)blockIdx.x * kCopyRows;
   if (threadIdx.x < kCopyRows) {
     // (without per-row gradients the largest is the one that every kept row has)
-    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : fabsf(rs.reaching(0)));
+    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : fabsf(rs.reaching(0)), lift);
     const long long r = r0 + threadIdx.x;
     const float c = r < rows ? rs.at(r) : 0.f;
     cf[threadIdx.x] = c;
@@ -729,6 +767,43 @@ head_dz3_kernel(GemmArgs g, HeadGrad a) {
         if (m < g.M && r < a.ldz) dz[m * a.ldz + r] = cf == 0.f || r >= g.N ? 0.f : p;
       }
   }
+}
+
+// p's part of dz of a piece from the logits that the forward kept: bound by
+// reading them and writing dz. 8 words of a row to a thread, or, fp32, 4 rows of a
+// word, as they lie. `blocks` of 16 bytes to a row of dz, n in all.
+template <class T>
+__global__ void __launch_bounds__(256)
+head_dz_kept_kernel(KeptLogits kept, HeadGrad a, int rows, int words, unsigned blocks,
+                    long long n) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= n) return;
+  const long long row = n < 0xFFFFFFFF ? (unsigned)id / blocks : id / blocks;
+  const int at = kVec<T> * (int)(id - row * blocks);
+  Vec<T> out;
+  if constexpr (__is_same(T, Fp32)) {
+    const float4 z = *reinterpret_cast<const float4*>(kept.z + (a.v0 + row) * kept.ld + at);
+    const float v[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 row2 = a.rows2[min(at + e, rows - 1)];
+      const float p = exp2_hw(__builtin_fmaf(v[e], a.c, -row2.y)) * row2.x;
+      out.v[e] = row2.x == 0.f || at + e >= rows ? 0.f : p;
+    }
+  } else {
+    const float2 row2 = a.rows2[row];
+    const float* const z = kept.z + row * kept.ld + a.v0 + at;
+    const float4 lo = *reinterpret_cast<const float4*>(z);
+    float4 hi = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at + 4 < words) hi = *reinterpret_cast<const float4*>(z + 4);
+    const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = exp2_hw(__builtin_fmaf(v[e], a.c, -row2.y)) * row2.x;
+      out.v[e] = T::from(row2.x == 0.f || at + e >= words ? 0.f : p);
+    }
+  }
+  *reinterpret_cast<Vec<T>*>(static_cast<elem_t<T>*>(a.dz) + row * a.ldz + at) = out;
 }
 
 // dz at the rows' ids within a piece of `words` words, over what head_dz wrote:

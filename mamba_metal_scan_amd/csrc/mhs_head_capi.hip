@@ -118,10 +118,14 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 
 bool few_rows(const Head& p) { return p.rows <= small_rows(elem_bytes(p.dtype)); }
 
+// Tile of the forward's fp32 product. (us with 64 and 128, 64 rows: 640 x 32768 40
+// and 48, 4096 x 131072 689 and 748; 96 rows: 54 and 48, 1050 and 797.)
+int gemm3_tile(int64_t rows) { return rows <= 64 ? mhs::kGemmSmallTile : mhs::kGemmTile; }
+
 // Tiles of the vocabulary in the forward's partials.
 int64_t lse_tiles(const Head& p) {
   if (few_rows(p)) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
-  const int bm = p.dtype == MHS_F32 ? mhs::kGemmTile : Shape::BM;
+  const int bm = p.dtype == MHS_F32 ? gemm3_tile(p.rows) : Shape::BM;
   return (p.vocab + bm - 1) / bm;
 }
 
@@ -170,7 +174,7 @@ unsigned stream_blocks(const mhs::MmArgs& g) {
 }
 
 // The logits' product for fp32: W (v0 .. v0 + words) h^T.
-mhs::GemmArgs gemm3_args(const Head& p, int64_t v0, int64_t words) {
+mhs::GemmArgs gemm3_args(const Head& p, int64_t v0, int64_t words, int tile) {
   mhs::GemmArgs g{};
   g.A = static_cast<const float*>(p.weight) + v0 * p.ldw;
   g.B = static_cast<const float*>(p.hidden);
@@ -179,42 +183,54 @@ mhs::GemmArgs gemm3_args(const Head& p, int64_t v0, int64_t words) {
   g.M = (int)words;
   g.N = (int)p.rows;
   g.K = (int)p.dim;
-  g.grid_m = (int)((words + mhs::kGemmTile - 1) / mhs::kGemmTile);
-  g.grid_n = (int)((p.rows + mhs::kGemmTile - 1) / mhs::kGemmTile);
+  g.grid_m = (int)((words + tile - 1) / tile);
+  g.grid_n = (int)((p.rows + tile - 1) / tile);
   return g;
 }
 
+// The kept logits' rows: of words of 16-bit operands, of rows of fp32 ones.
+mhs::KeptLogits kept_logits(const Head& p, float* z) {
+  return {z, (long long)round_up(p.dtype == MHS_F32 ? p.rows : p.vocab, 4)};
+}
+
 template <class T>
-int launch_lse16(const Head& p, float c, float2* part, hipStream_t s) {
+int launch_lse16(const Head& p, float c, float2* part, const mhs::KeptLogits& kept,
+                 hipStream_t s) {
   const mhs::MmArgs g = mm_args<Shape>(p.weight, p.ldw, p.hidden, p.ldh, p.vocab, p.rows, p.dim);
-  const auto fn = &mhs::head_lse_kernel<T, Shape>;
+  const auto fn = kept.z ? &mhs::head_lse_kernel<T, Shape, true>
+                         : &mhs::head_lse_kernel<T, Shape, false>;
   constexpr int lds = Shape::kLds + 2 * Shape::WM * Shape::BN * 4;
   allow_lds(fn, lds);
-  hipLaunchKernelGGL(fn, dim3(stream_blocks(g)), dim3(Shape::kThreads), lds, s, g, c, part);
+  hipLaunchKernelGGL(fn, dim3(stream_blocks(g)), dim3(Shape::kThreads), lds, s, g, c, part,
+                     kept);
   return check_launch("head log-sum-exp kernel");
 }
 
 template <class T>
-int launch_small(const Head& p, float c, float2* part, hipStream_t s) {
+int launch_small(const Head& p, float c, float2* part, const mhs::KeptLogits& kept,
+                 hipStream_t s) {
   const mhs::SmallArgs g{p.hidden, p.weight, p.ldh, p.ldw, (int)p.rows, (int)p.vocab, (int)p.dim};
   auto fn = &mhs::head_small_kernel<T, 1>;
   if constexpr (small_rows(sizeof(mhs::elem_t<T>)) > 16)
     if (p.rows > 16) fn = &mhs::head_small_kernel<T, 2>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)lse_tiles(p)), dim3(256), 0, s, g, c, part);
+  hipLaunchKernelGGL(fn, dim3((unsigned)lse_tiles(p)), dim3(256), 0, s, g, c, part, kept);
   return check_launch("head log-sum-exp kernel of few rows");
 }
 
-int launch_lse(const Head& p, float c, float2* part, hipStream_t s) {
+int launch_lse(const Head& p, float c, float2* part, const mhs::KeptLogits& kept,
+               hipStream_t s) {
   if (few_rows(p))
-    return p.dtype == MHS_F32    ? launch_small<Fp32>(p, c, part, s)
-           : p.dtype == MHS_BF16 ? launch_small<Bf16>(p, c, part, s)
-                                 : launch_small<Fp16>(p, c, part, s);
-  if (p.dtype == MHS_BF16) return launch_lse16<Bf16>(p, c, part, s);
-  if (p.dtype == MHS_F16) return launch_lse16<Fp16>(p, c, part, s);
-  const mhs::GemmArgs g = gemm3_args(p, 0, p.vocab);
-  hipLaunchKernelGGL(mhs::head_lse3_kernel<mhs::kGemmTile>,
+    return p.dtype == MHS_F32    ? launch_small<Fp32>(p, c, part, kept, s)
+           : p.dtype == MHS_BF16 ? launch_small<Bf16>(p, c, part, kept, s)
+                                 : launch_small<Fp16>(p, c, part, kept, s);
+  if (p.dtype == MHS_BF16) return launch_lse16<Bf16>(p, c, part, kept, s);
+  if (p.dtype == MHS_F16) return launch_lse16<Fp16>(p, c, part, kept, s);
+  const int tile = gemm3_tile(p.rows);
+  const mhs::GemmArgs g = gemm3_args(p, 0, p.vocab, tile);
+  hipLaunchKernelGGL((tile == mhs::kGemmTile ? &mhs::head_lse3_kernel<mhs::kGemmTile>
+                                             : &mhs::head_lse3_kernel<mhs::kGemmSmallTile>),
                      dim3((unsigned)g.grid_m * (unsigned)g.grid_n), dim3(mhs::kGemmThreads),
-                     mhs::gemm_lds_bytes(mhs::kGemmTile, mhs::kGemmTile), s, g, c, part);
+                     mhs::gemm_lds_bytes(tile, tile), s, g, c, part, kept);
   return check_launch("head log-sum-exp kernel");
 }
 
@@ -253,18 +269,19 @@ int launch_rows(const mhs::HeadRows& g, hipStream_t s) {
 }
 
 // The forward from the hidden states: g's ids, teacher and outputs are set.
-int head_fwd(const Head& p, mhs::HeadRows g, float* loss, float* count, int reduction,
-             void* workspace, size_t workspace_bytes, void* stream) {
+int head_fwd(const Head& p, mhs::HeadRows g, float* logits, float* loss, float* count,
+             int reduction, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_workspace(workspace, workspace_bytes, fwd_ws(p));
   if (rc) return rc;
   if (reduction != MHS_REDUCE_NONE && (!loss || !count))
     return fail(MHS_EINVAL, "null pointer argument");
+  if (!aligned16(logits)) return fail(MHS_EINVAL, "logits must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   float2* part = static_cast<float2*>(workspace);
   if (p.rows > 0) {
     if (!g.ids || !g.lse2 || !g.picked || !g.loss || !g.keep)
       return fail(MHS_EINVAL, "null pointer argument");
-    rc = launch_lse(p, mhs::kLog2e / g.temperature, part, s);
+    rc = launch_lse(p, mhs::kLog2e / g.temperature, part, kept_logits(p, logits), s);
     if (rc) return rc;
     g.h = p.hidden;
     g.w = p.weight;
@@ -362,9 +379,22 @@ int launch_ids(const Head& p, const mhs::HeadGrad& a, int64_t words, hipStream_t
   return check_launch("gradient of the ids kernel");
 }
 
+// p's part of dz of a piece from the kept logits.
 template <class T>
-int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, char* ws,
-          hipStream_t s) {
+int launch_dz_kept(const Head& p, const mhs::KeptLogits& kept, const mhs::HeadGrad& a,
+                   int64_t words, hipStream_t s) {
+  const bool f32 = p.dtype == MHS_F32;
+  const int64_t v = 16 / elem_bytes(p.dtype);
+  const int64_t blocks = ((f32 ? p.rows : words) + v - 1) / v;
+  const int64_t n = blocks * (f32 ? words : p.rows);
+  hipLaunchKernelGGL(mhs::head_dz_kept_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
+                     s, kept, a, (int)p.rows, (int)words, (unsigned)blocks, (long long)n);
+  return check_launch("gradient of kept logits kernel");
+}
+
+template <class T>
+int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogits& kept,
+          const BwdOut& out, char* ws, hipStream_t s) {
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
   const auto fh = &mhs::head_mm_kernel<T, HalfShape, true, false>;
   const auto fw = &mhs::head_mm_kernel<T, HalfShape, false, false>;
@@ -381,9 +411,13 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
     const int64_t words = std::min(b.piece, p.vocab - v0);
     mhs::MmArgs g = mm_args<Shape>(w + v0 * p.ldw, p.ldw, p.hidden, p.ldh, words, p.rows, p.dim);
     a.v0 = (int)v0;
-    hipLaunchKernelGGL(fz, dim3(stream_blocks(g)), dim3(Shape::kThreads),
-                       lds_z, s, g, a);
-    if ((rc = check_launch("head gradient kernel")) != 0) return rc;
+    if (kept.z) {
+      rc = launch_dz_kept<T>(p, kept, a, words, s);
+    } else {
+      hipLaunchKernelGGL(fz, dim3(stream_blocks(g)), dim3(Shape::kThreads), lds_z, s, g, a);
+      rc = check_launch("head gradient kernel");
+    }
+    if (rc) return rc;
     if ((rc = launch_ids<T>(p, a, words, s)) != 0) return rc;
     mhs::MmOut o{};
     o.scale = a.scale;
@@ -418,8 +452,8 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
   return MHS_OK;
 }
 
-int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, char* ws,
-          hipStream_t s) {
+int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogits& kept,
+          const BwdOut& out, char* ws, hipStream_t s) {
   const float* w = static_cast<const float*>(p.weight);
   const float* hz = reinterpret_cast<const float*>(ws + b.hidden);
   float* dz = static_cast<float*>(a.dz);
@@ -428,26 +462,34 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const BwdOut& out, c
   int rc;
   for (int64_t v0 = 0; v0 < p.vocab; v0 += b.piece) {
     const int64_t words = std::min(b.piece, p.vocab - v0);
-    const mhs::GemmArgs g = gemm3_args(p, v0, words);
+    const mhs::GemmArgs g = gemm3_args(p, v0, words, mhs::kGemmTile);
     a.v0 = (int)v0;
-    hipLaunchKernelGGL(mhs::head_dz3_kernel<mhs::kGemmTile>,
-                       dim3((unsigned)g.grid_m * (unsigned)g.grid_n), dim3(mhs::kGemmThreads),
-                       mhs::gemm_lds_bytes(mhs::kGemmTile, mhs::kGemmTile), s, g, a);
-    if ((rc = check_launch("head gradient kernel")) != 0) return rc;
+    if (kept.z) {
+      rc = launch_dz_kept<Fp32>(p, kept, a, words, s);
+    } else {
+      hipLaunchKernelGGL(mhs::head_dz3_kernel<mhs::kGemmTile>,
+                         dim3((unsigned)g.grid_m * (unsigned)g.grid_n), dim3(mhs::kGemmThreads),
+                         mhs::gemm_lds_bytes(mhs::kGemmTile, mhs::kGemmTile), s, g, a);
+      rc = check_launch("head gradient kernel");
+    }
+    if (rc) return rc;
     if ((rc = launch_ids<Fp32>(p, a, words, s)) != 0) return rc;
     if (out.dhidden &&
-        (rc = mhs_gemm_f32(MHS_GEMM_TN, dz, b.ldz, w + v0 * p.ldw, p.ldw,
-                           static_cast<float*>(out.dhidden), p.dim, p.rows, p.dim, words, v0 > 0,
-                           part, part_bytes, s)) != 0)
+        (rc = mhs::gemm_f32(MHS_GEMM_TN, dz, b.ldz, w + v0 * p.ldw, p.ldw,
+                            static_cast<float*>(out.dhidden), p.dim, p.rows, p.dim, words, v0 > 0,
+                            a.scale + 1, part, part_bytes, s)) != 0)
       return rc;
     if (out.dweight &&
-        (rc = mhs_gemm_f32(MHS_GEMM_NN, dz, b.ldz, hz, p.dim,
-                           static_cast<float*>(out.dweight) + v0 * p.dim, p.dim, words, p.dim,
-                           b.rows4, 0, part, part_bytes, s)) != 0)
+        (rc = mhs::gemm_f32(MHS_GEMM_NN, dz, b.ldz, hz, p.dim,
+                            static_cast<float*>(out.dweight) + v0 * p.dim, p.dim, words, p.dim,
+                            b.rows4, 0, a.scale + 1, part, part_bytes, s)) != 0)
       return rc;
   }
   return MHS_OK;
 }
+
+// See lift_of.
+int lift(int dtype) { return dtype == MHS_F16 ? 15 : dtype == MHS_F32 ? 32 : 0; }
 
 // The rows' coefficients, the scale and (hidden given) the copy of the rows.
 int launch_rows_in(const Head& p, const BwdPlan& b, const mhs::RowScale& rs, const float* lse2,
@@ -459,7 +501,7 @@ int launch_rows_in(const Head& p, const BwdPlan& b, const mhs::RowScale& rs, con
   hipLaunchKernelGGL(mhs::head_rows_in_kernel<>, dim3((unsigned)blocks), dim3(256), 0, s,
                      static_cast<const uint4*>(p.hidden), (long long)(p.ldh * es / 16), rs, lse2,
                      rows2, scale, static_cast<uint4*>(hidden), (long long)p.rows,
-                     (long long)b.rows4, (int)(p.dim * es / 16), p.dtype == MHS_F16 ? 1 : 0);
+                     (long long)b.rows4, (int)(p.dim * es / 16), lift(p.dtype));
   return check_launch("rows kernel");
 }
 
@@ -472,22 +514,24 @@ int launch_zero(void* p, int64_t n, int es, hipStream_t s) {
 }
 
 int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const float* lse2,
-             const BwdOut& out, void* workspace, size_t workspace_bytes, void* stream) {
+             const float* logits, const BwdOut& out, void* workspace, size_t workspace_bytes, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int es = elem_bytes(p.dtype);
   if (out.dhidden == nullptr && out.dweight == nullptr) return MHS_OK;
   if (p.rows == 0) return out.dweight ? launch_zero(out.dweight, p.vocab * p.dim, es, s) : MHS_OK;
   if (!a.ids || !lse2 || !a.picked || !rs.keep || !rs.upstream)
     return fail(MHS_EINVAL, "null pointer argument");
-  if (!aligned16(out.dhidden) || !aligned16(out.dweight))
-    return fail(MHS_EINVAL, "dhidden and dweight must be 16-byte aligned");
+  if (!aligned16(out.dhidden) || !aligned16(out.dweight) || !aligned16(logits))
+    return fail(MHS_EINVAL, "dhidden, dweight and logits must be 16-byte aligned");
+  if (p.dtype == MHS_F32 && p.rows >= (1LL << 22))   // (dz's row stride)
+    return fail(MHS_EINVAL, "the fp32 backward takes rows below 2^22; got %lld", (long long)p.rows);
   int rc = check_workspace(workspace, workspace_bytes, bwd_ws(p));
   if (rc) return rc;
   const BwdPlan b = bwd_plan(p);
   char* ws = static_cast<char*>(workspace);
   float* scale = reinterpret_cast<float*>(ws);
   float2* rows2 = reinterpret_cast<float2*>(ws + b.rows2);
-  if (p.dtype == MHS_F16 && rs.per_row) {
+  if (lift(p.dtype) && rs.per_row) {
     hipLaunchKernelGGL(mhs::head_largest_kernel<>, dim3(1), dim3(1024), 0, s, rs, scale + 2,
                        (long long)p.rows);
     if ((rc = check_launch("largest gradient kernel")) != 0) return rc;
@@ -498,9 +542,10 @@ int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const float* lse2
   a.scale = scale;
   a.dz = ws + b.dz;
   a.ldz = b.ldz;
-  return p.dtype == MHS_F32    ? bwd32(p, b, a, out, ws, s)
-         : p.dtype == MHS_BF16 ? bwd16<Bf16>(p, b, a, out, ws, s)
-                               : bwd16<Fp16>(p, b, a, out, ws, s);
+  const mhs::KeptLogits kept = kept_logits(p, const_cast<float*>(logits));   // (only read)
+  return p.dtype == MHS_F32    ? bwd32(p, b, a, kept, out, ws, s)
+         : p.dtype == MHS_BF16 ? bwd16<Bf16>(p, b, a, kept, out, ws, s)
+                               : bwd16<Fp16>(p, b, a, kept, out, ws, s);
 }
 
 mhs::RowScale row_scale(const float* upstream, const float* count, const float* keep, int reduction,
@@ -566,7 +611,7 @@ size_t mhs_linear_xent_fwd_workspace_bytes(int dtype, int64_t rows, int64_t voca
 
 int mhs_linear_xent_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                         const int64_t* targets, float* lse2, float* picked, float* keep,
-                        float* loss_rows, float* loss, float* count, int64_t rows, int64_t vocab,
+                        float* logits, float* loss_rows, float* loss, float* count, int64_t rows, int64_t vocab,
                         int64_t dim, int64_t ignore_index, int reduction, void* workspace,
                         size_t workspace_bytes, void* stream) {
   mhs::clear_error();
@@ -582,7 +627,7 @@ int mhs_linear_xent_fwd(int dtype, const void* hidden, int64_t ldh, const void* 
   g.k = 1;
   g.ignore = ignore_index;
   g.temperature = 1.f;
-  return head_fwd(p, g, loss, count, reduction, workspace, workspace_bytes, stream);
+  return head_fwd(p, g, logits, loss, count, reduction, workspace, workspace_bytes, stream);
 }
 
 size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t dim) {
@@ -593,8 +638,8 @@ size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t voca
 
 int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                         const int64_t* targets, const float* lse2, const float* picked,
-                        const float* keep, const float* upstream, const float* count,
-                        void* dhidden, void* dweight, int64_t rows, int64_t vocab, int64_t dim,
+                        const float* keep, const float* logits, const float* upstream,
+                        const float* count, void* dhidden, void* dweight, int64_t rows, int64_t vocab, int64_t dim,
                         int reduction, void* workspace, size_t workspace_bytes, void* stream) {
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
@@ -607,14 +652,14 @@ int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* 
   a.picked = picked;
   a.k = 1;
   a.c = mhs::kLog2e;
-  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, 1.f), lse2,
+  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, 1.f), lse2, logits,
                   BwdOut{dhidden, dweight}, workspace, workspace_bytes, stream);
 }
 
 int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                            int64_t ldw, const float* teacher, const int64_t* ids, float* lse2,
-                           float* picked, float* q, float* keep, float* loss_rows, float* loss,
-                           float* count, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
+                           float* picked, float* q, float* keep, float* logits, float* loss_rows,
+                           float* loss, float* count, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
                            float temperature, int reduction, void* workspace,
                            size_t workspace_bytes, void* stream) {
   mhs::clear_error();
@@ -632,13 +677,13 @@ int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const voi
   g.keep = keep;
   g.k = (int)top;
   g.temperature = temperature;
-  return head_fwd(p, g, loss, count, reduction, workspace, workspace_bytes, stream);
+  return head_fwd(p, g, logits, loss, count, reduction, workspace, workspace_bytes, stream);
 }
 
 int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                            int64_t ldw, const int64_t* ids, const float* lse2, const float* picked,
-                           const float* q, const float* keep, const float* upstream,
-                           const float* count, void* dhidden, void* dweight, int64_t rows,
+                           const float* q, const float* keep, const float* logits,
+                           const float* upstream, const float* count, void* dhidden, void* dweight, int64_t rows,
                            int64_t vocab, int64_t dim, int64_t top, float temperature,
                            int reduction, void* workspace, size_t workspace_bytes, void* stream) {
   mhs::clear_error();
@@ -653,7 +698,7 @@ int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const voi
   a.picked = picked;
   a.k = (int)top;
   a.c = mhs::kLog2e / temperature;
-  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, temperature), lse2,
+  return head_bwd(p, a, row_scale(upstream, count, keep, reduction, temperature), lse2, logits,
                   BwdOut{dhidden, dweight}, workspace, workspace_bytes, stream);
 }
 

@@ -13,6 +13,10 @@ void clear_error();
 int check_launch(const char* what);
 // Compute units of the current device.
 int device_cus();
+// mhs_gemm_f32 of alpha[0] (a device scalar; null: 1) times the product.
+int gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t ldb, float* c,
+             int64_t ldc, int64_t m, int64_t n, int64_t k, int accumulate, const float* alpha,
+             void* workspace, size_t workspace_bytes, void* stream);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }

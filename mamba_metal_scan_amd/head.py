@@ -5,10 +5,11 @@ The reference forms the head's logits and takes their cross entropy
 words) 1.07 GB of fp32 logits and as much again for their gradient.
 ``linear_cross_entropy`` computes the same loss and both gradients from the
 hidden states and the head's weight, the logits formed tile by tile on the
-matrix cores and never kept: the forward reduces each tile to its rows' maxima
-and sums of exponentials, the backward forms the tiles again, a piece of the
-vocabulary at a time, and multiplies their gradient with the weight and the
-hidden states.
+matrix cores: the forward reduces each tile to its rows' maxima and sums of
+exponentials, the backward forms the tiles again, a piece of the vocabulary at a
+time, and multiplies their gradient with the weight and the hidden states. Up to
+1 GB of fp32 logits the forward keeps for the backward instead, where that is the
+faster (``_native.keeps_logits``); without a backward it keeps none.
 
 ``distill_loss`` is the distillation of given logits from a teacher's top words,
 ``linear_distill_loss`` the same from the hidden states.
@@ -36,6 +37,10 @@ def _cut(g: torch.Tensor, dim: int) -> torch.Tensor:
     return g if g.shape[1] == dim else g[:, :dim].contiguous()
 
 
+def _keeps(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
+    return _native.keeps_logits(hidden.shape[0], weight.shape[0], hidden.shape[1], hidden.dtype)
+
+
 def _once() -> None:
     """The gradients have none of their own: refuses a backward that is to be
     differentiated (create_graph) rather than leave their part out."""
@@ -54,21 +59,22 @@ class LinearCrossEntropyHIP(torch.autograd.Function):
     int64; rows with target == ignore_index excluded."""
 
     @staticmethod
-    def loss(hidden, weight, targets, ignore_index, reduction):
+    def loss(hidden, weight, targets, ignore_index, reduction, backward=False):
         """(loss, what the backward needs)."""
         hidden, weight = _rows16(hidden), _rows16(weight)
         targets = targets.contiguous()
         if not torch.compiler.is_compiling():   # (the registered op checks itself)
             _native._check_linear_xent("linear_cross_entropy", hidden, weight, targets, reduction)
-        loss, saved = dispatch("linear_xent_fwd")(hidden, weight, targets, ignore_index,
-                                                  reduction)
+        loss, saved = dispatch("linear_xent_fwd")(hidden, weight, targets, ignore_index, reduction,
+                                                  backward and _keeps(hidden, weight))
         return loss, (hidden, weight, targets, saved)
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction):
         ctx.dim = hidden.shape[1]
         ctx.reduction = reduction
-        loss, saved = LinearCrossEntropyHIP.loss(hidden, weight, targets, ignore_index, reduction)
+        loss, saved = LinearCrossEntropyHIP.loss(hidden, weight, targets, ignore_index, reduction,
+                                                 any(ctx.needs_input_grad))
         ctx.save_for_backward(*saved)
         return loss
 
@@ -86,14 +92,15 @@ class LinearDistillHIP(torch.autograd.Function):
     ids (R, K) and their logits."""
 
     @staticmethod
-    def loss(hidden, weight, teacher_logits, ids, temperature, reduction):
+    def loss(hidden, weight, teacher_logits, ids, temperature, reduction, backward=False):
         """(loss, what the backward needs)."""
         hidden, weight = _rows16(hidden), _rows16(weight)
         if not torch.compiler.is_compiling():
             _native._check_linear_distill("linear_distill_loss", hidden, weight, teacher_logits,
                                           ids, temperature, reduction)
         loss, saved = dispatch("linear_distill_fwd")(hidden, weight, teacher_logits, ids,
-                                                     temperature, reduction)
+                                                     temperature, reduction,
+                                                     backward and _keeps(hidden, weight))
         return loss, (hidden, weight, ids, saved)
 
     @staticmethod
@@ -101,7 +108,7 @@ class LinearDistillHIP(torch.autograd.Function):
         ctx.dim = hidden.shape[1]
         ctx.temperature, ctx.reduction = temperature, reduction
         loss, saved = LinearDistillHIP.loss(hidden, weight, teacher_logits, ids, temperature,
-                                            reduction)
+                                            reduction, any(ctx.needs_input_grad))
         ctx.save_for_backward(*saved)
         return loss
 

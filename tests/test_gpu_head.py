@@ -11,7 +11,7 @@ import torch
 import torch.nn.functional as F
 
 from head_reference import assert_head, assert_within
-from mamba_metal_scan_amd import linear_cross_entropy, linear_distill_loss
+from mamba_metal_scan_amd import _native, linear_cross_entropy, linear_distill_loss
 from mamba_metal_scan_amd._native import HipScanError
 
 pytestmark = pytest.mark.gpu
@@ -98,10 +98,62 @@ def test_distillation(rows, dim, vocab, k, temperature, dtype):
                     words=(values, ids, temperature))
 
 
+def _keep(monkeypatch, keep):
+    """The forward keeps its logits, or the backward forms them again."""
+    monkeypatch.setattr(_native, "keeps_logits", lambda *a: keep)
+
+
+@pytest.mark.parametrize("keep", [True, False])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_pieces_of_the_vocabulary(dtype):
+@pytest.mark.parametrize("rows,dim,vocab", [(1, 64, 1), (5, 64, 130), (17, 64, 66), (33, 64, 257),
+                                            (64, 72, 1003), (65, 64, 515), (130, 64, 258),
+                                            (300, 200, 1030)])
+def test_logits_kept_or_formed_again(rows, dim, vocab, dtype, keep, monkeypatch):
+    print(f"[case] keep {keep} {dtype} {rows}x{dim}x{vocab}", flush=True)
+    _keep(monkeypatch, keep)
+    h, w, t = _operands(rows, dim, vocab, TYPES[dtype])
+    up = _upstream(rows, "none")
+    got = _run(linear_cross_entropy, h, w, up, t, reduction="none")
+    assert_head("xent", got, h, w, up, "none", TYPES[dtype], targets=t)
+    values, ids = _words(rows, vocab, 3)
+    up = _upstream(rows, "mean")
+    got = _run(linear_distill_loss, h, w, up, values, ids, temperature=2.0)
+    assert_head("distill", got, h, w, up, "mean", TYPES[dtype], words=(values, ids, 2.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_kept_logits_of_a_backward_twice(dtype, monkeypatch):
+    """The backward leaves what the forward kept as it was."""
+    _keep(monkeypatch, True)
+    h, w, t = _operands(70, 64, 300, TYPES[dtype])
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(a, b, t)
+    first = torch.autograd.grad(loss, [a, b], retain_graph=True)
+    for x, y in zip(first, torch.autograd.grad(loss, [a, b])):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("keep", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_peaked_rows(dtype, keep, monkeypatch):
+    """Upstream gradients far from 1, and rows whose probabilities span all of
+    fp32's exponents."""
+    _keep(monkeypatch, keep)
+    h, w, t = _operands(140, 64, 700, TYPES[dtype], spread=60.0)
+    for factor in (1.0, 2.0 ** -40, 2.0 ** 40):
+        if dtype == "f16" and factor != 1.0:
+            continue   # (the gradients are no fp16 numbers)
+        up = factor * _upstream(140, "none")
+        got = _run(linear_cross_entropy, h, w, up, t, reduction="none")
+        assert_head(f"upstream {factor}", got, h, w, up, "none", TYPES[dtype], targets=t)
+
+
+@pytest.mark.parametrize("keep", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pieces_of_the_vocabulary(dtype, keep, monkeypatch):
     """More than 256 MB of the logits' gradient: the backward in two pieces, the
     second a short one."""
+    _keep(monkeypatch, keep)
     rows, dim, vocab = (2048, 64, 66001) if dtype != "f32" else (2048, 64, 33001)
     print(f"[case] pieces {dtype}", flush=True)
     h, w, t = _operands(rows, dim, vocab, TYPES[dtype])
@@ -426,6 +478,10 @@ def test_op_argument_errors():
         ops.linear_xent_bwd(torch.ones((), device=DEV), h, w, t, saved[:-1], 1, True, True)
     with pytest.raises(HipScanError, match="grad"):
         ops.linear_xent_bwd(torch.ones(8, device=DEV), h, w, t, saved, 1, True, True)
+    loss, saved = ops.linear_xent_fwd(h, w, t, -100, 1, True)
+    off = torch.empty(saved.numel() + 1, device=DEV)[1:]
+    with pytest.raises(HipScanError, match="aligned"):
+        ops.linear_xent_bwd(torch.ones((), device=DEV), h, w, t, off, 1, True, True)
     values, ids = _words(8, 50, 4)
     with pytest.raises(HipScanError, match="int64"):
         ops.linear_distill_fwd(h, w, values, ids.int(), 1.0, 1)

@@ -73,11 +73,11 @@ def _err():
 
 
 def _xent_fwd(dtype=1, hidden=A, ldh=64, weight=A, ldw=64, targets=A, rows=4, vocab=50, dim=64,
-              reduction=1, loss=A, ws=A, nbytes=None):
+              reduction=1, loss=A, logits=None, ws=A, nbytes=None):
     lib = _native.library()
     if nbytes is None:
         nbytes = lib.mhs_linear_xent_fwd_workspace_bytes(1, 4, 50, 64)
-    return lib.mhs_linear_xent_fwd(dtype, hidden, ldh, weight, ldw, targets, A, A, A, A, loss, A,
+    return lib.mhs_linear_xent_fwd(dtype, hidden, ldh, weight, ldw, targets, A, A, A, logits, A, loss, A,
                                    rows, vocab, dim, -100, reduction, ws, nbytes, None)
 
 
@@ -88,7 +88,7 @@ def _xent_fwd(dtype=1, hidden=A, ldh=64, weight=A, ldw=64, targets=A, rows=4, vo
     (dict(ldh=65), "strides"), (dict(ldw=1 << 21), "strides"), (dict(hidden=MIS), "aligned"),
     (dict(weight=None), "null"), (dict(hidden=None), "null"), (dict(targets=None), "null"),
     (dict(loss=None), "null"), (dict(nbytes=16), "too small"), (dict(ws=None), "too small"),
-    (dict(ws=MIS), "256-byte"), (dict(rows=1 << 30, vocab=1 << 30), "too large")])
+    (dict(ws=MIS), "256-byte"), (dict(logits=MIS), "aligned"), (dict(rows=1 << 30, vocab=1 << 30), "too large")])
 def test_cross_entropy_entry_refuses(kw, match):
     assert _xent_fwd(**kw) == EINVAL
     assert match in _err(), _err()
@@ -99,17 +99,18 @@ def test_backward_entries_refuse():
     lib = _native.library()
     nbytes = lib.mhs_linear_xent_bwd_workspace_bytes(1, 4, 50, 64)
 
-    def bwd(upstream=A, count=A, dh=A, nbytes=nbytes, ws=A, reduction=1):
-        return lib.mhs_linear_xent_bwd(1, A, 64, A, 64, A, A, A, A, upstream, count, dh, A, 4, 50,
-                                       64, reduction, ws, nbytes, None)
+    def bwd(upstream=A, count=A, dh=A, nbytes=nbytes, ws=A, reduction=1, logits=None):
+        return lib.mhs_linear_xent_bwd(1, A, 64, A, 64, A, A, A, A, logits, upstream, count,
+                                       dh, A, 4, 50, 64, reduction, ws, nbytes, None)
     for kw, match in ((dict(upstream=None), "null"), (dict(count=None), "null"),
                       (dict(dh=MIS), "aligned"), (dict(nbytes=nbytes - 1), "too small"),
-                      (dict(ws=MIS), "256-byte"), (dict(reduction=-1), "reduction")):
+                      (dict(ws=MIS), "256-byte"), (dict(reduction=-1), "reduction"),
+                      (dict(logits=MIS), "aligned")):
         assert bwd(**kw) == EINVAL and match in _err(), (kw, _err())
 
     def distill(top=4, temperature=1.0, q=A, teacher=A):
-        return lib.mhs_linear_distill_fwd(1, A, 64, A, 64, teacher, A, A, A, q, A, A, A, A, 4, 50,
-                                          64, top, temperature, 1, A, nbytes, None)
+        return lib.mhs_linear_distill_fwd(1, A, 64, A, 64, teacher, A, A, A, q, A, None, A, A, A,
+                                          4, 50, 64, top, temperature, 1, A, nbytes, None)
     for kw, match in ((dict(top=0), "words"), (dict(top=1025), "words"),
                       (dict(temperature=0.0), "temperature"),
                       (dict(temperature=float("nan")), "temperature"),
@@ -159,6 +160,16 @@ def test_workspace_sizes():
     assert fwd(1, 0, 100, 64) > 0 and bwd(1, 0, 100, 64) > 0
 
 
+def test_rule_of_kept_logits():
+    """At most 1 GB of them; of 16-bit operands where that saves time."""
+    keeps = _native.keeps_logits
+    f, b = torch.float32, torch.bfloat16
+    assert keeps(8192, 32768, 640, f) and not keeps(8193, 32768, 640, f)
+    assert keeps(256, 32768, 640, b) and not keeps(257, 32768, 640, b)
+    assert keeps(2048, 131072, 2048, b) and not keeps(2049, 131072, 2048, b)
+    assert keeps(0, 5, 8, f)
+
+
 def test_fake_ops_have_the_kernels_shapes():
     """The shapes that tracing sees."""
     from torch._subclasses.fake_tensor import FakeTensorMode
@@ -172,6 +183,9 @@ def test_fake_ops_have_the_kernels_shapes():
         assert loss.shape == () and saved.dtype == torch.float32
         dh, dw = ops.linear_xent_bwd(loss, h, w, t, saved, 1, True, False)
         assert dh.shape == h.shape and dw.shape == (0,) and dh.dtype == h.dtype
+        assert saved.shape == (4 + 6 * 4,)
+        assert ops.linear_xent_fwd(h, w, t, -100, 1, True)[1].shape == (28 + 6 * 52,)
+        assert ops.linear_xent_fwd(h.float(), w.float(), t, -100, 1, True)[1].shape == (28 + 50 * 8,)
         loss, saved = ops.linear_distill_fwd(h, w, ids.float(), ids, 1.0, 0)
         assert loss.shape == (6,)
         dh, dw = ops.linear_distill_bwd(loss, h, w, ids, saved, 1.0, 0, True, True)
