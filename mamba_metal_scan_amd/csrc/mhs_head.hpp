@@ -830,16 +830,17 @@ head_ids_kernel(HeadGrad a, long long rows, int words) {
 }
 
 // What becomes of a 16-bit product: fp32 sums of split blockIdx.y (overwritten,
-// or added to for later pieces), or the rounded result times scale[1].
+// or added to for later pieces), or the rounded result times scale[1]; transposed,
+// so that a lane's neighbouring rows are neighbours in memory.
 struct MmOut {
-  float* part;          // (splits, M, N), or null
+  float* part;          // (splits, N, M), or null
   int accumulate;
-  unsigned short* out;  // (M, N) rows ldo apart
-  long long ldo;
+  unsigned short* out;  // (N, M) rows ldo apart
+  long long ldo;        // a multiple of 8, as M
   const float* scale;
 };
 
-template <class T, class S, bool AK, bool BK>
+template <class T, class S, bool BK>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_mm_kernel(MmArgs g, MmOut o) {
   extern __shared__ float lds_f[];
@@ -847,30 +848,50 @@ head_mm_kernel(MmArgs g, MmOut o) {
   mm_tile(g, blockIdx.x, tm, tn);
   const int k_first = blockIdx.y * g.kt_per_split * S::BK;
   typename S::acc acc[S::FM][S::FN];
-  mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
-                            min(g.K - k_first, g.kt_per_split * S::BK),
-                            reinterpret_cast<char*>(lds_f));
+  mm_products<T, S, false, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
+                               min(g.K - k_first, g.kt_per_split * S::BK),
+                               reinterpret_cast<char*>(lds_f));
+  static_assert(S::E == 4 && S::FM % 4 == 0, "a lane's 4 rows of 4 fragments");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int mb = tm * S::BM + S::wave_m(wave) * (S::FM * S::MI) + 4 * (lane / S::MI);
-  const int nb = tn * S::BN + S::wave_n(wave) * (S::FN * S::MI) + lane % S::MI;
+  const int mb = tm * S::BM + S::wave_m(wave) * (S::FM * 16);
+  const int nb = tn * S::BN + S::wave_n(wave) * (S::FN * 16) + (lane & 15);
   const float scale = o.part ? 1.f : o.scale[1];
 #pragma unroll
-  for (int i = 0; i < S::FM; ++i)
+  for (int j = 0; j < S::FN; ++j) {
+    const int n = nb + 16 * j;
+    if (o.part) {   // 16 bytes a lane, 64 of 16 rows at a time
+      float* const row = o.part + ((long long)blockIdx.y * g.N + n) * g.M;
 #pragma unroll
-    for (int e = 0; e < S::E; ++e) {
-      const int m = mb + i * S::MI + 8 * (e / 4) + e % 4;
-#pragma unroll
-      for (int j = 0; j < S::FN; ++j) {
-        const int n = nb + j * S::MI;
+      for (int i = 0; i < S::FM; ++i) {
+        const int m = mb + 16 * i + 4 * (lane >> 4);
         if (m >= g.M || n >= g.N) continue;
-        if (o.part) {
-          float* p = o.part + ((long long)blockIdx.y * g.M + m) * g.N + n;
-          *p = o.accumulate ? *p + acc[i][j][e] : acc[i][j][e];
-        } else {
-          o.out[(long long)m * o.ldo + n] = T::from(acc[i][j][e] * scale);
+        f32x4* const p = reinterpret_cast<f32x4*>(row + m);
+        const f32x4 v = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        *p = o.accumulate ? *p + v : v;
+      }
+    } else {        // a lane's 4 rows of 4 fragments become one fragment's 16
+#pragma unroll
+      for (int h = 0; h < S::FM / 4; ++h) {
+        unsigned lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          unsigned short v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = T::from(acc[4 * h + i][j][e] * scale);
+          lo[i] = v[0] | (unsigned)v[1] << 16;
+          hi[i] = v[2] | (unsigned)v[3] << 16;
         }
+        exchange4(lo);
+        exchange4(hi);
+        const int m = mb + 64 * h + 16 * (lane >> 4);
+        unsigned short* const row = o.out + (long long)n * o.ldo + m;
+        if (n < g.N && m < g.M)
+          *reinterpret_cast<uint4*>(row) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+        if (n < g.N && m + 8 < g.M)
+          *reinterpret_cast<uint4*>(row + 8) = make_uint4(lo[2], hi[2], lo[3], hi[3]);
       }
     }
+  }
 }
 
 // out (M, 4 N4) = scale[1] times the sum of the splits' sums, in order, rounded;

@@ -24,8 +24,7 @@ using mhs::Fp16;
 using mhs::Fp32;
 using mhs::round_up;
 
-typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64, false> Shape;
-typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64, true> HalfShape;   // (the gradients')
+typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64> Shape;
 
 // Rows that the kernel for few rows takes, by bytes of an element. us of it and of
 // the tiles, with the loss's kernel: fp32, 32 rows, 640 x 32768 36 and 46, 4096 x
@@ -396,8 +395,8 @@ template <class T>
 int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogits& kept,
           const BwdOut& out, char* ws, hipStream_t s) {
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
-  const auto fh = &mhs::head_mm_kernel<T, HalfShape, true, false>;
-  const auto fw = &mhs::head_mm_kernel<T, HalfShape, false, false>;
+  const auto fh = &mhs::head_mm_kernel<T, Shape, true>;
+  const auto fw = &mhs::head_mm_kernel<T, Shape, false>;
   constexpr int lds_z = Shape::kLds + 2 * 2048;
   allow_lds(fz, lds_z);
   allow_lds(fh, Shape::kLds);
@@ -422,7 +421,7 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogit
     mhs::MmOut o{};
     o.scale = a.scale;
     if (out.dhidden) {
-      g = mm_args<Shape>(a.dz, b.ldz, w + v0 * p.ldw, p.ldw, p.rows, p.dim, words);
+      g = mm_args<Shape>(w + v0 * p.ldw, p.ldw, a.dz, b.ldz, p.dim, p.rows, words);
       g.kt_per_split = b.kt_per_split;
       o.part = part;
       o.accumulate = v0 > 0;
@@ -431,7 +430,7 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogit
       if ((rc = check_launch("hidden gradient kernel")) != 0) return rc;
     }
     if (out.dweight) {
-      g = mm_args<Shape>(a.dz, b.ldz, hz, p.dim, words, p.dim, p.rows);
+      g = mm_args<Shape>(hz, p.dim, a.dz, b.ldz, p.dim, words, p.rows);
       o.part = nullptr;
       o.accumulate = 0;
       o.out = static_cast<u16*>(out.dweight) + v0 * p.dim;
