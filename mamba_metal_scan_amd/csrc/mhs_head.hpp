@@ -334,13 +334,13 @@ head_small_kernel(SmallArgs g, float c, float2* __restrict__ part, KeptLogits ke
 
 // The dot products of row a with U rows b[u] of dim elements (16-byte aligned,
 // whole accesses) over the wave's lanes, their loads in flight together; every
-// lane returns them.
-template <class T, int U>
+// lane returns them. Of W waves, each a part of every row.
+template <class T, int U, int W = 1>
 __device__ __forceinline__ void wave_dots(const elem_t<T>* a, const elem_t<T>* const (&b)[U],
                                           int dim, float (&s)[U]) {
 #pragma unroll
   for (int u = 0; u < U; ++u) s[u] = 0.f;
-  for (int i = (threadIdx.x & 63) * kVec<T>; i < dim; i += 64 * kVec<T>) {
+  for (int i = (threadIdx.x & (64 * W - 1)) * kVec<T>; i < dim; i += 64 * W * kVec<T>) {
     const Vec<T> x = *reinterpret_cast<const Vec<T>*>(a + i);
     Vec<T> y[U];
 #pragma unroll
@@ -374,27 +374,37 @@ struct HeadRows {
   float temperature;
 };
 
-// Cross entropy: a wave per row.
-template <class T>
+// Cross entropy: W waves (1 or 4) per row.
+template <class T, int W>
 __global__ void __launch_bounds__(256)
 head_xent_rows_kernel(HeadRows g) {
-  const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= g.rows) return;   // (whole waves; no barrier below)
+  __shared__ float red[W];
+  const int lane = threadIdx.x & (64 * W - 1);
+  const int r = blockIdx.x * (4 / W) + threadIdx.x / (64 * W);
+  if (r >= g.rows) return;   // (whole waves; with four, no block is past the rows)
   float m = -INFINITY, s = 0.f;
-  for (int t = lane; t < g.tiles; t += 64) {
+  for (int t = lane; t < g.tiles; t += 64 * W) {
     const float2 p = g.part[(long long)t * g.rows + r];
     lse2_combine(m, s, p.x, p.y);
   }
+  if constexpr (W == 4) {
+    block_lse2(m, s);
+  } else {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1)
-    lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    for (int o = 32; o >= 1; o >>= 1)
+      lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+  }
   const float lse2 = m + log2f(s);
   const long long t = g.ids[r];
   const bool in = t >= 0 && t < g.vocab;
   const elem_t<T>* const word[1] = {static_cast<const elem_t<T>*>(g.w) + (in ? t : 0) * g.ldw};
   float dot[1];
-  wave_dots<T, 1>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh, word, g.dim, dot);
+  wave_dots<T, 1, W>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh, word, g.dim, dot);
+  if constexpr (W == 4) {
+    if ((lane & 63) == 0) red[lane >> 6] = dot[0];
+    __syncthreads();
+    dot[0] = red[0] + red[1] + red[2] + red[3];
+  }
   const float z = in ? dot[0] : 0.f;
   if (lane == 0) {
     const bool keep = t != g.ignore;

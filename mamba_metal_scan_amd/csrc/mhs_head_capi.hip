@@ -256,14 +256,23 @@ int launch_loss(const float* rows_loss, const float* keep, float* loss, float* c
   return check_launch("loss kernel");
 }
 
+// Rows up to which each takes a block of the rows' kernel, then a wave. (us of the
+// forward with a block and with a wave, 640 x 32768 bf16: 16 rows 16.5 and 18.9,
+// 512 28.3 and 28.4, 1024 48.1 and 46.8, 8192 320 and 312; 4 rows of 4096 x 131072
+// 213 and 227.)
+constexpr int64_t kBlockRows = 512;
+
 template <class T>
 int launch_rows(const mhs::HeadRows& g, hipStream_t s) {
   if (g.teacher)
     hipLaunchKernelGGL(mhs::head_distill_rows_kernel<T>, dim3((unsigned)g.rows), dim3(256),
                        2 * g.k * sizeof(float), s, g);
+  else if (g.rows <= kBlockRows)
+    hipLaunchKernelGGL((mhs::head_xent_rows_kernel<T, 4>), dim3((unsigned)g.rows), dim3(256), 0, s,
+                       g);
   else
-    hipLaunchKernelGGL(mhs::head_xent_rows_kernel<T>, dim3((unsigned)((g.rows + 3) / 4)), dim3(256),
-                       0, s, g);
+    hipLaunchKernelGGL((mhs::head_xent_rows_kernel<T, 1>), dim3((unsigned)((g.rows + 3) / 4)),
+                       dim3(256), 0, s, g);
   return check_launch("head rows kernel");
 }
 

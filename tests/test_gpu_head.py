@@ -176,6 +176,15 @@ def test_one_gradient_only(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [512, 513])
+def test_rows_on_both_sides_of_a_block_each(rows, dtype):
+    h, w, t = _operands(rows, 264, 20000, TYPES[dtype])
+    up = _upstream(rows, "none")
+    got = _run(linear_cross_entropy, h, w, up, t, reduction="none")
+    assert_head("rows", got, h, w, up, "none", TYPES[dtype], targets=t)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [1, 5, 66, 100])
 def test_any_width(dim, dtype):
     """Widths whose rows are no whole 16-byte accesses."""
