@@ -183,6 +183,55 @@ head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part, KeptLogits kept
   store_partials<2>(lds_f, part, n0, g.N, TILE, m0 / TILE);
 }
 
+// The same from logits in memory, for products whose tiles are too few to fill the
+// CUs and which are cut up in k: bound by their latency, a few us. fp32, (words,
+// ld): 64 words by 64 rows a block, a wave 16 words of each.
+constexpr int kLogitWords = 64;
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(256)
+head_lse_of_logits_kernel(KeptLogits logits, int words, int rows, float c,
+                          float2* __restrict__ part) {
+  __shared__ float red[2 * 4 * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n0 = blockIdx.y * 64, v0 = blockIdx.x * kLogitWords + wave * 16;
+  const int left = words - v0, r = min(n0 + lane, rows - 1);
+  float z[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = i < left ? logits.z[(long long)(v0 + i) * logits.ld + r] : 0.f;
+  float m, s;
+  column_lse2<16>([&](int i) { return z[i]; }, [](int i) { return i; }, c, left, m, s);
+  red[2 * wave * 64 + lane] = m;
+  red[(2 * wave + 1) * 64 + lane] = s;
+  __syncthreads();
+  store_partials<4>(red, part, n0, rows, 64, blockIdx.x);
+}
+
+// 16 bits, the sums (splits, rows, ld) of the splits: a wave takes 256 words of a
+// row, sums the splits in order and, kept given, leaves the logits there.
+constexpr int kSplitWords = 256;
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(256)
+head_lse_of_splits_kernel(const float* __restrict__ sums, long long ld, int splits, int words,
+                          int rows, float c, float2* __restrict__ part, KeptLogits kept) {
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;   // (whole waves; no barrier below)
+  const int v = blockIdx.x * kSplitWords + 4 * lane;
+  float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (v < words) {
+    for (int k = 0; k < splits; ++k)
+      z = add(z, *reinterpret_cast<const float4*>(sums + ((long long)k * rows + r) * ld + v));
+    if (kept.z) *reinterpret_cast<float4*>(kept.z + r * kept.ld + v) = z;
+  }
+  const float y[4] = {z.x, z.y, z.z, z.w};
+  float m, s;
+  column_lse2<4>([&](int i) { return y[i]; }, [](int i) { return i; }, c, words - v, m, s);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1)
+    lse2_combine(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+  if (lane == 0) part[(long long)blockIdx.x * rows + r] = make_float2(m, s);
+}
+
 // --------------------------------------------------------------- few rows
 //
 // Up to 16 NF rows: bound by reading W once. A block takes 64 words straight from
@@ -843,14 +892,14 @@ head_ids_kernel(HeadGrad a, long long rows, int words) {
 // or added to for later pieces), or the rounded result times scale[1]; transposed,
 // so that a lane's neighbouring rows are neighbours in memory.
 struct MmOut {
-  float* part;          // (splits, N, M), or null
+  float* part;          // (splits, N, ldo), or null
   int accumulate;
-  unsigned short* out;  // (N, M) rows ldo apart
-  long long ldo;        // a multiple of 8, as M
+  unsigned short* out;  // (N, ldo)
+  long long ldo;        // M to a multiple of 4; of out, of 8, as M is
   const float* scale;
 };
 
-template <class T, class S, bool BK>
+template <class T, class S, bool AK, bool BK>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_mm_kernel(MmArgs g, MmOut o) {
   extern __shared__ float lds_f[];
@@ -858,9 +907,9 @@ head_mm_kernel(MmArgs g, MmOut o) {
   mm_tile(g, blockIdx.x, tm, tn);
   const int k_first = blockIdx.y * g.kt_per_split * S::BK;
   typename S::acc acc[S::FM][S::FN];
-  mm_products<T, S, false, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
-                               min(g.K - k_first, g.kt_per_split * S::BK),
-                               reinterpret_cast<char*>(lds_f));
+  mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
+                            min(g.K - k_first, g.kt_per_split * S::BK),
+                            reinterpret_cast<char*>(lds_f));
   static_assert(S::E == 4 && S::FM % 4 == 0, "a lane's 4 rows of 4 fragments");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int mb = tm * S::BM + S::wave_m(wave) * (S::FM * 16);
@@ -870,7 +919,7 @@ head_mm_kernel(MmArgs g, MmOut o) {
   for (int j = 0; j < S::FN; ++j) {
     const int n = nb + 16 * j;
     if (o.part) {   // 16 bytes a lane, 64 of 16 rows at a time
-      float* const row = o.part + ((long long)blockIdx.y * g.N + n) * g.M;
+      float* const row = o.part + ((long long)blockIdx.y * g.N + n) * o.ldo;
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
         const int m = mb + 16 * i + 4 * (lane >> 4);
@@ -905,7 +954,7 @@ head_mm_kernel(MmArgs g, MmOut o) {
 }
 
 // out (M, 4 N4) = scale[1] times the sum of the splits' sums, in order, rounded;
-// rows whose coef is 0 are zeros.
+// rows2 given, rows whose coef is 0 are zeros.
 template <class T>
 __global__ void __launch_bounds__(256)
 head_mm_reduce_kernel(const float4* __restrict__ part, ushort4* __restrict__ out,
@@ -917,7 +966,7 @@ head_mm_reduce_kernel(const float4* __restrict__ part, ushort4* __restrict__ out
        i += (long long)gridDim.x * 256) {
     float4 s = part[i];
     for (int k = 1; k < splits; ++k) s = add(s, part[k * n + i]);
-    const bool zero = rows2[i / N4].x == 0.f;
+    const bool zero = rows2 && rows2[i / N4].x == 0.f;
     out[i] = zero ? make_ushort4(0, 0, 0, 0)
                   : make_ushort4(T::from(s.x * f), T::from(s.y * f), T::from(s.z * f),
                                  T::from(s.w * f));

@@ -121,9 +121,52 @@ bool few_rows(const Head& p) { return p.rows <= small_rows(elem_bytes(p.dtype));
 // and 48, 4096 x 131072 689 and 748; 96 rows: 54 and 48, 1050 and 797.)
 int gemm3_tile(int64_t rows) { return rows <= 64 ? mhs::kGemmSmallTile : mhs::kGemmTile; }
 
+// Splits of a 16-bit forward's product in k: 1 where the tiles' own kernel takes
+// it whole. A k tile takes 1.07 us of a block (the direct kernel's blocks wait for
+// each: it has one per CU), the sums' kernel 5 us, and a split's sums are written
+// and read at 7.5 TB/s, from the caches. With tiles for more than a quarter of the
+// CUs W's bytes count instead. (us, whole and split: 33 x 1024 x 1360 30 and 17,
+// 64 x 4096 x 16384 81 and 39, 256 x 2048 x 8192 48 and 37; not split, 256 x 512 x
+// 16384 21 and 33, 512 x 1024 x 16384 33 and 45, 512 x 4096 x 24576 93 and 117.)
+struct KSplit {
+  int splits, kt_per_split;
+};
+KSplit lse_splits(const Head& p) {
+  const int64_t tiles = (p.vocab + Shape::BM - 1) / Shape::BM * ((p.rows + Shape::BN - 1) / Shape::BN);
+  const int kt = (int)((p.dim + Shape::BK - 1) / Shape::BK);
+  KSplit best{1, kt};
+  if (4 * tiles > device_cus()) return best;
+  double least = 1.07 * kt;
+  for (int n = 2; n <= std::min<int64_t>(device_cus() / std::max<int64_t>(tiles, 1), kt / 4); ++n) {
+    const int per = (kt + n - 1) / n;
+    const double us = 1.07 * per + 5 + n * (double)p.rows * p.vocab * 8 / 7.5e6;
+    if (us >= least) continue;
+    least = us;
+    best.kt_per_split = per;
+    best.splits = (kt + per - 1) / per;
+  }
+  return best;
+}
+
+// Whether a forward's tiles are so few, and its k's so many, that its product is
+// taken by itself, cut up in k, and the sums of exponentials from the logits in
+// memory. fp32 (us, tiles' own kernel and so): 33 x 640 x 1360, 22 tiles, 26 and 21,
+// 128 x 640 x 8192, 64 tiles, 37 and 36, 256 x 640 x 8192, 128, 39 and 43; with 2896
+// columns 89 and 30, 161 and 67, 160 and 104, and 256 x 16384, 256 tiles, 170 and
+// 178; with 256 columns 15 and 22, 20 and 24, 21 and 29.
+bool few_tiles(const Head& p) {
+  if (few_rows(p) || p.rows == 0) return false;
+  if (p.dtype != MHS_F32) return lse_splits(p).splits > 1;
+  const int t = gemm3_tile(p.rows);
+  const int64_t tiles = ((p.vocab + t - 1) / t) * ((p.rows + t - 1) / t);
+  return p.dim >= 512 && tiles <= std::min<int64_t>(p.dim / 10, device_cus() / 2);
+}
+
 // Tiles of the vocabulary in the forward's partials.
 int64_t lse_tiles(const Head& p) {
-  if (few_rows(p)) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
+  static_assert(mhs::kSmallWords == mhs::kLogitWords, "one size of partials");
+  static_assert(mhs::kSplitWords == Shape::BM, "and of 16 bits");
+  if (few_rows(p) || (p.dtype == MHS_F32 && few_tiles(p))) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
   const int bm = p.dtype == MHS_F32 ? gemm3_tile(p.rows) : Shape::BM;
   return (p.vocab + bm - 1) / bm;
 }
@@ -134,8 +177,22 @@ size_t loss_ws(int64_t rows) {
              : round_up((size_t)((rows + mhs::kLossRows - 1) / mhs::kLossRows) * 16, 256);
 }
 
-size_t fwd_ws(const Head& p) {
+// The forward's workspace: partials, the loss's sums and, of few tiles, the logits
+// and the product's own.
+size_t logits_at(const Head& p) {
   return round_up((size_t)lse_tiles(p) * p.rows * 8, 256) + loss_ws(p.rows);
+}
+
+size_t logits_bytes(const Head& p) {
+  return round_up(p.dtype == MHS_F32 ? (size_t)p.vocab * round_up(p.rows, 4) * 4
+                                     : (size_t)p.rows * round_up(p.vocab, 4) * 4, 256);
+}
+
+size_t fwd_ws(const Head& p) {
+  if (!few_tiles(p)) return logits_at(p);
+  if (p.dtype != MHS_F32) return logits_at(p) + lse_splits(p).splits * logits_bytes(p);
+  return logits_at(p) + logits_bytes(p) +
+         (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(p.vocab, p.rows, p.dim), 0);
 }
 
 template <class F>
@@ -216,8 +273,49 @@ int launch_small(const Head& p, float c, float2* part, const mhs::KeptLogits& ke
   return check_launch("head log-sum-exp kernel of few rows");
 }
 
-int launch_lse(const Head& p, float c, float2* part, const mhs::KeptLogits& kept,
-               hipStream_t s) {
+// Of few tiles: the logits (to kept, or the workspace) and their sums.
+int launch_lse_of_logits(const Head& p, float c, mhs::KeptLogits kept, char* ws, hipStream_t s) {
+  float2* part = reinterpret_cast<float2*>(ws);
+  if (!kept.z) kept.z = reinterpret_cast<float*>(ws + logits_at(p));
+  const size_t at = logits_at(p) + logits_bytes(p);
+  int rc = mhs::gemm_f32(MHS_GEMM_NT, static_cast<const float*>(p.weight), p.ldw,
+                         static_cast<const float*>(p.hidden), p.ldh, kept.z, kept.ld, p.vocab,
+                         p.rows, p.dim, 0, nullptr, ws + at, fwd_ws(p) - at, s);
+  if (rc) return rc;
+  hipLaunchKernelGGL(mhs::head_lse_of_logits_kernel<>,
+                     dim3((unsigned)lse_tiles(p), (unsigned)((p.rows + 63) / 64)), dim3(256), 0, s,
+                     kept, (int)p.vocab, (int)p.rows, c, part);
+  return check_launch("log-sum-exp of logits kernel");
+}
+
+template <class T>
+int launch_lse_of_splits(const Head& p, float c, const mhs::KeptLogits& kept, char* ws,
+                         hipStream_t s) {
+  mhs::MmArgs g = mm_args<Shape>(p.weight, p.ldw, p.hidden, p.ldh, p.vocab, p.rows, p.dim);
+  const KSplit k = lse_splits(p);
+  g.kt_per_split = k.kt_per_split;
+  mhs::MmOut o{};
+  o.part = reinterpret_cast<float*>(ws + logits_at(p));
+  o.ldo = (long long)round_up(p.vocab, 4);
+  const auto fn = &mhs::head_mm_kernel<T, Shape, true, true>;
+  allow_lds(fn, Shape::kLds);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(g.grid_m * g.grid_n), (unsigned)k.splits),
+                     dim3(Shape::kThreads), Shape::kLds, s, g, o);
+  int rc = check_launch("logits kernel");
+  if (rc) return rc;
+  hipLaunchKernelGGL(mhs::head_lse_of_splits_kernel<>,
+                     dim3((unsigned)lse_tiles(p), (unsigned)((p.rows + 3) / 4)), dim3(256), 0, s,
+                     o.part, o.ldo, k.splits, (int)p.vocab, (int)p.rows, c,
+                     reinterpret_cast<float2*>(ws), kept);
+  return check_launch("log-sum-exp of logits kernel");
+}
+
+int launch_lse(const Head& p, float c, char* ws, const mhs::KeptLogits& kept, hipStream_t s) {
+  float2* part = reinterpret_cast<float2*>(ws);
+  if (few_tiles(p))
+    return p.dtype == MHS_F32    ? launch_lse_of_logits(p, c, kept, ws, s)
+           : p.dtype == MHS_BF16 ? launch_lse_of_splits<Bf16>(p, c, kept, ws, s)
+                                 : launch_lse_of_splits<Fp16>(p, c, kept, ws, s);
   if (few_rows(p))
     return p.dtype == MHS_F32    ? launch_small<Fp32>(p, c, part, kept, s)
            : p.dtype == MHS_BF16 ? launch_small<Bf16>(p, c, part, kept, s)
@@ -289,7 +387,8 @@ int head_fwd(const Head& p, mhs::HeadRows g, float* logits, float* loss, float* 
   if (p.rows > 0) {
     if (!g.ids || !g.lse2 || !g.picked || !g.loss || !g.keep)
       return fail(MHS_EINVAL, "null pointer argument");
-    rc = launch_lse(p, mhs::kLog2e / g.temperature, part, kept_logits(p, logits), s);
+    rc = launch_lse(p, mhs::kLog2e / g.temperature, static_cast<char*>(workspace),
+                    kept_logits(p, logits), s);
     if (rc) return rc;
     g.h = p.hidden;
     g.w = p.weight;
@@ -317,14 +416,37 @@ int head_fwd(const Head& p, mhs::HeadRows g, float* logits, float* loss, float* 
 struct BwdPlan {
   int64_t piece, ldz;      // words per piece; dz's row stride
   int64_t rows4;           // fp32: the rows, to a multiple of 4
-  int splits = 1;          // of dh's sums over a piece's words
-  int kt_per_split = 0;
-  size_t rows2, hidden, dz, part, bytes;
+  KSplit dh, dw;           // 16 bits: of dh's sums over a piece's words, dW's over the rows
+  size_t rows2, hidden, dz, part, part_w, bytes;
 };
 
 int64_t piece_words(int64_t rows, int64_t vocab, int es) {
   const int64_t fit = kPieceBytes / (std::max<int64_t>(rows, 1) * es) / 256 * 256;
   return std::min(round_up(vocab, 256), (size_t)std::max<int64_t>(fit, 256));
+}
+
+// Splits of a product (M, N) over K in its k's, such that its tiles fill the CUs:
+// a k tile takes 1.5 us of a CU, a block's start and end about 4 more, and the sums
+// of a split are written and read at about 4 TB/s; whole: 1 if one split's sums go
+// through memory too. (dh, 1001 x 384 x 16384, us: 4 splits 80, 16 35, 32 32; 8192 x
+// 640 x 16384: 2 splits 182, 5 206. dW split and whole, the loss and its gradients:
+// 8192 x 64 x 1009 84 and 172, 8192 x 640 x 8192 400 and 413, 8192 x 64 x 32768 524
+// and 677, 4096 x 640 x 16384 372 and 366; whole by this, 8192 x 1024 x 32768.)
+KSplit bwd_splits(int64_t M, int64_t N, int64_t K, int whole) {
+  const int64_t tiles = (M + Shape::BM - 1) / Shape::BM * ((N + Shape::BN - 1) / Shape::BN);
+  const int64_t kt = (K + Shape::BK - 1) / Shape::BK;
+  const int cus = device_cus();
+  KSplit b{};
+  double best = 0;
+  for (int64_t n = 1; n <= std::min<int64_t>(64, kt); ++n) {
+    const double t = std::ceil((double)tiles * n / cus) * 1.5 * ((double)((kt + n - 1) / n) + 4) +
+                     (n > 1 || whole ? n * (double)M * N * 8 / 4e6 : 0) + (n > 1 && !whole ? 5 : 0);
+    if (n > 1 && t >= best) continue;
+    best = t;
+    b.kt_per_split = (int)((kt + n - 1) / n);
+  }
+  b.splits = (int)((kt + b.kt_per_split - 1) / b.kt_per_split);
+  return b;
 }
 
 BwdPlan bwd_plan(const Head& p) {
@@ -338,7 +460,7 @@ BwdPlan bwd_plan(const Head& p) {
   b.dz = b.hidden + round_up((size_t)b.rows4 * p.dim * es, 256);
   b.part = b.dz + round_up((size_t)(p.dtype == MHS_F32 ? b.piece * b.rows4 : p.rows * b.piece) * es,
                            256);
-  size_t part;
+  size_t part, part_w = 0;
   if (p.dtype == MHS_F32) {
     const int64_t words = std::min(b.piece, p.vocab);
     // (the last piece may be shorter, and its products' splits other ones)
@@ -348,28 +470,14 @@ BwdPlan bwd_plan(const Head& p) {
       part = std::max({part, (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(p.rows, p.dim, w), 0),
                        (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(w, p.dim, b.rows4), 0)});
   } else {
-    // Splits of dh's sums such that the tiles fill the CUs. A k tile takes 1.5 us
-    // of a CU, a block's start and end about 4 more, and the sums of a split are
-    // written and read at about 4 TB/s.
-    // (1001 x 384 x 16384, us: 4 splits 80, 16 35, 32 32; 8192 x 640 x 16384: 2
-    // splits 182, 5 206.)
-    const int64_t tiles = (p.rows + Shape::BM - 1) / Shape::BM *
-                          ((p.dim + Shape::BN - 1) / Shape::BN);
-    const int64_t kt = (std::min(b.piece, p.vocab) + Shape::BK - 1) / Shape::BK;
-    const int cus = device_cus();
-    double best = 0;
-    for (int64_t n = 1; n <= std::min<int64_t>(64, kt); ++n) {
-      const double t = std::ceil((double)tiles * n / cus) * 1.5 * ((double)((kt + n - 1) / n) + 4) +
-                       n * (double)p.rows * p.dim * 8 / 4e6;
-      if (n > 1 && t >= best) continue;
-      best = t;
-      b.splits = (int)n;
-      b.kt_per_split = (int)((kt + n - 1) / n);
-    }
-    b.splits = (int)((kt + b.kt_per_split - 1) / b.kt_per_split);
-    part = (size_t)b.splits * p.rows * p.dim * 4;
+    const int64_t words = std::min(b.piece, p.vocab);
+    b.dh = bwd_splits(p.dim, p.rows, words, 1);
+    b.dw = bwd_splits(p.dim, words, p.rows, 0);
+    part = (size_t)b.dh.splits * p.rows * p.dim * 4;
+    if (b.dw.splits > 1) part_w = (size_t)b.dw.splits * words * p.dim * 4;
   }
-  b.bytes = b.part + round_up(part, 256);
+  b.part_w = b.part + round_up(part, 256);
+  b.bytes = b.part_w + round_up(part_w, 256);
   return b;
 }
 
@@ -400,12 +508,24 @@ int launch_dz_kept(const Head& p, const mhs::KeptLogits& kept, const mhs::HeadGr
   return check_launch("gradient of kept logits kernel");
 }
 
+// out (rows, cols) of the splits' sums (head_mm_reduce_kernel).
+template <class T>
+int launch_reduce(const float* part, void* out, const float* scale, const float2* rows2,
+                  int splits, int64_t rows, int64_t cols, hipStream_t s) {
+  const int64_t n = rows * cols / 4;
+  hipLaunchKernelGGL(mhs::head_mm_reduce_kernel<T>,
+                     dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, s,
+                     reinterpret_cast<const float4*>(part), static_cast<ushort4*>(out), scale,
+                     rows2, splits, (long long)rows, (int)(cols / 4));
+  return check_launch("gradient reduction kernel");
+}
+
 template <class T>
 int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogits& kept,
           const BwdOut& out, char* ws, hipStream_t s) {
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
-  const auto fh = &mhs::head_mm_kernel<T, Shape, true>;
-  const auto fw = &mhs::head_mm_kernel<T, Shape, false>;
+  const auto fh = &mhs::head_mm_kernel<T, Shape, false, true>;
+  const auto fw = &mhs::head_mm_kernel<T, Shape, false, false>;
   constexpr int lds_z = Shape::kLds + 2 * 2048;
   allow_lds(fz, lds_z);
   allow_lds(fh, Shape::kLds);
@@ -431,32 +551,31 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogit
     o.scale = a.scale;
     if (out.dhidden) {
       g = mm_args<Shape>(w + v0 * p.ldw, p.ldw, a.dz, b.ldz, p.dim, p.rows, words);
-      g.kt_per_split = b.kt_per_split;
+      g.kt_per_split = b.dh.kt_per_split;
       o.part = part;
+      o.ldo = p.dim;
       o.accumulate = v0 > 0;
-      hipLaunchKernelGGL(fh, dim3((unsigned)(g.grid_m * g.grid_n), (unsigned)b.splits),
+      hipLaunchKernelGGL(fh, dim3((unsigned)(g.grid_m * g.grid_n), (unsigned)b.dh.splits),
                          dim3(Shape::kThreads), Shape::kLds, s, g, o);
       if ((rc = check_launch("hidden gradient kernel")) != 0) return rc;
     }
     if (out.dweight) {
       g = mm_args<Shape>(hz, p.dim, a.dz, b.ldz, p.dim, words, p.rows);
-      o.part = nullptr;
+      g.kt_per_split = b.dw.kt_per_split;
+      o.part = b.dw.splits > 1 ? reinterpret_cast<float*>(ws + b.part_w) : nullptr;
       o.accumulate = 0;
       o.out = static_cast<u16*>(out.dweight) + v0 * p.dim;
       o.ldo = p.dim;
-      hipLaunchKernelGGL(fw, dim3((unsigned)(g.grid_m * g.grid_n)), dim3(Shape::kThreads),
-                         Shape::kLds, s, g, o);
+      hipLaunchKernelGGL(fw, dim3((unsigned)(g.grid_m * g.grid_n), (unsigned)b.dw.splits),
+                         dim3(Shape::kThreads), Shape::kLds, s, g, o);
       if ((rc = check_launch("weight gradient kernel")) != 0) return rc;
+      if (o.part && (rc = launch_reduce<T>(o.part, o.out, a.scale, nullptr, b.dw.splits, words,
+                                           p.dim, s)) != 0)
+        return rc;
     }
   }
-  if (out.dhidden) {
-    const int64_t n = p.rows * p.dim / 4;
-    hipLaunchKernelGGL(mhs::head_mm_reduce_kernel<T>,
-                       dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, s,
-                       reinterpret_cast<const float4*>(part), static_cast<ushort4*>(out.dhidden),
-                       a.scale, a.rows2, b.splits, (long long)p.rows, (int)(p.dim / 4));
-    if ((rc = check_launch("hidden gradient reduction kernel")) != 0) return rc;
-  }
+  if (out.dhidden)
+    return launch_reduce<T>(part, out.dhidden, a.scale, a.rows2, b.dh.splits, p.rows, p.dim, s);
   return MHS_OK;
 }
 

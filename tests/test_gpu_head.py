@@ -175,6 +175,34 @@ def test_one_gradient_only(dtype):
     assert torch.equal(torch.autograd.grad(linear_cross_entropy(h, b, t), [b])[0], both[2])
 
 
+@pytest.mark.parametrize("keep", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,vocab", [(33, 1096, 1), (33, 2056, 131), (65, 1032, 1001),
+                                            (130, 2048, 258), (257, 1544, 515)])
+def test_few_tiles_of_long_sums(rows, dim, vocab, dtype, keep, monkeypatch):
+    """Products cut up in k, the sums of exponentials from the logits in memory."""
+    print(f"[case] few tiles {dtype} {rows}x{dim}x{vocab}", flush=True)
+    _keep(monkeypatch, keep)
+    h, w, t = _operands(rows, dim, vocab, TYPES[dtype])
+    up = _upstream(rows, "none")
+    got = _run(linear_cross_entropy, h, w, up, t, reduction="none")
+    assert_head("xent", got, h, w, up, "none", TYPES[dtype], targets=t)
+    values, ids = _words(rows, vocab, 3)
+    up = _upstream(rows, "mean")
+    got = _run(linear_distill_loss, h, w, up, values, ids, temperature=2.0)
+    assert_head("distill", got, h, w, up, "mean", TYPES[dtype], words=(values, ids, 2.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,vocab", [(2050, 72, 300), (4100, 264, 70)])
+def test_weight_gradient_of_many_rows(rows, dim, vocab, dtype):
+    """Few tiles of the weight's gradient, cut up in the rows."""
+    h, w, t = _operands(rows, dim, vocab, TYPES[dtype])
+    up = _upstream(rows, "sum")
+    got = _run(linear_cross_entropy, h, w, up, t, reduction="sum")
+    assert_head("rows", got, h, w, up, "sum", TYPES[dtype], targets=t)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [512, 513])
 def test_rows_on_both_sides_of_a_block_each(rows, dtype):
