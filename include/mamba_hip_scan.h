@@ -417,7 +417,8 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
 
 /*
  * Losses of the model's head from its hidden states, the logits z = hidden
- * weight^T not in memory (but where a caller keeps them, below). Beside mhs_xent_*, which read given logits; the
+ * weight^T not in memory (but where a caller keeps them, below, and of few tiles of
+ * many columns in the workspace). Beside mhs_xent_*, which read given logits; the
  * reference forms them (mamba_metal/model.py:294-297).
  *
  *   hidden (rows, dim) rows ldh elements apart, weight (vocab, dim) rows ldw
@@ -441,8 +442,7 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
  *   that are not kept add nothing, whatever they hold, and get zeros.
  * logits, if given (16-byte aligned, else NULL): the forward keeps the fp32 logits
  *   there, (rows, vocab to a multiple of 4), for MHS_F32 (vocab, rows to a multiple
- *   of 4), and the backward reads them instead of forming them a second time. The
- *   other calls hold no more of them than a tile.
+ *   of 4), and the backward reads them instead of forming them a second time.
  * Every sum runs in a fixed order (bit-for-bit reproducible). The workspace is
  * 256-byte aligned; its size is 0 for arguments that the calls reject.
  */
@@ -464,9 +464,9 @@ size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t voca
 int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                         int64_t ldw, const int64_t* targets, const float* lse2,
                         const float* picked, const float* keep, const float* logits,
-                        const float* upstream, const float* count, void* dhidden, void* dweight, int64_t rows,
-                        int64_t vocab, int64_t dim, int reduction, void* workspace,
-                        size_t workspace_bytes, void* stream);
+                        const float* upstream, const float* count, void* dhidden,
+                        void* dweight, int64_t rows, int64_t vocab, int64_t dim, int reduction,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Distillation from a teacher's top words: per row `top` (1..MHS_MAX_TOP) words

@@ -32,6 +32,10 @@ struct RowSplit {
   }
 };
 
+// fp32 8192 x 32768 237 us (4.5 TB/s; a large copy takes 4.7), bf16 4096 x 50257 110
+// us (3.7, bound by its arithmetic and by rows that start at any element). A row to
+// 512 threads takes 2% less there, but forward and backward of 4096 x 4096 66 us
+// against 53.
 template <class T>
 __global__ void __launch_bounds__(kXentThreads)
 distill_fwd_kernel(HeadRows g) {
@@ -84,7 +88,8 @@ distill_fwd_kernel(HeadRows g) {
 }
 
 // dlogits (rows, vocab) contiguous. The teacher's words are put right after the
-// row is written (a word named twice: the same value twice).
+// row is written (a word named twice: the same value twice). fp32 8192 x 32768 430
+// us (5.0 TB/s), bf16 4096 x 50257 210 us (3.9).
 template <class T>
 __global__ void __launch_bounds__(kXentThreads)
 distill_bwd_kernel(const elem_t<T>* __restrict__ logits, long long ld,

@@ -1,6 +1,6 @@
 // Losses of a language model's head from its hidden states, for gfx950: the
-// logits z = h W^T (h (rows, dim), W (vocab, dim)) are formed tile by tile and
-// never kept. With c = log2(e) / temperature and everything in base 2,
+// logits z = h W^T (h (rows, dim), W (vocab, dim)) are formed tile by tile. With
+// c = log2(e) / temperature and everything in base 2,
 //   lse2_r = log2 sum_v 2^(c z_rv),       p_rv = 2^(c z_rv - lse2_r)
 // and a row's targets (ids id_k with weights q_k; one of weight 1 for the
 // cross entropy, the teacher's words for distillation) give
@@ -14,10 +14,10 @@
 // Forward: the product W h^T, whose epilogue reduces each tile to a maximum and
 // a sum per row (head_lse); a pass over the rows joins the tiles, forms the
 // logits of the row's ids again as dot products, and the loss.
-// Backward, a piece of the vocabulary at a time: the product again, whose
-// epilogue writes dz (16 bits, or fp32 for fp32 operands) to the workspace,
-// then the products with W and h. dW's rows are complete with their piece, dh
-// sums over the pieces in fp32.
+// Backward, a piece of the vocabulary at a time: the product again, or the logits
+// that the forward kept in fp32, and from them dz (16 bits, or fp32 for fp32
+// operands) to the workspace, then the products with W and h. dW's rows are
+// complete with their piece, dh sums over the pieces in fp32.
 #pragma once
 
 #include "mhs_common.hpp"
@@ -91,7 +91,8 @@ __device__ __forceinline__ void store_partials(float* red, float2* part, int n0,
   for (int n = threadIdx.x; n < cols; n += blockDim.x) {
     float m = red[n], s = red[cols + n];
 #pragma unroll
-    for (int w = 1; w < WM; ++w) lse2_combine(m, s, red[2 * w * cols + n], red[(2 * w + 1) * cols + n]);
+    for (int w = 1; w < WM; ++w)
+      lse2_combine(m, s, red[2 * w * cols + n], red[(2 * w + 1) * cols + n]);
     if (n0 + n < rows) part[at * rows + n0 + n] = make_float2(m, s);
   }
 }
@@ -104,7 +105,10 @@ struct KeptLogits {
 };
 
 // part[tile of the vocabulary][row] = (m, s) of the tile's logits, and, KEEP, the
-// logits. A = W (M = vocab), B = h (N = rows).
+// logits. A = W (M = vocab), B = h (N = rows). Bound by the matrix cores: the tiles
+// run as one stream (mm_stream), so that a tile's exponentials overlap the next one's
+// loads. bf16 8192 x 640 x 32768 348 us (987 TFLOP/s; a block per tile 377), 8192 x
+// 4096 x 131072 6206 us (1417).
 template <class T, class S, bool KEEP>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_lse_kernel(MmArgs g, float c, float2* __restrict__ part, KeptLogits kept) {
@@ -146,7 +150,8 @@ head_lse_kernel(MmArgs g, float c, float2* __restrict__ part, KeptLogits kept) {
   });
 }
 
-// The same for fp32 operands, on the products of three bf16 parts.
+// The same for fp32 operands, on the products of three bf16 parts, whose rate
+// bounds it: 8192 x 640 x 32768 1820 us (189 TFLOP/s), 1985 with the logits kept.
 template <int TILE>
 __global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
 head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part, KeptLogits kept) {
@@ -175,7 +180,8 @@ head_lse3_kernel(GemmArgs g, float c, float2* __restrict__ part, KeptLogits kept
     if (kept.z && r < g.N)
 #pragma unroll
       for (int i = 0; i < F * 16; ++i) {
-        const int v = m0 + wm * (TILE / 2) + i / 16 * 32 + 8 * (i % 16 / 4) + 4 * (lane >> 5) + i % 4;
+        const int v = m0 + wm * (TILE / 2) + i / 16 * 32 + 8 * (i % 16 / 4) + 4 * (lane >> 5) +
+                      i % 4;
         if (v < g.M) kept.z[v * kept.ld + r] = acc[i / 16][j][i % 16];
       }
   }
@@ -197,7 +203,8 @@ head_lse_of_logits_kernel(KeptLogits logits, int words, int rows, float c,
   const int left = words - v0, r = min(n0 + lane, rows - 1);
   float z[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) z[i] = i < left ? logits.z[(long long)(v0 + i) * logits.ld + r] : 0.f;
+  for (int i = 0; i < 16; ++i)
+    z[i] = i < left ? logits.z[(long long)(v0 + i) * logits.ld + r] : 0.f;
   float m, s;
   column_lse2<16>([&](int i) { return z[i]; }, [](int i) { return i; }, c, left, m, s);
   red[2 * wave * 64 + lane] = m;
@@ -423,7 +430,8 @@ struct HeadRows {
   float temperature;
 };
 
-// Cross entropy: W waves (1 or 4) per row.
+// Cross entropy: W waves (1 or 4) per row. Bound by latency: 12 us at 8192 rows of
+// 640 and 128 tiles, 50 at 4096 and 512.
 template <class T, int W>
 __global__ void __launch_bounds__(256)
 head_xent_rows_kernel(HeadRows g) {
@@ -537,7 +545,8 @@ __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2
   }
 }
 
-// Distillation: a block per row.
+// Distillation: a block per row. Bound by the gathered rows of W, from the caches:
+// 8192 rows of 64 words of 640, 671 MB in 16 bits, 105 us (6.4 TB/s).
 template <class T>
 __global__ void __launch_bounds__(256)
 head_distill_rows_kernel(HeadRows g) {
@@ -669,8 +678,8 @@ __device__ __forceinline__ float lift_of(float largest, int to) {
 constexpr int kCopyRows = 8;   // rows per block
 
 // scale[0..1] = (s, 1 / s), dz's power of two (lift_of to `lift`, scale[2] the largest
-// per-row gradient; lift 0: 1); rows2[r] = (coef s, lse2); and, `out` given, out (out_rows, per) = in
-// (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
+// per-row gradient; lift 0: 1); rows2[r] = (coef s, lse2); and, `out` given, out
+// (out_rows, per) = in (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
 // `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
 // reach dW.
 template <int UNUSED = 0>
@@ -742,7 +751,9 @@ __device__ __forceinline__ void exchange4(unsigned (&v)[4]) {
   }
 }
 
-// p's part of dz of a piece, 16 bits, (rows, ldz). The tile has the words in m, dz
+// p's part of dz of a piece, 16 bits, (rows, ldz). Bound as head_lse_kernel, and by
+// writing dz: 8192 x 640 x 32768 381 us in two pieces (902 TFLOP/s), 8192 x 4096 x
+// 131072 6731 us in eight (1307). The tile has the words in m, dz
 // the rows: a lane's 4 words of 4 fragments become 16 of one row (exchange4), in
 // two stores of 16 bytes, each 64 bytes of 16 rows at a time; no LDS.
 template <class T, class S>
@@ -799,7 +810,8 @@ head_dz_kernel(MmArgs g, HeadGrad a) {
   });
 }
 
-// The same in fp32, transposed: (words, ldz), its rows contiguous.
+// The same in fp32, transposed: (words, ldz), its rows contiguous. Bound by the
+// product: 8192 x 640 x 32768 1870 us (184 TFLOP/s).
 template <int TILE>
 __global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
 head_dz3_kernel(GemmArgs g, HeadGrad a) {
@@ -829,7 +841,8 @@ head_dz3_kernel(GemmArgs g, HeadGrad a) {
 }
 
 // p's part of dz of a piece from the logits that the forward kept: bound by
-// reading them and writing dz. 8 words of a row to a thread, or, fp32, 4 rows of a
+// reading them and writing dz (fp32, 8192 x 32768: 348 us, 2.1 GB at 6.2 TB/s with
+// dz's pieces in the caches). 8 words of a row to a thread, or, fp32, 4 rows of a
 // word, as they lie. `blocks` of 16 bytes to a row of dz, n in all.
 template <class T>
 __global__ void __launch_bounds__(256)
@@ -899,18 +912,22 @@ struct MmOut {
   const float* scale;
 };
 
+// (16 bytes a lane where fragments stored as they lie, 2 bytes a lane, took 3 to 10%
+// more of a whole backward.) Bound by the matrix cores: 8192 x 640 x 32768 dh 417 us
+// and dW 394 (824 and 872 TFLOP/s; 640 columns are two and a half tiles), 8192 x 4096
+// x 131072 6545 and 6348 (1344 and 1386).
 template <class T, class S, bool AK, bool BK>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_mm_kernel(MmArgs g, MmOut o) {
   extern __shared__ float lds_f[];
   int tm, tn;
   mm_tile(g, blockIdx.x, tm, tn);
-  const int k_first = blockIdx.y * g.kt_per_split * S::BK;
-  typename S::acc acc[S::FM][S::FN];
+  const int k_first = blockIdx.y * g.kt_per_split * kMmK;
+  f32x4 acc[S::FM][S::FN];
   mm_products<T, S, AK, BK>(acc, g, tm * S::BM, tn * S::BN, k_first,
-                            min(g.K - k_first, g.kt_per_split * S::BK),
+                            min(g.K - k_first, g.kt_per_split * kMmK),
                             reinterpret_cast<char*>(lds_f));
-  static_assert(S::E == 4 && S::FM % 4 == 0, "a lane's 4 rows of 4 fragments");
+  static_assert(S::FM % 4 == 0, "a lane's 4 rows of 4 fragments");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int mb = tm * S::BM + S::wave_m(wave) * (S::FM * 16);
   const int nb = tn * S::BN + S::wave_n(wave) * (S::FN * 16) + (lane & 15);

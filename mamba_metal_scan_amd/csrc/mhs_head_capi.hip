@@ -24,7 +24,7 @@ using mhs::Fp16;
 using mhs::Fp32;
 using mhs::round_up;
 
-typedef mhs::MmShape<256, 256, 2, 4, 2, 16, 1, 64> Shape;
+typedef mhs::MmShape<256, 256, 2, 4> Shape;
 
 // Rows that the kernel for few rows takes, by bytes of an element. us of it and of
 // the tiles, with the loss's kernel: fp32, 32 rows, 640 x 32768 36 and 46, 4096 x
@@ -132,8 +132,9 @@ struct KSplit {
   int splits, kt_per_split;
 };
 KSplit lse_splits(const Head& p) {
-  const int64_t tiles = (p.vocab + Shape::BM - 1) / Shape::BM * ((p.rows + Shape::BN - 1) / Shape::BN);
-  const int kt = (int)((p.dim + Shape::BK - 1) / Shape::BK);
+  const int64_t tiles = (p.vocab + Shape::BM - 1) / Shape::BM *
+                        ((p.rows + Shape::BN - 1) / Shape::BN);
+  const int kt = (int)((p.dim + mhs::kMmK - 1) / mhs::kMmK);
   KSplit best{1, kt};
   if (4 * tiles > device_cus()) return best;
   double least = 1.07 * kt;
@@ -166,7 +167,8 @@ bool few_tiles(const Head& p) {
 int64_t lse_tiles(const Head& p) {
   static_assert(mhs::kSmallWords == mhs::kLogitWords, "one size of partials");
   static_assert(mhs::kSplitWords == Shape::BM, "and of 16 bits");
-  if (few_rows(p) || (p.dtype == MHS_F32 && few_tiles(p))) return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
+  if (few_rows(p) || (p.dtype == MHS_F32 && few_tiles(p)))
+    return (p.vocab + mhs::kSmallWords - 1) / mhs::kSmallWords;
   const int bm = p.dtype == MHS_F32 ? gemm3_tile(p.rows) : Shape::BM;
   return (p.vocab + bm - 1) / bm;
 }
@@ -183,6 +185,10 @@ size_t logits_at(const Head& p) {
   return round_up((size_t)lse_tiles(p) * p.rows * 8, 256) + loss_ws(p.rows);
 }
 
+size_t gemm_ws(int64_t m, int64_t n, int64_t k) {
+  return (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(m, n, k), 0);
+}
+
 size_t logits_bytes(const Head& p) {
   return round_up(p.dtype == MHS_F32 ? (size_t)p.vocab * round_up(p.rows, 4) * 4
                                      : (size_t)p.rows * round_up(p.vocab, 4) * 4, 256);
@@ -192,7 +198,7 @@ size_t fwd_ws(const Head& p) {
   if (!few_tiles(p)) return logits_at(p);
   if (p.dtype != MHS_F32) return logits_at(p) + lse_splits(p).splits * logits_bytes(p);
   return logits_at(p) + logits_bytes(p) +
-         (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(p.vocab, p.rows, p.dim), 0);
+         gemm_ws(p.vocab, p.rows, p.dim);
 }
 
 template <class F>
@@ -217,7 +223,7 @@ mhs::MmArgs mm_args(const void* a, int64_t lda, const void* b, int64_t ldb, int6
   g.M = (int)M;
   g.N = (int)N;
   g.K = (int)K;
-  g.kt_per_split = (int)((K + S::BK - 1) / S::BK);
+  g.kt_per_split = (int)((K + mhs::kMmK - 1) / mhs::kMmK);
   g.grid_m = (int)((M + S::BM - 1) / S::BM);
   g.grid_n = (int)((N + S::BN - 1) / S::BN);
   g.group_m = kGroupM;
@@ -406,7 +412,8 @@ int head_fwd(const Head& p, mhs::HeadRows g, float* logits, float* loss, float* 
   }
   if (reduction == MHS_REDUCE_NONE) return MHS_OK;
   return launch_loss(g.loss, g.keep, loss, count, p.rows, reduction,
-                     static_cast<char*>(workspace) + round_up((size_t)lse_tiles(p) * p.rows * 8, 256),
+                     static_cast<char*>(workspace) +
+                         round_up((size_t)lse_tiles(p) * p.rows * 8, 256),
                      s);
 }
 
@@ -434,7 +441,7 @@ int64_t piece_words(int64_t rows, int64_t vocab, int es) {
 // and 677, 4096 x 640 x 16384 372 and 366; whole by this, 8192 x 1024 x 32768.)
 KSplit bwd_splits(int64_t M, int64_t N, int64_t K, int whole) {
   const int64_t tiles = (M + Shape::BM - 1) / Shape::BM * ((N + Shape::BN - 1) / Shape::BN);
-  const int64_t kt = (K + Shape::BK - 1) / Shape::BK;
+  const int64_t kt = (K + mhs::kMmK - 1) / mhs::kMmK;
   const int cus = device_cus();
   KSplit b{};
   double best = 0;
@@ -467,8 +474,7 @@ BwdPlan bwd_plan(const Head& p) {
     const int64_t last = p.vocab % b.piece ? p.vocab % b.piece : words;
     part = 0;
     for (const int64_t w : {words, last})
-      part = std::max({part, (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(p.rows, p.dim, w), 0),
-                       (size_t)std::max<int64_t>(mhs_gemm_workspace_bytes(w, p.dim, b.rows4), 0)});
+      part = std::max({part, gemm_ws(p.rows, p.dim, w), gemm_ws(w, p.dim, b.rows4)});
   } else {
     const int64_t words = std::min(b.piece, p.vocab);
     b.dh = bwd_splits(p.dim, p.rows, words, 1);
@@ -490,8 +496,8 @@ struct BwdOut {
 
 template <class T>
 int launch_ids(const Head& p, const mhs::HeadGrad& a, int64_t words, hipStream_t s) {
-  hipLaunchKernelGGL(mhs::head_ids_kernel<T>, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s, a,
-                     (long long)p.rows, (int)words);
+  hipLaunchKernelGGL(mhs::head_ids_kernel<T>, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s,
+                     a, (long long)p.rows, (int)words);
   return check_launch("gradient of the ids kernel");
 }
 
@@ -635,13 +641,15 @@ int launch_rows_in(const Head& p, const BwdPlan& b, const mhs::RowScale& rs, con
 // zeros: a gradient that no row reaches.
 int launch_zero(void* p, int64_t n, int es, hipStream_t s) {
   const int64_t words = n * es / 4;   // (dim is a multiple of 16 bytes)
-  hipLaunchKernelGGL(mhs::head_zero_kernel<>, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 4096)),
-                     dim3(256), 0, s, static_cast<unsigned*>(p), (long long)words);
+  hipLaunchKernelGGL(mhs::head_zero_kernel<>,
+                     dim3((unsigned)std::min<int64_t>((words + 255) / 256, 4096)), dim3(256), 0, s,
+                     static_cast<unsigned*>(p), (long long)words);
   return check_launch("zero fill kernel");
 }
 
 int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const float* lse2,
-             const float* logits, const BwdOut& out, void* workspace, size_t workspace_bytes, void* stream) {
+             const float* logits, const BwdOut& out, void* workspace, size_t workspace_bytes,
+             void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int es = elem_bytes(p.dtype);
   if (out.dhidden == nullptr && out.dweight == nullptr) return MHS_OK;
@@ -706,9 +714,10 @@ template <class T>
 int launch_distill_bwd(const void* logits, int64_t ld, const int64_t* ids, const float* q,
                        const float* lse2, const mhs::RowScale& rs, void* dlogits, int64_t rows,
                        int64_t vocab, int64_t top, float c, hipStream_t s) {
-  hipLaunchKernelGGL(mhs::distill_bwd_kernel<T>, dim3((unsigned)rows), dim3(mhs::kXentThreads), 0, s,
-                     static_cast<const mhs::elem_t<T>*>(logits), (long long)ld, ll(ids), q, lse2, rs,
-                     static_cast<mhs::elem_t<T>*>(dlogits), (long long)vocab, (int)top, c);
+  hipLaunchKernelGGL(mhs::distill_bwd_kernel<T>, dim3((unsigned)rows), dim3(mhs::kXentThreads), 0,
+                     s, static_cast<const mhs::elem_t<T>*>(logits), (long long)ld, ll(ids), q,
+                     lse2, rs, static_cast<mhs::elem_t<T>*>(dlogits), (long long)vocab, (int)top,
+                     c);
   return check_launch("distillation backward kernel");
 }
 
@@ -738,9 +747,9 @@ size_t mhs_linear_xent_fwd_workspace_bytes(int dtype, int64_t rows, int64_t voca
 
 int mhs_linear_xent_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                         const int64_t* targets, float* lse2, float* picked, float* keep,
-                        float* logits, float* loss_rows, float* loss, float* count, int64_t rows, int64_t vocab,
-                        int64_t dim, int64_t ignore_index, int reduction, void* workspace,
-                        size_t workspace_bytes, void* stream) {
+                        float* logits, float* loss_rows, float* loss, float* count, int64_t rows,
+                        int64_t vocab, int64_t dim, int64_t ignore_index, int reduction,
+                        void* workspace, size_t workspace_bytes, void* stream) {
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
   int rc = check_head(p);
@@ -766,8 +775,9 @@ size_t mhs_linear_xent_bwd_workspace_bytes(int dtype, int64_t rows, int64_t voca
 int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                         const int64_t* targets, const float* lse2, const float* picked,
                         const float* keep, const float* logits, const float* upstream,
-                        const float* count, void* dhidden, void* dweight, int64_t rows, int64_t vocab, int64_t dim,
-                        int reduction, void* workspace, size_t workspace_bytes, void* stream) {
+                        const float* count, void* dhidden, void* dweight, int64_t rows,
+                        int64_t vocab, int64_t dim, int reduction, void* workspace,
+                        size_t workspace_bytes, void* stream) {
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
   int rc = check_head(p);
@@ -786,8 +796,8 @@ int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* 
 int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                            int64_t ldw, const float* teacher, const int64_t* ids, float* lse2,
                            float* picked, float* q, float* keep, float* logits, float* loss_rows,
-                           float* loss, float* count, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
-                           float temperature, int reduction, void* workspace,
+                           float* loss, float* count, int64_t rows, int64_t vocab, int64_t dim,
+                           int64_t top, float temperature, int reduction, void* workspace,
                            size_t workspace_bytes, void* stream) {
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
@@ -810,9 +820,9 @@ int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const voi
 int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const void* weight,
                            int64_t ldw, const int64_t* ids, const float* lse2, const float* picked,
                            const float* q, const float* keep, const float* logits,
-                           const float* upstream, const float* count, void* dhidden, void* dweight, int64_t rows,
-                           int64_t vocab, int64_t dim, int64_t top, float temperature,
-                           int reduction, void* workspace, size_t workspace_bytes, void* stream) {
+                           const float* upstream, const float* count, void* dhidden,
+                           void* dweight, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
+                           float temperature, int reduction, void* workspace, size_t workspace_bytes, void* stream) {
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
   int rc = check_head(p);
@@ -890,12 +900,10 @@ int mhs_distill_bwd(int dtype, const void* logits, int64_t ld, const int64_t* id
   const mhs::RowScale rs = row_scale(upstream, count, keep, reduction, temperature);
   const float c = mhs::kLog2e / temperature;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == MHS_F32
-             ? launch_distill_bwd<Fp32>(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c, s)
-         : dtype == MHS_BF16
-             ? launch_distill_bwd<Bf16>(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c, s)
-             : launch_distill_bwd<Fp16>(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c,
-                                        s);
+  const auto fn = dtype == MHS_F32    ? &launch_distill_bwd<Fp32>
+                  : dtype == MHS_BF16 ? &launch_distill_bwd<Bf16>
+                                      : &launch_distill_bwd<Fp16>;
+  return fn(logits, ld, ids, q, lse2, rs, dlogits, rows, vocab, top, c, s);
 }
 
 }  // extern "C"

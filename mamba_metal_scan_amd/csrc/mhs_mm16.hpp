@@ -1,18 +1,25 @@
 // Matrix products of 16-bit operands (bf16, fp16) on gfx950's matrix cores:
 //   acc(m, n) = sum_k A(m, k) B(n, k),  fp32 sums,
-// one BM x BN tile per block, fragments of 32 x 32 per wave; what becomes of a tile is up to the kernel's epilogue
-// (mhs_head.hpp).
+// a BM x BN tile at a time per block, in 16 x 16 fragments (MFMAs 32 deep); what
+// becomes of a tile is up to the kernel's epilogue (mhs_head.hpp).
 //
 // An operand is K-major ((rows, K), k contiguous) or row-major ((K, rows)); both
-// stage a k tile (32 deep) by 16-byte global loads that write LDS directly, and
+// stage a k tile (64 deep) by 16-byte global loads that write LDS directly, and
 // differ in how a wave then reads its fragments: K-major with 16-byte LDS
 // reads, row-major with the transposing 8-byte reads (within 16 lanes, lane i
 // gives the address of row i / 4, columns 4 (i % 4) .. + 3 and receives column
 // i of those four rows).
 //
-// The loads go kMmStages - 1 k tiles ahead of the products: a k tile's LDS
-// buffer is refilled as soon as every wave holds its fragments in registers,
-// and one barrier per k tile both publishes the next tile and frees this one.
+// Two k tiles lie in LDS. A wave reads the fragments of one step (32 deep) while
+// it multiplies those of the step before, from two sets of registers; at a k
+// tile's last step one wait and barrier publish the next tile and free this one,
+// which the loads of the tile after the next then refill. 256 x 256 tiles of 8
+// waves, one block per CU: a wave's step is 12 fragments read for 32 MFMAs. Bound by
+// the matrix cores at the power limit, 1.5 to 2.0 GHz of 2.4 (a library product of
+// 8192^3 reaches 1341 TFLOP/s here, one of 8192 x 16384 x 4096 1618); rates stand at
+// the kernels. (TFLOP/s at 8192 x 4096 x 16384, with the sums of exponentials and for
+// W's gradient: 1476 and 1334; with 32 x 32 fragments 1358 for the first; 256 x 128
+// tiles, two blocks per CU and 32 deep, 1148 for the second.)
 #pragma once
 
 #include "mhs_common.hpp"
@@ -26,14 +33,8 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-
-// Element types: tags with the MFMAs (32 x 32 x 16 and 16 x 16 x 32) and the
-// conversions.
+// Element types: tags with the MFMA and the conversions.
 struct Bf16 {
-  static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
   static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -46,10 +47,6 @@ struct Bf16 {
   }
 };
 struct Fp16 {
-  static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
-                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
   static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -105,13 +102,16 @@ __device__ __forceinline__ constexpr int mm_perm(int x) {
   return (x & ~63) + (x & 8) * 4 + ((x >> 4) & 3) * 8 + (x & 7);
 }
 
-// One operand of a block of WAVES waves: R rows from r0 of `rows`, k tiles BK
-// deep. PERM: its rows lie in LDS in mm_perm's order (K-major).
-template <int R, bool KMAJOR, int WAVES, int MI, int BK, bool PERM = false>
+constexpr int kMmK = 64;        // k's of a k tile
+constexpr int kMmStages = 2;    // k tiles in LDS
+
+// One operand of a block of WAVES waves: R rows from r0 of `rows`. PERM: its rows
+// lie in LDS in mm_perm's order (K-major).
+template <int R, bool KMAJOR, int WAVES, bool PERM = false>
 struct MmOperand {
-  static constexpr int kBytes = R * BK * 2;                // of a k tile
+  static constexpr int kBytes = R * kMmK * 2;                // of a k tile
   static constexpr int kLoads = kBytes / 1024 / WAVES;     // direct loads per wave and k tile
-  static constexpr int kLanes = (KMAJOR ? BK : R) / 8;     // lanes per row (K-major) or k row
+  static constexpr int kLanes = (KMAJOR ? kMmK : R) / 8;     // lanes per row (K-major) or k row
   static_assert(kLoads * 1024 * WAVES == kBytes, "whole loads");
   unsigned voff[kLoads];                       // byte offset of load j at a k tile, or kOOB
   int kpos[kLoads];                            // the k it starts at within the tile
@@ -121,12 +121,11 @@ struct MmOperand {
 
   // Chunk c (16 bytes) of row r (K-major) or k row r lies at place c ^ swz(r).
   // K-major: the 8 (and 16) lanes of one pass of a 16-byte read, on consecutive
-  // rows of 128 or 64 bytes, then hit different banks; row-major: the k rows that
-  // one pass of the transposing reads meets (4 in a row, and with 16 x 16
-  // fragments those 8 further) do. SQ_LDS_BANK_CONFLICT is 0.
+  // rows of 128 bytes, then hit different banks; row-major: the k rows that one
+  // pass of the transposing reads meets (4 in a row and those 8 further) do.
+  // SQ_LDS_BANK_CONFLICT is 0.
   static __device__ __forceinline__ constexpr int swz(int r) {
-    if (!KMAJOR) return ((r & 3) << 2) ^ (MI == 16 ? ((r >> 3) & 1) << 1 : 0);
-    return BK == 64 ? (r & 7) ^ ((r >> 3) & 1) : ((r >> 1) & 3) ^ ((r >> 3) & 1);
+    return KMAJOR ? (r & 7) ^ ((r >> 3) & 1) : ((r & 3) << 2) ^ ((r >> 3) & 1) << 1;
   }
 
   // wrow: the wave's first row within the tile.
@@ -134,15 +133,15 @@ struct MmOperand {
                                        int wave, int lane, int wrow) {
     place(p, ld, r0, rows, k_first, wave, lane);
     if constexpr (KMAJOR) {
-      step = BK * 2;
-      frag = (wrow + lane % MI) * (2 * BK) + ((lane / MI ^ swz(lane & 15)) << 4);
+      step = kMmK * 2;
+      frag = (wrow + (lane & 15)) * (2 * kMmK) + ((lane >> 4 ^ swz(lane & 15)) << 4);
     } else {
-      step = ld * (2 * BK);
-      // Fragment element (row, k) of a lane: row lane % MI, k 8 (lane / MI) + 0..7;
-      // the transposing read's own address: k row 8 (lane / MI) + (lane % 16) / 4
-      // (+ 4 for its second half), 4 rows from 16 (lane % MI / 16) + 4 (lane % 4).
-      const int k = 8 * (lane / MI) + ((lane & 15) >> 2);
-      const int row = wrow + 16 * (lane % MI / 16) + 4 * (lane & 3);
+      step = ld * (2 * kMmK);
+      // Fragment element (row, k) of a lane: row lane % 16, k 8 (lane / 16) + 0..7;
+      // the transposing read's own address: k row 8 (lane / 16) + (lane % 16) / 4
+      // (+ 4 for its second half), 4 rows from 4 (lane % 4).
+      const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+      const int row = wrow + 4 * (lane & 3);
       frag = k * (2 * R) + ((2 * row) ^ (swz(k) << 4));
     }
   }
@@ -173,15 +172,15 @@ struct MmOperand {
   __device__ __forceinline__ void load(i32x4 r, int j, unsigned lds, int left, int wave) const {
     mm_load_lds(r, kpos[j] < left ? voff[j] : kOOB, lds + (wave * kLoads + j) * 1024);
   }
-  // Fragment f (MI rows, 512 / MI deep) of step kk, from the operand's buffer.
+  // Fragment f (16 rows, 32 deep) of step kk, from the operand's buffer.
   __device__ __forceinline__ s16x8 read(const char* buf, int f, int kk) const {
     if constexpr (KMAJOR) {
-      return *reinterpret_cast<const s16x8*>(buf + f * (MI * 2 * BK) + (frag ^ (kk * (1024 / MI))));
+      return *reinterpret_cast<const s16x8*>(buf + f * (32 * kMmK) + (frag ^ (kk * 64)));
     } else {
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      // (MI rows are 2 MI bytes, bits that the swizzle flips and wrow leaves 0
-      // where there is more than one fragment; a step's k rows are 0 mod 16)
-      const char* p = buf + kk * (512 / MI * 2 * R) + (frag ^ (f * (2 * MI)));
+      // (16 rows are 32 bytes, bits that the swizzle flips and wrow leaves 0 where
+      // there is more than one fragment; a step's k rows are 0 mod 16)
+      const char* p = buf + kk * (64 * R) + (frag ^ (f * 32));
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 2 * R));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -204,130 +203,107 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g, int index, int& tm, int
   tn = i / size;
 }
 
-// A block's shape: BM x BN tile, WM x WN waves of FM x FN fragments (MI x MI),
-// ST k tiles BK deep in LDS; a wave's registers hold the fragments of SUB steps
-// (512 / MI deep) while it multiplies those of the SUB steps before.
-template <int BM_, int BN_, int WM_, int WN_, int ST_, int MI_, int SUB_, int BK_>
+// A block's shape: BM x BN tile, WM x WN waves of FM x FN fragments.
+template <int BM_, int BN_, int WM_, int WN_>
 struct MmShape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_, MI = MI_, SUB = SUB_;
-  static constexpr int BK = BK_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr int FM = BM / WM / MI, FN = BN / WN / MI;
-  static constexpr int E = MI * MI / 64;   // a lane's elements of a fragment
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static constexpr int kLds = kMmStages * (BM + BN) * kMmK * 2;
   // A wave's place in the tile. Waves w and w + 4, which share a SIMD, lie half a
   // tile apart in m, so that in a tile half past the end there each SIMD has one
   // wave at work (640 x 8192 x 16384, its third tile of 256 rows a half one: 184 us,
   // against 196 with two of the half's waves to a SIMD).
   static __device__ __forceinline__ int wave_m(int wave) { return wave / WN; }
   static __device__ __forceinline__ int wave_n(int wave) { return wave % WN; }
-  typedef float acc __attribute__((ext_vector_type(E)));
-  static constexpr int kLds = ST * (BM + BN) * BK * 2;
 };
 
 // acc = the tile's sums over k's k_first .. k_first + k_len - 1. A fragment's
-// element e of lane l: row 8 (e / 4) + 4 (l / MI) + e % 4, column l % MI. Ends on
-// a barrier, the LDS free.
-template <class T, class S, bool AK, bool BKM>
-__device__ __forceinline__ void mm_products(typename S::acc (&acc)[S::FM][S::FN], const MmArgs& g,
-                                            int m0, int n0, int k_first, int k_len, char* lds) {
-  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, MI = S::MI, BK = S::BK, KS = BK * MI / 512;
+// element e of lane l: row 4 (l / 16) + e, column l % 16. Ends on a barrier, the LDS
+// free.
+template <class T, class S, bool AK, bool BK>
+__device__ __forceinline__ void mm_products(f32x4 (&acc)[S::FM][S::FN], const MmArgs& g, int m0,
+                                            int n0, int k_first, int k_len, char* lds) {
+  constexpr int FM = S::FM, FN = S::FN, ST = kMmStages, PH = kMmK / 32;
+  static_assert(ST == 2 && PH % 2 == 0, "the register sets alternate over whole k tiles");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  typedef MmOperand<S::BM, AK, S::kWaves, MI, BK> OA;
-  typedef MmOperand<S::BN, BKM, S::kWaves, MI, BK> OB;
+  typedef MmOperand<S::BM, AK, S::kWaves> OA;
+  typedef MmOperand<S::BN, BK, S::kWaves> OB;
   constexpr int LA = OA::kLoads, LB = OB::kLoads, L = LA + LB;
   constexpr int TA = OA::kBytes, BUF = TA + OB::kBytes;
-  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, S::wave_m(wave) * (FM * MI));
-  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, S::wave_n(wave) * (FN * MI));
+  OA a(g.A, g.lda, m0, g.M, k_first, wave, lane, S::wave_m(wave) * (FM * 16));
+  OB b(g.B, g.ldb, n0, g.N, k_first, wave, lane, S::wave_n(wave) * (FN * 16));
   const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int e = 0; e < S::E; ++e) acc[i][j][e] = 0.f;
-  // Phases of SUB steps per k tile; the register sets alternate, so the loop goes
-  // over an even number of them (a k tile past the end is zeros).
-  constexpr int SUB = S::SUB, PH = KS / SUB, KT = PH % 2 ? 2 : 1;
-  static_assert(PH * SUB == KS, "whole phases");
-  const int nk = (k_len + BK - 1) / BK, round_nk = (nk + KT - 1) / KT * KT;
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int nk = (k_len + kMmK - 1) / kMmK;
 #pragma unroll
   for (int s = 0; s < ST; ++s) {
     const i32x4 ra = a.next(), rb = b.next();
 #pragma unroll
-    for (int j = 0; j < LA; ++j) a.load(ra, j, at + s * BUF, k_len - s * BK, wave);
+    for (int j = 0; j < LA; ++j) a.load(ra, j, at + s * BUF, k_len - s * kMmK, wave);
 #pragma unroll
-    for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, k_len - s * BK, wave);
+    for (int j = 0; j < LB; ++j) b.load(rb, j, at + s * BUF + TA, k_len - s * kMmK, wave);
   }
   mm_wait<(ST - 1) * L>();
-  if (m0 + S::wave_m(wave) * (FM * MI) >= g.M || n0 + S::wave_n(wave) * (FN * MI) >= g.N) {
+  if (m0 + S::wave_m(wave) * (FM * 16) >= g.M || n0 + S::wave_n(wave) * (FN * 16) >= g.N) {
     // Nothing of this wave's is within the product: its share of the loads alone.
-    for (int kt = 0, cur = 0; kt < round_nk; ++kt) {
-      mm_wait<(ST - 2) * L>();
+    for (int kt = 0, cur = 0; kt < nk; ++kt, cur ^= 1) {
+      mm_wait<0>();
       const i32x4 ra = a.next(), rb = b.next();
-      const int left = k_len - (kt + ST) * BK;
+      const int left = k_len - (kt + ST) * kMmK;
 #pragma unroll
       for (int j = 0; j < LA; ++j) a.load(ra, j, at + cur * BUF, left, wave);
 #pragma unroll
       for (int j = 0; j < LB; ++j) b.load(rb, j, at + cur * BUF + TA, left, wave);
-      cur = cur + 1 == ST ? 0 : cur + 1;
     }
     mm_wait<0>();
     return;
   }
-  s16x8 fa[2][SUB][FM], fb[2][SUB][FN];
+  s16x8 fa[2][FM], fb[2][FN];
 #pragma unroll
-  for (int u = 0; u < SUB; ++u) {
+  for (int i = 0; i < FM; ++i) fa[0][i] = a.read(lds, i, 0);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fa[0][u][i] = a.read(lds, i, u);
+  for (int j = 0; j < FN; ++j) fb[0][j] = b.read(lds + TA, j, 0);
+  // cur: the buffer of the k tile.
+  for (int kt = 0, cur = 0; kt < nk; ++kt, cur ^= 1) {
+    const int left = k_len - (kt + ST) * kMmK;
+    i32x4 ra, rb;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fb[0][u][j] = b.read(lds + TA, j, u);
-  }
-  int cur = 0;   // the buffer of the k tile
-  for (int kt = 0; kt < round_nk; kt += KT) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const int next = cur + 1 == ST ? 0 : cur + 1;
-      const int left = k_len - (kt + t + ST) * BK;
-      i32x4 ra, rb;
-#pragma unroll
-      for (int p = 0; p < PH; ++p) {
-        const int set = (t * PH + p) % 2;
-        if (p == PH - 1) {
-          // The next tile has landed, and every wave holds its last fragments of
-          // this one: its buffer takes the tile ST further.
-          mm_wait<(ST - 2) * L>();
-          ra = a.next();
-          rb = b.next();
-        }
-        const char* nb = lds + (p == PH - 1 ? next : cur) * BUF;
-        // A row of fragments' products at a time, with each its share of the
-        // next phase's fragments and of the direct loads: the wave issues them
-        // while the matrix core works.
-#pragma unroll
-        for (int q = 0; q < SUB * FM; ++q) {
-          constexpr int F = FM + FN, R = SUB * F;
-          const int u = q / FM, i = q % FM;
-#pragma unroll
-          for (int x = q * R / (SUB * FM); x < (q + 1) * R / (SUB * FM); ++x) {
-            const int step = (p + 1) % PH * SUB + x / F, f = x % F;
-            if (f < FM) fa[1 - set][x / F][f] = a.read(nb, f, step);
-            else fb[1 - set][x / F][f - FM] = b.read(nb + TA, f - FM, step);
-          }
-          if (p == PH - 1) {
-#pragma unroll
-            for (int l = q * L / (SUB * FM); l < (q + 1) * L / (SUB * FM); ++l) {
-              if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
-              else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-            acc[i][j] = T::mfma(fa[set][u][i], fb[set][u][j], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+    for (int p = 0; p < PH; ++p) {
+      if (p == PH - 1) {
+        // The next tile has landed, and every wave holds its last fragments of
+        // this one: its buffer takes the tile ST further.
+        mm_wait<0>();
+        ra = a.next();
+        rb = b.next();
       }
-      cur = next;
+      const char* nb = lds + (p == PH - 1 ? cur ^ 1 : cur) * BUF;
+      // A row of fragments' products at a time, with each its share of the next
+      // step's fragments and of the direct loads: the wave issues them while the
+      // matrix core works.
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        constexpr int F = FM + FN;
+#pragma unroll
+        for (int f = i * F / FM; f < (i + 1) * F / FM; ++f) {
+          if (f < FM) fa[1 - p % 2][f] = a.read(nb, f, (p + 1) % PH);
+          else fb[1 - p % 2][f - FM] = b.read(nb + TA, f - FM, (p + 1) % PH);
+        }
+        if (p == PH - 1) {
+#pragma unroll
+          for (int l = i * L / FM; l < (i + 1) * L / FM; ++l) {
+            if (l < LA) a.load(ra, l, at + cur * BUF, left, wave);
+            else b.load(rb, l - LA, at + cur * BUF + TA, left, wave);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fa[p % 2][i], fb[p % 2][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   mm_wait<0>();
@@ -349,17 +325,17 @@ __device__ __forceinline__ int mm_opaque(int v) {
 template <class T, class S, class Side, class Epi>
 __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side& side,
                                           const Epi& epi) {
-  static_assert(S::ST == 2, "every k tile waits for all loads before it: side's too");
-  constexpr int FM = S::FM, FN = S::FN, ST = S::ST, BK = S::BK, PH = BK * S::MI / 512;
-  static_assert(S::MI == 16 && S::SUB == 1 && PH % 2 == 0 && FM % 4 == 0, "the shape streams");
+  constexpr int FM = S::FM, FN = S::FN, ST = kMmStages, PH = kMmK / 32;
+  static_assert(ST == 2, "every k tile waits for all loads before it: side's too");
+  static_assert(PH % 2 == 0 && FM % 4 == 0, "the shape streams");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  typedef MmOperand<S::BM, true, S::kWaves, 16, BK, true> OA;
-  typedef MmOperand<S::BN, true, S::kWaves, 16, BK> OB;
+  typedef MmOperand<S::BM, true, S::kWaves, true> OA;
+  typedef MmOperand<S::BN, true, S::kWaves> OB;
   constexpr int LA = OA::kLoads, LB = OB::kLoads, L = LA + LB;
   constexpr int TA = OA::kBytes, BUF = TA + OB::kBytes;
   const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
-  const int tiles = g.grid_m * g.grid_n, nk = (g.K + BK - 1) / BK;
+  const int tiles = g.grid_m * g.grid_n, nk = (g.K + kMmK - 1) / kMmK;
   // Where the loads are: k tile load_kt of tile load_tile.
   int load_tile = blockIdx.x, load_kt = 0, load_odd = 0, tm, tn;
   mm_tile(g, load_tile, tm, tn);
@@ -382,7 +358,7 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
     }
     ra = a.next();
     rb = b.next();
-    return load_tile < tiles ? g.K - load_kt++ * BK : 0;
+    return load_tile < tiles ? g.K - load_kt++ * kMmK : 0;
   };
 #pragma unroll
   for (int s = 0; s < ST; ++s) {
@@ -401,19 +377,19 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
   for (int j = 0; j < FN; ++j) fb[0][j] = b.read(lds + TA, j, 0);
   int cur = 0, odd = 0;   // the buffer of the k tile; the tile's side
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, odd ^= 1) {
-    typename S::acc acc[FM][FN];
+    f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = typename S::acc{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int kt = 0; kt < nk; ++kt) {
-      const int next_buf = cur + 1 == ST ? 0 : cur + 1;
+      const int next_buf = cur ^ 1;
       i32x4 ra, rb;
       int left = 0;
 #pragma unroll
       for (int p = 0; p < PH; ++p) {
         if (p == PH - 1) {   // (as in mm_products)
-          mm_wait<(ST - 2) * L>();
+          mm_wait<0>();
           left = next(ra, rb);
         }
         const char* nb = lds + (p == PH - 1 ? next_buf : cur) * BUF;

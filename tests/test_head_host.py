@@ -77,7 +77,8 @@ def _xent_fwd(dtype=1, hidden=A, ldh=64, weight=A, ldw=64, targets=A, rows=4, vo
     lib = _native.library()
     if nbytes is None:
         nbytes = lib.mhs_linear_xent_fwd_workspace_bytes(1, 4, 50, 64)
-    return lib.mhs_linear_xent_fwd(dtype, hidden, ldh, weight, ldw, targets, A, A, A, logits, A, loss, A,
+    return lib.mhs_linear_xent_fwd(dtype, hidden, ldh, weight, ldw, targets, A, A, A, logits, A,
+                                   loss, A,
                                    rows, vocab, dim, -100, reduction, ws, nbytes, None)
 
 
@@ -88,7 +89,8 @@ def _xent_fwd(dtype=1, hidden=A, ldh=64, weight=A, ldw=64, targets=A, rows=4, vo
     (dict(ldh=65), "strides"), (dict(ldw=1 << 21), "strides"), (dict(hidden=MIS), "aligned"),
     (dict(weight=None), "null"), (dict(hidden=None), "null"), (dict(targets=None), "null"),
     (dict(loss=None), "null"), (dict(nbytes=16), "too small"), (dict(ws=None), "too small"),
-    (dict(ws=MIS), "256-byte"), (dict(logits=MIS), "aligned"), (dict(rows=1 << 30, vocab=1 << 30), "too large")])
+    (dict(ws=MIS), "256-byte"), (dict(logits=MIS), "aligned"),
+    (dict(rows=1 << 30, vocab=1 << 30), "too large")])
 def test_cross_entropy_entry_refuses(kw, match):
     assert _xent_fwd(**kw) == EINVAL
     assert match in _err(), _err()
@@ -185,7 +187,8 @@ def test_fake_ops_have_the_kernels_shapes():
         assert dh.shape == h.shape and dw.shape == (0,) and dh.dtype == h.dtype
         assert saved.shape == (4 + 6 * 4,)
         assert ops.linear_xent_fwd(h, w, t, -100, 1, True)[1].shape == (28 + 6 * 52,)
-        assert ops.linear_xent_fwd(h.float(), w.float(), t, -100, 1, True)[1].shape == (28 + 50 * 8,)
+        kept = ops.linear_xent_fwd(h.float(), w.float(), t, -100, 1, True)[1]
+        assert kept.shape == (28 + 50 * 8,)
         loss, saved = ops.linear_distill_fwd(h, w, ids.float(), ids, 1.0, 0)
         assert loss.shape == (6,)
         dh, dw = ops.linear_distill_bwd(loss, h, w, ids, saved, 1.0, 0, True, True)
