@@ -1405,8 +1405,9 @@ def _linear_xent_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor, targets: t
         rc = lib.mhs_linear_xent_fwd(
             dt, hidden.data_ptr(), hidden.stride(0) if rows else dim, weight.data_ptr(),
             weight.stride(0), targets.data_ptr(), lse2, picked, keep,
-            _kept_logits(saved, hidden, 1), losses if reduction else loss.data_ptr(), loss.data_ptr(), count, rows, vocab, dim,
-            ignore_index, reduction, ws.data_ptr(), nbytes, _stream(dev))
+            _kept_logits(saved, hidden, 1), losses if reduction else loss.data_ptr(),
+            loss.data_ptr(), count, rows, vocab, dim, ignore_index, reduction, ws.data_ptr(),
+            nbytes, _stream(dev))
     _check(rc, "mhs_linear_xent_fwd")
     return loss, saved
 

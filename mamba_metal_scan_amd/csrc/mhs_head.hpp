@@ -663,8 +663,8 @@ head_largest_kernel(RowScale rs, float* __restrict__ largest, long long rows) {
 
 // The power of two by which dz is stored larger, such that the largest |coef| lies
 // in [2^(to-1), 2^to); 1 where that is 0 or not finite. fp16: to 2^15, |dz| stays
-// below 2^16, and probabilities below 2^-24 of it keep their bits. fp32: to 2^32,
-// which takes the smallest probabilities (2^-126) to 2^-95, below which the fp32
+// below 2^16, and probabilities below 2^-24 of it keep their bits. fp32: to 2^32
+// (and never smaller: a row whose gradient is far below the largest keeps it), which takes the smallest probabilities (2^-126) to 2^-95, below which the fp32
 // product goes by fp32 MFMAs at half its rate (gemm3; 1024 x 4096 x 131072 of
 // logits of std 64 without it: 41.2 ms for loss and gradients, 22.5 with std 1).
 // bf16 products have no such bounds.
@@ -672,7 +672,7 @@ __device__ __forceinline__ float lift_of(float largest, int to) {
   if (!(largest > 0.f && largest < INFINITY)) return 1.f;
   int e = 0;
   (void)frexpf(largest, &e);   // largest in [2^(e-1), 2^e)
-  return ldexpf(1.f, min(max(to - e, -126), 126));
+  return ldexpf(1.f, min(max(to - e, to == 32 ? 0 : -126), 126));
 }
 
 constexpr int kCopyRows = 8;   // rows per block

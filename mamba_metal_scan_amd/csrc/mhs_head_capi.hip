@@ -658,7 +658,7 @@ int head_bwd(const Head& p, mhs::HeadGrad a, mhs::RowScale rs, const float* lse2
     return fail(MHS_EINVAL, "null pointer argument");
   if (!aligned16(out.dhidden) || !aligned16(out.dweight) || !aligned16(logits))
     return fail(MHS_EINVAL, "dhidden, dweight and logits must be 16-byte aligned");
-  if (p.dtype == MHS_F32 && p.rows >= (1LL << 22))   // (dz's row stride)
+  if (p.dtype == MHS_F32 && p.rows > (1LL << 22) - 4)   // (dz's row stride)
     return fail(MHS_EINVAL, "the fp32 backward takes rows below 2^22; got %lld", (long long)p.rows);
   int rc = check_workspace(workspace, workspace_bytes, bwd_ws(p));
   if (rc) return rc;

@@ -219,7 +219,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     The loss is float32: a scalar, or with reduction "none" one per row, of
     targets' shape (0 where ignored). Rows that are ignored add nothing to the
     gradients, whatever they hold. A target outside [0, V) that is not
-    ignore_index makes its row's loss NaN. Under autocast hidden and weight are
+    ignore_index makes its row's loss NaN. Between forward and backward it may hold
+    up to 1 GB of the logits (``_native.keeps_logits``). Under autocast hidden and weight are
     taken in its type. The gradients are once differentiable."""
     what = "linear_cross_entropy"
     _hip(what, hidden, weight, targets)

@@ -484,8 +484,8 @@ class TinyMamba(nn.Module):
                 and h.dtype in (torch.float32, torch.bfloat16, torch.float16))
 
     def loss(self, idx, targets, ignore_index: int = -100, reduction: str = "mean"):
-        """The cross entropy of forward(idx, targets) without its logits: on the
-        HIP path they are never in memory (linear_cross_entropy). reduction
+        """The cross entropy of forward(idx, targets) without its logits
+        (linear_cross_entropy, on the HIP path). reduction
         "none": one loss per token (the tokens' negative log-probabilities)."""
         h = self._hidden(self.tok(idx), [None] * len(self.blocks))
         if self._head_fused(h):

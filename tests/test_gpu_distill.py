@@ -93,6 +93,24 @@ def test_rows_of_any_length_and_alignment(vocab, offset, dtype):
     _check("transposed", got3, z, values, ids, 1.0, up, "mean", TYPES[dtype])
 
 
+def test_logits_past_32_bits():
+    """More than 2^31 logits: the last rows against 64 bits."""
+    rows, vocab, last = 66000, 32769, 50
+    z, values, ids = _case(last, vocab, 20, torch.bfloat16)
+    large = torch.zeros(rows, vocab, dtype=torch.bfloat16, device=DEV)
+    large[-last:] = z
+    all_ids = torch.zeros(rows, 20, dtype=torch.int64, device=DEV)
+    all_ids[-last:] = ids
+    all_values = torch.zeros(rows, 20, device=DEV)
+    all_values[-last:] = values
+    up = torch.randn(rows, generator=_gen(3), device=DEV)
+    got = _run(large, all_values, all_ids, up, temperature=2.0, reduction="none")
+    # (Not bit for bit a small call's: a row's sums begin at its first 16-byte boundary,
+    # and its first element lies (rows - last) 32769 mod 8 = 6 elements off one here.)
+    _check("last rows", (got[0][-last:], got[1][-last:]), z, values, ids, 2.0, up[-last:], "none",
+           torch.bfloat16)
+
+
 def test_large_and_masked_logits():
     z, values, ids = _case(20, 3000, 8, torch.float32, spread=100.0)
     up = torch.ones((), device=DEV)

@@ -10,7 +10,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from head_reference import assert_head, assert_within
+from head_reference import UNIT, assert_head, assert_within, sum_error
 from mamba_metal_scan_amd import _native, linear_cross_entropy, linear_distill_loss
 from mamba_metal_scan_amd._native import HipScanError
 
@@ -140,12 +140,13 @@ def test_gradients_of_peaked_rows(dtype, keep, monkeypatch):
     fp32's exponents."""
     _keep(monkeypatch, keep)
     h, w, t = _operands(140, 64, 700, TYPES[dtype], spread=60.0)
-    for factor in (1.0, 2.0 ** -40, 2.0 ** 40):
-        if dtype == "f16" and factor != 1.0:
+    spread = torch.linspace(-60, 60, 140, device=DEV).exp2()   # from row to row
+    for factor in (None, 2.0 ** -40, 2.0 ** 40, spread):
+        if dtype == "f16" and factor is not None:
             continue   # (the gradients are no fp16 numbers)
-        up = factor * _upstream(140, "none")
+        up = _upstream(140, "none") * (1.0 if factor is None else factor)
         got = _run(linear_cross_entropy, h, w, up, t, reduction="none")
-        assert_head(f"upstream {factor}", got, h, w, up, "none", TYPES[dtype], targets=t)
+        assert_head("upstream", got, h, w, up, "none", TYPES[dtype], targets=t)
 
 
 @pytest.mark.parametrize("keep", [True, False])
@@ -526,6 +527,39 @@ def test_op_argument_errors():
         ops.linear_distill_fwd(h, w, values, ids, 0.0, 1)
     with pytest.raises(HipScanError, match="teacher_logits"):
         ops.linear_distill_fwd(h, w, values[:, :3].contiguous(), ids, 1.0, 1)
+
+
+@pytest.mark.parametrize("rows,dtype,keep", [(4, "bf16", True), (40, "bf16", False),
+                                             (40, "bf16", True), (4, "f32", False)])
+def test_weights_past_32_bits(rows, dtype, keep, monkeypatch):
+    """A weight of more than 2^31 elements whose words but the last 1000 are out of
+    reach (their probabilities are 0 exactly): the small weight's results."""
+    print(f"[case] large weight {rows} {dtype} {keep}", flush=True)
+    _keep(monkeypatch, keep)
+    dim, vocab, last = 1032, (1 << 21) + 3, 1000
+    h, w, t = _operands(rows, dim, last, TYPES[dtype])
+    h[:, 0], w[:, 0] = 1.0, 0.0
+    up = _upstream(rows, "none")
+    want = _run(linear_cross_entropy, h, w, up, t, reduction="none")
+    large = torch.zeros(vocab, dim, dtype=TYPES[dtype], device=DEV)
+    large[:, 0] = -1024.0
+    large[-last:] = w
+    got = _run(linear_cross_entropy, h, large, up, torch.where(t < 0, t, t + vocab - last),
+               reduction="none")
+    assert (got[2][:-last] == 0).all()
+    # The sums' order differs: of the logits by the small bound, dh's by its rounding.
+    z = sum_error(dim) * (h.double().abs() @ w.double().abs().t())
+    p = 2 * z.amax(1) + 2.0 ** -16
+    assert_within("loss", got[0], want[0], p + 2.0 ** -20 * want[0].double().abs())
+    unit = 2 * max(UNIT[TYPES[dtype]], 2.0 ** -20)
+    dz = up.double().abs()[:, None] * (2 * p[:, None] + unit) * torch.ones_like(z)
+    assert_within("dW", got[2][-last:], want[2],
+                  dz.t() @ h.double().abs() + unit * want[2].double().abs())
+    z = h.double() @ w.double().t()
+    q = z.softmax(1)
+    q[torch.arange(rows, device=DEV), t.clamp(min=0)] += 1.0
+    assert_within("dh", got[1], want[1], (q * dz) @ w.double().abs()
+                  + unit * want[1].double().abs())
 
 
 def test_matches_the_logits_loss():
