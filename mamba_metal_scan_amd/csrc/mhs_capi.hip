@@ -41,7 +41,7 @@ MHS_FOR_PLANS(MHS_BWD_ATOM_INST, extern, 2)
 
 namespace {
 
-constexpr int kVersion = (0 << 16) | (7 << 8) | 0;   // 0.7: quad-broadcast B/C and DPP partner products in the backward
+constexpr int kVersion = (0 << 16) | (8 << 8) | 0;   // 0.8: losses of the head from hidden states, distillation
 
 thread_local char g_err[512] = "";
 

@@ -677,9 +677,14 @@ __device__ __forceinline__ float lift_of(float largest, int to) {
 
 constexpr int kCopyRows = 8;   // rows per block
 
-// scale[0..1] = (s, 1 / s), dz's power of two (lift_of to `lift`, scale[2] the largest
-// per-row gradient; lift 0: 1); rows2[r] = (coef s, lse2); and, `out` given, out
-// (out_rows, per) = in (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
+// What dz is stored with and what the products' sums are multiplied by. s is dz's
+// power of two (lift_of to `lift`, scale[2] the largest per-row gradient; lift 0:
+// 1). Where all rows share their coef = 2^e f, f in [1, 2), dz is stored with its
+// 2^e alone and the sums take f: stored with coef, the id's element, about -coef,
+// would be off by the same rounding in every row (errors relative to the gradients'
+// norm: fp16 1001 x 384 x 50257 0.00030 to 0.00032, so 0.00025, of which 0.00021 is
+// the results' own rounding; bf16 8192 x 4096 x 131072 0.0025, so 0.0019, and 0.0017). rows2[r] = (2^e s, or
+// the row's coef s, lse2); scale[0] = f / s; and, `out` given, out (out_rows, per) = in (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
 // `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
 // reach dW.
 template <int UNUSED = 0>
@@ -692,15 +697,16 @@ head_rows_in_kernel(const uint4* __restrict__ in, long long ldi, RowScale rs,
   const long long r0 = (long long)blockIdx.x * kCopyRows;
   if (threadIdx.x < kCopyRows) {
     // (without per-row gradients the largest is the one that every kept row has)
-    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : fabsf(rs.reaching(0)), lift);
+    const float all = rs.per_row ? 1.f : fabsf(rs.reaching(0));
+    const float s = !lift ? 1.f : lift_of(rs.per_row ? scale[2] : all, lift);
+    int e = 0;
+    const float f = all > 0.f && all < INFINITY ? 2.f * frexpf(all, &e) : 1.f;
     const long long r = r0 + threadIdx.x;
     const float c = r < rows ? rs.at(r) : 0.f;
     cf[threadIdx.x] = c;
-    if (r < ((rows + 1) & ~1LL)) rows2[r] = make_float2(c * s, r < rows ? lse2[r] : 0.f);
-    if (r == 0) {
-      scale[0] = s;
-      scale[1] = 1.f / s;
-    }
+    // (c / f: a power of two, exactly)
+    if (r < ((rows + 1) & ~1LL)) rows2[r] = make_float2(c / f * s, r < rows ? lse2[r] : 0.f);
+    if (r == 0) scale[0] = f / s;
   }
   if (!out) return;
   __syncthreads();
@@ -723,7 +729,7 @@ head_zero_kernel(unsigned* __restrict__ out, long long n) {
 
 struct HeadGrad {
   const float2* rows2;     // (rows, to an even number) (coef s, lse2)
-  const float* scale;      // [s, 1 / s]
+  const float* scale;      // what the sums are multiplied by
   const long long* ids;    // (rows, k)
   const float* q;          // (rows, k) the words' whole weights, or null: 1
   const float* picked;     // (rows, k)
@@ -902,7 +908,7 @@ head_ids_kernel(HeadGrad a, long long rows, int words) {
 }
 
 // What becomes of a 16-bit product: fp32 sums of split blockIdx.y (overwritten,
-// or added to for later pieces), or the rounded result times scale[1]; transposed,
+// or added to for later pieces), or the rounded result times scale[0]; transposed,
 // so that a lane's neighbouring rows are neighbours in memory.
 struct MmOut {
   float* part;          // (splits, N, ldo), or null
@@ -931,7 +937,7 @@ head_mm_kernel(MmArgs g, MmOut o) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int mb = tm * S::BM + S::wave_m(wave) * (S::FM * 16);
   const int nb = tn * S::BN + S::wave_n(wave) * (S::FN * 16) + (lane & 15);
-  const float scale = o.part ? 1.f : o.scale[1];
+  const float scale = o.part ? 1.f : o.scale[0];
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
     const int n = nb + 16 * j;
@@ -970,7 +976,7 @@ head_mm_kernel(MmArgs g, MmOut o) {
   }
 }
 
-// out (M, 4 N4) = scale[1] times the sum of the splits' sums, in order, rounded;
+// out (M, 4 N4) = scale[0] times the sum of the splits' sums, in order, rounded;
 // rows2 given, rows whose coef is 0 are zeros.
 template <class T>
 __global__ void __launch_bounds__(256)
@@ -978,7 +984,7 @@ head_mm_reduce_kernel(const float4* __restrict__ part, ushort4* __restrict__ out
                       const float* __restrict__ scale, const float2* __restrict__ rows2,
                       int splits, long long M, int N4) {
   const long long n = M * N4;
-  const float f = scale[1];
+  const float f = scale[0];
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
        i += (long long)gridDim.x * 256) {
     float4 s = part[i];

@@ -610,12 +610,12 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogit
     if (out.dhidden &&
         (rc = mhs::gemm_f32(MHS_GEMM_TN, dz, b.ldz, w + v0 * p.ldw, p.ldw,
                             static_cast<float*>(out.dhidden), p.dim, p.rows, p.dim, words, v0 > 0,
-                            a.scale + 1, part, part_bytes, s)) != 0)
+                            a.scale, part, part_bytes, s)) != 0)
       return rc;
     if (out.dweight &&
         (rc = mhs::gemm_f32(MHS_GEMM_NN, dz, b.ldz, hz, p.dim,
                             static_cast<float*>(out.dweight) + v0 * p.dim, p.dim, words, p.dim,
-                            b.rows4, 0, a.scale + 1, part, part_bytes, s)) != 0)
+                            b.rows4, 0, a.scale, part, part_bytes, s)) != 0)
       return rc;
   }
   return MHS_OK;
