@@ -120,12 +120,13 @@ struct MmOperand {
   unsigned frag;                               // byte offset of the lane's first fragment
 
   // Chunk c (16 bytes) of row r (K-major) or k row r lies at place c ^ swz(r).
-  // K-major: the 8 (and 16) lanes of one pass of a 16-byte read, on consecutive
-  // rows of 128 bytes, then hit different banks; row-major: the k rows that one
-  // pass of the transposing reads meets (4 in a row and those 8 further) do.
+  // K-major: the 16 lanes of a pass of a 16-byte read, lanes 0-3, 12-15 and 20-27
+  // (rows of 128 bytes, the last eight a chunk further) or their like, then hit all
+  // 64 banks, and so do 16 neighbours; row-major: the k rows that one pass of the
+  // transposing reads meets (4 in a row and those 8 further) do.
   // SQ_LDS_BANK_CONFLICT is 0.
   static __device__ __forceinline__ constexpr int swz(int r) {
-    return KMAJOR ? (r & 7) ^ ((r >> 3) & 1) : ((r & 3) << 2) ^ ((r >> 3) & 1) << 1;
+    return KMAJOR ? (r >> 1) & 7 : ((r & 3) << 2) ^ ((r >> 3) & 1) << 1;
   }
 
   // wrow: the wave's first row within the tile.
