@@ -297,6 +297,25 @@ AUDIT = [
     ("decode_state_kernel<4>", "token, state update and gate", None, 4, 0),
     ("xent_fwd_kernel<0>", "loss forward", None, 4, 0),
     ("xent_bwd_kernel<true>", "loss backward", None, 4, 0),
+    ("head_lse_kernel<Bf16, MmShape<256, 256, 2, 4>, false>", "head's losses, forward product",
+     "bytes", 8, 135168),
+    ("head_lse_kernel<Bf16, MmShape<256, 256, 2, 4>, true>", "the same, logits kept", "bytes", 8,
+     135168),
+    ("head_dz_kernel<Bf16, MmShape<256, 256, 2, 4> >", "gradient of the logits", "bytes", 8,
+     135168),
+    ("head_mm_kernel<Bf16, MmShape<256, 256, 2, 4>, false, true>",
+     "gradient of the hidden states", "bytes", 8, 131072),
+    ("head_mm_kernel<Bf16, MmShape<256, 256, 2, 4>, false, false>", "gradient of the weight",
+     "bytes", 8, 131072),
+    ("head_mm_kernel<Bf16, MmShape<256, 256, 2, 4>, true, true>", "logits of few tiles", "bytes",
+     8, 131072),
+    ("head_lse3_kernel<128>", "fp32 forward product", "gemm", 4, 128),
+    ("head_lse3_kernel<64>", "the same, up to 64 rows", "gemm", 4, 64),
+    ("head_dz3_kernel<128>", "fp32 gradient of the logits", "gemm", 4, 128),
+    ("head_small_kernel<Bf16, 1>", "forward product of few rows", "bytes", 4, 16896),
+    ("head_small_kernel<Fp32, 2>", "the same, fp32, 17 to 32 rows", "bytes", 4, 33792),
+    ("distill_fwd_kernel<Fp32>", "distillation of logits, forward", None, 4, 0),
+    ("distill_bwd_kernel<Fp32>", "distillation of logits, backward", None, 4, 0),
 ]
 
 
@@ -312,6 +331,7 @@ def resource_table(usage: dict) -> list:
             raise KeyError(f"no kernel {prefix} in the library's resource remarks")
         r = usage[hits[0]]
         lds = (gemm_lds_bytes(npl) if kind == "gemm"   # npl: the tile
+               else npl if kind == "bytes"
                else scan_lds_bytes(kind, waves_per_block, npl) if kind else 0)
         lds_waves = (f"{(LDS_PER_CU // lds) * waves_per_block // 4}" if lds else "-")
         out.append(f"| `{prefix}` | {what} | {r['VGPRs']} | {r['AGPRs']} | {r['TotalSGPRs']} | "
