@@ -1295,19 +1295,15 @@ def _saved_size(rows: int, *tops: int) -> int:
     return 4 + rows * (3 + sum(tops))
 
 
-KEPT_BYTES = 1 << 30
-
-
-def keeps_logits(rows: int, vocab: int, dim: int, dtype: torch.dtype) -> bool:
-    """Whether a forward that has a backward keeps its fp32 logits for it, up to
-    1 GB of them: three products instead of four, against writing and reading
+def keeps_logits(rows: int, vocab: int, dim: int, dtype: torch.dtype, most: int) -> bool:
+    """Whether a forward that has a backward keeps its fp32 logits for it, `most`
+    bytes of them or fewer: three products instead of four, against writing and reading
     them. us of the loss and its gradients, formed twice and kept: fp32 512 x 256
     x 32768 266 and 243, 512 x 4096 x 131072 11420 and 8770; bf16 by the rows, 128
     x 640 x 32768 149 and 138, 256 152 and 150, 512 174 and 181, 2048 409 and 575,
     but with 1024 columns 512 x 50257 335 either way, with 2048 563 and 510, with
     4096 512 x 131072 2370 and 2040."""
-    return rows * vocab * 4 <= KEPT_BYTES and (dtype == torch.float32 or rows <= 256
-                                               or dim >= 2048)
+    return rows * vocab * 4 <= most and (dtype == torch.float32 or rows <= 256 or dim >= 2048)
 
 
 def _kept_size(hidden: torch.Tensor, weight: torch.Tensor) -> int:

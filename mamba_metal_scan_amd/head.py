@@ -7,9 +7,10 @@ words) 1.07 GB of fp32 logits and as much again for their gradient.
 hidden states and the head's weight, the logits formed tile by tile on the
 matrix cores: the forward reduces each tile to its rows' maxima and sums of
 exponentials, the backward forms the tiles again, a piece of the vocabulary at a
-time, and multiplies their gradient with the weight and the hidden states. Up to
-1 GB of fp32 logits the forward keeps for the backward instead, where that is the
-faster (``_native.keeps_logits``); without a backward it keeps none.
+time, and multiplies their gradient with the weight and the hidden states. Of
+logits that take no more than ``logits_bytes`` (1 GB by default, 0: none) the forward
+keeps the fp32 values for the backward, where that is the faster; without a
+backward it keeps none.
 
 ``distill_loss`` is the distillation of given logits from a teacher's top words,
 ``linear_distill_loss`` the same from the hidden states.
@@ -37,8 +38,12 @@ def _cut(g: torch.Tensor, dim: int) -> torch.Tensor:
     return g if g.shape[1] == dim else g[:, :dim].contiguous()
 
 
-def _keeps(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
-    return _native.keeps_logits(hidden.shape[0], weight.shape[0], hidden.shape[1], hidden.dtype)
+LOGITS_BYTES = 1 << 30   # of fp32 logits that a forward may keep, unless told otherwise
+
+
+def _keeps(hidden: torch.Tensor, weight: torch.Tensor, most: int) -> bool:
+    return _native.keeps_logits(hidden.shape[0], weight.shape[0], hidden.shape[1], hidden.dtype,
+                                most)
 
 
 def _once() -> None:
@@ -59,22 +64,22 @@ class LinearCrossEntropyHIP(torch.autograd.Function):
     int64; rows with target == ignore_index excluded."""
 
     @staticmethod
-    def loss(hidden, weight, targets, ignore_index, reduction, backward=False):
+    def loss(hidden, weight, targets, ignore_index, reduction, most, backward=False):
         """(loss, what the backward needs)."""
         hidden, weight = _rows16(hidden), _rows16(weight)
         targets = targets.contiguous()
         if not torch.compiler.is_compiling():   # (the registered op checks itself)
             _native._check_linear_xent("linear_cross_entropy", hidden, weight, targets, reduction)
         loss, saved = dispatch("linear_xent_fwd")(hidden, weight, targets, ignore_index, reduction,
-                                                  backward and _keeps(hidden, weight))
+                                                  backward and _keeps(hidden, weight, most))
         return loss, (hidden, weight, targets, saved)
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction, most):
         ctx.dim = hidden.shape[1]
         ctx.reduction = reduction
         loss, saved = LinearCrossEntropyHIP.loss(hidden, weight, targets, ignore_index, reduction,
-                                                 any(ctx.needs_input_grad))
+                                                 most, any(ctx.needs_input_grad))
         ctx.save_for_backward(*saved)
         return loss
 
@@ -84,7 +89,7 @@ class LinearCrossEntropyHIP(torch.autograd.Function):
         hidden, weight, targets, saved = ctx.saved_tensors
         return (*_grads(ctx, *dispatch("linear_xent_bwd")(
             g.contiguous(), hidden, weight, targets, saved, ctx.reduction,
-            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None)
+            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None, None)
 
 
 class LinearDistillHIP(torch.autograd.Function):
@@ -92,7 +97,7 @@ class LinearDistillHIP(torch.autograd.Function):
     ids (R, K) and their logits."""
 
     @staticmethod
-    def loss(hidden, weight, teacher_logits, ids, temperature, reduction, backward=False):
+    def loss(hidden, weight, teacher_logits, ids, temperature, reduction, most, backward=False):
         """(loss, what the backward needs)."""
         hidden, weight = _rows16(hidden), _rows16(weight)
         if not torch.compiler.is_compiling():
@@ -100,15 +105,15 @@ class LinearDistillHIP(torch.autograd.Function):
                                           ids, temperature, reduction)
         loss, saved = dispatch("linear_distill_fwd")(hidden, weight, teacher_logits, ids,
                                                      temperature, reduction,
-                                                     backward and _keeps(hidden, weight))
+                                                     backward and _keeps(hidden, weight, most))
         return loss, (hidden, weight, ids, saved)
 
     @staticmethod
-    def forward(ctx, hidden, weight, teacher_logits, ids, temperature, reduction):
+    def forward(ctx, hidden, weight, teacher_logits, ids, temperature, reduction, most):
         ctx.dim = hidden.shape[1]
         ctx.temperature, ctx.reduction = temperature, reduction
         loss, saved = LinearDistillHIP.loss(hidden, weight, teacher_logits, ids, temperature,
-                                            reduction, any(ctx.needs_input_grad))
+                                            reduction, most, any(ctx.needs_input_grad))
         ctx.save_for_backward(*saved)
         return loss
 
@@ -118,7 +123,7 @@ class LinearDistillHIP(torch.autograd.Function):
         hidden, weight, ids, saved = ctx.saved_tensors
         return (*_grads(ctx, *dispatch("linear_distill_bwd")(
             g.contiguous(), hidden, weight, ids, saved, ctx.temperature, ctx.reduction,
-            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None, None)
+            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None, None, None)
 
 
 class DistillHIP(torch.autograd.Function):
@@ -166,6 +171,12 @@ def _reduction(what: str, reduction: str) -> int:
     return REDUCE[reduction]
 
 
+def _bytes(what: str, n: int) -> int:
+    if not isinstance(n, int) or n < 0:
+        raise ValueError(f"{what}: logits_bytes must be an integer of at least 0; got {n!r}")
+    return n
+
+
 def _hip(what: str, *ts: torch.Tensor) -> None:
     if torch.version.hip is None or not all(t.is_cuda for t in ts):
         raise RuntimeError(f"{what} needs its tensors on the ROCm device; got "
@@ -211,7 +222,8 @@ def _teacher(what: str, lead: torch.Size, teacher_logits: torch.Tensor,
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
-                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+                         ignore_index: int = -100, reduction: str = "mean",
+                         logits_bytes: int = LOGITS_BYTES) -> torch.Tensor:
     """``F.cross_entropy(hidden @ weight.T, targets, ignore_index=ignore_index,
     reduction=reduction)`` without the logits: hidden (..., D) and weight (V, D)
     in float32, bfloat16 or float16 on one ROCm device, targets (...) integers.
@@ -219,8 +231,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     The loss is float32: a scalar, or with reduction "none" one per row, of
     targets' shape (0 where ignored). Rows that are ignored add nothing to the
     gradients, whatever they hold. A target outside [0, V) that is not
-    ignore_index makes its row's loss NaN. Between forward and backward it may hold
-    up to 1 GB of the logits (``_native.keeps_logits``). Under autocast hidden and weight are
+    ignore_index makes its row's loss NaN. Up to logits_bytes of fp32 logits (rows x
+    V x 4) may be kept from forward to backward, where that is the faster; 0 keeps
+    none. Under autocast hidden and weight are
     taken in its type. The gradients are once differentiable."""
     what = "linear_cross_entropy"
     _hip(what, hidden, weight, targets)
@@ -231,16 +244,17 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
                          f"got {targets.dtype} {tuple(targets.shape)}")
     h, w = _head(what, hidden, weight)
     loss = _apply(LinearCrossEntropyHIP, 2, h, w, targets.to(torch.int64).reshape(-1),
-                  int(ignore_index), red)
+                  int(ignore_index), red, _bytes(what, logits_bytes))
     return loss if red else loss.view(targets.shape)
 
 
 def linear_distill_loss(hidden: torch.Tensor, weight: torch.Tensor,
                         teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
-                        temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
-    """``distill_loss(hidden @ weight.T, ...)`` without the logits: hidden (..., D)
-    and weight (V, D) as linear_cross_entropy takes them, teacher_logits and
-    teacher_ids (..., K)."""
+                        temperature: float = 1.0, reduction: str = "mean",
+                        logits_bytes: int = LOGITS_BYTES) -> torch.Tensor:
+    """``distill_loss(hidden @ weight.T, ...)`` without the logits: hidden (..., D),
+    weight (V, D) and logits_bytes as linear_cross_entropy takes them,
+    teacher_logits and teacher_ids (..., K)."""
     what = "linear_distill_loss"
     _hip(what, hidden, weight, teacher_logits, teacher_ids)
     red = _reduction(what, reduction)
@@ -248,7 +262,7 @@ def linear_distill_loss(hidden: torch.Tensor, weight: torch.Tensor,
     lead = hidden.shape[:-1]
     t, ids = _teacher(what, lead, teacher_logits, teacher_ids, temperature)
     h, w = _head(what, hidden, weight)
-    loss = _apply(LinearDistillHIP, 2, h, w, t, ids, temperature, red)
+    loss = _apply(LinearDistillHIP, 2, h, w, t, ids, temperature, red, _bytes(what, logits_bytes))
     return loss if red else loss.view(lead)
 
 

@@ -121,6 +121,27 @@ def test_logits_kept_or_formed_again(rows, dim, vocab, dtype, keep, monkeypatch)
     assert_head("distill", got, h, w, up, "mean", TYPES[dtype], words=(values, ids, 2.0))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bytes_of_logits_kept(dtype):
+    """What a loss holds until its backward: the logits, or none of them."""
+    h, w, t = _operands(200, 64, 40000, TYPES[dtype])
+    up = torch.ones((), device=DEV)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    held, grads = [], []
+    for most in (0, 200 * 40000 * 4 - 1, 200 * 40000 * 4):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(a, b, t, logits_bytes=most)
+        held.append(torch.cuda.memory_allocated() - before)
+        grads.append(torch.autograd.grad(loss, [a, b], up))
+        del loss
+        assert_head(f"{most}", (linear_cross_entropy(h.detach(), w.detach(), t), *grads[-1]),
+                    h.detach(), w.detach(), up, "mean", TYPES[dtype], targets=t)
+    assert held[0] < 1 << 20 and held[1] < 1 << 20 and held[2] >= 200 * 40000 * 4
+    for x, y in zip(grads[0], grads[1]):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_kept_logits_of_a_backward_twice(dtype, monkeypatch):
     """The backward leaves what the forward kept as it was."""
@@ -498,6 +519,31 @@ def test_on_another_stream_and_captured():
                 assert torch.equal(x, y)
             _run(linear_cross_entropy, *sets[1][:2], up, sets[1][2])
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_calls_at_once(dtype):
+    """Two threads, each on a stream of its own, with operands of their own."""
+    from concurrent.futures import ThreadPoolExecutor
+    sets = [_operands(rows, 128, vocab, TYPES[dtype], seed=rows)
+            for rows, vocab in ((40, 3000), (300, 1100))]
+    up = torch.ones((), device=DEV)
+    want = [_run(linear_cross_entropy, h, w, up, t) for h, w, t in sets]
+    torch.cuda.synchronize()
+
+    def work(i):
+        h, w, t = sets[i]
+        stream = torch.cuda.Stream()
+        out = []
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                out.append(_run(linear_cross_entropy, h, w, up, t))
+        stream.synchronize()
+        return out
+    with ThreadPoolExecutor(2) as pool:
+        for i, out in enumerate(pool.map(work, range(2))):
+            for got in out:
+                assert all(torch.equal(x, y) for x, y in zip(got, want[i]))
 
 
 def test_op_argument_errors():

@@ -43,6 +43,8 @@ def test_shapes_and_types_are_checked(monkeypatch):
     for args, kw, match in (
             ((h, w, t[:3]), {}, "targets"), ((h, w, t.float()), {}, "targets"),
             ((h, w, t), {"reduction": "avg"}, "reduction"),
+            ((h, w, t), {"logits_bytes": -1}, "logits_bytes"),
+            ((h, w, t), {"logits_bytes": 1e9}, "logits_bytes"),
             ((h, torch.zeros(5, 9), t), {}, "weight"), ((h, torch.zeros(0, 8), t), {}, "empty"),
             ((torch.zeros(4, 0), torch.zeros(5, 0), t), {}, "empty"),
             ((h, w.double(), t), {}, "float32, bfloat16"),
@@ -164,12 +166,14 @@ def test_workspace_sizes():
 
 def test_rule_of_kept_logits():
     """At most 1 GB of them; of 16-bit operands where that saves time."""
-    keeps = _native.keeps_logits
+    def keeps(*a, most=1 << 30):
+        return _native.keeps_logits(*a, most)
     f, b = torch.float32, torch.bfloat16
     assert keeps(8192, 32768, 640, f) and not keeps(8193, 32768, 640, f)
     assert keeps(256, 32768, 640, b) and not keeps(257, 32768, 640, b)
     assert keeps(2048, 131072, 2048, b) and not keeps(2049, 131072, 2048, b)
-    assert keeps(0, 5, 8, f)
+    assert keeps(0, 5, 8, f) and not keeps(1, 5, 8, f, most=0)
+    assert keeps(4, 5, 8, f, most=80) and not keeps(4, 5, 8, f, most=79)
 
 
 def test_fake_ops_have_the_kernels_shapes():
