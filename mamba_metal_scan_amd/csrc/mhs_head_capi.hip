@@ -33,9 +33,8 @@ typedef mhs::MmShape<256, 256, 2, 4> Shape;
 // 62 and 54 with 2048 x 50257 and 282 and 239 with 4096 x 131072.
 constexpr int64_t small_rows(int elem) { return elem == 4 ? 32 : 16; }
 // Bytes of dz that the backward holds at a time (at least 256 words' worth). us
-// with 64, 128, 256 and 512 MB: 8192 x 640 x 32768 bf16 2550, 1780, 1559, 1589;
-// 8192 x 4096 x 131072 29520, 27080, 26130, 25700; fp32 (the first) 8640, 7755,
-// 7407, 7257.
+// with 64, 128, 256 and 512 MB: 8192 x 640 x 32768 bf16 1620, 1488, 1446, 1467, fp32
+// 7226, 6400, 6126, 6014; 8192 x 4096 x 131072 27300, 26300, 26100, 25970.
 constexpr int64_t kPieceBytes = 256LL << 20;
 // Rows that one block sums. (us with one block and with blocks of 4096 rows and a
 // last one, behind a kernel of one block per row: 4096 rows 32.7 and 34.9, 8192 56.6
