@@ -302,7 +302,7 @@ AUDIT = [
     ("head_lse_kernel<Bf16, MmShape<256, 256, 2, 4>, true>", "the same, logits kept", "bytes", 8,
      135168),
     ("head_dz_kernel<Bf16, MmShape<256, 256, 2, 4> >", "gradient of the logits", "bytes", 8,
-     135168),
+     137216),
     ("head_mm_kernel<Bf16, MmShape<256, 256, 2, 4>, false, true>",
      "gradient of the hidden states", "bytes", 8, 131072),
     ("head_mm_kernel<Bf16, MmShape<256, 256, 2, 4>, false, false>", "gradient of the weight",

@@ -762,31 +762,32 @@ __device__ __forceinline__ void exchange4(unsigned (&v)[4]) {
 // 131072 6731 us in eight (1307). The tile has the words in m, dz
 // the rows: a lane's 4 words of 4 fragments become 16 of one row (exchange4), in
 // two stores of 16 bytes, each 64 bytes of 16 rows at a time; no LDS.
+constexpr int kPairBytes = 2048;   // of LDS per slot: 256 rows' (coef, lse2)
 template <class T, class S>
 __global__ void __launch_bounds__(S::kThreads, 2)
 head_dz_kernel(MmArgs g, HeadGrad a) {
   extern __shared__ float lds_f[];
-  // Two tiles' rows' (coef, lse2).
-  static_assert(S::BN == 256, "two direct loads hold a tile's rows");
+  // The rows' (coef, lse2) of the stream's slots.
+  static_assert(S::BN * 8 == kPairBytes, "two direct loads hold a tile's rows");
   char* const pairs = reinterpret_cast<char*>(lds_f) + S::kLds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = S::wave_m(wave), wn = S::wave_n(wave);
-  const auto load_pairs = [&](int n0, int odd) {
+  const auto load_pairs = [&](int n0, int slot) {
     if (wave >= 2) return;
     const int at = 128 * wave + 2 * (int)(threadIdx.x & 63);   // 2 rows a lane
     mm_load_lds(mm_resource(a.rows2 + n0), at < g.N - n0 ? 8u * (unsigned)at : kOOB,
                 (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)pairs +
-                    2048 * odd + 1024 * wave);
+                    kPairBytes * slot + 1024 * wave);
   };
   mm_stream<T, S>(g, reinterpret_cast<char*>(lds_f), load_pairs, [&](auto& acc, int m0, int n0,
-                                                                    int odd) {
+                                                                    int slot) {
     const int lane = mm_opaque(threadIdx.x & 63);
     m0 += wm * (S::FM * 16);
     const int left = g.M - m0 - 32 * (lane >> 5) - 4 * ((lane >> 4) & 1);
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
       const int in = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + in;
-      const float2 row2 = *reinterpret_cast<const float2*>(pairs + 2048 * odd + 8 * in);
+      const float2 row2 = *reinterpret_cast<const float2*>(pairs + kPairBytes * slot + 8 * in);
       const float f = row2.x, l2 = row2.y;
       unsigned short* const row = static_cast<unsigned short*>(a.dz) + (long long)n * a.ldz + m0 +
                                   8 * (lane >> 4);

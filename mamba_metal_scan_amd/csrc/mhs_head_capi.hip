@@ -531,7 +531,7 @@ int bwd16(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogit
   const auto fz = &mhs::head_dz_kernel<T, Shape>;
   const auto fh = &mhs::head_mm_kernel<T, Shape, false, true>;
   const auto fw = &mhs::head_mm_kernel<T, Shape, false, false>;
-  constexpr int lds_z = Shape::kLds + 2 * 2048;
+  constexpr int lds_z = Shape::kLds + mhs::kMmSlots * mhs::kPairBytes;
   allow_lds(fz, lds_z);
   allow_lds(fh, Shape::kLds);
   allow_lds(fw, Shape::kLds);

@@ -104,6 +104,11 @@ __device__ __forceinline__ constexpr int mm_perm(int x) {
 
 constexpr int kMmK = 64;        // k's of a k tile
 constexpr int kMmStages = 2;    // k tiles in LDS
+// What a stream's tiles have beside their k tiles (mm_stream's side) lies in as many
+// slots, a tile's number modulo them. The loads run kMmStages k tiles ahead: of tiles
+// of a single k tile as many whole tiles, whose sides come in before the epilogue of
+// the tile at hand has read its own.
+constexpr int kMmSlots = kMmStages + 1;
 
 // One operand of a block of WAVES waves: R rows from r0 of `rows`. PERM: its rows
 // lie in LDS in mm_perm's order (K-major).
@@ -320,7 +325,10 @@ __device__ __forceinline__ int mm_opaque(int v) {
 // The tiles blockIdx.x, + gridDim.x, ... of a product of two K-major operands as
 // one stream of k tiles: the direct loads run on into the next tile while this
 // one's last k tiles are multiplied and while epi(acc, m0, n0) works on its sums
-// (without the stages' LDS), so that only the first tile waits for memory. A's rows
+// (without the stages' LDS), so that only the first tile waits for memory. side(n0,
+// slot) issues direct loads into a slot when a tile's own loads begin, epi(acc, m0, n0,
+// slot) reads it: between a slot's last reads and its next loads lies a k tile's
+// barrier, from one tile to the third after it at least one (kMmSlots). A's rows
 // lie in mm_perm's order: a fragment's element e of lane l in fragment i is row
 // 64 (i / 4) + 32 (l / 32) + 8 (i % 4) + 4 (l / 16 % 2) + e of the wave's.
 template <class T, class S, class Side, class Epi>
@@ -328,6 +336,7 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
                                           const Epi& epi) {
   constexpr int FM = S::FM, FN = S::FN, ST = kMmStages, PH = kMmK / 32;
   static_assert(ST == 2, "every k tile waits for all loads before it: side's too");
+  static_assert(kMmSlots > ST, "a slot for every tile that loads run ahead, and the one at hand");
   static_assert(PH % 2 == 0 && FM % 4 == 0, "the shape streams");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -338,7 +347,7 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
   const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
   const int tiles = g.grid_m * g.grid_n, nk = (g.K + kMmK - 1) / kMmK;
   // Where the loads are: k tile load_kt of tile load_tile.
-  int load_tile = blockIdx.x, load_kt = 0, load_odd = 0, tm, tn;
+  int load_tile = blockIdx.x, load_kt = 0, load_slot = 0, tm, tn;
   mm_tile(g, load_tile, tm, tn);
   OA a(g.A, g.lda, tm * S::BM, g.M, 0, wave, lane, S::wave_m(wave) * (FM * 16));
   OB b(g.B, g.ldb, tn * S::BN, g.N, 0, wave, lane, S::wave_n(wave) * (FN * 16));
@@ -348,13 +357,13 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
     if (load_kt == nk) {
       load_kt = 0;
       load_tile += gridDim.x;
-      load_odd ^= 1;
+      load_slot = load_slot == kMmSlots - 1 ? 0 : load_slot + 1;
       if (load_tile < tiles) {
         mm_tile(g, load_tile, tm, tn);
         const int l = mm_opaque(lane);
         a.place(g.A, g.lda, tm * S::BM, g.M, 0, wave, l);
         b.place(g.B, g.ldb, tn * S::BN, g.N, 0, wave, l);
-        side(tn * S::BN, load_odd);
+        side(tn * S::BN, load_slot);
       }
     }
     ra = a.next();
@@ -376,8 +385,9 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
   for (int i = 0; i < FM; ++i) fa[0][i] = a.read(lds, i, 0);
 #pragma unroll
   for (int j = 0; j < FN; ++j) fb[0][j] = b.read(lds + TA, j, 0);
-  int cur = 0, odd = 0;   // the buffer of the k tile; the tile's side
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, odd ^= 1) {
+  int cur = 0, slot = 0;   // the buffer of the k tile; the tile's slot
+  for (int tile = blockIdx.x; tile < tiles;
+       tile += gridDim.x, slot = slot == kMmSlots - 1 ? 0 : slot + 1) {
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -419,7 +429,7 @@ __device__ __forceinline__ void mm_stream(const MmArgs& g, char* lds, const Side
     }
     int em, en;
     mm_tile(g, tile, em, en);
-    epi(acc, em * S::BM, en * S::BN, odd);
+    epi(acc, em * S::BM, en * S::BN, slot);
   }
   mm_wait<0>();   // (no load may outlive the block)
 }
