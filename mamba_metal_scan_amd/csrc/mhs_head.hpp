@@ -727,6 +727,19 @@ head_zero_kernel(unsigned* __restrict__ out, long long n) {
     out[i] = 0u;
 }
 
+// out's rows (rows, 4 per) whose coef is 0 are zeros: of an fp32 product their zeros
+// times an infinity or NaN of the weight are not (the 16-bit ones' reduction sees to
+// it). A wave a row: 3 us at 8 rows, 4 at 8192, of which none is zeroed.
+template <int UNUSED = 0>
+__global__ void __launch_bounds__(256)
+head_zero_rows_kernel(const float2* __restrict__ rows2, float4* __restrict__ out, long long rows,
+                      int per) {
+  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows || rows2[r].x != 0.f) return;
+  for (int i = threadIdx.x & 63; i < per; i += 64)
+    out[r * per + i] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
 struct HeadGrad {
   const float2* rows2;     // (rows, to an even number) (coef s, lse2)
   const float* scale;      // what the sums are multiplied by

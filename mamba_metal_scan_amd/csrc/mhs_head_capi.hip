@@ -617,7 +617,11 @@ int bwd32(const Head& p, const BwdPlan& b, mhs::HeadGrad a, const mhs::KeptLogit
                             b.rows4, 0, a.scale, part, part_bytes, s)) != 0)
       return rc;
   }
-  return MHS_OK;
+  if (!out.dhidden) return MHS_OK;
+  hipLaunchKernelGGL(mhs::head_zero_rows_kernel<>, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0,
+                     s, a.rows2, static_cast<float4*>(out.dhidden), (long long)p.rows,
+                     (int)(p.dim / 4));
+  return check_launch("zero rows kernel");
 }
 
 // See lift_of.
