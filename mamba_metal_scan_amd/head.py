@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native
 from ._native import REDUCE, HipScanError, dispatch
@@ -158,9 +159,11 @@ class DistillHIP(torch.autograd.Function):
 
 def _apply(cls, leaves: int, *args):
     """cls.apply, or without autograd to record (scoring, serving) its forward
-    alone."""
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled()
-                                         and any(t.requires_grad for t in args[:leaves])):
+    alone. (Leaves with a tangent go to apply too, which refuses forward-mode
+    derivatives: its forward alone would leave them out.)"""
+    if torch.compiler.is_compiling() \
+            or (torch.is_grad_enabled() and any(t.requires_grad for t in args[:leaves])) \
+            or any(unpack_dual(t).tangent is not None for t in args[:leaves]):
         return cls.apply(*args)
     return cls.loss(*args)[0]
 

@@ -1,0 +1,79 @@
+"""How the head's losses sit in autograd, on the CPU: the kernels' calls are replaced
+by recorders, the checks of the device taken out."""
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from mamba_metal_scan_amd import (_native, distill_loss, head, linear_cross_entropy,
+                                  linear_distill_loss)
+
+ROWS, DIM, VOCAB, TOP = 6, 16, 40, 3
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Every kernel call's (name, arguments); forwards give zeros of the ops' shapes,
+    backwards zero gradients."""
+    seen = []
+
+    def fwd(name, tops):
+        def call(a, *args):
+            seen.append((name, (a, *args)))
+            red = args[-2] if name != "distill_fwd" else args[-1]
+            n = _native._saved_size(a.shape[0], *tops)
+            return torch.zeros((a.shape[0],) if red == 0 else ()), torch.zeros(n)
+        return call
+
+    def bwd(name):
+        def call(grad, a, b, *args):
+            seen.append((name, (grad, a, b, *args)))
+            if name == "distill_bwd":
+                return torch.zeros(a.shape)
+            return torch.zeros(a.shape), torch.zeros(b.shape)
+        return call
+    for name, tops in (("linear_xent_fwd", (1,)), ("linear_distill_fwd", (TOP, TOP)),
+                       ("distill_fwd", (TOP,))):
+        monkeypatch.setitem(_native._IMPLS, name, fwd(name, tops))
+    for name in ("linear_xent_bwd", "linear_distill_bwd", "distill_bwd"):
+        monkeypatch.setitem(_native._IMPLS, name, bwd(name))
+    monkeypatch.setattr(head, "_hip", lambda *a: None)
+    monkeypatch.setattr(_native, "_on_one_device", lambda *a: None)
+    return seen
+
+
+def _losses():
+    """(name, loss of the leaves, the leaves) of each of the three."""
+    h, w = torch.randn(ROWS, DIM), torch.randn(VOCAB, DIM)
+    t = torch.arange(ROWS)
+    values, ids = torch.randn(ROWS, TOP), torch.arange(ROWS * TOP).view(ROWS, TOP)
+    return [("xent", lambda a, b: linear_cross_entropy(a, b, t, logits_bytes=0), [h, w]),
+            ("linear distill",
+             lambda a, b: linear_distill_loss(a, b, values, ids, logits_bytes=0), [h, w]),
+            ("distill", lambda a: distill_loss(a, values, ids), [torch.randn(ROWS, VOCAB)])]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(which, grad, calls):
+    """A tangent is not left out: with and without a leaf that requires grad, also
+    where gradients are off."""
+    _, loss, leaves = _losses()[which]
+    for i in range(len(leaves)):
+        for needs in (False, True):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                args = [x.clone().requires_grad_(needs) for x in leaves]
+                args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    loss(*args)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_alone_without_a_gradient(which, calls):
+    _, loss, leaves = _losses()[which]
+    assert not loss(*leaves).requires_grad
+    with torch.no_grad():
+        assert not loss(*(x.clone().requires_grad_() for x in leaves)).requires_grad
+    assert loss(*(x.clone().requires_grad_() for x in leaves)).requires_grad
+    assert len(calls) == 3
