@@ -34,6 +34,13 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return F.pad(t, (0, pad)) if pad else t.clone(memory_format=torch.contiguous_format)
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The 2-D t, or a copy of it with contiguous rows that do not overlap."""
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
 def _cut(g: torch.Tensor, dim: int) -> torch.Tensor:
     """A gradient without the columns that _rows16 added."""
     return g if g.shape[1] == dim else g[:, :dim].contiguous()
@@ -45,6 +52,15 @@ LOGITS_BYTES = 1 << 30   # of fp32 logits that a forward may keep, unless told o
 def _keeps(hidden: torch.Tensor, weight: torch.Tensor, most: int) -> bool:
     return _native.keeps_logits(hidden.shape[0], weight.shape[0], hidden.shape[1], hidden.dtype,
                                 most)
+
+
+def _restored(t: torch.Tensor) -> torch.Tensor:
+    """A saved tensor as the kernels read it, whatever layout a saved-tensor hook
+    gave it back in (its type, shape and device are checked after)."""
+    t = t.contiguous()
+    if torch.compiler.is_compiling() or t.data_ptr() % 16 == 0:
+        return t
+    return t.clone()
 
 
 def _once() -> None:
@@ -88,9 +104,11 @@ class LinearCrossEntropyHIP(torch.autograd.Function):
     def backward(ctx, g):
         _once()
         hidden, weight, targets, saved = ctx.saved_tensors
-        return (*_grads(ctx, *dispatch("linear_xent_bwd")(
-            g.contiguous(), hidden, weight, targets, saved, ctx.reduction,
-            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None, None)
+        args = (g.contiguous(), _rows16(hidden), _rows16(weight), _restored(targets),
+                _restored(saved), ctx.reduction, *ctx.needs_input_grad[:2])
+        if not torch.compiler.is_compiling():   # (what a saved-tensor hook gave back)
+            _native._check_linear_xent_bwd(*args)
+        return (*_grads(ctx, *dispatch("linear_xent_bwd")(*args)), None, None, None, None)
 
 
 class LinearDistillHIP(torch.autograd.Function):
@@ -122,9 +140,11 @@ class LinearDistillHIP(torch.autograd.Function):
     def backward(ctx, g):
         _once()
         hidden, weight, ids, saved = ctx.saved_tensors
-        return (*_grads(ctx, *dispatch("linear_distill_bwd")(
-            g.contiguous(), hidden, weight, ids, saved, ctx.temperature, ctx.reduction,
-            ctx.needs_input_grad[0], ctx.needs_input_grad[1])), None, None, None, None, None)
+        args = (g.contiguous(), _rows16(hidden), _rows16(weight), _restored(ids),
+                _restored(saved), ctx.temperature, ctx.reduction, *ctx.needs_input_grad[:2])
+        if not torch.compiler.is_compiling():
+            _native._check_linear_distill_bwd(*args)
+        return (*_grads(ctx, *dispatch("linear_distill_bwd")(*args)), None, None, None, None, None)
 
 
 class DistillHIP(torch.autograd.Function):
@@ -134,8 +154,7 @@ class DistillHIP(torch.autograd.Function):
     @staticmethod
     def loss(logits, teacher_logits, ids, temperature, reduction):
         """(loss, what the backward needs)."""
-        if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
-            logits = logits.contiguous()
+        logits = _rows(logits)
         if not torch.compiler.is_compiling():
             _native._check_distill("distill_loss", logits, teacher_logits, ids, temperature,
                                    reduction)
@@ -153,8 +172,11 @@ class DistillHIP(torch.autograd.Function):
     def backward(ctx, g):
         _once()
         logits, ids, saved = ctx.saved_tensors
-        return (dispatch("distill_bwd")(g.contiguous(), logits, ids, saved, ctx.temperature,
-                                        ctx.reduction), None, None, None, None)
+        args = (g.contiguous(), _rows(logits), _restored(ids), _restored(saved), ctx.temperature,
+                ctx.reduction)
+        if not torch.compiler.is_compiling():
+            _native._check_distill_bwd(*args)
+        return dispatch("distill_bwd")(*args), None, None, None, None
 
 
 def _apply(cls, leaves: int, *args):

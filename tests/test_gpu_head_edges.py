@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from mamba_metal_scan_amd import linear_cross_entropy, linear_distill_loss
+from mamba_metal_scan_amd import distill_loss, linear_cross_entropy, linear_distill_loss
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -46,3 +46,31 @@ def test_ignored_rows_beside_words_of_infinity(dtype, rows, bad):
                                    reduction="none", logits_bytes=most)
         ga, gb = torch.autograd.grad(loss, [a, b], torch.ones_like(loss))
         assert (loss[out] == 0).all() and (ga[out] == 0).all()
+
+
+@pytest.mark.parametrize("most", [0, 1 << 30])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_saved_tensors_in_another_layout(dtype, most):
+    """Saved tensors that a hook gives back strided: the same gradients."""
+    h, w, t = _operands(70, 64, 301, TYPES[dtype])
+    ids = torch.arange(4, device=DEV).repeat(70, 1)
+    values = torch.randn(70, 4, generator=_gen(1), device=DEV)
+
+    def strided(x):
+        if x.dim() == 2:
+            return x.t().contiguous().t()
+        wide = x.new_empty(2 * x.numel())
+        wide[::2] = x
+        return wide[::2]
+
+    def both(pack):
+        a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+        z = (h.float() @ w.float().t()).to(TYPES[dtype]).requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda x: x):
+            losses = (linear_cross_entropy(a, b, t, logits_bytes=most),
+                      linear_distill_loss(a, b, values, ids, logits_bytes=most),
+                      distill_loss(z, values, ids))
+        return [g for loss, leaves in zip(losses, ([a, b], [a, b], [z]))
+                for g in torch.autograd.grad(loss, leaves)]
+    for x, y in zip(both(strided), both(lambda x: x)):
+        assert torch.equal(x, y)

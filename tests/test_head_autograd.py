@@ -8,6 +8,7 @@ from torch.autograd import forward_ad
 
 from mamba_metal_scan_amd import (_native, distill_loss, head, linear_cross_entropy,
                                   linear_distill_loss)
+from mamba_metal_scan_amd._native import HipScanError
 
 ROWS, DIM, VOCAB, TOP = 6, 16, 40, 3
 
@@ -77,3 +78,50 @@ def test_forward_alone_without_a_gradient(which, calls):
         assert not loss(*(x.clone().requires_grad_() for x in leaves)).requires_grad
     assert loss(*(x.clone().requires_grad_() for x in leaves)).requires_grad
     assert len(calls) == 3
+
+
+def _strided(t):
+    """t's values in a layout of another kind: every second element, or transposed."""
+    if t.dim() == 2:
+        return t.t().contiguous().t()
+    wide = t.new_empty(2 * t.numel())
+    wide[::2] = t
+    return wide[::2]
+
+
+def _backward(loss, leaves, pack):
+    args = [x.clone().requires_grad_() for x in leaves]
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = loss(*args)
+    return torch.autograd.grad(out, args)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_saved_tensors_in_another_layout(which, calls):
+    """What a saved-tensor hook gives back strided reaches the kernel dense."""
+    _, loss, leaves = _losses()[which]
+    _backward(loss, leaves, _strided)
+    name, args = calls[-1]
+    tensors = [a for a in args if isinstance(a, torch.Tensor)]
+    assert name.endswith("_bwd") and len(tensors) == (4 if which == 2 else 5)
+    for t in tensors:
+        assert t.is_contiguous() and t.data_ptr() % 16 == 0
+    want = [x for x in leaves]
+    for got, x in zip(tensors[1:], want):
+        assert torch.equal(got, x)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("what", ["half", "int32", "short"])
+def test_saved_tensors_that_changed_are_refused(which, what, calls):
+    """Of another type or size they would be read past their end."""
+    def pack(t):
+        if what == "half":
+            return t.bfloat16() if t.dtype == torch.float32 and t.dim() == 1 else t
+        if what == "int32":
+            return t.int() if t.dtype == torch.int64 else t
+        return t[:-1] if t.dim() == 1 else t[:, :-1] if t.dtype == torch.int64 else t
+    _, loss, leaves = _losses()[which]
+    with pytest.raises(HipScanError):
+        _backward(loss, leaves, pack)
+    assert not any(name.endswith("_bwd") for name, _ in calls)
