@@ -424,7 +424,9 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
  *   hidden (rows, dim) rows ldh elements apart, weight (vocab, dim) rows ldw
  *   apart, both of `dtype`, 16-byte aligned; dim and the row strides multiples of
  *   8 (of 4 for MHS_F32), row strides below 2^21. fp32 products are those of
- *   mhs_gemm_f32; 16-bit ones multiply exactly and add in fp32.
+ *   mhs_gemm_f32; 16-bit ones multiply exactly and add in fp32. rows below 2^26
+ *   (the fp32 backward: 2^22), rows x vocab about 2^38 for MHS_F32 (2^24 tiles of 128
+ *   x 128), 2^43 otherwise: a launch counts its threads in 32 bits.
  *
  * Cross entropy against targets (rows) int64:
  *   loss_rows[r] = ln(2) lse2[r] - picked[r], lse2[r] = log2 sum_v exp(z[r, v]),
@@ -479,8 +481,9 @@ int mhs_linear_xent_bwd(int dtype, const void* hidden, int64_t ldh, const void* 
  * Outputs as above, and for the backward picked (rows, top), lse2 = log2 sum_v
  * exp(z / t) and q (rows, top), each word's whole weight in its row (a word that a
  * row names twice has the sum at both); dz[r, v] = t (p[v] - sum_{ids_k = v} q_k)
- * times the gradient that reaches the row's loss. The teacher gets no gradient. The
- * workspaces are the cross entropy's. No counterpart in the reference.
+ * times the gradient that reaches the row's loss. The teacher gets no gradient. rows
+ * below 2^24 (a block each), of given logits too. The workspaces are the cross
+ * entropy's. No counterpart in the reference.
  */
 #define MHS_MAX_TOP 1024
 

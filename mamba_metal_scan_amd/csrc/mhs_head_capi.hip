@@ -41,6 +41,9 @@ constexpr int64_t kPieceBytes = 256LL << 20;
 // and 57.8, 16384 101.9 and 100.5, 65536 384 and 367.)
 constexpr int64_t kLossOneBlock = 8192;
 
+// Blocks of 256 threads that a launch may have: it counts its threads in 32 bits.
+constexpr int64_t kMostBlocks = 1LL << 24;
+
 int elem_bytes(int dtype) { return dtype == MHS_F32 ? 4 : 2; }
 
 int check_dtype(int dtype) {
@@ -64,6 +67,12 @@ struct Head {
   int64_t ldh = 0, ldw = 0;
 };
 
+bool few_rows(const Head& p) { return p.rows <= small_rows(elem_bytes(p.dtype)); }
+
+// Tile of the forward's fp32 product. (us with 64 and 128, 64 rows: 640 x 32768 40
+// and 48, 4096 x 131072 689 and 748; 96 rows: 54 and 48, 1050 and 797.)
+int gemm3_tile(int64_t rows) { return rows <= 64 ? mhs::kGemmSmallTile : mhs::kGemmTile; }
+
 int check_sizes(const Head& p) {
   int rc = check_dtype(p.dtype);
   if (rc) return rc;
@@ -74,10 +83,23 @@ int check_sizes(const Head& p) {
   if (p.dim % v || p.dim > (1LL << 20))
     return fail(MHS_EINVAL, "dim must be a multiple of %d up to 2^20; got %lld", v,
                 (long long)p.dim);
-  // One block per tile: the grid of the products and of the rows.
-  if (((p.vocab + 63) / 64) * ((p.rows + 63) / 64) > 0x7FFFFFFF)
+  // The forward's product, a block per tile (16 bits: tiles counted in an int), and
+  // the rows' kernels, a wave per row.
+  const int t = few_rows(p) ? mhs::kSmallWords : gemm3_tile(p.rows);
+  const int64_t tiles = ((p.vocab + t - 1) / t) * (few_rows(p) ? 1 : (p.rows + t - 1) / t);
+  const bool streamed = p.dtype != MHS_F32 && !few_rows(p);
+  const bool fits = streamed ? ((p.vocab + 63) / 64) * ((p.rows + 63) / 64) <= 0x7FFFFFFF
+                             : tiles < kMostBlocks;
+  if (!fits || (p.rows + 3) / 4 >= kMostBlocks)
     return fail(MHS_EINVAL, "%lld rows x %lld words is too large", (long long)p.rows,
                 (long long)p.vocab);
+  return MHS_OK;
+}
+
+// Distillation takes a block per row.
+int check_block_rows(int64_t rows) {
+  if (rows < 0 || rows >= kMostBlocks)
+    return fail(MHS_EINVAL, "distillation takes rows in [0, 2^24); got %lld", (long long)rows);
   return MHS_OK;
 }
 
@@ -113,12 +135,6 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 }
 
 // ----------------------------------------------------------------- forward
-
-bool few_rows(const Head& p) { return p.rows <= small_rows(elem_bytes(p.dtype)); }
-
-// Tile of the forward's fp32 product. (us with 64 and 128, 64 rows: 640 x 32768 40
-// and 48, 4096 x 131072 689 and 748; 96 rows: 54 and 48, 1050 and 797.)
-int gemm3_tile(int64_t rows) { return rows <= 64 ? mhs::kGemmSmallTile : mhs::kGemmTile; }
 
 // Splits of a 16-bit forward's product in k: 1 where the tiles' own kernel takes
 // it whole. A k tile takes 1.07 us of a block (the direct kernel's blocks wait for
@@ -727,11 +743,12 @@ int launch_distill_bwd(const void* logits, int64_t ld, const int64_t* ids, const
 int check_logits(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
                  int64_t top, float temperature, int reduction) {
   int rc = check_dtype(dtype);
-  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature))) return rc;
-  if (rows < 0 || rows > 0x7FFFFFFF || vocab < 1 || vocab > 0x7FFFFFFF || ld < vocab)
-    return fail(MHS_EINVAL, "rows must be in [0, 2^31), vocab in [1, 2^31) and the row stride at "
-                "least vocab; got %lld, %lld, %lld", (long long)rows, (long long)vocab,
-                (long long)ld);
+  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature)) ||
+      (rc = check_block_rows(rows)))
+    return rc;
+  if (vocab < 1 || vocab > 0x7FFFFFFF || ld < vocab)
+    return fail(MHS_EINVAL, "vocab must be in [1, 2^31) and the row stride at least vocab; got "
+                "%lld, %lld", (long long)vocab, (long long)ld);
   if (rows > 0 && !logits) return fail(MHS_EINVAL, "null pointer argument");
   if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype))
     return fail(MHS_EINVAL, "logits must be aligned to their elements");
@@ -805,7 +822,9 @@ int mhs_linear_distill_fwd(int dtype, const void* hidden, int64_t ldh, const voi
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
   int rc = check_head(p);
-  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature))) return rc;
+  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature)) ||
+      (rc = check_block_rows(rows)))
+    return rc;
   if (rows > 0 && (!teacher || !q)) return fail(MHS_EINVAL, "null pointer argument");
   mhs::HeadRows g{};
   g.ids = ll(ids);
@@ -829,7 +848,9 @@ int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const voi
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
   int rc = check_head(p);
-  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature))) return rc;
+  if (rc || (rc = check_reduction(reduction)) || (rc = check_top(top, temperature)) ||
+      (rc = check_block_rows(rows)))
+    return rc;
   if (rows > 0 && (!q || (reduction == MHS_REDUCE_MEAN && !count)))
     return fail(MHS_EINVAL, "null pointer argument");
   mhs::HeadGrad a{};
@@ -844,7 +865,7 @@ int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const voi
 
 size_t mhs_distill_workspace_bytes(int64_t rows) {
   mhs::clear_error();
-  return rows < 0 ? 0 : std::max(loss_ws(rows), (size_t)256);
+  return check_block_rows(rows) ? 0 : std::max(loss_ws(rows), (size_t)256);
 }
 
 int mhs_distill_fwd(int dtype, const void* logits, int64_t ld, const float* teacher,
