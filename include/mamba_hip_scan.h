@@ -445,8 +445,10 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
  * logits, if given (16-byte aligned, else NULL): the forward keeps the fp32 logits
  *   there, (rows, vocab to a multiple of 4), for MHS_F32 (vocab, rows to a multiple
  *   of 4), and the backward reads them instead of forming them a second time.
- * Every sum runs in a fixed order (bit-for-bit reproducible). The workspace is
- * 256-byte aligned; its size is 0 for arguments that the calls reject.
+ * Every sum runs in a fixed order (bit-for-bit reproducible). lse2 is held in fp32,
+ * so a probability is off by 2^-24 |lse2| relative, and by more than that where the
+ * logits themselves lie beyond 2^20 (temperatures, for distillation). The workspace
+ * is 256-byte aligned; its size is 0 for arguments that the calls reject.
  */
 #define MHS_F32 0
 #define MHS_BF16 1
@@ -505,7 +507,9 @@ int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const voi
  * The same distillation of given logits (rows, vocab) of `dtype`, rows ld
  * elements apart, at any alignment of whole elements; dlogits (rows, vocab) is
  * contiguous, 16-byte aligned, fully written, and may not alias logits. The
- * workspace (the forward's) is mhs_distill_workspace_bytes(rows).
+ * workspace (the forward's) is mhs_distill_workspace_bytes(rows). Finite logits of
+ * any size: a row of one value, be it the type's lowest, is the uniform
+ * distribution; a row of -inf alone is NaN.
  */
 size_t mhs_distill_workspace_bytes(int64_t rows);
 int mhs_distill_fwd(int dtype, const void* logits, int64_t ld, const float* teacher,

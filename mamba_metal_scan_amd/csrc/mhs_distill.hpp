@@ -32,6 +32,27 @@ struct RowSplit {
   }
 };
 
+// A row's exponents are formed in one step, c z - (the rounded c max z): off by half a
+// unit of that product, 2^-12 at 4096 and anything from 2^31 on, where c z may overflow
+// besides. A row whose log-sum-exp lies further out (all its logits a mask's -1e9 or the
+// type's lowest value, say) goes a second way, by differences of the logits: two more
+// passes, here and in the backward (all rows so, fp32 8192 x 32768: 639 and 1392 us
+// for 236 and 432). Of other rows the branch takes nothing measurable.
+constexpr float kFarLse2 = 4096.f;
+__device__ __forceinline__ bool far_row(float lse2) { return !(fabsf(lse2) <= kFarLse2); }
+
+// (M, log2 sum 2^(c (z - M))) of the row, M its largest logit; the sum NaN where a logit
+// is NaN or infinity or all are -inf. The same in every thread.
+template <class T>
+__device__ __forceinline__ float2 far_row_lse2(const elem_t<T>* x, long long n, float c,
+                                               float* red) {
+  float m = -INFINITY, s = 0.f;
+  for (long long i = threadIdx.x; i < n; i += kXentThreads) m = fmaxf(m, T::to(x[i]));
+  m = block_max(m, red);
+  for (long long i = threadIdx.x; i < n; i += kXentThreads) s += exp2_hw((T::to(x[i]) - m) * c);
+  return make_float2(m, log2f(block_sum(s, red)));
+}
+
 // fp32 8192 x 32768 237 us (4.5 TB/s; a large copy takes 4.7), bf16 4096 x 50257 110
 // us (3.7, bound by its arithmetic and by rows that start at any element). A row to
 // 512 threads takes 2% less there, but forward and backward of 4096 x 4096 66 us
@@ -84,7 +105,13 @@ distill_fwd_kernel(HeadRows g) {
     lse2_combine(m, s, mc, sc);
   }
   block_lse2(m, s);   // (its barrier publishes zk)
-  teacher_row(g, r, m + log2f(s), zk, red);
+  teacher_row(g, r, m + log2f(s), zk, red, [&](float& lse2) {
+    if (!far_row(lse2)) return lse2;
+    const float2 far = far_row_lse2<T>(x, g.vocab, c, red);
+    for (int k = threadIdx.x; k < g.k; k += kXentThreads) zk[k] -= far.x;
+    lse2 = far.y;
+    return __builtin_fmaf(far.x, c, far.y);
+  });
 }
 
 // dlogits (rows, vocab) contiguous. The teacher's words are put right after the
@@ -96,6 +123,7 @@ distill_bwd_kernel(const elem_t<T>* __restrict__ logits, long long ld,
                    const long long* __restrict__ ids, const float* __restrict__ q,
                    const float* __restrict__ lse2, RowScale rs, elem_t<T>* __restrict__ dlogits,
                    long long vocab, int top, float c) {
+  __shared__ float red[4];
   constexpr int V = kVec<T>;
   const long long r = blockIdx.x;
   const elem_t<T>* x = logits + r * ld;
@@ -136,6 +164,19 @@ distill_bwd_kernel(const elem_t<T>* __restrict__ logits, long long ld,
     }
   }
   if (zero) return;
+  if (far_row(l2)) {   // the row again
+    const float2 far = far_row_lse2<T>(x, vocab, c, red);   // (its barriers: the stores above)
+    const auto p = [&](long long i) {
+      return exp2_hw(__builtin_fmaf(T::to(x[i]) - far.x, c, -far.y));
+    };
+    for (long long i = threadIdx.x; i < vocab; i += kXentThreads) dx[i] = T::from(cf * p(i));
+    __syncthreads();   // the row's stores before its words'
+    for (int k = threadIdx.x; k < top; k += kXentThreads) {
+      const long long id = ids[r * top + k];
+      if (id >= 0 && id < vocab) dx[id] = T::from(cf * (p(id) - q[r * top + k]));
+    }
+    return;
+  }
   __syncthreads();   // the row's stores before its words'
   for (int k = threadIdx.x; k < top; k += kXentThreads) {
     const long long id = ids[r * top + k];

@@ -492,12 +492,14 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 
 // The teacher's probabilities of row r over its kept words (id >= 0), and the
 // row's loss from the student's logits zk at the ids (LDS, k floats, then room
-// for k more) and lse2. To q goes each word's whole weight in the row: a word
+// for k more) and lse2; offset(lse2) may take one away from both, and returns the
+// lse2 that the backward gets. To q goes each word's whole weight in the row: a word
 // that the row names twice has both entries' sum at each. A row that keeps no
 // word, or whose kept logits are all -inf, is empty: loss 0, probabilities 0. An
 // id at or past the vocabulary: NaN.
+template <class Offset>
 __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2, float* zk,
-                                            float* red) {
+                                            float* red, const Offset& offset) {
   const long long at = (long long)r * g.k;
   const float c = kLog2e / g.temperature;
   float m = -INFINITY, bad = 0.f;
@@ -518,6 +520,7 @@ __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2
     }
   s = block_sum(s, red);
   any = block_max(any, red);
+  const float stored = offset(lse2);
   const float log2s = log2f(s), inv = any != 0.f ? 1.f / s : 0.f;
   float loss = 0.f;
   for (int k = threadIdx.x; k < g.k; k += 256) {
@@ -531,14 +534,18 @@ __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2
     zk[g.k + k] = q;
   }
   loss = block_sum(loss, red);   // (its barriers publish the q's)
+  // (constant memory: scalar loads, which the compiler gives up behind offset's branch;
+  // vector ones take 10 us of distill_fwd_kernel's 236 at 64 words)
+  typedef const __attribute__((address_space(4))) long long* ConstIds;
+  const ConstIds ids = (ConstIds)(unsigned long long)(g.ids + at);
   for (int k = threadIdx.x; k < g.k; k += 256) {
     const long long id = g.ids[at + k];
     float q = 0.f;
-    for (int j = 0; j < g.k; ++j) q += g.ids[at + j] == id ? zk[g.k + j] : 0.f;
+    for (int j = 0; j < g.k; ++j) q += ids[j] == id ? zk[g.k + j] : 0.f;
     g.q[at + k] = q;
   }
   if (threadIdx.x == 0) {
-    g.lse2[r] = lse2;
+    g.lse2[r] = stored;
     g.keep[r] = any;
     g.loss[r] = any == 0.f ? 0.f
                 : bad != 0.f ? __builtin_nanf("") : g.temperature * g.temperature * loss;
@@ -579,7 +586,7 @@ head_distill_rows_kernel(HeadRows g) {
     lse2_combine(m, s, p.x, p.y);
   }
   block_lse2(m, s);   // (its barrier publishes zk)
-  teacher_row(g, r, m + log2f(s), zk, red);
+  teacher_row(g, r, m + log2f(s), zk, red, [](float& lse2) { return lse2; });
 }
 
 // loss[0] = the sum of the rows' losses, over the count of rows kept for the

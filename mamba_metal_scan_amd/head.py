@@ -300,6 +300,8 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
     With q = softmax(teacher_logits / temperature) over a row's kept words and
     p = softmax(logits / temperature) over the vocabulary, a row's loss is
     temperature^2 sum_k q_k (log q_k - log p_k), terms with q_k = 0 being 0. A
+    row of logits that are all alike, be it the type's lowest value (a mask that leaves
+    nothing), is the uniform distribution; one of -inf alone is NaN. A
     row that keeps no word, or whose kept logits are all -inf, has loss 0 and no
     gradient, and the mean leaves it out (NaN where it leaves out all); an id at
     or past V makes its row's loss NaN; a word named twice has both weights. The
