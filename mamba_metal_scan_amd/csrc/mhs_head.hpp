@@ -548,7 +548,8 @@ __device__ __forceinline__ void teacher_row(const HeadRows& g, int r, float lse2
     g.lse2[r] = stored;
     g.keep[r] = any;
     g.loss[r] = any == 0.f ? 0.f
-                : bad != 0.f ? __builtin_nanf("") : g.temperature * g.temperature * loss;
+                // (t^2 by itself is 0 or infinite where the loss is neither)
+                : bad != 0.f ? __builtin_nanf("") : g.temperature * (g.temperature * loss);
   }
 }
 

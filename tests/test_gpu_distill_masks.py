@@ -100,3 +100,27 @@ def test_rows_of_the_lowest_value_beside_others():
     assert torch.equal(loss[rest], want[rest])
     assert torch.isfinite(loss[1]) and torch.isfinite(grad[1]).all()
     assert torch.isnan(loss[4]) and torch.isnan(grad[4]).all()
+
+
+@pytest.mark.parametrize("temperature", [1e-29, 1e-25, 1e-20, 1e-10, 1e-3, 1e2, 1e6, 1e12, 1e18])
+def test_any_temperature(temperature):
+    """From one word that has all the weight to the uniform distribution. The loss is a
+    sum of terms of one sign here (k of 3001 words), each of a few roundings and the
+    log-sum-exp's of 3001 2^-24 at most."""
+    g = _gen(11)
+    z = 3 * torch.randn(5, 3001, generator=g, device=DEV)
+    values = torch.randn(5, 6, generator=g, device=DEV)
+    ids = torch.randint(0, 3001, (5, 6), generator=g, device=DEV)
+    a = z.clone().requires_grad_()
+    t = float(torch.tensor(temperature))   # as the kernel has it
+    loss = distill_loss(a, values, ids, temperature=temperature, reduction="none")
+    grad, = torch.autograd.grad(loss, [a], torch.ones_like(loss))
+    logp = (z.double() / t).log_softmax(1)
+    q = (values.double() / t).softmax(1)
+    terms = torch.where(q > 0, q * ((values.double() / t).log_softmax(1) - logp.gather(1, ids)), 0.0)
+    want = t * t * terms.sum(1)
+    assert ((loss.double() - want).abs() <= 2.0 ** -12 * want.abs()).all(), (loss, want)
+    dz = (t * logp.exp())
+    err = 2.0 ** -12 * dz
+    dz.scatter_add_(1, ids, -t * q)
+    assert ((grad.double() - dz).abs() <= err + 2.0 ** -18 * dz.abs() + t * 2.0 ** -100).all()
