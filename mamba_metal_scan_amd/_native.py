@@ -1271,13 +1271,24 @@ HEAD_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_TOP = 1024   # the header's MHS_MAX_TOP
 
 
-def head_rows(t: torch.Tensor) -> bool:
-    """Whether the head's kernels read the 2-D t in place: rows of whole 16-byte
-    accesses, 16-byte aligned, less than 2^21 elements apart."""
+def head_layout(t: torch.Tensor) -> bool:
+    """Whether the 2-D t has rows of whole 16-byte accesses less than 2^21 elements
+    apart (what tracing can tell of head_rows)."""
     v = 16 // t.element_size()
     ld = t.stride(0)
     return (t.shape[1] % v == 0 and t.stride(1) == 1 and ld % v == 0
-            and t.shape[1] <= ld < 1 << 21 and t.data_ptr() % 16 == 0)
+            and t.shape[1] <= ld < 1 << 21)
+
+
+def head_rows(t: torch.Tensor) -> bool:
+    """Whether the head's kernels read the 2-D t in place: head_layout, and 16-byte
+    aligned."""
+    return head_layout(t) and t.data_ptr() % 16 == 0
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it that is 16-byte aligned."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _saved_parts(saved: torch.Tensor, rows: int, *tops: int) -> list[int]:
@@ -1338,10 +1349,10 @@ def _check_head(what: str, hidden, weight, reduction) -> None:
         raise HipScanError(f"{what}: hidden and weight must both be float32, bfloat16 or "
                            f"float16; got {hidden.dtype}, {weight.dtype}")
     for name, t in (("hidden", hidden), ("weight", weight)):
-        if t.numel() != 0 and not head_rows(t):
-            raise HipScanError(f"{what}: {name} needs rows of whole 16-byte accesses, 16-byte "
-                               f"aligned and less than 2^21 elements apart; got shape "
-                               f"{tuple(t.shape)}, strides {t.stride()}")
+        if t.numel() != 0 and not head_layout(t):
+            raise HipScanError(f"{what}: {name} needs rows of whole 16-byte accesses less than "
+                               f"2^21 elements apart; got shape {tuple(t.shape)}, strides "
+                               f"{t.stride()}")
     if reduction not in (0, 1, 2):
         raise HipScanError(f"{what}: reduction must be 0, 1 or 2; got {reduction!r}")
 
@@ -1386,6 +1397,7 @@ def _linear_xent_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor, targets: t
                           ignore_index: int, reduction: int, keep_logits: bool = False
                           ) -> tuple[torch.Tensor, torch.Tensor]:
     """(loss () or (rows,), saved) of hidden (rows, dim) against targets (rows)."""
+    hidden, weight = _aligned(hidden), _aligned(weight)
     rows, dim = hidden.shape
     vocab = weight.shape[0]
     dev = hidden.device
@@ -1441,6 +1453,7 @@ def _linear_xent_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: torc
                           need_hidden: bool, need_weight: bool
                           ) -> tuple[torch.Tensor, torch.Tensor]:
     """(dhidden, dweight) for the forward that gave saved; empty where not needed."""
+    hidden, weight = _aligned(hidden), _aligned(weight)
     rows, dim = hidden.shape
     vocab = weight.shape[0]
     dev = hidden.device
@@ -1485,6 +1498,7 @@ def _linear_distill_fwd_impl(hidden: torch.Tensor, weight: torch.Tensor,
                              ) -> tuple[torch.Tensor, torch.Tensor]:
     """(loss () or (rows,), saved) against the teacher's words ids (rows, top) and
     their logits."""
+    hidden, weight = _aligned(hidden), _aligned(weight)
     rows, dim = hidden.shape
     vocab, top = weight.shape[0], ids.shape[1]
     dev = hidden.device
@@ -1535,6 +1549,7 @@ def _linear_distill_bwd_impl(grad: torch.Tensor, hidden: torch.Tensor, weight: t
                              reduction: int, need_hidden: bool, need_weight: bool
                              ) -> tuple[torch.Tensor, torch.Tensor]:
     """(dhidden, dweight) for the forward that gave saved; empty where not needed."""
+    hidden, weight = _aligned(hidden), _aligned(weight)
     rows, dim = hidden.shape
     vocab, top = weight.shape[0], ids.shape[1]
     dev = hidden.device

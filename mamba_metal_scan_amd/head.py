@@ -27,8 +27,9 @@ from ._native import REDUCE, HipScanError, dispatch
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """The 2-D t, or a copy of it whose rows the kernels read in place (zeros
-    in the columns that fill up its rows)."""
-    if _native.head_rows(t):
+    in the columns that fill up its rows). While tracing of the right layout: the ops
+    see to the alignment, which is known only then."""
+    if (_native.head_layout if torch.compiler.is_compiling() else _native.head_rows)(t):
         return t
     pad = -t.shape[1] % (16 // t.element_size())
     return F.pad(t, (0, pad)) if pad else t.clone(memory_format=torch.contiguous_format)

@@ -74,3 +74,62 @@ def test_saved_tensors_in_another_layout(dtype, most):
                 for g in torch.autograd.grad(loss, leaves)]
     for x, y in zip(both(strided), both(lambda x: x)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_compiled_in_one_graph(dtype):
+    """torch.compile with fullgraph at several row counts, odd widths and unaligned
+    views: bit for bit the eager losses and gradients (in fp32, whose logits eager keeps
+    from a limit on, the same rule applies to both)."""
+    print(f"[case] compiled {dtype}", flush=True)
+
+    def losses(a, b, t, values, ids):
+        return (linear_cross_entropy(a, b, t),
+                linear_distill_loss(a, b, values, ids, temperature=2.0, reduction="none"),
+                distill_loss(a @ b.t(), values, ids))
+    torch._dynamo.reset()
+    f = torch.compile(losses, backend="aot_eager", fullgraph=True)
+    for rows, dim in ((40, 64), (3, 64), (300, 64), (40, 50)):
+        h, w, t = _operands(rows, dim, 301, TYPES[dtype])
+        ids = torch.randint(0, 301, (rows, 4), generator=_gen(rows), device=DEV)
+        values = torch.randn(rows, 4, generator=_gen(rows, 1), device=DEV)
+        off = torch.empty(h.numel() + 1, dtype=h.dtype, device=DEV)[1:].view(rows, dim)
+        off.copy_(h)
+        for a in (h, off):
+            results = []
+            for fn in (losses, f):
+                x, y = a.detach().requires_grad_(), w.detach().requires_grad_()
+                out = fn(x, y, t, values, ids)
+                up = [torch.ones_like(o) for o in out]
+                results.append((*(o.detach() for o in out),
+                                *torch.autograd.grad(out, [x, y], up)))
+            for one, two in zip(*results):
+                assert torch.equal(one, two)
+    torch._dynamo.reset()
+
+
+def test_compiled_model_losses():
+    from mamba_metal_scan_amd import MambaConfig, TinyMamba
+    torch.manual_seed(0)
+    model = TinyMamba(MambaConfig(vocab_size=601, d_model=64, n_layers=2, d_ff=256,
+                                  scan_impl="hip")).to(DEV)
+    idx = torch.randint(0, 601, (3, 41), generator=_gen(3), device=DEV)
+    x, t = idx[:, :-1].contiguous(), idx[:, 1:].contiguous()
+    ids = torch.randint(0, 601, (3, 40, 5), generator=_gen(4), device=DEV)
+    values = torch.randn(3, 40, 5, generator=_gen(5), device=DEV)
+
+    def both():
+        return model.loss(x, t) + model.distill(x, values, ids, temperature=2.0)
+    torch._dynamo.reset()
+    results = []
+    for fn in (both, torch.compile(both, backend="aot_eager", fullgraph=True)):
+        model.zero_grad(set_to_none=True)
+        loss = fn()
+        loss.backward()
+        results.append((loss.detach(), [p.grad.clone() for p in model.parameters()]))
+    torch._dynamo.reset()
+    (l1, g1), (l2, g2) = results
+    # (the bar of the compiled model's own test)
+    assert abs(float(l1) - float(l2)) <= 1e-6 * float(l1)
+    for a, b in zip(g1, g2):
+        assert float((a - b).abs().max()) <= 1e-5 * max(1.0, float(a.abs().max()))

@@ -125,3 +125,25 @@ def test_saved_tensors_that_changed_are_refused(which, what, calls):
     with pytest.raises(HipScanError):
         _backward(loss, leaves, pack)
     assert not any(name.endswith("_bwd") for name, _ in calls)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("dynamic", [None, True])
+def test_traced_in_one_graph(which, dynamic, monkeypatch):
+    """torch.compile takes each loss whole (fullgraph), as the package's other ops."""
+    monkeypatch.setattr(head, "_hip", lambda *a: None)
+    graphs = []
+
+    def backend(gm, example):
+        graphs.append(gm)
+        return lambda *a: [torch.zeros(())]
+    _, loss, leaves = _losses()[which]
+    torch._dynamo.reset()
+    with torch.no_grad():
+        torch.compile(loss, backend=backend, fullgraph=True, dynamic=dynamic)(*leaves)
+    op = ("linear_xent_fwd", "linear_distill_fwd", "distill_fwd")[which]
+    assert len(graphs) == 1 and f"mamba_hip.{op}" in graphs[0].code
+    torch.compile(loss, backend=backend, fullgraph=True, dynamic=dynamic)(
+        *(x.requires_grad_() for x in leaves))
+    assert len(graphs) == 2
+    torch._dynamo.reset()
