@@ -38,7 +38,8 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """The 2-D t, or a copy of it with contiguous rows that do not overlap."""
     if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
+        # (contiguous() would leave the strides of a single column as they are)
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 

@@ -147,3 +147,13 @@ def test_traced_in_one_graph(which, dynamic, monkeypatch):
         *(x.requires_grad_() for x in leaves))
     assert len(graphs) == 2
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("layout", ["transposed", "sliced"])
+def test_a_vocabulary_of_one_word(layout, calls):
+    """Logits (rows, 1) whose last stride is not 1: contiguous by torch's account."""
+    z = torch.randn(1, ROWS).t() if layout == "transposed" else torch.randn(1, 3)[:, ::3]
+    rows = z.shape[0]
+    values, ids = torch.randn(rows, TOP), torch.zeros(rows, TOP, dtype=torch.int64)
+    distill_loss(z, values, ids)
+    assert calls[-1][1][0].stride() == (1, 1)
