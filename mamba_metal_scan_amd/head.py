@@ -7,10 +7,14 @@ words) 1.07 GB of fp32 logits and as much again for their gradient.
 hidden states and the head's weight, the logits formed tile by tile on the
 matrix cores: the forward reduces each tile to its rows' maxima and sums of
 exponentials, the backward forms the tiles again, a piece of the vocabulary at a
-time, and multiplies their gradient with the weight and the hidden states. Of
-logits that take no more than ``logits_bytes`` (1 GB by default, 0: none) the forward
-keeps the fp32 values for the backward, where that is the faster; without a
-backward it keeps none.
+time, and multiplies their gradient with the weight and the hidden states.
+
+What a training call holds. From forward to backward, by default, up to 1 GiB
+(``logits_bytes``) of fp32 logits, where their total fits that and keeping them is the
+faster: always in fp32, so all of the batch above's 2^30 bytes, and up to 256 rows or from 2048
+columns in 16 bits. ``logits_bytes=0`` holds none, for a fourth product (at that batch in
+fp32 7330 us where 5980). During the backward up to 256 MB of the logits' gradient. Without
+a backward nothing is kept.
 
 ``distill_loss`` is the distillation of given logits from a teacher's top words,
 ``linear_distill_loss`` the same from the hidden states.
@@ -252,15 +256,15 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
                          ignore_index: int = -100, reduction: str = "mean",
                          logits_bytes: int = LOGITS_BYTES) -> torch.Tensor:
     """``F.cross_entropy(hidden @ weight.T, targets, ignore_index=ignore_index,
-    reduction=reduction)`` without the logits: hidden (..., D) and weight (V, D)
+    reduction=reduction)`` from the operands: hidden (..., D) and weight (V, D)
     in float32, bfloat16 or float16 on one ROCm device, targets (...) integers.
 
     The loss is float32: a scalar, or with reduction "none" one per row, of
     targets' shape (0 where ignored). Rows that are ignored add nothing to the
     gradients, whatever they hold. A target outside [0, V) that is not
-    ignore_index makes its row's loss NaN. Up to logits_bytes of fp32 logits (rows x
-    V x 4) may be kept from forward to backward, where that is the faster; 0 keeps
-    none. Under autocast hidden and weight are
+    ignore_index makes its row's loss NaN. Fp32 logits (rows x V x 4 bytes) that take
+    no more than logits_bytes, 1 GiB unless given, may be kept whole from forward to
+    backward, where that is the faster; 0 keeps none. Under autocast hidden and weight are
     taken in its type. The gradients are once differentiable."""
     what = "linear_cross_entropy"
     _hip(what, hidden, weight, targets)
@@ -279,7 +283,7 @@ def linear_distill_loss(hidden: torch.Tensor, weight: torch.Tensor,
                         teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                         temperature: float = 1.0, reduction: str = "mean",
                         logits_bytes: int = LOGITS_BYTES) -> torch.Tensor:
-    """``distill_loss(hidden @ weight.T, ...)`` without the logits: hidden (..., D),
+    """``distill_loss(hidden @ weight.T, ...)`` from the operands: hidden (..., D),
     weight (V, D) and logits_bytes as linear_cross_entropy takes them,
     teacher_logits and teacher_ids (..., K)."""
     what = "linear_distill_loss"

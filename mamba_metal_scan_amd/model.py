@@ -42,7 +42,7 @@ from .block import BlockHIP, block_forward, block_params
 from .conv import conv1d_silu
 from .decode import decode_step
 from .fused import mamba_inner, out_gate, selective_scan_gated
-from .head import distill_loss, linear_cross_entropy, linear_distill_loss
+from .head import LOGITS_BYTES, distill_loss, linear_cross_entropy, linear_distill_loss
 from .linear import PLAIN, linear, no_hooks
 from .norm import add_rms_norm, rms_norm, rms_norm_residual
 from .scan import SSM_CHUNK, _hip_device, selective_scan, selective_state_step
@@ -483,27 +483,30 @@ class TinyMamba(nn.Module):
                 and type(h) in PLAIN and h.dtype == head.weight.dtype
                 and h.dtype in (torch.float32, torch.bfloat16, torch.float16))
 
-    def loss(self, idx, targets, ignore_index: int = -100, reduction: str = "mean"):
-        """The cross entropy of forward(idx, targets) without its logits
-        (linear_cross_entropy, on the HIP path). reduction
+    def loss(self, idx, targets, ignore_index: int = -100, reduction: str = "mean",
+             logits_bytes: int = LOGITS_BYTES):
+        """The cross entropy of forward(idx, targets) from the hidden states
+        (linear_cross_entropy, on the HIP path). For its backward it may hold up to
+        logits_bytes (1 GiB) of fp32 logits, each such loss its own, 0: none. reduction
         "none": one loss per token (the tokens' negative log-probabilities)."""
         h = self._hidden(self.tok(idx), [None] * len(self.blocks))
         if self._head_fused(h):
-            return linear_cross_entropy(h, self.head.weight, targets, ignore_index, reduction)
+            return linear_cross_entropy(h, self.head.weight, targets, ignore_index, reduction,
+                                        logits_bytes)
         logits = self.head(h)
         loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), targets.reshape(-1),
                                ignore_index=ignore_index, reduction=reduction)
         return loss.view(targets.shape) if reduction == "none" else loss
 
     def distill(self, idx, teacher_logits, teacher_ids, temperature: float = 1.0,
-                reduction: str = "mean"):
+                reduction: str = "mean", logits_bytes: int = LOGITS_BYTES):
         """Distillation of the model's tokens idx (B, T) from a teacher's top words
-        (B, T, K) and their logits, without the model's own logits
-        (linear_distill_loss). On the HIP path only."""
+        (B, T, K) and their logits, from the model's hidden states
+        (linear_distill_loss; logits_bytes as for loss). On the HIP path only."""
         h = self._hidden(self.tok(idx), [None] * len(self.blocks))
         if self._head_fused(h):
             return linear_distill_loss(h, self.head.weight, teacher_logits, teacher_ids,
-                                       temperature, reduction)
+                                       temperature, reduction, logits_bytes)
         return distill_loss(self.head(h), teacher_logits, teacher_ids, temperature, reduction)
 
     def count_params(self) -> int:

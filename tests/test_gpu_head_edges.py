@@ -133,3 +133,32 @@ def test_compiled_model_losses():
     assert abs(float(l1) - float(l2)) <= 1e-6 * float(l1)
     for a, b in zip(g1, g2):
         assert float((a - b).abs().max()) <= 1e-5 * max(1.0, float(a.abs().max()))
+
+
+def test_the_model_passes_on_what_may_be_held():
+    """logits_bytes through TinyMamba.loss and .distill: what is held until the backward
+    grows by the logits where they may be kept, the gradients stay."""
+    from mamba_metal_scan_amd import MambaConfig, TinyMamba
+    torch.manual_seed(0)
+    model = TinyMamba(MambaConfig(vocab_size=20000, d_model=64, n_layers=1, d_ff=256,
+                                  scan_impl="hip")).to(DEV)
+    x = torch.randint(0, 20000, (4, 100), generator=_gen(3), device=DEV)
+    ids = torch.randint(0, 20000, (4, 100, 5), generator=_gen(4), device=DEV)
+    values = torch.randn(4, 100, 5, generator=_gen(5), device=DEV)
+    logits = 400 * 20000 * 4
+    for f in (lambda **kw: model.loss(x, x, **kw),
+              lambda **kw: model.distill(x, values, ids, 2.0, **kw)):
+        held, grads = [], []
+        for kw in ({"logits_bytes": 0}, {"logits_bytes": logits - 1}, {"logits_bytes": logits},
+                   {}):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            loss = f(**kw)
+            held.append(torch.cuda.memory_allocated() - before)
+            grads.append(torch.autograd.grad(loss, list(model.parameters())))
+            del loss
+        assert abs(held[1] - held[0]) < logits // 8
+        for n in held[2:]:
+            assert logits <= n - held[0] < logits + logits // 8
+        for a, b in zip(grads[0], grads[2]):   # (fp32's bar of the model's other paths)
+            assert float((a - b).abs().max()) <= 1e-4 * float(a.abs().max()) + 1e-9
