@@ -490,12 +490,14 @@ class TinyMamba(nn.Module):
         logits_bytes (1 GiB) of fp32 logits, each such loss its own, 0: none. reduction
         "none": one loss per token (the tokens' negative log-probabilities)."""
         h = self._hidden(self.tok(idx), [None] * len(self.blocks))
+        flat = targets.reshape(-1)   # (of any shape, as forward takes them)
         if self._head_fused(h):
-            return linear_cross_entropy(h, self.head.weight, targets, ignore_index, reduction,
-                                        logits_bytes)
-        logits = self.head(h)
-        loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), targets.reshape(-1),
-                               ignore_index=ignore_index, reduction=reduction)
+            loss = linear_cross_entropy(h.reshape(-1, h.size(-1)), self.head.weight, flat,
+                                        ignore_index, reduction, logits_bytes)
+        else:
+            logits = self.head(h)
+            loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), flat,
+                                   ignore_index=ignore_index, reduction=reduction)
         return loss.view(targets.shape) if reduction == "none" else loss
 
     def distill(self, idx, teacher_logits, teacher_ids, temperature: float = 1.0,

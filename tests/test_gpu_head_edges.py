@@ -162,3 +162,21 @@ def test_the_model_passes_on_what_may_be_held():
             assert logits <= n - held[0] < logits + logits // 8
         for a, b in zip(grads[0], grads[2]):   # (fp32's bar of the model's other paths)
             assert float((a - b).abs().max()) <= 1e-4 * float(a.abs().max()) + 1e-9
+
+
+def test_targets_of_any_shape():
+    """Targets (B T,) beside tokens (B, T), which forward takes: both of loss's paths."""
+    from mamba_metal_scan_amd import MambaConfig, TinyMamba
+    torch.manual_seed(0)
+    model = TinyMamba(MambaConfig(vocab_size=601, d_model=64, n_layers=1, d_ff=256,
+                                  scan_impl="hip")).to(DEV)
+    x = torch.randint(0, 601, (3, 40), generator=_gen(3), device=DEV)
+    for _ in range(2):
+        want = model.loss(x, x)
+        assert torch.equal(model.loss(x, x.view(-1)), want)
+        rows = model.loss(x, x.view(-1), reduction="none")
+        assert rows.shape == (120,)
+        assert torch.equal(rows.view(3, 40), model.loss(x, x, reduction="none"))
+        with pytest.raises(ValueError):
+            model.loss(x, x[:, :-1])
+        model.head.register_forward_hook(lambda m, a, o: None)   # then the logits' loss
