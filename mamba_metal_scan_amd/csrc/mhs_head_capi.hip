@@ -452,8 +452,8 @@ int64_t piece_words(int64_t rows, int64_t vocab, int es) {
 // of a split are written and read at about 4 TB/s; whole: 1 if one split's sums go
 // through memory too. (dh, 1001 x 384 x 16384, us: 4 splits 80, 16 35, 32 32; 8192 x
 // 640 x 16384: 2 splits 182, 5 206. dW split and whole, the loss and its gradients:
-// 8192 x 64 x 1009 84 and 172, 8192 x 640 x 8192 400 and 413, 8192 x 64 x 32768 524
-// and 677, 4096 x 640 x 16384 372 and 366; whole by this, 8192 x 1024 x 32768.)
+// 8192 x 64 x 1009 84 and 172, 8192 x 640 x 8192 400 and 413, 8192 x 64 x 32768 519
+// and 680, 4096 x 640 x 16384 372 and 366; whole by this, 8192 x 1024 x 32768.)
 KSplit bwd_splits(int64_t M, int64_t N, int64_t K, int whole) {
   const int64_t tiles = (M + Shape::BM - 1) / Shape::BM * ((N + Shape::BN - 1) / Shape::BN);
   const int64_t kt = (K + mhs::kMmK - 1) / mhs::kMmK;

@@ -60,13 +60,32 @@ def _keeps(hidden: torch.Tensor, weight: torch.Tensor, most: int) -> bool:
                                 most)
 
 
+def _layout(ts) -> list:
+    return [(t.dtype, t.device, t.shape, t.stride()) for t in ts]
+
+
+def _save(ctx, ts) -> None:
+    ctx.save_for_backward(*ts)
+    ctx.layout = None if torch.compiler.is_compiling() else _layout(ts)
+
+
 def _restored(t: torch.Tensor) -> torch.Tensor:
-    """A saved tensor as the kernels read it, whatever layout a saved-tensor hook
-    gave it back in (its type, shape and device are checked after)."""
     t = t.contiguous()
-    if torch.compiler.is_compiling() or t.data_ptr() % 16 == 0:
-        return t
-    return t.clone()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _saved(ctx, rows, check) -> tuple:
+    """The saved tensors as the kernels read them (the last one 16-byte aligned). A
+    saved-tensor hook may give them back in another layout, or changed: then matrices of
+    floats go through rows, the others are made dense, and check(*them) refuses what the
+    kernels would read past its end."""
+    ts = ctx.saved_tensors
+    if ctx.layout is None or torch.compiler.is_compiling() \
+            or (_layout(ts) == ctx.layout and ts[-1].data_ptr() % 16 == 0):
+        return ts
+    ts = tuple((rows if t.dim() == 2 and t.is_floating_point() else _restored)(t) for t in ts)
+    check(*ts)
+    return ts
 
 
 def _once() -> None:
@@ -103,18 +122,16 @@ class LinearCrossEntropyHIP(torch.autograd.Function):
         ctx.reduction = reduction
         loss, saved = LinearCrossEntropyHIP.loss(hidden, weight, targets, ignore_index, reduction,
                                                  most, any(ctx.needs_input_grad))
-        ctx.save_for_backward(*saved)
+        _save(ctx, saved)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         _once()
-        hidden, weight, targets, saved = ctx.saved_tensors
-        args = (g.contiguous(), _rows16(hidden), _rows16(weight), _restored(targets),
-                _restored(saved), ctx.reduction, *ctx.needs_input_grad[:2])
-        if not torch.compiler.is_compiling():   # (what a saved-tensor hook gave back)
-            _native._check_linear_xent_bwd(*args)
-        return (*_grads(ctx, *dispatch("linear_xent_bwd")(*args)), None, None, None, None)
+        g = g.contiguous()
+        rest = (ctx.reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        ts = _saved(ctx, _rows16, lambda *ts: _native._check_linear_xent_bwd(g, *ts, *rest))
+        return (*_grads(ctx, *dispatch("linear_xent_bwd")(g, *ts, *rest)), None, None, None, None)
 
 
 class LinearDistillHIP(torch.autograd.Function):
@@ -139,18 +156,17 @@ class LinearDistillHIP(torch.autograd.Function):
         ctx.temperature, ctx.reduction = temperature, reduction
         loss, saved = LinearDistillHIP.loss(hidden, weight, teacher_logits, ids, temperature,
                                             reduction, most, any(ctx.needs_input_grad))
-        ctx.save_for_backward(*saved)
+        _save(ctx, saved)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         _once()
-        hidden, weight, ids, saved = ctx.saved_tensors
-        args = (g.contiguous(), _rows16(hidden), _rows16(weight), _restored(ids),
-                _restored(saved), ctx.temperature, ctx.reduction, *ctx.needs_input_grad[:2])
-        if not torch.compiler.is_compiling():
-            _native._check_linear_distill_bwd(*args)
-        return (*_grads(ctx, *dispatch("linear_distill_bwd")(*args)), None, None, None, None, None)
+        g = g.contiguous()
+        rest = (ctx.temperature, ctx.reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        ts = _saved(ctx, _rows16, lambda *ts: _native._check_linear_distill_bwd(g, *ts, *rest))
+        return (*_grads(ctx, *dispatch("linear_distill_bwd")(g, *ts, *rest)),
+                None, None, None, None, None)
 
 
 class DistillHIP(torch.autograd.Function):
@@ -171,27 +187,32 @@ class DistillHIP(torch.autograd.Function):
     def forward(ctx, logits, teacher_logits, ids, temperature, reduction):
         ctx.temperature, ctx.reduction = temperature, reduction
         loss, saved = DistillHIP.loss(logits, teacher_logits, ids, temperature, reduction)
-        ctx.save_for_backward(*saved)
+        _save(ctx, saved)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         _once()
-        logits, ids, saved = ctx.saved_tensors
-        args = (g.contiguous(), _rows(logits), _restored(ids), _restored(saved), ctx.temperature,
-                ctx.reduction)
-        if not torch.compiler.is_compiling():
-            _native._check_distill_bwd(*args)
-        return dispatch("distill_bwd")(*args), None, None, None, None
+        g = g.contiguous()
+        rest = (ctx.temperature, ctx.reduction)
+        ts = _saved(ctx, _rows, lambda *ts: _native._check_distill_bwd(g, *ts, *rest))
+        return dispatch("distill_bwd")(g, *ts, *rest), None, None, None, None
+
+
+def _recorded(ts) -> bool:
+    """Whether autograd records what becomes of ts: one requires grad, or has a tangent."""
+    grad = torch.is_grad_enabled()
+    for t in ts:
+        if (grad and t.requires_grad) or unpack_dual(t).tangent is not None:
+            return True
+    return False
 
 
 def _apply(cls, leaves: int, *args):
     """cls.apply, or without autograd to record (scoring, serving) its forward
-    alone. (Leaves with a tangent go to apply too, which refuses forward-mode
+    alone. (Leaves with a tangent go to apply, which refuses forward-mode
     derivatives: its forward alone would leave them out.)"""
-    if torch.compiler.is_compiling() \
-            or (torch.is_grad_enabled() and any(t.requires_grad for t in args[:leaves])) \
-            or any(unpack_dual(t).tangent is not None for t in args[:leaves]):
+    if torch.compiler.is_compiling() or _recorded(args[:leaves]):
         return cls.apply(*args)
     return cls.loss(*args)[0]
 

@@ -10,7 +10,7 @@ from mamba_metal_scan_amd import (_native, distill_loss, head, linear_cross_entr
                                   linear_distill_loss)
 from mamba_metal_scan_amd._native import HipScanError
 
-ROWS, DIM, VOCAB, TOP = 6, 16, 40, 3
+ROWS, DIM, VOCAB, TOP = 6, 16, 41, 3
 
 
 @pytest.fixture
