@@ -425,10 +425,20 @@ struct HeadRows {
   float* q;               // (rows, k) the words' weights, see teacher_row
   float* loss;            // (rows)
   float* keep;            // (rows) 1: the row counts, 0: ignored or empty
+  KeptLogits kept;        // the forward's logits, or null
   int rows, vocab, dim, k, tiles;
   long long ignore;
   float temperature;
 };
+
+// The logit of row r and word id: one of the sums that lse2 is of. Where logits are kept
+// the ids' come from there, not from dot products of their own: their errors would not
+// cancel against lse2's in a row that is sure of its word (of 595 x 64 x 2832 fp32,
+// distillation, gradients off by 2.0e-6 of their norm for 1.0e-6 so).
+template <class T>
+__device__ __forceinline__ float kept_logit(const KeptLogits& kept, long long r, long long id) {
+  return kept.z[__is_same(T, Fp32) ? id * kept.ld + r : r * kept.ld + id];
+}
 
 // Cross entropy: W waves (1 or 4) per row. Bound by latency: 12 us at 8192 rows of
 // 640 and 128 tiles, 50 at 4096 and 512.
@@ -454,13 +464,17 @@ head_xent_rows_kernel(HeadRows g) {
   const float lse2 = m + log2f(s);
   const long long t = g.ids[r];
   const bool in = t >= 0 && t < g.vocab;
-  const elem_t<T>* const word[1] = {static_cast<const elem_t<T>*>(g.w) + (in ? t : 0) * g.ldw};
   float dot[1];
-  wave_dots<T, 1, W>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh, word, g.dim, dot);
-  if constexpr (W == 4) {
-    if ((lane & 63) == 0) red[lane >> 6] = dot[0];
-    __syncthreads();
-    dot[0] = red[0] + red[1] + red[2] + red[3];
+  if (g.kept.z) {
+    dot[0] = kept_logit<T>(g.kept, r, in ? t : 0);
+  } else {
+    const elem_t<T>* const word[1] = {static_cast<const elem_t<T>*>(g.w) + (in ? t : 0) * g.ldw};
+    wave_dots<T, 1, W>(static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh, word, g.dim, dot);
+    if constexpr (W == 4) {
+      if ((lane & 63) == 0) red[lane >> 6] = dot[0];
+      __syncthreads();
+      dot[0] = red[0] + red[1] + red[2] + red[3];
+    }
   }
   const float z = in ? dot[0] : 0.f;
   if (lane == 0) {
@@ -562,8 +576,16 @@ head_distill_rows_kernel(HeadRows g) {
   __shared__ float red[4];
   const int r = blockIdx.x, wave = threadIdx.x >> 6;
   const elem_t<T>* h = static_cast<const elem_t<T>*>(g.h) + (long long)r * g.ldh;
+  if (g.kept.z) {
+    for (int k = threadIdx.x; k < g.k; k += 256) {
+      const long long id = g.ids[(long long)r * g.k + k];
+      const bool in = id >= 0 && id < g.vocab;
+      zk[k] = in ? kept_logit<T>(g.kept, r, id) : 0.f;
+      g.picked[(long long)r * g.k + k] = zk[k];
+    }
+  }
   constexpr int U = 4;   // words at a time (8192 x 640, 64 words: one 138 us, four 105)
-  for (int k = U * wave; k < g.k; k += 4 * U) {
+  for (int k = U * wave; !g.kept.z && k < g.k; k += 4 * U) {
     const elem_t<T>* word[U];
     bool in[U];
 #pragma unroll

@@ -416,6 +416,7 @@ int head_fwd(const Head& p, mhs::HeadRows g, float* logits, float* loss, float* 
     g.ldh = p.ldh;
     g.ldw = p.ldw;
     g.part = part;
+    g.kept = kept_logits(p, logits);
     g.rows = (int)p.rows;
     g.vocab = (int)p.vocab;
     g.dim = (int)p.dim;

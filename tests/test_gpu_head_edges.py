@@ -180,3 +180,81 @@ def test_targets_of_any_shape():
         with pytest.raises(ValueError):
             model.loss(x, x[:, :-1])
         model.head.register_forward_hook(lambda m, a, o: None)   # then the logits' loss
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,vocab", [(4, 64, 900), (40, 1032, 301), (300, 64, 1300)])
+def test_captured_together(rows, dim, vocab, dtype):
+    """The three losses and their gradients in one graph, replayed with other data (rows
+    that do not count, a row of one value), eager work between the replays."""
+    print(f"[case] captured {dtype} {rows}x{dim}x{vocab}", flush=True)
+    dt = TYPES[dtype]
+
+    def data(seed):
+        h, w, t = _operands(rows, dim, vocab, dt, seed)
+        g = _gen(seed, rows)
+        t[1] = -100
+        ids = torch.randint(0, vocab, (rows, 4), generator=g, device=DEV)
+        ids[2] = -1
+        z = torch.randn(rows, vocab, generator=g, device=DEV).to(dt)
+        z[seed % 3] = torch.finfo(dt).min
+        return [h, w, t, ids, torch.randn(rows, 4, generator=g, device=DEV), z,
+                torch.randn(rows, generator=g, device=DEV)]
+
+    def run(h, w, t, ids, values, z, up):
+        h, w, z = (x.detach().requires_grad_() for x in (h, w, z))
+        losses = (linear_cross_entropy(h, w, t, reduction="none"),
+                  linear_distill_loss(h, w, values, ids, temperature=2.0, reduction="none"),
+                  distill_loss(z, values, ids, temperature=2.0, reduction="none"))
+        out = [x.detach() for x in losses]
+        out += torch.autograd.grad(losses[0], [h, w], up)
+        out += torch.autograd.grad(losses[1], [h, w], up)
+        return out + list(torch.autograd.grad(losses[2], [z], up))
+    sets = [data(i) for i in range(4)]
+    want = [run(*s) for s in sets]
+    held = [x.clone() for x in sets[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            run(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*held)
+    for s, ref in zip(sets, want):
+        for x, y in zip(held, s):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, ref):
+            assert torch.equal(x, y)
+        run(*sets[1])
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,vocab", [(3, 64, 130), (40, 64, 301), (33, 2056, 131),
+                                            (595, 64, 2832)])
+def test_logits_of_the_ids_are_those_of_the_sums(rows, dim, vocab, dtype):
+    """Where the forward keeps its logits, the ids' are taken from them: dot products of
+    their own would differ by the sums' rounding, which then does not cancel against the
+    log-sum-exp's in rows that are sure of their word."""
+    h, w, t = _operands(rows, dim, vocab, TYPES[dtype])
+    k = 5
+    ids = torch.randint(0, vocab, (rows, k), generator=_gen(rows), device=DEV)
+    ids[0, 0] = -1
+    ops = torch.ops.mamba_hip
+
+    def logits(saved, n):
+        n = (n + 3) // 4 * 4
+        a, b = (vocab, rows) if dtype == "f32" else (rows, vocab)
+        z = saved[n:].view(a, (b + 3) // 4 * 4)[:, :b]
+        return z.t() if dtype == "f32" else z
+    _, saved = ops.linear_xent_fwd(h, w, t, -100, 1, True)
+    z = logits(saved, 4 + 4 * rows)
+    assert torch.equal(saved[4 + 3 * rows:4 + 4 * rows], z.gather(1, t[:, None])[:, 0])
+    _, saved = ops.linear_distill_fwd(h, w, torch.zeros(rows, k, device=DEV), ids, 1.0, 1, True)
+    z = logits(saved, 4 + (3 + 2 * k) * rows)
+    picked = saved[4 + 3 * rows:4 + (3 + k) * rows].view(rows, k)
+    assert torch.equal(picked, torch.where(ids < 0, 0.0, z.gather(1, ids.clamp(min=0))))
