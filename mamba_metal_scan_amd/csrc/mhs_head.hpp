@@ -694,8 +694,9 @@ head_largest_kernel(RowScale rs, float* __restrict__ largest, long long rows) {
 // The power of two by which dz is stored larger, such that the largest |coef| lies
 // in [2^(to-1), 2^to); 1 where that is 0 or not finite. fp16: to 2^15, |dz| stays
 // below 2^16, and probabilities below 2^-24 of it keep their bits. fp32: to 2^32
-// (and never smaller: a row whose gradient is far below the largest keeps it), which takes the smallest probabilities (2^-126) to 2^-95, below which the fp32
-// product goes by fp32 MFMAs at half its rate (gemm3; 1024 x 4096 x 131072 of
+// (and never smaller: a row whose gradient is far below the largest keeps it), which
+// takes the smallest probabilities (2^-126) to 2^-95, below which the fp32 product goes
+// by fp32 MFMAs at half its rate (gemm3; 1024 x 4096 x 131072 of
 // logits of std 64 without it: 41.2 ms for loss and gradients, 22.5 with std 1).
 // bf16 products have no such bounds.
 __device__ __forceinline__ float lift_of(float largest, int to) {
@@ -713,9 +714,10 @@ constexpr int kCopyRows = 8;   // rows per block
 // 2^e alone and the sums take f: stored with coef, the id's element, about -coef,
 // would be off by the same rounding in every row (errors relative to the gradients'
 // norm: fp16 1001 x 384 x 50257 0.00030 to 0.00032, so 0.00025, of which 0.00021 is
-// the results' own rounding; bf16 8192 x 4096 x 131072 0.0025, so 0.0019, and 0.0017). rows2[r] = (2^e s, or
-// the row's coef s, lse2); scale[0] = f / s; and, `out` given, out (out_rows, per) = in (rows, per) in 16-byte words, rows ldi apart, with zeros in the rows past
-// `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
+// the results' own rounding; bf16 8192 x 4096 x 131072 0.0025, so 0.0019, and 0.0017).
+// rows2[r] = (2^e s, or the row's coef s, lse2); scale[0] = f / s; and, `out` given, out
+// (out_rows, per) = in (rows, per) in 16-byte words, rows ldi apart, with zeros in the
+// rows past `rows` and those whose coef is 0: what a padded row holds, NaN too, does not
 // reach dW.
 template <int UNUSED = 0>
 __global__ void __launch_bounds__(256)

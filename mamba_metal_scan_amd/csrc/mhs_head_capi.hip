@@ -845,7 +845,8 @@ int mhs_linear_distill_bwd(int dtype, const void* hidden, int64_t ldh, const voi
                            const float* q, const float* keep, const float* logits,
                            const float* upstream, const float* count, void* dhidden,
                            void* dweight, int64_t rows, int64_t vocab, int64_t dim, int64_t top,
-                           float temperature, int reduction, void* workspace, size_t workspace_bytes, void* stream) {
+                           float temperature, int reduction, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   mhs::clear_error();
   const Head p = head_of(dtype, hidden, ldh, weight, ldw, rows, vocab, dim);
   int rc = check_head(p);
