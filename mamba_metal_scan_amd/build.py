@@ -277,12 +277,12 @@ AUDIT = [
     ("bwd_reduce_kernel<4>", "dB / dC / dAneg partial sums", None, 4, 0),
     ("zero_grads_kernel<0>", "zero fill before the atomics", None, 4, 0),
     ("step_kernel_vec<1, 4>", "decode step, d_state 16", None, 4, 0),
-    ("gemm3_kernel<true, true, 128>", "product NT, 128 x 128 tiles", "gemm", 4, 128),
-    ("gemm3_kernel<true, false, 128>", "product NN, 128 x 128 tiles", "gemm", 4, 128),
-    ("gemm3_kernel<false, false, 128>", "product TN, 128 x 128 tiles", "gemm", 4, 128),
-    ("gemm3_kernel<true, true, 64>", "product NT, 64 x 64 tiles", "gemm", 4, 64),
-    ("gemm3_kernel<true, false, 64>", "product NN, 64 x 64 tiles", "gemm", 4, 64),
-    ("gemm3_kernel<false, false, 64>", "product TN, 64 x 64 tiles", "gemm", 4, 64),
+    ("gemm3_kernel<true, true, 128, false>", "product NT, 128 x 128 tiles", "gemm", 4, 128),
+    ("gemm3_kernel<true, false, 128, false>", "product NN, 128 x 128 tiles", "gemm", 4, 128),
+    ("gemm3_kernel<false, false, 128, false>", "product TN, 128 x 128 tiles", "gemm", 4, 128),
+    ("gemm3_kernel<true, true, 64, false>", "product NT, 64 x 64 tiles", "gemm", 4, 64),
+    ("gemm3_kernel<true, false, 64, false>", "product NN, 64 x 64 tiles", "gemm", 4, 64),
+    ("gemm3_kernel<false, false, 64, false>", "product TN, 64 x 64 tiles", "gemm", 4, 64),
     ("gemm_reduce_kernel<HIP_vector_type<float, 4u> >", "sum of a split product's partials",
      None, 4, 0),
     ("decode_product_kernel<0, 4, 2, 3>", "token, norm, in_proj and conv, batch 3 and 4", None,

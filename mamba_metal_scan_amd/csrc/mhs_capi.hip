@@ -1730,6 +1730,7 @@ int mhs::gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t
   if (form < MHS_GEMM_NT || form > MHS_GEMM_TN)
     return fail(MHS_EINVAL, "form must be MHS_GEMM_NT, _NN or _TN; got %d", form);
   if (!a || !b || !c) return fail(MHS_EINVAL, "null pointer argument");
+  if (alpha && form == MHS_GEMM_NT) return fail(MHS_EINVAL, "form NT takes no alpha");
   const bool a_k = form != MHS_GEMM_TN, b_k = form == MHS_GEMM_NT;   // K-major operands
   if (lda < (a_k ? k : m) || ldb < (b_k ? k : n) || ldc < n)
     return fail(MHS_EINVAL, "row strides too small: %lld %lld %lld", (long long)lda,
@@ -1765,11 +1766,16 @@ int mhs::gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t
   }
   const bool large = p.tile == mhs::kGemmTile;
   constexpr int L = mhs::kGemmTile, S = mhs::kGemmSmallTile;
-  const auto fn =
-      form == MHS_GEMM_NT ? (large ? &mhs::gemm3_kernel<true, true, L> : &mhs::gemm3_kernel<true, true, S>)
+  auto fn =
+      form == MHS_GEMM_NT
+          ? (large ? &mhs::gemm3_kernel<true, true, L, false> : &mhs::gemm3_kernel<true, true, S, false>)
       : form == MHS_GEMM_NN
-          ? (large ? &mhs::gemm3_kernel<true, false, L> : &mhs::gemm3_kernel<true, false, S>)
-          : (large ? &mhs::gemm3_kernel<false, false, L> : &mhs::gemm3_kernel<false, false, S>);
+          ? (large ? &mhs::gemm3_kernel<true, false, L, false> : &mhs::gemm3_kernel<true, false, S, false>)
+          : (large ? &mhs::gemm3_kernel<false, false, L, false> : &mhs::gemm3_kernel<false, false, S, false>);
+  if (alpha)
+    fn = form == MHS_GEMM_NN
+             ? (large ? &mhs::gemm3_kernel<true, false, L, true> : &mhs::gemm3_kernel<true, false, S, true>)
+             : (large ? &mhs::gemm3_kernel<false, false, L, true> : &mhs::gemm3_kernel<false, false, S, true>);
   hipLaunchKernelGGL(fn, dim3((unsigned)p.grid_m * (unsigned)p.grid_n, (unsigned)p.splits),
                      dim3(mhs::kGemmThreads), mhs::gemm_lds_bytes(p.tile, p.tile), s, g);
   rc = check_launch("matrix product kernel");

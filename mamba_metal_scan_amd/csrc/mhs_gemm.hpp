@@ -47,7 +47,7 @@ struct GemmArgs {
   long long lda, ldb, ldc;
   int kt_per_split;   // 16-deep k tiles per split
   int accumulate;     // C += (one split only)
-  const float* alpha; // device scalar that the product is multiplied by, or null: 1
+  const float* alpha; // SCALED: the device scalar that the product is multiplied by
   int grid_m, grid_n;
 };
 
@@ -370,8 +370,10 @@ __device__ __forceinline__ void gemm3_products(f32x16 (&acc)[TILE / 64][TILE / 6
 // i.e. 1.05-1.2 PFLOP/s of bf16, what an 8192^3 bf16 library product reaches
 // here (1.25). 256 x 128 tiles (two blocks per CU, a quarter fewer LDS reads)
 // were within 4% either way; each k tile's products summed from zero and then
-// added (a third of the error) took 8% longer.
-template <bool AK, bool BK, int TILE>
+// added (a third of the error) took 8% longer. SCALED: times alpha[0]; a kernel of its
+// own, for a multiplication by 1 in all of them cost 2% of short products (the 18M model's at
+// 509 rows: 30 launches 415 us, so 406).
+template <bool AK, bool BK, int TILE, bool SCALED>
 __global__ void __launch_bounds__(kGemmThreads, TILE == kGemmTile ? 3 : 4)
 gemm3_kernel(GemmArgs g) {
   constexpr int BM = TILE, BN = TILE;
@@ -386,7 +388,7 @@ gemm3_kernel(GemmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   float* const cb = g.C + (long long)blockIdx.y * g.M * g.ldc;
-  const float f = g.alpha ? *g.alpha : 1.f;
+  const float f = SCALED ? *g.alpha : 1.f;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -398,7 +400,8 @@ gemm3_kernel(GemmArgs g) {
         const int m = mb + 8 * (e / 4) + e % 4;
         if (m < g.M && n < g.N) {
           float* p = cb + (long long)m * g.ldc + n;
-          *p = g.accumulate ? *p + acc[i][j][e] * f : acc[i][j][e] * f;
+          const float v = SCALED ? acc[i][j][e] * f : acc[i][j][e];
+          *p = g.accumulate ? *p + v : v;
         }
       }
     }

@@ -13,7 +13,7 @@ void clear_error();
 int check_launch(const char* what);
 // Compute units of the current device.
 int device_cus();
-// mhs_gemm_f32 of alpha[0] (a device scalar; null: 1) times the product.
+// mhs_gemm_f32 of alpha[0] (a device scalar, forms NN and TN; null: 1) times the product.
 int gemm_f32(int form, const float* a, int64_t lda, const float* b, int64_t ldb, float* c,
              int64_t ldc, int64_t m, int64_t n, int64_t k, int accumulate, const float* alpha,
              void* workspace, size_t workspace_bytes, void* stream);
