@@ -258,3 +258,30 @@ def test_logits_of_the_ids_are_those_of_the_sums(rows, dim, vocab, dtype):
     z = logits(saved, 4 + (3 + 2 * k) * rows)
     picked = saved[4 + 3 * rows:4 + (3 + k) * rows].view(rows, k)
     assert torch.equal(picked, torch.where(ids < 0, 0.0, z.gather(1, ids.clamp(min=0))))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_kept_logits_past_32_bits(dtype, monkeypatch):
+    """More than 2^31 kept logits: the last rows' and words' gradients are those of
+    logits formed again (the ids' logits are another sum there, 2^-17 of a probability
+    by head_reference.py's bound of 64 terms; in bf16 they and the rest round once)."""
+    from mamba_metal_scan_amd import _native
+    print(f"[case] kept {dtype}", flush=True)
+    rows, dim, vocab = 70001, 64, 33003
+    h, w, t = _operands(rows, dim, vocab, TYPES[dtype])
+    t[-7:] = vocab - 1 - torch.arange(7, device=DEV)
+    up = torch.randn(rows, generator=_gen(2), device=DEV)
+    got = []
+    for keep in (True, False):
+        monkeypatch.setattr(_native, "keeps_logits", lambda *a: keep)
+        a, b = h.requires_grad_(), w.requires_grad_()
+        loss = linear_cross_entropy(a, b, t, reduction="none")
+        got.append((loss.detach(), *torch.autograd.grad(loss, [a, b], up)))
+        torch.cuda.empty_cache()
+    eps = torch.finfo(TYPES[dtype]).eps
+    assert float((got[0][0] - got[1][0]).abs().max()) <= 2.0 ** -14
+    rel = 2.0 ** -14 + (2 * eps if dtype == "bf16" else 0.0)
+    for x, y in zip(got[0][1:], got[1][1:]):
+        x, y = x.double(), y.double()
+        for part in (slice(None), slice(-300, None)):
+            assert float((x[part] - y[part]).norm()) <= rel * float(y[part].norm())
