@@ -446,9 +446,10 @@ int mhs_xent_bwd_f32(const float* logits, const int64_t* targets, const float* l
  *   there, (rows, vocab to a multiple of 4), for MHS_F32 (vocab, rows to a multiple
  *   of 4), and the backward reads them instead of forming them a second time.
  * Every sum runs in a fixed order (bit-for-bit reproducible). lse2 is held in fp32,
- * so a probability is off by 2^-24 |lse2| relative, and by more than that where the
- * logits themselves lie beyond 2^20 (temperatures, for distillation). The workspace
- * is 256-byte aligned; its size is 0 for arguments that the calls reject.
+ * so a probability is off by 2^-24 |lse2| relative: logits are meant to lie within
+ * 2^20 (temperatures, for distillation); from 2^30 on the sums of exponentials may
+ * overflow or vanish. The workspace is 256-byte aligned; its size is 0 for arguments
+ * that the calls reject.
  */
 #define MHS_F32 0
 #define MHS_BF16 1

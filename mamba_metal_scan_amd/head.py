@@ -286,7 +286,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     ignore_index makes its row's loss NaN. Fp32 logits (rows x V x 4 bytes) that take
     no more than logits_bytes, 1 GiB unless given, may be kept whole from forward to
     backward, where that is the faster; 0 keeps none. Under autocast hidden and weight are
-    taken in its type. The gradients are once differentiable."""
+    taken in its type. Logits are meant to lie within 2^20: a probability is off by 2^-24
+    of their size. The gradients are once differentiable."""
     what = "linear_cross_entropy"
     _hip(what, hidden, weight, targets)
     red = _reduction(what, reduction)
