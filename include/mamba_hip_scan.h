@@ -672,6 +672,101 @@ int mhs_block_bwd_f32(const mhs_block_weights* w, const float* x, const float* x
                       int64_t d_inner, int64_t d_state, int64_t conv_taps, int64_t chunk,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Packed sequences: nseq sequences of any lengths lie behind each other in the rows of
+ * (total, ...) tensors, row cu_seqlens[s] being the first of sequence s and
+ * cu_seqlens[s + 1] the first behind it (nseq + 1 numbers on the device, 32-bit, or
+ * 64-bit with cu64; cu_seqlens[0] is 0, none is smaller than the one before or larger
+ * than total; other numbers give undefined results but no access outside the
+ * tensors). Rows at or behind cu_seqlens[nseq] belong to no sequence: their outputs and
+ * gradients are zeros. dtype (MHS_F32, MHS_BF16, MHS_F16) is that of the activations
+ * and of their gradients; ld_* are the elements between their rows (the row's width
+ * and more, below 2^18); outputs are contiguous and overwritten. Sums and states are
+ * fp32, every reduction in a fixed order (bit-for-bit reproducible). Up to 2^17
+ * channels, 2^22 sequences, fewer than 2^31 rows. Workspaces are 256-byte aligned;
+ * two calls at once need two.
+ *
+ * The selective scan (the recurrence above, per sequence): aneg (dim, d_state) fp32; h0
+ * NULL (zeros) or (nseq, dim, d_state) fp32, the states before; h_last NULL or the
+ * states behind each sequence (h0's for one of no rows). ckpt: NULL, or
+ * mhs_packed_ckpt_floats floats for the backward. The backward takes the forward's
+ * inputs and ckpt, dy and dh_last (NULL: zeros); dh0 may be NULL.
+ */
+int64_t mhs_packed_ckpt_floats(int64_t total, int64_t dim, int64_t d_state);
+size_t mhs_packed_scan_workspace_bytes(int64_t nseq, int64_t total, int64_t dim, int64_t d_state,
+                                       int backward);
+int mhs_packed_scan_fwd(int dtype, const void* x, int64_t ld_x, const void* dt, int64_t ld_dt,
+                        const float* aneg, const void* B, int64_t ld_b, const void* C,
+                        int64_t ld_c, const void* cu_seqlens, int cu64, const float* h0, void* y,
+                        float* h_last, float* ckpt, int64_t nseq, int64_t total, int64_t dim,
+                        int64_t d_state, void* workspace, size_t workspace_bytes, void* stream);
+int mhs_packed_scan_bwd(int dtype, const void* x, int64_t ld_x, const void* dt, int64_t ld_dt,
+                        const float* aneg, const void* B, int64_t ld_b, const void* C,
+                        int64_t ld_c, const void* cu_seqlens, int cu64, const float* h0,
+                        const float* ckpt, const void* dy, int64_t ld_dy, const float* dh_last,
+                        void* dx, void* ddt, float* daneg, void* dB, void* dC, float* dh0,
+                        int64_t nseq, int64_t total, int64_t dim, int64_t d_state,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The causal depthwise conv1d + SiLU over packed sequences (the function of
+ * mhs_conv1d_silu_fwd_f32, per sequence): weight (dim, taps) and bias (dim) of
+ * dtype, or fp32 with weight_f32 (their gradients alike); taps in [1, 8]. window: NULL (zeros) or
+ * (nseq, dim, taps - 1) of dtype, the inputs before each sequence, oldest first;
+ * window_out: NULL or the last taps - 1 inputs behind it. The backward: dwindow_out NULL
+ * or window_out's gradient; dwindow NULL or window's.
+ */
+int mhs_packed_conv_fwd(int dtype, const void* x, int64_t ld_x, const void* weight,
+                        const void* bias, int weight_f32, const void* cu_seqlens, int cu64,
+                        const void* window, void* out, void* window_out, int64_t nseq,
+                        int64_t total, int64_t dim, int64_t taps, void* stream);
+size_t mhs_packed_conv_bwd_workspace_bytes(int64_t nseq, int64_t total, int64_t dim,
+                                           int64_t taps);
+int mhs_packed_conv_bwd(int dtype, const void* x, int64_t ld_x, const void* weight,
+                        const void* bias, int weight_f32, const void* cu_seqlens, int cu64,
+                        const void* window, const void* dout, int64_t ld_dout,
+                        const void* dwindow_out, void* dx, void* dweight, void* dbias,
+                        void* dwindow, int64_t nseq, int64_t total, int64_t dim, int64_t taps,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One token per row against a pool, in place: row r advances entry slots[r] (rows numbers
+ * on the device, 32-bit, or 64-bit with slots64; NULL: row r entry r, of a pool of at
+ * least as many). A slot below 0 is padding: the row's output is 0. A slot at or past
+ * `pool`, or one that an earlier row has too, makes the row's output NaN; neither
+ * touches an entry. window (pool, dim, taps - 1) of dtype; h (pool, dim, d_state)
+ * fp32; out, y (rows, dim) contiguous.
+ */
+int mhs_conv_step(int dtype, const void* x, int64_t ld_x, const void* weight, const void* bias,
+                  int weight_f32, void* window, const void* slots, int slots64, void* out,
+                  int64_t rows, int64_t pool, int64_t dim, int64_t taps, void* stream);
+int mhs_state_step(int dtype, float* h, const void* x, int64_t ld_x, const void* dt, int64_t ld_dt,
+                   const float* aneg, const void* B, int64_t ld_b, const void* C, int64_t ld_c,
+                   const void* slots, int slots64, void* y, int64_t rows, int64_t pool,
+                   int64_t dim, int64_t d_state, void* stream);
+
+/*
+ * Sampling of one token per row of logits (rows, vocab), rows ld elements apart, from a
+ * uniform number in [0, 1) per row. With m the row's largest logit, w_i = exp((l_i - m) /
+ * temperature) and the words in the order (logit descending, index ascending), kept are
+ * the first top_k (all if top_k < 1); of these those whose weight before them is below
+ * top_p of the k's total (all from top_p 1 on; the first always); of these those with
+ * w_i >= min_p. The token is the first kept word by index whose running sum of weights
+ * exceeds uniform times their total (a uniform number below 0 or NaN: the first; from 1
+ * on: the last). Temperature 0: the largest logit, at its lowest index. NaN logits count as
+ * -inf; a row that has +inf draws among those. Each setting is an array of a number per
+ * row or, where that is NULL, the value behind it. logprobs (or NULL): the log of the
+ * drawn word's share of the kept weight. A row whose logits are all -inf, or with a
+ * temperature below 0 or not finite, a min_p above 1 or a NaN setting, gives token -1 and
+ * NaN. Weights are summed as integers of 2^-45 (up to 2^17 words): the same token every
+ * run. vocab up to 2^24.
+ */
+int mhs_sample(int dtype, const void* logits, int64_t ld, const float* uniform,
+               const float* temperature, float temperature_value, const void* top_k, int top_k64,
+               int64_t top_k_value, const float* top_p, float top_p_value, const float* min_p,
+               float min_p_value, int64_t* tokens, float* logprobs, int64_t rows, int64_t vocab,
+               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

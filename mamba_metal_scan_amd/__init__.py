@@ -10,6 +10,9 @@ from .head import (DistillHIP, LinearCrossEntropyHIP, LinearDistillHIP, distill_
                    linear_cross_entropy, linear_distill_loss)
 from .model import MambaConfig, TinyMamba
 from .norm import AddRMSNormHIP, RMSNormHIP, add_rms_norm, rms_norm, rms_norm_residual
+from .packed import (ConvSiluPackedHIP, SelectiveScanPackedHIP, conv1d_silu_packed,
+                     conv1d_silu_step, selective_scan_packed, selective_state_step_slots)
+from .sampling import sample_tokens
 from .xent import CrossEntropyHIP, cross_entropy
 from .scan import (SSM_CHUNK, SelectiveScanHIP, selective_scan, selective_scan_hip,
                    selective_scan_metal, selective_scan_ref, selective_state_step)
@@ -20,4 +23,7 @@ __all__ = ["MambaConfig", "TinyMamba", "SSM_CHUNK", "SelectiveScanHIP", "selecti
            "SelectiveScanGatedHIP", "out_gate", "OutGateHIP", "mamba_inner", "MambaInnerHIP",
            "cross_entropy", "CrossEntropyHIP", "rms_norm", "rms_norm_residual", "RMSNormHIP",
            "add_rms_norm", "AddRMSNormHIP", "linear_cross_entropy", "LinearCrossEntropyHIP",
-           "distill_loss", "DistillHIP", "linear_distill_loss", "LinearDistillHIP"]
+           "distill_loss", "DistillHIP", "linear_distill_loss", "LinearDistillHIP",
+           "conv1d_silu_packed", "ConvSiluPackedHIP", "selective_scan_packed",
+           "SelectiveScanPackedHIP", "conv1d_silu_step", "selective_state_step_slots",
+           "sample_tokens"]

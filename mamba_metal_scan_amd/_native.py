@@ -44,7 +44,10 @@ EXPORTED_SYMBOLS = (
     "mhs_linear_xent_fwd_workspace_bytes", "mhs_linear_xent_fwd",
     "mhs_linear_xent_bwd_workspace_bytes", "mhs_linear_xent_bwd", "mhs_linear_distill_fwd",
     "mhs_linear_distill_bwd", "mhs_distill_workspace_bytes", "mhs_distill_fwd",
-    "mhs_distill_bwd",
+    "mhs_distill_bwd", "mhs_packed_ckpt_floats", "mhs_packed_scan_workspace_bytes",
+    "mhs_packed_scan_fwd", "mhs_packed_scan_bwd", "mhs_packed_conv_fwd",
+    "mhs_packed_conv_bwd_workspace_bytes", "mhs_packed_conv_bwd", "mhs_conv_step",
+    "mhs_state_step", "mhs_sample",
 )
 
 # Size of the static device scratch of mhs_scan_fwd_noalloc_f32 (the header's
@@ -196,6 +199,29 @@ def library() -> ctypes.CDLL:
                      [_int, _P, _I64] + [_P] * 8 + [_I64] * 3 + [_F32, _int, _P, _size, _P]),
                     ("mhs_distill_bwd",
                      [_int, _P, _I64] + [_P] * 7 + [_I64] * 3 + [_F32, _int, _P])):
+                getattr(lib, name).restype = _int
+                getattr(lib, name).argtypes = args
+            lib.mhs_packed_ckpt_floats.restype = _I64
+            lib.mhs_packed_ckpt_floats.argtypes = [_I64] * 3
+            lib.mhs_packed_scan_workspace_bytes.restype = _size
+            lib.mhs_packed_scan_workspace_bytes.argtypes = [_I64] * 4 + [_int]
+            lib.mhs_packed_conv_bwd_workspace_bytes.restype = _size
+            lib.mhs_packed_conv_bwd_workspace_bytes.argtypes = [_I64] * 4
+            row = [_P, _I64]                        # a tensor with its row stride
+            scan = [_int] + row * 2 + [_P] + row * 2 + [_P, _int, _P]
+            conv = [_int] + row + [_P, _P, _int, _P, _int, _P]
+            for name, args in (
+                    ("mhs_packed_scan_fwd", scan + [_P] * 3 + [_I64] * 4 + [_P, _size, _P]),
+                    ("mhs_packed_scan_bwd", scan + [_P] + row + [_P] * 7 + [_I64] * 4
+                     + [_P, _size, _P]),
+                    ("mhs_packed_conv_fwd", conv + [_P] * 2 + [_I64] * 4 + [_P]),
+                    ("mhs_packed_conv_bwd", conv + row + [_P] * 5 + [_I64] * 4 + [_P, _size, _P]),
+                    ("mhs_conv_step", [_int] + row + [_P, _P, _int, _P, _P, _int, _P]
+                     + [_I64] * 4 + [_P]),
+                    ("mhs_state_step", [_int, _P] + row * 2 + [_P] + row * 2 + [_P, _int, _P]
+                     + [_I64] * 4 + [_P]),
+                    ("mhs_sample", [_int] + row + [_P, _P, _F32, _P, _int, _I64, _P, _F32, _P, _F32,
+                                                   _P, _P, _I64, _I64, _P])):
                 getattr(lib, name).restype = _int
                 getattr(lib, name).argtypes = args
             _lib = lib

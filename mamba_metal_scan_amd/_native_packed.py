@@ -1,0 +1,411 @@
+"""The torch custom ops over packed sequences, tokens by slot and sampling: the
+part of the library's binding (``_native.py``) that packed.py and sampling.py use.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._native import (HEAD_DTYPES, HipScanError, _check, _fp32, _need, _on, _on_one_device, _ptr,
+                      _register, _shaped, _stream, library)
+
+DTYPES = HEAD_DTYPES            # activations: the library's number of each type
+MAX_TAPS = 8
+MAX_STATE = 64
+MAX_STRIDE = 1 << 18
+_INTS = (torch.int32, torch.int64)
+
+
+def rows_ok(t: torch.Tensor) -> bool:
+    """Whether the kernels read the 2-D t in place: its rows are dense, do not overlap,
+    and lie less than 2^18 elements apart."""
+    n, w = t.shape
+    return ((w <= 1 or t.stride(1) == 1)
+            and (n <= 1 or w <= t.stride(0) < MAX_STRIDE))
+
+
+def _ld(t: torch.Tensor) -> int:
+    n, w = t.shape
+    return t.stride(0) if n > 1 else w
+
+
+def _act(what: str, x: torch.Tensor, **like: Optional[torch.Tensor]) -> None:
+    """x (rows, D) and what is of its type, in rows that the kernels read."""
+    _need(x.dim() == 2, what, f"x must be (rows, D); got {tuple(x.shape)}")
+    for name, t in dict(x=x, **like).items():
+        if t is None:
+            continue
+        if t.dtype != x.dtype or x.dtype not in DTYPES:
+            raise HipScanError(f"{what}: {', '.join(['x', *like])} must all be float32, bfloat16 "
+                               f"or float16; got {x.dtype}, {name} {t.dtype}")
+        _need(t.dim() == 2 and rows_ok(t), what,
+              f"{name} needs dense rows less than 2^18 elements apart; got strides {t.stride()} "
+              f"for shape {tuple(t.shape)}")
+
+
+def _dense16(what: str, **ts: Optional[torch.Tensor]) -> None:
+    for name, t in ts.items():
+        if t is not None and not (t.is_contiguous() and t.data_ptr() % 16 == 0):
+            raise HipScanError(f"{what}: {name} must be contiguous and 16-byte aligned")
+
+
+def _seqs(what: str, cu: torch.Tensor) -> int:
+    """The number of sequences."""
+    _need(cu.dim() == 1 and cu.numel() >= 1 and cu.dtype in _INTS and cu.is_contiguous(), what,
+          "cu_seqlens must be a contiguous vector of int32 or int64, one number more than "
+          f"sequences; got {cu.dtype} {tuple(cu.shape)}")
+    return cu.numel() - 1
+
+
+def _no_state(x: torch.Tensor) -> torch.Tensor:
+    return x.new_empty((0,))
+
+
+# ----------------------------------------------------------------- the scan
+
+def _check_packed_scan(what: str, x, dt, aneg, b_in, c_in, cu, h0) -> None:
+    _on_one_device(what, x, dt, aneg, b_in, c_in, cu, h0)
+    _act(what, x, dt=dt, B=b_in, C=c_in)
+    _need(aneg.dim() == 2, what, f"Aneg must be (D, N); got {tuple(aneg.shape)}")
+    rows, d = x.shape
+    n = aneg.shape[1]
+    _need(1 <= n <= MAX_STATE and d >= 1, what,
+          f"D must be at least 1 and N in [1, {MAX_STATE}]; got {d}, {n}")
+    _shaped(what, "dt", dt, (rows, d))
+    _shaped(what, "Aneg", aneg, (d, n))
+    _shaped(what, "B", b_in, (rows, n))
+    _shaped(what, "C", c_in, (rows, n))
+    _shaped(what, "h0", h0, (_seqs(what, cu), d, n))
+    _fp32(what, Aneg=aneg, h0=h0)
+    _dense16(what, Aneg=aneg, h0=h0)
+
+
+def _scan_workspace(lib, x, n: int, seqs: int, backward: bool):
+    nbytes = lib.mhs_packed_scan_workspace_bytes(seqs, x.shape[0], x.shape[1], n, backward)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None), nbytes
+
+
+def _packed_scan_fwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
+                          b_in: torch.Tensor, c_in: torch.Tensor, cu: torch.Tensor,
+                          h0: Optional[torch.Tensor], want_state: bool, with_ckpt: bool
+                          ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, h_last, ckpt); the last two empty where not wanted."""
+    rows, d = x.shape
+    n, seqs = aneg.shape[1], cu.numel() - 1
+    lib = library()
+    y = x.new_empty((rows, d))
+    h_last = aneg.new_empty((seqs, d, n) if want_state else (0,))
+    ckpt = aneg.new_empty((lib.mhs_packed_ckpt_floats(rows, d, n) if with_ckpt else 0,))
+    with _on(x.device):
+        ws, nbytes = _scan_workspace(lib, x, n, seqs, False)
+        rc = lib.mhs_packed_scan_fwd(
+            DTYPES[x.dtype], x.data_ptr(), _ld(x), dt.data_ptr(), _ld(dt), aneg.data_ptr(),
+            b_in.data_ptr(), _ld(b_in), c_in.data_ptr(), _ld(c_in), cu.data_ptr(),
+            cu.dtype == torch.int64, _ptr(h0), y.data_ptr(),
+            h_last.data_ptr() if want_state else None, ckpt.data_ptr() if with_ckpt else None,
+            seqs, rows, d, n, _ptr(ws), nbytes, _stream(x.device))
+    _check(rc, "mhs_packed_scan_fwd")
+    return y, h_last, ckpt
+
+
+packed_scan_fwd = _register(
+    "packed_scan_fwd", _packed_scan_fwd_impl, (),
+    lambda x, dt, aneg, b_in, c_in, cu, h0, want_state, with_ckpt:
+    _check_packed_scan("packed_scan_fwd", x, dt, aneg, b_in, c_in, cu, h0))
+
+
+@packed_scan_fwd.register_fake
+def _packed_scan_fwd_fake(x, dt, aneg, b_in, c_in, cu, h0, want_state, with_ckpt):
+    rows, d = x.shape
+    n, seqs = aneg.shape[1], cu.shape[0] - 1
+    return (x.new_empty((rows, d)), aneg.new_empty((seqs, d, n) if want_state else (0,)),
+            aneg.new_empty((rows // 16 * d * n if with_ckpt else 0,)))
+
+
+def _packed_scan_bwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
+                          b_in: torch.Tensor, c_in: torch.Tensor, cu: torch.Tensor,
+                          h0: Optional[torch.Tensor], ckpt: torch.Tensor, dy: torch.Tensor,
+                          dh_last: Optional[torch.Tensor]
+                          ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                     torch.Tensor, torch.Tensor]:
+    """(dx, ddt, dAneg, dB, dC, dh0); the last empty without h0."""
+    rows, d = x.shape
+    n, seqs = aneg.shape[1], cu.numel() - 1
+    lib = library()
+    dx, ddt = x.new_empty((rows, d)), x.new_empty((rows, d))
+    db, dc = x.new_empty((rows, n)), x.new_empty((rows, n))
+    da = aneg.new_empty((d, n))
+    dh0 = aneg.new_empty((seqs, d, n) if h0 is not None else (0,))
+    with _on(x.device):
+        ws, nbytes = _scan_workspace(lib, x, n, seqs, True)
+        rc = lib.mhs_packed_scan_bwd(
+            DTYPES[x.dtype], x.data_ptr(), _ld(x), dt.data_ptr(), _ld(dt), aneg.data_ptr(),
+            b_in.data_ptr(), _ld(b_in), c_in.data_ptr(), _ld(c_in), cu.data_ptr(),
+            cu.dtype == torch.int64, _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy),
+            _ptr(dh_last), dx.data_ptr(), ddt.data_ptr(), da.data_ptr(), db.data_ptr(),
+            dc.data_ptr(), dh0.data_ptr() if h0 is not None else None, seqs, rows, d, n, _ptr(ws),
+            nbytes, _stream(x.device))
+    _check(rc, "mhs_packed_scan_bwd")
+    return dx, ddt, da, db, dc, dh0
+
+
+def _check_packed_scan_bwd(x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last) -> None:
+    what = "packed_scan_bwd"
+    _check_packed_scan(what, x, dt, aneg, b_in, c_in, cu, h0)
+    _on_one_device(what, x, ckpt, dy, dh_last)
+    _act(what, x, dy=dy)
+    rows, d = x.shape
+    n = aneg.shape[1]
+    _shaped(what, "dy", dy, (rows, d))
+    _shaped(what, "dh_last", dh_last, (cu.numel() - 1, d, n))
+    _shaped(what, "ckpt", ckpt, (rows // 16 * d * n,))
+    _fp32(what, ckpt=ckpt, dh_last=dh_last)
+    _dense16(what, ckpt=ckpt, dh_last=dh_last)
+
+
+packed_scan_bwd = _register("packed_scan_bwd", _packed_scan_bwd_impl, (), _check_packed_scan_bwd)
+
+
+@packed_scan_bwd.register_fake
+def _packed_scan_bwd_fake(x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last):
+    rows, d = x.shape
+    n = aneg.shape[1]
+    return (x.new_empty((rows, d)), x.new_empty((rows, d)), aneg.new_empty((d, n)),
+            x.new_empty((rows, n)), x.new_empty((rows, n)),
+            aneg.new_empty((cu.shape[0] - 1, d, n) if h0 is not None else (0,)))
+
+
+# ---------------------------------------------------------- the convolution
+
+def _check_taps(what: str, x, w, bias) -> None:
+    """w (D, K) and bias (D) of x's type, or both fp32."""
+    _need(w.dim() == 2 and 1 <= w.shape[1] <= MAX_TAPS and x.shape[1] >= 1, what,
+          f"w must be (D, K), D at least 1 and K in [1, {MAX_TAPS}]; got {tuple(w.shape)}")
+    _shaped(what, "w", w, (x.shape[1], w.shape[1]))
+    _shaped(what, "bias", bias, (x.shape[1],))
+    _need(w.dtype == bias.dtype and w.dtype in (x.dtype, torch.float32), what,
+          f"weight and bias must be of x's type {x.dtype} or both float32; got {w.dtype}, "
+          f"{bias.dtype}")
+    _need(w.is_contiguous() and bias.is_contiguous(), what, "weight and bias must be contiguous")
+
+
+def _check_packed_conv(what: str, x, w, bias, cu, window) -> None:
+    _on_one_device(what, x, w, bias, cu, window)
+    _act(what, x)
+    _check_taps(what, x, w, bias)
+    _shaped(what, "window", window, (_seqs(what, cu), x.shape[1], w.shape[1] - 1))
+    _need(window is None or (window.dtype == x.dtype and window.is_contiguous()), what,
+          f"window must be contiguous and of x's type {x.dtype}")
+
+
+def _packed_conv_fwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, cu: torch.Tensor,
+                          window: Optional[torch.Tensor], want_window: bool
+                          ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, the windows behind the sequences or an empty tensor)."""
+    rows, d = x.shape
+    k, seqs = w.shape[1], cu.numel() - 1
+    out = x.new_empty((rows, d))
+    last = x.new_empty((seqs, d, k - 1) if want_window else (0,))
+    with _on(x.device):
+        rc = library().mhs_packed_conv_fwd(
+            DTYPES[x.dtype], x.data_ptr(), _ld(x), w.data_ptr(), bias.data_ptr(),
+            w.dtype == torch.float32, cu.data_ptr(), cu.dtype == torch.int64, _ptr(window),
+            out.data_ptr(), last.data_ptr() if want_window else None, seqs, rows, d, k,
+            _stream(x.device))
+    _check(rc, "mhs_packed_conv_fwd")
+    return out, last
+
+
+packed_conv_fwd = _register(
+    "packed_conv_fwd", _packed_conv_fwd_impl, (),
+    lambda x, w, bias, cu, window, want_window:
+    _check_packed_conv("packed_conv_fwd", x, w, bias, cu, window))
+
+
+@packed_conv_fwd.register_fake
+def _packed_conv_fwd_fake(x, w, bias, cu, window, want_window):
+    rows, d = x.shape
+    return (x.new_empty((rows, d)),
+            x.new_empty((cu.shape[0] - 1, d, w.shape[1] - 1) if want_window else (0,)))
+
+
+def _packed_conv_bwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, cu: torch.Tensor,
+                          window: Optional[torch.Tensor], dout: torch.Tensor,
+                          dlast: Optional[torch.Tensor]
+                          ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw, dbias, dwindow); the last empty without a window."""
+    rows, d = x.shape
+    k, seqs = w.shape[1], cu.numel() - 1
+    lib = library()
+    dx, dw, db = x.new_empty((rows, d)), torch.empty_like(w), torch.empty_like(bias)
+    dwin = x.new_empty((seqs, d, k - 1) if window is not None else (0,))
+    with _on(x.device):
+        nbytes = lib.mhs_packed_conv_bwd_workspace_bytes(seqs, rows, d, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        rc = lib.mhs_packed_conv_bwd(
+            DTYPES[x.dtype], x.data_ptr(), _ld(x), w.data_ptr(), bias.data_ptr(),
+            w.dtype == torch.float32, cu.data_ptr(), cu.dtype == torch.int64, _ptr(window),
+            dout.data_ptr(), _ld(dout), _ptr(dlast), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+            dwin.data_ptr() if window is not None else None, seqs, rows, d, k, ws.data_ptr(),
+            nbytes, _stream(x.device))
+    _check(rc, "mhs_packed_conv_bwd")
+    return dx, dw, db, dwin
+
+
+def _check_packed_conv_bwd(x, w, bias, cu, window, dout, dlast) -> None:
+    what = "packed_conv_bwd"
+    _check_packed_conv(what, x, w, bias, cu, window)
+    _on_one_device(what, x, dout, dlast)
+    _act(what, x, dout=dout)
+    _shaped(what, "dout", dout, x.shape)
+    _shaped(what, "dlast", dlast, (cu.numel() - 1, x.shape[1], w.shape[1] - 1))
+    _need(dlast is None or (dlast.dtype == x.dtype and dlast.is_contiguous()), what,
+          f"dlast must be contiguous and of x's type {x.dtype}")
+
+
+packed_conv_bwd = _register("packed_conv_bwd", _packed_conv_bwd_impl, (), _check_packed_conv_bwd)
+
+
+@packed_conv_bwd.register_fake
+def _packed_conv_bwd_fake(x, w, bias, cu, window, dout, dlast):
+    return (x.new_empty(x.shape), torch.empty_like(w), torch.empty_like(bias),
+            x.new_empty((cu.shape[0] - 1, x.shape[1], w.shape[1] - 1) if window is not None
+                        else (0,)))
+
+
+# ------------------------------------------------------------ tokens by slot
+
+def _check_slots(what: str, slots, rows: int, pool: int) -> None:
+    if slots is None:
+        _need(rows <= pool, what, f"{rows} rows without slots need as many entries; got {pool}")
+    else:
+        _need(slots.dim() == 1 and slots.numel() == rows and slots.dtype in _INTS
+              and slots.is_contiguous(), what,
+              f"slots must be a contiguous int32 or int64 vector of {rows} numbers; got "
+              f"{slots.dtype} {tuple(slots.shape)}")
+
+
+def _check_conv_step(x, w, bias, window, slots) -> None:
+    what = "conv_step"
+    _on_one_device(what, x, w, bias, window, slots)
+    _act(what, x)
+    _check_taps(what, x, w, bias)
+    _need(window.dim() == 3 and window.dtype == x.dtype and window.is_contiguous(), what,
+          f"window must be contiguous (entries, D, K - 1) of x's type {x.dtype}; got "
+          f"{window.dtype} {tuple(window.shape)}")
+    _shaped(what, "window", window, (window.shape[0], x.shape[1], w.shape[1] - 1))
+    _check_slots(what, slots, x.shape[0], window.shape[0])
+
+
+def _conv_step_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, window: torch.Tensor,
+                    slots: Optional[torch.Tensor]) -> torch.Tensor:
+    """out (rows, D); window's entries advanced in place."""
+    rows, d = x.shape
+    out = x.new_empty((rows, d))
+    with _on(x.device):
+        rc = library().mhs_conv_step(
+            DTYPES[x.dtype], x.data_ptr(), _ld(x), w.data_ptr(), bias.data_ptr(),
+            w.dtype == torch.float32, window.data_ptr(), _ptr(slots),
+            slots is not None and slots.dtype == torch.int64, out.data_ptr(), rows,
+            window.shape[0], d, w.shape[1], _stream(x.device))
+    _check(rc, "mhs_conv_step")
+    return out
+
+
+conv_step = _register("conv_step", _conv_step_impl, ("window",), _check_conv_step)
+
+
+@conv_step.register_fake
+def _conv_step_fake(x, w, bias, window, slots):
+    return x.new_empty(x.shape)
+
+
+def _check_state_step(h, x, dt, aneg, b_in, c_in, slots) -> None:
+    what = "state_step"
+    _on_one_device(what, h, x, dt, aneg, b_in, c_in, slots)
+    _act(what, x, dt=dt, B=b_in, C=c_in)
+    _need(h.dim() == 3, what, f"h must be (entries, D, N); got {tuple(h.shape)}")
+    pool, d, n = h.shape
+    rows = x.shape[0]
+    _need(1 <= n <= MAX_STATE and d >= 1, what,
+          f"D must be at least 1 and N in [1, {MAX_STATE}]; got {d}, {n}")
+    for name, t, shape in (("x", x, (rows, d)), ("dt", dt, (rows, d)), ("Aneg", aneg, (d, n)),
+                           ("B", b_in, (rows, n)), ("C", c_in, (rows, n))):
+        _shaped(what, name, t, shape)
+    _fp32(what, h=h, Aneg=aneg)
+    _dense16(what, h=h, Aneg=aneg)
+    _check_slots(what, slots, rows, pool)
+
+
+def _state_step_impl(h: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
+                     b_in: torch.Tensor, c_in: torch.Tensor, slots: Optional[torch.Tensor]
+                     ) -> torch.Tensor:
+    """y (rows, D); h's entries advanced in place."""
+    rows, d = x.shape
+    y = x.new_empty((rows, d))
+    with _on(x.device):
+        rc = library().mhs_state_step(
+            DTYPES[x.dtype], h.data_ptr(), x.data_ptr(), _ld(x), dt.data_ptr(), _ld(dt),
+            aneg.data_ptr(), b_in.data_ptr(), _ld(b_in), c_in.data_ptr(), _ld(c_in), _ptr(slots),
+            slots is not None and slots.dtype == torch.int64, y.data_ptr(), rows, h.shape[0], d,
+            h.shape[2], _stream(x.device))
+    _check(rc, "mhs_state_step")
+    return y
+
+
+state_step = _register("state_step", _state_step_impl, ("h",), _check_state_step)
+
+
+@state_step.register_fake
+def _state_step_fake(h, x, dt, aneg, b_in, c_in, slots):
+    return x.new_empty(x.shape)
+
+
+# ----------------------------------------------------------------- sampling
+
+def _check_sample(logits, uniform, temperature, top_k, top_p, min_p, values_f, value_k) -> None:
+    what = "sample"
+    _on_one_device(what, logits, uniform, temperature, top_k, top_p, min_p)
+    _need(logits.dim() == 2 and logits.shape[1] >= 1 and logits.dtype in DTYPES, what,
+          "logits must be (rows, vocab) in float32, bfloat16 or float16; got "
+          f"{logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    _need((vocab <= 1 or logits.stride(1) == 1) and (rows <= 1 or logits.stride(0) >= vocab), what,
+          f"logits need contiguous rows; got strides {logits.stride()}")
+    for name, t, dtypes in (("uniform", uniform, (torch.float32,)),
+                            ("temperature", temperature, (torch.float32,)),
+                            ("top_k", top_k, _INTS), ("top_p", top_p, (torch.float32,)),
+                            ("min_p", min_p, (torch.float32,))):
+        _need(t is None or (t.shape == (rows,) and t.dtype in dtypes and t.is_contiguous()), what,
+              f"{name} must be a contiguous vector of {rows} {dtypes[0]}")
+    _need(len(values_f) == 3, what, "three values: temperature, top_p, min_p")
+
+
+def _sample_impl(logits: torch.Tensor, uniform: torch.Tensor, temperature: Optional[torch.Tensor],
+                 top_k: Optional[torch.Tensor], top_p: Optional[torch.Tensor],
+                 min_p: Optional[torch.Tensor], values_f: list[float], value_k: int
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(tokens, log-probabilities); settings of the rows, or where None the values."""
+    rows, vocab = logits.shape
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logps = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    with _on(logits.device):
+        rc = library().mhs_sample(
+            DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), uniform.data_ptr(),
+            _ptr(temperature), values_f[0], _ptr(top_k),
+            top_k is not None and top_k.dtype == torch.int64, value_k, _ptr(top_p), values_f[1],
+            _ptr(min_p), values_f[2], tokens.data_ptr(), logps.data_ptr(), rows, vocab,
+            _stream(logits.device))
+    _check(rc, "mhs_sample")
+    return tokens, logps
+
+
+sample = _register("sample", _sample_impl, (), _check_sample)
+
+
+@sample.register_fake
+def _sample_fake(logits, uniform, temperature, top_k, top_p, min_p, values_f, value_k):
+    rows = logits.shape[0]
+    return (torch.empty(rows, dtype=torch.int64, device=logits.device),
+            torch.empty(rows, dtype=torch.float32, device=logits.device))
