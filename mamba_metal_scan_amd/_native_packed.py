@@ -14,6 +14,7 @@ DTYPES = HEAD_DTYPES            # activations: the library's number of each type
 MAX_TAPS = 8
 MAX_STATE = 64
 MAX_STRIDE = 1 << 18
+CKPT = 8                        # rows between the scan's checkpoints
 _INTS = (torch.int32, torch.int64)
 
 
@@ -120,7 +121,7 @@ def _packed_scan_fwd_fake(x, dt, aneg, b_in, c_in, cu, h0, want_state, with_ckpt
     rows, d = x.shape
     n, seqs = aneg.shape[1], cu.shape[0] - 1
     return (x.new_empty((rows, d)), aneg.new_empty((seqs, d, n) if want_state else (0,)),
-            aneg.new_empty((rows // 16 * d * n if with_ckpt else 0,)))
+            aneg.new_empty((rows // CKPT * d * n if with_ckpt else 0,)))
 
 
 def _packed_scan_bwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
@@ -159,7 +160,7 @@ def _check_packed_scan_bwd(x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last) -
     n = aneg.shape[1]
     _shaped(what, "dy", dy, (rows, d))
     _shaped(what, "dh_last", dh_last, (cu.numel() - 1, d, n))
-    _shaped(what, "ckpt", ckpt, (rows // 16 * d * n,))
+    _shaped(what, "ckpt", ckpt, (rows // CKPT * d * n,))
     _fp32(what, ckpt=ckpt, dh_last=dh_last)
     _dense16(what, ckpt=ckpt, dh_last=dh_last)
 

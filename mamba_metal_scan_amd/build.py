@@ -27,11 +27,14 @@ ARCH = "gfx950"
 SOURCES = ["mhs_capi.hip", "mhs_kern_fwd_f32.hip", "mhs_kern_fwd_bf16.hip",
            "mhs_kern_bwd_f32.hip", "mhs_kern_bwd_bf16.hip", "mhs_kern_bwd_atom.hip",
            "mhs_kern_bwd_atom_bf16.hip", "mhs_head_capi.hip", "mhs_packed_capi.hip",
+           "mhs_packed_scan_f32.hip", "mhs_packed_scan_bf16.hip", "mhs_packed_scan_f16.hip",
            "mhs_sample_capi.hip"]
 HEADERS = ["mhs_common.hpp", "mhs_fwd.hpp", "mhs_bwd.hpp", "mhs_step.hpp", "mhs_conv.hpp",
            "mhs_gate.hpp", "mhs_instances.hpp", "mhs_xent.hpp", "mhs_norm.hpp", "mhs_gemm.hpp",
            "mhs_decode.hpp", "mhs_host.hpp", "mhs_mm16.hpp", "mhs_head.hpp", "mhs_distill.hpp",
-           "mhs_packed.hpp", "mhs_packed_scan.hpp", "mhs_packed_conv.hpp", "mhs_sample.hpp"]
+           "mhs_packed.hpp", "mhs_packed_scan.hpp", "mhs_packed_conv.hpp",
+           "mhs_packed_launch.hpp", "mhs_packed_instances.hpp", "mhs_packed_sum.hpp",
+           "mhs_sample.hpp"]
 
 
 def hipcc() -> str:

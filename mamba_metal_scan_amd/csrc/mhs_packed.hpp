@@ -1,5 +1,5 @@
-// What the kernels over packed sequences share: element types, the cut of the
-// sequences into pieces, and moves between lanes.
+// What the kernels over packed sequences share: element types and the cut of the
+// sequences into pieces.
 //
 // nseq sequences lie behind each other in the rows of (total, D) tensors: row
 // cu[s] is the first of sequence s, cu[s + 1] the first behind it; rows behind
@@ -127,90 +127,5 @@ __device__ __forceinline__ int seq_pieces(const Seqs& q, int tc, int s, int* fir
   *first = b / tc + s;
   return max(1, (e - b + tc - 1) / tc);
 }
-
-// ------------------------------------------------------- moves between lanes
-
-// Row r of the wave (its 16 lanes 16 r ..) holds step r in v: o[s] is step s in
-// every row.
-__device__ __forceinline__ void spread_rows(float v, float (&o)[4]) {
-  const unsigned u = __float_as_uint(v);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);   // rows 0101, 2323
-  const auto b = __builtin_amdgcn_permlane16_swap(a[0], a[0], false, false);
-  const auto c = __builtin_amdgcn_permlane16_swap(a[1], a[1], false, false);
-  o[0] = __uint_as_float(b[0]);
-  o[1] = __uint_as_float(b[1]);
-  o[2] = __uint_as_float(c[0]);
-  o[3] = __uint_as_float(c[1]);
-}
-
-// The way back: the sum over the four rows of v[s], in row s.
-__device__ __forceinline__ float gather_rows(const float (&v)[4]) {
-  const auto swap32 = [](float x, float y) {
-    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false,
-                                                    false);
-    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-  };
-  // rows 0, 1: the two halves' sum of v[0] (v[1]); rows 2, 3: of v[2] (v[3])
-  const float a = swap32(v[0], v[2]), b = swap32(v[1], v[3]);
-  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false,
-                                                  false);
-  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-}
-
-// Lane K of each row of b, times v (the compiler folds the broadcast into the
-// multiply); y += that (it does not fold it into a multiply-add: by hand. b
-// must not come from a VALU instruction less than two instructions before).
-template <int K>
-__device__ __forceinline__ float row_mul(float b, float v) {
-  return dpp_get<0x150 + K>(b) * v;
-}
-template <int K>
-__device__ __forceinline__ void row_fmac(float& y, float b, float v) {
-  asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf"
-      : "+v"(y)
-      : "v"(b), "v"(v), "n"(K));
-}
-// The two wait states between VALU writes of v and row_fmac's reads of it.
-template <int M>
-__device__ __forceinline__ void row_fmac_ready(float (&v)[M]) {
-  static_assert(M == 1 || M == 2 || M == 4, "one, two or four registers");
-  if constexpr (M == 1) asm("s_nop 1" : "+v"(v[0]));
-  else if constexpr (M == 2) asm("s_nop 1" : "+v"(v[0]), "+v"(v[1]));
-  else asm("s_nop 1" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
-}
-
-// ------------------------------------------------------------- states
-
-// The NPL states n0 .. of channel d in a (D, N) slice: an address of the first
-// and how many of them there are; whole vectors where N allows them.
-template <int NPL>
-struct StateAt {
-  size_t off;
-  int valid;   // 0 .. NPL
-  bool vec;
-  __device__ __forceinline__ StateAt(int d, int n0, int D, int N)
-      : off((size_t)d * N + n0), valid(d < D ? max(0, min(NPL, N - n0)) : 0),
-        vec(N % NPL == 0) {}
-  __device__ __forceinline__ void load(float (&v)[NPL], const float* p) const {
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) v[j] = 0.f;
-    if (vec) {
-      if (valid) load_vec<NPL>(v, p + off);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NPL; ++j)
-        if (j < valid) v[j] = p[off + j];
-    }
-  }
-  __device__ __forceinline__ void store(float* p, const float (&v)[NPL]) const {
-    if (vec) {
-      if (valid) store_vec<NPL>(p + off, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NPL; ++j)
-        if (j < valid) p[off + j] = v[j];
-    }
-  }
-};
 
 }  // namespace mhs

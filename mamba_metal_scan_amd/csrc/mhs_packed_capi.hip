@@ -8,7 +8,8 @@
 #include "mamba_hip_scan.h"
 #include "mhs_host.hpp"
 #include "mhs_packed_conv.hpp"
-#include "mhs_packed_scan.hpp"
+#include "mhs_packed_launch.hpp"
+#include "mhs_packed_sum.hpp"
 
 namespace {
 
@@ -65,30 +66,22 @@ int64_t piece_count(int64_t total, int64_t nseq, int tc) { return total / tc + n
 
 // ---------------------------------------------------------------- the scan
 
-// State groups (waves) of a block and states of a lane, by d_state.
-int states_per_lane(int64_t n) { return n <= 4 ? 1 : n <= 8 ? 2 : 4; }
-int state_waves(int64_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
-int block_chans(int64_t n) { return 16 * (4 / state_waves(n)); }
-
-// Rows of a piece: enough pieces to fill the GPU, as long as they go with that.
-int scan_piece(int64_t total, int64_t dim, int64_t n) {
-  const int64_t blocks = (dim + block_chans(n) - 1) / block_chans(n);
-  const int64_t want = 2 * device_cus();           // blocks of 4 waves
-  const int64_t pieces = std::max<int64_t>(1, want / blocks);
+// Rows of a piece: as many pieces as give each SIMD twelve waves, eight in the backward, which
+// holds two at a time (their latencies then hide each other's, and pieces of unlike
+// length even out).
+int scan_piece(int64_t total, int64_t dim, int64_t n, bool back) {
+  const int64_t waves = (dim + 31) / 32 * mhs::scan_state_waves(n);
+  const int64_t pieces = std::max<int64_t>(1, (back ? 32 : 48) * device_cus() / waves);
   const int64_t tc = total / pieces / mhs::kSub * mhs::kSub;
-  return (int)std::min<int64_t>(1024, std::max<int64_t>(64, tc));
+  return (int)std::min<int64_t>(1024, std::max<int64_t>(32, tc));
 }
 
-struct ScanPlan {
-  int tc;
-  int64_t pieces, blocks;
-  bool carried;   // whether a sequence can be longer than a piece
-};
-ScanPlan scan_plan(int64_t total, int64_t nseq, int64_t dim, int64_t n) {
+using mhs::ScanPlan;
+ScanPlan scan_plan(int64_t total, int64_t nseq, int64_t dim, int64_t n, bool back) {
   ScanPlan p;
-  p.tc = scan_piece(total, dim, n);
+  p.tc = scan_piece(total, dim, n, back);
   p.pieces = piece_count(total, nseq, p.tc);
-  p.blocks = (dim + block_chans(n) - 1) / block_chans(n);
+  p.blocks = (dim + mhs::scan_block_chans(n) - 1) / mhs::scan_block_chans(n);
   p.carried = total > p.tc;
   return p;
 }
@@ -99,7 +92,7 @@ int check_scan(int dtype, const void* cu, int64_t nseq, int64_t total, int64_t d
   if ((rc = check_packed(cu, nseq, total, dim))) return rc;
   if (n < 1 || n > MHS_MAX_DSTATE)
     return fail(MHS_EINVAL, "d_state must be in [1, %d]; got %lld", MHS_MAX_DSTATE, (long long)n);
-  const ScanPlan p = scan_plan(total, nseq, dim, n);
+  const ScanPlan p = scan_plan(total, nseq, dim, n, false);   // (the shorter pieces)
   // (a launch counts its threads in 32 bits: the pass, the fold, the sums)
   if (p.pieces * p.blocks >= 1LL << 24 || nseq * ((dim * n + 255) / 256) >= 1LL << 24 ||
       total * 2 * n >= 1LL << 32)
@@ -137,41 +130,11 @@ size_t scan_parts(void* ws, const ScanPlan& p, int64_t total, int64_t dim, int64
   return w.used;
 }
 
-template <class T, int NPL, int WS, bool CARRY>
-void launch_scan(bool back, const mhs::PackedScanArgs& a, const ScanPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.pieces, (unsigned)p.blocks);
-  if (back) mhs::packed_scan_bwd_kernel<T, NPL, WS, CARRY><<<grid, 256, 0, s>>>(a);
-  else mhs::packed_scan_fwd_kernel<T, NPL, WS, CARRY><<<grid, 256, 0, s>>>(a);
-}
-template <class T, int NPL, int WS>
-int run_scan(bool back, const mhs::PackedScanArgs& a, const ScanPlan& p, hipStream_t s) {
-  if (p.carried && a.q.nseq > 0) {
-    launch_scan<T, NPL, WS, true>(back, a, p, s);
-    int rc = check_launch("packed scan carry kernel");
-    if (rc) return rc;
-    const dim3 grid((unsigned)a.q.nseq, (unsigned)(((int64_t)a.D * a.N + 255) / 256));
-    if (back) mhs::packed_fold_kernel<true><<<grid, 256, 0, s>>>(a);
-    else mhs::packed_fold_kernel<false><<<grid, 256, 0, s>>>(a);
-    if ((rc = check_launch("packed scan fold kernel"))) return rc;
-  }
-  launch_scan<T, NPL, WS, false>(back, a, p, s);
-  return check_launch("packed scan kernel");
-}
-template <class T>
-int run_scan_n(bool back, const mhs::PackedScanArgs& a, const ScanPlan& p, hipStream_t s) {
-  switch (states_per_lane(a.N) * 8 + state_waves(a.N)) {
-    case 1 * 8 + 1: return run_scan<T, 1, 1>(back, a, p, s);
-    case 2 * 8 + 1: return run_scan<T, 2, 1>(back, a, p, s);
-    case 4 * 8 + 1: return run_scan<T, 4, 1>(back, a, p, s);
-    case 4 * 8 + 2: return run_scan<T, 4, 2>(back, a, p, s);
-    default: return run_scan<T, 4, 4>(back, a, p, s);
-  }
-}
 int run_scan_t(int dtype, bool back, const mhs::PackedScanArgs& a, const ScanPlan& p,
                hipStream_t s) {
-  if (dtype == MHS_F32) return run_scan_n<mhs::F32>(back, a, p, s);
-  if (dtype == MHS_BF16) return run_scan_n<mhs::Bf16>(back, a, p, s);
-  return run_scan_n<mhs::Fp16>(back, a, p, s);
+  if (dtype == MHS_F32) return mhs::run_packed_scan<mhs::F32>(back, a, p, s);
+  if (dtype == MHS_BF16) return mhs::run_packed_scan<mhs::Bf16>(back, a, p, s);
+  return mhs::run_packed_scan<mhs::Fp16>(back, a, p, s);
 }
 
 // --------------------------------------------------------- the convolution
@@ -288,15 +251,15 @@ void run_state_step(const mhs::StateStepArgs& a, hipStream_t s) {
 extern "C" {
 
 int64_t mhs_packed_ckpt_floats(int64_t total, int64_t dim, int64_t d_state) {
-  return total / mhs::kSub * dim * d_state;
+  return total / mhs::kCkpt * dim * d_state;
 }
 
 size_t mhs_packed_scan_workspace_bytes(int64_t nseq, int64_t total, int64_t dim, int64_t d_state,
                                        int backward) {
   mhs::clear_error();
   if (check_scan(MHS_F32, &nseq, nseq, total, dim, d_state)) return 0;
-  return scan_parts(nullptr, scan_plan(total, nseq, dim, d_state), total, dim, d_state,
-                    backward != 0, nullptr);
+  return scan_parts(nullptr, scan_plan(total, nseq, dim, d_state, backward != 0), total, dim,
+                    d_state, backward != 0, nullptr);
 }
 
 int mhs_packed_scan_fwd(int dtype, const void* x, int64_t ld_x, const void* dt, int64_t ld_dt,
@@ -315,7 +278,7 @@ int mhs_packed_scan_fwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
   for (const float* p : {aneg, h0, (const float*)h_last, (const float*)ckpt})
     if (!aligned16(p)) return fail(MHS_EINVAL, "fp32 tensors must be 16-byte aligned");
   mhs::PackedScanArgs a{};
-  const ScanPlan p = scan_plan(total, nseq, dim, d_state);
+  const ScanPlan p = scan_plan(total, nseq, dim, d_state, false);
   if ((rc = check_workspace(workspace, workspace_bytes,
                             scan_parts(workspace, p, total, dim, d_state, false, &a))))
     return rc;
@@ -339,7 +302,7 @@ int mhs_packed_scan_bwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
   if (rc) return rc;
   if (!aneg || !daneg ||
       (total > 0 && (!x || !dt || !B || !C || !dy || !dx || !ddt || !dB || !dC)) ||
-      (total >= mhs::kSub && !ckpt))
+      (total >= mhs::kCkpt && !ckpt))
     return fail(MHS_EINVAL, "null pointer argument");
   if ((rc = check_ld("x", ld_x, dim)) || (rc = check_ld("dt", ld_dt, dim)) ||
       (rc = check_ld("B", ld_b, d_state)) || (rc = check_ld("C", ld_c, d_state)) ||
@@ -348,7 +311,7 @@ int mhs_packed_scan_bwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
   for (const float* p : {aneg, h0, ckpt, dh_last, (const float*)daneg, (const float*)dh0})
     if (!aligned16(p)) return fail(MHS_EINVAL, "fp32 tensors must be 16-byte aligned");
   mhs::PackedScanArgs a{};
-  const ScanPlan p = scan_plan(total, nseq, dim, d_state);
+  const ScanPlan p = scan_plan(total, nseq, dim, d_state, true);
   if ((rc = check_workspace(workspace, workspace_bytes,
                             scan_parts(workspace, p, total, dim, d_state, true, &a))))
     return rc;
@@ -374,7 +337,7 @@ int mhs_packed_scan_bwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
     if ((rc = check_launch("packed scan dB / dC sums"))) return rc;
   }
   const int slice = a.D * a.N;
-  mhs::packed_sum_a_kernel<<<(slice + 63) / 64, 256, 0, s>>>(a.part_a, daneg, (int)p.pieces, slice);
+  mhs::packed_sum_a_kernel<<<(slice + 63) / 64, 1024, 0, s>>>(a.part_a, daneg, (int)p.pieces, slice);
   return check_launch("packed scan dAneg sum");
 }
 

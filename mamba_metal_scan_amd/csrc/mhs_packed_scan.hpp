@@ -3,14 +3,15 @@
 //   h_t = exp(-dt_t Aneg) h_{t-1} + dt_t x_t B_t,   y_t = sum_n C_tn h_tn
 // per sequence, from h0 (nseq, D, N) or from zero.
 //
-// Mapping. A wave holds 16 channels in its four rows of 16 lanes; the rows
-// split the states, NPL each (4 NPL states a wave; a block has WS waves for
-// the states and 4 / WS times 16 channels). Time goes in sub-chunks of 16
-// steps. A register of x or dt is loaded for four steps at once, row r step r,
-// and spread to the rows by swaps between them; B and C lie in the lanes of a
-// row, 16 / NPL steps of the row's NPL states a register, and are broadcast
-// within the multiply that uses them. The waves of a block run without
-// barriers (but for the sum of y over WS > 1 waves).
+// Mapping. The four lanes of a quad split the states of two neighbouring channels, NPL
+// each (4 NPL states a wave; a block has WS waves for the states and 4 / WS
+// times 32 channels). A register of x, dt or dy holds four steps, lane q of the
+// quad step q, and is broadcast within the multiply or multiply-add that uses it (a quad
+// permutation). B and C, which all channels share, go through LDS: a lane reads
+// its NPL states of a step at once. Each wave has its own tile of them, so that the waves
+// of a block run without barriers (but for sums over waves). The sums over the
+// states are sums over a quad, those over the channels sums over the other four bits of
+// the lane, which every step of a reduce-scatter halves without a select.
 //
 // A sequence longer than a piece takes three launches: the carry pass walks
 // each piece but the last from a zero state and leaves its end state and its
@@ -23,7 +24,8 @@
 
 namespace mhs {
 
-constexpr int kSub = 16;   // steps of a sub-chunk
+constexpr int kCkpt = 8;   // rows between checkpoints, and of a sub-chunk of the backward
+constexpr int kSub = 16;   // rows of a sub-chunk of the forward and the carry passes
 
 struct PackedScanArgs {
   Seqs q;
@@ -33,8 +35,8 @@ struct PackedScanArgs {
   const float* h0;       // null: zeros
   void* y;               // (total, D)
   float* h_last;         // null: not wanted
-  float* ckpt;           // (total / 16, D, N), null: not wanted. Entry begin / 16 + g - 1 is the
-                         // state before step 16 g of its sequence, g >= 1
+  float* ckpt;           // (total / 8, D, N), null: not wanted. Entry begin / 8 + g - 1 is the
+                         // state before step 8 g of its sequence, g >= 1
   float* carry;          // (pieces, D, N): the carry pass's states (adjoints) at the pieces' ends
   float* sdt;            // (pieces, D): its sums of dt
   float* start;          // (pieces, D, N): the states (adjoints) that the main pass starts from
@@ -60,69 +62,217 @@ __device__ __forceinline__ void zero_rows(void* out, int t0, int len, int D, int
 template <int NPL, int WS>
 struct ScanLane {
   static constexpr int kStates = 4 * NPL;        // of a wave
-  static constexpr int kChans = 16 * (4 / WS);   // of a block
-  int wave, lane, row, c, ws, wc, d, n0;
-  bool act;
+  static constexpr int kChans = 32 * (4 / WS);   // of a block
+  int wave, lane, q, ws, wc, d, n0;
+  bool act[2];
   __device__ __forceinline__ explicit ScanLane(int D) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     lane = threadIdx.x & 63;
-    row = lane >> 4;
-    c = lane & 15;
+    q = lane & 3;
     ws = wave % WS;
     wc = wave / WS;
-    d = blockIdx.y * kChans + wc * 16 + c;
-    n0 = ws * kStates + row * NPL;
-    act = d < D;
+    d = blockIdx.y * kChans + wc * 32 + 2 * (lane >> 2);
+    n0 = ws * kStates + q * NPL;
+    act[0] = d < D;
+    act[1] = d + 1 < D;
   }
 };
 
-// One operand of the channels, (rows, D): register k of sub-chunk i holds step
-// 4 k + r of it in row r, 0 behind the piece's end.
-template <class T>
+// The states of a lane's two channels in (D, N) slices. VEC: whole vectors of them (N
+// divides by NPL). No access has a branch: what is not there lies past the slice.
+template <int NPL, bool VEC>
+struct StatePair {
+  unsigned bytes, off[2];
+  int valid;
+  __device__ __forceinline__ StatePair(int d, int n0, int D, int N, const bool (&act)[2])
+      : bytes(4u * (unsigned)D * (unsigned)N), valid(N - n0) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      off[c] = act[c] && valid > 0 ? 4u * ((unsigned)(d + c) * (unsigned)N + n0) : kOOB;
+  }
+  __device__ __forceinline__ void load(float (&v)[2][NPL], const float* p, bool there = true) const {
+    const GBuf g(p, there ? bytes : 0u);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if constexpr (VEC && NPL == 4) {
+        const auto r = __builtin_amdgcn_raw_buffer_load_b128(g.r, off[c], 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[c][j] = __uint_as_float(r[j]);
+      } else if constexpr (VEC && NPL == 2) {
+        const auto r = __builtin_amdgcn_raw_buffer_load_b64(g.r, off[c], 0, 0);
+        v[c][0] = __uint_as_float(r[0]);
+        v[c][1] = __uint_as_float(r[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) v[c][j] = g.ld(j < valid ? off[c] + 4u * j : kOOB);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* p, const float (&v)[2][NPL],
+                                        bool there = true) const {
+    const GBuf g(p, there ? bytes : 0u);
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if constexpr (VEC && NPL == 4) {
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u4{__float_as_uint(v[c][0]), __float_as_uint(v[c][1]), __float_as_uint(v[c][2]),
+               __float_as_uint(v[c][3])}, g.r, off[c], 0, 0);
+      } else if constexpr (VEC && NPL == 2) {
+        __builtin_amdgcn_raw_buffer_store_b64(
+            u2{__float_as_uint(v[c][0]), __float_as_uint(v[c][1])}, g.r, off[c], 0, 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) g.st(v[c][j], j < valid ? off[c] + 4u * j : kOOB);
+      }
+    }
+  }
+};
+
+// One operand of the channels, (rows, D): register [c][k] of the S rows from row i S of the
+// piece on holds row 4 k + q of channel d + c, 0 behind the piece's end.
+// VEC: both channels in one access.
+template <class T, int S, bool VEC>
 struct ChanLoad {
+  static constexpr int E = kElem<T>;
   GBuf g;
-  unsigned off, step4, sub;
+  unsigned off[2], step4, sub;
   __device__ __forceinline__ ChanLoad(const void* base, int ld, int t0, int len, int D, int d,
-                                      int row, bool act)
-      : g(buf_t<T>(base, (size_t)t0 * ld,
-                   len > 0 ? kElem<T> * ((unsigned)(len - 1) * ld + D) : 0u)),
-        off(act ? kElem<T> * ((unsigned)row * ld + d) : kOOB), step4(4 * kElem<T> * ld),
-        sub(16 * kElem<T> * ld) {}
-  __device__ __forceinline__ void load(float (&v)[4], int i) const {
+                                      int q, const bool (&act)[2])
+      : g(buf_t<T>(base, (size_t)t0 * ld, len > 0 ? E * ((unsigned)(len - 1) * ld + D) : 0u)),
+        step4(4 * E * ld), sub(S * E * ld) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = ld_t<T>(g, off + (unsigned)i * sub + k * step4);
+    for (int c = 0; c < 2; ++c) off[c] = act[c] ? E * ((unsigned)q * ld + d + c) : kOOB;
   }
-  __device__ __forceinline__ void store(float v, int i, int k) const {
-    st_t<T>(g, v, off + (unsigned)i * sub + k * step4);
+  __device__ __forceinline__ void load(float (&v)[2][S / 4], int i) const {
+#pragma unroll
+    for (int k = 0; k < S / 4; ++k) {
+      const unsigned o = (unsigned)i * sub + k * step4;
+      if constexpr (!VEC) {
+        v[0][k] = ld_t<T>(g, off[0] + o);
+        v[1][k] = ld_t<T>(g, off[1] + o);
+      } else if constexpr (E == 4) {
+        const auto r = __builtin_amdgcn_raw_buffer_load_b64(g.r, off[0] + o, 0, 0);
+        v[0][k] = __uint_as_float(r[0]);
+        v[1][k] = __uint_as_float(r[1]);
+      } else {
+        const unsigned r = __builtin_amdgcn_raw_buffer_load_b32(g.r, off[0] + o, 0, 0);
+        v[0][k] = T::to((unsigned short)r);
+        v[1][k] = T::to((unsigned short)(r >> 16));
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float v0, float v1, int i, int k) const {
+    const unsigned o = (unsigned)i * sub + k * step4;
+    if constexpr (!VEC) {
+      st_t<T>(g, v0, off[0] + o);
+      st_t<T>(g, v1, off[1] + o);
+    } else if constexpr (E == 4) {
+      typedef unsigned u2 __attribute__((ext_vector_type(2)));
+      __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(v0), __float_as_uint(v1)}, g.r,
+                                            off[0] + o, 0, 0);
+    } else {
+      __builtin_amdgcn_raw_buffer_store_b32((unsigned)T::from(v0) | (unsigned)T::from(v1) << 16,
+                                            g.r, off[0] + o, 0, 0);
+    }
   }
 };
-// B or C, (rows, N): register k holds, in lane l of row r, step
-// k * (16 / NPL) + l / NPL of state n0 + l % NPL.
-template <class T, int NPL>
+
+// S rows of B or C, (rows, N), on their way to LDS: lane (row, q) takes the row's NPL
+// states from n0 on (S 8: for the lanes 0 .. 31 of the wave, or the others).
+template <class T, int NPL, int S, bool VEC>
 struct StateLoad {
-  static constexpr int kPer = 16 / NPL;
+  static constexpr int E = kElem<T>;
   GBuf g;
-  unsigned off, stepk, sub;
+  unsigned off, sub;
+  int valid;
   __device__ __forceinline__ StateLoad(const void* base, int ld, int t0, int len, int N, int n0,
-                                       int c)
-      : g(buf_t<T>(base, (size_t)t0 * ld,
-                   len > 0 ? kElem<T> * ((unsigned)(len - 1) * ld + N) : 0u)),
-        off(n0 + c % NPL < N ? kElem<T> * ((unsigned)(c / NPL) * ld + n0 + c % NPL) : kOOB),
-        stepk(kPer * kElem<T> * ld), sub(16 * kElem<T> * ld) {}
+                                       int row)
+      : g(buf_t<T>(base, (size_t)t0 * ld, len > 0 ? E * ((unsigned)(len - 1) * ld + N) : 0u)),
+        off(E * ((unsigned)row * ld + n0)), sub(S * E * ld), valid(N - n0) {}
   __device__ __forceinline__ void load(float (&v)[NPL], int i) const {
+    const unsigned o = off + (unsigned)i * sub;
+    if constexpr (NPL == 1) {
+      v[0] = ld_t<T>(g, valid > 0 ? o : kOOB);
+    } else if constexpr (!VEC) {
 #pragma unroll
-    for (int k = 0; k < NPL; ++k) v[k] = ld_t<T>(g, off + (unsigned)i * sub + k * stepk);
+      for (int j = 0; j < NPL; ++j) v[j] = ld_t<T>(g, j < valid ? o + E * j : kOOB);
+    } else {
+      unsigned r[4] = {0, 0, 0, 0};
+      constexpr int W = NPL * E / 4;   // words
+      if constexpr (W == 4) {
+        const auto l = __builtin_amdgcn_raw_buffer_load_b128(g.r, o, 0, 0);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) r[w] = l[w];
+      } else if constexpr (W == 2) {
+        const auto l = __builtin_amdgcn_raw_buffer_load_b64(g.r, o, 0, 0);
+        r[0] = l[0];
+        r[1] = l[1];
+      } else {
+        r[0] = __builtin_amdgcn_raw_buffer_load_b32(g.r, o, 0, 0);
+      }
+      // (states past N are the next row's numbers)
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        float f;
+        if constexpr (E == 4) f = __uint_as_float(r[j]);
+        else f = T::to((unsigned short)(r[j / 2] >> (16 * (j & 1))));
+        v[j] = j < valid ? f : 0.f;
+      }
+    }
   }
 };
+
+// Lane K of each quad of b, times v; acc += that (b must not come from a VALU
+// instruction less than two instructions before: quad_ready).
+constexpr int quad_bcast(int k) { return k * 0x55; }
+template <int K>
+__device__ __forceinline__ float quad_mul(float b, float v) {
+  return dpp_get<quad_bcast(K)>(b) * v;
+}
+template <int K>
+__device__ __forceinline__ void quad_fmac(float& acc, float b, float v) {
+  asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[%3,%3,%3,%3] row_mask:0xf bank_mask:0xf"
+      : "+v"(acc)
+      : "v"(b), "v"(v), "n"(K));
+}
+template <int M>
+__device__ __forceinline__ void quad_ready(float (&v)[2][M]) {
+  static_assert(M == 2 || M == 4, "two or four registers a channel");
+  if constexpr (M == 2)
+    asm("s_nop 1" : "+v"(v[0][0]), "+v"(v[0][1]), "+v"(v[1][0]), "+v"(v[1][1]));
+  else
+    asm("s_nop 1" : "+v"(v[0][0]), "+v"(v[0][1]), "+v"(v[0][2]), "+v"(v[0][3]), "+v"(v[1][0]),
+        "+v"(v[1][1]), "+v"(v[1][2]), "+v"(v[1][3]));
+}
+// Sums over the quad of v[s], s < 4: lane q ends with that of v[q].
+__device__ __forceinline__ float quad_gather(const float (&v)[4], int q) {
+  float a[2], b[1];
+  rs_stage_dpp<kDppXor1>(v, a, q & 1);
+  rs_stage_dpp<kDppXor2>(a, b, q >> 1);
+  return b[0];
+}
+
+// Sum of dt over the piece, by channel: the quad's lanes hold each a part.
+__device__ __forceinline__ void store_sdt(const PackedScanArgs& a, int q, int d,
+                                          const bool (&act)[2], float s0, float s1) {
+  s0 = group_sum<4>(s0);
+  s1 = group_sum<4>(s1);
+  float* p = a.sdt + (size_t)blockIdx.x * a.D + d;
+  if (q == 0 && act[0]) p[0] = s0;
+  if (q == 0 && act[1]) p[1] = s1;
+}
 
 // ----------------------------------------------------------------- forward
 
-template <class T, int NPL, int WS, bool CARRY>
+template <class T, int NPL, int WS, bool VEC, bool CARRY, bool CKPT>
 __global__ void __launch_bounds__(256)
 packed_scan_fwd_kernel(PackedScanArgs a) {
   typedef ScanLane<NPL, WS> Lane;
-  constexpr int PER = 16 / NPL;
-  __shared__ float ysum[WS > 1 ? 2 : 1][WS > 1 ? 4 : 1][WS > 1 ? 4 : 1][64];
+  constexpr int NS = Lane::kStates;
+  __shared__ float tiles[4][2][kSub * NS];   // B, C of a wave's sub-chunk
+  __shared__ float2 ysum[WS > 1 ? 2 : 1][WS > 1 ? 4 : 1][WS > 1 ? 4 : 1][64];
   const Piece pc = find_piece(a.q, a.tc, blockIdx.x);
   if (pc.seq < 0) return;
   const Lane L(a.D);
@@ -134,92 +284,102 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
   }
   if (CARRY && pc.last) return;
   const size_t slice = (size_t)a.D * a.N;
-  const StateAt<NPL> at(L.d, L.n0, a.D, a.N);
-  float a2[NPL], h[NPL];
+  const StatePair<NPL, VEC> at(L.d, L.n0, a.D, a.N, L.act);
+  float a2[2][NPL], h[2][NPL];
   at.load(a2, a.aneg);
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
-    a2[j] *= -kLog2e;
-    h[j] = 0.f;
+    a2[0][j] *= -kLog2e;
+    a2[1][j] *= -kLog2e;
+    h[0][j] = h[1][j] = 0.f;
   }
-  if (!CARRY) {
+  if constexpr (!CARRY) {
     if (pc.j > 0) at.load(h, a.start + (size_t)blockIdx.x * slice);
     else if (a.h0) at.load(h, a.h0 + (size_t)pc.seq * slice);
   }
-  const ChanLoad<T> lx(a.x, a.ld_x, pc.t0, pc.len, a.D, L.d, L.row, L.act);
-  const ChanLoad<T> ldt(a.dt, a.ld_dt, pc.t0, pc.len, a.D, L.d, L.row, L.act);
-  const StateLoad<T, NPL> lb(a.B, a.ld_b, pc.t0, pc.len, a.N, L.n0, L.c);
-  const StateLoad<T, NPL> lc(a.C, a.ld_c, pc.t0, CARRY ? 0 : pc.len, a.N, L.n0, L.c);
-  const ChanLoad<T> sy(a.y, a.D, pc.t0, CARRY ? 0 : pc.len, a.D, L.d, L.row, L.act);
-  float* ck = a.ckpt ? a.ckpt + ((size_t)(pc.begin / kSub) + (size_t)pc.j * (a.tc / kSub)) * slice
-                     : nullptr;
+  const int row = L.lane >> 2;
+  const ChanLoad<T, kSub, VEC> lx(a.x, a.ld_x, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const ChanLoad<T, kSub, VEC> ldt(a.dt, a.ld_dt, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const StateLoad<T, NPL, kSub, VEC> lb(a.B, a.ld_b, pc.t0, pc.len, a.N, L.n0, row);
+  const StateLoad<T, NPL, kSub, VEC> lc(a.C, a.ld_c, pc.t0, CARRY ? 0 : pc.len, a.N, L.n0, row);
+  const ChanLoad<T, kSub, VEC> sy(a.y, a.D, pc.t0, CARRY ? 0 : pc.len, a.D, L.d, L.q, L.act);
+  // the checkpoint before row 0 of the piece (not there for a sequence's first)
+  float* ck = a.ckpt + ((ptrdiff_t)(pc.begin / kCkpt + pc.j * (a.tc / kCkpt)) - 1) *
+                           (ptrdiff_t)slice;
+  float* const tb = tiles[L.wave][0];
+  float* const tc = tiles[L.wave][1];
   const int nsub = (pc.len + kSub - 1) / kSub;
-  float nx[4], nd[4], nb[NPL], nc[NPL];   // the next sub-chunk's
-  lx.load(nx, 0);
-  ldt.load(nd, 0);
-  lb.load(nb, 0);
-  if (!CARRY) lc.load(nc, 0);
-  float sum_dt = 0.f;
+  float nx[2][4], nd[2][4], nb[NPL], nc[NPL];   // the next sub-chunk's
+  const auto load = [&](int i) {
+    ldt.load(nd, i);
+    lx.load(nx, i);
+    lb.load(nb, i);
+    if (!CARRY) lc.load(nc, i);
+  };
+  load(0);
+  float sum_dt[2] = {0.f, 0.f};
   for (int i = 0; i < nsub; ++i) {
-    float bx[4], dc[4], b[NPL], cc[NPL];
+    float bx[2][4], dt[2][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      dc[k] = nd[k];
-      bx[k] = nd[k] * nx[k];
-      if (CARRY) sum_dt += nd[k];
-    }
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int k = 0; k < NPL; ++k) {
-      b[k] = nb[k];
-      if (!CARRY) cc[k] = nc[k];
-    }
-    if (!CARRY) row_fmac_ready(cc);
-    lx.load(nx, i + 1);
-    ldt.load(nd, i + 1);
-    lb.load(nb, i + 1);
-    if (!CARRY) lc.load(nc, i + 1);
-    if (!CARRY && ck && (i > 0 || pc.j > 0)) at.store(ck + ((ptrdiff_t)i - 1) * (ptrdiff_t)slice, h);
-    static_for<4>([&](auto qc) {
-      constexpr int q = decltype(qc)::value;
-      float dts[4], bxs[4], y[4];
-      spread_rows(dc[q], dts);
-      spread_rows(bx[q], bxs);
+      for (int k = 0; k < 4; ++k) {
+        dt[c][k] = nd[c][k];
+        bx[c][k] = nd[c][k] * nx[c][k];
+        if (CARRY) sum_dt[c] += nd[c][k];
+      }
+    wave_lds_sync();
+    store_vec<NPL>(tb + L.lane * NPL, nb);
+    if (!CARRY) store_vec<NPL>(tc + L.lane * NPL, nc);
+    wave_lds_sync();
+    load(i + 1);
+    static_for<4>([&](auto kc) {
+      constexpr int k = decltype(kc)::value;
+      if constexpr (CKPT && (4 * k) % kCkpt == 0)
+        at.store(ck + (ptrdiff_t)(i * (kSub / kCkpt) + 4 * k / kCkpt) * (ptrdiff_t)slice, h,
+                 (i > 0 || pc.j > 0 || k > 0) && i * kSub + 4 * k < pc.len);
+      float y[2][4];
       static_for<4>([&](auto sc) {
-        constexpr int s = decltype(sc)::value, t = 4 * q + s;
-        static_for<NPL>([&](auto jc) {
-          constexpr int j = decltype(jc)::value, k = (t % PER) * NPL + j;
-          const float u = row_mul<k>(b[t / PER], bxs[s]);
-          h[j] = __builtin_fmaf(exp2_hw(dts[s] * a2[j]), h[j], u);
-          if constexpr (!CARRY) {
-            if constexpr (j == 0) y[s] = row_mul<k>(cc[t / PER], h[j]);
-            else row_fmac<k>(y[s], cc[t / PER], h[j]);
+        constexpr int s = decltype(sc)::value;
+        float b[NPL], cv[NPL];
+        load_vec<NPL>(b, tb + (4 * k + s) * NS + L.q * NPL);
+        if (!CARRY) load_vec<NPL>(cv, tc + (4 * k + s) * NS + L.q * NPL);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int j = 0; j < NPL; ++j) {
+            const float da = exp2_hw(quad_mul<s>(dt[c][k], a2[c][j]));
+            h[c][j] = __builtin_fmaf(da, h[c][j], quad_mul<s>(bx[c][k], b[j]));
+            if (!CARRY) y[c][s] = j ? __builtin_fmaf(cv[j], h[c][j], y[c][s]) : cv[j] * h[c][j];
           }
-        });
+        }
       });
-      if (!CARRY) {
-        const float yr = gather_rows(y);
-        if constexpr (WS == 1) sy.store(yr, i, q);
-        else ysum[i & 1][L.wave][q][L.lane] = yr;
+      if constexpr (!CARRY) {
+        const float y0 = quad_gather(y[0], L.q), y1 = quad_gather(y[1], L.q);
+        if constexpr (WS == 1) sy.store(y0, y1, i, k);
+        else ysum[i & 1][L.wave][k][L.lane] = make_float2(y0, y1);
       }
     });
     if constexpr (WS > 1 && !CARRY) {
       // the WS waves of the same channels share out the four registers of y
       __syncthreads();
 #pragma unroll
-      for (int q = L.ws; q < 4; q += WS) {
-        float v = ysum[i & 1][L.wc * WS][q][L.lane];
+      for (int k = 0; k < 4; ++k) {
+        if (k % WS != L.ws) continue;
+        float2 v = ysum[i & 1][L.wc * WS][k][L.lane];
 #pragma unroll
-        for (int w = 1; w < WS; ++w) v += ysum[i & 1][L.wc * WS + w][q][L.lane];
-        sy.store(v, i, q);
+        for (int w = 1; w < WS; ++w) {
+          const float2 o = ysum[i & 1][L.wc * WS + w][k][L.lane];
+          v.x += o.x;
+          v.y += o.y;
+        }
+        sy.store(v.x, v.y, i, k);
       }
     }
   }
   if (CARRY) {
     at.store(a.carry + (size_t)blockIdx.x * slice, h);
-    // the four rows' steps of the channel
-    const float s4[4] = {sum_dt, 0.f, 0.f, 0.f};
-    const float total = gather_rows(s4);
-    if (L.ws == 0 && L.row == 0 && L.act) a.sdt[(size_t)blockIdx.x * a.D + L.d] = total;
+    if (L.ws == 0) store_sdt(a, L.q, L.d, L.act, sum_dt[0], sum_dt[1]);
   } else if (pc.last && a.h_last) {
     at.store(a.h_last + (size_t)pc.seq * slice, h);
   }
@@ -266,262 +426,305 @@ packed_fold_kernel(PackedScanArgs a) {
 //   G_t = dy_t C_t + u_{t+1},   q_t = u_t h_{t-1}
 //   dx_t = dt_t sum_n G B,  ddt_t = x_t sum_n G B - sum_n Aneg q,  dAneg -= dt_t q
 //   dB_tn = sum_d G dt x,  dC_tn = sum_d dy h,  dh0 = u_0
-// The main pass walks the sub-chunks of a piece from the last: dA and h of its 16
-// steps are formed again, from the checkpoint before it, in registers, then
-// the steps are walked back. The sums over the states go over the rows as y's do;
-// those over the channels over the 16 lanes of a row, two steps of four states and
-// two kinds at a time so that each lane ends with one of them, then in LDS over the
-// block's waves, and over the blocks in packed_sum_bc_kernel: always in
-// the same order. The adjoint's carry pass and fold mirror the forward's.
+// The main pass walks the sub-chunks (8 rows) of a piece from the last: their dA and h
+// are formed again, from the checkpoint before them, in registers, then the rows
+// are walked back. The sums over the channels add a lane's two channels in the products,
+// then go over the wave's 16 channel pairs, two rows of four states and two kinds at a time
+// so that each lane ends with one of them, in LDS over the block's waves, and over the
+// blocks in packed_sum_bc_kernel: always in the same order.
+// (Checkpoints every 8 rows rather than 16: what the sums over the channels cost falls with
+// the channels a lane holds, and registers hold 8 rows of two.)
 
-// Sum over the 16 lanes of each row of v[i], i < 16: lane l ends with that of
-// index row_sum_index(l).
-__device__ __forceinline__ float row_sum16(const float (&v)[16], int lane) {
-  float b[8], c[4], d[2];
+// The adjoint's carry pass: each piece but the first from a zero adjoint.
+template <class T, int NPL, int WS, bool VEC>
+__global__ void __launch_bounds__(256)
+packed_scan_back_carry_kernel(PackedScanArgs a) {
+  typedef ScanLane<NPL, WS> Lane;
+  constexpr int NS = Lane::kStates;
+  __shared__ float tiles[4][kSub * NS];   // C of a wave's sub-chunk
+  const Piece pc = find_piece(a.q, a.tc, blockIdx.x);
+  if (pc.seq < 0 || pc.seq == a.q.nseq || pc.j == 0) return;
+  const Lane L(a.D);
+  const size_t slice = (size_t)a.D * a.N;
+  const StatePair<NPL, VEC> at(L.d, L.n0, a.D, a.N, L.act);
+  float a2[2][NPL], u[2][NPL];
+  at.load(a2, a.aneg);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) b[i] = 0.f;
-  rs_stage_dpp<kDppRor8>(v, b, (lane >> 3) & 1);
-  rs_stage_dpp<kDppHalfMirror>(b, c, (lane >> 2) & 1);
-  rs_stage_dpp<kDppXor2>(c, d, (lane >> 1) & 1);
-  float e[1];
-  rs_stage_dpp<kDppXor1>(d, e, lane & 1);
-  return e[0];
-}
-__device__ __forceinline__ int row_sum_index(int lane) {
-  return 8 * (lane & 1) + 4 * ((lane >> 1) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 3) & 1);
+  for (int j = 0; j < NPL; ++j) {
+    a2[0][j] *= -kLog2e;
+    a2[1][j] *= -kLog2e;
+    u[0][j] = u[1][j] = 0.f;
+  }
+  const ChanLoad<T, kSub, VEC> ldt(a.dt, a.ld_dt, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const ChanLoad<T, kSub, VEC> ldy(a.dy, a.ld_dy, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const StateLoad<T, NPL, kSub, VEC> lc(a.C, a.ld_c, pc.t0, pc.len, a.N, L.n0, L.lane >> 2);
+  float* const tc = tiles[L.wave];
+  float nd[2][4], ny[2][4], nc[NPL];
+  const auto load = [&](int i) {   // (of a sub-chunk -1: zeros)
+    ldt.load(nd, i);
+    ldy.load(ny, i);
+    lc.load(nc, i);
+  };
+  const int nsub = (pc.len + kSub - 1) / kSub;
+  load(nsub - 1);
+  float sum_dt[2] = {0.f, 0.f};
+  for (int i = nsub - 1; i >= 0; --i) {
+    float dt[2][4], dy[2][4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        dt[c][k] = nd[c][k];
+        dy[c][k] = ny[c][k];
+        sum_dt[c] += nd[c][k];
+      }
+    quad_ready(dy);
+    wave_lds_sync();
+    store_vec<NPL>(tc + L.lane * NPL, nc);
+    wave_lds_sync();
+    load(i - 1);
+    static_for<16>([&](auto tcn) {
+      constexpr int t = 15 - decltype(tcn)::value, k = t / 4, s = t % 4;
+      float cv[NPL];
+      load_vec<NPL>(cv, tc + t * NS + L.q * NPL);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+          quad_fmac<s>(u[c][j], dy[c][k], cv[j]);
+          u[c][j] *= exp2_hw(quad_mul<s>(dt[c][k], a2[c][j]));
+        }
+      }
+    });
+  }
+  at.store(a.carry + (size_t)blockIdx.x * slice, u);
+  if (L.ws == 0) store_sdt(a, L.q, L.d, L.act, sum_dt[0], sum_dt[1]);
 }
 
-template <class T, int NPL, int WS, bool CARRY>
+// Sums over the lanes that share lane & 3 of v[i], i < 16: each lane ends with that of
+// index chan_sum_index(lane).
+__device__ __forceinline__ float chan_sum16(const float (&v)[16]) {
+  float a[8], b[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[2 * i]),
+                                                    __float_as_uint(v[2 * i + 1]), false, false);
+    a[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[2 * i]),
+                                                    __float_as_uint(a[2 * i + 1]), false, false);
+    b[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
+  return rs_bits32_shift(b);
+}
+__device__ __forceinline__ int chan_sum_index(int lane) {
+  return (lane >> 5 & 1) + 2 * (lane >> 4 & 1) + 4 * (lane >> 2 & 1) + 8 * (lane >> 3 & 1);
+}
+
+template <class T, int NPL, int WS, bool VEC>
 __global__ void __launch_bounds__(256, 2)
 packed_scan_bwd_kernel(PackedScanArgs a) {
   typedef ScanLane<NPL, WS> Lane;
-  constexpr int PER = 16 / NPL;
   constexpr int WC = 4 / WS;
   constexpr int NS = Lane::kStates;
-  // dB, dC of the sub-chunk by wave [kind][step][state], and s1, s2 by wave
-  __shared__ float tbc[CARRY ? 1 : 2][CARRY ? 1 : 4][CARRY ? 1 : 2 * kSub * NS];
-  __shared__ float tss[WS > 1 && !CARRY ? 2 : 1][WS > 1 && !CARRY ? 4 : 1][2][4]
-                      [WS > 1 && !CARRY ? 64 : 1];
+  constexpr int S = kCkpt, K = S / 4;
+  // dB, dC of the sub-chunk by wave: [kind][row][state], the kinds apart by half the banks more
+  constexpr int KIND = S * NS + 32;
+  __shared__ float tiles[4][2][S * NS];   // B, C of a wave's sub-chunk
+  __shared__ float tbc[2][4][2 * KIND];
+  __shared__ float4 tss[WS > 1 ? 2 : 1][WS > 1 ? 4 : 1][K][WS > 1 ? 64 : 1];
   const Piece pc = find_piece(a.q, a.tc, blockIdx.x);
   const Lane L(a.D);
   const size_t slice = (size_t)a.D * a.N;
-  const StateAt<NPL> at(L.d, L.n0, a.D, a.N);
-  float zero[NPL] = {};
+  const StatePair<NPL, VEC> at(L.d, L.n0, a.D, a.N, L.act);
+  float* part = a.part_bc + ((size_t)blockIdx.y * a.q.total + max(0, pc.t0)) * 2 * a.N;
   if (pc.seq < 0 || pc.seq == a.q.nseq) {
-    if (CARRY) return;
+    const float zero[2][NPL] = {};
     at.store(a.part_a + (size_t)blockIdx.x * slice, zero);
     if (pc.seq < 0) return;
     const int d_lo = blockIdx.y * Lane::kChans, d_hi = d_lo + Lane::kChans;
     zero_rows<T>(a.dx, pc.t0, pc.len, a.D, d_lo, d_hi);
     zero_rows<T>(a.ddt, pc.t0, pc.len, a.D, d_lo, d_hi);
-    float* part = a.part_bc + ((size_t)blockIdx.y * a.q.total + pc.t0) * 2 * a.N;
     for (size_t i = threadIdx.x; i < (size_t)pc.len * 2 * a.N; i += blockDim.x) part[i] = 0.f;
     return;
   }
-  if (CARRY && pc.j == 0) return;
-  float an[NPL], a2[NPL], u[NPL], acc[NPL];
-  at.load(an, a.aneg);
+  // (sums of -Aneg log2(e) q and of dt q, scaled once at the end)
+  float a2[2][NPL], u[2][NPL], acc[2][NPL];
+  at.load(a2, a.aneg);
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
-    a2[j] = -an[j] * kLog2e;
-    u[j] = acc[j] = 0.f;
+    a2[0][j] *= -kLog2e;
+    a2[1][j] *= -kLog2e;
+    u[0][j] = u[1][j] = acc[0][j] = acc[1][j] = 0.f;
   }
-  if (!CARRY) {
-    if (!pc.last) at.load(u, a.start + (size_t)blockIdx.x * slice);
-    else if (a.dh_last) at.load(u, a.dh_last + (size_t)pc.seq * slice);
-  }
-  const int xlen = CARRY ? 0 : pc.len;
-  const ChanLoad<T> lx(a.x, a.ld_x, pc.t0, xlen, a.D, L.d, L.row, L.act);
-  const ChanLoad<T> ldt(a.dt, a.ld_dt, pc.t0, pc.len, a.D, L.d, L.row, L.act);
-  const ChanLoad<T> ldy(a.dy, a.ld_dy, pc.t0, pc.len, a.D, L.d, L.row, L.act);
-  const StateLoad<T, NPL> lb(a.B, a.ld_b, pc.t0, xlen, a.N, L.n0, L.c);
-  const StateLoad<T, NPL> lc(a.C, a.ld_c, pc.t0, pc.len, a.N, L.n0, L.c);
-  const ChanLoad<T> sdx(a.dx, a.D, pc.t0, xlen, a.D, L.d, L.row, L.act);
-  const ChanLoad<T> sddt(a.ddt, a.D, pc.t0, xlen, a.D, L.d, L.row, L.act);
-  const int g0 = pc.j * (a.tc / kSub);   // the piece's first sub-chunk in its sequence
-  const int nsub = (pc.len + kSub - 1) / kSub;
-  const float* ck = a.ckpt + ((size_t)(pc.begin / kSub) + (size_t)g0) * slice;
-  const float* h_first = a.h0 ? a.h0 + (size_t)pc.seq * slice : nullptr;
-  auto load_state = [&](float (&v)[NPL], int i) {   // the state before sub-chunk i
-    if (i < 0) return;
-    if (g0 + i > 0) {
-      at.load(v, ck + ((ptrdiff_t)i - 1) * (ptrdiff_t)slice);
-    } else if (h_first) {
-      at.load(v, h_first);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) v[j] = 0.f;
-    }
-  };
-  float nx[4], nd[4], ny[4], nb[NPL], nc[NPL], nh[NPL] = {};
-  auto load_sub = [&](int i) {
-    if (i < 0) return;
+  if (!pc.last) at.load(u, a.start + (size_t)blockIdx.x * slice);
+  else if (a.dh_last) at.load(u, a.dh_last + (size_t)pc.seq * slice);
+  const ChanLoad<T, S, VEC> lx(a.x, a.ld_x, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const ChanLoad<T, S, VEC> ldt(a.dt, a.ld_dt, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const ChanLoad<T, S, VEC> ldy(a.dy, a.ld_dy, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  // lanes 0 .. 31 bring B's rows to LDS, the others C's
+  const bool half = L.lane >= 32;
+  const int row = L.lane >> 2 & 7;
+  const StateLoad<T, NPL, S, VEC> lb(a.B, a.ld_b, pc.t0, pc.len, a.N, L.n0, row);
+  const StateLoad<T, NPL, S, VEC> lc(a.C, a.ld_c, pc.t0, pc.len, a.N, L.n0, row);
+  const ChanLoad<T, S, VEC> sdx(a.dx, a.D, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const ChanLoad<T, S, VEC> sddt(a.ddt, a.D, pc.t0, pc.len, a.D, L.d, L.q, L.act);
+  const int g0 = pc.j * (a.tc / S);   // the piece's first sub-chunk in its sequence
+  const int nsub = (pc.len + S - 1) / S;
+  const float* ck = a.ckpt + ((ptrdiff_t)(pc.begin / S + g0) - 1) * (ptrdiff_t)slice;
+  const float* h_first = a.h0 + (size_t)pc.seq * slice;
+  float nx[2][K], nd[2][K], ny[2][K], nb[NPL], nc[NPL], nh[2][NPL];
+  const auto load = [&](int i) {   // (of a sub-chunk -1: zeros)
     ldt.load(nd, i);
-    ldy.load(ny, i);
-    lc.load(nc, i);
-    if (CARRY) return;
     lx.load(nx, i);
+    ldy.load(ny, i);
     lb.load(nb, i);
-    load_state(nh, i);
+    lc.load(nc, i);
+    const bool first = g0 + i <= 0;
+    at.load(nh, first ? h_first : ck + (ptrdiff_t)i * (ptrdiff_t)slice,
+            i >= 0 && (!first || a.h0 != nullptr));
   };
-  load_sub(nsub - 1);
-  float sum_dt = 0.f;
-  float* part = a.part_bc + ((size_t)blockIdx.y * a.q.total + pc.t0) * 2 * a.N;
+  load(nsub - 1);
+  float* const tb = tiles[L.wave][0];
+  float* const tc = tiles[L.wave][1];
+  const int ix = chan_sum_index(L.lane);
+  // where this lane's sums go: kind ix / 8, row parity ix / 4 % 2, state ix % 4 of its quad's
+  const bool sums = (ix & 3) < NPL;
+  const int to = (ix >> 3) * KIND + (ix >> 2 & 1) * NS + L.q * NPL + (ix & 3);
   for (int i = nsub - 1; i >= 0; --i) {
-    float xc[4], dc[4], yc[4], b[NPL], cc[NPL], h0[NPL];
+    float x[2][K], dt[2][K], dy[2][K], bx[2][K], h0[2][NPL];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      dc[k] = nd[k];
-      yc[k] = ny[k];
-      if (!CARRY) xc[k] = nx[k];
-      if (CARRY) sum_dt += nd[k];
-    }
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int k = 0; k < NPL; ++k) {
-      cc[k] = nc[k];
-      if (!CARRY) b[k] = nb[k];
-      if (!CARRY) h0[k] = nh[k];
-    }
-    row_fmac_ready(cc);
-    if (!CARRY) row_fmac_ready(b);
-    load_sub(i - 1);
-    float da[kSub][NPL], hs[CARRY ? 1 : kSub][NPL];
-    static_for<4>([&](auto qc) {
-      constexpr int q = decltype(qc)::value;
-      float dts[4], bxs[4];
-      spread_rows(dc[q], dts);
-      if (!CARRY) spread_rows(dc[q] * xc[q], bxs);
-      static_for<4>([&](auto sc) {
-        constexpr int s = decltype(sc)::value, t = 4 * q + s;
-        static_for<NPL>([&](auto jc) {
-          constexpr int j = decltype(jc)::value, k = (t % PER) * NPL + j;
-          da[t][j] = exp2_hw(dts[s] * a2[j]);
-          if constexpr (!CARRY)
-            hs[t][j] = __builtin_fmaf(da[t][j], t == 0 ? h0[j] : hs[t == 0 ? 0 : t - 1][j],
-                                      row_mul<k>(b[t / PER], bxs[s]));
-        });
-      });
-    });
-    float* const mine = tbc[CARRY ? 0 : i & 1][CARRY ? 0 : L.wave];
-    static_for<4>([&](auto qc) {
-      constexpr int q = 3 - decltype(qc)::value;
-      float dys[4], dts[4], bxs[4], s1[4], s2[4];
-      spread_rows(yc[q], dys);
-      if (!CARRY) {
-        spread_rows(dc[q], dts);
-        spread_rows(dc[q] * xc[q], bxs);
+      for (int k = 0; k < K; ++k) {
+        x[c][k] = nx[c][k];
+        dt[c][k] = nd[c][k];
+        dy[c][k] = ny[c][k];
+        bx[c][k] = nd[c][k] * nx[c][k];
       }
-      float v[16];   // products of two steps: [kind][step parity][state], kinds G dt x, dy h
-      static_for<4>([&](auto sc) {
-        constexpr int s = 3 - decltype(sc)::value, t = 4 * q + s;
-        static_for<NPL>([&](auto jc) {
-          constexpr int j = decltype(jc)::value, k = (t % PER) * NPL + j;
-          float g = u[j];
-          row_fmac<k>(g, cc[t / PER], dys[s]);
-          u[j] = da[t][j] * g;
-          if constexpr (!CARRY) {
-            const float qv = u[j] * (t == 0 ? h0[j] : hs[t == 0 ? 0 : t - 1][j]);
-            if constexpr (j == 0) {
-              s1[s] = row_mul<k>(b[t / PER], g);
-              s2[s] = an[j] * qv;
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) h0[c][j] = nh[c][j];
+    }
+    quad_ready(dt);
+    quad_ready(dy);
+    quad_ready(bx);
+    wave_lds_sync();
+    float nbc[NPL];
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) nbc[j] = half ? nc[j] : nb[j];
+    store_vec<NPL>(tb + L.lane * NPL, nbc);   // (C's tile follows B's)
+    wave_lds_sync();
+    load(i - 1);
+    float da[S][2][NPL], hs[S][2][NPL];
+    static_for<S>([&](auto tcn) {
+      constexpr int t = decltype(tcn)::value, k = t / 4, s = t % 4;
+      float b[NPL];
+      load_vec<NPL>(b, tb + t * NS + L.q * NPL);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+          da[t][c][j] = exp2_hw(quad_mul<s>(dt[c][k], a2[c][j]));
+          hs[t][c][j] = __builtin_fmaf(da[t][c][j], t ? hs[t ? t - 1 : 0][c][j] : h0[c][j],
+                                       quad_mul<s>(bx[c][k], b[j]));
+        }
+      }
+    });
+    float* const mine = tbc[i & 1][L.wave] + to;
+    static_for<K>([&](auto kcn) {
+      constexpr int k = K - 1 - decltype(kcn)::value;
+      float s1[2][4], s2[2][4];
+      float v[16];   // of two rows: [kind][row parity][state], kinds G dt x, dy h
+      static_for<4>([&](auto scn) {
+        constexpr int s = 3 - decltype(scn)::value, t = 4 * k + s;
+        float b[NPL], cv[NPL];
+        load_vec<NPL>(b, tb + t * NS + L.q * NPL);
+        load_vec<NPL>(cv, tc + t * NS + L.q * NPL);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int j = 0; j < NPL; ++j) {
+            float& vb = v[(s & 1) * 4 + j];
+            float& vc = v[8 + (s & 1) * 4 + j];
+            quad_fmac<s>(u[c][j], dy[c][k], cv[j]);   // G
+            const float g = u[c][j];
+            u[c][j] = da[t][c][j] * g;
+            const float qv = u[c][j] * (t ? hs[t ? t - 1 : 0][c][j] : h0[c][j]);
+            s1[c][s] = j ? __builtin_fmaf(b[j], g, s1[c][s]) : b[j] * g;
+            s2[c][s] = j ? __builtin_fmaf(a2[c][j], qv, s2[c][s]) : a2[c][j] * qv;
+            quad_fmac<s>(acc[c][j], dt[c][k], qv);
+            if (c == 0) {
+              vb = quad_mul<s>(bx[c][k], g);
+              vc = quad_mul<s>(dy[c][k], hs[t][c][j]);
             } else {
-              row_fmac<k>(s1[s], b[t / PER], g);
-              s2[s] = __builtin_fmaf(an[j], qv, s2[s]);
+              quad_fmac<s>(vb, bx[c][k], g);
+              quad_fmac<s>(vc, dy[c][k], hs[t][c][j]);
             }
-            acc[j] = __builtin_fmaf(dts[s], qv, acc[j]);
-            v[(s & 1) * 4 + j] = g * bxs[s];
-            v[8 + (s & 1) * 4 + j] = hs[t][j] * dys[s];
           }
-        });
-        if constexpr (!CARRY && (s & 1) == 0) {
+        }
+        if constexpr ((s & 1) == 0) {
 #pragma unroll
           for (int j = NPL; j < 4; ++j) v[j] = v[4 + j] = v[8 + j] = v[12 + j] = 0.f;
-          const float sum = row_sum16(v, L.lane);
-          const int ix = row_sum_index(L.lane);
-          const int j = ix & 3, kind = ix >> 3, step = t + ((ix >> 2) & 1);
-          if (j < NPL) mine[(kind * kSub + step) * NS + L.row * NPL + j] = sum;
+          const float sum = chan_sum16(v);
+          if (sums) mine[t * NS] = sum;
         }
       });
-      if constexpr (!CARRY) {
-        const float r1 = gather_rows(s1), r2 = gather_rows(s2);
-        if constexpr (WS == 1) {
-          sdx.store(dc[q] * r1, i, q);
-          sddt.store(__builtin_fmaf(xc[q], r1, -r2), i, q);
-        } else {
-          tss[i & 1][L.wave][0][q][L.lane] = r1;
-          tss[i & 1][L.wave][1][q][L.lane] = r2;
-        }
+      float r1[2], r2[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        r1[c] = quad_gather(s1[c], L.q);
+        r2[c] = quad_gather(s2[c], L.q);
+      }
+      if constexpr (WS == 1) {
+        sdx.store(dt[0][k] * r1[0], dt[1][k] * r1[1], i, k);
+        sddt.store(__builtin_fmaf(x[0][k], r1[0], r2[0] * kLn2),
+                   __builtin_fmaf(x[1][k], r1[1], r2[1] * kLn2), i, k);
+      } else {
+        tss[i & 1][L.wave][k][L.lane] = make_float4(r1[0], r1[1], r2[0], r2[1]);
       }
     });
-    if constexpr (!CARRY) {
-      __syncthreads();
-      if constexpr (WS > 1) {
+    __syncthreads();
+    if constexpr (WS > 1) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q % WS != L.ws) continue;
-          float r1 = 0.f, r2 = 0.f;
+      for (int k = 0; k < K; ++k) {
+        if (k % WS != L.ws) continue;
+        float4 r = tss[i & 1][L.wc * WS][k][L.lane];
 #pragma unroll
-          for (int w = 0; w < WS; ++w) {
-            r1 += tss[i & 1][L.wc * WS + w][0][q][L.lane];
-            r2 += tss[i & 1][L.wc * WS + w][1][q][L.lane];
-          }
-          sdx.store(dc[q] * r1, i, q);
-          sddt.store(__builtin_fmaf(xc[q], r1, -r2), i, q);
+        for (int w = 1; w < WS; ++w) {
+          const float4 o = tss[i & 1][L.wc * WS + w][k][L.lane];
+          r.x += o.x;
+          r.y += o.y;
+          r.z += o.z;
+          r.w += o.w;
         }
-      }
-      // the block's sums of dB and dC: over its waves of channels
-      const int len = min(kSub, pc.len - i * kSub);
-      for (int r = threadIdx.x; r < 2 * kSub * WS * NS; r += 256) {
-        const int n = r % (WS * NS), kind = r / (WS * NS) & 1, step = r / (2 * WS * NS);
-        if (n >= a.N || step >= len) continue;
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < WC; ++w)
-          sum += tbc[i & 1][w * WS + n / NS][(kind * kSub + step) * NS + n % NS];
-        part[((size_t)(i * kSub + step) * 2 + kind) * a.N + n] = sum;
+        sdx.store(dt[0][k] * r.x, dt[1][k] * r.y, i, k);
+        sddt.store(__builtin_fmaf(x[0][k], r.x, r.z * kLn2),
+                   __builtin_fmaf(x[1][k], r.y, r.w * kLn2), i, k);
       }
     }
-  }
-  if (CARRY) {
-    at.store(a.carry + (size_t)blockIdx.x * slice, u);
-    const float s4[4] = {sum_dt, 0.f, 0.f, 0.f};
-    const float total = gather_rows(s4);
-    if (L.ws == 0 && L.row == 0 && L.act) a.sdt[(size_t)blockIdx.x * a.D + L.d] = total;
-    return;
+    // the block's sums of dB and dC: over its waves of channels
+    const int len = min(S, pc.len - i * S);
+#pragma unroll
+    for (int r0 = 0; r0 < 2 * S * WS * NS; r0 += 256) {
+      const int r = r0 + threadIdx.x;
+      const int n = r % (WS * NS), kind = r / (WS * NS) & 1, step = r / (2 * WS * NS);
+      if (n >= a.N || step >= len) continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WC; ++w)
+        sum += tbc[i & 1][w * WS + n / NS][kind * KIND + step * NS + n % NS];
+      part[((size_t)(i * S + step) * 2 + kind) * a.N + n] = sum;
+    }
   }
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) acc[j] = -acc[j];
+  for (int j = 0; j < NPL; ++j) {
+    acc[0][j] = -acc[0][j];
+    acc[1][j] = -acc[1][j];
+  }
   at.store(a.part_a + (size_t)blockIdx.x * slice, acc);
   if (pc.j == 0 && a.dh0) at.store(a.dh0 + (size_t)pc.seq * slice, u);
-}
-
-// dB, dC (total, N): the blocks' partials in order, rounded to T once.
-template <class T>
-__global__ void __launch_bounds__(256)
-packed_sum_bc_kernel(const float* part, void* dB, void* dC, int nblk, long long rows, int N) {
-  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;   // (row, kind, n)
-  if (e >= rows * 2 * N) return;
-  const long long all = rows * 2 * N;
-  float s = 0.f;
-  for (int k = 0; k < nblk; ++k) s += part[(long long)k * all + e];
-  const long long row = e / (2 * N);
-  const int n = (int)(e % (2 * N));
-  st_p<T>(n < N ? dB : dC, (size_t)(row * N + n % N), s);
-}
-
-// dAneg (D, N): the pieces' partials. Each wave of a block adds every fourth, then the block its
-// four sums: a fixed order.
-__global__ void __launch_bounds__(256)
-packed_sum_a_kernel(const float* part, float* da, int pieces, int slice) {
-  __shared__ float sums[4][64];
-  const int w = threadIdx.x >> 6, e = blockIdx.x * 64 + (threadIdx.x & 63);
-  float s = 0.f;
-  if (e < slice)
-    for (int p = w; p < pieces; p += 4) s += part[(size_t)p * slice + e];
-  sums[w][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (w == 0 && e < slice)
-    da[e] = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
 }
 
 }  // namespace mhs

@@ -1,0 +1,6 @@
+// Packed scan, f32: the instantiations of mhs_packed_instances.hpp.
+#include "mhs_packed_instances.hpp"
+
+namespace mhs {
+template int run_packed_scan<F32>(bool, const PackedScanArgs&, const ScanPlan&, hipStream_t);
+}

@@ -8,6 +8,20 @@
 using mhs::check_launch;
 using mhs::fail;
 
+namespace {
+
+// Threads of a row's block.
+constexpr int64_t kSmallVocab = 8192;
+
+template <class T>
+void launch(const mhs::SampleArgs& a, int64_t rows, hipStream_t s) {
+  const unsigned grid = (unsigned)rows;
+  if (a.vocab <= kSmallVocab) mhs::sample_kernel<T, 256><<<grid, 256, 0, s>>>(a);
+  else mhs::sample_kernel<T, 1024><<<grid, 1024, 0, s>>>(a);
+}
+
+}  // namespace
+
 extern "C" {
 
 int mhs_sample(int dtype, const void* logits, int64_t ld, const float* uniform,
@@ -33,10 +47,9 @@ int mhs_sample(int dtype, const void* logits, int64_t ld, const float* uniform,
                     reinterpret_cast<long long*>(tokens), logprobs, (int)vocab,
                     words <= 17 ? 45 : 62 - words};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned grid = (unsigned)rows;
-  if (dtype == MHS_F32) mhs::sample_kernel<mhs::F32><<<grid, mhs::kSampleThreads, 0, s>>>(a);
-  else if (dtype == MHS_BF16) mhs::sample_kernel<mhs::Bf16><<<grid, mhs::kSampleThreads, 0, s>>>(a);
-  else mhs::sample_kernel<mhs::Fp16><<<grid, mhs::kSampleThreads, 0, s>>>(a);
+  if (dtype == MHS_F32) launch<mhs::F32>(a, rows, s);
+  else if (dtype == MHS_BF16) launch<mhs::Bf16>(a, rows, s);
+  else launch<mhs::Fp16>(a, rows, s);
   return check_launch("sample kernel");
 }
 

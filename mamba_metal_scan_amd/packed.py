@@ -157,7 +157,7 @@ def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     without). Returns y (L, D), zeros in the rows behind the last sequence, and with
     return_state the (S, D, N) float32 states behind each sequence (h0's for an empty one).
     The gradients (x, dt, Aneg, B, C, h0) are summed in a fixed order. For them the
-    states at every sixteenth row are kept, L D N / 4 bytes."""
+    states at every eighth row are kept, L D N / 2 bytes."""
     what = "selective_scan_packed"
     _hip(what, x, dt, aneg, b_in, c_in, cu_seqlens, h0)
     for name, t in (("x", x), ("dt", dt), ("B", b_in), ("C", c_in)):

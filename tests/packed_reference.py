@@ -14,6 +14,7 @@ over n random terms that value is about sqrt(n) of theirs.
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 
 import torch
 
@@ -90,23 +91,25 @@ def sample(row, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return order[0], 0.0
     w = {i: (1.0 if row[i] == top else
              0.0 if top == math.inf else math.exp((row[i] - top) / temperature)) for i in order}
+    # sums without rounding: integers of 2^-200 (the fp32 settings are whole ones of 2^-149 or more)
+    n = {i: int(Fraction(v) * 2 ** 200) for i, v in w.items()}
     if 0 < top_k < len(order):
         order = order[:top_k]
     if top_p < 1:
-        total, run, kept = math.fsum(w[i] for i in order), 0.0, []
+        border, run, kept = Fraction(top_p) * sum(n[i] for i in order), 0, []
         for i in order:
-            if kept and not run < top_p * total:
+            if kept and not run < border:
                 break
             kept.append(i)
-            run += w[i]
+            run += n[i]
         order = kept
     order = sorted(i for i in order if w[i] >= min_p)
-    total = math.fsum(w[i] for i in order)
-    run, token = 0.0, None
+    total = sum(n[i] for i in order)
+    border, run, token = Fraction(u) * total, 0, None
     for i in order:
-        run += w[i]
-        if w[i] > 0:
+        run += n[i]
+        if n[i]:
             token = i
-            if run > u * total:
+            if run > border:
                 break
-    return token, math.log(w[token] / total)
+    return token, math.log(n[token] / total)
