@@ -759,13 +759,16 @@ int mhs_state_step(int dtype, float* h, const void* x, int64_t ld_x, const void*
  * drawn word's share of the kept weight. A row whose logits are all -inf, or with a
  * temperature below 0 or not finite, a min_p above 1 or a NaN setting, gives token -1 and
  * NaN. Weights are summed as integers of 2^-45 (up to 2^17 words): the same token every
- * run. vocab up to 2^24.
+ * run. Fewer than 2^16 rows, vocab up to 2^24. The workspace's size goes by whether top_k is an
+ * array and the value behind it; it is 256-byte aligned, and two calls at once need two.
  */
+size_t mhs_sample_workspace_bytes(int64_t rows, int64_t vocab, int top_k_array,
+                                  int64_t top_k_value);
 int mhs_sample(int dtype, const void* logits, int64_t ld, const float* uniform,
                const float* temperature, float temperature_value, const void* top_k, int top_k64,
                int64_t top_k_value, const float* top_p, float top_p_value, const float* min_p,
                float min_p_value, int64_t* tokens, float* logprobs, int64_t rows, int64_t vocab,
-               void* stream);
+               void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

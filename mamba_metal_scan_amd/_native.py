@@ -47,7 +47,7 @@ EXPORTED_SYMBOLS = (
     "mhs_distill_bwd", "mhs_packed_ckpt_floats", "mhs_packed_scan_workspace_bytes",
     "mhs_packed_scan_fwd", "mhs_packed_scan_bwd", "mhs_packed_conv_fwd",
     "mhs_packed_conv_bwd_workspace_bytes", "mhs_packed_conv_bwd", "mhs_conv_step",
-    "mhs_state_step", "mhs_sample",
+    "mhs_state_step", "mhs_sample_workspace_bytes", "mhs_sample",
 )
 
 # Size of the static device scratch of mhs_scan_fwd_noalloc_f32 (the header's
@@ -207,6 +207,8 @@ def library() -> ctypes.CDLL:
             lib.mhs_packed_scan_workspace_bytes.argtypes = [_I64] * 4 + [_int]
             lib.mhs_packed_conv_bwd_workspace_bytes.restype = _size
             lib.mhs_packed_conv_bwd_workspace_bytes.argtypes = [_I64] * 4
+            lib.mhs_sample_workspace_bytes.restype = _size
+            lib.mhs_sample_workspace_bytes.argtypes = [_I64, _I64, _int, _I64]
             row = [_P, _I64]                        # a tensor with its row stride
             scan = [_int] + row * 2 + [_P] + row * 2 + [_P, _int, _P]
             conv = [_int] + row + [_P, _P, _int, _P, _int, _P]
@@ -221,7 +223,7 @@ def library() -> ctypes.CDLL:
                     ("mhs_state_step", [_int, _P] + row * 2 + [_P] + row * 2 + [_P, _int, _P]
                      + [_I64] * 4 + [_P]),
                     ("mhs_sample", [_int] + row + [_P, _P, _F32, _P, _int, _I64, _P, _F32, _P, _F32,
-                                                   _P, _P, _I64, _I64, _P])):
+                                                   _P, _P, _I64, _I64, _P, _size, _P])):
                 getattr(lib, name).restype = _int
                 getattr(lib, name).argtypes = args
             _lib = lib

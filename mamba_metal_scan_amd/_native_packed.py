@@ -391,13 +391,16 @@ def _sample_impl(logits: torch.Tensor, uniform: torch.Tensor, temperature: Optio
     rows, vocab = logits.shape
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logps = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    lib = library()
     with _on(logits.device):
-        rc = library().mhs_sample(
+        nbytes = lib.mhs_sample_workspace_bytes(rows, vocab, top_k is not None, value_k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        rc = lib.mhs_sample(
             DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), uniform.data_ptr(),
             _ptr(temperature), values_f[0], _ptr(top_k),
             top_k is not None and top_k.dtype == torch.int64, value_k, _ptr(top_p), values_f[1],
-            _ptr(min_p), values_f[2], tokens.data_ptr(), logps.data_ptr(), rows, vocab,
-            _stream(logits.device))
+            _ptr(min_p), values_f[2], tokens.data_ptr(), logps.data_ptr(), rows, vocab, _ptr(ws),
+            nbytes, _stream(logits.device))
     _check(rc, "mhs_sample")
     return tokens, logps
 

@@ -143,3 +143,29 @@ def test_frequencies():
     t = sample_tokens(z.cuda().expand(n, 5), u.cuda(), temperature=0.8).cpu()
     p = torch.softmax(z.double() / 0.8, 0)
     assert (torch.bincount(t, minlength=5) - p * n).abs().max() <= 2
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_words_alike(dtype):
+    """More words of one weight, or about it, than any list holds; k above 1024; a flat
+    distribution; NaN among the words of a large k."""
+    flat = torch.zeros(4, 20000)
+    near, u = _rand(4, 40000, F32, 11, scale=0.05)
+    masked = near.clone()
+    masked[:, ::3] = math.nan
+    masked[:, 1::3] = -INF
+    steps = torch.randint(0, 3, (4, 30000), generator=torch.Generator().manual_seed(1)).float()
+    for z in (flat, near, masked, steps):
+        z = z.to(dtype)
+        for s in (dict(top_p=0.5), dict(top_k=5000), dict(top_k=15000, top_p=0.7), dict(min_p=0.5),
+                  dict(top_p=0.9, min_p=0.3), dict(top_k=1000), dict(top_k=39000), dict()):
+            check(z, u, **s)
+
+
+def test_middle_vocabularies():
+    """About 8192 words (one part) and 1024 (one list), settings by row."""
+    for vocab in (1023, 1025, 8191, 8192, 8193, 16385):
+        z, u = _rand(8, vocab, F16, vocab)
+        k = torch.tensor([0, 0, 0, 5, 900, 1500, 0, vocab])
+        check(z, u, top_k=k, top_p=torch.tensor([1.0, 0.9, 0.2, 0.9, 0.9, 0.8, 1.0, 0.99]),
+              min_p=torch.tensor([0.0, 0.0, 0.1, 0.0, 0.0, 0.0, 0.01, 0.0]))
