@@ -148,8 +148,8 @@ int conv_vec(int dtype, int64_t dim, std::initializer_list<const void*> ps,
   for (const int64_t ld : lds) ok = ok && ld % v == 0;
   return ok ? v : 1;
 }
-// Rows of a piece, forward and backward.
-constexpr int kConvPiece = 16, kConvBackPiece = 64;
+using mhs::kConvBackPiece;
+using mhs::kConvPiece;
 
 int check_conv(int dtype, const void* cu, int64_t nseq, int64_t total, int64_t dim, int64_t taps) {
   int rc = check_dtype(dtype);
@@ -166,7 +166,7 @@ int check_conv(int dtype, const void* cu, int64_t nseq, int64_t total, int64_t d
 
 template <class T, int K, int V>
 int run_conv(bool back, const mhs::PackedConvArgs& a, hipStream_t s) {
-  const int64_t pieces = piece_count(a.q.total, a.q.nseq, a.tc);
+  const int64_t pieces = piece_count(a.q.total, a.q.nseq, back ? kConvBackPiece : kConvPiece);
   const dim3 grid((unsigned)((pieces + 3) / 4), (unsigned)((a.D + 64 * V - 1) / (64 * V)));
   if (back) mhs::packed_conv_bwd_kernel<T, K, V><<<grid, 256, 0, s>>>(a, (int)pieces);
   else mhs::packed_conv_fwd_kernel<T, K, V><<<grid, 256, 0, s>>>(a, (int)pieces);
@@ -363,8 +363,8 @@ int mhs_packed_conv_fwd(int dtype, const void* x, int64_t ld_x, const void* weig
   a.q = seqs(cu_seqlens, cu64, nseq, total);
   a.x = x; a.ld_x = ld_x; a.w = weight; a.bias = bias; a.wf32 = weight_f32;
   a.window = window; a.out = out; a.window_out = window_out;
-  a.D = (int)dim; a.tc = kConvPiece;
-  return run_conv_t(dtype, taps, conv_vec(dtype, dim, {x, out}, {ld_x}), false, a,
+  a.D = (int)dim;
+  return run_conv_t(dtype, taps, conv_vec(dtype, dim, {x, out, weight, bias}, {ld_x}), false, a,
                     static_cast<hipStream_t>(stream));
 }
 
@@ -388,19 +388,19 @@ int mhs_packed_conv_bwd(int dtype, const void* x, int64_t ld_x, const void* weig
   a.x = x; a.ld_x = ld_x; a.w = weight; a.bias = bias; a.wf32 = weight_f32;
   a.window = window; a.dout = dout; a.ld_g = ld_dout; a.dwindow_out = dwindow_out;
   a.dx = dx; a.dwindow = dwindow; a.part = static_cast<float*>(workspace);
-  a.D = (int)dim; a.tc = kConvBackPiece;
+  a.D = (int)dim;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  rc = run_conv_t(dtype, taps, conv_vec(dtype, dim, {x, dout, dx}, {ld_x, ld_dout}), true, a, s);
+  rc = run_conv_t(dtype, taps, conv_vec(dtype, dim, {x, dout, dx, weight, bias}, {ld_x, ld_dout}), true, a, s);
   if (rc) return rc;
   const int n = (int)((piece_count(total, nseq, kConvBackPiece) + 3) / 4);
   const dim3 grid((unsigned)((dim + 63) / 64), (unsigned)(taps + 1));
   const int k = (int)taps;
   if (dtype == MHS_F32)
-    mhs::packed_conv_sum_kernel<mhs::F32><<<grid, 256, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
+    mhs::packed_conv_sum_kernel<mhs::F32><<<grid, 1024, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
   else if (dtype == MHS_BF16)
-    mhs::packed_conv_sum_kernel<mhs::Bf16><<<grid, 256, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
+    mhs::packed_conv_sum_kernel<mhs::Bf16><<<grid, 1024, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
   else
-    mhs::packed_conv_sum_kernel<mhs::Fp16><<<grid, 256, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
+    mhs::packed_conv_sum_kernel<mhs::Fp16><<<grid, 1024, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
   return check_launch("packed conv weight gradient sum");
 }
 

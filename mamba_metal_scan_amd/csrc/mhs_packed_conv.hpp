@@ -26,7 +26,7 @@ struct PackedConvArgs {
   const void* window;   // (nseq, D, K - 1) or null
   void* out;            // (total, D)
   void* window_out;     // (nseq, D, K - 1) or null
-  int D, tc;
+  int D;
   // backward
   const void* dout;     // (total, D), rows ld_g apart
   long long ld_g;
@@ -36,21 +36,25 @@ struct PackedConvArgs {
   float* part;          // (block rows, K + 1, D): dw, dbias
 };
 
-// V neighbouring elements of T from idx on (V elements are 16 bytes, aligned, or one).
+// V neighbouring elements of T (16 bytes, aligned, or one) as they lie in memory.
 template <class T, int V>
-__device__ __forceinline__ void load_chans(float (&v)[V], const void* p, size_t idx) {
-  if constexpr (V == 1) {
-    v[0] = ld_p<T>(p, idx);
-  } else {
-    const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + idx * kElem<T>);
-    const unsigned u[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if constexpr (kElem<T> == 4) v[i] = __uint_as_float(u[i]);
-      else v[i] = T::to((unsigned short)(u[i / 2] >> (16 * (i & 1))));
-    }
+struct Chans {
+  uint4 r;
+  __device__ __forceinline__ void load(const void* p, size_t idx) {
+    if constexpr (V == 1) r.x = __float_as_uint(ld_p<T>(p, idx));
+    else r = *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + idx * kElem<T>);
   }
-}
+  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ float get(int i) const {
+    const unsigned u[4] = {r.x, r.y, r.z, r.w};
+    if constexpr (V == 1 || kElem<T> == 4) return __uint_as_float(u[i]);
+    else return T::to((unsigned short)(u[i / 2] >> (16 * (i & 1))));
+  }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = get(i);
+  }
+};
 template <class T, int V>
 __device__ __forceinline__ void store_chans(void* p, size_t idx, const float (&v)[V]) {
   if constexpr (V == 1) {
@@ -66,19 +70,40 @@ __device__ __forceinline__ void store_chans(void* p, size_t idx, const float (&v
         make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
+// N elements of TW from idx on; VEC: the address and N allow 16-byte accesses.
+template <class TW, int N, bool VEC>
+__device__ __forceinline__ void load_run(float (&v)[N], const void* p, size_t idx) {
+  constexpr int W = 16 / kElem<TW>;
+  if constexpr (VEC && N % W == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+      Chans<TW, W> c;
+      c.load(p, idx + i);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[i + e] = c.get(e);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = ld_p<TW>(p, idx + i);
+  }
+}
 
 template <class T, int K, int V>
 struct ConvLane {
   float w[K][V], bias[V];
+  template <class TW>
+  __device__ __forceinline__ void load(const PackedConvArgs& a, int d) {
+    float all[V * K];   // (D, K): a channel's taps are neighbours
+    load_run<TW, V * K, (V > 1)>(all, a.w, (size_t)d * K);
+    load_run<TW, V, (V > 1)>(bias, a.bias, d);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < K; ++k) w[k][v] = all[v * K + k];
+  }
   __device__ __forceinline__ ConvLane(const PackedConvArgs& a, int d) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      bias[v] = a.wf32 ? ld_p<F32>(a.bias, d + v) : ld_p<T>(a.bias, d + v);
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        w[k][v] = a.wf32 ? ld_p<F32>(a.w, (size_t)(d + v) * K + k)
-                         : ld_p<T>(a.w, (size_t)(d + v) * K + k);
-    }
+    if (a.wf32) load<F32>(a, d);
+    else load<T>(a, d);
   }
   // The pre-activation of the step whose K inputs are win[0 .. K - 1].
   __device__ __forceinline__ float pre(const float (&win)[K][V], int v) const {
@@ -95,7 +120,9 @@ template <class T, int K, int V>
 __device__ __forceinline__ void conv_input(float (&v)[V], const PackedConvArgs& a,
                                            const Piece& pc, int t, int d) {
   if (t >= pc.begin) {
-    load_chans<T, V>(v, a.x, (size_t)t * a.ld_x + d);
+    Chans<T, V> c;
+    c.load(a.x, (size_t)t * a.ld_x + d);
+    c.get(v);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -105,13 +132,17 @@ __device__ __forceinline__ void conv_input(float (&v)[V], const PackedConvArgs& 
   }
 }
 
-// Block (pieces / 4, channels / (64 V)): 64 channel lanes by 4 pieces, so that a wave has one piece.
+// Rows of a piece, and those of them whose loads are in flight together.
+constexpr int kConvPiece = 16, kConvBackPiece = 32, kConvBackRows = 4;
+
+// Block (pieces / 4, channels / (64 V)): 64 channel lanes by 4 pieces, so that a wave has one
+// piece; all its rows are asked for at once (8192 x 1536 bf16: 24 us four at a time).
 template <class T, int K, int V>
 __global__ void __launch_bounds__(256)
 packed_conv_fwd_kernel(PackedConvArgs a, int pieces) {
   const int p = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (p >= pieces) return;
-  const Piece pc = find_piece(a.q, a.tc, p);
+  const Piece pc = find_piece(a.q, kConvPiece, p);
   if (pc.seq < 0) return;
   const int d = (blockIdx.y * 64 + (threadIdx.x & 63)) * V;
   if (d >= a.D) return;
@@ -122,28 +153,26 @@ packed_conv_fwd_kernel(PackedConvArgs a, int pieces) {
     for (int i = 0; i < pc.len; ++i) store_chans<T, V>(a.out, (size_t)(pc.t0 + i) * a.D + d, y);
     return;
   }
-  const ConvLane<T, K, V> L(a, d);
+  Chans<T, V> in[kConvPiece];
+#pragma unroll
+  for (int i = 0; i < kConvPiece; ++i)   // (rows behind the piece: its last one again)
+    if (pc.len > 0) in[i].load(a.x, (size_t)(pc.t0 + min(i, pc.len - 1)) * a.ld_x + d);
   float win[K][V];
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) conv_input<T, K, V>(win[k], a, pc, pc.t0 - K + 1 + k, d);
-  constexpr int U = 4;   // rows whose loads are in flight together
-  for (int i0 = 0; i0 < pc.len; i0 += U) {
-    float in[U][V];
+  const ConvLane<T, K, V> L(a, d);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u < pc.len) load_chans<T, V>(in[u], a.x, (size_t)(pc.t0 + i0 + u) * a.ld_x + d);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i0 + u >= pc.len) break;
+  for (int i = 0; i < kConvPiece; ++i) {
+    if (i < pc.len) {
+      in[i].get(win[K - 1]);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        win[K - 1][v] = in[u][v];
         const float s = L.pre(win, v);
         y[v] = s * sigmoid_f(s);
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) win[k][v] = win[k + 1][v];
       }
-      store_chans<T, V>(a.out, (size_t)(pc.t0 + i0 + u) * a.D + d, y);
+      store_chans<T, V>(a.out, (size_t)(pc.t0 + i) * a.D + d, y);
     }
   }
   if (pc.last && a.window_out) {
@@ -165,13 +194,14 @@ packed_conv_fwd_kernel(PackedConvArgs a, int pieces) {
 template <class T, int K, int V>
 __global__ void __launch_bounds__(256)
 packed_conv_bwd_kernel(PackedConvArgs a, int pieces) {
+  constexpr int U = kConvBackRows;
   __shared__ float sums[4][64 * V];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int p = blockIdx.x * 4 + wave;
   const int d = (blockIdx.y * 64 + lane) * V;
   Piece pc;
   pc.seq = -1;
-  if (p < pieces) pc = find_piece(a.q, a.tc, p);
+  if (p < pieces) pc = find_piece(a.q, kConvBackPiece, p);
   float dw[K + 1][V];
 #pragma unroll
   for (int k = 0; k <= K; ++k)
@@ -183,64 +213,83 @@ packed_conv_bwd_kernel(PackedConvArgs a, int pieces) {
     for (int v = 0; v < V; ++v) z[v] = 0.f;
     for (int i = 0; i < pc.len; ++i) store_chans<T, V>(a.dx, (size_t)(pc.t0 + i) * a.D + d, z);
   } else if (pc.seq >= 0 && d < a.D) {
-    const ConvLane<T, K, V> L(a, d);
-    const int end = pc.last ? pc.t0 + pc.len : max(cu_at(a.q, pc.seq + 1), pc.begin);
+    const int end = pc.last ? pc.t0 + pc.len
+                            : max(__builtin_amdgcn_readfirstlane(cu_at(a.q, pc.seq + 1)),
+                                  pc.begin);
+    const int rows = pc.len + K - 1;   // of the walk
+    Chans<T, V> nx[U], ng[U];
+    const auto load = [&](int i0) {   // (0 behind the sequence)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = pc.t0 + i0 + u;
+        nx[u].zero();
+        ng[u].zero();
+        if (i0 + u < rows && t < end) {
+          nx[u].load(a.x, (size_t)t * a.ld_x + d);
+          ng[u].load(a.dout, (size_t)t * a.ld_g + d);
+        }
+      }
+    };
+    load(0);
     float win[K][V], s[K][V];   // inputs t - K + 1 .. t; s of the same rows
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) conv_input<T, K, V>(win[k], a, pc, pc.t0 - K + 1 + k, d);
+    const ConvLane<T, K, V> L(a, d);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) s[k][v] = 0.f;
     // The rows t of the piece, and K - 1 behind it for their s (0 behind the sequence).
-    for (int i = 0; i < pc.len + K - 1; ++i) {
-      const int t = pc.t0 + i;
-      float in[V], g[V];
+    for (int i0 = 0; i0 < rows; i0 += U) {
+      Chans<T, V> cx[U], cg[U];
 #pragma unroll
-      for (int v = 0; v < V; ++v) in[v] = g[v] = 0.f;
-      if (t < end) {
-        load_chans<T, V>(in, a.x, (size_t)t * a.ld_x + d);
-        load_chans<T, V>(g, a.dout, (size_t)t * a.ld_g + d);
+      for (int u = 0; u < U; ++u) {
+        cx[u] = nx[u];
+        cg[u] = ng[u];
       }
-      float o[V];
+      if (i0 + U < rows) load(i0 + U);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        win[K - 1][v] = in[v];
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u, t = pc.t0 + i;
+        if (i >= rows) continue;
+        float o[V];
+        cx[u].get(win[K - 1]);
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) s[k][v] = s[k + 1][v];
-        float st = 0.f;
-        if (t < end) {
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+          for (int k = 0; k < K - 1; ++k) s[k][v] = s[k + 1][v];
           const float pre = L.pre(win, v), sg = sigmoid_f(pre);
-          st = g[v] * sg * __builtin_fmaf(pre, 1.f - sg, 1.f);
+          // (behind the sequence dout counts as 0, whatever pre is)
+          const float st = t < end ? cg[u].get(v) * sg * __builtin_fmaf(pre, 1.f - sg, 1.f) : 0.f;
+          s[K - 1][v] = st;
+          if (i < pc.len) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(st, win[k][v], dw[k][v]);
+            dw[K][v] += st;
+          }
+          // row t - K + 1: s_{t-K+1+m}, m = 0 .. K - 1, meets w_{K-1-m}
+          float acc = 0.f;
+#pragma unroll
+          for (int m = 0; m < K; ++m) acc = __builtin_fmaf(L.w[K - 1 - m][v], s[m][v], acc);
+          o[v] = acc;
+#pragma unroll
+          for (int k = 0; k < K - 1; ++k) win[k][v] = win[k + 1][v];
         }
-        s[K - 1][v] = st;
-        if (i < pc.len) {
+        const int r = t - K + 1;   // the row that o is the gradient of
+        if (a.dwindow_out && r >= end - (K - 1) && r < end) {
 #pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(st, win[k][v], dw[k][v]);
-          dw[K][v] += st;
+          for (int v = 0; v < V; ++v)
+            o[v] += ld_p<T>(a.dwindow_out,
+                            ((size_t)pc.seq * a.D + d + v) * (K - 1) + r - (end - (K - 1)));
         }
-        // row t - K + 1: s_{t-K+1+m}, m = 0 .. K - 1, meets w_{K-1-m}
-        float acc = 0.f;
+        if (r >= pc.t0) {
+          store_chans<T, V>(a.dx, (size_t)r * a.D + d, o);
+        } else if (pc.j == 0 && a.dwindow) {   // the window's, rows begin - K + 1 .. begin - 1
 #pragma unroll
-        for (int m = 0; m < K; ++m) acc = __builtin_fmaf(L.w[K - 1 - m][v], s[m][v], acc);
-        o[v] = acc;
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k) win[k][v] = win[k + 1][v];
-      }
-      const int r = t - K + 1;   // the row that o is the gradient of
-      if (a.dwindow_out && r >= end - (K - 1) && r < end) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          o[v] += ld_p<T>(a.dwindow_out,
-                          ((size_t)pc.seq * a.D + d + v) * (K - 1) + r - (end - (K - 1)));
-      }
-      if (r >= pc.t0) {
-        store_chans<T, V>(a.dx, (size_t)r * a.D + d, o);
-      } else if (pc.j == 0 && a.dwindow) {   // the window's, rows begin - K + 1 .. begin - 1
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          st_p<T>(a.dwindow, ((size_t)pc.seq * a.D + d + v) * (K - 1) + r - (pc.begin - (K - 1)),
-                  o[v]);
+          for (int v = 0; v < V; ++v)
+            st_p<T>(a.dwindow, ((size_t)pc.seq * a.D + d + v) * (K - 1) + r - (pc.begin - (K - 1)),
+                    o[v]);
+        }
       }
     }
   }
@@ -260,20 +309,22 @@ packed_conv_bwd_kernel(PackedConvArgs a, int pieces) {
 }
 
 // dw (D, K), dbias (D): the blocks' partials (n, K + 1, D). A wave's lanes are
-// channels; each of a block's four waves adds every fourth partial.
+// channels; each of a block's 16 waves adds every sixteenth partial.
 template <class T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 packed_conv_sum_kernel(const float* part, void* dw, void* dbias, int wf32, int n, int K, int D) {
-  __shared__ float sums[4][64];
+  __shared__ float sums[16][64];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int d = blockIdx.x * 64 + lane, k = blockIdx.y;
   float s = 0.f;
   if (d < D)
-    for (int p = w; p < n; p += 4) s += part[((size_t)p * (K + 1) + k) * D + d];
+    for (int p = w; p < n; p += 16) s += part[((size_t)p * (K + 1) + k) * D + d];
   sums[w][lane] = s;
   __syncthreads();
   if (w || d >= D) return;
-  s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  s = sums[0][lane];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += sums[i][lane];
   void* to = k < K ? dw : dbias;
   const size_t at = k < K ? (size_t)d * K + k : (size_t)d;
   if (wf32) st_p<F32>(to, at, s);
