@@ -26,9 +26,28 @@ def rows_ok(t: torch.Tensor) -> bool:
             and (n <= 1 or w <= t.stride(0) < MAX_STRIDE))
 
 
-def _ld(t: torch.Tensor) -> int:
-    n, w = t.shape
-    return t.stride(0) if n > 1 else w
+def _ld(t: torch.Tensor, rows: int, width: int) -> int:
+    return t.stride(0) if rows > 1 else width
+
+
+# Each check has a quick form first, a single expression over what usually holds, and only
+# where that is false the one that names what is wrong (the checks were a third of a small
+# call's host time: a conv step 15.8 us, 6.0 of them the check's).
+
+def _like(t: torch.Tensor, shape, dtype, index: int) -> bool:
+    """t has the shape, type and device, and rows that the kernels read."""
+    return (t.shape == shape and t.dtype is dtype and t.get_device() == index and rows_ok(t))
+
+
+def _f32(t: Optional[torch.Tensor], shape, index: int) -> bool:
+    return t is None or (t.shape == shape and t.dtype is torch.float32
+                         and t.get_device() == index and t.is_contiguous()
+                         and not t.data_ptr() & 15)
+
+
+def _ints(t: torch.Tensor, index: int) -> bool:
+    return (t.dim() == 1 and t.dtype in _INTS and t.get_device() == index
+            and t.is_contiguous())
 
 
 def _act(what: str, x: torch.Tensor, **like: Optional[torch.Tensor]) -> None:
@@ -65,7 +84,22 @@ def _no_state(x: torch.Tensor) -> torch.Tensor:
 
 # ----------------------------------------------------------------- the scan
 
+def _scan_ok(x, dt, aneg, b_in, c_in, cu, h0) -> bool:
+    if x.dim() != 2 or aneg.dim() != 2 or x.dtype not in DTYPES:
+        return False
+    index, dtype, shape = x.get_device(), x.dtype, x.shape
+    d, n = aneg.shape
+    bc = (shape[0], n)
+    return (index >= 0 and 1 <= n <= MAX_STATE and d >= 1 and shape[1] == d and rows_ok(x)
+            and _like(dt, shape, dtype, index) and _like(b_in, bc, dtype, index)
+            and _like(c_in, bc, dtype, index) and _f32(aneg, (d, n), index)
+            and _ints(cu, index) and cu.shape[0] >= 1
+            and _f32(h0, (cu.shape[0] - 1, d, n), index))
+
+
 def _check_packed_scan(what: str, x, dt, aneg, b_in, c_in, cu, h0) -> None:
+    if _scan_ok(x, dt, aneg, b_in, c_in, cu, h0):
+        return
     _on_one_device(what, x, dt, aneg, b_in, c_in, cu, h0)
     _act(what, x, dt=dt, B=b_in, C=c_in)
     _need(aneg.dim() == 2, what, f"Aneg must be (D, N); got {tuple(aneg.shape)}")
@@ -82,11 +116,6 @@ def _check_packed_scan(what: str, x, dt, aneg, b_in, c_in, cu, h0) -> None:
     _dense16(what, Aneg=aneg, h0=h0)
 
 
-def _scan_workspace(lib, x, n: int, seqs: int, backward: bool):
-    nbytes = lib.mhs_packed_scan_workspace_bytes(seqs, x.shape[0], x.shape[1], n, backward)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None), nbytes
-
-
 def _packed_scan_fwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
                           b_in: torch.Tensor, c_in: torch.Tensor, cu: torch.Tensor,
                           h0: Optional[torch.Tensor], want_state: bool, with_ckpt: bool
@@ -98,14 +127,16 @@ def _packed_scan_fwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     y = x.new_empty((rows, d))
     h_last = aneg.new_empty((seqs, d, n) if want_state else (0,))
     ckpt = aneg.new_empty((lib.mhs_packed_ckpt_floats(rows, d, n) if with_ckpt else 0,))
-    with _on(x.device):
-        ws, nbytes = _scan_workspace(lib, x, n, seqs, False)
+    dev = x.device
+    with _on(dev):
+        nbytes = lib.mhs_packed_scan_workspace_bytes(seqs, rows, d, n, 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.mhs_packed_scan_fwd(
-            DTYPES[x.dtype], x.data_ptr(), _ld(x), dt.data_ptr(), _ld(dt), aneg.data_ptr(),
-            b_in.data_ptr(), _ld(b_in), c_in.data_ptr(), _ld(c_in), cu.data_ptr(),
-            cu.dtype == torch.int64, _ptr(h0), y.data_ptr(),
+            DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
+            _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
+            c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64, _ptr(h0), y.data_ptr(),
             h_last.data_ptr() if want_state else None, ckpt.data_ptr() if with_ckpt else None,
-            seqs, rows, d, n, _ptr(ws), nbytes, _stream(x.device))
+            seqs, rows, d, n, _ptr(ws), nbytes, _stream(dev))
     _check(rc, "mhs_packed_scan_fwd")
     return y, h_last, ckpt
 
@@ -138,21 +169,34 @@ def _packed_scan_bwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     db, dc = x.new_empty((rows, n)), x.new_empty((rows, n))
     da = aneg.new_empty((d, n))
     dh0 = aneg.new_empty((seqs, d, n) if h0 is not None else (0,))
-    with _on(x.device):
-        ws, nbytes = _scan_workspace(lib, x, n, seqs, True)
+    dev = x.device
+    with _on(dev):
+        nbytes = lib.mhs_packed_scan_workspace_bytes(seqs, rows, d, n, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.mhs_packed_scan_bwd(
-            DTYPES[x.dtype], x.data_ptr(), _ld(x), dt.data_ptr(), _ld(dt), aneg.data_ptr(),
-            b_in.data_ptr(), _ld(b_in), c_in.data_ptr(), _ld(c_in), cu.data_ptr(),
-            cu.dtype == torch.int64, _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy),
+            DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
+            _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
+            c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64, _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy, rows, d),
             _ptr(dh_last), dx.data_ptr(), ddt.data_ptr(), da.data_ptr(), db.data_ptr(),
             dc.data_ptr(), dh0.data_ptr() if h0 is not None else None, seqs, rows, d, n, _ptr(ws),
-            nbytes, _stream(x.device))
+            nbytes, _stream(dev))
     _check(rc, "mhs_packed_scan_bwd")
     return dx, ddt, da, db, dc, dh0
 
 
+def _scan_bwd_ok(x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last) -> bool:
+    if not _scan_ok(x, dt, aneg, b_in, c_in, cu, h0):
+        return False
+    index = x.get_device()
+    d, n = aneg.shape
+    return (_like(dy, x.shape, x.dtype, index) and _f32(dh_last, (cu.shape[0] - 1, d, n), index)
+            and _f32(ckpt, (x.shape[0] // CKPT * d * n,), index))
+
+
 def _check_packed_scan_bwd(x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last) -> None:
     what = "packed_scan_bwd"
+    if _scan_bwd_ok(x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last):
+        return
     _check_packed_scan(what, x, dt, aneg, b_in, c_in, cu, h0)
     _on_one_device(what, x, ckpt, dy, dh_last)
     _act(what, x, dy=dy)
@@ -191,7 +235,30 @@ def _check_taps(what: str, x, w, bias) -> None:
     _need(w.is_contiguous() and bias.is_contiguous(), what, "weight and bias must be contiguous")
 
 
+def _taps_ok(x, w, bias, index: int) -> bool:
+    if x.dim() != 2 or w.dim() != 2 or x.dtype not in DTYPES or not rows_ok(x):
+        return False
+    d, k = w.shape
+    return (index >= 0 and d >= 1 and 1 <= k <= MAX_TAPS and x.shape[1] == d
+            and (w.dtype is x.dtype or w.dtype is torch.float32) and w.get_device() == index
+            and w.is_contiguous() and bias.shape == (d,) and bias.dtype is w.dtype
+            and bias.get_device() == index and bias.is_contiguous())
+
+
+def _window_ok(t, x, entries: int, taps: int, index: int) -> bool:
+    return t is None or (t.shape == (entries, x.shape[1], taps - 1) and t.dtype is x.dtype
+                         and t.get_device() == index and t.is_contiguous())
+
+
+def _conv_ok(x, w, bias, cu, window) -> bool:
+    index = x.get_device()
+    return (_taps_ok(x, w, bias, index) and _ints(cu, index) and cu.shape[0] >= 1
+            and _window_ok(window, x, cu.shape[0] - 1, w.shape[1], index))
+
+
 def _check_packed_conv(what: str, x, w, bias, cu, window) -> None:
+    if _conv_ok(x, w, bias, cu, window):
+        return
     _on_one_device(what, x, w, bias, cu, window)
     _act(what, x)
     _check_taps(what, x, w, bias)
@@ -208,12 +275,13 @@ def _packed_conv_fwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, 
     k, seqs = w.shape[1], cu.numel() - 1
     out = x.new_empty((rows, d))
     last = x.new_empty((seqs, d, k - 1) if want_window else (0,))
-    with _on(x.device):
+    dev = x.device
+    with _on(dev):
         rc = library().mhs_packed_conv_fwd(
-            DTYPES[x.dtype], x.data_ptr(), _ld(x), w.data_ptr(), bias.data_ptr(),
+            DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), w.data_ptr(), bias.data_ptr(),
             w.dtype == torch.float32, cu.data_ptr(), cu.dtype == torch.int64, _ptr(window),
             out.data_ptr(), last.data_ptr() if want_window else None, seqs, rows, d, k,
-            _stream(x.device))
+            _stream(dev))
     _check(rc, "mhs_packed_conv_fwd")
     return out, last
 
@@ -241,21 +309,29 @@ def _packed_conv_bwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, 
     lib = library()
     dx, dw, db = x.new_empty((rows, d)), torch.empty_like(w), torch.empty_like(bias)
     dwin = x.new_empty((seqs, d, k - 1) if window is not None else (0,))
-    with _on(x.device):
+    dev = x.device
+    with _on(dev):
         nbytes = lib.mhs_packed_conv_bwd_workspace_bytes(seqs, rows, d, k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.mhs_packed_conv_bwd(
-            DTYPES[x.dtype], x.data_ptr(), _ld(x), w.data_ptr(), bias.data_ptr(),
+            DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), w.data_ptr(), bias.data_ptr(),
             w.dtype == torch.float32, cu.data_ptr(), cu.dtype == torch.int64, _ptr(window),
-            dout.data_ptr(), _ld(dout), _ptr(dlast), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
-            dwin.data_ptr() if window is not None else None, seqs, rows, d, k, ws.data_ptr(),
-            nbytes, _stream(x.device))
+            dout.data_ptr(), _ld(dout, rows, d), _ptr(dlast), dx.data_ptr(), dw.data_ptr(),
+            db.data_ptr(), dwin.data_ptr() if window is not None else None, seqs, rows, d, k, ws.data_ptr(),
+            nbytes, _stream(dev))
     _check(rc, "mhs_packed_conv_bwd")
     return dx, dw, db, dwin
 
 
+def _conv_bwd_ok(x, w, bias, cu, window, dout, dlast) -> bool:
+    return (_conv_ok(x, w, bias, cu, window) and _like(dout, x.shape, x.dtype, x.get_device())
+            and _window_ok(dlast, x, cu.shape[0] - 1, w.shape[1], x.get_device()))
+
+
 def _check_packed_conv_bwd(x, w, bias, cu, window, dout, dlast) -> None:
     what = "packed_conv_bwd"
+    if _conv_bwd_ok(x, w, bias, cu, window, dout, dlast):
+        return
     _check_packed_conv(what, x, w, bias, cu, window)
     _on_one_device(what, x, dout, dlast)
     _act(what, x, dout=dout)
@@ -287,8 +363,17 @@ def _check_slots(what: str, slots, rows: int, pool: int) -> None:
               f"{slots.dtype} {tuple(slots.shape)}")
 
 
+def _slots_ok(slots, rows: int, pool: int, index: int) -> bool:
+    return rows <= pool if slots is None else _ints(slots, index) and slots.shape[0] == rows
+
+
 def _check_conv_step(x, w, bias, window, slots) -> None:
     what = "conv_step"
+    index = x.get_device()
+    if (_taps_ok(x, w, bias, index) and window.dim() == 3
+            and _window_ok(window, x, window.shape[0], w.shape[1], index)
+            and _slots_ok(slots, x.shape[0], window.shape[0], index)):
+        return
     _on_one_device(what, x, w, bias, window, slots)
     _act(what, x)
     _check_taps(what, x, w, bias)
@@ -304,12 +389,13 @@ def _conv_step_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, window
     """out (rows, D); window's entries advanced in place."""
     rows, d = x.shape
     out = x.new_empty((rows, d))
-    with _on(x.device):
+    dev = x.device
+    with _on(dev):
         rc = library().mhs_conv_step(
-            DTYPES[x.dtype], x.data_ptr(), _ld(x), w.data_ptr(), bias.data_ptr(),
+            DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), w.data_ptr(), bias.data_ptr(),
             w.dtype == torch.float32, window.data_ptr(), _ptr(slots),
             slots is not None and slots.dtype == torch.int64, out.data_ptr(), rows,
-            window.shape[0], d, w.shape[1], _stream(x.device))
+            window.shape[0], d, w.shape[1], _stream(dev))
     _check(rc, "mhs_conv_step")
     return out
 
@@ -324,6 +410,15 @@ def _conv_step_fake(x, w, bias, window, slots):
 
 def _check_state_step(h, x, dt, aneg, b_in, c_in, slots) -> None:
     what = "state_step"
+    if x.dim() == 2 and h.dim() == 3 and x.dtype in DTYPES:
+        index, dtype, shape = x.get_device(), x.dtype, x.shape
+        pool, d, n = h.shape
+        bc = (shape[0], n)
+        if (index >= 0 and 1 <= n <= MAX_STATE and d >= 1 and shape[1] == d and rows_ok(x)
+                and _like(dt, shape, dtype, index) and _like(b_in, bc, dtype, index)
+                and _like(c_in, bc, dtype, index) and _f32(aneg, (d, n), index)
+                and _f32(h, (pool, d, n), index) and _slots_ok(slots, shape[0], pool, index)):
+            return
     _on_one_device(what, h, x, dt, aneg, b_in, c_in, slots)
     _act(what, x, dt=dt, B=b_in, C=c_in)
     _need(h.dim() == 3, what, f"h must be (entries, D, N); got {tuple(h.shape)}")
@@ -344,13 +439,16 @@ def _state_step_impl(h: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, aneg: t
                      ) -> torch.Tensor:
     """y (rows, D); h's entries advanced in place."""
     rows, d = x.shape
+    n = h.shape[2]
     y = x.new_empty((rows, d))
-    with _on(x.device):
+    dev = x.device
+    with _on(dev):
         rc = library().mhs_state_step(
-            DTYPES[x.dtype], h.data_ptr(), x.data_ptr(), _ld(x), dt.data_ptr(), _ld(dt),
-            aneg.data_ptr(), b_in.data_ptr(), _ld(b_in), c_in.data_ptr(), _ld(c_in), _ptr(slots),
+            DTYPES[x.dtype], h.data_ptr(), x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
+            _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
+            c_in.data_ptr(), _ld(c_in, rows, n), _ptr(slots),
             slots is not None and slots.dtype == torch.int64, y.data_ptr(), rows, h.shape[0], d,
-            h.shape[2], _stream(x.device))
+            n, _stream(dev))
     _check(rc, "mhs_state_step")
     return y
 
@@ -365,8 +463,23 @@ def _state_step_fake(h, x, dt, aneg, b_in, c_in, slots):
 
 # ----------------------------------------------------------------- sampling
 
+def _vector(t, rows: int, index: int) -> bool:
+    return t is None or (t.shape == (rows,) and t.dtype is torch.float32
+                         and t.get_device() == index and t.is_contiguous())
+
+
 def _check_sample(logits, uniform, temperature, top_k, top_p, min_p, values_f, value_k) -> None:
     what = "sample"
+    if logits.dim() == 2 and logits.dtype in DTYPES:
+        rows, vocab = logits.shape
+        index = logits.get_device()
+        if (index >= 0 and vocab >= 1 and (vocab == 1 or logits.stride(1) == 1)
+                and (rows <= 1 or logits.stride(0) >= vocab) and len(values_f) == 3
+                and uniform is not None and _vector(uniform, rows, index)
+                and _vector(temperature, rows, index) and _vector(top_p, rows, index)
+                and _vector(min_p, rows, index)
+                and (top_k is None or (_ints(top_k, index) and top_k.shape[0] == rows))):
+            return
     _on_one_device(what, logits, uniform, temperature, top_k, top_p, min_p)
     _need(logits.dim() == 2 and logits.shape[1] >= 1 and logits.dtype in DTYPES, what,
           "logits must be (rows, vocab) in float32, bfloat16 or float16; got "
@@ -389,18 +502,19 @@ def _sample_impl(logits: torch.Tensor, uniform: torch.Tensor, temperature: Optio
                  ) -> tuple[torch.Tensor, torch.Tensor]:
     """(tokens, log-probabilities); settings of the rows, or where None the values."""
     rows, vocab = logits.shape
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    logps = torch.empty(rows, dtype=torch.float32, device=logits.device)
     lib = library()
-    with _on(logits.device):
+    dev = logits.device
+    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+    logps = torch.empty(rows, dtype=torch.float32, device=dev)
+    with _on(dev):
         nbytes = lib.mhs_sample_workspace_bytes(rows, vocab, top_k is not None, value_k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.mhs_sample(
-            DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), uniform.data_ptr(),
+            DTYPES[logits.dtype], logits.data_ptr(), _ld(logits, rows, vocab), uniform.data_ptr(),
             _ptr(temperature), values_f[0], _ptr(top_k),
             top_k is not None and top_k.dtype == torch.int64, value_k, _ptr(top_p), values_f[1],
             _ptr(min_p), values_f[2], tokens.data_ptr(), logps.data_ptr(), rows, vocab, _ptr(ws),
-            nbytes, _stream(logits.device))
+            nbytes, _stream(dev))
     _check(rc, "mhs_sample")
     return tokens, logps
 

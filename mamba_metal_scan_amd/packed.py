@@ -23,15 +23,35 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native, _native_packed
 from ._native import HipScanError, dispatch
 
 
 def _hip(what: str, *ts: Optional[torch.Tensor]) -> None:
-    if torch.version.hip is None or not all(t is None or t.is_cuda for t in ts):
-        raise RuntimeError(f"{what} needs its tensors on the ROCm device; got "
-                           + ", ".join(str(t.device) for t in ts if t is not None))
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            break
+    else:
+        if torch.version.hip is not None:
+            return
+    raise RuntimeError(f"{what} needs its tensors on the ROCm device; got "
+                       + ", ".join(str(t.device) for t in ts if t is not None))
+
+
+def _records(*ts: Optional[torch.Tensor]) -> bool:
+    """Whether autograd records what becomes of ts (requires_grad, or a forward-mode tangent):
+    else the forward runs without it."""
+    if torch.compiler.is_compiling():
+        return True
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    # (tangents there are only within a dual level)
+    return (getattr(forward_ad, "_current_level", 0) >= 0
+            and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts))
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -59,17 +79,24 @@ class SelectiveScanPackedHIP(torch.autograd.Function):
     """selective_scan_packed on the HIP kernels: (y, h_last) or y."""
 
     @staticmethod
+    def run(x, dt, aneg, b_in, c_in, cu, h0, return_state, with_ckpt):
+        """((y, h_last, ckpt), the operands as the kernels read them)."""
+        ts = (x, dt, aneg, b_in, c_in, cu, h0)
+        # (while tracing the registered op checks itself)
+        if torch.compiler.is_compiling() or not _native_packed._scan_ok(*ts):
+            ts = (_rows(x), _rows(dt), _dense(aneg), _rows(b_in), _rows(c_in), cu.contiguous(),
+                  _dense(h0))
+            if not torch.compiler.is_compiling():
+                _native_packed._check_packed_scan("selective_scan_packed", *ts)
+        return dispatch("packed_scan_fwd")(*ts, return_state, with_ckpt), ts
+
+    @staticmethod
     def forward(ctx, x, dt, aneg, b_in, c_in, cu, h0, return_state):
-        x, dt, b_in, c_in = (_rows(t) for t in (x, dt, b_in, c_in))
-        aneg, h0, cu = _dense(aneg), _dense(h0), cu.contiguous()
-        if not torch.compiler.is_compiling():   # (the registered op checks itself)
-            _native_packed._check_packed_scan("selective_scan_packed", x, dt, aneg, b_in, c_in,
-                                              cu, h0)
         grad = any(ctx.needs_input_grad)
-        y, h_last, ckpt = dispatch("packed_scan_fwd")(x, dt, aneg, b_in, c_in, cu, h0,
-                                                      return_state, grad)
+        (y, h_last, ckpt), ts = SelectiveScanPackedHIP.run(x, dt, aneg, b_in, c_in, cu, h0,
+                                                           return_state, grad)
         if grad:
-            ctx.save_for_backward(x, dt, aneg, b_in, c_in, cu, h0, ckpt)
+            ctx.save_for_backward(*ts, ckpt)
         ctx.set_materialize_grads(False)
         return (y, h_last) if return_state else y
 
@@ -77,13 +104,15 @@ class SelectiveScanPackedHIP(torch.autograd.Function):
     def backward(ctx, dy, dh_last=None):
         _once("selective_scan_packed")
         x, dt, aneg, b_in, c_in, cu, h0, ckpt = ctx.saved_tensors
-        # (a saved-tensor hook may give them back in another layout)
-        x, dt, b_in, c_in = (_rows(t) for t in (x, dt, b_in, c_in))
-        aneg, h0, cu, ckpt = _dense(aneg), _dense(h0), cu.contiguous(), _dense(ckpt)
-        dy = torch.zeros_like(x) if dy is None else _rows(dy)
-        args = (x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, _dense(dh_last))
-        if not torch.compiler.is_compiling():
-            _native_packed._check_packed_scan_bwd(*args)
+        if dy is None:
+            dy = torch.zeros_like(x)
+        args = (x, dt, aneg, b_in, c_in, cu, h0, ckpt, dy, dh_last)
+        if torch.compiler.is_compiling() or not _native_packed._scan_bwd_ok(*args):
+            # (gradients of any layout; a saved-tensor hook may give another one, too)
+            args = (_rows(x), _rows(dt), _dense(aneg), _rows(b_in), _rows(c_in), cu.contiguous(),
+                    _dense(h0), _dense(ckpt), _rows(dy), _dense(dh_last))
+            if not torch.compiler.is_compiling():
+                _native_packed._check_packed_scan_bwd(*args)
         dx, ddt, da, db, dc, dh0 = dispatch("packed_scan_bwd")(*args)
         return dx, ddt, da, db, dc, None, dh0 if h0 is not None else None, None
 
@@ -92,15 +121,22 @@ class ConvSiluPackedHIP(torch.autograd.Function):
     """conv1d_silu_packed on the HIP kernels: (out, windows) or out."""
 
     @staticmethod
+    def run(x, weight, bias, cu, window, return_window):
+        """((out, windows), the operands as the kernels read them)."""
+        ts = (x, weight if weight.dim() == 2 else weight.reshape(weight.shape[0], -1), bias, cu,
+              window)
+        if torch.compiler.is_compiling() or not _native_packed._conv_ok(*ts):
+            ts = (_rows(x), ts[1].contiguous(), bias.contiguous(), cu.contiguous(),
+                  window.contiguous() if window is not None else None)
+            if not torch.compiler.is_compiling():
+                _native_packed._check_packed_conv("conv1d_silu_packed", *ts)
+        return dispatch("packed_conv_fwd")(*ts, return_window), ts
+
+    @staticmethod
     def forward(ctx, x, weight, bias, cu, window, return_window):
-        x, cu = _rows(x), cu.contiguous()
-        w = weight.reshape(weight.shape[0], -1).contiguous()
-        bias, window = bias.contiguous(), window.contiguous() if window is not None else None
-        if not torch.compiler.is_compiling():
-            _native_packed._check_packed_conv("conv1d_silu_packed", x, w, bias, cu, window)
-        out, last = dispatch("packed_conv_fwd")(x, w, bias, cu, window, return_window)
+        (out, last), ts = ConvSiluPackedHIP.run(x, weight, bias, cu, window, return_window)
         if any(ctx.needs_input_grad):
-            ctx.save_for_backward(x, w, bias, cu, window)
+            ctx.save_for_backward(*ts)
         ctx.wshape = weight.shape
         ctx.set_materialize_grads(False)
         return (out, last) if return_window else out
@@ -109,12 +145,15 @@ class ConvSiluPackedHIP(torch.autograd.Function):
     def backward(ctx, dout, dlast=None):
         _once("conv1d_silu_packed")
         x, w, bias, cu, window = ctx.saved_tensors
-        x, w, bias, cu = _rows(x), w.contiguous(), bias.contiguous(), cu.contiguous()
-        window = window.contiguous() if window is not None else None
-        dout = torch.zeros_like(x) if dout is None else _rows(dout)
-        args = (x, w, bias, cu, window, dout, dlast.contiguous() if dlast is not None else None)
-        if not torch.compiler.is_compiling():
-            _native_packed._check_packed_conv_bwd(*args)
+        if dout is None:
+            dout = torch.zeros_like(x)
+        args = (x, w, bias, cu, window, dout, dlast)
+        if torch.compiler.is_compiling() or not _native_packed._conv_bwd_ok(*args):
+            args = (_rows(x), w.contiguous(), bias.contiguous(), cu.contiguous(),
+                    window.contiguous() if window is not None else None, _rows(dout),
+                    dlast.contiguous() if dlast is not None else None)
+            if not torch.compiler.is_compiling():
+                _native_packed._check_packed_conv_bwd(*args)
         dx, dw, db, dwin = dispatch("packed_conv_bwd")(*args)
         return (dx, dw.view(ctx.wshape), db, None, dwin if window is not None else None, None)
 
@@ -143,7 +182,10 @@ def conv1d_silu_packed(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be (L, D); got {tuple(x.shape)}")
     _conv_weight(what, weight, x.shape[1])
-    return ConvSiluPackedHIP.apply(x, weight, bias, cu_seqlens, window, return_window)
+    if _records(x, weight, bias, window):
+        return ConvSiluPackedHIP.apply(x, weight, bias, cu_seqlens, window, return_window)
+    out = ConvSiluPackedHIP.run(x, weight, bias, cu_seqlens, window, return_window)[0]
+    return out if return_window else out[0]
 
 
 def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
@@ -163,7 +205,11 @@ def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     for name, t in (("x", x), ("dt", dt), ("B", b_in), ("C", c_in)):
         if t.dim() != 2:
             raise ValueError(f"{what}: {name} must have two dimensions; got {tuple(t.shape)}")
-    return SelectiveScanPackedHIP.apply(x, dt, aneg, b_in, c_in, cu_seqlens, h0, return_state)
+    if _records(x, dt, aneg, b_in, c_in, h0):
+        return SelectiveScanPackedHIP.apply(x, dt, aneg, b_in, c_in, cu_seqlens, h0, return_state)
+    y, h_last, _ = SelectiveScanPackedHIP.run(x, dt, aneg, b_in, c_in, cu_seqlens, h0,
+                                              return_state, False)[0]
+    return (y, h_last) if return_state else y
 
 
 def _in_place(what: str, name: str, t: torch.Tensor) -> None:
@@ -173,7 +219,7 @@ def _in_place(what: str, name: str, t: torch.Tensor) -> None:
 
 
 def _no_grad(what: str, *ts: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if _records(*ts) and not torch.compiler.is_compiling():
         raise RuntimeError(f"{what} updates its pool in place and has no gradients; call it "
                            "under torch.no_grad()")
 
@@ -195,8 +241,9 @@ def conv1d_silu_step(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
     _no_grad(what, x, weight, bias, window)
     if not window.is_contiguous():
         raise ValueError(f"{what} updates window in place; it must be contiguous")
-    args = (_rows(x), weight.reshape(weight.shape[0], -1).contiguous(), bias.contiguous(), window,
-            slots.contiguous() if slots is not None else None)
+    args = (_rows(x),
+            (weight if weight.dim() == 2 else weight.reshape(weight.shape[0], -1)).contiguous(),
+            bias.contiguous(), window, slots.contiguous() if slots is not None else None)
     if not torch.compiler.is_compiling():
         _native_packed._check_conv_step(*args)
     return dispatch("conv_step")(*args)
