@@ -134,8 +134,8 @@ def _packed_scan_fwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
         rc = lib.mhs_packed_scan_fwd(
             DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
             _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
-            c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64, _ptr(h0), y.data_ptr(),
-            h_last.data_ptr() if want_state else None, ckpt.data_ptr() if with_ckpt else None,
+            c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64,
+            _ptr(h0), y.data_ptr(), h_last.data_ptr() if want_state else None, ckpt.data_ptr() if with_ckpt else None,
             seqs, rows, d, n, _ptr(ws), nbytes, _stream(dev))
     _check(rc, "mhs_packed_scan_fwd")
     return y, h_last, ckpt
@@ -176,8 +176,8 @@ def _packed_scan_bwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
         rc = lib.mhs_packed_scan_bwd(
             DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
             _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
-            c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64, _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy, rows, d),
-            _ptr(dh_last), dx.data_ptr(), ddt.data_ptr(), da.data_ptr(), db.data_ptr(),
+            c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64,
+            _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy, rows, d), _ptr(dh_last), dx.data_ptr(), ddt.data_ptr(), da.data_ptr(), db.data_ptr(),
             dc.data_ptr(), dh0.data_ptr() if h0 is not None else None, seqs, rows, d, n, _ptr(ws),
             nbytes, _stream(dev))
     _check(rc, "mhs_packed_scan_bwd")
@@ -317,8 +317,8 @@ def _packed_conv_bwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, 
             DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), w.data_ptr(), bias.data_ptr(),
             w.dtype == torch.float32, cu.data_ptr(), cu.dtype == torch.int64, _ptr(window),
             dout.data_ptr(), _ld(dout, rows, d), _ptr(dlast), dx.data_ptr(), dw.data_ptr(),
-            db.data_ptr(), dwin.data_ptr() if window is not None else None, seqs, rows, d, k, ws.data_ptr(),
-            nbytes, _stream(dev))
+            db.data_ptr(), dwin.data_ptr() if window is not None else None, seqs, rows, d, k,
+            ws.data_ptr(), nbytes, _stream(dev))
     _check(rc, "mhs_packed_conv_bwd")
     return dx, dw, db, dwin
 

@@ -24,6 +24,9 @@ plain torch; the selective scan is the only custom kernel:
   a one-token call then advances the state. On a ROCm device without
   autograd that step is the fused ``selective_state_step`` kernel; with
   autograd enabled it is the differentiable torch update.
+* Packed sequences: ``prefill`` fills the cache from prompts of unlike length,
+  ``generate`` samples from there, ``loss`` takes packed documents (packed.py,
+  sampling.py); on the HIP path.
 * d_inner is solved so that a Mamba block costs what a transformer block of
   the same d_model / d_ff costs (model.py:58-82).
 """
@@ -45,6 +48,8 @@ from .fused import mamba_inner, out_gate, selective_scan_gated
 from .head import LOGITS_BYTES, distill_loss, linear_cross_entropy, linear_distill_loss
 from .linear import PLAIN, linear, no_hooks
 from .norm import add_rms_norm, rms_norm, rms_norm_residual
+from .packed import conv1d_silu_packed, selective_scan_packed
+from .sampling import sample_tokens
 from .scan import SSM_CHUNK, _hip_device, selective_scan, selective_state_step
 from .xent import cross_entropy
 
@@ -372,6 +377,30 @@ class MambaBlock(nn.Module):
         return self.out_proj(y * F.silu(z))
 
 
+    def mix_packed(self, h, cu_seqlens, cache=None):
+        """mix() of packed sequences: h (L, d_model), cu_seqlens as conv1d_silu_packed
+        takes them. With a cache every sequence goes on from its window and state there
+        (from nothing if the cache is empty), and leaves those behind its last token. On
+        the HIP path only."""
+        x, z = self._linear(self.in_proj, h).chunk(2, dim=-1)            # (L, d_inner)
+        before = cache if cache else {}
+        keep = cache is not None
+        x = conv1d_silu_packed(x, self.conv.weight, self.conv.bias, cu_seqlens,
+                               window=before.get("conv"), return_window=keep)
+        if keep:
+            x, window = x
+        dt, b_t, c_t, aneg = self._proj(x)
+        y = selective_scan_packed(x, dt, aneg, b_t, c_t, cu_seqlens, h0=before.get("h"),
+                                  return_state=keep)
+        if keep:
+            y, state = y
+            cache["conv"], cache["h"] = window, state
+        if self._fused(y):
+            y = out_gate(y.unsqueeze(0), self.D_skip, z.unsqueeze(0)).squeeze(0)
+            return self._linear(self.out_proj, y)
+        return self.out_proj((y + self.D_skip) * F.silu(z))
+
+
 _METHODS = frozenset(k for k, v in vars(MambaBlock).items() if callable(v))
 
 
@@ -445,6 +474,54 @@ class TinyMamba(nn.Module):
             x = block(x, bc)
         return self.ln_f(x)
 
+    def _hidden_packed(self, idx, cu_seqlens, caches):
+        """The final norm's output (L, d_model) for the packed tokens idx (L)."""
+        x = self.tok(idx)
+        if idx.dim() != 1 or self.cfg.scan_impl == "torch" or not _hip_device(x):
+            raise RuntimeError("packed sequences take tokens (L) on the HIP path; got "
+                               f"{tuple(idx.shape)} on {x.device}, scan_impl "
+                               f"{self.cfg.scan_impl!r}")
+        for block, bc in zip(self.blocks, caches):
+            x = x + block.mix_packed(block.norm(x), cu_seqlens, bc).to(x.dtype)
+        return self.ln_f(x)
+
+    def prefill(self, idx, cu_seqlens, cache):
+        """The logits (S, vocab) behind the last token of each of S packed prompts, idx (L)
+        and cu_seqlens (S + 1) as conv1d_silu_packed takes them (NaN for a prompt of no token).
+        The cache, a dict, is filled for S sequences, as forward's: a call with one token each
+        goes on from there, and so does a further prefill with the prompts' next parts."""
+        blocks = cache.setdefault("blocks", [{} for _ in self.blocks])
+        h = self._hidden_packed(idx, cu_seqlens, blocks)
+        ends = cu_seqlens[1:].long()
+        if idx.shape[0] == 0:
+            return h.new_full((ends.shape[0], self.cfg.vocab_size), float("nan"))
+        logits = linear(self.head, h[(ends - 1).clamp(min=0)])
+        return logits.masked_fill((ends <= cu_seqlens[:-1]).unsqueeze(1), float("nan"))
+
+    @torch.no_grad()
+    def generate(self, idx, cu_seqlens, max_new_tokens: int, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0, uniform=None, generator=None):
+        """max_new_tokens sampled for each of S packed prompts: (S, max_new_tokens) int64.
+
+        The settings are sample_tokens', numbers or a tensor (S) each; uniform
+        (S, max_new_tokens) holds the numbers to draw with (torch.rand's with generator, if not
+        given). Prefill, then a token per sequence and call."""
+        n = cu_seqlens.shape[0] - 1
+        if uniform is None:
+            uniform = torch.rand(n, max_new_tokens, generator=generator, device=idx.device)
+        if uniform.shape != (n, max_new_tokens):
+            raise ValueError(f"generate: uniform must be {(n, max_new_tokens)}; got "
+                             f"{tuple(uniform.shape)}")
+        out = idx.new_empty((n, max_new_tokens), dtype=torch.int64)
+        cache = {}
+        logits = self.prefill(idx, cu_seqlens, cache) if max_new_tokens else None
+        for i in range(max_new_tokens):
+            out[:, i] = sample_tokens(logits, uniform[:, i], temperature, top_k, top_p, min_p)
+            if i + 1 < max_new_tokens:
+                # (-1, of logits that leave no word, goes on with word 0)
+                logits = self(out[:, i:i + 1].clamp(min=0), cache=cache)[0][:, -1]
+        return out
+
     def _token(self, x, cache):
         """The logits of one embedded token per sequence against the cache as
         one native call, or None where that does not apply (see decode_step)."""
@@ -484,12 +561,15 @@ class TinyMamba(nn.Module):
                 and h.dtype in (torch.float32, torch.bfloat16, torch.float16))
 
     def loss(self, idx, targets, ignore_index: int = -100, reduction: str = "mean",
-             logits_bytes: int = LOGITS_BYTES):
+             logits_bytes: int = LOGITS_BYTES, cu_seqlens=None):
         """The cross entropy of forward(idx, targets) from the hidden states
         (linear_cross_entropy, on the HIP path). For its backward it may hold up to
         logits_bytes (1 GiB) of fp32 logits, each such loss its own, 0: none. reduction
-        "none": one loss per token (the tokens' negative log-probabilities)."""
-        h = self._hidden(self.tok(idx), [None] * len(self.blocks))
+        "none": one loss per token (the tokens' negative log-probabilities). With cu_seqlens
+        (S + 1) idx (L) holds packed documents, none of which sees another."""
+        none = [None] * len(self.blocks)
+        h = (self._hidden(self.tok(idx), none) if cu_seqlens is None
+             else self._hidden_packed(idx, cu_seqlens, none))
         flat = targets.reshape(-1)   # (of any shape, as forward takes them)
         if self._head_fused(h):
             loss = linear_cross_entropy(h.reshape(-1, h.size(-1)), self.head.weight, flat,
