@@ -236,9 +236,13 @@ def _check_taps(what: str, x, w, bias) -> None:
 
 
 def _taps_ok(x, w, bias, index: int) -> bool:
-    if x.dim() != 2 or w.dim() != 2 or x.dtype not in DTYPES or not rows_ok(x):
+    """(w (D, K), or (D, 1, K) as nn.Conv1d holds it: the same numbers in memory)"""
+    if x.dim() != 2 or x.dtype not in DTYPES or not rows_ok(x):
         return False
-    d, k = w.shape
+    shape = w.shape
+    if len(shape) != 2 and (len(shape) != 3 or shape[1] != 1):
+        return False
+    d, k = shape[0], shape[-1]
     return (index >= 0 and d >= 1 and 1 <= k <= MAX_TAPS and x.shape[1] == d
             and (w.dtype is x.dtype or w.dtype is torch.float32) and w.get_device() == index
             and w.is_contiguous() and bias.shape == (d,) and bias.dtype is w.dtype
@@ -253,7 +257,7 @@ def _window_ok(t, x, entries: int, taps: int, index: int) -> bool:
 def _conv_ok(x, w, bias, cu, window) -> bool:
     index = x.get_device()
     return (_taps_ok(x, w, bias, index) and _ints(cu, index) and cu.shape[0] >= 1
-            and _window_ok(window, x, cu.shape[0] - 1, w.shape[1], index))
+            and _window_ok(window, x, cu.shape[0] - 1, w.shape[-1], index))
 
 
 def _check_packed_conv(what: str, x, w, bias, cu, window) -> None:
@@ -272,7 +276,7 @@ def _packed_conv_fwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, 
                           ) -> tuple[torch.Tensor, torch.Tensor]:
     """(out, the windows behind the sequences or an empty tensor)."""
     rows, d = x.shape
-    k, seqs = w.shape[1], cu.numel() - 1
+    k, seqs = w.shape[-1], cu.numel() - 1
     out = x.new_empty((rows, d))
     last = x.new_empty((seqs, d, k - 1) if want_window else (0,))
     dev = x.device
@@ -305,7 +309,7 @@ def _packed_conv_bwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, 
                           ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dw, dbias, dwindow); the last empty without a window."""
     rows, d = x.shape
-    k, seqs = w.shape[1], cu.numel() - 1
+    k, seqs = w.shape[-1], cu.numel() - 1
     lib = library()
     dx, dw, db = x.new_empty((rows, d)), torch.empty_like(w), torch.empty_like(bias)
     dwin = x.new_empty((seqs, d, k - 1) if window is not None else (0,))
@@ -325,7 +329,7 @@ def _packed_conv_bwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, 
 
 def _conv_bwd_ok(x, w, bias, cu, window, dout, dlast) -> bool:
     return (_conv_ok(x, w, bias, cu, window) and _like(dout, x.shape, x.dtype, x.get_device())
-            and _window_ok(dlast, x, cu.shape[0] - 1, w.shape[1], x.get_device()))
+            and _window_ok(dlast, x, cu.shape[0] - 1, w.shape[-1], x.get_device()))
 
 
 def _check_packed_conv_bwd(x, w, bias, cu, window, dout, dlast) -> None:
@@ -367,12 +371,16 @@ def _slots_ok(slots, rows: int, pool: int, index: int) -> bool:
     return rows <= pool if slots is None else _ints(slots, index) and slots.shape[0] == rows
 
 
+def _conv_step_ok(x, w, bias, window, slots) -> bool:
+    index = x.get_device()
+    return (_taps_ok(x, w, bias, index) and window.dim() == 3
+            and _window_ok(window, x, window.shape[0], w.shape[-1], index)
+            and _slots_ok(slots, x.shape[0], window.shape[0], index))
+
+
 def _check_conv_step(x, w, bias, window, slots) -> None:
     what = "conv_step"
-    index = x.get_device()
-    if (_taps_ok(x, w, bias, index) and window.dim() == 3
-            and _window_ok(window, x, window.shape[0], w.shape[1], index)
-            and _slots_ok(slots, x.shape[0], window.shape[0], index)):
+    if _conv_step_ok(x, w, bias, window, slots):
         return
     _on_one_device(what, x, w, bias, window, slots)
     _act(what, x)
@@ -395,7 +403,7 @@ def _conv_step_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, window
             DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), w.data_ptr(), bias.data_ptr(),
             w.dtype == torch.float32, window.data_ptr(), _ptr(slots),
             slots is not None and slots.dtype == torch.int64, out.data_ptr(), rows,
-            window.shape[0], d, w.shape[1], _stream(dev))
+            window.shape[0], d, w.shape[-1], _stream(dev))
     _check(rc, "mhs_conv_step")
     return out
 
@@ -408,17 +416,22 @@ def _conv_step_fake(x, w, bias, window, slots):
     return x.new_empty(x.shape)
 
 
+def _state_step_ok(h, x, dt, aneg, b_in, c_in, slots) -> bool:
+    if x.dim() != 2 or h.dim() != 3 or x.dtype not in DTYPES:
+        return False
+    index, dtype, shape = x.get_device(), x.dtype, x.shape
+    pool, d, n = h.shape
+    bc = (shape[0], n)
+    return (index >= 0 and 1 <= n <= MAX_STATE and d >= 1 and shape[1] == d and rows_ok(x)
+            and _like(dt, shape, dtype, index) and _like(b_in, bc, dtype, index)
+            and _like(c_in, bc, dtype, index) and _f32(aneg, (d, n), index)
+            and _f32(h, (pool, d, n), index) and _slots_ok(slots, shape[0], pool, index))
+
+
 def _check_state_step(h, x, dt, aneg, b_in, c_in, slots) -> None:
     what = "state_step"
-    if x.dim() == 2 and h.dim() == 3 and x.dtype in DTYPES:
-        index, dtype, shape = x.get_device(), x.dtype, x.shape
-        pool, d, n = h.shape
-        bc = (shape[0], n)
-        if (index >= 0 and 1 <= n <= MAX_STATE and d >= 1 and shape[1] == d and rows_ok(x)
-                and _like(dt, shape, dtype, index) and _like(b_in, bc, dtype, index)
-                and _like(c_in, bc, dtype, index) and _f32(aneg, (d, n), index)
-                and _f32(h, (pool, d, n), index) and _slots_ok(slots, shape[0], pool, index)):
-            return
+    if _state_step_ok(h, x, dt, aneg, b_in, c_in, slots):
+        return
     _on_one_device(what, h, x, dt, aneg, b_in, c_in, slots)
     _act(what, x, dt=dt, B=b_in, C=c_in)
     _need(h.dim() == 3, what, f"h must be (entries, D, N); got {tuple(h.shape)}")
@@ -468,18 +481,23 @@ def _vector(t, rows: int, index: int) -> bool:
                          and t.get_device() == index and t.is_contiguous())
 
 
+def _sample_ok(logits, uniform, temperature, top_k, top_p, min_p, values_f) -> bool:
+    if logits.dim() != 2 or logits.dtype not in DTYPES:
+        return False
+    rows, vocab = logits.shape
+    index = logits.get_device()
+    return (index >= 0 and vocab >= 1 and (vocab == 1 or logits.stride(1) == 1)
+            and (rows <= 1 or logits.stride(0) >= vocab) and len(values_f) == 3
+            and uniform is not None and _vector(uniform, rows, index)
+            and _vector(temperature, rows, index) and _vector(top_p, rows, index)
+            and _vector(min_p, rows, index)
+            and (top_k is None or (_ints(top_k, index) and top_k.shape[0] == rows)))
+
+
 def _check_sample(logits, uniform, temperature, top_k, top_p, min_p, values_f, value_k) -> None:
     what = "sample"
-    if logits.dim() == 2 and logits.dtype in DTYPES:
-        rows, vocab = logits.shape
-        index = logits.get_device()
-        if (index >= 0 and vocab >= 1 and (vocab == 1 or logits.stride(1) == 1)
-                and (rows <= 1 or logits.stride(0) >= vocab) and len(values_f) == 3
-                and uniform is not None and _vector(uniform, rows, index)
-                and _vector(temperature, rows, index) and _vector(top_p, rows, index)
-                and _vector(min_p, rows, index)
-                and (top_k is None or (_ints(top_k, index) and top_k.shape[0] == rows))):
-            return
+    if _sample_ok(logits, uniform, temperature, top_k, top_p, min_p, values_f):
+        return
     _on_one_device(what, logits, uniform, temperature, top_k, top_p, min_p)
     _need(logits.dim() == 2 and logits.shape[1] >= 1 and logits.dtype in DTYPES, what,
           "logits must be (rows, vocab) in float32, bfloat16 or float16; got "

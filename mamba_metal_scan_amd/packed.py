@@ -123,11 +123,11 @@ class ConvSiluPackedHIP(torch.autograd.Function):
     @staticmethod
     def run(x, weight, bias, cu, window, return_window):
         """((out, windows), the operands as the kernels read them)."""
-        ts = (x, weight if weight.dim() == 2 else weight.reshape(weight.shape[0], -1), bias, cu,
-              window)
+        ts = (x, weight, bias, cu, window)
         if torch.compiler.is_compiling() or not _native_packed._conv_ok(*ts):
-            ts = (_rows(x), ts[1].contiguous(), bias.contiguous(), cu.contiguous(),
-                  window.contiguous() if window is not None else None)
+            _conv_weight("conv1d_silu_packed", weight, x.shape[1])
+            ts = (_rows(x), weight.reshape(weight.shape[0], -1).contiguous(), bias.contiguous(),
+                  cu.contiguous(), window.contiguous() if window is not None else None)
             if not torch.compiler.is_compiling():
                 _native_packed._check_packed_conv("conv1d_silu_packed", *ts)
         return dispatch("packed_conv_fwd")(*ts, return_window), ts
@@ -149,8 +149,9 @@ class ConvSiluPackedHIP(torch.autograd.Function):
             dout = torch.zeros_like(x)
         args = (x, w, bias, cu, window, dout, dlast)
         if torch.compiler.is_compiling() or not _native_packed._conv_bwd_ok(*args):
-            args = (_rows(x), w.contiguous(), bias.contiguous(), cu.contiguous(),
-                    window.contiguous() if window is not None else None, _rows(dout),
+            args = (_rows(x), w.reshape(w.shape[0], -1).contiguous(), bias.contiguous(),
+                    cu.contiguous(), window.contiguous() if window is not None else None,
+                    _rows(dout),
                     dlast.contiguous() if dlast is not None else None)
             if not torch.compiler.is_compiling():
                 _native_packed._check_packed_conv_bwd(*args)
@@ -181,7 +182,6 @@ def conv1d_silu_packed(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     _hip(what, x, weight, bias, cu_seqlens, window)
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be (L, D); got {tuple(x.shape)}")
-    _conv_weight(what, weight, x.shape[1])
     if _records(x, weight, bias, window):
         return ConvSiluPackedHIP.apply(x, weight, bias, cu_seqlens, window, return_window)
     out = ConvSiluPackedHIP.run(x, weight, bias, cu_seqlens, window, return_window)[0]
@@ -234,6 +234,9 @@ def conv1d_silu_step(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
     row has too, gives a row of NaN; neither changes an entry. weight and bias as for
     conv1d_silu_packed. Returns the (R, D) output. Not differentiable."""
     what = "conv1d_silu_step"
+    if not torch.compiler.is_compiling() and not _records(x, weight, bias, window) \
+            and _native_packed._conv_step_ok(x, weight, bias, window, slots):
+        return dispatch("conv_step")(x, weight, bias, window, slots)
     _hip(what, x, weight, bias, window, slots)
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be (R, D); got {tuple(x.shape)}")
@@ -259,6 +262,9 @@ def selective_state_step_slots(h: torch.Tensor, x: torch.Tensor, dt: torch.Tenso
     slots entry r), with padding and slots that do not hold as in conv1d_silu_step. Returns y (R, D)
     of x's type. Not differentiable."""
     what = "selective_state_step_slots"
+    if not torch.compiler.is_compiling() and not _records(h, x, dt, aneg, b_in, c_in) \
+            and _native_packed._state_step_ok(h, x, dt, aneg, b_in, c_in, slots):
+        return dispatch("state_step")(h, x, dt, aneg, b_in, c_in, slots)
     _hip(what, h, x, dt, aneg, b_in, c_in, slots)
     _no_grad(what, h, x, dt, aneg, b_in, c_in)
     if not torch.compiler.is_compiling():

@@ -56,12 +56,17 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     top_k, k = _setting(what, "top_k", top_k, lead, True)
     top_p, p = _setting(what, "top_p", top_p, lead, False)
     min_p, m = _setting(what, "min_p", min_p, lead, False)
-    z = logits.detach().reshape(-1, logits.shape[-1])
+    z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if (z.shape[1] > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < z.shape[1]):
         z = z.clone(memory_format=torch.contiguous_format)
-    args = (z, uniform.detach().to(torch.float32).reshape(-1).contiguous(), temperature, top_k,
-            top_p, min_p, [t, p, m], k)
+    if uniform.dim() != 1 or uniform.dtype is not torch.float32 or not uniform.is_contiguous():
+        uniform = uniform.to(torch.float32).reshape(-1).contiguous()
+    args = (z.detach() if z.requires_grad else z,
+            uniform.detach() if uniform.requires_grad else uniform, temperature, top_k, top_p,
+            min_p, [t, p, m], k)
     if not torch.compiler.is_compiling():
         _native_packed._check_sample(*args)
     tokens, logps = dispatch("sample")(*args)
-    return (tokens.view(lead), logps.view(lead)) if return_logprobs else tokens.view(lead)
+    if len(lead) != 1:
+        tokens, logps = tokens.view(lead), logps.view(lead)
+    return (tokens, logps) if return_logprobs else tokens
