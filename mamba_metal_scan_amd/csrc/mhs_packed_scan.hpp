@@ -5,13 +5,22 @@
 //
 // Mapping. The four lanes of a quad split the states of two neighbouring channels, NPL
 // each (4 NPL states a wave; a block has WS waves for the states and 4 / WS
-// times 32 channels). A register of x, dt or dy holds four steps, lane q of the
-// quad step q, and is broadcast within the multiply or multiply-add that uses it (a quad
-// permutation). B and C, which all channels share, go through LDS: a lane reads
-// its NPL states of a step at once. Each wave has its own tile of them, so that the waves
-// of a block run without barriers (but for sums over waves). The sums over the
+// times 32 channels). A register of x, dt or dy holds four steps as loaded, lane q of the
+// quad step q. B and C, which all channels share, go through LDS: a lane reads its NPL states of
+// a step at once; each wave has its own tiles, so that the waves of a block run without
+// barriers (but for sums over waves). So do dt and dt x (dy) in the forward and
+// the carry passes, four steps of a channel a read; the backward's main pass
+// takes them from its quad within the multiply or multiply-add (DPP). The sums over the
 // states are sums over a quad, those over the channels sums over the other four bits of
 // the lane, which every step of a reduce-scatter halves without a select.
+//
+// The vector units bound it: cycles of a wave's instruction, measured with four waves a
+// SIMD, multiply 2.9, multiply-add 4.8, exponential 8.3, and with a broadcast of a
+// lane of the quad in it 4.4 and 5.0, v_permlane swaps 8.3. Per step, channel and state the
+// carry passes need 19 of them, the forward 24 and the backward 70. (Operands by LDS or by DPP,
+// us, 32768 x 2048 x 16 bf16 | 8192 x 1536 x 16 fp32: carry 167 or 190 | 43 or 44, its
+// adjoint 175 or 185 | 40 or 43, the forward 277 or 282 | 66 or 65; the backward 655 or 660
+// | 170 or 146, its registers being full. The quad's sums by LDS too: 280 | 65, 665 | 153.)
 //
 // A sequence longer than a piece takes three launches: the carry pass walks
 // each piece but the last from a zero state and leaves its end state and its
@@ -90,7 +99,8 @@ struct StatePair {
     for (int c = 0; c < 2; ++c)
       off[c] = act[c] && valid > 0 ? 4u * ((unsigned)(d + c) * (unsigned)N + n0) : kOOB;
   }
-  __device__ __forceinline__ void load(float (&v)[2][NPL], const float* p, bool there = true) const {
+  __device__ __forceinline__ void load(float (&v)[2][NPL], const float* p,
+                                       bool there = true) const {
     const GBuf g(p, there ? bytes : 0u);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -246,6 +256,28 @@ __device__ __forceinline__ void quad_ready(float (&v)[2][M]) {
     asm("s_nop 1" : "+v"(v[0][0]), "+v"(v[0][1]), "+v"(v[0][2]), "+v"(v[0][3]), "+v"(v[1][0]),
         "+v"(v[1][1]), "+v"(v[1][2]), "+v"(v[1][3]));
 }
+
+// Rows of R floats per channel of a wave in LDS, channel c of pair p in row 16 c + p: of R =
+// 12 and 20 the 16 pairs' float4s lie in distinct banks. Register [c][k] (row 4 k + q of
+// channel c) goes to its place; a lane reads four rows of a channel.
+template <int S>
+struct ChanTile {
+  static constexpr int R = S + 4, kFloats = 32 * R;
+  static __device__ __forceinline__ void store(float* t, int pair, int q,
+                                               const float (&v)[2][S / 4]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int k = 0; k < S / 4; ++k) t[(16 * c + pair) * R + 4 * k + q] = v[c][k];
+  }
+  static __device__ __forceinline__ float4 rows(const float* t, int pair, int c, int k) {
+    return lds4(t + (16 * c + pair) * R + 4 * k);
+  }
+};
+__device__ __forceinline__ float at4(const float4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
 // Sums over the quad of v[s], s < 4: lane q ends with that of v[q].
 __device__ __forceinline__ float quad_gather(const float (&v)[4], int q) {
   float a[2], b[1];
@@ -271,7 +303,10 @@ __global__ void __launch_bounds__(256)
 packed_scan_fwd_kernel(PackedScanArgs a) {
   typedef ScanLane<NPL, WS> Lane;
   constexpr int NS = Lane::kStates;
-  __shared__ float tiles[4][2][kSub * NS];   // B, C of a wave's sub-chunk
+  typedef ChanTile<kSub> Tile;
+  // of a wave's sub-chunk: dt, dt x; B, C
+  __shared__ __align__(16) float chans[4][2][Tile::kFloats];
+  __shared__ __align__(16) float tiles[4][CARRY ? 1 : 2][kSub * NS];
   __shared__ float2 ysum[WS > 1 ? 2 : 1][WS > 1 ? 4 : 1][WS > 1 ? 4 : 1][64];
   const Piece pc = find_piece(a.q, a.tc, blockIdx.x);
   if (pc.seq < 0) return;
@@ -307,7 +342,9 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
   float* ck = a.ckpt + ((ptrdiff_t)(pc.begin / kCkpt + pc.j * (a.tc / kCkpt)) - 1) *
                            (ptrdiff_t)slice;
   float* const tb = tiles[L.wave][0];
-  float* const tc = tiles[L.wave][1];
+  float* const tc = tiles[L.wave][CARRY ? 0 : 1];
+  float* const td = chans[L.wave][0];
+  float* const tx = chans[L.wave][1];
   const int nsub = (pc.len + kSub - 1) / kSub;
   float nx[2][4], nd[2][4], nb[NPL], nc[NPL];   // the next sub-chunk's
   const auto load = [&](int i) {
@@ -319,16 +356,16 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
   load(0);
   float sum_dt[2] = {0.f, 0.f};
   for (int i = 0; i < nsub; ++i) {
-    float bx[2][4], dt[2][4];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        dt[c][k] = nd[c][k];
-        bx[c][k] = nd[c][k] * nx[c][k];
+        nx[c][k] *= nd[c][k];
         if (CARRY) sum_dt[c] += nd[c][k];
       }
     wave_lds_sync();
+    Tile::store(td, row, L.q, nd);
+    Tile::store(tx, row, L.q, nx);
     store_vec<NPL>(tb + L.lane * NPL, nb);
     if (!CARRY) store_vec<NPL>(tc + L.lane * NPL, nc);
     wave_lds_sync();
@@ -339,6 +376,8 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
         at.store(ck + (ptrdiff_t)(i * (kSub / kCkpt) + 4 * k / kCkpt) * (ptrdiff_t)slice, h,
                  (i > 0 || pc.j > 0 || k > 0) && i * kSub + 4 * k < pc.len);
       float y[2][4];
+      const float4 dt[2] = {Tile::rows(td, row, 0, k), Tile::rows(td, row, 1, k)};
+      const float4 bx[2] = {Tile::rows(tx, row, 0, k), Tile::rows(tx, row, 1, k)};
       static_for<4>([&](auto sc) {
         constexpr int s = decltype(sc)::value;
         float b[NPL], cv[NPL];
@@ -348,8 +387,8 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int j = 0; j < NPL; ++j) {
-            const float da = exp2_hw(quad_mul<s>(dt[c][k], a2[c][j]));
-            h[c][j] = __builtin_fmaf(da, h[c][j], quad_mul<s>(bx[c][k], b[j]));
+            const float da = exp2_hw(at4(dt[c], s) * a2[c][j]);
+            h[c][j] = __builtin_fmaf(da, h[c][j], at4(bx[c], s) * b[j]);
             if (!CARRY) y[c][s] = j ? __builtin_fmaf(cv[j], h[c][j], y[c][s]) : cv[j] * h[c][j];
           }
         }
@@ -441,7 +480,10 @@ __global__ void __launch_bounds__(256)
 packed_scan_back_carry_kernel(PackedScanArgs a) {
   typedef ScanLane<NPL, WS> Lane;
   constexpr int NS = Lane::kStates;
-  __shared__ float tiles[4][kSub * NS];   // C of a wave's sub-chunk
+  typedef ChanTile<kSub> Tile;
+  // of a wave's sub-chunk: dt, dy; C
+  __shared__ __align__(16) float chans[4][2][Tile::kFloats];
+  __shared__ __align__(16) float tiles[4][kSub * NS];
   const Piece pc = find_piece(a.q, a.tc, blockIdx.x);
   if (pc.seq < 0 || pc.seq == a.q.nseq || pc.j == 0) return;
   const Lane L(a.D);
@@ -459,6 +501,9 @@ packed_scan_back_carry_kernel(PackedScanArgs a) {
   const ChanLoad<T, kSub, VEC> ldy(a.dy, a.ld_dy, pc.t0, pc.len, a.D, L.d, L.q, L.act);
   const StateLoad<T, NPL, kSub, VEC> lc(a.C, a.ld_c, pc.t0, pc.len, a.N, L.n0, L.lane >> 2);
   float* const tc = tiles[L.wave];
+  float* const td = chans[L.wave][0];
+  float* const ty = chans[L.wave][1];
+  const int row = L.lane >> 2;
   float nd[2][4], ny[2][4], nc[NPL];
   const auto load = [&](int i) {   // (of a sub-chunk -1: zeros)
     ldt.load(nd, i);
@@ -469,32 +514,32 @@ packed_scan_back_carry_kernel(PackedScanArgs a) {
   load(nsub - 1);
   float sum_dt[2] = {0.f, 0.f};
   for (int i = nsub - 1; i >= 0; --i) {
-    float dt[2][4], dy[2][4];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        dt[c][k] = nd[c][k];
-        dy[c][k] = ny[c][k];
-        sum_dt[c] += nd[c][k];
-      }
-    quad_ready(dy);
+      for (int k = 0; k < 4; ++k) sum_dt[c] += nd[c][k];
     wave_lds_sync();
+    Tile::store(td, row, L.q, nd);
+    Tile::store(ty, row, L.q, ny);
     store_vec<NPL>(tc + L.lane * NPL, nc);
     wave_lds_sync();
     load(i - 1);
-    static_for<16>([&](auto tcn) {
-      constexpr int t = 15 - decltype(tcn)::value, k = t / 4, s = t % 4;
-      float cv[NPL];
-      load_vec<NPL>(cv, tc + t * NS + L.q * NPL);
+    static_for<4>([&](auto kcn) {
+      constexpr int k = 3 - decltype(kcn)::value;
+      const float4 dt[2] = {Tile::rows(td, row, 0, k), Tile::rows(td, row, 1, k)};
+      const float4 dy[2] = {Tile::rows(ty, row, 0, k), Tile::rows(ty, row, 1, k)};
+      static_for<4>([&](auto scn) {
+        constexpr int s = 3 - decltype(scn)::value;
+        float cv[NPL];
+        load_vec<NPL>(cv, tc + (4 * k + s) * NS + L.q * NPL);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-          quad_fmac<s>(u[c][j], dy[c][k], cv[j]);
-          u[c][j] *= exp2_hw(quad_mul<s>(dt[c][k], a2[c][j]));
+          for (int j = 0; j < NPL; ++j)
+            u[c][j] = __builtin_fmaf(at4(dy[c], s), cv[j], u[c][j]) *
+                      exp2_hw(at4(dt[c], s) * a2[c][j]);
         }
-      }
+      });
     });
   }
   at.store(a.carry + (size_t)blockIdx.x * slice, u);
