@@ -12,18 +12,22 @@
 // 2^17 words): sums that no order of additions changes, off by less than 2^-S of the
 // likeliest word's weight per word.
 //
-// The first kernel has a block per row. It reads the words for the maximum, each thread's own
-// being kept; the k-th largest of the threads' maxima bounds the k-th largest logit from
-// below (min-p bounds the kept words in the same way), and a second reading collects the few
-// words from there on in LDS. Up to 1024 words are all taken. What is asked of such a list
-// (the k-th word, the one at top-p's border, by index the one that is drawn) is each the first, in
-// an order, at which a running sum reaches a number: a descent over the order's bits, six at a
-// time, with the digits' sums in LDS.
-// The rows whose settings keep more words are left to further kernels: the weights by bins
-// of their logarithm (1/16 of a factor of 2), by part of 8192 words and by row, a block per part;
-// the words of the bin in which top-p's border falls, collected; and, by a block per row, their
-// cut, the part in which the draw falls (from the bins), and the word.
-// What no list holds (very many words of one weight, k above 1024 of many words) is found by
+// The first kernel has a block per row. It reads the words for the maximum, each thread
+// keeping those of its vectors (or, of a large vocabulary, of 16 groups of them). The k-th
+// largest of the threads' maxima bounds the k-th largest logit from below (min-p bounds
+// the kept words in the same way), and the few vectors that reach it are read again, their
+// words from there on collected in LDS. A list of up to 256 words is put in order by counting,
+// for each word, those before it by place and by index, and one wave then goes through its
+// running sums. What is asked of a longer list (the k-th word, the one at top-p's border,
+// by index the one that is drawn) is each the first, in an order, at which a running sum
+// reaches a number: a descent over the order's bits, six at a time, with the digits' sums
+// in LDS.
+// Rows whose settings keep more words (top-p alone, or no setting) are left to two further
+// kernels: the weights by bins of their logarithm (1/16 of a factor of 2), by part of 8192
+// words and by row, a block per part; and, a block per row, the words of the bin in which
+// top-p's border falls, their cut, the part in which the draw falls (from the bins), and the
+// word.
+// What no list holds (very many words of one weight, k above 2048 of many words) is found by
 // a search over the bits of the logits' keys, a reading each.
 #pragma once
 
@@ -32,10 +36,9 @@
 namespace mhs {
 
 constexpr int kMassBins = 1024;   // of 2^-1/16, down to 2^-64
-constexpr int kAllWords = 1024;   // up to this many words the first kernel takes all
 constexpr int kPart = 8192;       // words of a part
-constexpr int kFirstList = 2048;  // words of the first kernel's list
-constexpr int kRowList = 4096;    // of a row's list behind it
+constexpr int kSlots = 16;        // maxima that a thread keeps
+constexpr int kFlight = 8;        // loads in flight
 
 struct SampleArgs {
   const void* logits;        // (rows, vocab), rows ld apart
@@ -51,20 +54,14 @@ struct SampleArgs {
   int vocab, scale;          // weights are counted in 2^-scale
   // what the first kernel leaves
   struct SampleRow* state;   // (rows)
-  unsigned long long* bins;  // (rows, parts, kMassBins)
+  unsigned long long* bins;  // (rows, parts, kMassBins); of a row that has no top-p a part's sum
   int parts;
 };
-// What is left of a row: nothing; to look at all words; to cut and draw from list; to
-// search for the border.
-constexpr int kRowDone = 0, kRowAll = 1, kRowCut = 2, kRowSearch = 3;
 struct SampleRow {
   float m;
-  int left;
-  unsigned count;    // of list
-  int unused;
-  unsigned long long total[kMassBins], list[kRowList];
+  int left;                  // whether the row is left to the further kernels
+  unsigned long long total[kMassBins];
 };
-
 // Bits of an fp32 that a T's value never sets.
 template <class T> constexpr int kLowBits = 0;
 template <> constexpr int kLowBits<Bf16> = 16;
@@ -98,18 +95,26 @@ __device__ __forceinline__ u64 place_of(unsigned key, int i) {
 }
 __device__ __forceinline__ int index_at(u64 place) { return (int)(0xFFFFFFFFu - (unsigned)place); }
 
-template <int NTH_, int LIST>
-struct SampleShared {
-  static constexpr int NTH = NTH_, kWaves = NTH / 64, kList = LIST, E = LIST / NTH;
-  union {
-    u64 bins[kMassBins];
-    u64 list[LIST];
-  };
+// kList: words of a block's list; kShort: of one put in order by counting (the square of
+// that many comparisons, shared by the threads, 64 each).
+template <int NTH_>
+struct ListShared {
+  static constexpr int NTH = NTH_, kWaves = NTH / 64, kList = 4 * NTH,
+                       kShort = NTH == 1024 ? 256 : 128;
+  u64 list[kList];
+  u64 sorted[kShort], by_index[kShort];   // weights by place; places by index
+  unsigned order[kShort], ranks[kShort];  // by index the place's number; both of the list's
   u64 digits[3][64];
   u64 wave[kWaves];
-  float wave_f[kWaves];
+  float wave_f[2][kWaves];
+  unsigned count;
+};
+// Of the last kernel.
+struct RowShared : ListShared<1024> {
+  u64 bins[kMassBins];
+  u64 part[256];
   u64 above;
-  unsigned bin, count;
+  unsigned bin;
 };
 
 // v of the lane that CTRL names in the rows of ROWS, 0 where there is none.
@@ -169,47 +174,42 @@ __device__ __forceinline__ u64 block_before(Sh& sh, u64 v, u64* total) {
   return before;
 }
 
-// f(i, word i, group) for the words lo .. lo + n - 1, each once, by `threads` threads (this one
-// is number t): 16 bytes at a time but for the ends, four such loads in flight. The group
-// (0 .. 3) names one of four about equal shares of the thread's words.
+// f(i, word i) for the words of vector r, whose first is word b.
 template <class T, class F>
-__device__ __forceinline__ void for_groups(const char* row, int lo, int n, int t, int threads,
-                                           F&& f) {
+__device__ __forceinline__ void vector_words(const uint4& r, int b, F&& f) {
   constexpr int E = kElem<T>, W = 16 / E;
-  const char* p = row + (size_t)lo * E;
-  const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / E);
-  for (int i = t; i < head; i += threads) f(lo + i, ld_p<T>(row, lo + i), 0);
-  const int vecs = (n - head) / W;
-  const uint4* q = reinterpret_cast<const uint4*>(p + (size_t)head * E);
-  const int b = lo + head;
-  const auto word = [&](const uint4& r, int v, int group) {
-    const unsigned u[4] = {r.x, r.y, r.z, r.w};
+  const unsigned u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int e = 0; e < W; ++e) {
-      float x;
-      if constexpr (E == 4) x = __uint_as_float(u[e]);
-      else x = T::to((unsigned short)(u[e / 2] >> (16 * (e & 1))));
-      f(b + v * W + e, x, group);
-    }
-  };
-  int v = t;
-  for (; v + 3 * threads < vecs; v += 4 * threads) {
-    const uint4 r0 = q[v], r1 = q[v + threads], r2 = q[v + 2 * threads], r3 = q[v + 3 * threads];
-    word(r0, v, 0);
-    word(r1, v + threads, 1);
-    word(r2, v + 2 * threads, 2);
-    word(r3, v + 3 * threads, 3);
+  for (int e = 0; e < W; ++e) {
+    float x;
+    if constexpr (E == 4) x = __uint_as_float(u[e]);
+    else x = T::to((unsigned short)(u[e / 2] >> (16 * (e & 1))));
+    f(b + e, x);
   }
-  if (v < vecs) word(q[v], v, 0);
-  if (v + threads < vecs) word(q[v + threads], v + threads, 1);
-  if (v + 2 * threads < vecs) word(q[v + 2 * threads], v + 2 * threads, 2);
-  const int tail = head + vecs * W;
-  for (int i = tail + t; i < n; i += threads) f(lo + i, ld_p<T>(row, lo + i), 3);
 }
+
+// f(i, word i) for the words lo .. lo + n - 1, each once, by `threads` threads (this one is number t):
+// 16 bytes at a time but for the ends, four such loads in flight.
 template <class T, class F>
 __device__ __forceinline__ void for_words(const char* row, int lo, int n, int t, int threads,
                                           F&& f) {
-  for_groups<T>(row, lo, n, t, threads, [&](int i, float v, int) { f(i, v); });
+  constexpr int E = kElem<T>, W = 16 / E;
+  const char* p = row + (size_t)lo * E;
+  const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / E);
+  for (int i = t; i < head; i += threads) f(lo + i, ld_p<T>(row, lo + i));
+  const int vecs = (n - head) / W, b = lo + head;
+  const uint4* q = reinterpret_cast<const uint4*>(p + (size_t)head * E);
+  int v = t;
+  for (; v + 3 * threads < vecs; v += 4 * threads) {
+    const uint4 r0 = q[v], r1 = q[v + threads], r2 = q[v + 2 * threads], r3 = q[v + 3 * threads];
+    vector_words<T>(r0, b + v * W, f);
+    vector_words<T>(r1, b + (v + threads) * W, f);
+    vector_words<T>(r2, b + (v + 2 * threads) * W, f);
+    vector_words<T>(r3, b + (v + 3 * threads) * W, f);
+  }
+  for (; v < vecs; v += threads) vector_words<T>(q[v], b + v * W, f);
+  const int tail = head + vecs * W;
+  for (int i = tail + t; i < n; i += threads) f(lo + i, ld_p<T>(row, lo + i));
 }
 
 // The first index i of [from, from + n) with f(from) + .. + f(i) > target(total), total the
@@ -255,17 +255,17 @@ __device__ __forceinline__ int locate(Sh& sh, const char* row, int from, int n,
   return hit ? lo + __ffsll((long long)hit) - 1 : from + n;
 }
 
-// Of the entries order[e] (below 2^bits, those with w[e] > 0), from the largest on,
+// Of the n entries order[e] (below 2^bits, those with w[e] > 0), from the largest on,
 // the first at which the sum of w reaches `want` (1 .. their total). All threads of the block
 // call it; one barrier a digit of six bits, whose sums lie in one of three buffers: the one in
 // use, the next one's being cleared, the last one's still being read. (A bitonic sort
 // of 1024 entries took 28 us through LDS, 41 with its strides below 64 in registers; this
 // about 0.3 us a digit.)
 template <class Sh, int E>
-__device__ __forceinline__ u64 select(Sh& sh, const u64 (&order)[E], const u64 (&w)[E], int bits,
-                                      u64 want) {
+__device__ __forceinline__ u64 select(Sh& sh, const u64 (&order)[E], const u64 (&w)[E], int n,
+                                      int bits, u64 want, u64* found = nullptr) {
   const int tid = threadIdx.x, lane = tid & 63;
-  u64 prefix = 0, above = 0;
+  u64 prefix = 0, above = 0, reached = 0;
   __syncthreads();
   if (tid < 64) sh.digits[0][tid] = 0;
   __syncthreads();
@@ -278,48 +278,213 @@ __device__ __forceinline__ u64 select(Sh& sh, const u64 (&order)[E], const u64 (
     if (tid < 64) sh.digits[at][tid] = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (w[e] && order[e] >> up == prefix)
+      if (e * Sh::NTH < n && w[e] && order[e] >> up == prefix)
         atomicAdd(&now[(order[e] >> shift) & ((1u << (up - shift)) - 1)], w[e]);
     __syncthreads();
     const u64 v = now[63 - lane], run = above + wave_scan(v);
     const u64 hit = __ballot(run >= want);
     const int l = hit ? __ffsll((long long)hit) - 1 : 63;
+    reached = lane_u64(run, l);
     above = lane_u64(run - v, l);
     prefix = prefix << (up - shift) | (63 - l);
   }
+  if (found) *found = reached;
   return prefix;
 }
 __device__ __forceinline__ int bits_of(u64 v) { return v ? 64 - __clzll((long long)v) : 0; }
 
-// The places of the words that take(v) names go to list (of `most` entries, in LDS or not);
-// *count, 0 before, is how many there are.
-template <class T, class F>
-__device__ __forceinline__ void collect(u64* list, int most, unsigned* count, const char* row,
-                                        int lo, int n, int t, int threads, F&& take) {
-  for_words<T>(row, lo, n, t, threads, [&](int i, float v) {
-    if (!take(v)) return;
-    const unsigned at = atomicAdd(count, 1u);
-    if (at < (unsigned)most) list[at] = place_of(key_of<T>(as_logit(v)), i);
-  });
-}
-// The same of a whole row by its block, to the list in LDS (or another).
+// A row as its `head` words before the first whole vector, `vecs` vectors and `tail` words.
+template <class T>
+struct Vectors {
+  static constexpr int E = kElem<T>, W = 16 / E;
+  const char* row;
+  const uint4* q;
+  int V, head, vecs, tail;
+  __device__ __forceinline__ Vectors(const char* row_, int V_) : row(row_), V(V_) {
+    head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / E);
+    vecs = (V - head) / W;
+    tail = V - head - vecs * W;
+    q = reinterpret_cast<const uint4*>(row + (size_t)head * E);
+  }
+  template <class F>
+  __device__ __forceinline__ void in_head(F&& f) const {
+    if ((int)threadIdx.x < head) f((int)threadIdx.x, ld_p<T>(row, threadIdx.x));
+  }
+  template <class F>
+  __device__ __forceinline__ void in_tail(F&& f) const {
+    const int i = V - tail + threadIdx.x;
+    if (i < V) f(i, ld_p<T>(row, i));
+  }
+};
+
+// A row's words, a thread's largest ones kept: those of vectors t, t + kSlots, .. of the thread
+// in slot t (of NaN and where there is none -inf).
+template <class T, int NTH>
+struct SlotMaxima : Vectors<T> {
+  using Vectors<T>::q;
+  using Vectors<T>::vecs;
+  using Vectors<T>::head;
+  static constexpr int W = Vectors<T>::W;
+  float slot[kSlots], most;   // most: of the words before and behind the vectors too
+  __device__ __forceinline__ SlotMaxima(const char* row, int V) : Vectors<T>(row, V) {
+    const GBuf g(reinterpret_cast<const float*>(q), 16u * (unsigned)vecs);
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) slot[t] = -INFINITY;
+    for (int v0 = 0; v0 < vecs; v0 += kSlots * NTH) {
+#pragma unroll
+      for (int h = 0; h < kSlots; h += kFlight) {
+        if (v0 + h * NTH >= vecs) break;
+        uint4 r[kFlight];
+#pragma unroll
+        for (int t = 0; t < kFlight; ++t) {
+          const auto l = __builtin_amdgcn_raw_buffer_load_b128(
+              g.r, 16u * (unsigned)(v0 + (h + t) * NTH + (int)threadIdx.x), 0, 0);
+          r[t] = uint4{l[0], l[1], l[2], l[3]};
+        }
+#pragma unroll
+        for (int t = 0; t < kFlight; ++t) {
+          float w = -INFINITY;
+          vector_words<T>(r[t], 0, [&](int, float v) { w = fmaxf(w, v); });
+          if (v0 + (h + t) * NTH + (int)threadIdx.x >= vecs) w = -INFINITY;
+          slot[h + t] = fmaxf(slot[h + t], w);
+        }
+      }
+    }
+    most = -INFINITY;
+    const auto end = [&](int, float v) { most = fmaxf(most, v); };
+    this->in_head(end);
+    this->in_tail(end);
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) {
+      slot[t] += 0.f;   // (-0 as 0)
+      most = fmaxf(most, slot[t]);
+    }
+  }
+  // the largest of every fourth slot, from g on
+  __device__ __forceinline__ float group(int g) const {
+    return fmaxf(fmaxf(slot[g], slot[g + 4]), fmaxf(slot[g + 8], slot[g + 12]));
+  }
+  // f(vector, its first word) of the vectors in whose slot a word is >= from
+  template <class F>
+  __device__ __forceinline__ void vectors_from(float from, F&& f) const {
+    unsigned mask = 0;
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) mask |= slot[t] >= from ? 1u << t : 0u;
+    const auto next = [&] {   // (a thread's few loads: the next under way before one is used)
+      const int t = __ffs((int)mask) - 1;
+      mask &= mask - 1;
+      return t * NTH + (int)threadIdx.x;
+    };
+    if (!mask) return;
+    int v = next();
+    uint4 r = q[v];   // (a slot that has such a word has a vector)
+    for (;;) {
+      const int own = v;
+      const uint4 mine = r;
+      v += kSlots * NTH;
+      const bool more = v < vecs || mask;
+      if (v >= vecs && mask) v = next();
+      if (more) r = q[v];
+      f(mine, head + own * W);
+      if (!more) break;
+    }
+  }
+  // The first word that is m, the largest, of the thread's; V if there is none.
+  __device__ __forceinline__ int first(float m) const {
+    int at = this->V;
+    const auto look = [&](int i, float v) { at = v == m ? min(at, i) : at; };
+    vectors_from(m, [&](const uint4& r, int b) { vector_words<T>(r, b, look); });
+    this->in_head(look);
+    this->in_tail(look);
+    return at;
+  }
+  // The places of the words >= from (a finite number) to the list in LDS; how many there are.
+  template <class Sh>
+  __device__ __forceinline__ int collect(Sh& sh, float from) const {
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    const auto put = [&](unsigned at, int i, float v) {
+      if (at < (unsigned)Sh::kList) sh.list[at] = place_of(key_of<T>(v + 0.f), i);
+    };
+    vectors_from(from, [&](const uint4& r, int b) {
+      int n = 0;
+      vector_words<T>(r, b, [&](int, float v) { n += v >= from; });
+      unsigned at = n ? atomicAdd(&sh.count, (unsigned)n) : 0;
+      vector_words<T>(r, b, [&](int i, float v) {
+        if (v >= from) put(at++, i, v);
+      });
+    });
+    const auto end = [&](int i, float v) {
+      if (v >= from) put(atomicAdd(&sh.count, 1u), i, v);
+    };
+    this->in_head(end);
+    this->in_tail(end);
+    __syncthreads();
+    return (int)sh.count;
+  }
+};
+
+// The places of the row's words v in [lo, hi] that take(v) names, to the list in LDS; how many
+// there are. Of 16 vectors a thread notes which words are in the range, then looks at those
+// few again. (us of 465 words among 131072, looked at as they come: 16; this way 6.)
 template <class T, class Sh, class F>
-__device__ __forceinline__ int collect_row(Sh& sh, const char* row, int n, F&& take,
-                                           u64* list = nullptr, int most = 0) {
+__device__ __forceinline__ int collect(Sh& sh, const char* row, int n, float lo, float hi,
+                                       F&& take) {
+  constexpr int W = Vectors<T>::W, NTH = Sh::NTH;
+  const Vectors<T> words(row, n);
   __syncthreads();
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
-  collect<T>(list ? list : sh.list, list ? most : Sh::kList, &sh.count, row, 0, n, threadIdx.x,
-             Sh::NTH, take);
+  const auto word = [&](int i, float v) {
+    if (!(v >= lo && v <= hi && take(v))) return;
+    const unsigned at = atomicAdd(&sh.count, 1u);
+    if (at < (unsigned)Sh::kList) sh.list[at] = place_of(key_of<T>(as_logit(v)), i);
+  };
+  const GBuf g(reinterpret_cast<const float*>(words.q), 16u * (unsigned)words.vecs);
+  for (int v0 = 0; v0 < words.vecs; v0 += 16 * NTH) {
+    unsigned in[4] = {0, 0, 0, 0};   // a byte for a vector
+#pragma unroll
+    for (int h = 0; h < 16; h += kFlight) {
+      if (v0 + h * NTH >= words.vecs) break;
+      uint4 r[kFlight];
+#pragma unroll
+      for (int t = 0; t < kFlight; ++t) {
+        const auto l = __builtin_amdgcn_raw_buffer_load_b128(
+            g.r, 16u * (unsigned)(v0 + (h + t) * NTH + (int)threadIdx.x), 0, 0);
+        r[t] = uint4{l[0], l[1], l[2], l[3]};
+      }
+#pragma unroll
+      for (int t = 0; t < kFlight; ++t) {
+        unsigned bits = 0;
+        vector_words<T>(r[t], 0, [&](int e, float v) {
+          bits |= v >= lo && v <= hi ? 1u << e : 0u;
+        });
+        if (v0 + (h + t) * NTH + (int)threadIdx.x >= words.vecs) bits = 0;
+        in[(h + t) / 4] |= bits << (h + t) % 4 * 8;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      while (in[w]) {
+        const int b = __ffs((int)in[w]) - 1, v = v0 + (4 * w + b / 8) * NTH + (int)threadIdx.x;
+        in[w] &= in[w] - 1;
+        const int i = words.head + v * W + b % 8;
+        word(i, ld_p<T>(row, i));
+      }
+    }
+  }
+  words.in_head(word);
+  words.in_tail(word);
   __syncthreads();
   return (int)sh.count;
 }
 
 // 2^y for y <= 0 (0 below -64): e^(f ln 2) for the fraction |f| <= 1/2 by its series to the
-// 12th power (what is left out is below 2^-52), scaled by the integer part.
+// 12th power (what is left out is below 2^-52), scaled by the integer part, which an addition
+// of 1.5 2^52 rounds to and leaves in the sum's low bits.
 __device__ __forceinline__ double exp2_64(double y) {
   if (!(y > -64.0)) return 0.0;
-  const double n = rint(y), f = y - n;
+  const double t = y + 6755399441055744.0, f = y - (t - 6755399441055744.0);
   double p = 2.5678435993488196e-11;   // ln2^k / k!, k = 12 .. 0
   p = fma(p, f, 4.44553827187081e-10);
   p = fma(p, f, 7.054911620801121e-09);
@@ -333,7 +498,7 @@ __device__ __forceinline__ double exp2_64(double y) {
   p = fma(p, f, 0.2402265069591007);
   p = fma(p, f, 0.6931471805599453);
   p = fma(p, f, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
 // A row: its words, settings and largest logit, and what follows from them.
@@ -373,7 +538,8 @@ struct RowOf {
     return temp >= 0.f && temp < INFINITY && min_p <= 1.f && top_p == top_p && m > -INFINITY;
   }
   __device__ __forceinline__ double power(float v) const {   // log2 of the weight
-    return v == m ? 0.0 : peak ? -INFINITY : ((double)v - md) * rate;
+    if (peak) return v == m ? 0.0 : -INFINITY;
+    return ((double)v - md) * rate;
   }
   __device__ __forceinline__ u64 fixed(double w) const {   // w 2^scale, below 2^52, rounded
     return (u64)__double_as_longlong(w * one + 4503599627370496.0) & 0xFFFFFFFFFFFFFULL;
@@ -420,15 +586,16 @@ struct RowOf {
 // The list's entries in the threads' registers: their places (0: none) and weights.
 template <class T, class Sh>
 struct ListOf {
-  static constexpr int E = Sh::E;
+  static constexpr int E = Sh::kList / Sh::NTH;
   Sh& sh;
   const RowOf<T>& R;
   u64 place[E], w[E];
+  int n;
   int ib;           // bits of an index
   unsigned base;    // the smallest key
   int bits;         // of an order
-  __device__ __forceinline__ ListOf(Sh& shared, const RowOf<T>& row, int n, float from)
-      : sh(shared), R(row), ib(max(1, bits_of((u64)row.V - 1))), base(key_of<T>(from)) {
+  __device__ __forceinline__ ListOf(Sh& shared, const RowOf<T>& row, int count, float from)
+      : sh(shared), R(row), n(count), ib(max(1, bits_of((u64)row.V - 1))), base(key_of<T>(from)) {
     bits = bits_of(key_of<T>(R.m) - base) + ib;
     __syncthreads();
 #pragma unroll
@@ -443,7 +610,8 @@ struct ListOf {
     return (u64)((unsigned)(p >> 32) - base) << ib | ((1u << ib) - 1 - (unsigned)index_at(p));
   }
   __device__ __forceinline__ u64 place_at(u64 o) const {
-    return place_of((unsigned)(o >> ib) + base, (int)((1u << ib) - 1 - ((unsigned)o & ((1u << ib) - 1))));
+    const unsigned low = (1u << ib) - 1;
+    return place_of((unsigned)(o >> ib) + base, (int)(low - ((unsigned)o & low)));
   }
   // The place of the k-th entry.
   __device__ __forceinline__ u64 kth(int k) {
@@ -453,7 +621,7 @@ struct ListOf {
       o[e] = place[e] ? order(place[e]) : 0;
       w[e] = place[e] != 0;
     }
-    return place_at(select(sh, o, w, bits, (u64)k));
+    return place_at(select(sh, o, w, n, bits, (u64)k));
   }
   // The place of the last entry, of those from `least` on, that has less than top_p of
   // `all` (0: of their own weight) before it, `above` being the weight before them.
@@ -466,7 +634,7 @@ struct ListOf {
       sum += w[e];
     }
     if (all == 0) all = block_total(sh, sum);
-    return place_at(select(sh, o, w, bits, max((u64)1, R.border_of(all)) - above));
+    return place_at(select(sh, o, w, n, bits, max((u64)1, R.border_of(all)) - above));
   }
   // The draw from the entries from `least` on, with min-p: they are all that is kept.
   __device__ __forceinline__ void draw(u64 least) {
@@ -478,7 +646,7 @@ struct ListOf {
       sum += w[e];
     }
     const u64 total = block_total(sh, sum);
-    const u64 at = select(sh, o, w, ib, R.target_of(total) + 1);
+    const u64 at = select(sh, o, w, n, ib, R.target_of(total) + 1);
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (w[e] && o[e] == at) R.answer(index_at(place[e]), value(place[e]), total);
@@ -518,160 +686,153 @@ __device__ __forceinline__ int border_bin(Sh& sh, const RowOf<T>& R, F&& bin_at,
   return b;
 }
 
-// The weights of the words with bin(y) >= 0, y a weight's logarithm, added to the bins in LDS.
-template <class T, class Sh, class F>
-__device__ __forceinline__ void fill_bins(Sh& sh, const RowOf<T>& R, int lo, int n, F&& bin) {
+// The weights of a part's words with bin(y) >= 0, y a weight's logarithm, added to the bins:
+// `copies` of them in LDS, a lane's own by its number, whose adds to one bin wait for
+// each other.
+template <class T, int NTH, int COPIES, class F>
+__device__ __forceinline__ void fill_bins(u64* bins, const RowOf<T>& R, int lo, int n, F&& bin) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kMassBins; i += Sh::NTH) sh.bins[i] = 0;
+  for (int i = threadIdx.x; i < COPIES * kMassBins; i += NTH) bins[i] = 0;
   __syncthreads();
-  for_words<T>(R.row, lo, n, threadIdx.x, Sh::NTH, [&](int, float v) {
+  u64* const own = bins + threadIdx.x % COPIES * kMassBins;
+  for_words<T>(R.row, lo, n, threadIdx.x, NTH, [&](int, float v) {
     const double y = R.power(v);
     const int b = y > -64.0 ? bin(y) : -1;
     if (b < 0) return;
     const u64 w = R.fixed(exp2_64(y));
-    if (w) atomicAdd(&sh.bins[b], w);
+    if (w) atomicAdd(&own[b], w);
   });
   __syncthreads();
 }
 
-// The first kernel. PARTS: rows may be left.
-template <class T, class Sh, bool PARTS>
-__global__ void __launch_bounds__(Sh::NTH)
-sample_kernel(SampleArgs a) {
-  constexpr int NTH = Sh::NTH;
-  __shared__ Sh sh;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  RowOf<T> R(a, blockIdx.x);
-  const int V = a.vocab;
-  const char* row = R.row;
-  // ---- the largest logit
-  float mine[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  for_groups<T>(row, 0, V, tid, NTH,
-                [&](int, float v, int group) { mine[group] = fmaxf(mine[group], v); });
-#pragma unroll
-  for (int g = 0; g < 4; ++g) mine[g] = as_logit(mine[g]);
-  float m = fmaxf(fmaxf(mine[0], mine[1]), fmaxf(mine[2], mine[3]));
-  const float thread_max = m;
-#pragma unroll
-  for (int s = 32; s; s /= 2) m = fmaxf(m, __shfl_xor(m, s));
-  if (lane == 0) sh.wave_f[wave] = m;
+// A list of up to kShort words in order: sh.sorted, by_index, order. Every word is compared with
+// every other, a share of them by each thread. This thread's word (of tid < n) and its number.
+template <class T, class Sh>
+__device__ __forceinline__ u64 short_order(Sh& sh, const RowOf<T>& R, int n, unsigned* number) {
+  const int tid = threadIdx.x;
+  if (tid < Sh::kShort) sh.ranks[tid] = 0;
   __syncthreads();
+  int bits = 6;
+  while (1 << bits < n) ++bits;
+  const int e = tid & ((1 << bits) - 1), share = (1 << 2 * bits) / Sh::NTH;
+  const int j0 = (tid >> bits) * share, j1 = min(n, j0 + share);
+  const u64 p = e < n ? sh.list[e] : 0;
+  unsigned before = 0;   // by place and, in the upper half, by index
+  for (int j = j0; j < j1; ++j) {
+    const u64 o = sh.list[j];
+    before += (o > p) + ((unsigned)o > (unsigned)p ? 1u << 16 : 0u);
+  }
+  if (e < n && before) atomicAdd(&sh.ranks[e], before);
+  const u64 own = tid < n ? R.weight(value_of<T>((unsigned)(p >> 32))) : 0;
+  __syncthreads();
+  *number = ~0u;
+  if (tid < n) {
+    const unsigned r = sh.ranks[tid];
+    *number = r & 0xFFFF;
+    sh.sorted[r & 0xFFFF] = own;
+    sh.by_index[r >> 16] = p;
+    sh.order[r >> 16] = r & 0xFFFF;
+  }
+  __syncthreads();
+  return p;
+}
+// Of the first `kept` words in order, how many top-p keeps, `above` being the weight before
+// them and `all` (0: their own) the total. By one wave, four words a lane.
+template <class T, class Sh>
+__device__ __forceinline__ int short_kept(Sh& sh, const RowOf<T>& R, int kept, u64 above, u64 all) {
+  const int lane = threadIdx.x & 63;
+  u64 w[4], sum = 0;
 #pragma unroll
-  for (int w = 0; w < Sh::kWaves; ++w) m = fmaxf(m, sh.wave_f[w]);
-  R.set_max(m);
-  SampleRow* const st = PARTS ? a.state + R.r : nullptr;
-  if (PARTS && tid == 0) {
-    st->m = m;
-    st->left = kRowDone;
-    st->count = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int at = 4 * lane + i;
+    w[i] = at < kept ? sh.sorted[at] : 0;
+    sum += w[i];
   }
-  if (!R.valid()) {
-    if (tid == 0) {
-      a.tokens[R.r] = -1;
-      if (a.logprobs) a.logprobs[R.r] = __builtin_nanf("");
-    }
-    return;
-  }
-  if (R.temp == 0.f) {
-    u64 total;
-    const int token = locate<T>(sh, row, 0, V, [&](int, float v) { return (u64)(v == m); },
-                                [&](u64) -> u64 { return 0; }, &total);
-    if (tid == 0) R.answer(token, m, (u64)R.one);
-    return;
-  }
-  const int k = R.k > 0 && R.k < V ? (int)R.k : 0;
-  float from = -INFINITY;
-  if constexpr (PARTS) {
-    if (k > 2 * NTH || (k == 0 && (R.top_p < 1.f || !(R.low_v > -INFINITY)))) {
-      if (tid == 0) st->left = k ? kRowSearch : kRowAll;
-      for (int i = tid; i < kMassBins; i += NTH) st->total[i] = 0;
-      return;
-    }
-    if (k) {
-      // The k-th largest of the threads' own maxima, to 18 bits, rounded down; from
-      // k 129 on of four a thread (1024 maxima of which 1000 are wanted would let in a tenth of
-      // 131072 words, 4096 let in 1150).
-      constexpr int kBits = 32 - kLowBits<T>, kDrop = kBits > 18 ? kBits - 18 : 0;
-      unsigned at;
-      if (k <= NTH / 8) {
-        const u64 x[1] = {key_of<T>(thread_max) >> kDrop}, one[1] = {1};
-        at = (unsigned)select(sh, x, one, kBits - kDrop, (u64)k);
-      } else {
-        u64 x[4];
-        const u64 one[4] = {1, 1, 1, 1};
+  u64 run = wave_scan(sum);
+  const u64 border = R.border_of(all ? all : lane_u64(run, 63));
+  run += above - sum;
+  int count = 0;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) x[g] = key_of<T>(mine[g]) >> kDrop;
-        at = (unsigned)select(sh, x, one, kBits - kDrop, (u64)k);
-      }
-      if (at > key_of<T>(-INFINITY) >> kDrop) from = value_of<T>(at << kDrop);
-    } else {
-      from = R.low_v;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int at = 4 * lane + i;
+    count += __popcll(__ballot(at < kept && (at == 0 || run < border)));
+    run += w[i];
   }
-  // (!PARTS: all words; NaN too, as -inf)
-  const int n = collect_row<T>(sh, row, V, [&](float v) { return !PARTS || v >= from; });
-  if (PARTS && (n > Sh::kList || n < k)) {
-    // too many for this list: to the row's (the search where that is too short, or NaNs count)
-    if (n >= k && n <= kRowList) {
-      collect_row<T>(sh, row, V, [&](float v) { return v >= from; }, st->list, kRowList);
-      if (tid == 0) {
-        st->count = n;
-        st->left = kRowCut;
-      }
-    } else {
-      for (int i = tid; i < kMassBins; i += NTH) st->total[i] = 0;
-      if (tid == 0) st->left = k ? kRowSearch : kRowAll;
-    }
-    return;
+  return count;
+}
+// The place of the last word that top-p keeps of a list of up to kShort words.
+template <class T, class Sh>
+__device__ __forceinline__ u64 short_cut(Sh& sh, const RowOf<T>& R, int n, u64 above, u64 all) {
+  unsigned number;
+  const u64 p = short_order(sh, R, n, &number);
+  const int kept = short_kept(sh, R, n, above, all);   // (every wave alike)
+  if ((int)number == kept - 1) sh.wave[0] = p;
+  __syncthreads();
+  return sh.wave[0];
+}
+// The draw from a list of up to kShort words, with k (0: all), top-p and min-p.
+template <class T, class Sh>
+__device__ __forceinline__ void short_draw(Sh& sh, const RowOf<T>& R, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  const auto value = [](u64 p) { return value_of<T>((unsigned)(p >> 32)); };
+  unsigned number;
+  short_order(sh, R, n, &number);
+  if (threadIdx.x >= 64) return;
+  int kept = k && k < n ? k : n;
+  if (R.top_p < 1.f) kept = short_kept(sh, R, kept, 0, 0);
+  // four words by index
+  u64 w[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = 4 * lane + i;
+    const unsigned r = at < n ? sh.order[at] : ~0u;
+    w[i] = r >= (unsigned)kept ? 0
+           : R.min_p > 0.f ? R.counted(value(sh.by_index[at])) : sh.sorted[r];
+    sum += w[i];
   }
-  ListOf<T, Sh> list(sh, R, n, from);
-  u64 least = 0;
-  if (k) least = list.kth(k);
-  if (R.top_p < 1.f) least = list.cut(least, 0, 0);
-  list.draw(least);
+  u64 run = wave_scan(sum);
+  const u64 total = lane_u64(run, 63), target = R.target_of(total);
+  run -= sum;
+  int hit = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    run += w[i];
+    if (hit < 0 && run > target) hit = 4 * lane + i;
+  }
+  const u64 hits = __ballot(hit >= 0);
+  if (hits && lane == __ffsll((long long)hits) - 1) {
+    const u64 at = sh.by_index[hit];
+    R.answer(index_at(at), value(at), total);
+  }
 }
 
-// Part blockIdx.x of row blockIdx.y: its weights by bin, to the part's and to the row's.
-template <class T>
-__global__ void __launch_bounds__(256)
-sample_bins_kernel(SampleArgs a) {
-  __shared__ SampleShared<256, 1024> sh;
-  SampleRow& st = a.state[blockIdx.y];
-  if (st.left != kRowAll) return;
-  RowOf<T> R(a, blockIdx.y);
-  R.set_max(st.m);
-  if (R.peak) return;
-  const int lo = blockIdx.x * kPart;
-  fill_bins(sh, R, lo, min(kPart, R.V - lo), [&](double y) { return R.bin_of(y); });
-  u64* out = a.bins + ((size_t)blockIdx.y * a.parts + blockIdx.x) * kMassBins;
-  for (int i = threadIdx.x; i < kMassBins; i += 256) {
-    const u64 w = sh.bins[i];
-    out[i] = w;
-    if (w) atomicAdd(&st.total[i], w);
+// The same as locate of up to kPart words, each thread having 8 neighbouring ones: its
+// answer goes out at once.
+template <class T, class Sh, class F>
+__device__ __forceinline__ void locate_part(Sh& sh, const RowOf<T>& R, int from, int n, F&& f,
+                                            u64 before, u64 target, u64 total) {
+  constexpr int PER = kPart / Sh::NTH;
+  float v[PER];
+  u64 w[PER], sum = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = PER * threadIdx.x + e;
+    v[e] = i < n ? logit_at<T>(R.row, from + i) : -INFINITY;
   }
-}
-
-// The words of the border's bin, of a part, to the row's list.
-template <class T>
-__global__ void __launch_bounds__(256)
-sample_border_kernel(SampleArgs a) {
-  __shared__ SampleShared<256, 1024> sh;
-  SampleRow& st = a.state[blockIdx.y];
-  if (st.left != kRowAll) return;
-  RowOf<T> R(a, blockIdx.y);
-  R.set_max(st.m);
-  if (R.peak || !(R.top_p < 1.f)) return;
-  u64 above, all;
-  const int bin = border_bin(sh, R, [&](int i) { return st.total[i]; }, 0, &above, &all, ~0ULL);
-  const int lo = blockIdx.x * kPart;
-  float least, most;
-  R.bin_range(bin, &least, &most);
-  collect<T>(st.list, kRowList, &st.count, R.row, lo, min(kPart, R.V - lo), threadIdx.x, 256,
-             [&](float v) {
-               if (!(v >= least && v <= most)) return false;
-               const double y = R.power(v);
-               return y > -64.0 && R.bin_of(y) == bin;
-             });
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    w[e] = f(from + PER * (int)threadIdx.x + e, v[e]);
+    sum += w[e];
+  }
+  u64 all;
+  u64 run = before + block_before(sh, sum, &all);
+  if (!(run <= target && run + sum > target)) return;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (run <= target && run + w[e] > target)
+      R.answer(from + PER * (int)threadIdx.x + e, v[e], total);
+    run += w[e];
+  }
 }
 
 // The last kept place by a search over the bits of the keys: of the words, a reading a bit.
@@ -744,66 +905,212 @@ __device__ __forceinline__ u64 search_border(Sh& sh, const RowOf<T>& R) {
   return place_of(edge, last);
 }
 
+// The first kernel: rows of up to kList words, and those whose kept words fit the list.
+template <class T, int NTH>
+__global__ void __launch_bounds__(NTH)
+sample_kernel(SampleArgs a) {
+  typedef ListShared<NTH> Sh;
+  __shared__ Sh sh;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  RowOf<T> R(a, blockIdx.x);
+  const int V = a.vocab;
+  const SlotMaxima<T, NTH> words(R.row, V);
+  float m = words.most;
+  // (the least of the threads' finite maxima)
+  float least_most = words.most > -INFINITY ? words.most : INFINITY;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (words.group(g) > -INFINITY) least_most = fminf(least_most, words.group(g));
+#pragma unroll
+  for (int s = 32; s; s /= 2) {
+    m = fmaxf(m, __shfl_xor(m, s));
+    least_most = fminf(least_most, __shfl_xor(least_most, s));
+  }
+  if (lane == 0) {
+    sh.wave_f[0][wave] = m;
+    sh.wave_f[1][wave] = least_most;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < Sh::kWaves; ++w) {
+    m = fmaxf(m, sh.wave_f[0][w]);
+    least_most = fminf(least_most, sh.wave_f[1][w]);
+  }
+  R.set_max(m);
+  SampleRow* const st = V > Sh::kList ? a.state + R.r : nullptr;
+  if (st && tid == 0) {
+    st->m = m;
+    st->left = 0;
+  }
+  if (!R.valid()) {
+    if (tid == 0) {
+      a.tokens[R.r] = -1;
+      if (a.logprobs) a.logprobs[R.r] = __builtin_nanf("");
+    }
+    return;
+  }
+  if (R.temp == 0.f) {
+    int first = words.most == m ? words.first(m) : V;
+#pragma unroll
+    for (int s = 32; s; s /= 2) first = min(first, __shfl_xor(first, s));
+    if (lane == 0) sh.wave[wave] = (u64)first;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < Sh::kWaves; ++w) first = min(first, (int)sh.wave[w]);
+    if (tid == 0) R.answer(first, m, (u64)R.one);
+    return;
+  }
+  // ---- a list of all words that can be kept. (Words of -inf, and NaN, weigh nothing.)
+  int k = R.k > 0 && R.k < V ? (int)R.k : 0;
+  const bool nucleus = R.top_p < 1.f;
+  bool few = V <= Sh::kList;
+  float from = -__FLT_MAX__;
+  if (k && k <= 2 * NTH) {
+    // The k-th largest of the threads' own maxima, in 4096 steps between the least and the
+    // largest of them, rounded down; from k 129 on of four a thread (1024 maxima of which 1000
+    // are wanted would let in a tenth of 131072 words, 4096 let in 1150).
+    const unsigned base = key_of<T>(least_most), range = key_of<T>(m) - base;
+    const int drop = max(0, bits_of(range) - 12), bits = max(1, bits_of(range) - drop);
+    const auto step = [&](float v) -> u64 { return (key_of<T>(v) - base) >> drop; };
+    const auto counts = [](float v) -> u64 { return v > -INFINITY; };
+    u64 steps, found;
+    if (k <= NTH / 8) {
+      const u64 x[1] = {step(words.most)}, one[1] = {counts(words.most)};
+      steps = select(sh, x, one, NTH, bits, (u64)k, &found);
+    } else {
+      u64 x[4], one[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        x[g] = step(words.group(g));
+        one[g] = counts(words.group(g));
+      }
+      steps = select(sh, x, one, 4 * NTH, bits, (u64)k, &found);
+    }
+    if (found >= (u64)k) from = value_of<T>(base + ((unsigned)steps << drop));
+    few = true;
+  } else if (!k && !nucleus && R.low_v > -INFINITY) {
+    from = fmaxf(from, R.low_v);
+    few = true;
+  }
+  const int n = few ? words.collect(sh, from) : 0;
+  if (!few || n > Sh::kList) {
+    if (tid == 0) st->left = 1;
+    for (int i = tid; i < kMassBins; i += NTH) st->total[i] = 0;
+    return;
+  }
+  if (n <= k) k = 0;
+  if (n <= Sh::kShort) {
+    short_draw(sh, R, n, k);
+    return;
+  }
+  ListOf<T, Sh> list(sh, R, n, from);
+  u64 least = 0;
+  if (k) least = list.kth(k);
+  if (nucleus) least = list.cut(least, 0, 0);
+  list.draw(least);
+}
+
+// Of the rows left those that no k or +inf leaves to the search: part blockIdx.x of row
+// blockIdx.y, its weights by bin, to the part's and to the row's; without top-p their sum.
+template <class T>
+__global__ void __launch_bounds__(256)
+sample_bins_kernel(SampleArgs a) {
+  constexpr int kCopies = 4;
+  __shared__ u64 bins[kCopies][kMassBins];
+  SampleRow& st = a.state[blockIdx.y];
+  if (!st.left) return;
+  RowOf<T> R(a, blockIdx.y);
+  R.set_max(st.m);
+  const int lo = blockIdx.x * kPart, n = min(kPart, R.V - lo);
+  u64* out = a.bins + ((size_t)blockIdx.y * a.parts + blockIdx.x) * kMassBins;
+  if (!(R.top_p < 1.f)) {
+    u64 s = 0;
+    for_words<T>(R.row, lo, n, threadIdx.x, 256, [&](int, float v) { s += R.counted(v); });
+    s = wave_total(s);
+    if ((threadIdx.x & 63) == 0) bins[0][threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) out[0] = (bins[0][0] + bins[0][1]) + (bins[0][2] + bins[0][3]);
+    return;
+  }
+  if (R.peak || (R.k > 0 && R.k < R.V)) return;
+  fill_bins<T, 256, kCopies>(bins[0], R, lo, n, [&](double y) { return R.bin_of(y); });
+  for (int i = threadIdx.x; i < kMassBins; i += 256) {
+    u64 w = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) w += bins[c][i];
+    out[i] = w;
+    if (w) atomicAdd(&st.total[i], w);
+  }
+}
+
 // The rows left.
 template <class T>
 __global__ void __launch_bounds__(1024)
-sample_finish_kernel(SampleArgs a) {
-  constexpr int NTH = 1024;
-  typedef SampleShared<NTH, kRowList> Sh;
+sample_rest_kernel(SampleArgs a) {
+  typedef RowShared Sh;
+  constexpr int NTH = Sh::NTH;
   __shared__ Sh sh;
-  __shared__ u64 part_sum[256];
-  SampleRow& st = a.state[blockIdx.x];
-  if (st.left == kRowDone) return;
+  const SampleRow& st = a.state[blockIdx.x];
+  if (!st.left) return;
+  const int tid = threadIdx.x;
   RowOf<T> R(a, blockIdx.x);
   R.set_max(st.m);
-  const int tid = threadIdx.x, V = R.V, left = st.left;
-  const int k = R.k > 0 && R.k < V ? (int)R.k : 0;
-  u64 least = 0, total;
-  int bin = kMassBins;   // the bins before it are kept whole
-  int n = 0;             // words of it
-  const bool binned = left == kRowAll && a.parts > 1 && !R.peak;   // (by the kernels before)
-  bool search = left == kRowSearch || (R.peak && R.top_p < 1.f), by_parts = binned && a.parts <= 256;
-  if (left == kRowCut) {
-    n = (int)st.count;
-    for (int i = tid; i < n; i += NTH) sh.list[i] = st.list[i];
-    ListOf<T, Sh> list(sh, R, n, -INFINITY);
-    if (k) least = list.kth(k);
-    if (R.top_p < 1.f) least = list.cut(least, 0, 0);
-    list.draw(least);
-    return;
-  }
-  if (!search && R.top_p < 1.f) {
+  const int V = R.V;
+  const bool nucleus = R.top_p < 1.f, k = R.k > 0 && R.k < V;
+  // ---- the place of the last word that k and top-p keep
+  u64 least = 0;
+  bool search = k || (R.peak && nucleus);
+  bool by_parts = a.parts > 1 && a.parts <= 256 && !search;
+  int bin = 0, n = 0;   // the bins before it are kept whole; words of it
+  if (nucleus && !search) {
     u64 above, all;
-    if (binned) {
+    if (a.parts > 1) {
       bin = border_bin(sh, R, [&](int i) { return st.total[i]; }, 0, &above, &all, ~0ULL);
-      n = (int)st.count;
-      for (int i = tid; i < min(n, kRowList); i += NTH) sh.list[i] = st.list[i];
     } else {
-      fill_bins(sh, R, 0, V, [&](double y) { return R.bin_of(y); });
+      fill_bins<T, NTH, 1>(sh.bins, R, 0, V, [&](double y) { return R.bin_of(y); });
       bin = border_bin(sh, R, [&](int i) { return sh.bins[i]; }, 0, &above, &all, ~0ULL);
-      n = collect_row<T>(sh, R.row, V, [&](float v) {
-        const double y = R.power(v);
-        return y > -64.0 && R.bin_of(y) == bin;
-      });
     }
-    if (n > kRowList) {
+    // (where min-p's border is in a bin before it, that is the border; too near to a bin's end to
+    // tell, the words are gone through)
+    bool cut = true;
+    if (R.min_p > 0.f) {
+      const double y = log2(R.low);
+      if (R.bin_of(y + 1e-9) != R.bin_of(y - 1e-9)) {
+        by_parts = false;
+      } else if (R.bin_of(y) < bin) {
+        bin = R.bin_of(y);
+        cut = false;
+      }
+    }
+    float lo, hi;
+    R.bin_range(bin, &lo, &hi);
+    n = collect<T>(sh, R.row, V, lo, hi, [&](float v) {
+      const double y = R.power(v);
+      return y > -64.0 && R.bin_of(y) == bin;
+    });
+    if (n > Sh::kList && cut) {
       // a bin of many words (a flat distribution): 1024 bins of it
       by_parts = false;
       const auto sub = [&](double y) {
         return R.bin_of(y) == bin ? max(0, min(kMassBins - 1, (int)((y * -16.0 - bin) * kMassBins)))
                                   : -1;
       };
-      fill_bins(sh, R, 0, V, sub);
+      fill_bins<T, NTH, 1>(sh.bins, R, 0, V, sub);
       u64 none;
       const int at = border_bin(sh, R, [&](int i) { return sh.bins[i]; }, above, &above, &none,
                                 max((u64)1, R.border_of(all)));
-      n = collect_row<T>(sh, R.row, V, [&](float v) {
+      n = collect<T>(sh, R.row, V, lo, hi, [&](float v) {
         const double y = R.power(v);
         return y > -64.0 && sub(y) == at;
       });
     }
-    search = n > kRowList;
-    if (!search) {
+    if (!cut) {
+      by_parts = by_parts && n <= Sh::kList;
+    } else if (n > Sh::kList) {
+      search = true;
+    } else if (n <= Sh::kShort) {
+      least = short_cut(sh, R, n, above, all);
+    } else {
       ListOf<T, Sh> list(sh, R, n, -INFINITY);
       least = list.cut(0, above, all);
       __syncthreads();
@@ -814,52 +1121,43 @@ sample_finish_kernel(SampleArgs a) {
     least = search_border(sh, R);
     __syncthreads();
   }
-  const float from = value_of<T>((unsigned)(least >> 32));
-  const auto kept = [&](int i, float v) { return R.counted_from(least, from, i, v); };
-  if (R.min_p > 0.f) {
-    // (min-p may leave fewer)
-    const float lo = least ? fmaxf(from, R.low_v) : R.low_v;
-    n = collect_row<T>(sh, R.row, V, [&](float v) { return v >= lo; });
-    if (n <= kRowList) {
-      ListOf<T, Sh>(sh, R, n, lo).draw(least);
-      return;
-    }
-    by_parts = false;
-  }
-  int lo = 0, words = V;
-  u64 before = 0, want = 0;
+  const float low = value_of<T>((unsigned)(least >> 32));
+  const auto kept = [&](int i, float v) { return R.counted_from(least, low, i, v); };
+  // ---- the draw, from the part in which it falls
+  u64 total = 0;
   if (by_parts) {
     // the parts' kept weights: their bins before the border's, and its words that are kept
-    for (int p = tid; p < 256; p += NTH) part_sum[p] = 0;
-    __syncthreads();
     const u64* bins = a.bins + (size_t)R.r * a.parts * kMassBins;
-    for (int p = tid >> 6; p < a.parts; p += NTH / 64) {
+    for (int p = tid >> 6; p < a.parts; p += Sh::kWaves) {
       u64 s = 0;
-      for (int b = tid & 63; b < bin; b += 64) s += bins[(size_t)p * kMassBins + b];
-      s = wave_total(s);
-      if ((tid & 63) == 0) atomicAdd(&part_sum[p], s);
-    }
-    for (int i = tid; i < n; i += NTH) {
-      const u64 x = sh.list[i];
-      if (x >= least)
-        atomicAdd(&part_sum[index_at(x) / kPart], R.weight(value_of<T>((unsigned)(x >> 32))));
+      if (nucleus) {
+#pragma unroll 4
+        for (int b = tid & 63; b < bin; b += 64) s += bins[(size_t)p * kMassBins + b];
+        s = wave_total(s);
+      } else {
+        s = bins[(size_t)p * kMassBins];
+      }
+      if ((tid & 63) == 0) sh.part[p] = s;
     }
     __syncthreads();
-    total = 0;
-    for (int p = 0; p < a.parts; ++p) total += part_sum[p];
-    want = R.target_of(total);
+    if (nucleus) {
+      for (int i = tid; i < n; i += NTH) {
+        const u64 x = sh.list[i];
+        if (x >= least)
+          atomicAdd(&sh.part[index_at(x) / kPart], R.counted(value_of<T>((unsigned)(x >> 32))));
+      }
+      __syncthreads();
+    }
+    for (int p = 0; p < a.parts; ++p) total += sh.part[p];
+    const u64 want = R.target_of(total);
+    u64 before = 0;
     int p = 0;
-    while (p < a.parts - 1 && before + part_sum[p] <= want) before += part_sum[p++];
-    lo = p * kPart;
-    words = min(kPart, V - lo);
-    __syncthreads();
+    while (p < a.parts - 1 && before + sh.part[p] <= want) before += sh.part[p++];
+    locate_part(sh, R, p * kPart, min(kPart, V - p * kPart), kept, before, want, total);
+    return;
   }
-  u64 own;
-  const int token = locate<T>(sh, R.row, lo, words, kept, [&](u64 all) {
-    if (by_parts) return want - before;
-    total = all;
-    return R.target_of(all);
-  }, &own);
+  const int token = locate<T>(sh, R.row, 0, V, kept, [&](u64 all) { return R.target_of(all); },
+                              &total);
   if (tid == 0) R.answer(token, logit_at<T>(R.row, token), total);
 }
 

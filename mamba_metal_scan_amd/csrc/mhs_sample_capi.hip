@@ -10,6 +10,15 @@ using mhs::fail;
 
 namespace {
 
+// Words up to which a row has 256 threads in the first kernel.
+constexpr int64_t kSmallVocab = 8192;
+
+// Whether rows may be left: they may have more words than fit the list.
+bool may_leave(int64_t vocab) {
+  return vocab >
+         (vocab <= kSmallVocab ? mhs::ListShared<256>::kList : mhs::ListShared<1024>::kList);
+}
+
 // Whether some row may be looked at by parts: it has more words than a part, and top-k may be off.
 bool in_parts(const void* top_k, int64_t top_k_value, int64_t vocab) {
   return vocab > mhs::kPart && (top_k || top_k_value < 1 || top_k_value >= vocab);
@@ -19,19 +28,12 @@ int64_t part_count(int64_t vocab) { return (vocab + mhs::kPart - 1) / mhs::kPart
 template <class T>
 int launch(const mhs::SampleArgs& a, int64_t rows, bool parts, hipStream_t s) {
   const unsigned grid = (unsigned)rows;
-  if (a.vocab <= mhs::kAllWords) {   // all words fit the first kernel's list
-    mhs::sample_kernel<T, mhs::SampleShared<256, mhs::kAllWords>, false><<<grid, 256, 0, s>>>(a);
-    return check_launch("sample kernel");
-  }
-  mhs::sample_kernel<T, mhs::SampleShared<1024, mhs::kFirstList>, true><<<grid, 1024, 0, s>>>(a);
+  if (a.vocab <= kSmallVocab) mhs::sample_kernel<T, 256><<<grid, 256, 0, s>>>(a);
+  else mhs::sample_kernel<T, 1024><<<grid, 1024, 0, s>>>(a);
   const int rc = check_launch("sample kernel");
-  if (rc) return rc;
-  if (parts) {
-    const dim3 all((unsigned)a.parts, grid);
-    mhs::sample_bins_kernel<T><<<all, 256, 0, s>>>(a);
-    mhs::sample_border_kernel<T><<<all, 256, 0, s>>>(a);
-  }
-  mhs::sample_finish_kernel<T><<<grid, 1024, 0, s>>>(a);
+  if (rc || !a.state) return rc;
+  if (parts) mhs::sample_bins_kernel<T><<<dim3((unsigned)a.parts, grid), 256, 0, s>>>(a);
+  mhs::sample_rest_kernel<T><<<grid, 1024, 0, s>>>(a);
   return check_launch("sample kernels of the rows left");
 }
 
@@ -52,7 +54,7 @@ extern "C" {
 size_t mhs_sample_workspace_bytes(int64_t rows, int64_t vocab, int top_k_array,
                                   int64_t top_k_value) {
   mhs::clear_error();
-  if (check_sizes(rows, vocab) || vocab <= mhs::kAllWords) return 0;
+  if (check_sizes(rows, vocab) || !may_leave(vocab)) return 0;
   const int64_t parts =
       in_parts(top_k_array ? &rows : nullptr, top_k_value, vocab) ? part_count(vocab) : 0;
   return mhs::round_up((size_t)rows * sizeof(mhs::SampleRow), 256) +
@@ -85,7 +87,8 @@ int mhs_sample(int dtype, const void* logits, int64_t ld, const float* uniform,
   mhs::SampleArgs a{logits, ld, uniform, temperature, top_p, min_p, top_k, top_k64,
                     temperature_value, top_p_value, min_p_value, (long long)top_k_value,
                     reinterpret_cast<long long*>(tokens), logprobs, (int)vocab,
-                    words <= 17 ? 45 : 62 - words, static_cast<mhs::SampleRow*>(workspace),
+                    words <= 17 ? 45 : 62 - words,
+                    need ? static_cast<mhs::SampleRow*>(workspace) : nullptr,
                     reinterpret_cast<unsigned long long*>(
                         static_cast<char*>(workspace) +
                         mhs::round_up((size_t)rows * sizeof(mhs::SampleRow), 256)),
