@@ -78,10 +78,6 @@ def _seqs(what: str, cu: torch.Tensor) -> int:
     return cu.numel() - 1
 
 
-def _no_state(x: torch.Tensor) -> torch.Tensor:
-    return x.new_empty((0,))
-
-
 # ----------------------------------------------------------------- the scan
 
 def _scan_ok(x, dt, aneg, b_in, c_in, cu, h0) -> bool:
@@ -135,7 +131,8 @@ def _packed_scan_fwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
             DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
             _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
             c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64,
-            _ptr(h0), y.data_ptr(), h_last.data_ptr() if want_state else None, ckpt.data_ptr() if with_ckpt else None,
+            _ptr(h0), y.data_ptr(), h_last.data_ptr() if want_state else None,
+            ckpt.data_ptr() if with_ckpt else None,
             seqs, rows, d, n, _ptr(ws), nbytes, _stream(dev))
     _check(rc, "mhs_packed_scan_fwd")
     return y, h_last, ckpt
@@ -177,7 +174,8 @@ def _packed_scan_bwd_impl(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
             DTYPES[x.dtype], x.data_ptr(), _ld(x, rows, d), dt.data_ptr(),
             _ld(dt, rows, d), aneg.data_ptr(), b_in.data_ptr(), _ld(b_in, rows, n),
             c_in.data_ptr(), _ld(c_in, rows, n), cu.data_ptr(), cu.dtype == torch.int64,
-            _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy, rows, d), _ptr(dh_last), dx.data_ptr(), ddt.data_ptr(), da.data_ptr(), db.data_ptr(),
+            _ptr(h0), ckpt.data_ptr(), dy.data_ptr(), _ld(dy, rows, d), _ptr(dh_last),
+            dx.data_ptr(), ddt.data_ptr(), da.data_ptr(), db.data_ptr(),
             dc.data_ptr(), dh0.data_ptr() if h0 is not None else None, seqs, rows, d, n, _ptr(ws),
             nbytes, _stream(dev))
     _check(rc, "mhs_packed_scan_bwd")

@@ -59,6 +59,14 @@ int check_workspace(const void* ws, size_t have, size_t need) {
   return MHS_OK;
 }
 
+// f(a value of the type that dtype names).
+template <class F>
+auto by_type(int dtype, F&& f) {
+  if (dtype == MHS_F32) return f(mhs::F32{});
+  if (dtype == MHS_BF16) return f(mhs::Bf16{});
+  return f(mhs::Fp16{});
+}
+
 mhs::Seqs seqs(const void* cu, int cu64, int64_t nseq, int64_t total) {
   return {cu, cu64, (int)nseq, (int)total};
 }
@@ -132,21 +140,19 @@ size_t scan_parts(void* ws, const ScanPlan& p, int64_t total, int64_t dim, int64
 
 int run_scan_t(int dtype, bool back, const mhs::PackedScanArgs& a, const ScanPlan& p,
                hipStream_t s) {
-  if (dtype == MHS_F32) return mhs::run_packed_scan<mhs::F32>(back, a, p, s);
-  if (dtype == MHS_BF16) return mhs::run_packed_scan<mhs::Bf16>(back, a, p, s);
-  return mhs::run_packed_scan<mhs::Fp16>(back, a, p, s);
+  return by_type(dtype, [&](auto t) { return mhs::run_packed_scan<decltype(t)>(back, a, p, s); });
 }
 
 // --------------------------------------------------------- the convolution
 
-// Channels of a thread: a 16-byte access where width, strides and addresses allow it.
-int conv_vec(int dtype, int64_t dim, std::initializer_list<const void*> ps,
-             std::initializer_list<int64_t> lds) {
-  const int v = 16 / elem(dtype);
+// Whether a thread may have several channels: width, strides and addresses allow it.
+bool conv_wide(int dtype, bool back, int64_t dim, std::initializer_list<const void*> ps,
+               std::initializer_list<int64_t> lds) {
+  const int v = back ? mhs::kConvBackVec : 8 / elem(dtype);
   bool ok = dim % v == 0;
   for (const void* p : ps) ok = ok && aligned16(p);
   for (const int64_t ld : lds) ok = ok && ld % v == 0;
-  return ok ? v : 1;
+  return ok;
 }
 using mhs::kConvBackPiece;
 using mhs::kConvPiece;
@@ -173,28 +179,27 @@ int run_conv(bool back, const mhs::PackedConvArgs& a, hipStream_t s) {
   return check_launch("packed conv kernel");
 }
 template <class T, int K>
-int run_conv_v(int vec, bool back, const mhs::PackedConvArgs& a, hipStream_t s) {
-  return vec == 1 ? run_conv<T, K, 1>(back, a, s)
-                  : run_conv<T, K, 16 / mhs::kElem<T>>(back, a, s);
+int run_conv_v(bool wide, bool back, const mhs::PackedConvArgs& a, hipStream_t s) {
+  if (!wide) return run_conv<T, K, 1>(back, a, s);
+  return back ? run_conv<T, K, mhs::kConvBackVec>(true, a, s)
+              : run_conv<T, K, mhs::kConvVec<T>>(false, a, s);
 }
 template <class T>
-int run_conv_k(int64_t taps, int vec, bool back, const mhs::PackedConvArgs& a, hipStream_t s) {
+int run_conv_k(int64_t taps, bool wide, bool back, const mhs::PackedConvArgs& a, hipStream_t s) {
   switch (taps) {
-    case 1: return run_conv_v<T, 1>(vec, back, a, s);
-    case 2: return run_conv_v<T, 2>(vec, back, a, s);
-    case 3: return run_conv_v<T, 3>(vec, back, a, s);
-    case 4: return run_conv_v<T, 4>(vec, back, a, s);
-    case 5: return run_conv_v<T, 5>(vec, back, a, s);
-    case 6: return run_conv_v<T, 6>(vec, back, a, s);
-    case 7: return run_conv_v<T, 7>(vec, back, a, s);
-    default: return run_conv_v<T, 8>(vec, back, a, s);
+    case 1: return run_conv_v<T, 1>(wide, back, a, s);
+    case 2: return run_conv_v<T, 2>(wide, back, a, s);
+    case 3: return run_conv_v<T, 3>(wide, back, a, s);
+    case 4: return run_conv_v<T, 4>(wide, back, a, s);
+    case 5: return run_conv_v<T, 5>(wide, back, a, s);
+    case 6: return run_conv_v<T, 6>(wide, back, a, s);
+    case 7: return run_conv_v<T, 7>(wide, back, a, s);
+    default: return run_conv_v<T, 8>(wide, back, a, s);
   }
 }
-int run_conv_t(int dtype, int64_t taps, int vec, bool back, const mhs::PackedConvArgs& a,
+int run_conv_t(int dtype, int64_t taps, bool wide, bool back, const mhs::PackedConvArgs& a,
                hipStream_t s) {
-  if (dtype == MHS_F32) return run_conv_k<mhs::F32>(taps, vec, back, a, s);
-  if (dtype == MHS_BF16) return run_conv_k<mhs::Bf16>(taps, vec, back, a, s);
-  return run_conv_k<mhs::Fp16>(taps, vec, back, a, s);
+  return by_type(dtype, [&](auto t) { return run_conv_k<decltype(t)>(taps, wide, back, a, s); });
 }
 
 // ------------------------------------------------------------------ tokens
@@ -328,16 +333,15 @@ int mhs_packed_scan_bwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
   if (sums) {
     const unsigned grid = (unsigned)((sums + 255) / 256);
     const int nblk = (int)p.blocks;
-    if (dtype == MHS_F32)
-      mhs::packed_sum_bc_kernel<mhs::F32><<<grid, 256, 0, s>>>(a.part_bc, dB, dC, nblk, total, a.N);
-    else if (dtype == MHS_BF16)
-      mhs::packed_sum_bc_kernel<mhs::Bf16><<<grid, 256, 0, s>>>(a.part_bc, dB, dC, nblk, total, a.N);
-    else
-      mhs::packed_sum_bc_kernel<mhs::Fp16><<<grid, 256, 0, s>>>(a.part_bc, dB, dC, nblk, total, a.N);
+    by_type(dtype, [&](auto t) {
+      mhs::packed_sum_bc_kernel<decltype(t)><<<grid, 256, 0, s>>>(a.part_bc, dB, dC, nblk, total,
+                                                                  a.N);
+    });
     if ((rc = check_launch("packed scan dB / dC sums"))) return rc;
   }
   const int slice = a.D * a.N;
-  mhs::packed_sum_a_kernel<<<(slice + 63) / 64, 1024, 0, s>>>(a.part_a, daneg, (int)p.pieces, slice);
+  mhs::packed_sum_a_kernel<<<(slice + 63) / 64, 1024, 0, s>>>(a.part_a, daneg, (int)p.pieces,
+                                                              slice);
   return check_launch("packed scan dAneg sum");
 }
 
@@ -364,8 +368,8 @@ int mhs_packed_conv_fwd(int dtype, const void* x, int64_t ld_x, const void* weig
   a.x = x; a.ld_x = ld_x; a.w = weight; a.bias = bias; a.wf32 = weight_f32;
   a.window = window; a.out = out; a.window_out = window_out;
   a.D = (int)dim;
-  return run_conv_t(dtype, taps, conv_vec(dtype, dim, {x, out, weight, bias}, {ld_x}), false, a,
-                    static_cast<hipStream_t>(stream));
+  const bool wide = conv_wide(dtype, false, dim, {x, out, weight, bias}, {ld_x});
+  return run_conv_t(dtype, taps, wide, false, a, static_cast<hipStream_t>(stream));
 }
 
 int mhs_packed_conv_bwd(int dtype, const void* x, int64_t ld_x, const void* weight,
@@ -390,17 +394,16 @@ int mhs_packed_conv_bwd(int dtype, const void* x, int64_t ld_x, const void* weig
   a.dx = dx; a.dwindow = dwindow; a.part = static_cast<float*>(workspace);
   a.D = (int)dim;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  rc = run_conv_t(dtype, taps, conv_vec(dtype, dim, {x, dout, dx, weight, bias}, {ld_x, ld_dout}), true, a, s);
+  const bool wide = conv_wide(dtype, true, dim, {x, dout, dx, weight, bias}, {ld_x, ld_dout});
+  rc = run_conv_t(dtype, taps, wide, true, a, s);
   if (rc) return rc;
   const int n = (int)((piece_count(total, nseq, kConvBackPiece) + 3) / 4);
   const dim3 grid((unsigned)((dim + 63) / 64), (unsigned)(taps + 1));
   const int k = (int)taps;
-  if (dtype == MHS_F32)
-    mhs::packed_conv_sum_kernel<mhs::F32><<<grid, 1024, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
-  else if (dtype == MHS_BF16)
-    mhs::packed_conv_sum_kernel<mhs::Bf16><<<grid, 1024, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
-  else
-    mhs::packed_conv_sum_kernel<mhs::Fp16><<<grid, 1024, 0, s>>>(a.part, dweight, dbias, weight_f32, n, k, a.D);
+  by_type(dtype, [&](auto t) {
+    mhs::packed_conv_sum_kernel<decltype(t)><<<grid, 1024, 0, s>>>(a.part, dweight, dbias,
+                                                                   weight_f32, n, k, a.D);
+  });
   return check_launch("packed conv weight gradient sum");
 }
 

@@ -36,19 +36,23 @@ struct PackedConvArgs {
   float* part;          // (block rows, K + 1, D): dw, dbias
 };
 
-// V neighbouring elements of T (16 bytes, aligned, or one) as they lie in memory.
+// V neighbouring elements of T (4, 8 or 16 bytes, aligned, or one) as they lie in memory.
 template <class T, int V>
 struct Chans {
-  uint4 r;
+  static constexpr int kWords = V == 1 ? 1 : V * kElem<T> / 4;
+  struct alignas(4 * kWords) Words { unsigned u[kWords]; };
+  Words r;
   __device__ __forceinline__ void load(const void* p, size_t idx) {
-    if constexpr (V == 1) r.x = __float_as_uint(ld_p<T>(p, idx));
-    else r = *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + idx * kElem<T>);
+    if constexpr (V == 1) r.u[0] = __float_as_uint(ld_p<T>(p, idx));
+    else r = *reinterpret_cast<const Words*>(static_cast<const char*>(p) + idx * kElem<T>);
   }
-  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r.u[i] = 0;
+  }
   __device__ __forceinline__ float get(int i) const {
-    const unsigned u[4] = {r.x, r.y, r.z, r.w};
-    if constexpr (V == 1 || kElem<T> == 4) return __uint_as_float(u[i]);
-    else return T::to((unsigned short)(u[i / 2] >> (16 * (i & 1))));
+    if constexpr (V == 1 || kElem<T> == 4) return __uint_as_float(r.u[i]);
+    else return T::to((unsigned short)(r.u[i / 2] >> (16 * (i & 1))));
   }
   __device__ __forceinline__ void get(float (&v)[V]) const {
 #pragma unroll
@@ -60,21 +64,20 @@ __device__ __forceinline__ void store_chans(void* p, size_t idx, const float (&v
   if constexpr (V == 1) {
     st_p<T>(p, idx, v[0]);
   } else {
-    unsigned u[4] = {0, 0, 0, 0};
+    typename Chans<T, V>::Words r;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if constexpr (kElem<T> == 4) u[i] = __float_as_uint(v[i]);
-      else u[i / 2] |= (unsigned)T::from(v[i]) << (16 * (i & 1));
+      if constexpr (kElem<T> == 4) r.u[i] = __float_as_uint(v[i]);
+      else if (i % 2) r.u[i / 2] |= (unsigned)T::from(v[i]) << 16;
+      else r.u[i / 2] = (unsigned)T::from(v[i]);
     }
-    *reinterpret_cast<uint4*>(static_cast<char*>(p) + idx * kElem<T>) =
-        make_uint4(u[0], u[1], u[2], u[3]);
+    *reinterpret_cast<typename Chans<T, V>::Words*>(static_cast<char*>(p) + idx * kElem<T>) = r;
   }
 }
-// N elements of TW from idx on; VEC: the address and N allow 16-byte accesses.
-template <class TW, int N, bool VEC>
+// N elements of TW from idx on, which W divides; the address is that of whole W's.
+template <class TW, int N, int W>
 __device__ __forceinline__ void load_run(float (&v)[N], const void* p, size_t idx) {
-  constexpr int W = 16 / kElem<TW>;
-  if constexpr (VEC && N % W == 0) {
+  if constexpr (W > 1) {
 #pragma unroll
     for (int i = 0; i < N; i += W) {
       Chans<TW, W> c;
@@ -94,8 +97,9 @@ struct ConvLane {
   template <class TW>
   __device__ __forceinline__ void load(const PackedConvArgs& a, int d) {
     float all[V * K];   // (D, K): a channel's taps are neighbours
-    load_run<TW, V * K, (V > 1)>(all, a.w, (size_t)d * K);
-    load_run<TW, V, (V > 1)>(bias, a.bias, d);
+    constexpr int W = V < 16 / kElem<TW> ? V : 16 / kElem<TW>;
+    load_run<TW, V * K, W>(all, a.w, (size_t)d * K);
+    load_run<TW, V, W>(bias, a.bias, d);
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -133,10 +137,18 @@ __device__ __forceinline__ void conv_input(float (&v)[V], const PackedConvArgs& 
 }
 
 // Rows of a piece, and those of them whose loads are in flight together.
-constexpr int kConvPiece = 16, kConvBackPiece = 32, kConvBackRows = 4;
+constexpr int kConvPiece = 16, kConvBackPiece = 16, kConvBackRows = 4;
+// Channels of a thread where the layout allows it. (us of 8192 x 1536 in bf16 | fp32 |
+// 32768 x 2048 in bf16. Forward with 16 bytes a thread 17.7 | 22.2 | 55.2, with 8 17.5 | 20.6 |
+// 55.6, with 4 16.2 | 22.6 | 60.7. Backward, pieces of 32 rows, with 16 bytes 38.2 | 36.5 | 123.6,
+// its registers leaving two waves a SIMD and the rows too few of those, with 8 29.9 | 34.0 | 105.0,
+// with 4 27.9 | 34.6 | 97.8; so two channels, and in pieces of 16 rows 25.4 | 36.7 | 97.4.)
+template <class T> constexpr int kConvVec = 8 / kElem<T>;
+constexpr int kConvBackVec = 2;
 
 // Block (pieces / 4, channels / (64 V)): 64 channel lanes by 4 pieces, so that a wave has one
-// piece; all its rows are asked for at once (8192 x 1536 bf16: 24 us four at a time).
+// piece; all its rows are asked for at once (8192 x 1536 bf16: 17.5 us, 2.9 TB/s;
+// 24 us four at a time).
 template <class T, int K, int V>
 __global__ void __launch_bounds__(256)
 packed_conv_fwd_kernel(PackedConvArgs a, int pieces) {
@@ -309,20 +321,25 @@ packed_conv_bwd_kernel(PackedConvArgs a, int pieces) {
 }
 
 // dw (D, K), dbias (D): the blocks' partials (n, K + 1, D). A wave's lanes are
-// channels; each of a block's 16 waves adds every sixteenth partial.
+// channels; each of a block's 16 waves adds every sixteenth partial, in four sums.
 template <class T>
 __global__ void __launch_bounds__(1024)
 packed_conv_sum_kernel(const float* part, void* dw, void* dbias, int wf32, int n, int K, int D) {
   __shared__ float sums[16][64];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int d = blockIdx.x * 64 + lane, k = blockIdx.y;
-  float s = 0.f;
-  if (d < D)
-    for (int p = w; p < n; p += 16) s += part[((size_t)p * (K + 1) + k) * D + d];
-  sums[w][lane] = s;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  if (d < D) {
+    for (int p = w; p < n; p += 64) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (p + 16 * j < n) t[j] += part[((size_t)(p + 16 * j) * (K + 1) + k) * D + d];
+    }
+  }
+  sums[w][lane] = (t[0] + t[1]) + (t[2] + t[3]);
   __syncthreads();
   if (w || d >= D) return;
-  s = sums[0][lane];
+  float s = sums[0][lane];
 #pragma unroll
   for (int i = 1; i < 16; ++i) s += sums[i][lane];
   void* to = k < K ? dw : dbias;

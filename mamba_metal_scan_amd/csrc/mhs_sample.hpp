@@ -188,8 +188,8 @@ __device__ __forceinline__ void vector_words(const uint4& r, int b, F&& f) {
   }
 }
 
-// f(i, word i) for the words lo .. lo + n - 1, each once, by `threads` threads (this one is number t):
-// 16 bytes at a time but for the ends, four such loads in flight.
+// f(i, word i) for the words lo .. lo + n - 1, each once, by `threads` threads (this one is
+// number t): 16 bytes at a time but for the ends, four such loads in flight.
 template <class T, class F>
 __device__ __forceinline__ void for_words(const char* row, int lo, int n, int t, int threads,
                                           F&& f) {
