@@ -142,13 +142,13 @@ def test_sample_arguments():
                      (dict(tokens=None), "null"), (dict(ld=999), "apart"),
                      (dict(rows=1 << 16), "rows"), (dict(vocab=0), "vocab"),
                      (dict(vocab=(1 << 24) + 1, ld=1 << 25), "vocab"),
-                     (dict(vocab=2000, ld=2000, ws=None), "workspace"),
-                     (dict(vocab=2000, ld=2000, nbytes=8), "workspace"),
-                     (dict(vocab=2000, ld=2000, ws=MIS), "256")):
+                     (dict(vocab=5000, ld=5000, ws=None), "workspace"),
+                     (dict(vocab=5000, ld=5000, nbytes=8), "workspace"),
+                     (dict(vocab=5000, ld=5000, ws=MIS), "256")):
         assert call(**kw) == 1 and text in _err(), (kw, _err())
     assert call(rows=0) == 0
     size = lib.mhs_sample_workspace_bytes
-    assert size(4, 1000, 1, 0) == 0                      # all words fit one list
+    assert size(4, 4096, 1, 0) == 0                      # all words fit one list
     assert 0 < size(4, 100000, 0, 50) < size(4, 100000, 1, 0) == size(4, 100000, 0, 0)
 
 
