@@ -252,8 +252,8 @@ def resource_usage(verbose: bool = False) -> dict:
 
 # The kernels of the benchmarked workloads (d_state 16: NPL 2, G 4; beside
 # them the one-state-per-lane plan NPL 1, G 8 and the four-state plans of
-# d_state 32 and 64), the products, the token's and the loss's, with what each
-# one is.
+# d_state 32 and 64), the products, the token's and the loss's, the packed sequences'
+# and the sampling's, with what each one is.
 AUDIT = [
     ("fwd_kernel<2, 4, 3, true, false, 0, 4>", "forward, checkpoint stride a multiple of 16",
      "fwd", 4, 2),
@@ -321,6 +321,20 @@ AUDIT = [
     ("head_small_kernel<Fp32, 2>", "the same, fp32, 17 to 32 rows", "bytes", 4, 33792),
     ("distill_fwd_kernel<Fp32>", "distillation of logits, forward", None, 4, 0),
     ("distill_bwd_kernel<Fp32>", "distillation of logits, backward", None, 4, 0),
+    ("packed_scan_fwd_kernel<Bf16, 4, 1, true, true, false>", "packed forward, carry pass",
+     "bytes", 4, 24576),
+    ("packed_scan_fwd_kernel<Bf16, 4, 1, true, false, true>", "packed forward with checkpoints",
+     "bytes", 4, 28672),
+    ("packed_scan_back_carry_kernel<Bf16, 4, 1, true>", "packed backward, carry pass", "bytes",
+     4, 24576),
+    ("packed_scan_bwd_kernel<Bf16, 4, 1, true>", "packed backward", "bytes", 4, 14336),
+    ("packed_conv_fwd_kernel<Bf16, 4, 4>", "packed conv, four taps", None, 4, 0),
+    ("packed_conv_bwd_kernel<Bf16, 4, 2>", "packed conv backward", "bytes", 4, 2048),
+    ("conv_step_kernel<Bf16, 4>", "conv of a token by slot", None, 4, 0),
+    ("state_step_kernel<Bf16, 4, 4>", "state of a token by slot", None, 4, 0),
+    ("sample_kernel<Bf16, 1024>", "sampling: maxima and lists", "bytes", 16, 40712),
+    ("sample_bins_kernel<Bf16>", "sampling: weights by bins", "bytes", 4, 32768),
+    ("sample_rest_kernel<Bf16>", "sampling: rows of many kept words", "bytes", 16, 50968),
 ]
 
 

@@ -202,7 +202,8 @@ packed_conv_fwd_kernel(PackedConvArgs a, int pieces) {
 // and, for the inputs that window_out holds, its gradient. A thread walks the
 // rows of its piece and the K - 1 behind it, keeping K of s; a block's four pieces
 // are summed in LDS for dw and dbias, the blocks by packed_conv_sum_kernel, always in
-// the same order.
+// the same order. (8192 x 1536 bf16: 24.5 us, 3.1 TB/s; 32768 x 2048 97 us, 4.1 TB/s: then the
+// copy's rate nearly, before that the launch's first loads and the sums at its end.)
 template <class T, int K, int V>
 __global__ void __launch_bounds__(256)
 packed_conv_bwd_kernel(PackedConvArgs a, int pieces) {
@@ -388,7 +389,9 @@ struct ConvStepArgs {
   int rows, pool, D;
 };
 
-// Block (row, channels).
+// Block (row, channels), a channel a thread: its taps, its window and two numbers are all there
+// is, a few scattered elements each. Bound by launch and latency: 4 x 1536 in fp32 3.0 us, 256 x
+// 4096 in bf16 9.1 us (1.8 TB/s), as long as the host takes for the call.
 template <class T, int K>
 __global__ void __launch_bounds__(256)
 conv_step_kernel(ConvStepArgs a) {
@@ -431,7 +434,8 @@ struct StateStepArgs {
 
 // h <- exp(-dt Aneg) h + dt x B, y = sum_n C h. Block (row, channels). LPC lanes
 // share a channel, V neighbouring states each (V 4: whole float4s; V 1: any N); y is summed over
-// them by DPP. Memory-bound: h is read and written once.
+// them by DPP. Memory-bound: h is read and written once (256 x 4096 x 16 in bf16, 141 MB:
+// 34 us, 4.1 TB/s; 27 us where it is cached; 4 x 1536 x 16 in fp32 3.3 us, latency).
 template <class T, int V, int LPC>
 __global__ void __launch_bounds__(256)
 state_step_kernel(StateStepArgs a) {

@@ -297,6 +297,11 @@ __device__ __forceinline__ void store_sdt(const PackedScanArgs& a, int q, int d,
 }
 
 // ----------------------------------------------------------------- forward
+//
+// CARRY: the carry pass, else the main one. All is branch-free buffer accesses, what is not
+// there lying past the buffer: a branch within the loop made the compiler wait for all loads
+// in flight (twice the time). 32768 x 2048 x 16 in bf16: 156 and 261 us, 8192 x 1536 x 16 in fp32
+// 43 and 68 us, of 129 and 162, 24 and 30 that the vector units need for the formula alone.
 
 template <class T, int NPL, int WS, bool VEC, bool CARRY, bool CKPT>
 __global__ void __launch_bounds__(256)
@@ -425,7 +430,9 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
 }
 
 // carry and sdt -> start of the pieces 1 .. of each sequence of several; with BACK
-// of the pieces .. n - 2, from the last (dh_last) down. Block (s, channels x states).
+// of the pieces .. n - 2, from the last (dh_last) down. Block (s, channels x states). Bound by the
+// states' bytes, read and written once, and by the chain of a sequence's pieces, eight of
+// which are loaded at once (8192 x 1536 x 16 fp32 in pieces of 32 rows, 54 MB: 15 us).
 template <bool BACK>
 __global__ void __launch_bounds__(256)
 packed_fold_kernel(PackedScanArgs a) {
@@ -472,7 +479,8 @@ packed_fold_kernel(PackedScanArgs a) {
 // so that each lane ends with one of them, in LDS over the block's waves, and over the
 // blocks in packed_sum_bc_kernel: always in the same order.
 // (Checkpoints every 8 rows rather than 16: what the sums over the channels cost falls with
-// the channels a lane holds, and registers hold 8 rows of two.)
+// the channels a lane holds, and registers hold 8 rows of two.) 32768 x 2048 x 16 in bf16: 169
+// (carry) and 632 us, 8192 x 1536 x 16 in fp32 39 and 144 us.
 
 // The adjoint's carry pass: each piece but the first from a zero adjoint.
 template <class T, int NPL, int WS, bool VEC>

@@ -5,7 +5,8 @@
 
 namespace mhs {
 
-// dB, dC (total, N): the blocks' partials in order, rounded to T once.
+// dB, dC (total, N): the blocks' partials in order, rounded to T once. Bound by the partials' bytes
+// (16 blocks of 32768 x 16 x 2: 67 MB, 19.5 us; 12 of 8192: 12.6 MB, 6.5 us).
 template <class T>
 __global__ void __launch_bounds__(256)
 packed_sum_bc_kernel(const float* part, void* dB, void* dC, int nblk, long long rows, int N) {

@@ -905,7 +905,12 @@ __device__ __forceinline__ u64 search_border(Sh& sh, const RowOf<T>& R) {
   return place_of(edge, last);
 }
 
-// The first kernel: rows of up to kList words, and those whose kept words fit the list.
+// The first kernel: rows of up to kList words, and those whose kept words fit the list. us: 4 x
+// 32768 in fp32, top-k 50 and top-p 0.9, 11, of which the maxima 1.8, the bound 2.6, the list
+// 1.8, its draw 2.1, the rest the launch and the settings; 256 x 131072 in bf16 the same 18 (the
+// maxima 9 to 12: the words at 6 to 7 TB/s), and with k up to 1000 in some rows 39 (their
+// bound 6, list 10, descents 13). Loads: eight in flight; all 16 with the words kept in
+// registers for the second pass took 14 us for the maxima, and spilled.
 template <class T, int NTH>
 __global__ void __launch_bounds__(NTH)
 sample_kernel(SampleArgs a) {
@@ -1010,6 +1015,8 @@ sample_kernel(SampleArgs a) {
   list.draw(least);
 }
 
+// Bound by the weights' arithmetic, some 50 instructions a word, most in 64 bits, and by the
+// adds to LDS: 256 x 131072 words 58 us, a third of those rows 18 us.
 // Of the rows left those that no k or +inf leaves to the search: part blockIdx.x of row
 // blockIdx.y, its weights by bin, to the part's and to the row's; without top-p their sum.
 template <class T>
@@ -1043,7 +1050,8 @@ sample_bins_kernel(SampleArgs a) {
   }
 }
 
-// The rows left.
+// The rows left. Bound by its steps' latencies (us, 4 x 131072 words: the border's bin 2.3, its
+// words 8 to 9, their cut 2.3 or, of more than 256 words, 5.8, the parts' sums 3.3, the word 6.5).
 template <class T>
 __global__ void __launch_bounds__(1024)
 sample_rest_kernel(SampleArgs a) {
