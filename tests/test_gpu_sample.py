@@ -169,3 +169,47 @@ def test_middle_vocabularies():
         k = torch.tensor([0, 0, 0, 5, 900, 1500, 0, vocab])
         check(z, u, top_k=k, top_p=torch.tensor([1.0, 0.9, 0.2, 0.9, 0.9, 0.8, 1.0, 0.99]),
               min_p=torch.tensor([0.0, 0.0, 0.1, 0.0, 0.0, 0.0, 0.01, 0.0]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_words_past_the_threads_maxima(dtype):
+    """More than 16 vectors a thread; rows that start at any element; k at the bound's limits."""
+    z, u = _rand(3, 140003, dtype, 21)
+    for s in (dict(top_k=50, top_p=0.9), dict(top_k=2048, temperature=0.7),
+              dict(top_k=2049, top_p=0.9), dict(top_p=0.9, min_p=0.001), dict(temperature=0.0)):
+        check(z[:, 1:], u, **s)
+    check(z[:1, 3:70000], u[:1], top_k=1000, top_p=0.95)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_words_in_order_and_few_words_left(dtype):
+    """The likeliest words next to each other; masks that leave 1 and 30 words; one level."""
+    up = torch.linspace(-8, 8, 20011).to(dtype)
+    left = torch.full((20011,), -INF, dtype=dtype)
+    left[7::667] = torch.randn(30, generator=torch.Generator().manual_seed(2)).to(dtype)
+    one = torch.full((20011,), torch.finfo(dtype).min, dtype=dtype)
+    one[20010] = 1.0
+    low = torch.full((20011,), torch.finfo(dtype).min, dtype=dtype)
+    z = torch.stack([up, up.flip(0), left, one, low])
+    u = torch.tensor([0.1, 0.4, 0.9, 0.5, 0.77])
+    for s in (dict(top_k=50), dict(top_k=1000, top_p=0.9), dict(top_k=20), dict(top_p=0.9), dict(),
+              dict(min_p=0.02), dict(top_p=0.5, min_p=0.7), dict(temperature=0.0)):
+        check(z, u, **s)
+
+
+@pytest.mark.parametrize("vocab", [4097, 20000])
+def test_top_p_and_min_p_at_the_bins(vocab):
+    """min-p within, at the end of, before and behind the bin of top-p's border, by row."""
+    z, u = _rand(12, vocab, F32, vocab)
+    low = torch.tensor([0.5, 0.25, 0.3, 2.0 ** -0.0625, 0.001, 1e-9, 1e-30, 0.9, 1.0, 0.01, 0.07,
+                        0.0])
+    for p in (0.05, 0.5, 0.95, 0.9999):
+        check(z, u, top_p=p, min_p=low, temperature=0.9)
+    spread = (z * 0.02).clone()   # thousands of words a bin
+    check(spread, u, top_p=0.6, min_p=low)
+
+
+def test_a_very_large_vocabulary():
+    """More than 256 parts: the draw goes through the row."""
+    z, u = _rand(1, 2 ** 21 + 8195, F16, 3)
+    check(z, u, top_p=0.8)
