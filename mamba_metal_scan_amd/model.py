@@ -376,12 +376,11 @@ class MambaBlock(nn.Module):
         y = y + self.D_skip
         return self.out_proj(y * F.silu(z))
 
-
     def mix_packed(self, h, cu_seqlens, cache=None):
         """mix() of packed sequences: h (L, d_model), cu_seqlens as conv1d_silu_packed
         takes them. With a cache every sequence goes on from its window and state there
         (from nothing if the cache is empty), and leaves those behind its last token. On
-        the HIP path only."""
+        the HIP path only; the conv is read as weights (hooks of its module do not run)."""
         x, z = self._linear(self.in_proj, h).chunk(2, dim=-1)            # (L, d_inner)
         before = cache if cache else {}
         keep = cache is not None
@@ -495,7 +494,8 @@ class TinyMamba(nn.Module):
         ends = cu_seqlens[1:].long()
         if idx.shape[0] == 0:
             return h.new_full((ends.shape[0], self.cfg.vocab_size), float("nan"))
-        logits = linear(self.head, h[(ends - 1).clamp(min=0)])
+        # (an end past the tokens does not index past them)
+        logits = linear(self.head, h[(ends - 1).clamp(min=0, max=idx.shape[0] - 1)])
         return logits.masked_fill((ends <= cu_seqlens[:-1]).unsqueeze(1), float("nan"))
 
     @torch.no_grad()

@@ -211,3 +211,13 @@ def test_requests_that_come_and_go():
     assert torch.isnan(windows[[1, 3]]).all() and torch.isnan(states[[1, 3]]).all()
     logits = F.linear(torch.randn(4, d, generator=g, device="cuda"), randn(100, d))
     assert sample_tokens(logits, torch.rand(4, device="cuda"), top_k=10).shape == (4,)
+
+
+def test_prefill_of_an_end_past_the_tokens():
+    """Lengths that the documentation does not allow: no access past the tokens."""
+    model = _model()
+    idx, _, _ = _prompts([6])
+    with torch.no_grad():
+        out = model.prefill(idx, torch.tensor([0, 4, 99], device="cuda"), {})
+        want = model.prefill(idx, torch.tensor([0, 4, 6], device="cuda"), {})
+    assert torch.equal(out, want)
