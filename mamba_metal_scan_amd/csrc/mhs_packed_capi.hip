@@ -79,13 +79,13 @@ int64_t piece_count(int64_t total, int64_t nseq, int tc) { return total / tc + n
 // length even out). Pieces of 32 rows | 64 | 128 | 176, us: 8192 x 1536 x 16 in fp32, where this
 // gives 32 and 48, the forward's launches 125 | 122 | 151 | 165, the backward's 218 | 210 | 238 |
 // 251; 32768 x 2048 x 16 in bf16, where it gives 176 and 256, 518 | 487 | 466 | 467 and 985 |
-// 903 | 878 | 875; one prompt of 509 x 640 x 16 in fp32, where it gives the least, 32,
-// 21 | 28 | 44 | 54.
+// 903 | 878 | 875; one prompt of 509 x 640 x 16 in fp32, where it gives the least, 16:
+// 18, then 21 | 28 | 44 | 54.
 int scan_piece(int64_t total, int64_t dim, int64_t n, bool back) {
   const int64_t waves = (dim + 31) / 32 * mhs::scan_state_waves(n);
   const int64_t pieces = std::max<int64_t>(1, (back ? 32 : 48) * device_cus() / waves);
   const int64_t tc = total / pieces / mhs::kSub * mhs::kSub;
-  return (int)std::min<int64_t>(1024, std::max<int64_t>(32, tc));
+  return (int)std::min<int64_t>(1024, std::max<int64_t>(16, tc));
 }
 
 using mhs::ScanPlan;
