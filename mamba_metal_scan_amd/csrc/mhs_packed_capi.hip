@@ -81,7 +81,11 @@ int64_t piece_count(int64_t total, int64_t nseq, int tc) { return total / tc + n
 // 251; 32768 x 2048 x 16 in bf16, where it gives 176 and 256, 518 | 487 | 466 | 467 and 985 |
 // 903 | 878 | 875; one prompt of 509 x 640 x 16 in fp32, where it gives the least, 16:
 // 18, then 21 | 28 | 44 | 54.
+// Few rows are one piece, without carries: of 640 x 16 in fp32 at 32 | 64 | 96 rows one launch
+// takes 8.2 | 12.8 | 17.4 us and the three 13.1 | 13.3 | 13.4 (captured; a call 14.4 | 14.3 | 17.5
+// and 20), the backward in one piece 18.9 | 30.0 | 40.8, in several 20.8 | 21.1 | 21.3.
 int scan_piece(int64_t total, int64_t dim, int64_t n, bool back) {
+  if (total <= (back ? 32 : 64)) return back ? 32 : 64;
   const int64_t waves = (dim + 31) / 32 * mhs::scan_state_waves(n);
   const int64_t pieces = std::max<int64_t>(1, (back ? 32 : 48) * device_cus() / waves);
   const int64_t tc = total / pieces / mhs::kSub * mhs::kSub;

@@ -247,14 +247,8 @@ __device__ __forceinline__ void quad_fmac(float& acc, float b, float v) {
       : "+v"(acc)
       : "v"(b), "v"(v), "n"(K));
 }
-template <int M>
-__device__ __forceinline__ void quad_ready(float (&v)[2][M]) {
-  static_assert(M == 2 || M == 4, "two or four registers a channel");
-  if constexpr (M == 2)
-    asm("s_nop 1" : "+v"(v[0][0]), "+v"(v[0][1]), "+v"(v[1][0]), "+v"(v[1][1]));
-  else
-    asm("s_nop 1" : "+v"(v[0][0]), "+v"(v[0][1]), "+v"(v[0][2]), "+v"(v[0][3]), "+v"(v[1][0]),
-        "+v"(v[1][1]), "+v"(v[1][2]), "+v"(v[1][3]));
+__device__ __forceinline__ void quad_ready(float (&v)[2][2]) {
+  asm("s_nop 1" : "+v"(v[0][0]), "+v"(v[0][1]), "+v"(v[1][0]), "+v"(v[1][1]));
 }
 
 // Rows of R floats per channel of a wave in LDS, channel c of pair p in row 16 c + p: of R =

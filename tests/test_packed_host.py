@@ -75,9 +75,9 @@ def test_packed_scan_arguments():
         assert text in _err(), (kw, _err())
     lib = _native.library()
     assert lib.mhs_packed_scan_workspace_bytes(3, 100, 64, 65, 0) == 0
-    # a sequence cannot be longer than a piece of at least 32 rows: no carries
-    assert lib.mhs_packed_scan_workspace_bytes(3, 32, 64, 16, 0) == 0
-    assert lib.mhs_packed_scan_workspace_bytes(3, 33, 64, 16, 0) > 0
+    # up to 64 rows no sequence is longer than a piece: no carries
+    assert lib.mhs_packed_scan_workspace_bytes(3, 64, 64, 16, 0) == 0
+    assert lib.mhs_packed_scan_workspace_bytes(3, 65, 64, 16, 0) > 0
     assert lib.mhs_packed_ckpt_floats(100, 64, 16) == 12 * 64 * 16
 
 
