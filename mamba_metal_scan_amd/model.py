@@ -380,7 +380,7 @@ class MambaBlock(nn.Module):
         """mix() of packed sequences: h (L, d_model), cu_seqlens as conv1d_silu_packed
         takes them. With a cache every sequence goes on from its window and state there
         (from nothing if the cache is empty), and leaves those behind its last token. On
-        the HIP path only; the conv is read as weights (hooks of its module do not run)."""
+        the HIP path only; the conv is read as weights, so that it has to be a plain one."""
         x, z = self._linear(self.in_proj, h).chunk(2, dim=-1)            # (L, d_inner)
         before = cache if cache else {}
         keep = cache is not None
@@ -416,6 +416,13 @@ def _plain_block(b: nn.Module) -> bool:
     class's own methods, and neither b, its norm nor the module-global
     registries hold forward or backward hooks."""
     return _own_methods(b) and no_hooks(b) and no_hooks(b._modules["norm"])
+
+
+def _packs(b: nn.Module) -> bool:
+    """Whether b.mix_packed() of b's norm in place of b(x) skips nothing: as
+    _plain_block, but that the norm is called and the conv is not."""
+    return (_own_methods(b) and no_hooks(b) and type(b._modules["conv"]) is nn.Conv1d
+            and no_hooks(b._modules["conv"]))
 
 
 class TinyMamba(nn.Module):
@@ -474,7 +481,16 @@ class TinyMamba(nn.Module):
         return self.ln_f(x)
 
     def _hidden_packed(self, idx, cu_seqlens, caches):
-        """The final norm's output (L, d_model) for the packed tokens idx (L)."""
+        """The final norm's output (L, d_model) for the packed tokens idx (L).
+
+        A block's packed form is mix_packed(), not a call of the block, and reads the conv's
+        weights: a wrapper, a subclass, methods set on the instance and hooks of either would
+        be left out, and are refused."""
+        for i, b in enumerate(self.blocks):
+            if not _packs(b):
+                raise RuntimeError("packed sequences call neither a block nor its conv: block "
+                                   f"{i} ({type(b).__name__}) must be a MambaBlock and its conv a "
+                                   "Conv1d, without hooks or methods of their own")
         x = self.tok(idx)
         if idx.dim() != 1 or self.cfg.scan_impl == "torch" or not _hip_device(x):
             raise RuntimeError("packed sequences take tokens (L) on the HIP path; got "
