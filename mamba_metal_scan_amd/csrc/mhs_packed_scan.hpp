@@ -272,6 +272,25 @@ __device__ __forceinline__ float at4(const float4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
+// Steps behind a piece's rows, in its last sub-chunk, have dt = 0: exp2(0) keeps the state. A rate
+// that is infinite would make them NaN. The backward's products are therefore 0 wherever dt is
+// (v_mul_legacy_f32: 0 times anything; in a row of the sequence the forward gave NaN there), the
+// forward walks the rows of such a sub-chunk once more. (A select of every step is one in 24
+// of the forward's instructions; a copy of the loop for the last sub-chunk takes 35 registers,
+// in the backward spills.)
+__device__ __forceinline__ float zero_mul(float dt, float rate) {
+  float v;
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(v) : "v"(dt), "v"(rate));
+  return v;
+}
+template <int NPL>
+__device__ __forceinline__ bool endless_rate(const float (&a2)[2][NPL]) {   // in any lane
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) any |= __builtin_isinf(a2[0][j]) || __builtin_isinf(a2[1][j]);
+  return __any(any);
+}
+
 // Sums over the quad of v[s], s < 4: lane q ends with that of v[q].
 __device__ __forceinline__ float quad_gather(const float (&v)[4], int q) {
   float a[2], b[1];
@@ -354,7 +373,15 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
   };
   load(0);
   float sum_dt[2] = {0.f, 0.f};
+  float before[2][NPL];   // the states before the sub-chunk
   for (int i = 0; i < nsub; ++i) {
+    if constexpr (!CARRY) {
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        before[0][j] = h[0][j];
+        before[1][j] = h[1][j];
+      }
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -419,7 +446,24 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
     at.store(a.carry + (size_t)blockIdx.x * slice, h);
     if (L.ws == 0) store_sdt(a, L.q, L.d, L.act, sum_dt[0], sum_dt[1]);
   } else if (pc.last && a.h_last) {
-    at.store(a.h_last + (size_t)pc.seq * slice, h);
+    const int rows = pc.len % kSub;
+    if (rows && endless_rate<NPL>(a2)) {   // the last sub-chunk's rows again, without those behind
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+        float b[NPL];
+        load_vec<NPL>(b, tb + r * NS + L.q * NPL);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float dt = td[(16 * c + row) * Tile::R + r], bx = tx[(16 * c + row) * Tile::R + r];
+#pragma unroll
+          for (int j = 0; j < NPL; ++j)
+            before[c][j] = __builtin_fmaf(exp2_hw(dt * a2[c][j]), before[c][j], bx * b[j]);
+        }
+      }
+      at.store(a.h_last + (size_t)pc.seq * slice, before);
+    } else {
+      at.store(a.h_last + (size_t)pc.seq * slice, h);
+    }
   }
 }
 
@@ -539,7 +583,7 @@ packed_scan_back_carry_kernel(PackedScanArgs a) {
 #pragma unroll
           for (int j = 0; j < NPL; ++j)
             u[c][j] = __builtin_fmaf(at4(dy[c], s), cv[j], u[c][j]) *
-                      exp2_hw(at4(dt[c], s) * a2[c][j]);
+                      exp2_hw(zero_mul(at4(dt[c], s), a2[c][j]));
         }
       });
     });
@@ -671,9 +715,10 @@ packed_scan_bwd_kernel(PackedScanArgs a) {
       load_vec<NPL>(b, tb + t * NS + L.q * NPL);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        const float now = dpp_get<quad_bcast(s)>(dt[c][k]);
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-          da[t][c][j] = exp2_hw(quad_mul<s>(dt[c][k], a2[c][j]));
+          da[t][c][j] = exp2_hw(zero_mul(now, a2[c][j]));
           hs[t][c][j] = __builtin_fmaf(da[t][c][j], t ? hs[t ? t - 1 : 0][c][j] : h0[c][j],
                                        quad_mul<s>(bx[c][k], b[j]));
         }
