@@ -102,16 +102,19 @@ ScanPlan scan_plan(int64_t total, int64_t nseq, int64_t dim, int64_t n, bool bac
   return p;
 }
 
-int check_scan(int dtype, const void* cu, int64_t nseq, int64_t total, int64_t dim, int64_t n) {
+// A direction's launches are counted by its own plan: of 33 to 64 rows the backward has the shorter
+// pieces, of more the forward.
+int check_scan(int dtype, const void* cu, int64_t nseq, int64_t total, int64_t dim, int64_t n,
+               bool back) {
   int rc = check_dtype(dtype);
   if (rc) return rc;
   if ((rc = check_packed(cu, nseq, total, dim))) return rc;
   if (n < 1 || n > MHS_MAX_DSTATE)
     return fail(MHS_EINVAL, "d_state must be in [1, %d]; got %lld", MHS_MAX_DSTATE, (long long)n);
-  const ScanPlan p = scan_plan(total, nseq, dim, n, false);   // (the shorter pieces)
+  const ScanPlan p = scan_plan(total, nseq, dim, n, back);
   // (a launch counts its threads in 32 bits: the pass, the fold, the sums)
   if (p.pieces * p.blocks >= 1LL << 24 || nseq * ((dim * n + 255) / 256) >= 1LL << 24 ||
-      total * 2 * n >= 1LL << 32)
+      (total * 2 * n + 255) / 256 >= 1LL << 24)
     return fail(MHS_EINVAL, "%lld rows x %lld channels are too many", (long long)total,
                 (long long)dim);
   return MHS_OK;
@@ -270,7 +273,7 @@ int64_t mhs_packed_ckpt_floats(int64_t total, int64_t dim, int64_t d_state) {
 size_t mhs_packed_scan_workspace_bytes(int64_t nseq, int64_t total, int64_t dim, int64_t d_state,
                                        int backward) {
   mhs::clear_error();
-  if (check_scan(MHS_F32, &nseq, nseq, total, dim, d_state)) return 0;
+  if (check_scan(MHS_F32, &nseq, nseq, total, dim, d_state, backward != 0)) return 0;
   return scan_parts(nullptr, scan_plan(total, nseq, dim, d_state, backward != 0), total, dim,
                     d_state, backward != 0, nullptr);
 }
@@ -281,8 +284,9 @@ int mhs_packed_scan_fwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
                         float* h_last, float* ckpt, int64_t nseq, int64_t total, int64_t dim,
                         int64_t d_state, void* workspace, size_t workspace_bytes, void* stream) {
   mhs::clear_error();
-  int rc = check_scan(dtype, cu_seqlens, nseq, total, dim, d_state);
+  int rc = check_scan(dtype, cu_seqlens, nseq, total, dim, d_state, false);
   if (rc) return rc;
+  if (ckpt && (rc = check_scan(dtype, cu_seqlens, nseq, total, dim, d_state, true))) return rc;
   if (!aneg || (total > 0 && (!x || !dt || !B || !C || !y)))
     return fail(MHS_EINVAL, "null pointer argument");
   if ((rc = check_ld("x", ld_x, dim)) || (rc = check_ld("dt", ld_dt, dim)) ||
@@ -311,7 +315,7 @@ int mhs_packed_scan_bwd(int dtype, const void* x, int64_t ld_x, const void* dt, 
                         int64_t nseq, int64_t total, int64_t dim, int64_t d_state,
                         void* workspace, size_t workspace_bytes, void* stream) {
   mhs::clear_error();
-  int rc = check_scan(dtype, cu_seqlens, nseq, total, dim, d_state);
+  int rc = check_scan(dtype, cu_seqlens, nseq, total, dim, d_state, true);
   if (rc) return rc;
   if (!aneg || !daneg ||
       (total > 0 && (!x || !dt || !B || !C || !dy || !dx || !ddt || !dB || !dC)) ||
