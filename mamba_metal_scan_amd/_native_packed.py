@@ -298,7 +298,7 @@ packed_conv_fwd = _register(
 def _packed_conv_fwd_fake(x, w, bias, cu, window, want_window):
     rows, d = x.shape
     return (x.new_empty((rows, d)),
-            x.new_empty((cu.shape[0] - 1, d, w.shape[1] - 1) if want_window else (0,)))
+            x.new_empty((cu.shape[0] - 1, d, w.shape[-1] - 1) if want_window else (0,)))
 
 
 def _packed_conv_bwd_impl(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor, cu: torch.Tensor,
@@ -349,7 +349,7 @@ packed_conv_bwd = _register("packed_conv_bwd", _packed_conv_bwd_impl, (), _check
 @packed_conv_bwd.register_fake
 def _packed_conv_bwd_fake(x, w, bias, cu, window, dout, dlast):
     return (x.new_empty(x.shape), torch.empty_like(w), torch.empty_like(bias),
-            x.new_empty((cu.shape[0] - 1, x.shape[1], w.shape[1] - 1) if window is not None
+            x.new_empty((cu.shape[0] - 1, x.shape[1], w.shape[-1] - 1) if window is not None
                         else (0,)))
 
 
