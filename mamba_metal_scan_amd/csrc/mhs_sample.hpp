@@ -354,9 +354,10 @@ struct SlotMaxima : Vectors<T> {
     const auto end = [&](int, float v) { most = fmaxf(most, v); };
     this->in_head(end);
     this->in_tail(end);
+    most += 0.f;   // (-0 as 0: its key is the words' in the list)
 #pragma unroll
     for (int t = 0; t < kSlots; ++t) {
-      slot[t] += 0.f;   // (-0 as 0)
+      slot[t] += 0.f;
       most = fmaxf(most, slot[t]);
     }
   }
