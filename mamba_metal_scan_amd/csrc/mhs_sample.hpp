@@ -1018,8 +1018,8 @@ sample_kernel(SampleArgs a) {
 
 // Bound by the weights' arithmetic, some 50 instructions a word, most in 64 bits, and by the
 // adds to LDS: 256 x 131072 words 58 us, a third of those rows 18 us.
-// Of the rows left those that no k or +inf leaves to the search: part blockIdx.x of row
-// blockIdx.y, its weights by bin, to the part's and to the row's; without top-p their sum.
+// Of the rows left those that neither k nor +inf with top-p leaves to the search: part blockIdx.x of
+// row blockIdx.y, its weights by bin, to the part's and to the row's; without top-p their sum.
 template <class T>
 __global__ void __launch_bounds__(256)
 sample_bins_kernel(SampleArgs a) {
@@ -1028,6 +1028,7 @@ sample_bins_kernel(SampleArgs a) {
   SampleRow& st = a.state[blockIdx.y];
   if (!st.left) return;
   RowOf<T> R(a, blockIdx.y);
+  if (R.k > 0 && R.k < R.V) return;
   R.set_max(st.m);
   const int lo = blockIdx.x * kPart, n = min(kPart, R.V - lo);
   u64* out = a.bins + ((size_t)blockIdx.y * a.parts + blockIdx.x) * kMassBins;
@@ -1040,7 +1041,7 @@ sample_bins_kernel(SampleArgs a) {
     if (threadIdx.x == 0) out[0] = (bins[0][0] + bins[0][1]) + (bins[0][2] + bins[0][3]);
     return;
   }
-  if (R.peak || (R.k > 0 && R.k < R.V)) return;
+  if (R.peak) return;
   fill_bins<T, 256, kCopies>(bins[0], R, lo, n, [&](double y) { return R.bin_of(y); });
   for (int i = threadIdx.x; i < kMassBins; i += 256) {
     u64 w = 0;
