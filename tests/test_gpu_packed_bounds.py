@@ -1,6 +1,7 @@
-"""The packed kernels with cu_seqlens that are no lengths (tests/test_packed_pieces.py has their indexes on
-the host): the C entry points on tensors that lie between others. What lies around the inputs is NaN
-and reaches no output, what lies around the outputs and the workspace keeps its bits."""
+"""The packed kernels with cu_seqlens that are no lengths (tests/test_packed_pieces.py has their
+indexes on the host): the C entry points on tensors that lie between others. What lies around the
+inputs is NaN and reaches no output, what lies around the outputs and the workspace keeps its
+bits."""
 from __future__ import annotations
 
 import pytest
@@ -97,8 +98,8 @@ def test_scan_stays_within(which, cu_dtype, dtype):
     ws = ar.workspace(nbytes)
     _ok(lib.mhs_packed_scan_bwd(
         TYPES[dtype], _ptr(x), d + 8, _ptr(dt), d + 8, _ptr(aneg), _ptr(b), n + 8, _ptr(c), n + 8,
-        _ptr(cu), cu_dtype == torch.int64, _ptr(h0), _ptr(ckpt), _ptr(dy), d + 8, _ptr(dh), _ptr(dx),
-        _ptr(ddt), _ptr(da), _ptr(db), _ptr(dc), _ptr(dh0), nseq, rows, d, n, _ptr(ws), nbytes,
+        _ptr(cu), cu_dtype == torch.int64, _ptr(h0), _ptr(ckpt), _ptr(dy), d + 8, _ptr(dh),
+        _ptr(dx), _ptr(ddt), _ptr(da), _ptr(db), _ptr(dc), _ptr(dh0), nseq, rows, d, n, _ptr(ws), nbytes,
         None))
     ar.check()
 
