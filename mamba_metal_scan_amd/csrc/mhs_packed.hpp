@@ -125,7 +125,7 @@ __device__ __forceinline__ Piece find_piece(const Seqs& q, int tc, int p) {
 __device__ __forceinline__ int seq_pieces(const Seqs& q, int tc, int s, int* first) {
   const int b = cu_at(q, s), e = max(b, cu_at(q, s + 1));
   *first = b / tc + s;
-  return max(1, (e - b + tc - 1) / tc);
+  return e > b ? (e - b - 1) / tc + 1 : 1;   // (e - b may be next to 2^31)
 }
 
 }  // namespace mhs
