@@ -683,10 +683,10 @@ int mhs_block_bwd_f32(const mhs_block_weights* w, const float* x, const float* x
  * and of their gradients; ld_* are the elements between their rows (the row's width
  * and more, below 2^18); outputs are contiguous and overwritten. Sums and states are
  * fp32, every reduction in a fixed order (bit-for-bit reproducible). Up to 2^17
- * channels, 2^22 sequences, fewer than 2^31 rows. Workspaces are 256-byte aligned;
- * two calls at once need two.
+ * channels, 2^22 sequences, fewer than 2^31 rows; less where a launch would have
+ * 2^32 threads. Workspaces are 256-byte aligned; two calls at once need two.
  *
- * The selective scan (the recurrence above, per sequence): aneg (dim, d_state) fp32; h0
+ * The selective scan (the recurrence above, per sequence): aneg (dim, d_state) fp32, +inf allowed; h0
  * NULL (zeros) or (nseq, dim, d_state) fp32, the states before; h_last NULL or the
  * states behind each sequence (h0's for one of no rows). ckpt: NULL, or
  * mhs_packed_ckpt_floats floats for the backward. The backward takes the forward's

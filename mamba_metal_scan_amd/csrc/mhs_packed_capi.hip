@@ -76,11 +76,20 @@ int64_t piece_count(int64_t total, int64_t nseq, int tc) { return total / tc + n
 
 // Rows of a piece: as many pieces as give each SIMD twelve waves, eight in the backward, which
 // holds two at a time (their latencies then hide each other's, and pieces of unlike
-// length even out). Pieces of 32 rows | 64 | 128 | 176, us: 8192 x 1536 x 16 in fp32, where this
-// gives 32 and 48, the forward's launches 125 | 122 | 151 | 165, the backward's 218 | 210 | 238 |
-// 251; 32768 x 2048 x 16 in bf16, where it gives 176 and 256, 518 | 487 | 466 | 467 and 985 |
-// 903 | 878 | 875; one prompt of 509 x 640 x 16 in fp32, where it gives the least, 16:
-// 18, then 21 | 28 | 44 | 54.
+// length even out), rounded down to whole sub-chunks. The launches of a captured call, us, in
+// pieces of 16 rows | 32 | 48 | 64 | 80 | 96 | 128 | 160 | 256:
+//   8192 x 1536 x 16 in fp32, 24 sequences,
+//     forward (this gives 32)   153 | 122 | 117 | 115 | 118 | 121 | 137 | 141 | 150
+//     backward (48)             247 | 208 | 197 | 193 | 204 | 218 | 221 | 228 | 262
+//   32768 x 2048 x 16 in bf16, 9 sequences,
+//     forward (160)             616 | 495 | 477 | 456 | 444 | 449 | 444 | 438 | 449
+//     backward (256)           1079 | 893 | 827 | 798 | 791 | 786 | 780 | 791 | 804
+//   4096 x 4096 x 16 in bf16, 12 prompts to states (32)
+//                               141 | 122 | 114 | 113 | 119 | 124 | 137 | 153 | 162
+//   one prompt of 509 x 640 x 16 in fp32 (16)
+//                                18 |  20 |  24 |  28 |  32 |  36 |  45 |  53 |  77
+// It counts the waves alone and not the states that a piece more has carried, written and
+// read, and loses up to 7% to the best of these: 64 rows in the first case and the third.
 // Few rows are one piece, without carries: of 640 x 16 in fp32 at 32 | 64 | 96 rows one launch
 // takes 8.2 | 12.8 | 17.4 us and the three 13.1 | 13.3 | 13.4 (captured; a call 14.4 | 14.3 | 17.5
 // and 20), the backward in one piece 18.9 | 30.0 | 40.8, in several 20.8 | 21.1 | 21.3.

@@ -4,10 +4,10 @@
 // within each sequence; the K - 1 inputs before its first row come from window
 // (nseq, D, K - 1) or are zero, its last K - 1 go to window_out.
 //
-// HBM-bound stencils: a thread owns V neighbouring channels (a 16-byte access,
-// or one channel where the layout allows no more) and the rows of a piece, the
-// K - 1 rows before each kept in registers. No row needs a test of its
-// sequence: a piece belongs to one.
+// HBM-bound stencils: a thread owns V neighbouring channels (8 bytes of a row in the forward, two
+// channels in the backward; one where the width, a stride or an address is no multiple of that, or
+// the address none of 16) and the rows of a piece, the K - 1 rows before each kept in registers. No
+// row needs a test of its sequence: a piece belongs to one.
 #pragma once
 
 #include "mhs_packed.hpp"

@@ -18,9 +18,10 @@
 // SIMD, multiply 2.9, multiply-add 4.8, exponential 8.3, and with a broadcast of a
 // lane of the quad in it 4.4 and 5.0, v_permlane swaps 8.3. Per step, channel and state the
 // carry passes need 19 of them, the forward 24 and the backward 70. (Operands by LDS or by DPP,
-// us, 32768 x 2048 x 16 bf16 | 8192 x 1536 x 16 fp32: carry 167 or 190 | 43 or 44, its
-// adjoint 175 or 185 | 40 or 43, the forward 277 or 282 | 66 or 65; the backward 655 or 660
-// | 170 or 146, its registers being full. The quad's sums by LDS too: 280 | 65, 665 | 153.)
+// us, each pair in one run, 32768 x 2048 x 16 bf16 | 8192 x 1536 x 16 fp32: carry 167 or 190 | 43
+// or 44, its adjoint 175 or 185 | 40 or 43, the forward 277 or 282 | 66 or 65; the backward 655
+// or 660 | 170 or 146, its registers being full. The quad's sums by LDS too: 280 | 65, 665 | 153.
+// What the kernels take now stands at each, at steady clocks; from idle 5 to 10% more.)
 //
 // A sequence longer than a piece takes three launches: the carry pass walks
 // each piece but the last from a zero state and leaves its end state and its
@@ -313,8 +314,8 @@ __device__ __forceinline__ void store_sdt(const PackedScanArgs& a, int q, int d,
 //
 // CARRY: the carry pass, else the main one. All is branch-free buffer accesses, what is not
 // there lying past the buffer: a branch within the loop made the compiler wait for all loads
-// in flight (twice the time). 32768 x 2048 x 16 in bf16: 156 and 261 us, 8192 x 1536 x 16 in fp32
-// 43 and 68 us, of 129 and 162, 24 and 30 that the vector units need for the formula alone.
+// in flight (twice the time). 32768 x 2048 x 16 in bf16: 149 and 267 us, 8192 x 1536 x 16 in fp32
+// 39 and 66 us, of 129 and 162, 24 and 30 that the vector units need for the formula alone.
 
 template <class T, int NPL, int WS, bool VEC, bool CARRY, bool CKPT>
 __global__ void __launch_bounds__(256)
@@ -470,7 +471,7 @@ packed_scan_fwd_kernel(PackedScanArgs a) {
 // carry and sdt -> start of the pieces 1 .. of each sequence of several; with BACK
 // of the pieces .. n - 2, from the last (dh_last) down. Block (s, channels x states). Bound by the
 // states' bytes, read and written once, and by the chain of a sequence's pieces, eight of
-// which are loaded at once (8192 x 1536 x 16 fp32 in pieces of 32 rows, 54 MB: 15 us).
+// which are loaded at once (8192 x 1536 x 16 fp32 in pieces of 32 rows, 54 MB: 17 us).
 template <bool BACK>
 __global__ void __launch_bounds__(256)
 packed_fold_kernel(PackedScanArgs a) {
@@ -517,8 +518,8 @@ packed_fold_kernel(PackedScanArgs a) {
 // so that each lane ends with one of them, in LDS over the block's waves, and over the
 // blocks in packed_sum_bc_kernel: always in the same order.
 // (Checkpoints every 8 rows rather than 16: what the sums over the channels cost falls with
-// the channels a lane holds, and registers hold 8 rows of two.) 32768 x 2048 x 16 in bf16: 169
-// (carry) and 632 us, 8192 x 1536 x 16 in fp32 39 and 144 us.
+// the channels a lane holds, and registers hold 8 rows of two.) 32768 x 2048 x 16 in bf16: 159
+// (carry) and 609 us, 8192 x 1536 x 16 in fp32 36 and 133 us.
 
 // The adjoint's carry pass: each piece but the first from a zero adjoint.
 template <class T, int NPL, int WS, bool VEC>

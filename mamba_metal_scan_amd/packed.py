@@ -198,8 +198,11 @@ def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     up, none above L. h0 (S, D, N) float32: the states before each sequence (zeros
     without). Returns y (L, D), zeros in the rows behind the last sequence, and with
     return_state the (S, D, N) float32 states behind each sequence (h0's for an empty one).
-    The gradients (x, dt, Aneg, B, C, h0) are summed in a fixed order. For them the
-    states at every eighth row are kept, L D N / 2 bytes."""
+    An Aneg of +inf is a state that keeps nothing of the row before. The gradients (x, dt,
+    Aneg, B, C, h0) are summed in a fixed order. For them the states at every eighth row
+    are kept, L D N / 2 bytes. While it runs, a call of more than 64 rows holds some
+    8 P D N bytes, its backward 12 P D N + L D N / 16, P pieces of 16 to 1024 rows, L over their
+    length and one a sequence."""
     what = "selective_scan_packed"
     _hip(what, x, dt, aneg, b_in, c_in, cu_seqlens, h0)
     for name, t in (("x", x), ("dt", dt), ("B", b_in), ("C", c_in)):

@@ -39,6 +39,11 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     index. NaN logits count as -inf. A row that has no logit above -inf, or settings that do not
     hold (temperature below 0 or infinite, min_p above 1, NaN), gives token -1.
 
+    Fewer than 2^16 rows (of logits' leading dimensions), vocab up to 2^24. While it runs, a
+    call of more than 4096 words holds 8 KB a row; and where top_k is a tensor, or off (below 1 or
+    from vocab on), 8 KB more for each row and 8192 words above 8192, which in 16 bits is half
+    of what the logits take.
+
     With return_logprobs also the log-probabilities (...) float32 of the tokens in the
     distributions that they were drawn from (NaN for token -1). Weights are formed in 64
     bits: which word a number falls on does not change from run to run."""
