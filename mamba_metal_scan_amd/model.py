@@ -418,11 +418,21 @@ def _plain_block(b: nn.Module) -> bool:
     return _own_methods(b) and no_hooks(b) and no_hooks(b._modules["norm"])
 
 
+_PACKED_METHODS = tuple(sorted(_METHODS - {"__init__"})) + ("__call__",)
+
+
+def _runs_own(m: nn.Module, cls: type, methods) -> bool:
+    """Whether calling m runs cls's methods and nothing else: a subclass may add
+    parametrized weights, or whatever leaves these methods alone."""
+    return (isinstance(m, cls) and all(getattr(type(m), k) is getattr(cls, k) for k in methods)
+            and not any(k in m.__dict__ for k in methods) and no_hooks(m))
+
+
 def _packs(b: nn.Module) -> bool:
-    """Whether b.mix_packed() of b's norm in place of b(x) skips nothing: as
-    _plain_block, but that the norm is called and the conv is not."""
-    return (_own_methods(b) and no_hooks(b) and type(b._modules["conv"]) is nn.Conv1d
-            and no_hooks(b._modules["conv"]))
+    """Whether b.mix_packed() of b's norm in place of b(x), which calls b's
+    modules but for the conv and reads the conv's weights, skips nothing."""
+    return (_runs_own(b, MambaBlock, _PACKED_METHODS)
+            and _runs_own(b.conv, nn.Conv1d, ("forward", "_conv_forward", "__call__")))
 
 
 class TinyMamba(nn.Module):
@@ -484,8 +494,8 @@ class TinyMamba(nn.Module):
         """The final norm's output (L, d_model) for the packed tokens idx (L).
 
         A block's packed form is mix_packed(), not a call of the block, and reads the conv's
-        weights: a wrapper, a subclass, methods set on the instance and hooks of either would
-        be left out, and are refused."""
+        weights: a wrapper, methods of a subclass or set on the instance, and hooks of either
+        would be left out, and are refused."""
         for i, b in enumerate(self.blocks):
             if not _packs(b):
                 raise RuntimeError("packed sequences call neither a block nor its conv: block "

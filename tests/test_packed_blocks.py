@@ -7,6 +7,8 @@ import pytest
 import torch
 import torch.nn as nn
 
+from torch.nn.utils import parametrize
+
 from helpers import assert_close
 from mamba_metal_scan_amd.model import MambaBlock, MambaConfig, TinyMamba
 
@@ -65,6 +67,15 @@ def _scan(m):
     m.blocks[1]._scan = lambda x, return_state=False: x
 
 
+def _call(m):
+    m.blocks[1].__class__ = type("Called", (MambaBlock,),
+                                 {"__call__": lambda self, x, cache=None: 2 * x})
+
+
+def _conv_subclass(m):
+    m.blocks[1].conv.__class__ = type("Scaled", (nn.Conv1d,), {"forward": lambda self, x: 2 * x})
+
+
 def _conv_hook(m):
     m.blocks[1].conv.register_forward_hook(lambda mod, args, out: 2 * out)
 
@@ -74,7 +85,7 @@ def _conv_forward(m):
 
 
 CHANGES = [_hook, _pre_hook, _backward_hook, _subclass, _wrapper, _forward, _mix, _scan,
-           _conv_hook, _conv_forward]
+           _call, _conv_subclass, _conv_hook, _conv_forward]
 
 
 def _refused(m, dev):
@@ -133,3 +144,42 @@ def test_modules_that_are_called_keep_their_hooks(name):
         assert calls == [1, 1, 1]
     assert_close("logits", got, want, 2e-5)
     assert not torch.allclose(got, plain)
+
+
+class Twice(nn.Module):
+    def forward(self, w):
+        return 2 * w
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["conv.weight", "A", "D_skip", "in_proj.weight", "subclass"])
+def test_what_leaves_the_methods_alone_is_taken(where):
+    """Parametrized weights (a subclass of the module's class) are read as they are, and so is a
+    subclass that overrides none of the methods: as of each document alone."""
+    m = _model().cuda()
+    block = m.blocks[1]
+    idx = torch.arange(9, device="cuda")
+    cu = torch.tensor([0, 4, 9], device="cuda")
+    with torch.no_grad():
+        plain = m.prefill(idx, cu, {})
+    if where == "subclass":
+        block.__class__ = type("Named", (MambaBlock,), {"extra": lambda self: 1})
+    else:
+        owner = block if "." not in where else getattr(block, where.split(".")[0])
+        parametrize.register_parametrization(owner, where.split(".")[-1], Twice(), unsafe=True)
+    with torch.no_grad():
+        got = m.prefill(idx, cu, {})
+        want = torch.stack([m(p[None], cache={})[0][0, -1] for p in (idx[:4], idx[4:])])
+    assert_close("logits", got, want, 2e-5)
+    assert torch.allclose(got, plain) == (where == "subclass")
+
+
+@pytest.mark.gpu
+def test_the_loss_of_packed_documents_is_traced():
+    m = _model().cuda()
+    idx = torch.arange(9, device="cuda")
+    cu = torch.tensor([0, 4, 9], device="cuda")
+    want = m.loss(idx, idx, cu_seqlens=cu)
+    got = torch.compile(lambda i, c: m.loss(i, i, cu_seqlens=c), backend="aot_eager",
+                        fullgraph=True)(idx, cu)
+    assert_close("loss", got, want, 1e-6)
